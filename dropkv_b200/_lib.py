@@ -79,6 +79,20 @@ SIGNATURES = {
     "dropkv_compress_varlen": (_c_int, [_c_int, ctypes.POINTER(VarlenSeq), _c_int, _c_int, _c_int, _c_int, _c_int,
                                         _c_f, _c_int, _c_int, _c_int, ctypes.c_double, _c_int, _c_p, _c_p, _c_p,
                                         _c_p, _c_sz, _c_p]),
+    "dropkv_block_tables": (_c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p, _c_int, _c_int, _c_p, _c_int, _c_int, _c_int,
+                                     _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "dropkv_store_rows": (_c_int, ([_c_p] + [_c_i64] * 3) * 2 + [_c_p] + ([_c_p] + [_c_i64] * 3) * 2
+                          + [_c_int] * 7 + [_c_p]),
+    "dropkv_qk_norm_rope": (_c_int, ([_c_p] + [_c_i64] * 3) * 2 + [_c_p, _c_p, _c_f, _c_p, _c_p, _c_int, _c_int,
+                                     _c_int, _c_p, _c_i64] + [_c_int] * 6 + [_c_p, _c_p] + [_c_p] + [_c_i64] * 3
+                            + [_c_p] + ([_c_p] + [_c_i64] * 3) * 2 + [_c_int, _c_int, _c_p]),
+    "dropkv_tree_attention_workspace_size": (_c_sz, [_c_int] * 6),
+    "dropkv_tree_attention": (_c_int, [_c_p] + [_c_i64] * 4 + ([_c_p] + [_c_i64] * 3) * 2
+                              + [_c_p, _c_int, _c_int, _c_int, _c_p, _c_p] + [_c_i64] * 3 + [_c_int] * 7
+                              + [_c_f, _c_p, _c_p, _c_sz, _c_p]),
+    "dropkv_token_logprobs_workspace_size": (_c_sz, [_c_i64, _c_int, _c_int]),
+    "dropkv_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_i64, _c_int, _c_p, _c_int, _c_int, _c_f]
+                              + [_c_p] * 5 + [_c_sz, _c_p]),
 }
 
 

@@ -621,5 +621,141 @@ int dropkv_decode_append_attention(const void* q, int64_t q_sb, int64_t q_sh, in
                                  pos);
 }
 
+// ---------------------------------------------------------------------------
+// Paged caches and the speculative decode step
+// ---------------------------------------------------------------------------
+int dropkv_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* table_in, int64_t table_in_stride,
+                        const int32_t* held, int B, int block_size, const int32_t* free_blocks, int n_free,
+                        int max_blocks, int max_new, int32_t* table, int32_t* held_out, int64_t* slots, int64_t* used,
+                        void* stream) {
+  if (!lens || !table || !held_out || !used) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if (B < 1 || B > 65535) return fail(DROPKV_ERR_ARG, "B must be in [1, 65535], got %d", B);
+  if (block_size < 1) return fail(DROPKV_ERR_ARG, "block_size must be positive, got %d", block_size);
+  if (max_blocks < 1 || max_new < 0 || n_free < 0)
+    return fail(DROPKV_ERR_ARG, "need max_blocks >= 1, max_new >= 0 and n_free >= 0 (got %d, %d, %d)", max_blocks, max_new, n_free);
+  if (max_new > 0 && !slots) return fail(DROPKV_ERR_ARG, "slots must be non-NULL");
+  if (n_free > 0 && !free_blocks) return fail(DROPKV_ERR_ARG, "free_blocks must be non-NULL");
+  if (!table_in != !held) return fail(DROPKV_ERR_ARG, "table_in and held go together");
+  if (table_in && table_in_stride < max_blocks) return fail(DROPKV_ERR_ARG, "table_in rows shorter than max_blocks");
+  return launch_block_tables(lens, new_lens, table_in, table_in_stride, held, B, block_size, free_blocks, n_free,
+                             max_blocks, max_new, table, held_out, slots, used, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dropkv_store_rows(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sb,
+                      int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages, int64_t kp_sb, int64_t kp_sh,
+                      int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh, int64_t vp_st, int n_pages,
+                      int block_size, int elem_bytes, int B, int Hkv, int N, int D, void* stream) {
+  if (elem_bytes != 2 && elem_bytes != 4) return fail(DROPKV_ERR_ARG, "elem_bytes must be 2 or 4, got %d", elem_bytes);
+  if (B < 0 || Hkv < 1 || N < 0 || D < 1 || n_pages < 0 || block_size < 1)
+    return fail(DROPKV_ERR_ARG, "invalid sizes B=%d Hkv=%d N=%d D=%d pages=%d block_size=%d", B, Hkv, N, D, n_pages, block_size);
+  if (B == 0 || N == 0 || n_pages == 0) return DROPKV_OK;  // nothing to store, or nowhere
+  if (!k || !v || !slots || !k_pages || !v_pages) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_pages) |
+       reinterpret_cast<uintptr_t>(v_pages)) % elem_bytes)
+    return fail(DROPKV_ERR_ARG, "rows must be aligned to their elements");
+  StoreRows s{k, k_sb, k_sh, k_sn, v, v_sb, v_sh, v_sn, slots, k_pages, kp_sb, kp_sh, kp_st, v_pages, vp_sb, vp_sh, vp_st,
+              n_pages, block_size, elem_bytes, B, Hkv, N, D};
+  return launch_store_rows(s, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dropkv_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k, int64_t k_sb,
+                        int64_t k_sh, int64_t k_sl, const void* q_weight, const void* k_weight, float eps,
+                        const float* cos, const float* sin, int P, int R, int interleaved, const int64_t* positions,
+                        int64_t pos_sb, int dtype, int B, int Hq, int Hkv, int L, int D, void* q_out, void* k_out,
+                        const void* v, int64_t v_sb, int64_t v_sh, int64_t v_sl, const int64_t* slots, void* k_pages,
+                        int64_t kp_sb, int64_t kp_sh, int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh,
+                        int64_t vp_st, int n_pages, int block_size, void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (!eb) return fail(DROPKV_ERR_ARG, "unknown dtype %d", dtype);
+  if (B < 0 || L < 0 || Hq < 1 || Hkv < 1 || D < 1)
+    return fail(DROPKV_ERR_ARG, "invalid sizes B=%d Hq=%d Hkv=%d L=%d D=%d", B, Hq, Hkv, L, D);
+  if (D > 1024) return fail(DROPKV_ERR_UNSUPPORTED, "qk_norm_rope needs D <= 1024, got %d", D);
+  if (R < 0 || R > D || R % 2) return fail(DROPKV_ERR_ARG, "R must be even and in [0, D], got %d", R);
+  if (P < 0 || (R > 0 && P > 0 && (!cos || !sin))) return fail(DROPKV_ERR_ARG, "cos and sin must be non-NULL [P, R / 2]");
+  if (!(eps >= 0.f)) return fail(DROPKV_ERR_ARG, "eps must be >= 0");
+  if (B == 0 || L == 0) return DROPKV_OK;
+  if (!q || !k || !positions || !q_out || !k_out) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if (slots) {
+    if (!v || !k_pages || !v_pages) return fail(DROPKV_ERR_ARG, "slots need v, k_pages and v_pages");
+    if (n_pages < 0 || block_size < 1) return fail(DROPKV_ERR_ARG, "invalid pool: %d pages of %d rows", n_pages, block_size);
+  }
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(k_pages) |
+       reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight)) % eb)
+    return fail(DROPKV_ERR_ARG, "tensors must be aligned to their elements");
+  QkRope a{q, q_sb, q_sh, q_sl, k, k_sb, k_sh, k_sl, q_weight, k_weight, eps, cos, sin, P, R, interleaved != 0,
+           positions, pos_sb, B, Hq, Hkv, L, D, q_out, k_out, v, v_sb, v_sh, v_sl, slots, k_pages, kp_sb, kp_sh, kp_st,
+           v_pages, vp_sb, vp_sh, vp_st, n_pages, block_size};
+  return launch_qk_norm_rope(a, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static bool tree_sizes_ok(int B, int Hq, int Hkv, int T, int D, int cap) {
+  return B >= 1 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && T >= 1 && T <= 256 && (D == 64 || D == 128) && cap >= 0 &&
+         (int64_t)B * Hkv <= 65535 && (int64_t)Hq * T <= 65535LL * 128;
+}
+
+size_t dropkv_tree_attention_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
+  return tree_sizes_ok(B, Hq, Hkv, T, D, cap) ? tree_attention_workspace_size(B, Hq, Hkv, T, D, cap) : 0;
+}
+
+int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd, const void* k,
+                          int64_t k_s0, int64_t k_sh, int64_t k_ss, const void* v, int64_t v_s0, int64_t v_sh,
+                          int64_t v_ss, const int32_t* table, int max_blocks, int block_size, int n_pages,
+                          const int32_t* cache_lens, const uint8_t* mask, int64_t mask_sb, int64_t mask_sr,
+                          int64_t mask_sc, int dtype, int B, int Hq, int Hkv, int T, int D, int cap, float scale,
+                          void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !cache_lens || !out) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if (dtype != DROPKV_DTYPE_BF16 && dtype != DROPKV_DTYPE_F16)
+    return fail(DROPKV_ERR_UNSUPPORTED, "tree attention takes bf16 or fp16 inputs");
+  if (D != 64 && D != 128) return fail(DROPKV_ERR_UNSUPPORTED, "tree attention needs D of 64 or 128 (got %d)", D);
+  if (T > 256) return fail(DROPKV_ERR_UNSUPPORTED, "tree attention takes at most 256 nodes (got %d)", T);
+  if (!tree_sizes_ok(B, Hq, Hkv, T, D, cap))
+    return fail(DROPKV_ERR_ARG, "invalid sizes B=%d Hq=%d Hkv=%d T=%d cap=%d", B, Hq, Hkv, T, cap);
+  if (table) {
+    if (block_size < 8 || block_size > 1024 || (block_size & (block_size - 1)))
+      return fail(DROPKV_ERR_UNSUPPORTED, "tree attention needs a block_size that is a power of two from 8 to 1024 (got %d)", block_size);
+    if (n_pages < 0 || max_blocks < 0 || (int64_t)max_blocks * block_size != cap)
+      return fail(DROPKV_ERR_ARG, "cap must be max_blocks * block_size");
+  }
+  const bool rows = cap > 0 && (!table || n_pages > 0);
+  if (rows && (!k || !v)) return fail(DROPKV_ERR_ARG, "K and V must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 ||
+      ((k_s0 | k_sh | k_ss | v_s0 | v_sh | v_ss) * 2) % 16)
+    return fail(DROPKV_ERR_ARG, "K/V rows must start on 16-byte boundaries");
+  if (rows && (k_ss < D || v_ss < D || k_sh < D || v_sh < D || k_s0 < D || v_s0 < D))
+    return fail(DROPKV_ERR_ARG, "K/V strides too small");
+  if (!(scale > 0.f)) return fail(DROPKV_ERR_ARG, "scale must be positive");
+  int rc = check_ws(workspace, workspace_bytes, tree_attention_workspace_size(B, Hq, Hkv, T, D, cap));
+  if (rc) return rc;
+  TreeAttn a{q, q_sb, q_sh, q_ss, q_sd, k, k_s0, k_sh, k_ss, v, v_s0, v_sh, v_ss, table, max_blocks, block_size, n_pages,
+             cache_lens, mask, mask_sb, mask_sr, mask_sc, B, Hq, Hkv, T, D, rows ? cap : 0, scale, out};
+  return launch_tree_attention(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dropkv_token_logprobs_workspace_size(int64_t N, int V, int top_k) {
+  if (N < 1 || V < 1 || top_k < 0 || top_k > 64 || top_k > V) return 0;
+  return token_logprobs_workspace_size(N, V, top_k);
+}
+
+int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t N, int V, const int64_t* tokens,
+                          int C, int top_k, float temperature, float* logprob, float* entropy, float* top_logprobs,
+                          int64_t* top_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (!eb) return fail(DROPKV_ERR_ARG, "unknown dtype %d", dtype);
+  if (N < 0 || N > 0x7fffffff || V < 1 || C < 0) return fail(DROPKV_ERR_ARG, "invalid sizes N=%lld V=%d C=%d", (long long)N, V, C);
+  if (top_k < 0 || top_k > 64 || top_k > V) return fail(DROPKV_ERR_ARG, "top_k must be in [0, min(64, V)], got %d", top_k);
+  if (!(temperature > 0.f) || std::isinf(temperature)) return fail(DROPKV_ERR_ARG, "temperature must be positive and finite");
+  if (N == 0) return DROPKV_OK;
+  if (!logits || !entropy || (C > 0 && (!tokens || !logprob)) || (top_k > 0 && (!top_logprobs || !top_tokens)))
+    return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if (row_stride < 0) return fail(DROPKV_ERR_ARG, "row_stride must not be negative");
+  if (reinterpret_cast<uintptr_t>(logits) % eb) return fail(DROPKV_ERR_ARG, "logits must be aligned to their elements");
+  int rc = check_ws(workspace, workspace_bytes, token_logprobs_workspace_size(N, V, top_k));
+  if (rc) return rc;
+  Logprobs a{logits, row_stride, N, V, C, top_k, tokens, (float)(1.4426950408889634 / (double)temperature),
+             (float)(1.0 / (double)temperature), logprob, entropy, top_logprobs, top_tokens};
+  return launch_token_logprobs(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 

@@ -212,4 +212,89 @@ int launch_gather(const void* k, const void* v, int elem_bytes, int BH, int Lk, 
 // the table (t.scores filled); the longest row must pass select_gather_supported.
 int launch_select_gather_varlen(const VarlenTable& t, int kernel_size, int elem_bytes, int D, cudaStream_t st);
 
+// ---------------------------------------------------------------------------
+// Paged caches and the speculative step (paged.cu, qk_rope.cu, tree_attn.cu,
+// logprobs.cu). Strides are in elements; a pool's pages are [pages, H, block, D].
+// ---------------------------------------------------------------------------
+int launch_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* table_in, int64_t table_in_stride,
+                        const int32_t* held_in, int B, int block, const int32_t* free_blocks, int n_free,
+                        int max_blocks, int max_new, int32_t* table, int32_t* held, int64_t* slots, int64_t* used,
+                        cudaStream_t st);
+
+struct StoreRows {
+  const void* k;
+  int64_t k_sb, k_sh, k_sn;
+  const void* v;
+  int64_t v_sb, v_sh, v_sn;
+  const int64_t* slots;
+  void* k_pages;
+  int64_t kp_sb, kp_sh, kp_st;
+  void* v_pages;
+  int64_t vp_sb, vp_sh, vp_st;
+  int n_pages, block, elem_bytes, B, H, N, D;
+};
+int launch_store_rows(const StoreRows& s, cudaStream_t st);
+
+struct QkRope {
+  const void* q;
+  int64_t q_sb, q_sh, q_sl;
+  const void* k;
+  int64_t k_sb, k_sh, k_sl;
+  const void* q_weight;  // [D] or nullptr: no norm
+  const void* k_weight;
+  float eps;
+  const float* cos;  // [P, R / 2]
+  const float* sin;
+  int P, R, interleaved;
+  const int64_t* positions;  // [B, L], pos_sb = 0: one row for all
+  int64_t pos_sb;
+  int B, Hq, Hkv, L, D;
+  void* q_out;  // [B, Hq, L, D], contiguous
+  void* k_out;
+  const void* v;  // with slots only
+  int64_t v_sb, v_sh, v_sl;
+  const int64_t* slots;  // [B, L] or nullptr: no cache write
+  void* k_pages;
+  int64_t kp_sb, kp_sh, kp_st;
+  void* v_pages;
+  int64_t vp_sb, vp_sh, vp_st;
+  int n_pages, block;
+};
+int launch_qk_norm_rope(const QkRope& a, int dtype, cudaStream_t st);
+
+struct TreeAttn {
+  const void* q;
+  int64_t q_sb, q_sh, q_ss, q_sd;
+  const void* k;  // row buffers [B, Hkv, cap, D] or, with a table, pages [n_pages, Hkv, block, D]
+  int64_t k_s0, k_sh, k_ss;
+  const void* v;
+  int64_t v_s0, v_sh, v_ss;
+  const int32_t* table;  // [B, max_blocks] or nullptr
+  int max_blocks, block, n_pages;
+  const int32_t* cache_lens;  // [B]
+  const uint8_t* mask;        // [B, T, T] truth values, or nullptr: a chain
+  int64_t mask_sb, mask_sr, mask_sc;
+  int B, Hq, Hkv, T, D;
+  int cap;  // rows a sequence's cache can hold
+  float scale;
+  void* out;  // [B, Hq, T, D], contiguous
+};
+size_t tree_attention_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
+int launch_tree_attention(const TreeAttn& a, int dtype, void* ws, cudaStream_t st);
+
+struct Logprobs {
+  const void* logits;
+  int64_t row_stride, N;
+  int V, C, top_k;
+  const int64_t* tokens;  // [N, C]
+  float scale_log2;       // log2(e) / temperature
+  float inv_temperature;
+  float* logprob;         // [N, C]
+  float* entropy;         // [N]
+  float* top_logprobs;    // [N, top_k]
+  int64_t* top_tokens;    // [N, top_k]
+};
+size_t token_logprobs_workspace_size(int64_t N, int V, int top_k);
+int launch_token_logprobs(const Logprobs& a, int dtype, void* ws, cudaStream_t st);
+
 }  // namespace dropkv

@@ -1,0 +1,165 @@
+// Pages of a shared K/V pool for a ragged batch of caches: block tables and slot
+// maps from lengths that exist on the device only (an eviction's keep_len, a decode
+// loop's counters), and the rows that go to those slots.
+#include "common.cuh"
+
+namespace dropkv {
+namespace {
+
+constexpr int BT_NT = 256;
+constexpr int BT_TOKENS = 8 * BT_NT;  // slots of one CTA
+
+struct BtArgs {
+  const int32_t* lens;
+  const int32_t* new_lens;  // nullptr: every token is new
+  const int32_t* table_in;  // nullptr: no pages held
+  int64_t table_in_stride;
+  const int32_t* held_in;
+  const int32_t* free_blocks;
+  int B, block, n_free, max_blocks, max_new;
+  int32_t* table;
+  int32_t* held;
+  int64_t* slots;
+  int64_t* used;
+};
+
+__device__ __forceinline__ int bt_len(const BtArgs& a, int b) { return max(a.lens[b], 0); }
+__device__ __forceinline__ int bt_held(const BtArgs& a, int b) {
+  return a.held_in ? min(max(a.held_in[b], 0), a.max_blocks) : 0;
+}
+// pages request b still needs
+__device__ __forceinline__ int bt_take(const BtArgs& a, int b) {
+  const int need = (int)(((int64_t)bt_len(a, b) + a.block - 1) / a.block);
+  return max(min(need, a.max_blocks) - bt_held(a, b), 0);
+}
+
+// CTA (b, y): table row b (y = 0) and the slots [y, y + 1) * BT_TOKENS of request b.
+// A request's pages start where those of the requests before it end in the free
+// list, so each CTA sums the needs of the requests before its own; no CTA waits
+// for another.
+__global__ void __launch_bounds__(BT_NT) block_tables_kernel(BtArgs a) {
+  __shared__ long long part[BT_NT / 32];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  long long sum = 0;
+  for (int i = tid; i < b; i += BT_NT) sum += bt_take(a, i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((tid & 31) == 0) part[tid >> 5] = sum;
+  __syncthreads();
+  long long first = 0;
+#pragma unroll
+  for (int w = 0; w < BT_NT / 32; ++w) first += part[w];
+  const int held = bt_held(a, b), take = bt_take(a, b);
+  const long long left = a.n_free - first;
+  const int got = (int)(left < 0 ? 0 : (left < take ? left : take));
+  const int32_t* old = a.table_in ? a.table_in + b * a.table_in_stride : nullptr;
+  auto page = [&](int col) -> int {
+    if (col < held) return old[col];
+    return col < held + got ? a.free_blocks[first + (col - held)] : -1;
+  };
+  if (blockIdx.y == 0) {
+    int32_t* row = a.table + (int64_t)b * a.max_blocks;
+    for (int c = tid; c < a.max_blocks; c += BT_NT) row[c] = page(c);
+    if (tid == 0) {
+      a.held[b] = held + got;
+      if (b == a.B - 1) *a.used = first + take;
+    }
+  }
+  const int len = bt_len(a, b), nn = a.new_lens ? min(max(a.new_lens[b], 0), len) : len;
+  const int64_t i0 = (int64_t)blockIdx.y * BT_TOKENS;
+  int64_t* out = a.slots + (int64_t)b * a.max_new;
+  for (int64_t i = i0 + tid; i < a.max_new && i < i0 + BT_TOKENS; i += BT_NT) {
+    int64_t slot = -1;
+    if (i < nn) {
+      const int t = len - nn + (int)i, col = t / a.block;
+      if (col < a.max_blocks) {
+        const int p = page(col);
+        if (p >= 0) slot = (int64_t)p * a.block + (t - col * a.block);
+      }
+    }
+    out[i] = slot;
+  }
+}
+
+constexpr int SR_NT = 256;
+
+struct SrArgs {
+  const char* k;  // [B, H, N, row bytes], byte strides
+  const char* v;
+  int64_t k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;
+  const int64_t* slots;  // [B, N]
+  char* kp;              // [pages, H, block, row bytes], byte strides
+  char* vp;
+  int64_t kp_sb, kp_sh, kp_st, vp_sb, vp_sh, vp_st;
+  int64_t n_slots;       // pages * block
+  int B, H, N, block, vecs;  // vecs: vectors of a row
+};
+
+template <typename T>
+__global__ void __launch_bounds__(SR_NT) store_rows_kernel(SrArgs a) {
+  const int64_t total = (int64_t)a.B * a.H * a.N * a.vecs;
+  for (int64_t e = (int64_t)blockIdx.x * SR_NT + threadIdx.x; e < total; e += (int64_t)gridDim.x * SR_NT) {
+    const int c = (int)(e % a.vecs);
+    int64_t r = e / a.vecs;
+    const int n = (int)(r % a.N);
+    r /= a.N;
+    const int h = (int)(r % a.H), b = (int)(r / a.H);
+    const int64_t slot = a.slots[(int64_t)b * a.N + n];
+    if (slot < 0 || slot >= a.n_slots) continue;
+    const int64_t page = slot / a.block, at = slot % a.block;
+    *reinterpret_cast<T*>(a.kp + page * a.kp_sb + h * a.kp_sh + at * a.kp_st + c * (int)sizeof(T)) =
+        *reinterpret_cast<const T*>(a.k + b * a.k_sb + h * a.k_sh + n * a.k_sn + c * (int)sizeof(T));
+    *reinterpret_cast<T*>(a.vp + page * a.vp_sb + h * a.vp_sh + at * a.vp_st + c * (int)sizeof(T)) =
+        *reinterpret_cast<const T*>(a.v + b * a.v_sb + h * a.v_sh + n * a.v_sn + c * (int)sizeof(T));
+  }
+}
+
+}  // namespace
+
+int launch_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* table_in, int64_t table_in_stride,
+                        const int32_t* held_in, int B, int block, const int32_t* free_blocks, int n_free,
+                        int max_blocks, int max_new, int32_t* table, int32_t* held, int64_t* slots, int64_t* used,
+                        cudaStream_t st) {
+  BtArgs a{lens, new_lens, table_in, table_in_stride, held_in, free_blocks, B, block, n_free, max_blocks, max_new,
+           table, held, slots, used};
+  const int ys = (int)(((int64_t)max_new + BT_TOKENS - 1) / BT_TOKENS);
+  if (ys > 65535) return fail(DROPKV_ERR_UNSUPPORTED, "block tables: max_new %d exceeds %d", max_new, 65535 * BT_TOKENS);
+  block_tables_kernel<<<dim3(B, ys > 0 ? ys : 1), BT_NT, 0, st>>>(a);
+  return check_launch("block_tables");
+}
+
+int launch_store_rows(const StoreRows& s, cudaStream_t st) {
+  SrArgs a;
+  const int eb = s.elem_bytes;
+  a.k = static_cast<const char*>(s.k);
+  a.v = static_cast<const char*>(s.v);
+  a.kp = static_cast<char*>(s.k_pages);
+  a.vp = static_cast<char*>(s.v_pages);
+  a.k_sb = s.k_sb * eb, a.k_sh = s.k_sh * eb, a.k_sn = s.k_sn * eb;
+  a.v_sb = s.v_sb * eb, a.v_sh = s.v_sh * eb, a.v_sn = s.v_sn * eb;
+  a.kp_sb = s.kp_sb * eb, a.kp_sh = s.kp_sh * eb, a.kp_st = s.kp_st * eb;
+  a.vp_sb = s.vp_sb * eb, a.vp_sh = s.vp_sh * eb, a.vp_st = s.vp_st * eb;
+  a.slots = s.slots;
+  a.n_slots = (int64_t)s.n_pages * s.block;
+  a.B = s.B, a.H = s.H, a.N = s.N, a.block = s.block;
+  // 16-byte vectors where every address they form is a multiple of 16
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                        reinterpret_cast<uintptr_t>(a.kp) | reinterpret_cast<uintptr_t>(a.vp) |
+                        (uint64_t)(a.k_sb | a.k_sh | a.k_sn | a.v_sb | a.v_sh | a.v_sn | a.kp_sb | a.kp_sh | a.kp_st |
+                                   a.vp_sb | a.vp_sh | a.vp_st) |
+                        (uint64_t)s.D * eb;
+  const int w = bits % 16 == 0 ? 16 : eb;
+  a.vecs = s.D * eb / w;
+  const int64_t total = (int64_t)s.B * s.H * s.N * a.vecs;
+  const int64_t want = (total + SR_NT - 1) / SR_NT, most = 32 * (int64_t)num_sms_current_device();
+  const int grid = (int)(want < most ? want : most);
+  if (w == 16)
+    store_rows_kernel<uint4><<<grid, SR_NT, 0, st>>>(a);
+  else if (w == 4)
+    store_rows_kernel<uint32_t><<<grid, SR_NT, 0, st>>>(a);
+  else
+    store_rows_kernel<uint16_t><<<grid, SR_NT, 0, st>>>(a);
+  return check_launch("store_rows");
+}
+
+}  // namespace dropkv

@@ -1,0 +1,326 @@
+"""A speculative decode step over paged, compressed caches (tensor functions over the C ABI).
+
+``compress_varlen`` leaves a ragged batch whose kept lengths exist on the device only,
+and decoding over it needs nothing of the host if the pages are handed out there too:
+
+* ``block_tables``   -- pages and slots from lengths on the device, in one launch;
+* ``store_rows``     -- K/V rows to slots (the eviction's outputs, accepted drafts);
+* ``qk_norm_rope``   -- head norms, position rotation and the cache write in one pass;
+* ``tree_attention`` -- a tree of drafted tokens over a cache in pages or row buffers;
+* ``token_logprobs`` -- log probabilities of given tokens, entropy, top alternatives.
+
+K and V pools are ``[pages, Hkv, block_size, D]``, any strides with contiguous rows (a
+pool stored ``[pages, block_size, Hkv, D]`` is passed transposed); slot ``s`` is row
+``s % block_size`` of page ``s // block_size``. Nothing here synchronises the host. The
+reference keeps one tensor per layer (dropkv_cache.py:581-617) and has no counterparts.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .ops import _DTYPE_CODE, _on_device, _stream, _workspace
+
+__all__ = ["BlockTables", "TokenLogprobs", "block_tables", "store_rows", "qk_norm_rope", "tree_attention",
+           "token_logprobs", "tree_mask_from_parents"]
+
+
+class BlockTables(NamedTuple):
+    table: torch.Tensor   # [B, max_blocks] int32, -1 past a request's pages
+    held: torch.Tensor    # [B] int32
+    slots: torch.Tensor   # [B, max_new] int64, -1 past a request's new tokens
+    used: torch.Tensor    # [1] int64: free pages asked for
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor                 # fp32, the shape of tokens
+    entropy: torch.Tensor                 # fp32, the shape of the rows
+    top_logprobs: Optional[torch.Tensor]  # fp32 [..., top_k], None for top_k = 0
+    top_tokens: Optional[torch.Tensor]    # int64 [..., top_k]
+
+
+def _on_one_device(*ts):
+    dev = ts[0].device
+    for t in ts:
+        if not t.is_cuda:
+            raise RuntimeError("dropkv_b200 runs on CUDA tensors only (no CPU path); got a "
+                               f"tensor on {t.device}")
+        if t.device != dev:
+            raise RuntimeError(f"all tensors must be on one device; got {dev} and {t.device}")
+    return dev
+
+
+def _ints(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _rows_strides(t: torch.Tensor, what: str):
+    """Strides of the three outer dimensions of [A, B, C, D] rows; a dimension of one
+    takes the packed stride, which its own cannot contradict."""
+    a, b, c, d = t.shape
+    if d > 1 and t.stride(3) != 1:
+        raise ValueError(f"{what} needs rows of D contiguous elements")
+    s2 = t.stride(2) if c > 1 else d
+    s1 = t.stride(1) if b > 1 else c * s2
+    s0 = t.stride(0) if a > 1 else max(b * s1, c * s2)
+    return s0, s1, s2
+
+
+def _check_pool(K_pages, V_pages, Hkv, D, dtype):
+    if K_pages.dim() != 4 or K_pages.shape != V_pages.shape or K_pages.shape[1] != Hkv or K_pages.shape[3] != D:
+        raise ValueError(f"expected K and V pages [pages, {Hkv}, block_size, {D}], got {tuple(K_pages.shape)} and "
+                         f"{tuple(V_pages.shape)}")
+    if K_pages.dtype != dtype or V_pages.dtype != dtype:
+        raise TypeError(f"pages must be {dtype}, got {K_pages.dtype} and {V_pages.dtype}")
+
+
+def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor, max_blocks: int, max_new: int,
+                 new_lens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                 held: Optional[torch.Tensor] = None) -> BlockTables:
+    """Block tables and slot maps from request lengths on the device.
+
+    ``lens`` [B] int32: tokens that each request's cache holds once this step is done;
+    the last ``new_lens`` [B] int32 of them (all, if None) are new and get slots.
+    ``table`` [B, max_blocks] int32 with ``held`` [B] int32 are the pages that the
+    requests hold already; the missing ones are taken from ``free_blocks`` [F] int32
+    in order, request after request. Returns new tensors (``BlockTables``); the
+    caller drops the first ``used`` entries of its free list. Where the list runs
+    short, entries and slots are -1, ``held`` counts the pages really held and
+    ``used`` is more than F.
+    """
+    if lens.dim() != 1:
+        raise ValueError(f"lens must be [B], got {tuple(lens.shape)}")
+    if (table is None) != (held is None):
+        raise ValueError("table and held go together")
+    dev = _on_one_device(*[t for t in (lens, free_blocks, new_lens, table, held) if t is not None])
+    B = lens.shape[0]
+    lens = _ints(lens, torch.int32, (B,), "lens")
+    free_blocks = _ints(free_blocks, torch.int32, (free_blocks.numel(),), "free_blocks")
+    if new_lens is not None:
+        new_lens = _ints(new_lens, torch.int32, (B,), "new_lens")
+    if table is not None:
+        table = _ints(table, torch.int32, (B, int(max_blocks)), "table")
+        held = _ints(held, torch.int32, (B,), "held")
+    with _on_device(dev):
+        out = BlockTables(torch.empty(B, max_blocks, dtype=torch.int32, device=dev),
+                          torch.empty(B, dtype=torch.int32, device=dev),
+                          torch.empty(B, max_new, dtype=torch.int64, device=dev),
+                          torch.empty(1, dtype=torch.int64, device=dev))
+        if B == 0:
+            out.used.zero_()
+            return out
+        rc = _lib.load().dropkv_block_tables(
+            lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None,
+            table.data_ptr() if table is not None else None, int(max_blocks),
+            held.data_ptr() if held is not None else None, B, int(block_size), free_blocks.data_ptr(),
+            free_blocks.numel(), int(max_blocks), int(max_new), out.table.data_ptr(), out.held.data_ptr(),
+            out.slots.data_ptr(), out.used.data_ptr(), _stream(dev))
+        _lib.check(rc, "dropkv_block_tables")
+    return out
+
+
+def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: torch.Tensor,
+               V_pages: torch.Tensor) -> None:
+    """Rows of K and V [B, Hkv, N, D] (any strides, rows of D contiguous) to slots [B, N]
+    (int64) of the pools, in place; rows whose slot is outside the pool (-1) are left
+    out. Where rows share a slot, any of them may stay. fp32, fp16 or bf16."""
+    dev = _on_one_device(K, V, slots, K_pages, V_pages)
+    if K.dim() != 4 or K.shape != V.shape:
+        raise ValueError("expected K, V [B, Hkv, N, D] of one shape")
+    if K.dtype not in _DTYPE_CODE or V.dtype != K.dtype:
+        raise TypeError(f"K and V must share one of fp32/fp16/bf16; got {K.dtype}, {V.dtype}")
+    B, Hkv, N, D = K.shape
+    _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
+    slots = _ints(slots, torch.int64, (B, N), "slots")
+    with _on_device(dev):
+        rc = _lib.load().dropkv_store_rows(
+            K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(),
+            K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
+            *_rows_strides(V_pages, "V_pages"), K_pages.shape[0], K_pages.shape[2], K.element_size(), B, Hkv, N, D,
+            _stream(dev))
+        _lib.check(rc, "dropkv_store_rows")
+
+
+def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False, V: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                 K_pages: Optional[torch.Tensor] = None, V_pages: Optional[torch.Tensor] = None):
+    """(Q_out, K_out): the heads of Q [B, Hq, L, D] and K [B, Hkv, L, D] (any strides,
+    rows of D contiguous) normed and rotated, contiguous and in the input dtype.
+
+    ``q_weight`` / ``k_weight`` [D]: RMS norm over each head with ``eps`` and that weight
+    (None: no norm). ``cos`` / ``sin`` [P, R / 2] fp32: the first R elements of a head
+    turn by row ``positions`` ([B, L] or [L], int64) of them, in pairs (i, i + R / 2), or
+    (2i, 2i + 1) if ``interleaved``; a position outside [0, P) gives NaN. After an
+    eviction positions go on from the tokens seen, not from the rows stored, and a drafted
+    node's position is its depth's. With ``V``, ``slots`` [B, L], ``K_pages`` and
+    ``V_pages`` the finished K rows and V's also go to the pool, as ``store_rows`` puts
+    them. fp32, fp16 or bf16; sums in fp32, rounded once.
+    """
+    cache = [t for t in (V, slots, K_pages, V_pages) if t is not None]
+    if cache and len(cache) != 4:
+        raise ValueError("V, slots, K_pages and V_pages go together")
+    dev = _on_one_device(Q, K, cos, sin, positions, *[t for t in (q_weight, k_weight) if t is not None], *cache)
+    if Q.dim() != 4 or K.dim() != 4 or Q.shape[0] != K.shape[0] or Q.shape[2:] != K.shape[2:]:
+        raise ValueError(f"expected Q [B,Hq,L,D] and K [B,Hkv,L,D], got {tuple(Q.shape)} and {tuple(K.shape)}")
+    dt = _DTYPE_CODE.get(Q.dtype)
+    if dt is None or K.dtype != Q.dtype:
+        raise TypeError(f"Q and K must share one of fp32/fp16/bf16; got {Q.dtype}, {K.dtype}")
+    B, Hq, L, D = Q.shape
+    Hkv = K.shape[1]
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError(f"cos and sin must be [P, R / 2] of one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("cos and sin must be float32")
+    cos, sin = cos.contiguous(), sin.contiguous()
+    if positions.dim() == 1:
+        positions, pos_sb = _ints(positions, torch.int64, (L,), "positions"), 0
+    else:
+        positions, pos_sb = _ints(positions, torch.int64, (B, L), "positions"), L
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (D,) or w.dtype != Q.dtype):
+            raise ValueError(f"{name} must be [{D}] {Q.dtype}, got {tuple(w.shape)} {w.dtype}")
+    q_weight = q_weight.contiguous() if q_weight is not None else None
+    k_weight = k_weight.contiguous() if k_weight is not None else None
+    if cache:
+        if V.shape != K.shape or V.dtype != K.dtype:
+            raise ValueError(f"V must be {tuple(K.shape)} {K.dtype}, got {tuple(V.shape)} {V.dtype}")
+        _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
+        slots = _ints(slots, torch.int64, (B, L), "slots")
+        tail = (V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(), K_pages.data_ptr(),
+                *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(), *_rows_strides(V_pages, "V_pages"),
+                K_pages.shape[0], K_pages.shape[2])
+    else:
+        tail = (None, 0, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, 0, 1)
+    with _on_device(dev):
+        q_out = torch.empty(B, Hq, L, D, dtype=Q.dtype, device=dev)
+        k_out = torch.empty(B, Hkv, L, D, dtype=Q.dtype, device=dev)
+        rc = _lib.load().dropkv_qk_norm_rope(
+            Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
+            q_weight.data_ptr() if q_weight is not None else None,
+            k_weight.data_ptr() if k_weight is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(),
+            cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
+            D, q_out.data_ptr(), k_out.data_ptr(), *tail, _stream(dev))
+        _lib.check(rc, "dropkv_qk_norm_rope")
+    return q_out, k_out
+
+
+def tree_mask_from_parents(parents: torch.Tensor):
+    """(mask, depth) of draft trees given by parents [..., T] (the index of a node's
+    parent, below its own; -1 for a child of the last cached token): mask
+    [..., T, T] bool shows each node its ancestors and itself, depth [..., T] int64
+    counts its ancestors (its position after the last cached token's). On the
+    parents' device, without synchronising."""
+    T = parents.shape[-1]
+    node = torch.arange(T, device=parents.device)
+    mask = (parents.unsqueeze(-1) == node) | torch.eye(T, dtype=torch.bool, device=parents.device)
+    n = 1
+    while n < T:  # nodes within n steps up, doubled (counts stay exact: at most T)
+        mask = (mask.float() @ mask.float()) > 0
+        n *= 2
+    return mask, mask.sum(-1) - 1
+
+
+def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens: torch.Tensor,
+                   tree_mask: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of a tree of T drafted tokens over a cache: Q [B, Hq, T, D] (any
+    strides) -> [B, Hq, T, D].
+
+    Row b's cache holds ``cache_lens[b]`` (int32, on the device) rows, and after them the
+    tree's own K/V rows in node order. Node i sees every cached row and the nodes j with
+    ``tree_mask[i, j]`` (bool [T, T] or [B, T, T]; None: j <= i, a chain). K and V are
+    row buffers [B, Hkv, cap, D] or, with ``block_table`` ([B, max_blocks] int32), pools
+    [pages, Hkv, block_size, D]; any strides with contiguous rows on 16-byte boundaries.
+    Rows past the capacity are not seen, nor are those on missing pages (-1); a node that
+    sees nothing gives zeros; what is in rows that no node sees does not matter. bf16 or
+    fp16, D 64 or 128, T <= 256, block_size a power of two from 8 to 1024. Products of 16
+    bits, sums and softmax statistics in fp32.
+    """
+    dev = _on_one_device(Q, K, V, cache_lens, *[t for t in (tree_mask, block_table) if t is not None])
+    if Q.dim() != 4 or K.dim() != 4 or K.shape != V.shape:
+        raise ValueError("expected Q [B,Hq,T,D] and K, V [B,Hkv,cap,D] or [pages,Hkv,block_size,D] of one shape")
+    if not (Q.dtype == K.dtype == V.dtype) or Q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("tree attention takes bf16 or fp16 Q, K and V of one dtype")
+    B, Hq, T, D = Q.shape
+    n0, Hkv, rows, Dk = K.shape
+    if Dk != D or Hq % Hkv or (block_table is None and n0 != B):
+        raise ValueError(f"shape mismatch: Q {tuple(Q.shape)}, K {tuple(K.shape)}")
+    cache_lens = _ints(cache_lens, torch.int32, (B,), "cache_lens")
+    if block_table is not None:
+        if block_table.dim() != 2:
+            raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
+        block_table = _ints(block_table, torch.int32, (B, block_table.shape[1]), "block_table")
+        paging = (block_table.data_ptr(), block_table.shape[1], rows, n0)
+        cap = block_table.shape[1] * rows
+    else:
+        paging = (None, 0, 0, 0)
+        cap = rows
+    mask = (None, 0, 0, 0)
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.bool:
+            raise TypeError(f"tree_mask must be bool, got {tree_mask.dtype}")
+        if tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
+            raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(tree_mask.shape)}")
+        mask = (tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2),
+                tree_mask.stride(-1))
+    scale = float(D ** -0.5 if scale is None else scale)
+    lib = _lib.load()
+    with _on_device(dev):
+        out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=dev)
+        if B == 0 or T == 0:
+            return out
+        # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
+        ws = _workspace(lib.dropkv_tree_attention_workspace_size(B, Hq, Hkv, T, D, cap), dev)
+        rc = lib.dropkv_tree_attention(
+            Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
+            *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
+            out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
+        _lib.check(rc, "dropkv_tree_attention")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
+                   temperature: float = 1.0) -> TokenLogprobs:
+    """Under softmax(logits / temperature) for rows of logits [..., V] (fp32, fp16 or
+    bf16): log probabilities of ``tokens`` (int64, [...] or [..., C]; -inf for one outside
+    [0, V), such as a draft tree's padding), the entropy of each row, and its ``top_k``
+    (at most 64) likeliest tokens, best first, ties to the lower index. fp32 sums and
+    results. A row that holds NaN or +inf, or nothing but -inf, gives NaN."""
+    dev = _on_one_device(logits, tokens)
+    dt = _DTYPE_CODE.get(logits.dtype)
+    if dt is None:
+        raise TypeError(f"logits must be fp32/fp16/bf16; got {logits.dtype}")
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"tokens must be int64, got {tokens.dtype}")
+    if logits.dim() < 1 or tokens.dim() - logits.dim() not in (-1, 0) or tokens.shape[:logits.dim() - 1] != logits.shape[:-1]:
+        raise ValueError(f"expected logits [..., V] and tokens [...] or [..., C], got {tuple(logits.shape)} and "
+                         f"{tuple(tokens.shape)}")
+    V = logits.shape[-1]
+    lead = logits.shape[:-1]
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if V > 1 and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    N = rows.shape[0]
+    C = tokens.shape[-1] if tokens.dim() == logits.dim() else 1
+    tokens = tokens.contiguous()
+    lib = _lib.load()
+    with _on_device(dev):
+        logprob = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+        top_lp = torch.empty(*lead, top_k, dtype=torch.float32, device=dev) if top_k else None
+        top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
+        ws = _workspace(lib.dropkv_token_logprobs_workspace_size(N, V, int(top_k)), dev)
+        rc = lib.dropkv_token_logprobs(rows.data_ptr(), rows.stride(0), dt, N, V, tokens.data_ptr(), C, int(top_k),
+                                       float(temperature), logprob.data_ptr(), entropy.data_ptr(),
+                                       top_lp.data_ptr() if top_k else None, top_id.data_ptr() if top_k else None,
+                                       ws.data_ptr(), ws.numel(), _stream(dev))
+        _lib.check(rc, "dropkv_token_logprobs")
+    return TokenLogprobs(logprob, entropy, top_lp, top_id)

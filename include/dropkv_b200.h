@@ -301,6 +301,89 @@ DROPKV_API int dropkv_decode_append_attention(const void* q, int64_t q_sb, int64
                                               float scale, void* out, void* workspace, size_t workspace_bytes,
                                               void* stream);
 
+/* ---- Paged caches and the speculative decode step ---------------------------
+ * A batch of compressed caches in the pages of a shared pool: K and V pages are
+ * [n_pages, Hkv, block_size, D] with element strides per page, head and row (rows
+ * of D contiguous); slot s is row s % block_size of page s / block_size. No
+ * counterparts in the reference, whose cache is one tensor per layer. Shapes,
+ * strides and pointers are checked here; lengths, page numbers and slots live on
+ * the device and are bounded by the kernels: nothing outside the given arrays is
+ * read or written, whatever they hold. */
+
+/* Block tables and slot maps from request lengths on the device. lens[b]: tokens
+ * request b's cache holds once this step is done; new_lens[b] of them (NULL: all)
+ * are new, the last ones. held[b] (with table_in; both NULL: none) pages are in
+ * row b of table_in ([B, max_blocks], table_in_stride between rows) already; the
+ * missing min(ceil(lens[b] / block_size), max_blocks) - held[b] are taken from
+ * free_blocks[n_free] in order, request after request.
+ *   table[B, max_blocks]  page numbers, -1 past a request's pages
+ *   held_out[B]           pages each request holds now
+ *   slots[B, max_new]     slot of each new token, -1 past new_lens[b] and where no page is left
+ *   used[1]               free pages asked for (more than n_free: some requests went short)
+ * Negative lengths count as 0, new_lens[b] above lens[b] as lens[b]. Outputs and
+ * inputs must not overlap. block_size >= 1, B <= 65535. */
+DROPKV_API int dropkv_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* table_in,
+                                   int64_t table_in_stride, const int32_t* held, int B, int block_size,
+                                   const int32_t* free_blocks, int n_free, int max_blocks, int max_new,
+                                   int32_t* table, int32_t* held_out, int64_t* slots, int64_t* used, void* stream);
+
+/* k_pages / v_pages row slots[b, n] = row n of K / V [B, Hkv, N, D] for every head;
+ * slots outside the pool are skipped. Element strides: k_s* / v_s* of a sequence,
+ * head and row, kp_s* / vp_s* of a page, head and row. elem_bytes 2 or 4. Of rows
+ * with one slot any may stay. */
+DROPKV_API int dropkv_store_rows(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sb,
+                                 int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages, int64_t kp_sb,
+                                 int64_t kp_sh, int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh,
+                                 int64_t vp_st, int n_pages, int block_size, int elem_bytes, int B, int Hkv, int N,
+                                 int D, void* stream);
+
+/* Heads of Q [B, Hq, L, D] and K [B, Hkv, L, D] normed (RMS over D, eps, weight
+ * q_weight / k_weight [D]; NULL: not normed) and their first R elements rotated by
+ * cos / sin [P, R / 2] (fp32) at positions[b * pos_sb + l]: pairs (i, i + R / 2),
+ * or (2i, 2i + 1) if `interleaved`. q_out, k_out contiguous, in the input dtype
+ * (fp32, fp16 or bf16), rounded once. With slots[B, L] (else NULL, and v and the
+ * pages too) K's rows and V's (as they are) also go to their pages. R even, R <= D;
+ * a position outside [0, P) gives NaN rows. q_out / k_out may not overlap inputs. */
+DROPKV_API int dropkv_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl, const void* k,
+                                   int64_t k_sb, int64_t k_sh, int64_t k_sl, const void* q_weight,
+                                   const void* k_weight, float eps, const float* cos, const float* sin, int P, int R,
+                                   int interleaved, const int64_t* positions, int64_t pos_sb, int dtype, int B, int Hq,
+                                   int Hkv, int L, int D, void* q_out, void* k_out, const void* v, int64_t v_sb,
+                                   int64_t v_sh, int64_t v_sl, const int64_t* slots, void* k_pages, int64_t kp_sb,
+                                   int64_t kp_sh, int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh,
+                                   int64_t vp_st, int n_pages, int block_size, void* stream);
+
+/* Attention of a tree of T drafted tokens (their K/V rows in the cache after the
+ * cache_lens[b] rows of sequence b, at cache_lens[b] + node): out[b, h, i, :] =
+ * softmax(scale q[b, h, i, :] . K) V over every cached row and the nodes j with
+ * mask[b * mask_sb + i * mask_sr + j * mask_sc] != 0 (bytes; NULL: j <= i, a chain).
+ * K and V are row buffers [B, Hkv, cap, D] (table NULL; s0 strides of a sequence)
+ * or pages [n_pages, Hkv, block_size, D] (s0 strides of a page; table
+ * [B, max_blocks], cap = max_blocks * block_size). Rows past cap are not seen; a
+ * row that sees nothing gives zeros; keys on pages outside the pool are not seen.
+ * A row that no node sees is not used, whatever it holds. bf16 or fp16, D 64 or 128,
+ * T <= 256, block_size a power of two from 8 to 1024, K/V rows on 16-byte
+ * boundaries; out [B, Hq, T, D] contiguous. */
+DROPKV_API size_t dropkv_tree_attention_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
+DROPKV_API int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd,
+                                     const void* k, int64_t k_s0, int64_t k_sh, int64_t k_ss, const void* v,
+                                     int64_t v_s0, int64_t v_sh, int64_t v_ss, const int32_t* table, int max_blocks,
+                                     int block_size, int n_pages, const int32_t* cache_lens, const uint8_t* mask,
+                                     int64_t mask_sb, int64_t mask_sr, int64_t mask_sc, int dtype, int B, int Hq,
+                                     int Hkv, int T, int D, int cap, float scale, void* out, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* For each row of logits [N, V] (row_stride elements apart, fp32 / fp16 / bf16) and
+ * p = softmax(logits / temperature): logprob[N, C] = log p of tokens[N, C] (-inf for
+ * a token outside [0, V)), entropy[N] = -sum p log p, and the top_k (0 to 64) most
+ * likely tokens, best first, ties to the lower index, with their log probabilities.
+ * A row with NaN or +inf, or of -inf alone, gives NaN (top_tokens order NaN first). */
+DROPKV_API size_t dropkv_token_logprobs_workspace_size(int64_t N, int V, int top_k);
+DROPKV_API int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t N, int V,
+                                     const int64_t* tokens, int C, int top_k, float temperature, float* logprob,
+                                     float* entropy, float* top_logprobs, int64_t* top_tokens, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 /* Diagnostic: one 128-row tile through a tcgen05 MMA form used by the fused
  * scorer (mode 0: out[128][n] = A[128][128] B[n][128]^T with A loaded by TMA;
  * mode 1: out[128][n] = A[128][128]^T B[n][128]^T with A read MN-major; modes 2/3:
