@@ -83,7 +83,7 @@ int make_kv_tensor_map(CUtensorMap* map, const void* base, int BH, int L, int D,
 }
 
 int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, int L, int D, bool bf16, int64_t sb,
-                          int64_t sh, int64_t ss) {
+                          int64_t sh, int64_t ss, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(DROPKV_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   if (reinterpret_cast<uintptr_t>(base) % 16) return fail(DROPKV_ERR_ARG, "K/V must be 16-byte aligned");
@@ -91,7 +91,7 @@ int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, in
     return fail(DROPKV_ERR_ARG, "K/V strides must be multiples of 8 elements");
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)Hkv, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)ss * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -240,6 +240,31 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
 }
 
 // ---------------------------------------------------------------------------
+// Stores to TMEM, and matrix products whose A operand lies there
+// ---------------------------------------------------------------------------
+// 16 consecutive 32-bit columns of this thread's TMEM lane written; tmem_st_wait() waits for the stores.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n"
+      :
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16: a lane of A holds a row of M, a
+// 32-bit column two consecutive elements of K.
+__device__ __forceinline__ void mma_f16_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// ---------------------------------------------------------------------------
 // Descriptors
 // ---------------------------------------------------------------------------
 // tcgen05 descriptor layout codes (bits 61-63)
@@ -297,8 +322,8 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int M, int N, bool a
 // head_stride: elements between consecutive [L, D] heads (0: L * D, contiguous).
 int make_kv_tensor_map(CUtensorMap* map, const void* base, int BH, int L, int D, bool bf16, int64_t head_stride = 0);
 // K or V [B, Hkv, L, D] with element strides (sb, sh, ss) and rows of D contiguous
-// elements, as a 4-D map {d, key, head, b} of 64 x 128 boxes (128-byte swizzle).
+// elements, as a 4-D map {d, key, head, b} of 64 x box_rows boxes (128-byte swizzle).
 int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, int L, int D, bool bf16, int64_t sb,
-                          int64_t sh, int64_t ss);
+                          int64_t sh, int64_t ss, int box_rows = 128);
 
 }  // namespace dropkv

@@ -1,93 +1,809 @@
 // Attention of a tree of drafted tokens over a cache: for sequence b, query head h
 // and node i, O = sum_j softmax_j(scale q_i . k_j) v_j over the len_b cached rows
 // and the tree's nodes j (rows len_b + j of the cache) that mask[i][j] shows.
-#include "common.cuh"
+//
+// The M = g T query rows of a KV head read the same keys, so a tile of 128 keys is
+// fetched once for up to 256 rows: 4 D bytes and 4 D M operations a key, which HBM
+// bounds below about 250 rows and the tensor cores above. Both products run on
+// them: S = Q K^T with Q and K in shared memory, O += P V with the weights P left in
+// tensor memory, where S was. One warp issues the TMA loads (a box per page), one
+// the products, and two groups of four warps do the softmax, a thread for each row:
+//   * up to 128 rows: both groups have the same rows and take key tiles in turn,
+//     each with a maximum, a sum and an output of its own, joined at the end;
+//   * above: each group has 128 rows, and both use every key tile.
+// Either way one group's softmax runs beside the products of the other.
+//
+// The keys of all (sequence, KV head, group of 256 rows) segments form one line of
+// tiles that is cut evenly over the CTAs, one to an SM, from the lengths on the
+// device: a ragged batch is balanced without the host knowing it. A segment that
+// falls into several CTAs leaves partials (output, maximum, sum; fp32) in the
+// workspace, and a second kernel joins them in the order of the CTAs. No CTA waits
+// for another.
+#include <algorithm>
+#include <type_traits>
+
+#include "tc_common.cuh"
 
 namespace dropkv {
 namespace {
 
-constexpr int TA_NT = 128;
+constexpr int TA_TK = 128;               // keys of a tile
+constexpr int TA_ROWS = 256;             // query rows of a segment
+constexpr int TA_NT = 256 + 64;          // two softmax groups, a TMA warp, an MMA warp
+constexpr int TA_WARP_TMA = 8, TA_WARP_MMA = 9;
+constexpr uint64_t kTaWaitNs = 1000000000ull;
+// The reference a row's weights are taken against is moved only when its maximum has
+// grown by this much (base 2): weights then stay below 2^8, and the accumulated
+// output, in tensor memory, is hardly ever rescaled.
+constexpr float kTaSlack = 8.f;
 
-// Row `key` of KV head h: in a row buffer, or in the page the table names (nullptr:
-// no such page).
+struct TaArgs {
+  TreeAttn a;
+  int g, M, RT;            // query rows of a KV head: M = g T, in RT segments of 256
+  int box;                 // rows of a TMA box
+  int rows_pad;            // rows of a partial
+  float scale_log2;
+  float bias;              // weights are 2^(s - m + bias): fp16 has few bits below 1
+  int* status;             // [CTAs]: 0, or which wait gave up
+  float* part_o;           // [2 CTAs][D / 4][rows_pad] float4
+  float* part_ml;          // [2 CTAs][2][rows_pad]
+};
+
+template <int D>
+struct TaSmem {
+  static constexpr int TILE = TA_TK * D * 2;  // K, V or Q tile: D / 64 slabs of 128 rows x 128 B
+  static constexpr int SLOTS = D == 128 ? 5 : 10;
+  static constexpr int Q = 0;                 // two tiles; a group's maxima and sums once its products are done
+  static constexpr int RING = 2 * TILE;
+  static constexpr int BARS = RING + SLOTS * TILE;        // full[SLOTS], empty[SLOTS], then B_*
+  static constexpr int BAD = BARS + (2 * SLOTS + 10) * 8;  // uint32 [2][8]: nodes with non-finite V
+  static constexpr int MISC = BAD + 64;
+  static constexpr int BYTES = MISC + 64;
+  static constexpr int ALLOC = BYTES + 1024;  // the base is aligned to 1024
+};
+static_assert(TaSmem<128>::ALLOC <= 232448, "shared memory");
+
+// per softmax group s: Q written, S ready, P ready, O ready; and: every product done
+enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_END = 8 };
+
+struct TaMisc {
+  long long w0, w1, base;  // this CTA's tiles, and the first tile of sequence b0
+  int b0;
+  uint32_t tmem;
+  int dead;
+};
+
+// Keys of sequence b (cached rows and nodes that fit), its cached rows, its tiles.
+__device__ __forceinline__ int ta_len(const TreeAttn& a, int b) { return min(max(a.cache_lens[b], 0), a.cap); }
+__device__ __forceinline__ int ta_keys(const TreeAttn& a, int len) { return (int)min((int64_t)len + a.T, (int64_t)a.cap); }
+__device__ __forceinline__ int ta_tiles(const TreeAttn& a, int b) { return (ta_keys(a, ta_len(a, b)) + TA_TK - 1) / TA_TK; }
+
+// A CTA's part of one segment: tiles [t0, t1) of sequence b, KV head h, row group rt.
+struct TaPiece {
+  int b, h, rt, t0, t1, tiles, len, keys, rows;
+  bool two;    // two groups of rows, else tiles in turn
+  int items;   // (tile, group) pairs
+};
+
+// Steps through a CTA's pieces; every role has one of its own and sees the same.
+struct TaWalk {
+  long long w, w1, base;
+  int b;
+  __device__ __forceinline__ bool next(const TaArgs& A, TaPiece& p) {
+    if (w >= w1) return false;
+    const TreeAttn& a = A.a;
+    p.b = b;
+    p.len = ta_len(a, b);
+    p.keys = ta_keys(a, p.len);
+    p.tiles = (p.keys + TA_TK - 1) / TA_TK;
+    const long long rel = w - base;
+    const int seg = (int)(rel / p.tiles);
+    p.t0 = (int)(rel - (long long)seg * p.tiles);
+    p.t1 = (int)min((long long)p.tiles, p.t0 + (w1 - w));
+    p.h = seg / A.RT;
+    p.rt = seg % A.RT;
+    p.rows = min(TA_ROWS, A.M - p.rt * TA_ROWS);
+    p.two = p.rows > 128;
+    p.items = (p.t1 - p.t0) * (p.two ? 2 : 1);
+    w += p.t1 - p.t0;
+    if (w - base == (long long)p.tiles * a.Hkv * A.RT) {
+      base = w;
+      ++b;
+    }
+    return true;
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ const T* ta_row(const TreeAttn& a, const void* base, int64_t s0, int64_t sh, int64_t ss, int b,
-                                           int h, int key) {
-  const T* p = static_cast<const T*>(base);
-  if (!a.table) return p + b * s0 + h * sh + key * ss;
-  const int page = a.table[b * (int64_t)a.max_blocks + key / a.block];
-  if (page < 0 || page >= a.n_pages) return nullptr;
-  return p + page * s0 + h * sh + (key % a.block) * ss;
+struct TaType;
+template <>
+struct TaType<__nv_bfloat16> {
+  static constexpr uint32_t kInf = 0x7F80u;  // the exponent bits
+  static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+template <>
+struct TaType<__half> {
+  static constexpr uint32_t kInf = 0x7C00u;
+  static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ float ta_ex2(float x) {  // 2^x, hardware approximation; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T>
-__device__ __forceinline__ T ta_from(float x);
-template <>
-__device__ __forceinline__ __half ta_from<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 ta_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+// What a partial of maximum m weighs under the joint maximum `to`; parts that saw
+// nothing (or NaN alone) have -inf, which must not turn into NaN (or hide it).
+__device__ __forceinline__ float ta_factor(float m, float to) { return m == to ? 1.f : ta_ex2(m - to); }
 
-// One CTA per (b, query head, node): TA_NT keys at a time, a thread for each key's
-// score, then a thread for each column of the output.
+// A word with its non-finite halves zeroed; *bad is set if there were any.
 template <typename T>
-__global__ void __launch_bounds__(TA_NT) tree_attn_rows_kernel(TreeAttn a) {
-  __shared__ float q[128], p[TA_NT], red[TA_NT / 32];
-  const int tid = threadIdx.x, b = blockIdx.y, hq = blockIdx.x / a.T, i = blockIdx.x % a.T;
-  const int h = hq / (a.Hq / a.Hkv);
-  const int len = min(max(a.cache_lens[b], 0), a.cap), keys = min((int64_t)len + a.T, (int64_t)a.cap);
-  if (tid < a.D) q[tid] = to_f(static_cast<const T*>(a.q)[b * a.q_sb + hq * a.q_sh + i * a.q_ss + tid * a.q_sd]) * a.scale;
-  const uint8_t* mask = a.mask ? a.mask + b * a.mask_sb + i * a.mask_sr : nullptr;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int j0 = 0; j0 < keys; j0 += TA_NT) {
-    __syncthreads();
-    const int j = j0 + tid;
-    float s = -INFINITY;
-    const T* kr = nullptr;
-    if (j < keys && (j < len || (mask ? mask[(j - len) * a.mask_sc] != 0 : j - len <= i)))
-      kr = ta_row<T>(a, a.k, a.k_s0, a.k_sh, a.k_ss, b, h, j);
-    if (kr) {
-      s = 0.f;
-      for (int d = 0; d < a.D; ++d) s = fmaf(q[d], to_f(kr[d]), s);
+__device__ __forceinline__ uint32_t ta_finite(uint32_t x, bool* bad) {
+  constexpr uint32_t E = TaType<T>::kInf;
+  if ((x & E) == E) x &= 0xFFFF0000u, *bad = true;
+  if ((x & (E << 16)) == (E << 16)) x &= 0x0000FFFFu, *bad = true;
+  return x;
+}
+
+__device__ __forceinline__ void ta_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TA_NT, 1)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, TaArgs A) {
+  using L = TaSmem<D>;
+  constexpr int SLABS = D / 64, NS = L::SLOTS;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::BARS);
+  uint64_t* empty = full + NS;
+  uint64_t* bars = empty + NS;
+  uint32_t* bad = reinterpret_cast<uint32_t*>(sm + L::BAD);
+  TaMisc* misc = reinterpret_cast<TaMisc*>(sm + L::MISC);
+  volatile int* dead = &misc->dead;
+  const TreeAttn& a = A.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
     }
-    float mx = s;
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(&bars[B_Q + s], 128);
+      tc::mbar_init(&bars[B_S + s], 1);
+      tc::mbar_init(&bars[B_P + s], 128);
+      tc::mbar_init(&bars[B_O + s], 1);
+    }
+    tc::mbar_init(&bars[B_END], 1);
+    tc::fence_mbar_init();
+    misc->dead = 0;
+  }
+  if (tid < 16) bad[tid] = 0;
+  if (warp == TA_WARP_MMA) {
+    tc::tmem_alloc(&misc->tmem, 512);
+    tc::tmem_relinquish();
+  }
+  if (warp == TA_WARP_TMA && lane == 0) {
+    tc::tma_prefetch_desc(&kmap);
+    tc::tma_prefetch_desc(&vmap);
+  }
+  pdl_launch_dependents();
+  pdl_wait();
+  if (warp == 0) {  // where this CTA's share of the line of tiles starts
+    const long long HR = (long long)a.Hkv * A.RT;
+    long long total = 0;
+    for (int b = lane; b < a.B; b += 32) total += ta_tiles(a, b);
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    const float mn = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-    const float use = mn == -INFINITY ? 0.f : mn;
-    p[tid] = kr ? __expf(s - use) : -1.f;  // -1: not seen
-    const float alpha = __expf(m - use);
-    m = mn;
-    __syncthreads();
-    o *= alpha;
-    l *= alpha;
-    for (int t = 0; t < TA_NT && j0 + t < keys; ++t) {
-      const float w = p[t];
-      if (w == -1.f) continue;
-      l += w;
-      if (tid < a.D) o = fmaf(w, to_f(ta_row<T>(a, a.v, a.v_s0, a.v_sh, a.v_ss, b, h, j0 + t)[tid]), o);
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const long long W = total * HR, per = max(1ll, (W + gridDim.x - 1) / gridDim.x);
+    const long long w0 = min(W, per * blockIdx.x), w1 = min(W, w0 + per);
+    long long before = 0;
+    if (w0 < w1) {
+      for (int c = 0; c < a.B; c += 32) {
+        const long long own = c + lane < a.B ? ta_tiles(a, c + lane) : 0;
+        long long upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * HR > w0);
+        if (past) {
+          const int at = __ffs(past) - 1;
+          if (lane == at) {
+            misc->b0 = c + at;
+            misc->base = (before + upto - own) * HR;
+          }
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      misc->w0 = w0;
+      misc->w1 = w1;
     }
   }
-  if (tid < a.D)
-    static_cast<T*>(a.out)[((b * (int64_t)a.Hq + hq) * a.T + i) * a.D + tid] = ta_from<T>(l == 0.f ? 0.f : o / l);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = misc->tmem;
+  TaWalk walk{misc->w0, misc->w1, misc->base, misc->b0};
+  TaPiece p;
+  // a wait that gives up marks the CTA dead: every role then ends without waiting
+  int code = 0;
+  auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
+    if (*dead) return false;
+    if (tc::mbar_wait(bar, count & 1, kTaWaitNs)) return true;
+    *dead = code = why;
+    return false;
+  };
+
+  if (warp == TA_WARP_TMA) {
+    // ======================= TMA producer =======================================
+    // Order of use: K tiles run one tile ahead of V (two where groups take tiles in turn).
+    uint32_t k = 0;  // ring position
+    const int boxes = TA_TK / A.box;
+    while (walk.next(A, p)) {
+      const int nt = p.t1 - p.t0, lead = p.two ? 1 : 2;
+      auto load = [&](const CUtensorMap* map, int tile) {
+        const uint32_t slot = k % NS;
+        if (k >= (uint32_t)NS && !__all_sync(0xffffffffu, wait(&empty[slot], k / NS - 1, 1))) return false;
+        if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], L::TILE);
+        __syncwarp();
+        if (lane < boxes) {
+          const int key = tile * TA_TK + lane * A.box;
+          int row = key, outer = p.b;
+          if (a.table) {
+            // a box past the keys, or on no page of the pool, is out of range: zeros
+            const int col = key / a.block;
+            outer = key < p.keys ? a.table[(int64_t)p.b * a.max_blocks + col] : -1;
+            if (outer < 0 || outer >= a.n_pages) outer = a.n_pages;
+            row = key - col * a.block;
+          }
+          uint8_t* dst = sm + L::RING + slot * L::TILE + lane * A.box * 128;
+#pragma unroll
+          for (int s = 0; s < SLABS; ++s)
+            tc::tma_load_4d(dst + s * (TA_TK * 128), map, &full[slot], 64 * s, row, p.h, outer);
+        }
+        __syncwarp();
+        ++k;
+        return true;
+      };
+      bool ok = true;
+      for (int i = 0; i < min(lead, nt) && ok; ++i) ok = load(&kmap, p.t0 + i);
+      for (int i = 0; i < nt && ok; ++i) {
+        ok = load(&vmap, p.t0 + i);
+        if (ok && i + lead < nt) ok = load(&kmap, p.t0 + i + lead);
+      }
+      if (!ok) break;
+    }
+    if (*dead) {  // every issued copy lands before the CTA may exit
+      for (uint32_t j = k > (uint32_t)NS ? k - NS : 0u; j < k; ++j) tc::mbar_wait(&full[j % NS], (j / NS) & 1, kTaWaitNs);
+    }
+  } else if (warp == TA_WARP_MMA) {
+    // ======================= MMA issuer =========================================
+    if (lane == 0) {
+      constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
+      constexpr uint32_t ID_PV = tc::idesc_f16(BF16, 128, D, false, true);
+      constexpr uint32_t LBO_V = SLABS == 2 ? TA_TK * 128 : 0;
+      const uint32_t ring0 = tc::smem_addr(sm + L::RING);
+      uint64_t qd[2];
+      for (int s = 0; s < 2; ++s) qd[s] = tc::smem_desc(tc::smem_addr(sm + L::Q + s * L::TILE), 16, 1024);
+      uint32_t k = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+      bool ok = true;
+      while (ok && walk.next(A, p)) {
+        const int per_tile = p.two ? 2 : 1, lead = p.two ? 1 : 2;
+        // ring positions: K_i is load number i (i < lead) or lead + 2 (i - lead) + 1, V_i number lead + 2 i,
+        // short of the K loads that do not exist
+        const int nt = p.t1 - p.t0, ahead = min(lead, nt);
+        auto k_at = [&](int i) { return k + (i < lead ? i : lead + 2 * (i - lead) + 1); };
+        auto v_at = [&](int i) { return k + ahead + i + min(i, max(nt - lead, 0)); };
+        auto qk = [&](int item) {
+          const int s = item & 1, i = item / per_tile;
+          const uint32_t at = k_at(i), slot = at % NS;
+          if (item < 2 && !wait(&bars[B_Q + s], n_q[s]++, 2)) return false;
+          if (!wait(&full[slot], at / NS, 3)) return false;
+          tc::tc_fence_after();
+          const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
+            tc::mma_f16(tmem + s * 128, tc::desc_add(qd[s], off), tc::desc_add(kd, off), ID_QK, kk > 0);
+          }
+          tc::mma_commit(&bars[B_S + s]);
+          if (!p.two || s == 1) tc::mma_commit(&empty[slot]);
+          return true;
+        };
+        for (int item = 0; item < min(2, p.items) && ok; ++item) ok = qk(item);
+        for (int item = 0; item < p.items && ok; ++item) {
+          const int s = item & 1, i = item / per_tile;
+          const uint32_t at = v_at(i), slot = at % NS;
+          ok = wait(&full[slot], at / NS, 4) && wait(&bars[B_P + s], n_p[s]++, 5);
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
+#pragma unroll
+          for (int kk = 0; kk < TA_TK / 16; ++kk)
+            tc::mma_f16_tmem_a(tmem + 256 + s * 128, tmem + s * 128 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV,
+                               item >= 2 || kk > 0);
+          if (!p.two || s == 1) tc::mma_commit(&empty[slot]);
+          if (item + 2 < p.items)
+            ok = qk(item + 2);
+          else
+            tc::mma_commit(&bars[B_O + s]);
+        }
+        k += 2 * nt;
+      }
+      if (*dead) {  // no product may run on when tensor memory is given back
+        tc::mma_commit(&bars[B_END]);
+        tc::mbar_wait(&bars[B_END], 0, kTaWaitNs);
+      }
+    }
+  } else {
+    // ======================= softmax groups =====================================
+    const int s = warp >> 2, r = tid & 127;  // group and TMEM lane
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256;
+    float* ml0 = reinterpret_cast<float*>(sm + L::Q);  // [2][128]
+    float* ml1 = reinterpret_cast<float*>(sm + L::Q + L::TILE);
+    uint32_t n_s = 0, n_o = 0, k = 0;
+    bool ok = true;
+    for (int piece = 0; walk.next(A, p); ++piece) {
+      const int nt = p.t1 - p.t0;
+      const bool mine = p.two || s < nt;  // this group has work in the piece
+      const int row0 = p.rt * TA_ROWS + (p.two ? s * 128 : 0);  // the group's first row
+      const int rows = min(128, A.M - row0);
+      const bool live = (warp & 3) * 32 < rows;  // some row of this warp exists
+      uint32_t* bad_now = bad + 8 * (piece & 1);
+      float m = -INFINITY, l = 0.f;
+      uint32_t mw[8];  // nodes that this thread's row sees
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mw[i] = 0;
+      if (mine) {
+        // Q rows into shared memory, 16 bytes a thread: row = head of the group, then node
+        const bool vec = a.q_sd == 1 && ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_sb * 2) |
+                                          (uintptr_t)(a.q_sh * 2) | (uintptr_t)(a.q_ss * 2)) % 16) == 0;
+        const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh;
+        for (int e = r; e < 128 * (D / 8); e += 128) {
+          const int row = e / (D / 8), c = e % (D / 8);
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (row < rows) {
+            const int mrow = row0 + row;
+            const T* src = qb + (mrow / a.T) * a.q_sh + (mrow % a.T) * a.q_ss + c * 8 * a.q_sd;
+            if (vec) {
+              x = *reinterpret_cast<const uint4*>(src);
+            } else {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = (uint32_t) * reinterpret_cast<const uint16_t*>(src + 2 * i * a.q_sd) |
+                       ((uint32_t) * reinterpret_cast<const uint16_t*>(src + (2 * i + 1) * a.q_sd) << 16);
+              x = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
+                                    tc::sw128_offset(row, (c % 8) * 8)) = x;
+        }
+        tc::fence_proxy_async_smem();
+        tc::mbar_arrive(&bars[B_Q + s]);
+        // the mask's rows, where the piece reaches the tree: a warp reads each of its rows
+        if (p.t1 * TA_TK > p.len && live) {
+          const int fit = p.keys - p.len;  // nodes that fit the cache
+          for (int q = 0; q < 32 && (warp & 3) * 32 + q < rows; ++q) {
+            const int node = (row0 + (warp & 3) * 32 + q) % a.T;
+            const uint8_t* mr = a.mask ? a.mask + p.b * a.mask_sb + node * a.mask_sr : nullptr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (i * 32 >= fit) break;
+              const int j = i * 32 + lane;
+              const bool see = j < fit && (mr ? mr[j * a.mask_sc] != 0 : j <= node);
+              const uint32_t word = __ballot_sync(0xffffffffu, see);
+              if (q == lane) mw[i] = word;
+            }
+          }
+        }
+      }
+      const int lead = p.two ? 1 : 2, ahead = min(lead, nt);
+      for (int i = p.two ? 0 : s; i < nt && ok; i += p.two ? 1 : 2) {
+        const int j0 = (p.t0 + i) * TA_TK;
+        // which of the tile's pages exist (a lane for each): 16 bits, from 8 rows up
+        uint32_t gone = 0;
+        if (a.table) {
+          const int key = j0 + lane * A.box;
+          bool no = false;
+          if (lane < TA_TK / A.box && key < p.keys) {
+            const int page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
+            no = page < 0 || page >= a.n_pages;
+          }
+          gone = __ballot_sync(0xffffffffu, no);
+        }
+        const bool tree = j0 + TA_TK > p.len;  // the tile holds nodes, or ends the keys
+        ok = __all_sync(0xffffffffu, wait(&bars[B_S + s], n_s++, 6));
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (live) {
+          uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          const bool masked = tree || gone;
+          if (masked) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int at = j0 + 32 * w - p.len;  // the node of the word's first key, negative in the cache
+              uint32_t lo = 0, hi = 0;
+              const int q = at >> 5;               // rounds down
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                lo = q == i ? mw[i] : lo;
+                hi = q + 1 == i ? mw[i] : hi;
+              }
+              if (q < 0) lo = 0xffffffffu;
+              if (q + 1 < 0) hi = 0xffffffffu;
+              see[w] = __funnelshift_r(lo, hi, at & 31);
+              for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
+                if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+            }
+          }
+          // S is read twice, for the maximum and for the weights: a row of 128 does not stay in registers
+          float x[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            tc::tmem_ld32(ts + 32 * w, x);
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+          const bool grow = top > m + kTaSlack || m == -INFINITY;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? fmaxf(m, top) : m;
+            const float alpha = mn == -INFINITY ? 1.f : ta_ex2(m - mn);
+            m = mn;
+            l *= alpha;
+            if (i >= 2 || (p.two && i >= 1)) {  // something has been accumulated
+              float o[16];
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                tc::tmem_ld16(to + s * 128 + c, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                tc::tmem_st16(to + s * 128 + c, o);
+                tc::tmem_st_wait();
+              }
+            }
+          }
+          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {  // P's columns [16 w, 16 w + 16) lie in columns of S already read
+            tc::tmem_ld32(ts + 32 * w, x);
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float u = ta_ex2(fmaf(x[e], A.scale_log2, -ref)), v = ta_ex2(fmaf(x[e + 1], A.scale_log2, -ref));
+              sum[e & 3] += u;
+              sum[(e & 3) + 1] += v;
+              pk[e / 2] = TaType<T>::pack(u, v);
+            }
+            tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tc::tmem_st_wait();
+        }
+        if (tree) {
+          // rows of V that a weight of 0 would not silence: past the keys they are cleared, and
+          // non-finite values of a node are taken out here and given to its viewers at the end
+          const uint32_t at = k + ahead + i + min(i, max(nt - lead, 0)), slot = at % NS;
+          ok = __all_sync(0xffffffffu, wait(&full[slot], at / NS, 7));
+          if (!ok) break;
+          const int key = j0 + r;
+          if (key >= p.len) {
+            bool off = false;
+#pragma unroll 1
+            for (int c = 0; c < SLABS * 8; ++c) {
+              uint4* at = reinterpret_cast<uint4*>(sm + L::RING + slot * L::TILE + (c / 8) * (TA_TK * 128) + r * 128 +
+                                                   ((c + r) % 8) * 16);
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              bool change = true;
+              if (key < p.keys) {
+                v = *at;
+                change = false;
+                v.x = ta_finite<T>(v.x, &change);
+                v.y = ta_finite<T>(v.y, &change);
+                v.z = ta_finite<T>(v.z, &change);
+                v.w = ta_finite<T>(v.w, &change);
+                off |= change;
+              }
+              if (change) *at = v;
+            }
+            if (off) atomicOr(&bad_now[(key - p.len) >> 5], 1u << ((key - p.len) & 31));
+          }
+          tc::fence_proxy_async_smem();
+        }
+        tc::tc_fence_before();
+        tc::mbar_arrive(&bars[B_P + s]);
+      }
+      k += 2 * nt;
+      // ---- the piece's output ---------------------------------------------------
+      if (mine && ok) ok = __all_sync(0xffffffffu, wait(&bars[B_O + s], n_o++, 8));
+      m -= A.bias;  // the reference the weights were taken against
+      (s ? ml1 : ml0)[r] = m;
+      (s ? ml1 : ml0)[128 + r] = l;
+      ta_group_sync();
+      tc::tc_fence_after();
+      if (tid < 8) bad[8 * ((piece + 1) & 1) + tid] = 0;
+      const bool whole = p.t0 == 0 && p.t1 == p.tiles;
+      // rows in turn: this group writes columns [s D / 2, (s + 1) D / 2) of the joined
+      // output; else all columns of its own rows
+      const int c_lo = p.two ? 0 : s * (D / 2), c_hi = p.two ? D : c_lo + D / 2;
+      float f0 = 1.f, f1 = 0.f;  // factors of the two outputs (own rows: of this one alone)
+      if (!p.two) {
+        m = ml0[r];
+        l = ml0[128 + r];
+        if (nt > 1) {
+          const float m0 = m, m1 = ml1[r];
+          m = fmaxf(m0, m1);
+          f0 = ta_factor(m0, m);
+          f1 = ta_factor(m1, m);
+          l = l * f0 + ml1[128 + r] * f1;
+        }
+      }
+      if (live && ok) {
+        const bool own = r < rows;
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const int mrow = row0 + r;
+        const int64_t out_row = ((int64_t)p.b * a.Hq + p.h * A.g + mrow / a.T) * a.T + mrow % a.T;
+        const int slot = 2 * blockIdx.x + (p.t0 > 0 ? 0 : 1);
+        const int prow = (p.two ? s * 128 : 0) + r;
+        uint32_t any_bad = 0;
+        if (p.t1 * TA_TK > p.len) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) any_bad |= bad_now[i];
+        }
+#pragma unroll 1
+        for (int c = c_lo; c < c_hi; c += 32) {
+          float o[32];
+          tc::tmem_ld32(to + (p.two ? s * 128 : 0) + c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= f0;
+          if (!p.two && nt > 1) {
+            float o1[32];
+            tc::tmem_ld32(to + 128 + c, o1);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], f1, o[e]);
+          }
+          if (any_bad && own) {  // the non-finite values of the nodes this row sees
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+              uint32_t seen = 0;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) seen = q == i ? mw[q] & bad_now[q] : seen;
+              for (; seen; seen &= seen - 1) {
+                const int key = p.len + 32 * i + __ffs(seen) - 1;
+                const T* v = static_cast<const T*>(a.v) + p.h * a.v_sh;
+                if (a.table) {
+                  const int page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
+                  v += page * a.v_s0 + (key % a.block) * a.v_ss;  // a page that was read
+                } else {
+                  v += p.b * a.v_s0 + key * a.v_ss;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float y = to_f(v[c + e]);
+                  if (!isfinite(y)) o[e] += y;
+                }
+              }
+            }
+          }
+          if (own && whole) {
+            T* dst = static_cast<T*>(a.out) + out_row * D + c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 y;
+              y.x = TaType<T>::pack(o[e] * inv, o[e + 1] * inv);
+              y.y = TaType<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
+              y.z = TaType<T>::pack(o[e + 4] * inv, o[e + 5] * inv);
+              y.w = TaType<T>::pack(o[e + 6] * inv, o[e + 7] * inv);
+              *reinterpret_cast<uint4*>(dst + e) = y;
+            }
+          } else if (own) {
+            float4* po = reinterpret_cast<float4*>(A.part_o) + (int64_t)slot * (D / 4) * A.rows_pad + prow;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              po[((c + e) / 4) * (int64_t)A.rows_pad] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (own && !whole && (p.two || s == 0)) {
+          float* pm = A.part_ml + (int64_t)slot * 2 * A.rows_pad + prow;
+          pm[0] = m;
+          pm[A.rows_pad] = l;
+        }
+      }
+      tc::tc_fence_before();
+      ta_group_sync();  // outputs are read: the next piece may overwrite them
+      tc::tc_fence_after();
+    }
+  }
+  if (code) *dead = code;
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == TA_WARP_MMA) tc::tmem_dealloc(tmem, 512);
+  if (tid == 0) A.status[blockIdx.x] = *dead;
+}
+
+constexpr int TM_NT = 128;
+
+// Joins the partials of the segments that fell into several CTAs. Grid: (segments,
+// 32-row blocks x blocks of 32 columns); a thread has a row and eight columns. The
+// partials lie [column / 4][row], so a warp reads 32 rows of 16 bytes in one piece.
+template <typename T, int D>
+__global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ctas) {
+  __shared__ long long red[2][TM_NT / 32];
+  const TreeAttn& a = A.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long HR = (long long)a.Hkv * A.RT;
+  const int b = (int)(blockIdx.x / HR), seg = (int)(blockIdx.x % HR);
+  const int rt = seg % A.RT, h = seg / A.RT;
+  pdl_wait();
+  long long before = 0, total = 0;
+  for (int i = tid; i < a.B; i += TM_NT) {
+    const int t = ta_tiles(a, i);
+    total += t;
+    before += i < b ? t : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) red[0][warp] = total, red[1][warp] = before;
+  __syncthreads();
+  total = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+  before = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const long long W = total * HR, per = max(1ll, (W + ctas - 1) / ctas);
+  const int tiles = ta_tiles(a, b);
+  const long long w0 = before * HR + (long long)seg * tiles, w1 = w0 + tiles;
+  const int c0 = (int)(w0 / per), c1 = (int)((w1 - 1) / per);
+  if (c0 == c1) return;  // written by its one CTA
+  const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
+  const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
+  if (row >= TA_ROWS || mrow >= A.M) return;
+  // CTA c's partial: its first piece if the segment starts before the CTA's share
+  auto slot = [&](int c) { return (int64_t)2 * c + (w0 < (long long)c * per ? 0 : 1); };
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(A.part_ml + slot(c) * 2 * A.rows_pad + row));
+  float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int q = cb * 8 + warp * 2;  // first of the thread's two groups of four columns
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const int64_t sl = slot(c);
+    const float* pm = A.part_ml + sl * 2 * A.rows_pad + row;
+    const float4* po = reinterpret_cast<const float4*>(A.part_o) + (sl * (D / 4) + q) * A.rows_pad + row;
+    const float f = ta_factor(__ldcg(pm), m);
+    const float4 x = __ldcg(po), y = __ldcg(po + A.rows_pad);
+    l = fmaf(__ldcg(pm + A.rows_pad), f, l);
+    o[0] = fmaf(x.x, f, o[0]);
+    o[1] = fmaf(x.y, f, o[1]);
+    o[2] = fmaf(x.z, f, o[2]);
+    o[3] = fmaf(x.w, f, o[3]);
+    o[4] = fmaf(y.x, f, o[4]);
+    o[5] = fmaf(y.y, f, o[5]);
+    o[6] = fmaf(y.z, f, o[6]);
+    o[7] = fmaf(y.w, f, o[7]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t out_row = ((int64_t)b * a.Hq + h * A.g + mrow / a.T) * a.T + mrow % a.T;
+  uint4 y;
+  y.x = TaType<T>::pack(o[0] * inv, o[1] * inv);
+  y.y = TaType<T>::pack(o[2] * inv, o[3] * inv);
+  y.z = TaType<T>::pack(o[4] * inv, o[5] * inv);
+  y.w = TaType<T>::pack(o[6] * inv, o[7] * inv);
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + out_row * D + 4 * q) = y;
+}
+
+struct TaPlan {
+  int ctas, rows_pad;
+  size_t off_o, off_ml, bytes;
+};
+
+TaPlan ta_plan(int Hq, int Hkv, int T, int D) {
+  TaPlan p;
+  p.ctas = num_sms_current_device();
+  p.rows_pad = std::min(TA_ROWS, (Hq / Hkv * T + 31) / 32 * 32);
+  p.off_o = align_up((size_t)p.ctas * 4, 256);
+  p.off_ml = p.off_o + (size_t)2 * p.ctas * p.rows_pad * D * 4;
+  p.bytes = align_up(p.off_ml + (size_t)2 * p.ctas * 2 * p.rows_pad * 4, 256);
+  return p;
+}
+
+template <typename T, int D>
+int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
+  using L = TaSmem<D>;
+  const bool bf16 = dtype == DROPKV_DTYPE_BF16;
+  const TaPlan plan = ta_plan(a.Hq, a.Hkv, a.T, D);
+  TaArgs A;
+  A.a = a;
+  A.g = a.Hq / a.Hkv;
+  A.M = A.g * a.T;
+  A.RT = (A.M + TA_ROWS - 1) / TA_ROWS;
+  A.box = a.table ? std::min(a.block, TA_TK) : TA_TK;
+  A.rows_pad = plan.rows_pad;
+  A.scale_log2 = a.scale * 1.4426950408889634f;
+  A.bias = bf16 ? 0.f : 7.f;
+  A.status = static_cast<int*>(ws);
+  A.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_o);
+  A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_ml);
+  const int n0 = a.table ? a.n_pages : a.B, rows = a.table ? a.block : a.cap;
+  CUtensorMap km, vm;
+  int rc = make_kv_tensor_map_4d(&km, a.k, n0, a.Hkv, rows, D, bf16, a.k_s0, a.k_sh, a.k_ss, A.box);
+  if (!rc) rc = make_kv_tensor_map_4d(&vm, a.v, n0, a.Hkv, rows, D, bf16, a.v_s0, a.v_sh, a.v_ss, A.box);
+  if (rc) return rc;
+  auto kern = tree_attn_kernel<T, D>;
+  auto merge = tree_attn_merge_kernel<T, D>;
+  static DeviceOnce done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!done.done(dev)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "cannot set tree attention shared memory size %d", L::ALLOC);
+    done.mark(dev);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(TA_NT);
+  cfg.dynamicSmemBytes = L::ALLOC;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "tree attention launch: %s", cudaGetErrorString(e));
+  rc = check_launch("tree_attention");
+  if (rc || a.cap <= TA_TK) return rc;  // a cache of one tile: nothing is split
+  cfg.gridDim = dim3(a.B * a.Hkv * A.RT, (A.rows_pad / 32) * (D / 32));
+  cfg.blockDim = dim3(TM_NT);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, merge, A, plan.ctas);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "tree attention merge launch: %s", cudaGetErrorString(e));
+  return check_launch("tree_attention_merge");
 }
 
 }  // namespace
 
 size_t tree_attention_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
-  (void)B, (void)Hq, (void)Hkv, (void)T, (void)D, (void)cap;
-  return 0;
+  (void)B, (void)cap;
+  return ta_plan(Hq, Hkv, T, D).bytes;
 }
 
 int launch_tree_attention(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
-  (void)ws;
-  const dim3 grid(a.Hq * a.T, a.B);
+  if (a.cap == 0) {  // no rows at all: nothing is seen
+    if (cudaMemsetAsync(a.out, 0, (size_t)a.B * a.Hq * a.T * a.D * 2, st) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "tree attention: memset failed");
+    return DROPKV_OK;
+  }
   if (dtype == DROPKV_DTYPE_BF16)
-    tree_attn_rows_kernel<__nv_bfloat16><<<grid, TA_NT, 0, st>>>(a);
-  else
-    tree_attn_rows_kernel<__half><<<grid, TA_NT, 0, st>>>(a);
-  return check_launch("tree_attention");
+    return a.D == 128 ? ta_launch<__nv_bfloat16, 128>(a, dtype, ws, st) : ta_launch<__nv_bfloat16, 64>(a, dtype, ws, st);
+  return a.D == 128 ? ta_launch<__half, 128>(a, dtype, ws, st) : ta_launch<__half, 64>(a, dtype, ws, st);
 }
 
 }  // namespace dropkv

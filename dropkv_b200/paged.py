@@ -22,7 +22,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE, _on_device, _stream, _workspace
+from .ops import _CHECK_STATUS, _DTYPE_CODE, _on_device, _stream, _workspace
 
 __all__ = ["BlockTables", "TokenLogprobs", "block_tables", "store_rows", "qk_norm_rope", "tree_attention",
            "token_logprobs", "tree_mask_from_parents"]
@@ -284,6 +284,12 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
             *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
             out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
         _lib.check(rc, "dropkv_tree_attention")
+        if _CHECK_STATUS and cap * n0 > 0 and not torch.cuda.is_current_stream_capturing():
+            n = torch.cuda.get_device_properties(dev).multi_processor_count  # a word for each CTA comes first
+            st = int(ws[:4 * n].view(torch.int32).max().item()) if ws.numel() >= 4 * n else 0
+            if st != 0:
+                raise _lib.DropKVError(_lib.ERR_DEVICE, f"dropkv_tree_attention: device status {st} "
+                                                        "(a bounded wait timed out)")
     return out
 
 
