@@ -43,6 +43,7 @@ struct TaArgs {
   int box;                 // rows of a TMA box
   int rows_pad;            // rows of a partial
   float scale_log2;
+  int q_vec;               // Q's rows are read 16 bytes at a time
   float bias;              // weights are 2^(s - m + bias): fp16 has few bits below 1
   int* status;             // [CTAs]: 0, or which wait gave up
   float* part_o;           // [2 CTAs][D / 4][rows_pad] float4
@@ -118,6 +119,8 @@ template <typename T>
 struct TaType;
 template <>
 struct TaType<__nv_bfloat16> {
+  using Two = __nv_bfloat162;
+  static __device__ __forceinline__ Two two(float x) { return __float2bfloat162_rn(x); }
   static constexpr uint32_t kInf = 0x7F80u;  // the exponent bits
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -127,6 +130,8 @@ struct TaType<__nv_bfloat16> {
 };
 template <>
 struct TaType<__half> {
+  using Two = __half2;
+  static __device__ __forceinline__ Two two(float x) { return __float2half2_rn(x); }
   static constexpr uint32_t kInf = 0x7C00u;
   static __device__ __forceinline__ __half from(float x) { return __float2half_rn(x); }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -145,12 +150,12 @@ __device__ __forceinline__ float ta_ex2(float x) {  // 2^x, hardware approximati
 // nothing (or NaN alone) have -inf, which must not turn into NaN (or hide it).
 __device__ __forceinline__ float ta_factor(float m, float to) { return m == to ? 1.f : ta_ex2(m - to); }
 
-// A word with its non-finite halves zeroed; *bad is set if there were any.
+// A word with its non-finite halves zeroed.
 template <typename T>
-__device__ __forceinline__ uint32_t ta_finite(uint32_t x, bool* bad) {
+__device__ __forceinline__ uint32_t ta_finite(uint32_t x) {
   constexpr uint32_t E = TaType<T>::kInf;
-  if ((x & E) == E) x &= 0xFFFF0000u, *bad = true;
-  if ((x & (E << 16)) == (E << 16)) x &= 0x0000FFFFu, *bad = true;
+  if ((x & E) == E) x &= 0xFFFF0000u;
+  if ((x & (E << 16)) == (E << 16)) x &= 0x0000FFFFu;
   return x;
 }
 
@@ -293,62 +298,69 @@ __global__ void __launch_bounds__(TA_NT, 1)
     }
   } else if (warp == TA_WARP_MMA) {
     // ======================= MMA issuer =========================================
-    if (lane == 0) {
-      constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
-      constexpr uint32_t ID_PV = tc::idesc_f16(BF16, 128, D, false, true);
-      constexpr uint32_t LBO_V = SLABS == 2 ? TA_TK * 128 : 0;
-      const uint32_t ring0 = tc::smem_addr(sm + L::RING);
-      uint64_t qd[2];
-      for (int s = 0; s < 2; ++s) qd[s] = tc::smem_desc(tc::smem_addr(sm + L::Q + s * L::TILE), 16, 1024);
-      uint32_t k = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-      bool ok = true;
-      while (ok && walk.next(A, p)) {
-        const int per_tile = p.two ? 2 : 1, lead = p.two ? 1 : 2;
-        // ring positions: K_i is load number i (i < lead) or lead + 2 (i - lead) + 1, V_i number lead + 2 i,
-        // short of the K loads that do not exist
-        const int nt = p.t1 - p.t0, ahead = min(lead, nt);
-        auto k_at = [&](int i) { return k + (i < lead ? i : lead + 2 * (i - lead) + 1); };
-        auto v_at = [&](int i) { return k + ahead + i + min(i, max(nt - lead, 0)); };
-        auto qk = [&](int item) {
-          const int s = item & 1, i = item / per_tile;
-          const uint32_t at = k_at(i), slot = at % NS;
-          if (item < 2 && !wait(&bars[B_Q + s], n_q[s]++, 2)) return false;
-          if (!wait(&full[slot], at / NS, 3)) return false;
-          tc::tc_fence_after();
-          const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
+    // The whole warp runs this and one lane of it issues: counts, addresses and
+    // descriptors, taken from lane 0, stay in uniform registers. Issued from a branch of
+    // one lane, each MMA cost about 115 cycles of moves to them, against 64 of work.
+    constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
+    constexpr uint32_t ID_PV = tc::idesc_f16(BF16, 128, D, false, true);
+    constexpr uint32_t LBO_V = SLABS == 2 ? TA_TK * 128 : 0;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t ring0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::RING), 0);
+    const uint32_t q0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0);
+    auto all = [&](bool x) { return __all_sync(0xffffffffu, x) != 0; };
+    uint32_t k = 0, n_q = 0, n_p = 0;  // pieces and items of a group: both have had as many, or group 0 one more
+    uint32_t n_q1 = 0, n_p1 = 0;
+    bool ok = true;
+    while (ok && walk.next(A, p)) {
+      // load numbers from k on: K_i is number i (i < lead) or lead + 2 (i - lead) + 1, V_i number
+      // lead + 2 i, short of the K loads that do not exist
+      const int two = __shfl_sync(0xffffffffu, (int)p.two, 0), nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
+      const int items = two ? 2 * nt : nt, lead = two ? 1 : 2, ahead = min(lead, nt);
+      auto qk = [&](int item) {
+        const int s = item & 1, i = two ? item >> 1 : item;
+        const uint32_t at = k + (i < lead ? i : lead + 2 * (i - lead) + 1), slot = at % NS;
+        if (item < 2 && !all(wait(&bars[B_Q + s], s ? n_q1++ : n_q++, 2))) return false;
+        if (!all(wait(&full[slot], at / NS, 3))) return false;
+        tc::tc_fence_after();
+        const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
+        const uint64_t qd = tc::smem_desc(q0 + s * L::TILE, 16, 1024);
+        if (tc::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
-            tc::mma_f16(tmem + s * 128, tc::desc_add(qd[s], off), tc::desc_add(kd, off), ID_QK, kk > 0);
+            tc::mma_f16(tm + s * 128, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
           }
           tc::mma_commit(&bars[B_S + s]);
-          if (!p.two || s == 1) tc::mma_commit(&empty[slot]);
-          return true;
-        };
-        for (int item = 0; item < min(2, p.items) && ok; ++item) ok = qk(item);
-        for (int item = 0; item < p.items && ok; ++item) {
-          const int s = item & 1, i = item / per_tile;
-          const uint32_t at = v_at(i), slot = at % NS;
-          ok = wait(&full[slot], at / NS, 4) && wait(&bars[B_P + s], n_p[s]++, 5);
-          if (!ok) break;
-          tc::tc_fence_after();
-          const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
+          if (!two || s == 1) tc::mma_commit(&empty[slot]);
+        }
+        __syncwarp();
+        return true;
+      };
+      for (int item = 0; item < min(2, items) && ok; ++item) ok = qk(item);
+      for (int item = 0; item < items && ok; ++item) {
+        const int s = item & 1, i = two ? item >> 1 : item;
+        const uint32_t at = k + ahead + i + min(i, max(nt - lead, 0)), slot = at % NS;
+        ok = all(wait(&full[slot], at / NS, 4));
+        ok = ok && all(wait(&bars[B_P + s], s ? n_p1++ : n_p++, 5));
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
+        if (tc::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < TA_TK / 16; ++kk)
-            tc::mma_f16_tmem_a(tmem + 256 + s * 128, tmem + s * 128 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV,
+            tc::mma_f16_tmem_a(tm + 256 + s * 128, tm + s * 128 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV,
                                item >= 2 || kk > 0);
-          if (!p.two || s == 1) tc::mma_commit(&empty[slot]);
-          if (item + 2 < p.items)
-            ok = qk(item + 2);
-          else
-            tc::mma_commit(&bars[B_O + s]);
+          if (!two || s == 1) tc::mma_commit(&empty[slot]);
+          if (item + 2 >= items) tc::mma_commit(&bars[B_O + s]);
         }
-        k += 2 * nt;
+        __syncwarp();
+        if (item + 2 < items) ok = qk(item + 2);
       }
-      if (*dead) {  // no product may run on when tensor memory is given back
-        tc::mma_commit(&bars[B_END]);
-        tc::mbar_wait(&bars[B_END], 0, kTaWaitNs);
-      }
+      k += 2 * nt;
+    }
+    if (*dead) {  // no product may run on when tensor memory is given back
+      if (lane == 0) tc::mma_commit(&bars[B_END]);
+      tc::mbar_wait(&bars[B_END], 0, kTaWaitNs);
     }
   } else {
     // ======================= softmax groups =====================================
@@ -371,45 +383,59 @@ __global__ void __launch_bounds__(TA_NT, 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) mw[i] = 0;
       if (mine) {
-        // Q rows into shared memory, 16 bytes a thread: row = head of the group, then node
-        const bool vec = a.q_sd == 1 && ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)(a.q_sb * 2) |
-                                          (uintptr_t)(a.q_sh * 2) | (uintptr_t)(a.q_ss * 2)) % 16) == 0;
+        // Q rows into shared memory, 16 bytes a thread and step: row = head of the group, then
+        // node. The loads of eight steps are on their way before the first is stored.
         const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh;
-        for (int e = r; e < 128 * (D / 8); e += 128) {
-          const int row = e / (D / 8), c = e % (D / 8);
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (row < rows) {
-            const int mrow = row0 + row;
-            const T* src = qb + (mrow / a.T) * a.q_sh + (mrow % a.T) * a.q_ss + c * 8 * a.q_sd;
-            if (vec) {
-              x = *reinterpret_cast<const uint4*>(src);
-            } else {
-              uint32_t w[4];
+        const int c = r % (D / 8);  // a thread's column of vectors stays, its row moves on
+#pragma unroll 1
+        for (int e0 = r / (D / 8); e0 < 128; e0 += 8 * (1024 / D)) {
+          uint4 x[8];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = (uint32_t) * reinterpret_cast<const uint16_t*>(src + 2 * i * a.q_sd) |
-                       ((uint32_t) * reinterpret_cast<const uint16_t*>(src + (2 * i + 1) * a.q_sd) << 16);
-              x = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int i = 0; i < 8; ++i) {
+            const int row = e0 + i * (1024 / D), mrow = row0 + min(row, rows - 1);
+            const T* src = qb + (mrow / a.T) * a.q_sh + (mrow % a.T) * a.q_ss + c * 8 * a.q_sd;
+            if (A.q_vec) {
+              x[i] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+              x[i].x = h[0] | (uint32_t)h[a.q_sd] << 16;
+              x[i].y = h[2 * a.q_sd] | (uint32_t)h[3 * a.q_sd] << 16;
+              x[i].z = h[4 * a.q_sd] | (uint32_t)h[5 * a.q_sd] << 16;
+              x[i].w = h[6 * a.q_sd] | (uint32_t)h[7 * a.q_sd] << 16;
             }
           }
-          *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
-                                    tc::sw128_offset(row, (c % 8) * 8)) = x;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int row = e0 + i * (1024 / D);
+            if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
+                                      tc::sw128_offset(row, (c % 8) * 8)) = x[i];
+          }
         }
         tc::fence_proxy_async_smem();
         tc::mbar_arrive(&bars[B_Q + s]);
         // the mask's rows, where the piece reaches the tree: a warp reads each of its rows
         if (p.t1 * TA_TK > p.len && live) {
           const int fit = p.keys - p.len;  // nodes that fit the cache
-          for (int q = 0; q < 32 && (warp & 3) * 32 + q < rows; ++q) {
-            const int node = (row0 + (warp & 3) * 32 + q) % a.T;
-            const uint8_t* mr = a.mask ? a.mask + p.b * a.mask_sb + node * a.mask_sr : nullptr;
+          const int first = row0 + (warp & 3) * 32, count = min(32, rows - (warp & 3) * 32);
+          const uint8_t* mb = a.mask ? a.mask + p.b * a.mask_sb : nullptr;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (i * 32 >= fit) break;
-              const int j = i * 32 + lane;
-              const bool see = j < fit && (mr ? mr[j * a.mask_sc] != 0 : j <= node);
-              const uint32_t word = __ballot_sync(0xffffffffu, see);
-              if (q == lane) mw[i] = word;
+          for (int i = 0; i < 8; ++i) {
+            if (i * 32 >= fit) break;
+            const int j = i * 32 + lane;
+            const int jc = min(j, fit - 1);
+            for (int q0 = 0; q0 < count; q0 += 16) {  // sixteen rows' bytes on their way at once
+              uint32_t see[16];
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                const int node = (first + min(q0 + q, count - 1)) % a.T;
+                see[q] = mb ? mb[node * a.mask_sr + jc * a.mask_sc] : jc <= node;
+              }
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                const uint32_t word = __ballot_sync(0xffffffffu, see[q] != 0 && j < fit);
+                if (q0 + q == lane) mw[i] = word;
+              }
             }
           }
         }
@@ -514,23 +540,37 @@ __global__ void __launch_bounds__(TA_NT, 1)
           if (!ok) break;
           const int key = j0 + r;
           if (key >= p.len) {
+            uint8_t* row = sm + L::RING + slot * L::TILE + r * 128;
+            auto vec = [&](int c) {  // lanes start at different columns: no bank conflicts
+              return reinterpret_cast<uint4*>(row + (c / 8) * (TA_TK * 128) + ((c + r) % 8) * 16);
+            };
             bool off = false;
-#pragma unroll 1
-            for (int c = 0; c < SLABS * 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(sm + L::RING + slot * L::TILE + (c / 8) * (TA_TK * 128) + r * 128 +
-                                                   ((c + r) % 8) * 16);
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              bool change = true;
-              if (key < p.keys) {
-                v = *at;
-                change = false;
-                v.x = ta_finite<T>(v.x, &change);
-                v.y = ta_finite<T>(v.y, &change);
-                v.z = ta_finite<T>(v.z, &change);
-                v.w = ta_finite<T>(v.w, &change);
-                off |= change;
+            if (key >= p.keys) {
+#pragma unroll
+              for (int c = 0; c < SLABS * 8; ++c) *vec(c) = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              using T2 = typename TaType<T>::Two;
+              T2 z = TaType<T>::two(0.f);  // stays 0 unless some value is infinite or NaN
+#pragma unroll
+              for (int c = 0; c < SLABS * 8; ++c) {
+                const uint4 v = *vec(c);
+                z = __hfma2(reinterpret_cast<const T2&>(v.x), TaType<T>::two(0.f), z);
+                z = __hfma2(reinterpret_cast<const T2&>(v.y), TaType<T>::two(0.f), z);
+                z = __hfma2(reinterpret_cast<const T2&>(v.z), TaType<T>::two(0.f), z);
+                z = __hfma2(reinterpret_cast<const T2&>(v.w), TaType<T>::two(0.f), z);
               }
-              if (change) *at = v;
+              off = __hisnan(z.x) || __hisnan(z.y);
+            }
+            if (off) {
+#pragma unroll 1
+              for (int c = 0; c < SLABS * 8; ++c) {
+                uint4 v = *vec(c);
+                v.x = ta_finite<T>(v.x);
+                v.y = ta_finite<T>(v.y);
+                v.z = ta_finite<T>(v.z);
+                v.w = ta_finite<T>(v.w);
+                *vec(c) = v;
+              }
             }
             if (off) atomicOr(&bad_now[(key - p.len) >> 5], 1u << ((key - p.len) & 31));
           }
@@ -748,6 +788,7 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   A.rows_pad = plan.rows_pad;
   A.scale_log2 = a.scale * 1.4426950408889634f;
   A.bias = bf16 ? 0.f : 7.f;
+  A.q_vec = a.q_sd == 1 && (reinterpret_cast<uintptr_t>(a.q) | (uint64_t)((a.q_sb | a.q_sh | a.q_ss) * 2)) % 16 == 0;
   A.status = static_cast<int*>(ws);
   A.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_o);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_ml);
