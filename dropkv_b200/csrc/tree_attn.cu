@@ -29,7 +29,8 @@ namespace {
 
 constexpr int TA_TK = 128;               // keys of a tile
 constexpr int TA_ROWS = 256;             // query rows of a segment
-constexpr int TA_NT = 256 + 64;          // two softmax groups, a TMA warp, an MMA warp
+constexpr int TA_SM = 128;               // threads of a softmax group, one for each row
+constexpr int TA_NT = 2 * TA_SM + 64;    // two softmax groups, a TMA warp, an MMA warp
 constexpr int TA_WARP_TMA = 8, TA_WARP_MMA = 9;
 constexpr uint64_t kTaWaitNs = 1000000000ull;
 // The reference a row's weights are taken against is moved only when its maximum has
@@ -37,8 +38,15 @@ constexpr uint64_t kTaWaitNs = 1000000000ull;
 // output, in tensor memory, is hardly ever rescaled.
 constexpr float kTaSlack = 8.f;
 
+// Division by a node count from 1 to 256 of numbers below 2^24.
+struct TaDiv {
+  uint32_t mul, d;
+  __device__ __forceinline__ int quot(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, mul); }
+};
+
 struct TaArgs {
   TreeAttn a;
+  TaDiv by_t;
   int g, M, RT;            // query rows of a KV head: M = g T, in RT segments of 256
   int box;                 // rows of a TMA box
   int rows_pad;            // rows of a partial
@@ -60,9 +68,8 @@ struct TaSmem {
   static constexpr int BAD = BARS + (2 * SLOTS + 10) * 8;  // uint32 [2][8]: nodes with non-finite V
   static constexpr int MISC = BAD + 64;
   static constexpr int BYTES = MISC + 64;
-  static constexpr int ALLOC = BYTES + 1024;  // the base is aligned to 1024
 };
-static_assert(TaSmem<128>::ALLOC <= 232448, "shared memory");
+static_assert(TaSmem<128>::BYTES <= 232448, "shared memory");
 
 // per softmax group s: Q written, S ready, P ready, O ready; and: every product done
 enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_END = 8 };
@@ -159,7 +166,7 @@ __device__ __forceinline__ uint32_t ta_finite(uint32_t x) {
   return x;
 }
 
-__device__ __forceinline__ void ta_group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void ta_softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TA_NT, 1)
@@ -167,8 +174,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
   using L = TaSmem<D>;
   constexpr int SLABS = D / 64, NS = L::SLOTS;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  extern __shared__ uint8_t raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t sm[];  // swizzled tiles start on multiples of 1024
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::BARS);
   uint64_t* empty = full + NS;
   uint64_t* bars = empty + NS;
@@ -178,15 +184,20 @@ __global__ void __launch_bounds__(TA_NT, 1)
   const TreeAttn& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+  if (tc::smem_addr(sm) % 1024) {  // as declared; nothing may run on any other layout
+    pdl_launch_dependents();
+    if (tid == 0) A.status[blockIdx.x] = 9;
+    return;
+  }
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(&bars[B_Q + s], 128);
+      tc::mbar_init(&bars[B_Q + s], TA_SM / 32);
       tc::mbar_init(&bars[B_S + s], 1);
-      tc::mbar_init(&bars[B_P + s], 128);
+      tc::mbar_init(&bars[B_P + s], TA_SM / 32);
       tc::mbar_init(&bars[B_O + s], 1);
     }
     tc::mbar_init(&bars[B_END], 1);
@@ -206,8 +217,9 @@ __global__ void __launch_bounds__(TA_NT, 1)
   pdl_wait();
   if (warp == 0) {  // where this CTA's share of the line of tiles starts
     const long long HR = (long long)a.Hkv * A.RT;
-    long long total = 0;
-    for (int b = lane; b < a.B; b += 32) total += ta_tiles(a, b);
+    const int own0 = lane < a.B ? ta_tiles(a, lane) : 0;
+    long long total = own0;
+    for (int b = lane + 32; b < a.B; b += 32) total += ta_tiles(a, b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const long long W = total * HR, per = max(1ll, (W + gridDim.x - 1) / gridDim.x);
@@ -215,7 +227,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
     long long before = 0;
     if (w0 < w1) {
       for (int c = 0; c < a.B; c += 32) {
-        const long long own = c + lane < a.B ? ta_tiles(a, c + lane) : 0;
+        const long long own = c == 0 ? own0 : (c + lane < a.B ? ta_tiles(a, c + lane) : 0);
         long long upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -248,9 +260,12 @@ __global__ void __launch_bounds__(TA_NT, 1)
   // a wait that gives up marks the CTA dead: every role then ends without waiting
   int code = 0;
   auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
-    if (*dead) return false;
-    if (tc::mbar_wait(bar, count & 1, kTaWaitNs)) return true;
-    *dead = code = why;
+    if (tc::mbar_try_wait(bar, count & 1)) return true;
+    const uint64_t t0 = tc::globaltimer_ns();
+    while (!*dead) {
+      if (tc::mbar_try_wait(bar, count & 1)) return true;
+      if (tc::globaltimer_ns() - t0 > kTaWaitNs) *dead = code = why;
+    }
     return false;
   };
 
@@ -298,63 +313,75 @@ __global__ void __launch_bounds__(TA_NT, 1)
     }
   } else if (warp == TA_WARP_MMA) {
     // ======================= MMA issuer =========================================
-    // The whole warp runs this and one lane of it issues: counts, addresses and
-    // descriptors, taken from lane 0, stay in uniform registers. Issued from a branch of
-    // one lane, each MMA cost about 115 cycles of moves to them, against 64 of work.
+    // The products of one group run while the other group's softmax does: one warp issues
+    // both, item after item (a tile of a group), which keeps the groups half a period
+    // apart. Two warps, one for each group, let the tensor cores serve both in turn, the
+    // groups fell into step and nothing overlapped (295K keys x 224 rows: 210 us
+    // against 180). The whole warp runs this and one lane issues, so that counts,
+    // addresses and descriptors can stay in uniform registers.
     constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
     constexpr uint32_t ID_PV = tc::idesc_f16(BF16, 128, D, false, true);
     constexpr uint32_t LBO_V = SLABS == 2 ? TA_TK * 128 : 0;
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t ring0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::RING), 0);
-    const uint32_t q0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0);
-    auto all = [&](bool x) { return __all_sync(0xffffffffu, x) != 0; };
-    uint32_t k = 0, n_q = 0, n_p = 0;  // pieces and items of a group: both have had as many, or group 0 one more
-    uint32_t n_q1 = 0, n_p1 = 0;
+    const uint64_t qd0 = tc::smem_desc(__shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0), 16, 1024);
+    uint32_t k = 0, n_q0 = 0, n_q1 = 0, n_p0 = 0, n_p1 = 0;
     bool ok = true;
     while (ok && walk.next(A, p)) {
       // load numbers from k on: K_i is number i (i < lead) or lead + 2 (i - lead) + 1, V_i number
       // lead + 2 i, short of the K loads that do not exist
       const int two = __shfl_sync(0xffffffffu, (int)p.two, 0), nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
       const int items = two ? 2 * nt : nt, lead = two ? 1 : 2, ahead = min(lead, nt);
+      auto k_at = [&](int i) { return k + (i < lead ? i : lead + 2 * (i - lead) + 1); };
       auto qk = [&](int item) {
-        const int s = item & 1, i = two ? item >> 1 : item;
-        const uint32_t at = k + (i < lead ? i : lead + 2 * (i - lead) + 1), slot = at % NS;
-        if (item < 2 && !all(wait(&bars[B_Q + s], s ? n_q1++ : n_q++, 2))) return false;
-        if (!all(wait(&full[slot], at / NS, 3))) return false;
-        tc::tc_fence_after();
+        const int s = item & 1;
+        const uint32_t slot = k_at(two ? item >> 1 : item) % NS;
         const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
-        const uint64_t qd = tc::smem_desc(q0 + s * L::TILE, 16, 1024);
-        if (tc::elect_one()) {
+        const uint64_t qd = tc::desc_add(qd0, s * L::TILE);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
-            tc::mma_f16(tm + s * 128, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
-          }
-          tc::mma_commit(&bars[B_S + s]);
-          if (!two || s == 1) tc::mma_commit(&empty[slot]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
+          tc::mma_f16(tm + s * 128, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
         }
-        __syncwarp();
-        return true;
+        tc::mma_commit(&bars[B_S + s]);
+        if (!two || s == 1) tc::mma_commit(&empty[slot]);
       };
-      for (int item = 0; item < min(2, items) && ok; ++item) ok = qk(item);
+      for (int item = 0; item < min(2, items) && ok; ++item) {
+        const uint32_t at = k_at(two ? item >> 1 : item);
+        ok = wait(&bars[B_Q + item], item ? n_q1++ : n_q0++, 2) && wait(&full[at % NS], at / NS, 3);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) qk(item);
+        __syncwarp();
+      }
       for (int item = 0; item < items && ok; ++item) {
         const int s = item & 1, i = two ? item >> 1 : item;
         const uint32_t at = k + ahead + i + min(i, max(nt - lead, 0)), slot = at % NS;
-        ok = all(wait(&full[slot], at / NS, 4));
-        ok = ok && all(wait(&bars[B_P + s], s ? n_p1++ : n_p++, 5));
+        const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
+        const bool more = item + 2 < items;
+        // V and the next K are mostly there before the weights are: nothing waits between the products
+        ok = wait(&full[slot], at / NS, 4);
+        if (more) {
+          const uint32_t kat = k_at(two ? (item + 2) >> 1 : item + 2);
+          ok = ok && wait(&full[kat % NS], kat / NS, 3);
+        }
+        ok = ok && wait(&bars[B_P + s], s ? n_p1++ : n_p0++, 5);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
         if (tc::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < TA_TK / 16; ++kk)
             tc::mma_f16_tmem_a(tm + 256 + s * 128, tm + s * 128 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV,
                                item >= 2 || kk > 0);
           if (!two || s == 1) tc::mma_commit(&empty[slot]);
-          if (item + 2 >= items) tc::mma_commit(&bars[B_O + s]);
+          if (more)
+            qk(item + 2);
+          else
+            tc::mma_commit(&bars[B_O + s]);
         }
         __syncwarp();
-        if (item + 2 < items) ok = qk(item + 2);
       }
       k += 2 * nt;
     }
@@ -364,10 +391,11 @@ __global__ void __launch_bounds__(TA_NT, 1)
     }
   } else {
     // ======================= softmax groups =====================================
-    const int s = warp >> 2, r = tid & 127;  // group and TMEM lane
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    // group s, its TMEM lane (row) and its warp's quarter of the lanes
+    const int s = warp >> 2, quad = warp & 3, r = tid & 127;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256;
-    float* ml0 = reinterpret_cast<float*>(sm + L::Q);  // [2][128]
+    float* ml0 = reinterpret_cast<float*>(sm + L::Q);  // [2][128]: maxima, sums
     float* ml1 = reinterpret_cast<float*>(sm + L::Q + L::TILE);
     uint32_t n_s = 0, n_o = 0, k = 0;
     bool ok = true;
@@ -376,7 +404,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
       const bool mine = p.two || s < nt;  // this group has work in the piece
       const int row0 = p.rt * TA_ROWS + (p.two ? s * 128 : 0);  // the group's first row
       const int rows = min(128, A.M - row0);
-      const bool live = (warp & 3) * 32 < rows;  // some row of this warp exists
+      const bool live = quad * 32 < rows;  // some row of this warp exists
       uint32_t* bad_now = bad + 8 * (piece & 1);
       float m = -INFINITY, l = 0.f;
       uint32_t mw[8];  // nodes that this thread's row sees
@@ -386,14 +414,15 @@ __global__ void __launch_bounds__(TA_NT, 1)
         // Q rows into shared memory, 16 bytes a thread and step: row = head of the group, then
         // node. The loads of eight steps are on their way before the first is stored.
         const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh;
-        const int c = r % (D / 8);  // a thread's column of vectors stays, its row moves on
+        constexpr int STEP = TA_SM / (D / 8);  // rows a step of the group covers
+        const int c = r % (D / 8);             // a thread's column of vectors stays, its row moves on
 #pragma unroll 1
-        for (int e0 = r / (D / 8); e0 < 128; e0 += 8 * (1024 / D)) {
+        for (int e0 = r / (D / 8); e0 < 128; e0 += 8 * STEP) {
           uint4 x[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int row = e0 + i * (1024 / D), mrow = row0 + min(row, rows - 1);
-            const T* src = qb + (mrow / a.T) * a.q_sh + (mrow % a.T) * a.q_ss + c * 8 * a.q_sd;
+            const int mrow = row0 + min(e0 + i * STEP, rows - 1), head = A.by_t.quot(mrow);
+            const T* src = qb + head * a.q_sh + (mrow - head * a.T) * a.q_ss + c * 8 * a.q_sd;
             if (A.q_vec) {
               x[i] = *reinterpret_cast<const uint4*>(src);
             } else {
@@ -406,30 +435,33 @@ __global__ void __launch_bounds__(TA_NT, 1)
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int row = e0 + i * (1024 / D);
+            const int row = e0 + i * STEP;
             if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
             *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
                                       tc::sw128_offset(row, (c % 8) * 8)) = x[i];
           }
         }
         tc::fence_proxy_async_smem();
-        tc::mbar_arrive(&bars[B_Q + s]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars[B_Q + s]);
         // the mask's rows, where the piece reaches the tree: a warp reads each of its rows
         if (p.t1 * TA_TK > p.len && live) {
           const int fit = p.keys - p.len;  // nodes that fit the cache
-          const int first = row0 + (warp & 3) * 32, count = min(32, rows - (warp & 3) * 32);
+          const int first = row0 + quad * 32, count = min(32, rows - quad * 32);
+          const int node0 = first - A.by_t.quot(first) * a.T;
           const uint8_t* mb = a.mask ? a.mask + p.b * a.mask_sb : nullptr;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (i * 32 >= fit) break;
-            const int j = i * 32 + lane;
-            const int jc = min(j, fit - 1);
+            const int j = i * 32 + lane, jc = min(j, fit - 1);
+            const uint8_t* mc = mb + jc * a.mask_sc;
+            int node = node0;  // rows follow one another, their nodes too, around the tree
             for (int q0 = 0; q0 < count; q0 += 16) {  // sixteen rows' bytes on their way at once
               uint32_t see[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
-                const int node = (first + min(q0 + q, count - 1)) % a.T;
-                see[q] = mb ? mb[node * a.mask_sr + jc * a.mask_sc] : jc <= node;
+                see[q] = mb ? mc[node * a.mask_sr] : jc <= node;
+                node = node + 1 == a.T ? 0 : node + 1;
               }
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
@@ -440,10 +472,10 @@ __global__ void __launch_bounds__(TA_NT, 1)
           }
         }
       }
-      const int lead = p.two ? 1 : 2, ahead = min(lead, nt);
-      for (int i = p.two ? 0 : s; i < nt && ok; i += p.two ? 1 : 2) {
+      const int lead = p.two ? 1 : 2, ahead = min(lead, nt), step = lead;
+      for (int i = p.two ? 0 : s; i < nt && ok; i += step) {
         const int j0 = (p.t0 + i) * TA_TK;
-        // which of the tile's pages exist (a lane for each): 16 bits, from 8 rows up
+        // which of the tile's pages are missing (a lane for each): 16 bits, from 8 rows up
         uint32_t gone = 0;
         if (a.table) {
           const int key = j0 + lane * A.box;
@@ -459,8 +491,8 @@ __global__ void __launch_bounds__(TA_NT, 1)
         if (!ok) break;
         tc::tc_fence_after();
         if (live) {
-          uint32_t see[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
           const bool masked = tree || gone;
+          uint32_t see[4];
           if (masked) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -475,30 +507,62 @@ __global__ void __launch_bounds__(TA_NT, 1)
               if (q < 0) lo = 0xffffffffu;
               if (q + 1 < 0) hi = 0xffffffffu;
               see[w] = __funnelshift_r(lo, hi, at & 31);
-              for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
-                if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+              if (gone) {
+                for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
+                  if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+              }
             }
           }
-          // S is read twice, for the maximum and for the weights: a row of 128 does not stay in registers
-          float x[32], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top = -INFINITY, sum = 0.f;
+          uint32_t pk[64];
+          // the weights against the reference m, and the maximum, in one pass over S
+          auto weigh = [&](auto hide) {
+            const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sm4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            tc::tmem_ld32(ts + 32 * w, x);
-            if (masked) {
+            for (int w = 0; w < 4; ++w) {
+              float x[32];
+              tc::tmem_ld32(ts + 32 * w, x);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+              for (int e = 0; e < 32; e += 2) {
+                if (decltype(hide)::value) {
+                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
+                }
+                mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+                mx[(e & 3) + 1] = fmaxf(mx[(e & 3) + 1], x[e + 1]);
+                const float u = ta_ex2(fmaf(x[e], A.scale_log2, -ref)), v = ta_ex2(fmaf(x[e + 1], A.scale_log2, -ref));
+                sm4[e & 3] += u;
+                sm4[(e & 3) + 1] += v;
+                pk[16 * w + e / 2] = TaType<T>::pack(u, v);
+              }
             }
+            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+            sum = (sm4[0] + sm4[1]) + (sm4[2] + sm4[3]);
+          };
+          const bool first = i < step;
+          if (first) {  // no reference yet: the maximum alone
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], x[e]);
+            for (int w = 0; w < 4; ++w) {
+              float x[32];
+              tc::tmem_ld32(ts + 32 * w, x);
+              const uint32_t sw = masked ? see[w] : 0xffffffffu;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (sw >> e) & 1 ? x[e] : -INFINITY);
+            }
+            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+          } else if (masked) {
+            weigh(std::true_type());
+          } else {
+            weigh(std::false_type());
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-          const bool grow = top > m + kTaSlack || m == -INFINITY;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float mn = grow ? fmaxf(m, top) : m;
-            const float alpha = mn == -INFINITY ? 1.f : ta_ex2(m - mn);
+          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves: weigh (again)
+            const float mn = top > m + kTaSlack ? top : m;
+            const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
             m = mn;
             l *= alpha;
-            if (i >= 2 || (p.two && i >= 1)) {  // something has been accumulated
+            if (!first) {
               float o[16];
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
@@ -509,27 +573,14 @@ __global__ void __launch_bounds__(TA_NT, 1)
                 tc::tmem_st_wait();
               }
             }
+            if (masked)
+              weigh(std::true_type());
+            else
+              weigh(std::false_type());
           }
-          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          l += sum;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {  // P's columns [16 w, 16 w + 16) lie in columns of S already read
-            tc::tmem_ld32(ts + 32 * w, x);
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
-            }
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float u = ta_ex2(fmaf(x[e], A.scale_log2, -ref)), v = ta_ex2(fmaf(x[e + 1], A.scale_log2, -ref));
-              sum[e & 3] += u;
-              sum[(e & 3) + 1] += v;
-              pk[e / 2] = TaType<T>::pack(u, v);
-            }
-            tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          for (int c = 0; c < 64; c += 16) tc::tmem_st16(ts + c, reinterpret_cast<const float*>(pk + c));  // over S, which is read
           tc::tmem_st_wait();
         }
         if (tree) {
@@ -544,15 +595,16 @@ __global__ void __launch_bounds__(TA_NT, 1)
             auto vec = [&](int c) {  // lanes start at different columns: no bank conflicts
               return reinterpret_cast<uint4*>(row + (c / 8) * (TA_TK * 128) + ((c + r) % 8) * 16);
             };
+            constexpr int VECS = SLABS * 8;
             bool off = false;
             if (key >= p.keys) {
 #pragma unroll
-              for (int c = 0; c < SLABS * 8; ++c) *vec(c) = make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < VECS; ++c) *vec(c) = make_uint4(0u, 0u, 0u, 0u);
             } else {
               using T2 = typename TaType<T>::Two;
               T2 z = TaType<T>::two(0.f);  // stays 0 unless some value is infinite or NaN
 #pragma unroll
-              for (int c = 0; c < SLABS * 8; ++c) {
+              for (int c = 0; c < VECS; ++c) {
                 const uint4 v = *vec(c);
                 z = __hfma2(reinterpret_cast<const T2&>(v.x), TaType<T>::two(0.f), z);
                 z = __hfma2(reinterpret_cast<const T2&>(v.y), TaType<T>::two(0.f), z);
@@ -563,7 +615,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
             }
             if (off) {
 #pragma unroll 1
-              for (int c = 0; c < SLABS * 8; ++c) {
+              for (int c = 0; c < VECS; ++c) {
                 uint4 v = *vec(c);
                 v.x = ta_finite<T>(v.x);
                 v.y = ta_finite<T>(v.y);
@@ -571,27 +623,28 @@ __global__ void __launch_bounds__(TA_NT, 1)
                 v.w = ta_finite<T>(v.w);
                 *vec(c) = v;
               }
+              atomicOr(&bad_now[(key - p.len) >> 5], 1u << ((key - p.len) & 31));
             }
-            if (off) atomicOr(&bad_now[(key - p.len) >> 5], 1u << ((key - p.len) & 31));
           }
           tc::fence_proxy_async_smem();
         }
         tc::tc_fence_before();
-        tc::mbar_arrive(&bars[B_P + s]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars[B_P + s]);
       }
       k += 2 * nt;
       // ---- the piece's output ---------------------------------------------------
       if (mine && ok) ok = __all_sync(0xffffffffu, wait(&bars[B_O + s], n_o++, 8));
       m -= A.bias;  // the reference the weights were taken against
-      (s ? ml1 : ml0)[r] = m;
-      (s ? ml1 : ml0)[128 + r] = l;
-      ta_group_sync();
+      float* ml = s ? ml1 : ml0;
+      ml[r] = m;
+      ml[128 + r] = l;
+      ta_softmax_sync();
       tc::tc_fence_after();
       if (tid < 8) bad[8 * ((piece + 1) & 1) + tid] = 0;
       const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-      // rows in turn: this group writes columns [s D / 2, (s + 1) D / 2) of the joined
-      // output; else all columns of its own rows
-      const int c_lo = p.two ? 0 : s * (D / 2), c_hi = p.two ? D : c_lo + D / 2;
+      // tiles in turn: each group writes half the columns of the joined rows; else all of its own
+      const int part = p.two ? 0 : s, width = p.two ? D : D / 2;
       float f0 = 1.f, f1 = 0.f;  // factors of the two outputs (own rows: of this one alone)
       if (!p.two) {
         m = ml0[r];
@@ -608,7 +661,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
         const bool own = r < rows;
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         const int mrow = row0 + r;
-        const int64_t out_row = ((int64_t)p.b * a.Hq + p.h * A.g + mrow / a.T) * a.T + mrow % a.T;
+        const int64_t out_row = ((int64_t)p.b * a.Hq + p.h * A.g) * a.T + mrow;  // heads of T rows follow one another
         const int slot = 2 * blockIdx.x + (p.t0 > 0 ? 0 : 1);
         const int prow = (p.two ? s * 128 : 0) + r;
         uint32_t any_bad = 0;
@@ -617,16 +670,16 @@ __global__ void __launch_bounds__(TA_NT, 1)
           for (int i = 0; i < 8; ++i) any_bad |= bad_now[i];
         }
 #pragma unroll 1
-        for (int c = c_lo; c < c_hi; c += 32) {
-          float o[32];
-          tc::tmem_ld32(to + (p.two ? s * 128 : 0) + c, o);
+        for (int c = part * width; c < (part + 1) * width; c += 16) {
+          float o[16];
+          tc::tmem_ld16(to + (p.two ? s * 128 : 0) + c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= f0;
+          for (int e = 0; e < 16; ++e) o[e] *= f0;
           if (!p.two && nt > 1) {
-            float o1[32];
-            tc::tmem_ld32(to + 128 + c, o1);
+            float o1[16];
+            tc::tmem_ld16(to + 128 + c, o1);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = fmaf(o1[e], f1, o[e]);
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(o1[e], f1, o[e]);
           }
           if (any_bad && own) {  // the non-finite values of the nodes this row sees
 #pragma unroll 1
@@ -644,7 +697,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
                   v += p.b * a.v_s0 + key * a.v_ss;
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                for (int e = 0; e < 16; ++e) {
                   const float y = to_f(v[c + e]);
                   if (!isfinite(y)) o[e] += y;
                 }
@@ -654,7 +707,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
           if (own && whole) {
             T* dst = static_cast<T*>(a.out) + out_row * D + c;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
+            for (int e = 0; e < 16; e += 8) {
               uint4 y;
               y.x = TaType<T>::pack(o[e] * inv, o[e + 1] * inv);
               y.y = TaType<T>::pack(o[e + 2] * inv, o[e + 3] * inv);
@@ -665,18 +718,18 @@ __global__ void __launch_bounds__(TA_NT, 1)
           } else if (own) {
             float4* po = reinterpret_cast<float4*>(A.part_o) + (int64_t)slot * (D / 4) * A.rows_pad + prow;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
+            for (int e = 0; e < 16; e += 4)
               po[((c + e) / 4) * (int64_t)A.rows_pad] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        if (own && !whole && (p.two || s == 0)) {
+        if (own && !whole && part == 0) {
           float* pm = A.part_ml + (int64_t)slot * 2 * A.rows_pad + prow;
           pm[0] = m;
           pm[A.rows_pad] = l;
         }
       }
       tc::tc_fence_before();
-      ta_group_sync();  // outputs are read: the next piece may overwrite them
+      ta_softmax_sync();  // outputs are read: the next piece may overwrite them
       tc::tc_fence_after();
     }
   }
@@ -688,19 +741,25 @@ __global__ void __launch_bounds__(TA_NT, 1)
   if (tid == 0) A.status[blockIdx.x] = *dead;
 }
 
-constexpr int TM_NT = 128;
+constexpr int TM_NT = 256;
+constexpr int TM_PIECES = 64;  // partials whose factors are held at once
 
 // Joins the partials of the segments that fell into several CTAs. Grid: (segments,
-// 32-row blocks x blocks of 32 columns); a thread has a row and eight columns. The
+// 32-row blocks x blocks of 32 columns); a thread has a row and four columns. The
 // partials lie [column / 4][row], so a warp reads 32 rows of 16 bytes in one piece.
+// The eight warps first share out the partials' maxima and sums.
 template <typename T, int D>
 __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ctas) {
   __shared__ long long red[2][TM_NT / 32];
+  __shared__ float fac[TM_PIECES][32], mxs[TM_NT / 32][32], sums[TM_NT / 32][32];
   const TreeAttn& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long HR = (long long)a.Hkv * A.RT;
-  const int b = (int)(blockIdx.x / HR), seg = (int)(blockIdx.x % HR);
+  const int HR = a.Hkv * A.RT;
+  const int b = (int)(blockIdx.x / (unsigned)HR), seg = (int)(blockIdx.x % (unsigned)HR);
   const int rt = seg % A.RT, h = seg / A.RT;
+  const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
+  const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
+  if (rt * TA_ROWS + rb * 32 >= A.M) return;
   pdl_wait();
   long long before = 0, total = 0;
   for (int i = tid; i < a.B; i += TM_NT) {
@@ -715,48 +774,75 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   }
   if (lane == 0) red[0][warp] = total, red[1][warp] = before;
   __syncthreads();
-  total = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
-  before = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < TM_NT / 32; ++w) total += red[0][w], before += red[1][w];
   const long long W = total * HR, per = max(1ll, (W + ctas - 1) / ctas);
   const int tiles = ta_tiles(a, b);
   const long long w0 = before * HR + (long long)seg * tiles, w1 = w0 + tiles;
-  const int c0 = (int)(w0 / per), c1 = (int)((w1 - 1) / per);
-  if (c0 == c1) return;  // written by its one CTA
-  const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
-  const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
-  if (row >= TA_ROWS || mrow >= A.M) return;
-  // CTA c's partial: its first piece if the segment starts before the CTA's share
-  auto slot = [&](int c) { return (int64_t)2 * c + (w0 < (long long)c * per ? 0 : 1); };
-  float m = -INFINITY;
+  const int c0 = (int)(w0 / per), n = (int)((w1 - 1) / per) - c0 + 1;
+  if (n == 1) return;  // written by its one CTA
+  // partial i is CTA c0 + i's: the segment is the last piece of the first CTA, the first of the others
+  auto slot = [&](int i) { return (int64_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
+  const bool own = row < A.rows_pad && mrow < A.M;
+  const float* pml = A.part_ml + row;
+  float mine = -INFINITY;
+  if (own) {
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(A.part_ml + slot(c) * 2 * A.rows_pad + row));
-  float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const int q = cb * 8 + warp * 2;  // first of the thread's two groups of four columns
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const int64_t sl = slot(c);
-    const float* pm = A.part_ml + sl * 2 * A.rows_pad + row;
-    const float4* po = reinterpret_cast<const float4*>(A.part_o) + (sl * (D / 4) + q) * A.rows_pad + row;
-    const float f = ta_factor(__ldcg(pm), m);
-    const float4 x = __ldcg(po), y = __ldcg(po + A.rows_pad);
-    l = fmaf(__ldcg(pm + A.rows_pad), f, l);
-    o[0] = fmaf(x.x, f, o[0]);
-    o[1] = fmaf(x.y, f, o[1]);
-    o[2] = fmaf(x.z, f, o[2]);
-    o[3] = fmaf(x.w, f, o[3]);
-    o[4] = fmaf(y.x, f, o[4]);
-    o[5] = fmaf(y.y, f, o[5]);
-    o[6] = fmaf(y.z, f, o[6]);
-    o[7] = fmaf(y.w, f, o[7]);
+    for (int i = warp; i < n; i += TM_NT / 32) mine = fmaxf(mine, __ldcg(pml + slot(i) * 2 * A.rows_pad));
   }
+  mxs[warp][lane] = mine;
+  __syncthreads();
+  float m = mxs[0][lane];
+#pragma unroll
+  for (int w = 1; w < TM_NT / 32; ++w) m = fmaxf(m, mxs[w][lane]);
+  const int q = cb * 8 + warp;  // the thread's group of four columns
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += TM_PIECES) {
+    const int cnt = min(TM_PIECES, n - i0);
+    if (i0) __syncthreads();  // the factors before have been used
+    for (int i = warp; i < cnt; i += TM_NT / 32) {
+      float f = 0.f;
+      if (own) {
+        const float* pm = pml + slot(i0 + i) * 2 * A.rows_pad;
+        f = ta_factor(__ldcg(pm), m);
+        l = fmaf(__ldcg(pm + A.rows_pad), f, l);
+      }
+      fac[i][lane] = f;
+    }
+    __syncthreads();
+    if (own) {
+      for (int i = 0; i < cnt; i += 8) {  // eight partials on their way at once
+        float4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          x[u] = __ldcg(reinterpret_cast<const float4*>(A.part_o) +
+                        (slot(i0 + min(i + u, cnt - 1)) * (D / 4) + q) * A.rows_pad + row);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (i + u >= cnt) break;
+          const float f = fac[i + u][lane];
+          o.x = fmaf(x[u].x, f, o.x);
+          o.y = fmaf(x[u].y, f, o.y);
+          o.z = fmaf(x[u].z, f, o.z);
+          o.w = fmaf(x[u].w, f, o.w);
+        }
+      }
+    }
+  }
+  sums[warp][lane] = l;
+  __syncthreads();
+  if (!own) return;
+  l = sums[0][lane];
+#pragma unroll
+  for (int w = 1; w < TM_NT / 32; ++w) l += sums[w][lane];
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t out_row = ((int64_t)b * a.Hq + h * A.g + mrow / a.T) * a.T + mrow % a.T;
-  uint4 y;
-  y.x = TaType<T>::pack(o[0] * inv, o[1] * inv);
-  y.y = TaType<T>::pack(o[2] * inv, o[3] * inv);
-  y.z = TaType<T>::pack(o[4] * inv, o[5] * inv);
-  y.w = TaType<T>::pack(o[6] * inv, o[7] * inv);
-  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + out_row * D + 4 * q) = y;
+  const int64_t out_row = ((int64_t)b * a.Hq + h * A.g) * a.T + mrow;  // heads of T rows follow one another
+  uint2 y;
+  y.x = TaType<T>::pack(o.x * inv, o.y * inv);
+  y.y = TaType<T>::pack(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + out_row * D + 4 * q) = y;
 }
 
 struct TaPlan {
@@ -781,6 +867,8 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   const TaPlan plan = ta_plan(a.Hq, a.Hkv, a.T, D);
   TaArgs A;
   A.a = a;
+  A.by_t.d = (uint32_t)a.T;
+  A.by_t.mul = a.T == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + a.T - 1) / a.T);
   A.g = a.Hq / a.Hkv;
   A.M = A.g * a.T;
   A.RT = (A.M + TA_ROWS - 1) / TA_ROWS;
@@ -803,8 +891,8 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (!done.done(dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC) != cudaSuccess)
-      return fail(DROPKV_ERR_CUDA, "cannot set tree attention shared memory size %d", L::ALLOC);
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "cannot set tree attention shared memory size %d", L::BYTES);
     done.mark(dev);
   }
   cudaLaunchConfig_t cfg = {};
@@ -816,7 +904,7 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   cfg.stream = st;
   cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(TA_NT);
-  cfg.dynamicSmemBytes = L::ALLOC;
+  cfg.dynamicSmemBytes = L::BYTES;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "tree attention launch: %s", cudaGetErrorString(e));
   rc = check_launch("tree_attention");
