@@ -30,8 +30,8 @@ namespace {
 constexpr int TA_TK = 128;               // keys of a tile
 constexpr int TA_ROWS = 256;             // query rows of a segment
 constexpr int TA_SM = 128;               // threads of a softmax group, one for each row
-constexpr int TA_NT = 2 * TA_SM + 64;    // two softmax groups, a TMA warp, an MMA warp
-constexpr int TA_WARP_TMA = 8, TA_WARP_MMA = 9;
+constexpr int TA_NT = 2 * TA_SM + 128;   // two softmax groups, a TMA warp for K and for V, an MMA warp for each group
+constexpr int TA_WARP_TMA = 8, TA_WARP_MMA = 10;
 constexpr uint64_t kTaWaitNs = 1000000000ull;
 // The reference a row's weights are taken against is moved only when its maximum has
 // grown by this much (base 2): weights then stay below 2^8, and the accumulated
@@ -58,6 +58,9 @@ struct TaArgs {
   float* part_ml;          // [2 CTAs][2][rows_pad]
 };
 
+// per softmax group s: Q written, S ready, P ready, O ready, its turn to issue, every product done
+enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_T = 8, B_END = 10, B_COUNT = 12 };
+
 template <int D>
 struct TaSmem {
   static constexpr int TILE = TA_TK * D * 2;  // K, V or Q tile: D / 64 slabs of 128 rows x 128 B
@@ -65,17 +68,14 @@ struct TaSmem {
   static constexpr int Q = 0;                 // two tiles; a group's maxima and sums once its products are done
   static constexpr int RING = 2 * TILE;
   static constexpr int BARS = RING + SLOTS * TILE;        // full[SLOTS], empty[SLOTS], then B_*
-  static constexpr int BAD = BARS + (2 * SLOTS + 10) * 8;  // uint32 [2][8]: nodes with non-finite V
+  static constexpr int BAD = BARS + (2 * SLOTS + B_COUNT) * 8;  // uint32 [2][8]: nodes with non-finite V
   static constexpr int MISC = BAD + 64;
   static constexpr int BYTES = MISC + 64;
 };
 static_assert(TaSmem<128>::BYTES <= 232448, "shared memory");
 
-// per softmax group s: Q written, S ready, P ready, O ready; and: every product done
-enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_END = 8 };
-
 struct TaMisc {
-  long long w0, w1, base;  // this CTA's tiles, and the first tile of sequence b0
+  long long w0, w1, base;  // this CTA's units, and the first unit of sequence b0
   int b0;
   uint32_t tmem;
   int dead;
@@ -90,35 +90,41 @@ __device__ __forceinline__ int ta_tiles(const TreeAttn& a, int b) { return (ta_k
 struct TaPiece {
   int b, h, rt, t0, t1, tiles, len, keys, rows;
   bool two;    // two groups of rows, else tiles in turn
-  int items;   // (tile, group) pairs
 };
 
-// Steps through a CTA's pieces; every role has one of its own and sees the same.
+// Steps through a CTA's pieces; every role has one of its own and sees the same. On the line
+// each segment takes kTaLead units before its tiles, about what a further piece costs a CTA
+// (Q, an output, an empty pipeline): a CTA that ends a segment gets that much less of the next.
+constexpr int kTaLead = 4;
 struct TaWalk {
-  long long w, w1, base;
+  long long w, w1, base;  // units
   int b;
   __device__ __forceinline__ bool next(const TaArgs& A, TaPiece& p) {
-    if (w >= w1) return false;
     const TreeAttn& a = A.a;
-    p.b = b;
-    p.len = ta_len(a, b);
-    p.keys = ta_keys(a, p.len);
-    p.tiles = (p.keys + TA_TK - 1) / TA_TK;
-    const long long rel = w - base;
-    const int seg = (int)(rel / p.tiles);
-    p.t0 = (int)(rel - (long long)seg * p.tiles);
-    p.t1 = (int)min((long long)p.tiles, p.t0 + (w1 - w));
-    p.h = seg / A.RT;
-    p.rt = seg % A.RT;
-    p.rows = min(TA_ROWS, A.M - p.rt * TA_ROWS);
-    p.two = p.rows > 128;
-    p.items = (p.t1 - p.t0) * (p.two ? 2 : 1);
-    w += p.t1 - p.t0;
-    if (w - base == (long long)p.tiles * a.Hkv * A.RT) {
-      base = w;
-      ++b;
+    while (w < w1) {
+      p.b = b;
+      p.len = ta_len(a, b);
+      p.keys = ta_keys(a, p.len);
+      p.tiles = (p.keys + TA_TK - 1) / TA_TK;
+      const int units = p.tiles + kTaLead;
+      const long long rel = w - base;
+      const int seg = (int)(rel / units);
+      const int u0 = (int)(rel - (long long)seg * units);
+      const int u1 = (int)min((long long)units, u0 + (w1 - w));
+      p.t0 = max(u0 - kTaLead, 0);
+      p.t1 = u1 - kTaLead;
+      p.h = seg / A.RT;
+      p.rt = seg % A.RT;
+      p.rows = min(TA_ROWS, A.M - p.rt * TA_ROWS);
+      p.two = p.rows > 128;
+      w += u1 - u0;
+      if (w - base == (long long)units * a.Hkv * A.RT) {
+        base = w;
+        ++b;
+      }
+      if (p.t1 > p.t0) return true;
     }
-    return true;
+    return false;
   }
 };
 
@@ -151,6 +157,59 @@ __device__ __forceinline__ float ta_ex2(float x) {  // 2^x, hardware approximati
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two floats in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t ta_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void ta_unpair(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t ta_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t ta_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ta_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float ta_max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// 2^y of a pair without the special-function unit, which the weights keep busy (128 rows x
+// 128 keys take it 1024 cycles): y = n + f with n the nearest integer, a polynomial of degree 4
+// fitted to 2^f on [-1/2, 1/2] (relative error 3e-6, far under a weight's 16 bits), n added to
+// the exponent. Below -126 it stays at 2^-126. One pair in four goes this way: a tile's weights
+// take 1410 cycles against 1570 alone, 2240 against 2410 beside the other group's.
+__device__ __forceinline__ uint64_t ta_ex2_poly(uint64_t y) {
+  float u, v;
+  ta_unpair(y, u, v);
+  y = ta_pair(ta_max_nan(u, -126.f), ta_max_nan(v, -126.f));
+  const float big = 12582912.f;  // 1.5 * 2^23: the sum's low bits hold n
+  const uint64_t t = ta_add2(y, ta_pair(big, big)), n = ta_add2(t, ta_pair(-big, -big));
+  const uint64_t f = ta_fma2(n, ta_pair(-1.f, -1.f), y);
+  uint64_t p = ta_pair(0.009570097550749779f, 0.009570097550749779f);
+  p = ta_fma2(p, f, ta_pair(0.05591785907745361f, 0.05591785907745361f));
+  p = ta_fma2(p, f, ta_pair(0.240247443318367f, 0.240247443318367f));
+  p = ta_fma2(p, f, ta_pair(0.6931217908859253f, 0.6931217908859253f));
+  p = ta_fma2(p, f, ta_pair(0.9999992847442627f, 0.9999992847442627f));
+  float c, d;
+  ta_unpair(p, u, v);
+  ta_unpair(t, c, d);
+  return ta_pair(__int_as_float(__float_as_int(u) + (__float_as_int(c) << 23)),
+                 __int_as_float(__float_as_int(v) + (__float_as_int(d) << 23)));
 }
 
 // What a partial of maximum m weighs under the joint maximum `to`; parts that saw
@@ -192,15 +251,16 @@ __global__ void __launch_bounds__(TA_NT, 1)
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       tc::mbar_init(&full[i], 1);
-      tc::mbar_init(&empty[i], 1);
+      tc::mbar_init(&empty[i], 2);
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(&bars[B_Q + s], TA_SM / 32);
       tc::mbar_init(&bars[B_S + s], 1);
       tc::mbar_init(&bars[B_P + s], TA_SM / 32);
       tc::mbar_init(&bars[B_O + s], 1);
+      tc::mbar_init(&bars[B_T + s], 1);
+      tc::mbar_init(&bars[B_END + s], 1);
     }
-    tc::mbar_init(&bars[B_END], 1);
     tc::fence_mbar_init();
     misc->dead = 0;
   }
@@ -217,9 +277,9 @@ __global__ void __launch_bounds__(TA_NT, 1)
   pdl_wait();
   if (warp == 0) {  // where this CTA's share of the line of tiles starts
     const long long HR = (long long)a.Hkv * A.RT;
-    const int own0 = lane < a.B ? ta_tiles(a, lane) : 0;
+    const int own0 = lane < a.B ? ta_tiles(a, lane) + kTaLead : 0;
     long long total = own0;
-    for (int b = lane + 32; b < a.B; b += 32) total += ta_tiles(a, b);
+    for (int b = lane + 32; b < a.B; b += 32) total += ta_tiles(a, b) + kTaLead;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const long long W = total * HR, per = max(1ll, (W + gridDim.x - 1) / gridDim.x);
@@ -227,7 +287,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
     long long before = 0;
     if (w0 < w1) {
       for (int c = 0; c < a.B; c += 32) {
-        const long long own = c == 0 ? own0 : (c + lane < a.B ? ta_tiles(a, c + lane) : 0);
+        const long long own = c == 0 ? own0 : (c + lane < a.B ? ta_tiles(a, c + lane) + kTaLead : 0);
         long long upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -269,125 +329,164 @@ __global__ void __launch_bounds__(TA_NT, 1)
     return false;
   };
 
-  if (warp == TA_WARP_TMA) {
-    // ======================= TMA producer =======================================
-    // Order of use: K tiles run one tile ahead of V (two where groups take tiles in turn).
-    uint32_t k = 0;  // ring position
+  // Load numbers from a piece's first on: K_i is number i (i < lead) or lead + 2 (i - lead) + 1, V_i
+  // number lead + 2 i, short of the K loads that do not exist; the order of use, in which K runs one
+  // tile ahead of V (two where the groups take tiles in turn). Load number n uses slot n % NS.
+  auto k_load = [&](int i, int lead) { return i < lead ? i : 2 * i - lead + 1; };
+  auto v_load = [&](int i, int lead, int nt) { return min(lead, nt) + i + min(i, max(nt - lead, 0)); };
+
+  if (warp == TA_WARP_TMA || warp == TA_WARP_TMA + 1) {
+    // ======================= TMA producers: K tiles, V tiles ====================
+    const bool is_v = __shfl_sync(0xffffffffu, warp, 0) != TA_WARP_TMA;
+    const CUtensorMap* map = is_v ? &vmap : &kmap;
     const int boxes = TA_TK / A.box;
+    uint32_t base = 0;  // load number of the piece's first
+    uint32_t last = 0, any = 0;
     while (walk.next(A, p)) {
-      const int nt = p.t1 - p.t0, lead = p.two ? 1 : 2;
-      auto load = [&](const CUtensorMap* map, int tile) {
-        const uint32_t slot = k % NS;
-        if (k >= (uint32_t)NS && !__all_sync(0xffffffffu, wait(&empty[slot], k / NS - 1, 1))) return false;
-        if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], L::TILE);
-        __syncwarp();
-        if (lane < boxes) {
-          const int key = tile * TA_TK + lane * A.box;
-          int row = key, outer = p.b;
-          if (a.table) {
-            // a box past the keys, or on no page of the pool, is out of range: zeros
-            const int col = key / a.block;
-            outer = key < p.keys ? a.table[(int64_t)p.b * a.max_blocks + col] : -1;
-            if (outer < 0 || outer >= a.n_pages) outer = a.n_pages;
-            row = key - col * a.block;
-          }
-          uint8_t* dst = sm + L::RING + slot * L::TILE + lane * A.box * 128;
-#pragma unroll
-          for (int s = 0; s < SLABS; ++s)
-            tc::tma_load_4d(dst + s * (TA_TK * 128), map, &full[slot], 64 * s, row, p.h, outer);
-        }
-        __syncwarp();
-        ++k;
-        return true;
+      const int nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0), lead = __shfl_sync(0xffffffffu, p.two ? 1 : 2, 0);
+      const int h = __shfl_sync(0xffffffffu, p.h, 0), b = __shfl_sync(0xffffffffu, p.b, 0);
+      const int t0 = __shfl_sync(0xffffffffu, p.t0, 0);
+      // the page of a lane's box of a tile: -1 past the keys
+      auto page_of = [&](int i) {
+        const int key = (t0 + i) * TA_TK + lane * A.box;
+        return i < nt && lane < boxes && key < p.keys ? a.table[(int64_t)b * a.max_blocks + key / a.block] : -1;
       };
+      int page = a.table ? page_of(0) : 0;
       bool ok = true;
-      for (int i = 0; i < min(lead, nt) && ok; ++i) ok = load(&kmap, p.t0 + i);
-      for (int i = 0; i < nt && ok; ++i) {
-        ok = load(&vmap, p.t0 + i);
-        if (ok && i + lead < nt) ok = load(&kmap, p.t0 + i + lead);
+      for (int i = 0; i < nt; ++i) {
+        const int next = a.table ? page_of(i + 1) : 0;
+        const uint32_t k = base + (is_v ? v_load(i, lead, nt) : k_load(i, lead)), slot = k % NS;
+        ok = k < (uint32_t)NS || wait(&empty[slot], k / NS - 1, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* dst = sm + L::RING + slot * L::TILE;
+        if (tc::elect_one()) tc::mbar_arrive_expect_tx(&full[slot], L::TILE);
+        __syncwarp();
+        const int key0 = (t0 + i) * TA_TK;
+        if (!a.table) {
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int s = 0; s < SLABS; ++s)
+              tc::tma_load_4d(dst + s * (TA_TK * 128), map, &full[slot], 64 * s, key0, h, b);
+          }
+          __syncwarp();
+        } else {
+          // on no page of the pool: out of range, and read as zeros
+          const int there = page < 0 || page > a.n_pages ? a.n_pages : page;
+          const int row = a.block > TA_TK ? key0 & (a.block - 1) : 0;
+          auto issue = [&](auto count) {  // the boxes of a tile, all by one lane
+            constexpr int N = decltype(count)::value;
+            int at[N];
+#pragma unroll
+            for (int x = 0; x < N; ++x) at[x] = __shfl_sync(0xffffffffu, there, x);
+            if (tc::elect_one()) {
+#pragma unroll
+              for (int x = 0; x < N; ++x)
+#pragma unroll
+                for (int s = 0; s < SLABS; ++s)
+                  tc::tma_load_4d(dst + s * (TA_TK * 128) + x * (TA_TK / N) * 128, map, &full[slot], 64 * s, row, h, at[x]);
+            }
+            __syncwarp();
+          };
+          if (boxes == 1)
+            issue(std::integral_constant<int, 1>());
+          else if (boxes == 2)
+            issue(std::integral_constant<int, 2>());
+          else if (boxes == 4)
+            issue(std::integral_constant<int, 4>());
+          else if (boxes == 8)
+            issue(std::integral_constant<int, 8>());
+          else
+            issue(std::integral_constant<int, 16>());
+        }
+        last = k, any = 1;
+        page = next;
       }
       if (!ok) break;
+      base += 2 * nt;
     }
-    if (*dead) {  // every issued copy lands before the CTA may exit
-      for (uint32_t j = k > (uint32_t)NS ? k - NS : 0u; j < k; ++j) tc::mbar_wait(&full[j % NS], (j / NS) & 1, kTaWaitNs);
+    if (*dead && any) {  // every issued copy lands before the CTA may exit
+      for (uint32_t j = last >= (uint32_t)NS ? last - NS + 1 : 0u; j <= last; ++j)  // (some are the other's, or not issued)
+        tc::mbar_wait(&full[j % NS], (j / NS) & 1, kTaWaitNs / 8);
     }
-  } else if (warp == TA_WARP_MMA) {
-    // ======================= MMA issuer =========================================
-    // The products of one group run while the other group's softmax does: one warp issues
-    // both, item after item (a tile of a group), which keeps the groups half a period
-    // apart. Two warps, one for each group, let the tensor cores serve both in turn, the
-    // groups fell into step and nothing overlapped (295K keys x 224 rows: 210 us
-    // against 180). The whole warp runs this and one lane issues, so that counts,
-    // addresses and descriptors can stay in uniform registers.
+  } else if (warp >= TA_WARP_MMA) {
+    // ======================= MMA issuers ========================================
+    // A warp for each softmax group, in turns: while one issues the products of its item (a
+    // tile of its group), the other waits for its own data. The products of one group then run
+    // beside the softmax of the other. (Without turns the tensor cores served both at once, the
+    // groups fell into step and nothing overlapped: 295K keys x 224 rows in 210 us against 180.)
+    // The whole warp runs this and one lane issues, so that counts, addresses and descriptors
+    // can stay in uniform registers.
     constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
     constexpr uint32_t ID_PV = tc::idesc_f16(BF16, 128, D, false, true);
     constexpr uint32_t LBO_V = SLABS == 2 ? TA_TK * 128 : 0;
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int s = __shfl_sync(0xffffffffu, warp - TA_WARP_MMA, 0);
+    const uint32_t ts = __shfl_sync(0xffffffffu, tmem, 0) + s * 128, to = ts + 256;
     const uint32_t ring0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::RING), 0);
-    const uint64_t qd0 = tc::smem_desc(__shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0), 16, 1024);
-    uint32_t k = 0, n_q0 = 0, n_q1 = 0, n_p0 = 0, n_p1 = 0;
+    const uint64_t qd = tc::smem_desc(__shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0) + s * L::TILE, 16, 1024);
+    uint32_t base = 0, n_q = 0, n_p = 0, n_t = 0;
+    bool handed = false;  // group 1 issued the last item of the piece before, and handed the turn over
     bool ok = true;
     while (ok && walk.next(A, p)) {
-      // load numbers from k on: K_i is number i (i < lead) or lead + 2 (i - lead) + 1, V_i number
-      // lead + 2 i, short of the K loads that do not exist
       const int two = __shfl_sync(0xffffffffu, (int)p.two, 0), nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
-      const int items = two ? 2 * nt : nt, lead = two ? 1 : 2, ahead = min(lead, nt);
-      auto k_at = [&](int i) { return k + (i < lead ? i : lead + 2 * (i - lead) + 1); };
-      auto qk = [&](int item) {
-        const int s = item & 1;
-        const uint32_t slot = k_at(two ? item >> 1 : item) % NS;
+      const int lead = two ? 1 : 2, step = lead, first = two ? 0 : s;
+      auto release = [&](uint64_t* bar) {  // two arrivals empty a slot: one of each group, or both of its only one
+        tc::mma_commit(bar);
+        if (!two) tc::mma_commit(bar);
+      };
+      auto qk = [&](uint32_t slot) {
         const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
-        const uint64_t qd = tc::desc_add(qd0, s * L::TILE);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
-          tc::mma_f16(tm + s * 128, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
+          tc::mma_f16(ts, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
         }
         tc::mma_commit(&bars[B_S + s]);
-        if (!two || s == 1) tc::mma_commit(&empty[slot]);
+        release(&empty[slot]);
       };
-      for (int item = 0; item < min(2, items) && ok; ++item) {
-        const uint32_t at = k_at(two ? item >> 1 : item);
-        ok = wait(&bars[B_Q + item], item ? n_q1++ : n_q0++, 2) && wait(&full[at % NS], at / NS, 3);
+      if (first < nt) {  // the first product, out of turn: nothing is running yet
+        const uint32_t at = base + k_load(first, lead), slot = at % NS;
+        ok = wait(&bars[B_Q + s], n_q++, 2) && wait(&full[slot], at / NS, 3);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) qk(item);
-        __syncwarp();
-      }
-      for (int item = 0; item < items && ok; ++item) {
-        const int s = item & 1, i = two ? item >> 1 : item;
-        const uint32_t at = k + ahead + i + min(i, max(nt - lead, 0)), slot = at % NS;
-        const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
-        const bool more = item + 2 < items;
-        // V and the next K are mostly there before the weights are: nothing waits between the products
-        ok = wait(&full[slot], at / NS, 4);
-        if (more) {
-          const uint32_t kat = k_at(two ? (item + 2) >> 1 : item + 2);
-          ok = ok && wait(&full[kat % NS], kat / NS, 3);
+        if (ok) {
+          tc::tc_fence_after();
+          if (tc::elect_one()) qk(slot);
+          __syncwarp();
         }
-        ok = ok && wait(&bars[B_P + s], s ? n_p1++ : n_p0++, 5);
+      }
+      for (int i = first; i < nt && ok; i += step) {
+        const uint32_t at = base + v_load(i, lead, nt), slot = at % NS;
+        const uint32_t kat = base + k_load(i + step, lead), kslot = kat % NS;
+        const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
+        const bool more = i + step < nt;
+        ok = wait(&full[slot], at / NS, 4) && (!more || wait(&full[kslot], kat / NS, 3));
+        // the group's turn comes when the other has issued the item before this one
+        if (s == 1 || i > first || handed) ok = ok && wait(&bars[B_T + s], n_t++, 10);
+        ok = ok && wait(&bars[B_P + s], n_p++, 5);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::tc_fence_after();
         if (tc::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < TA_TK / 16; ++kk)
-            tc::mma_f16_tmem_a(tm + 256 + s * 128, tm + s * 128 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV,
-                               item >= 2 || kk > 0);
-          if (!two || s == 1) tc::mma_commit(&empty[slot]);
+            tc::mma_f16_tmem_a(to, ts + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV, i > first || kk > 0);
+          release(&empty[slot]);
           if (more)
-            qk(item + 2);
+            qk(kslot);
           else
             tc::mma_commit(&bars[B_O + s]);
+          // the next item is the other group's; after a piece's last it is group 0's
+          if (s == 1 || two || i + 1 < nt) tc::mbar_arrive(&bars[B_T + 1 - s]);
         }
         __syncwarp();
       }
-      k += 2 * nt;
+      base += 2 * nt;
+      handed = two || nt % 2 == 0;
     }
     if (*dead) {  // no product may run on when tensor memory is given back
-      if (lane == 0) tc::mma_commit(&bars[B_END]);
-      tc::mbar_wait(&bars[B_END], 0, kTaWaitNs);
+      if (tc::elect_one()) tc::mma_commit(&bars[B_END + s]);
+      __syncwarp();
+      tc::mbar_wait(&bars[B_END + s], 0, kTaWaitNs);
     }
   } else {
     // ======================= softmax groups =====================================
@@ -397,7 +496,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
     const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256;
     float* ml0 = reinterpret_cast<float*>(sm + L::Q);  // [2][128]: maxima, sums
     float* ml1 = reinterpret_cast<float*>(sm + L::Q + L::TILE);
-    uint32_t n_s = 0, n_o = 0, k = 0;
+    uint32_t n_s = 0, n_o = 0, base = 0;
     bool ok = true;
     for (int piece = 0; walk.next(A, p); ++piece) {
       const int nt = p.t1 - p.t0;
@@ -407,9 +506,6 @@ __global__ void __launch_bounds__(TA_NT, 1)
       const bool live = quad * 32 < rows;  // some row of this warp exists
       uint32_t* bad_now = bad + 8 * (piece & 1);
       float m = -INFINITY, l = 0.f;
-      uint32_t mw[8];  // nodes that this thread's row sees
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mw[i] = 0;
       if (mine) {
         // Q rows into shared memory, 16 bytes a thread and step: row = head of the group, then
         // node. The loads of eight steps are on their way before the first is stored.
@@ -444,35 +540,8 @@ __global__ void __launch_bounds__(TA_NT, 1)
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bars[B_Q + s]);
-        // the mask's rows, where the piece reaches the tree: a warp reads each of its rows
-        if (p.t1 * TA_TK > p.len && live) {
-          const int fit = p.keys - p.len;  // nodes that fit the cache
-          const int first = row0 + quad * 32, count = min(32, rows - quad * 32);
-          const int node0 = first - A.by_t.quot(first) * a.T;
-          const uint8_t* mb = a.mask ? a.mask + p.b * a.mask_sb : nullptr;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (i * 32 >= fit) break;
-            const int j = i * 32 + lane, jc = min(j, fit - 1);
-            const uint8_t* mc = mb + jc * a.mask_sc;
-            int node = node0;  // rows follow one another, their nodes too, around the tree
-            for (int q0 = 0; q0 < count; q0 += 16) {  // sixteen rows' bytes on their way at once
-              uint32_t see[16];
-#pragma unroll
-              for (int q = 0; q < 16; ++q) {
-                see[q] = mb ? mc[node * a.mask_sr] : jc <= node;
-                node = node + 1 == a.T ? 0 : node + 1;
-              }
-#pragma unroll
-              for (int q = 0; q < 16; ++q) {
-                const uint32_t word = __ballot_sync(0xffffffffu, see[q] != 0 && j < fit);
-                if (q0 + q == lane) mw[i] = word;
-              }
-            }
-          }
-        }
       }
-      const int lead = p.two ? 1 : 2, ahead = min(lead, nt), step = lead;
+      const int lead = p.two ? 1 : 2, step = lead;
       for (int i = p.two ? 0 : s; i < nt && ok; i += step) {
         const int j0 = (p.t0 + i) * TA_TK;
         // which of the tile's pages are missing (a lane for each): 16 bits, from 8 rows up
@@ -487,78 +556,68 @@ __global__ void __launch_bounds__(TA_NT, 1)
           gone = __ballot_sync(0xffffffffu, no);
         }
         const bool tree = j0 + TA_TK > p.len;  // the tile holds nodes, or ends the keys
+        uint32_t see[4];  // the keys of the tile that this thread's row sees
+        if ((tree || gone) && live) {
+          const int first = row0 + quad * 32, count = min(32, rows - quad * 32);
+          const int node0 = first - A.by_t.quot(first) * a.T;
+          const uint8_t* mb = a.mask ? a.mask + p.b * a.mask_sb : nullptr;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int n0 = j0 + 32 * w - p.len, n = n0 + lane;  // the word's and this lane's node, negative in the cache
+            see[w] = n0 + 31 < 0 ? 0xffffffffu : 0u;
+            if (n0 + 31 >= 0 && p.len + n0 < p.keys) {  // the warp reads the mask bytes of each of its rows
+              const bool node_there = n >= 0 && p.len + n < p.keys;
+              const uint8_t* mc = mb + (node_there ? n : 0) * a.mask_sc;
+              int node = node0;  // rows follow one another, their nodes too, around the tree
+              for (int q0 = 0; q0 < count; q0 += 16) {  // sixteen rows' bytes on their way at once
+                uint32_t x[16];
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                  x[q] = mb ? mc[node * a.mask_sr] : n <= node;
+                  node = node + 1 == a.T ? 0 : node + 1;
+                }
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                  const uint32_t word = __ballot_sync(0xffffffffu, n < 0 || (node_there && x[q] != 0));
+                  if (q0 + q == lane) see[w] = word;
+                }
+              }
+            }
+            if (gone) {
+              for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
+                if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+            }
+          }
+        }
         ok = __all_sync(0xffffffffu, wait(&bars[B_S + s], n_s++, 6));
         if (!ok) break;
         tc::tc_fence_after();
         if (live) {
           const bool masked = tree || gone;
-          uint32_t see[4];
+          // S is read twice, for the maximum and for the weights, which overwrite it as they come:
+          // a row of 128 does not stay in registers
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           if (masked) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const int at = j0 + 32 * w - p.len;  // the node of the word's first key, negative in the cache
-              uint32_t lo = 0, hi = 0;
-              const int q = at >> 5;               // rounds down
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                lo = q == i ? mw[i] : lo;
-                hi = q + 1 == i ? mw[i] : hi;
-              }
-              if (q < 0) lo = 0xffffffffu;
-              if (q + 1 < 0) hi = 0xffffffffu;
-              see[w] = __funnelshift_r(lo, hi, at & 31);
-              if (gone) {
-                for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
-                  if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
-              }
-            }
-          }
-          float top = -INFINITY, sum = 0.f;
-          uint32_t pk[64];
-          // the weights against the reference m, and the maximum, in one pass over S
-          auto weigh = [&](auto hide) {
-            const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sm4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
               float x[32];
               tc::tmem_ld32(ts + 32 * w, x);
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                if (decltype(hide)::value) {
-                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
-                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
-                }
-                mx[e & 3] = fmaxf(mx[e & 3], x[e]);
-                mx[(e & 3) + 1] = fmaxf(mx[(e & 3) + 1], x[e + 1]);
-                const float u = ta_ex2(fmaf(x[e], A.scale_log2, -ref)), v = ta_ex2(fmaf(x[e + 1], A.scale_log2, -ref));
-                sm4[e & 3] += u;
-                sm4[(e & 3) + 1] += v;
-                pk[16 * w + e / 2] = TaType<T>::pack(u, v);
-              }
+              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (see[w] >> e) & 1 ? x[e] : -INFINITY);
             }
-            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-            sum = (sm4[0] + sm4[1]) + (sm4[2] + sm4[3]);
-          };
-          const bool first = i < step;
-          if (first) {  // no reference yet: the maximum alone
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              float x[32];
-              tc::tmem_ld32(ts + 32 * w, x);
-              const uint32_t sw = masked ? see[w] : 0xffffffffu;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (sw >> e) & 1 ? x[e] : -INFINITY);
-            }
-            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-          } else if (masked) {
-            weigh(std::true_type());
           } else {
-            weigh(std::false_type());
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              float x[64];
+              tc::tmem_ld64(ts + 64 * w, x);
+#pragma unroll
+              for (int e = 0; e < 64; e += 2) mx[(e / 2) & 3] = ta_max3(mx[(e / 2) & 3], x[e], x[e + 1]);
+            }
           }
-          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves: weigh (again)
-            const float mn = top > m + kTaSlack ? top : m;
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+          const bool first = i < step;
+          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves
+            const float mn = first || top > m + kTaSlack ? top : m;
             const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
             m = mn;
             l *= alpha;
@@ -573,20 +632,52 @@ __global__ void __launch_bounds__(TA_NT, 1)
                 tc::tmem_st_wait();
               }
             }
-            if (masked)
-              weigh(std::true_type());
-            else
-              weigh(std::false_type());
           }
-          l += sum;
+          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
+          const uint64_t scale2 = ta_pair(A.scale_log2, A.scale_log2), ref2 = ta_pair(-ref, -ref);
+          uint64_t sum[2] = {0, 0};
+          auto weigh = [&](auto hide) {
 #pragma unroll
-          for (int c = 0; c < 64; c += 16) tc::tmem_st16(ts + c, reinterpret_cast<const float*>(pk + c));  // over S, which is read
+            for (int w = 0; w < 4; ++w) {
+              float x[32];
+              tc::tmem_ld32(ts + 32 * w, x);
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                if (decltype(hide)::value) {
+                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
+                }
+                uint64_t y = ta_fma2(ta_pair(x[e], x[e + 1]), scale2, ref2);
+                if (!decltype(hide)::value && (e / 2) % 4 == 3) {
+                  y = ta_ex2_poly(y);
+                } else {
+                  float u, v;
+                  ta_unpair(y, u, v);
+                  y = ta_pair(ta_ex2(u), ta_ex2(v));
+                }
+                sum[(e / 2) & 1] = ta_add2(sum[(e / 2) & 1], y);
+                float u, v;
+                ta_unpair(y, u, v);
+                pk[e / 2] = TaType<T>::pack(u, v);
+              }
+              tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
+            }
+          };
+          if (masked)
+            weigh(std::true_type());
+          else
+            weigh(std::false_type());
+          float s0, s1, s2, s3;
+          ta_unpair(sum[0], s0, s1);
+          ta_unpair(sum[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
           tc::tmem_st_wait();
         }
         if (tree) {
           // rows of V that a weight of 0 would not silence: past the keys they are cleared, and
           // non-finite values of a node are taken out here and given to its viewers at the end
-          const uint32_t at = k + ahead + i + min(i, max(nt - lead, 0)), slot = at % NS;
+          const uint32_t at = base + v_load(i, lead, nt), slot = at % NS;
           ok = __all_sync(0xffffffffu, wait(&full[slot], at / NS, 7));
           if (!ok) break;
           const int key = j0 + r;
@@ -632,7 +723,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bars[B_P + s]);
       }
-      k += 2 * nt;
+      base += 2 * nt;
       // ---- the piece's output ---------------------------------------------------
       if (mine && ok) ok = __all_sync(0xffffffffu, wait(&bars[B_O + s], n_o++, 8));
       m -= A.bias;  // the reference the weights were taken against
@@ -682,25 +773,23 @@ __global__ void __launch_bounds__(TA_NT, 1)
             for (int e = 0; e < 16; ++e) o[e] = fmaf(o1[e], f1, o[e]);
           }
           if (any_bad && own) {  // the non-finite values of the nodes this row sees
+            const int node = mrow - A.by_t.quot(mrow) * a.T;
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-              uint32_t seen = 0;
+            for (int n = 0; n < a.T; ++n) {
+              if (!((bad_now[n >> 5] >> (n & 31)) & 1)) continue;
+              if (a.mask ? a.mask[p.b * a.mask_sb + node * a.mask_sr + n * a.mask_sc] == 0 : n > node) continue;
+              const int key = p.len + n;
+              const T* v = static_cast<const T*>(a.v) + p.h * a.v_sh;
+              if (a.table) {
+                const int page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
+                v += page * a.v_s0 + (key % a.block) * a.v_ss;  // a page that was read
+              } else {
+                v += p.b * a.v_s0 + key * a.v_ss;
+              }
 #pragma unroll
-              for (int q = 0; q < 8; ++q) seen = q == i ? mw[q] & bad_now[q] : seen;
-              for (; seen; seen &= seen - 1) {
-                const int key = p.len + 32 * i + __ffs(seen) - 1;
-                const T* v = static_cast<const T*>(a.v) + p.h * a.v_sh;
-                if (a.table) {
-                  const int page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
-                  v += page * a.v_s0 + (key % a.block) * a.v_ss;  // a page that was read
-                } else {
-                  v += p.b * a.v_s0 + key * a.v_ss;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float y = to_f(v[c + e]);
-                  if (!isfinite(y)) o[e] += y;
-                }
+              for (int e = 0; e < 16; ++e) {
+                const float y = to_f(v[c + e]);
+                if (!isfinite(y)) o[e] += y;
               }
             }
           }
@@ -763,7 +852,7 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   pdl_wait();
   long long before = 0, total = 0;
   for (int i = tid; i < a.B; i += TM_NT) {
-    const int t = ta_tiles(a, i);
+    const int t = ta_tiles(a, i) + kTaLead;
     total += t;
     before += i < b ? t : 0;
   }
@@ -779,7 +868,7 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   for (int w = 0; w < TM_NT / 32; ++w) total += red[0][w], before += red[1][w];
   const long long W = total * HR, per = max(1ll, (W + ctas - 1) / ctas);
   const int tiles = ta_tiles(a, b);
-  const long long w0 = before * HR + (long long)seg * tiles, w1 = w0 + tiles;
+  const long long w0 = before * HR + (long long)seg * (tiles + kTaLead) + kTaLead, w1 = w0 + tiles;
   const int c0 = (int)(w0 / per), n = (int)((w1 - 1) / per) - c0 + 1;
   if (n == 1) return;  // written by its one CTA
   // partial i is CTA c0 + i's: the segment is the last piece of the first CTA, the first of the others
