@@ -48,10 +48,12 @@ struct TaArgs {
   TreeAttn a;
   TaDiv by_t;
   int g, M, RT;            // query rows of a KV head: M = g T, in RT segments of 256
+  int HR;                  // segments of a sequence: Hkv RT
   int box;                 // rows of a TMA box
   int rows_pad;            // rows of a partial
   float scale_log2;
   int q_vec;               // Q's rows are read 16 bytes at a time
+  int mask_vec;            // the mask's rows are read 4 bytes at a time
   float bias;              // weights are 2^(s - m + bias): fp16 has few bits below 1
   int* status;             // [CTAs]: 0, or which wait gave up
   float* part_o;           // [2 CTAs][D / 4][rows_pad] float4
@@ -75,7 +77,7 @@ struct TaSmem {
 static_assert(TaSmem<128>::BYTES <= 232448, "shared memory");
 
 struct TaMisc {
-  long long w0, w1, base;  // this CTA's units, and the first unit of sequence b0
+  int w0, w1, base;  // this CTA's units, and the first unit of sequence b0
   int b0;
   uint32_t tmem;
   int dead;
@@ -97,7 +99,7 @@ struct TaPiece {
 // (Q, an output, an empty pipeline): a CTA that ends a segment gets that much less of the next.
 constexpr int kTaLead = 4;
 struct TaWalk {
-  long long w, w1, base;  // units
+  int w, w1, base;  // units
   int b;
   __device__ __forceinline__ bool next(const TaArgs& A, TaPiece& p) {
     const TreeAttn& a = A.a;
@@ -107,10 +109,8 @@ struct TaWalk {
       p.keys = ta_keys(a, p.len);
       p.tiles = (p.keys + TA_TK - 1) / TA_TK;
       const int units = p.tiles + kTaLead;
-      const long long rel = w - base;
-      const int seg = (int)(rel / units);
-      const int u0 = (int)(rel - (long long)seg * units);
-      const int u1 = (int)min((long long)units, u0 + (w1 - w));
+      const int rel = w - base, seg = rel / units, u0 = rel - seg * units;
+      const int u1 = min(units, u0 + (w1 - w));
       p.t0 = max(u0 - kTaLead, 0);
       p.t1 = u1 - kTaLead;
       p.h = seg / A.RT;
@@ -118,7 +118,7 @@ struct TaWalk {
       p.rows = min(TA_ROWS, A.M - p.rt * TA_ROWS);
       p.two = p.rows > 128;
       w += u1 - u0;
-      if (w - base == (long long)units * a.Hkv * A.RT) {
+      if (w - base == units * A.HR) {
         base = w;
         ++b;
       }
@@ -276,30 +276,29 @@ __global__ void __launch_bounds__(TA_NT, 1)
   pdl_launch_dependents();
   pdl_wait();
   if (warp == 0) {  // where this CTA's share of the line of tiles starts
-    const long long HR = (long long)a.Hkv * A.RT;
     const int own0 = lane < a.B ? ta_tiles(a, lane) + kTaLead : 0;
-    long long total = own0;
+    int total = own0;
     for (int b = lane + 32; b < a.B; b += 32) total += ta_tiles(a, b) + kTaLead;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const long long W = total * HR, per = max(1ll, (W + gridDim.x - 1) / gridDim.x);
-    const long long w0 = min(W, per * blockIdx.x), w1 = min(W, w0 + per);
-    long long before = 0;
+    const int W = total * A.HR, per = (W + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int w0 = min((long long)W, (long long)per * blockIdx.x), w1 = min(W, w0 + per);
     if (w0 < w1) {
+      int before = 0;
       for (int c = 0; c < a.B; c += 32) {
-        const long long own = c == 0 ? own0 : (c + lane < a.B ? ta_tiles(a, c + lane) + kTaLead : 0);
-        long long upto = own;
+        const int own = c == 0 ? own0 : (c + lane < a.B ? ta_tiles(a, c + lane) + kTaLead : 0);
+        int upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+          const int x = __shfl_up_sync(0xffffffffu, upto, o);
           if (lane >= o) upto += x;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * HR > w0);
+        const unsigned past = __ballot_sync(0xffffffffu, (before + upto) * A.HR > w0);
         if (past) {
           const int at = __ffs(past) - 1;
           if (lane == at) {
             misc->b0 = c + at;
-            misc->base = (before + upto - own) * HR;
+            misc->base = (before + upto - own) * A.HR;
           }
           break;
         }
@@ -508,34 +507,41 @@ __global__ void __launch_bounds__(TA_NT, 1)
       float m = -INFINITY, l = 0.f;
       if (mine) {
         // Q rows into shared memory, 16 bytes a thread and step: row = head of the group, then
-        // node. The loads of eight steps are on their way before the first is stored.
+        // node. The loads of all steps are on their way before the first is stored.
         const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh;
         constexpr int STEP = TA_SM / (D / 8);  // rows a step of the group covers
         const int c = r % (D / 8);             // a thread's column of vectors stays, its row moves on
+        const int e0 = r / (D / 8);
+        uint4 x[128 / STEP];
+        auto src = [&](int i) {
+          const int mrow = row0 + min(e0 + i * STEP, rows - 1), head = A.by_t.quot(mrow);
+          return qb + head * a.q_sh + (mrow - head * a.T) * a.q_ss + c * 8 * a.q_sd;
+        };
+        if (A.q_vec) {
+#pragma unroll
+          for (int i = 0; i < 128 / STEP; ++i) x[i] = *reinterpret_cast<const uint4*>(src(i));
+        } else {
 #pragma unroll 1
-        for (int e0 = r / (D / 8); e0 < 128; e0 += 8 * STEP) {
-          uint4 x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int mrow = row0 + min(e0 + i * STEP, rows - 1), head = A.by_t.quot(mrow);
-            const T* src = qb + head * a.q_sh + (mrow - head * a.T) * a.q_ss + c * 8 * a.q_sd;
-            if (A.q_vec) {
-              x[i] = *reinterpret_cast<const uint4*>(src);
-            } else {
-              const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-              x[i].x = h[0] | (uint32_t)h[a.q_sd] << 16;
-              x[i].y = h[2 * a.q_sd] | (uint32_t)h[3 * a.q_sd] << 16;
-              x[i].z = h[4 * a.q_sd] | (uint32_t)h[5 * a.q_sd] << 16;
-              x[i].w = h[6 * a.q_sd] | (uint32_t)h[7 * a.q_sd] << 16;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 128 / STEP; ++i) {  // (x stays in registers: rows are stored as they come)
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(src(i));
+            uint4 y;
+            y.x = h[0] | (uint32_t)h[a.q_sd] << 16;
+            y.y = h[2 * a.q_sd] | (uint32_t)h[3 * a.q_sd] << 16;
+            y.z = h[4 * a.q_sd] | (uint32_t)h[5 * a.q_sd] << 16;
+            y.w = h[6 * a.q_sd] | (uint32_t)h[7 * a.q_sd] << 16;
             const int row = e0 + i * STEP;
-            if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (row >= rows) y = make_uint4(0u, 0u, 0u, 0u);
             *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
-                                      tc::sw128_offset(row, (c % 8) * 8)) = x[i];
+                                      tc::sw128_offset(row, (c % 8) * 8)) = y;
           }
+        }
+        if (A.q_vec)
+#pragma unroll
+        for (int i = 0; i < 128 / STEP; ++i) {
+          const int row = e0 + i * STEP;
+          if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
+                                    tc::sw128_offset(row, (c % 8) * 8)) = x[i];
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -544,53 +550,70 @@ __global__ void __launch_bounds__(TA_NT, 1)
       const int lead = p.two ? 1 : 2, step = lead;
       for (int i = p.two ? 0 : s; i < nt && ok; i += step) {
         const int j0 = (p.t0 + i) * TA_TK;
-        // which of the tile's pages are missing (a lane for each): 16 bits, from 8 rows up
-        uint32_t gone = 0;
+        // the page of a lane's box of the tile, looked at once S is there
+        int page = 0;
         if (a.table) {
           const int key = j0 + lane * A.box;
-          bool no = false;
-          if (lane < TA_TK / A.box && key < p.keys) {
-            const int page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
-            no = page < 0 || page >= a.n_pages;
-          }
-          gone = __ballot_sync(0xffffffffu, no);
+          if (lane < TA_TK / A.box && key < p.keys) page = a.table[(int64_t)p.b * a.max_blocks + key / a.block];
         }
         const bool tree = j0 + TA_TK > p.len;  // the tile holds nodes, or ends the keys
-        uint32_t see[4];  // the keys of the tile that this thread's row sees
-        if ((tree || gone) && live) {
-          const int first = row0 + quad * 32, count = min(32, rows - quad * 32);
-          const int node0 = first - A.by_t.quot(first) * a.T;
-          const uint8_t* mb = a.mask ? a.mask + p.b * a.mask_sb : nullptr;
+        uint32_t see[4] = {0u, 0u, 0u, 0u};    // the keys of the tile that this thread's row sees
+        if (tree && live) {
+          const int mrow = row0 + min(r, rows - 1), node = mrow - A.by_t.quot(mrow) * a.T, fit = p.keys - p.len;
+          const uint8_t* mr = a.mask ? a.mask + p.b * a.mask_sb + node * a.mask_sr : nullptr;
+          const int n0 = j0 - p.len, q0 = n0 >> 5;  // the tile's first node, and its word of 32 nodes (rounded down)
+          uint32_t words[5];                         // words q0 .. q0 + 4 of what the row sees
+          if (mr && A.mask_vec) {
+            uint32_t x[5][8];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int n0 = j0 + 32 * w - p.len, n = n0 + lane;  // the word's and this lane's node, negative in the cache
-            see[w] = n0 + 31 < 0 ? 0xffffffffu : 0u;
-            if (n0 + 31 >= 0 && p.len + n0 < p.keys) {  // the warp reads the mask bytes of each of its rows
-              const bool node_there = n >= 0 && p.len + n < p.keys;
-              const uint8_t* mc = mb + (node_there ? n : 0) * a.mask_sc;
-              int node = node0;  // rows follow one another, their nodes too, around the tree
-              for (int q0 = 0; q0 < count; q0 += 16) {  // sixteen rows' bytes on their way at once
-                uint32_t x[16];
+            for (int w = 0; w < 5; ++w)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                  x[q] = mb ? mc[node * a.mask_sr] : n <= node;
-                  node = node + 1 == a.T ? 0 : node + 1;
-                }
+              for (int e = 0; e < 8; ++e) {
+                const int n = 32 * (q0 + w) + 4 * e;
+                x[w][e] = n >= 0 && n < fit ? *reinterpret_cast<const uint32_t*>(mr + n) : 0u;
+              }
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                  const uint32_t word = __ballot_sync(0xffffffffu, n < 0 || (node_there && x[q] != 0));
-                  if (q0 + q == lane) see[w] = word;
-                }
+            for (int w = 0; w < 5; ++w) {
+              words[w] = 0;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {  // four truth values to four bits
+                const uint32_t y = __vcmpne4(x[w][e], 0u) & 0x01010101u;
+                words[w] |= ((y * 0x10204080u) >> 28) << (4 * e);
               }
             }
-            if (gone) {
-              for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
-                if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+          } else {
+#pragma unroll
+            for (int w = 0; w < 5; ++w) {
+              words[w] = 0;
+              if (32 * (q0 + w) + 32 <= 0 || 32 * (q0 + w) >= fit) continue;
+#pragma unroll 8
+              for (int e = 0; e < 32; ++e) {
+                const int n = 32 * (q0 + w) + e;
+                if (n >= 0 && n < fit && (mr ? mr[n * a.mask_sc] != 0 : n <= node)) words[w] |= 1u << e;
+              }
             }
           }
+#pragma unroll
+          for (int w = 0; w < 5; ++w) {  // every cached row is seen, nothing past the last node that fits
+            const int n = 32 * (q0 + w);
+            if (n < 0) words[w] = 0xffffffffu;
+            if (n + 32 > fit) words[w] &= n >= fit ? 0u : 0xffffffffu >> (32 - (fit - n));
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) see[w] = __funnelshift_r(words[w], words[w + 1], n0 & 31);
         }
         ok = __all_sync(0xffffffffu, wait(&bars[B_S + s], n_s++, 6));
         if (!ok) break;
+        uint32_t gone = 0;  // which of the tile's pages are missing: 16 bits, from 8 rows up
+        if (a.table) gone = __ballot_sync(0xffffffffu, page < 0 || page >= a.n_pages);
+        if (gone) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if (!tree) see[w] = 0xffffffffu;
+            for (int key = 0; key < 32; key += 8)  // boxes have 8 rows at least
+              if ((gone >> ((32 * w + key) / A.box)) & 1) see[w] &= ~(0xffu << key);
+          }
+        }
         tc::tc_fence_after();
         if (live) {
           const bool masked = tree || gone;
@@ -839,18 +862,17 @@ constexpr int TM_PIECES = 64;  // partials whose factors are held at once
 // The eight warps first share out the partials' maxima and sums.
 template <typename T, int D>
 __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ctas) {
-  __shared__ long long red[2][TM_NT / 32];
+  __shared__ int red[2][TM_NT / 32];
   __shared__ float fac[TM_PIECES][32], mxs[TM_NT / 32][32], sums[TM_NT / 32][32];
   const TreeAttn& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int HR = a.Hkv * A.RT;
-  const int b = (int)(blockIdx.x / (unsigned)HR), seg = (int)(blockIdx.x % (unsigned)HR);
+  const int b = blockIdx.x / A.HR, seg = blockIdx.x % A.HR;
   const int rt = seg % A.RT, h = seg / A.RT;
   const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
   const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
   if (rt * TA_ROWS + rb * 32 >= A.M) return;
   pdl_wait();
-  long long before = 0, total = 0;
+  int before = 0, total = 0;
   for (int i = tid; i < a.B; i += TM_NT) {
     const int t = ta_tiles(a, i) + kTaLead;
     total += t;
@@ -866,10 +888,9 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   total = before = 0;
 #pragma unroll
   for (int w = 0; w < TM_NT / 32; ++w) total += red[0][w], before += red[1][w];
-  const long long W = total * HR, per = max(1ll, (W + ctas - 1) / ctas);
-  const int tiles = ta_tiles(a, b);
-  const long long w0 = before * HR + (long long)seg * (tiles + kTaLead) + kTaLead, w1 = w0 + tiles;
-  const int c0 = (int)(w0 / per), n = (int)((w1 - 1) / per) - c0 + 1;
+  const int per = (total * A.HR + ctas - 1) / ctas, tiles = ta_tiles(a, b);
+  const int w0 = before * A.HR + seg * (tiles + kTaLead) + kTaLead, w1 = w0 + tiles;
+  const int c0 = w0 / per, n = (w1 - 1) / per - c0 + 1;
   if (n == 1) return;  // written by its one CTA
   // partial i is CTA c0 + i's: the segment is the last piece of the first CTA, the first of the others
   auto slot = [&](int i) { return (int64_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
@@ -961,10 +982,14 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   A.g = a.Hq / a.Hkv;
   A.M = A.g * a.T;
   A.RT = (A.M + TA_ROWS - 1) / TA_ROWS;
+  A.HR = a.Hkv * A.RT;
+  if ((int64_t)a.B * A.HR * ((a.cap + TA_TK - 1) / TA_TK + 1 + kTaLead) > 0x7fffffff)
+    return fail(DROPKV_ERR_UNSUPPORTED, "tree attention: %d sequences of up to %d rows are too many tiles", a.B, a.cap);
   A.box = a.table ? std::min(a.block, TA_TK) : TA_TK;
   A.rows_pad = plan.rows_pad;
   A.scale_log2 = a.scale * 1.4426950408889634f;
   A.bias = bf16 ? 0.f : 7.f;
+  A.mask_vec = a.mask_sc == 1 && a.T % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mask) | (uint64_t)(a.mask_sb | a.mask_sr)) % 4 == 0;
   A.q_vec = a.q_sd == 1 && (reinterpret_cast<uintptr_t>(a.q) | (uint64_t)((a.q_sb | a.q_sh | a.q_ss) * 2)) % 16 == 0;
   A.status = static_cast<int*>(ws);
   A.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_o);
