@@ -60,8 +60,9 @@ struct TaArgs {
   float* part_ml;          // [2 CTAs][2][rows_pad]
 };
 
-// per softmax group s: Q written, S ready, P ready, O ready, its turn to issue, every product done
-enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 6, B_T = 8, B_END = 10, B_COUNT = 12 };
+// per softmax group s: Q written, S ready, P ready (keys 0 to 63; and, at + 2, 64 to 127), O ready,
+// its turn to issue, every product done
+enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 8, B_T = 10, B_END = 12, B_COUNT = 14 };
 
 template <int D>
 struct TaSmem {
@@ -257,6 +258,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
       tc::mbar_init(&bars[B_Q + s], TA_SM / 32);
       tc::mbar_init(&bars[B_S + s], 1);
       tc::mbar_init(&bars[B_P + s], TA_SM / 32);
+      tc::mbar_init(&bars[B_P + 2 + s], TA_SM / 32);
       tc::mbar_init(&bars[B_O + s], 1);
       tc::mbar_init(&bars[B_T + s], 1);
       tc::mbar_init(&bars[B_END + s], 1);
@@ -400,6 +402,8 @@ __global__ void __launch_bounds__(TA_NT, 1)
         }
         last = k, any = 1;
         page = next;
+        // the first piece's Q comes before the rest of the ring: 160 KB an SM at once hold it up by 3 us
+        if (base == 0 && i == 0) wait(&bars[B_Q], 0, 11);
       }
       if (!ok) break;
       base += 2 * nt;
@@ -461,14 +465,21 @@ __global__ void __launch_bounds__(TA_NT, 1)
         ok = wait(&full[slot], at / NS, 4) && (!more || wait(&full[kslot], kat / NS, 3));
         // the group's turn comes when the other has issued the item before this one
         if (s == 1 || i > first || handed) ok = ok && wait(&bars[B_T + s], n_t++, 10);
-        ok = ok && wait(&bars[B_P + s], n_p++, 5);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc::tc_fence_after();
-        if (tc::elect_one()) {
+        for (int half = 0; half < 2 && ok; ++half) {
+          ok = __all_sync(0xffffffffu, ok && wait(&bars[B_P + 2 * half + s], n_p, 5));
+          if (!ok) break;
+          tc::tc_fence_after();
+          if (tc::elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < TA_TK / 16; ++kk)
-            tc::mma_f16_tmem_a(to, ts + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV, i > first || kk > 0);
+            for (int kk = 0; kk < TA_TK / 32; ++kk)
+              tc::mma_f16_tmem_a(to, ts + half * 32 + kk * 8, tc::desc_add(vd, half * (TA_TK * 64) + kk * 2048), ID_PV,
+                                 i > first || half > 0 || kk > 0);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        ++n_p;
+        if (tc::elect_one()) {
           release(&empty[slot]);
           if (more)
             qk(kslot);
@@ -615,88 +626,6 @@ __global__ void __launch_bounds__(TA_NT, 1)
           }
         }
         tc::tc_fence_after();
-        if (live) {
-          const bool masked = tree || gone;
-          // S is read twice, for the maximum and for the weights, which overwrite it as they come:
-          // a row of 128 does not stay in registers
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (masked) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              float x[32];
-              tc::tmem_ld32(ts + 32 * w, x);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (see[w] >> e) & 1 ? x[e] : -INFINITY);
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              float x[64];
-              tc::tmem_ld64(ts + 64 * w, x);
-#pragma unroll
-              for (int e = 0; e < 64; e += 2) mx[(e / 2) & 3] = ta_max3(mx[(e / 2) & 3], x[e], x[e + 1]);
-            }
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
-          const bool first = i < step;
-          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves
-            const float mn = first || top > m + kTaSlack ? top : m;
-            const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
-            m = mn;
-            l *= alpha;
-            if (!first) {
-              float o[16];
-#pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                tc::tmem_ld16(to + s * 128 + c, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= alpha;
-                tc::tmem_st16(to + s * 128 + c, o);
-                tc::tmem_st_wait();
-              }
-            }
-          }
-          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
-          const uint64_t scale2 = ta_pair(A.scale_log2, A.scale_log2), ref2 = ta_pair(-ref, -ref);
-          uint64_t sum[2] = {0, 0};
-          auto weigh = [&](auto hide) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              float x[32];
-              tc::tmem_ld32(ts + 32 * w, x);
-              uint32_t pk[16];
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                if (decltype(hide)::value) {
-                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
-                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
-                }
-                uint64_t y = ta_fma2(ta_pair(x[e], x[e + 1]), scale2, ref2);
-                if (!decltype(hide)::value && (e / 2) % 4 == 3) {
-                  y = ta_ex2_poly(y);
-                } else {
-                  float u, v;
-                  ta_unpair(y, u, v);
-                  y = ta_pair(ta_ex2(u), ta_ex2(v));
-                }
-                sum[(e / 2) & 1] = ta_add2(sum[(e / 2) & 1], y);
-                float u, v;
-                ta_unpair(y, u, v);
-                pk[e / 2] = TaType<T>::pack(u, v);
-              }
-              tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
-            }
-          };
-          if (masked)
-            weigh(std::true_type());
-          else
-            weigh(std::false_type());
-          float s0, s1, s2, s3;
-          ta_unpair(sum[0], s0, s1);
-          ta_unpair(sum[1], s2, s3);
-          l += (s0 + s1) + (s2 + s3);
-          tc::tmem_st_wait();
-        }
         if (tree) {
           // rows of V that a weight of 0 would not silence: past the keys they are cleared, and
           // non-finite values of a node are taken out here and given to its viewers at the end
@@ -742,9 +671,101 @@ __global__ void __launch_bounds__(TA_NT, 1)
           }
           tc::fence_proxy_async_smem();
         }
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bars[B_P + s]);
+        if (live) {
+          const bool masked = tree || gone;
+          // S is read twice, for the maximum and for the weights, which overwrite it as they come:
+          // a row of 128 does not stay in registers
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (masked) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              float x[32];
+              tc::tmem_ld32(ts + 32 * w, x);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (see[w] >> e) & 1 ? x[e] : -INFINITY);
+            }
+          } else {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              float x[64];
+              tc::tmem_ld64(ts + 64 * w, x);
+#pragma unroll
+              for (int e = 0; e < 64; e += 2) mx[(e / 2) & 3] = ta_max3(mx[(e / 2) & 3], x[e], x[e + 1]);
+            }
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+          const bool first = i < step;
+          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves
+            const float mn = first || top > m + kTaSlack ? top : m;
+            const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
+            m = mn;
+            l *= alpha;
+            if (!first) {
+              float o[16];
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                tc::tmem_ld16(to + s * 128 + c, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                tc::tmem_st16(to + s * 128 + c, o);
+                tc::tmem_st_wait();
+              }
+            }
+          }
+          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
+          const uint64_t scale2 = ta_pair(A.scale_log2, A.scale_log2), ref2 = ta_pair(-ref, -ref);
+          uint64_t sum[2] = {0, 0};
+          auto weigh = [&](auto hide, int w0) {
+#pragma unroll
+            for (int w = w0; w < w0 + 2; ++w) {
+              float x[32];
+              tc::tmem_ld32(ts + 32 * w, x);
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                if (decltype(hide)::value) {
+                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
+                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
+                }
+                uint64_t y = ta_fma2(ta_pair(x[e], x[e + 1]), scale2, ref2);
+                if (!decltype(hide)::value && (e / 2) % 4 == 3) {
+                  y = ta_ex2_poly(y);
+                } else {
+                  float u, v;
+                  ta_unpair(y, u, v);
+                  y = ta_pair(ta_ex2(u), ta_ex2(v));
+                }
+                sum[(e / 2) & 1] = ta_add2(sum[(e / 2) & 1], y);
+                float u, v;
+                ta_unpair(y, u, v);
+                pk[e / 2] = TaType<T>::pack(u, v);
+              }
+              tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
+            }
+          };
+          // the first half's products start beside the second half's weights
+#pragma unroll
+          for (int w0 = 0; w0 < 4; w0 += 2) {
+            if (masked)
+              weigh(std::true_type(), w0);
+            else
+              weigh(std::false_type(), w0);
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bars[B_P + w0 + s]);
+          }
+          float s0, s1, s2, s3;
+          ta_unpair(sum[0], s0, s1);
+          ta_unpair(sum[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
+        } else {
+          __syncwarp();
+          if (lane == 0) {
+            tc::mbar_arrive(&bars[B_P + s]);
+            tc::mbar_arrive(&bars[B_P + 2 + s]);
+          }
+        }
       }
       base += 2 * nt;
       // ---- the piece's output ---------------------------------------------------
