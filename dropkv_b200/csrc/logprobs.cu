@@ -1,77 +1,529 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of logits.
 // With y = (x - max x) log2(e) / tau, S = sum 2^y and A = sum 2^y y:
-// log p(t) = (x_t - max x) / tau - ln2 log2 S, H = ln2 (log2 S - A / S). The maximum is taken off
-// before the product, which would overflow for logits at the type's lowest value.
+// log p(t) = (x_t - max x) / tau - ln2 log2 S, H = ln2 (log2 S - A / S). The maximum is
+// taken off before the product, which would overflow for logits at the type's lowest value.
+//
+// The logits are read once: a thread keeps a maximum and both sums of its own, moved to a
+// new maximum chunk by chunk. The alternatives come along: a CTA keeps a list of candidates
+// and a threshold that at least top_k logits reach, and an ordinary chunk costs one barrier
+// that finds nothing above it. Few rows are split over the CTAs of a cluster, which join
+// through shared memory; there is no workspace and no atomic on global memory.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace dropkv {
 namespace {
 
-constexpr int LP_NT = 512;
+constexpr int LP_NT = 256;
 constexpr int LP_WARPS = LP_NT / 32;
+constexpr int LP_CTAS = 4;                      // CTAs an SM holds
+constexpr int LP_MAX_K = 64;
+constexpr int LP_MAX_E = 32;                    // logits of a thread and chunk, at most
+constexpr int LP_CAP = LP_MAX_K * (1 + LP_MAX_E);  // candidates: a full list and all of top_k threads
+constexpr int LP_MAX_S = 8;                     // CTAs of a cluster, at most
+constexpr int LP_GROUPS = 64;                   // groups of four threads
+static_assert(LP_GROUPS >= LP_MAX_K && LP_NT == 4 * LP_GROUPS, "the top_k-th of the groups' best");
 
-// Order of the alternatives: larger logits first (NaN above all), then lower index.
+// Order of the alternatives: larger logits first (NaN above all), then lower index. 0 is
+// below every logit's key.
 __device__ __forceinline__ uint64_t lp_key(float x, int i) {
   const uint32_t k = x != x ? 0xffffffffu : ordered_key(x);
   return ((uint64_t)k << 32) | (uint32_t)~i;
 }
+__device__ __forceinline__ float lp_value(uint64_t key) { return key_to_float((uint32_t)(key >> 32)); }
+
+__device__ __forceinline__ float lp_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lp_max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// What a thread, a CTA or a row knows: maximum, S and A against it.
+struct LpSums {
+  float m, s, t;
+};
+// Both sums moved to the maximum of two parts; an empty part has m = -inf and sums of 0.
+__device__ __forceinline__ void lp_move(LpSums& a, float m, float c) {
+  if (a.m == m) return;                 // (-inf too)
+  if (a.m != -INFINITY || a.s != 0.f) {  // a part of NaN alone has m = -inf as well: it stays NaN
+    const float d = (a.m - m) * c, f = lp_ex2(d);
+    a.t = f * fmaf(d == -INFINITY ? 0.f : d, a.s, a.t);
+    a.s *= f;
+  }
+  a.m = m;
+}
+__device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  lp_move(a, m, c);
+  lp_move(b, m, c);
+  return {m, a.s + b.s, a.t + b.t};
+}
+
+struct LpSmem {
+  uint64_t list[LP_CAP];
+  uint64_t lists[LP_MAX_S * LP_MAX_K];  // in a cluster's first CTA: every CTA's best
+  LpSums parts[LP_MAX_S];               // and sums
+  uint64_t tops[LP_NT];
+  uint32_t groups[LP_GROUPS];           // the best value of each group of threads, as an ordered key
+  uint32_t level;                       // the top_k-th of them
+  uint64_t edge;                        // the top_k-th best key of the threads
+  LpSums warps[LP_WARPS];
+  int count;
+};
+
+// The first n entries of `list` sorted, the best k of them kept: an entry's place is the
+// number of entries above it. A thread has one entry; a longer list goes through LP_NT entries
+// at a time, the best so far among them. All threads; returns the number kept.
+__device__ __forceinline__ int lp_keep_best(uint64_t* list, int n, int k) {
+  const int tid = threadIdx.x;
+  int done = min(n, LP_NT), m = done;  // entries seen, entries in the round
+  while (true) {
+    __syncthreads();
+    uint64_t mine = 0;
+    int rank = LP_CAP;
+    if (tid - (tid & 31) < m) {  // (warps without an entry have nothing to count)
+      if (tid < m) mine = list[tid];
+      rank = 0;
+      int e = 0;
+#pragma unroll 2
+      for (; e + 4 <= m; e += 4) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + e), y = *reinterpret_cast<const ulonglong2*>(list + e + 2);
+        rank += (x.x > mine) + (x.y > mine) + (y.x > mine) + (y.y > mine);
+      }
+      for (; e < m; ++e) rank += list[e] > mine;
+    }
+    __syncthreads();
+    if (tid < m && rank < k) list[rank] = mine;
+    m = min(m, k);
+    if (done >= n) break;
+    const int more = min(n - done, LP_NT - m);
+    uint64_t x = 0;
+    if (tid < more) x = list[done + tid];
+    __syncthreads();
+    if (tid < more) list[m + tid] = x;
+    done += more;
+    m += more;
+  }
+  __syncthreads();
+  return m;
+}
+
+// Two floats in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t lp_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void lp_unpair(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(LP_NT) logprobs_rows_kernel(Logprobs a) {
-  __shared__ float rf[LP_WARPS], rg[LP_WARPS];
-  __shared__ uint64_t rk[LP_WARPS];
+struct LpVec;  // 16 bytes of logits
+template <>
+struct LpVec<float> {
+  static constexpr int N = 4, U = 4;  // logits of a vector, vectors of a thread and chunk
+  static __device__ __forceinline__ void get(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+  }
+};
+template <>
+struct LpVec<__nv_bfloat16> {
+  static constexpr int N = 8, U = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+};
+template <>
+struct LpVec<__half> {
+  static constexpr int N = 8, U = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+};
+
+// The largest logit of a vector, NaN if one is.
+__device__ __forceinline__ float lp_top(const uint4& v, float) {
+  return lp_max_nan(lp_max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), lp_max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+__device__ __forceinline__ float lp_top(const uint4& v, __nv_bfloat16) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return lp_max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float lp_top(const uint4& v, __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+  const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return lp_max_nan(__low2float(m), __high2float(m));
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 lp_lowest();
+template <>
+__device__ __forceinline__ uint4 lp_lowest<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+template <>
+__device__ __forceinline__ uint4 lp_lowest<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+template <>
+__device__ __forceinline__ uint4 lp_lowest<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+
+// The alternatives found so far: at least top_k logits reach the threshold (0: none yet), and
+// every logit read that does is among the list's first `kept`.
+struct LpCandidates {
+  uint64_t floor_key;
+  int kept;
+};
+__device__ __forceinline__ float lp_floor_value(uint64_t key) {  // what a logit has to reach
+  return key ? lp_value(key) : __int_as_float(0xff800000);
+}
+
+// f(key) for each of a thread's logits in the chunk that reaches the threshold's value. A bit for
+// each of them first, then the few that are set, read again (they are in a cache).
+template <typename T, typename F>
+__device__ __forceinline__ void lp_look(uint64_t floor_key, const uint4* cur, const T* x0, int V, int v0, int v_end, float mx,
+                                        F f) {
+  constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
+  const float fv = lp_floor_value(floor_key);
+  if (!__any_sync(0xffffffffu, !(mx < fv))) return;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float x[N];
+    LpVec<T>::get(cur[u], x);
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits |= x[i] < fv ? 0u : 1u << (u * N + i);
+  }
+  for (; bits; bits &= bits - 1) {
+    const int q = __ffs(bits) - 1, v = v0 + (q / N) * LP_NT + (int)threadIdx.x;
+    const int64_t e = (int64_t)v * N + q % N;
+    if (v < v_end && e < V) f(lp_key(to_f(x0[e]), (int)e));
+  }
+  __syncwarp();
+}
+// Those that reach it go to the list, while there is room; all are counted.
+template <typename T>
+__device__ __forceinline__ void lp_collect(LpSmem& sm, uint64_t floor_key, const uint4* cur, const T* x0, int V, int v0,
+                                           int v_end, float mx) {
+  lp_look<T>(floor_key, cur, x0, V, v0, v_end, mx, [&](uint64_t key) {
+    if (key < floor_key) return;
+    const int at = atomicAdd(&sm.count, 1);
+    if (at < LP_CAP) sm.list[at] = key;
+  });
+}
+// The list of n entries cut to the best top_k, and the threshold moved up to the last of them.
+// All threads; ends without a barrier.
+__device__ __forceinline__ void lp_cut(LpSmem& sm, LpCandidates& cand, int n, int k) {
+  cand.kept = lp_keep_best(sm.list, n, k);
+  if (cand.kept == k && sm.list[k - 1] > cand.floor_key) cand.floor_key = sm.list[k - 1];
+  if (threadIdx.x == 0) sm.count = cand.kept;
+}
+
+// A chunk whose candidates may be many: the threshold is raised from the chunk itself first.
+template <typename T>
+__device__ __forceinline__ void lp_top_chunk(LpSmem& sm, LpCandidates& cand, const uint4* cur, const T* x0, int V, int v0,
+                                             int v_end, float mx, int k) {
+  const int tid = threadIdx.x;
+  // The k-th of the best of 64 groups of four threads is a threshold that k logits reach, and
+  // few more. A group's four threads count a quarter each of the groups above theirs. (Padding
+  // counts as -inf, which every logit reaches.)
+  uint32_t best = mx != mx ? 0xffffffffu : ordered_key(mx);
+  best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+  best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
+  if (tid % 4 == 0) sm.groups[tid / 4] = best;
+  __syncthreads();
+  int over = 0, same = 0;
+#pragma unroll
+  for (int q = 0; q < LP_GROUPS / 4; q += 4) {
+    const uint4 g = *reinterpret_cast<const uint4*>(&sm.groups[(tid % 4) * (LP_GROUPS / 4) + q]);
+    over += (g.x > best) + (g.y > best) + (g.z > best) + (g.w > best);
+    same += (g.x == best) + (g.y == best) + (g.z == best) + (g.w == best);
+  }
+  over += __shfl_xor_sync(0xffffffffu, over, 1);
+  over += __shfl_xor_sync(0xffffffffu, over, 2);
+  same += __shfl_xor_sync(0xffffffffu, same, 1);
+  same += __shfl_xor_sync(0xffffffffu, same, 2);
+  if (over < k && over + same >= k) sm.level = best;  // (all that write it have one value)
+  __syncthreads();
+  const uint64_t least = (uint64_t)sm.level << 32;  // the lowest key of that value
+  if (least > cand.floor_key) cand.floor_key = least;
+  lp_collect<T>(sm, cand.floor_key, cur, x0, V, v0, v_end, mx);
+  __syncthreads();
+  if (sm.count > LP_CAP) {
+    // Too many (logits in an order that defeats the groups). The exact k-th of the threads' best
+    // keys is a threshold that all but k threads stay below; with the list before this chunk cut
+    // to k, whatever they hold fits.
+    uint64_t top = 0;
+    lp_look<T>(cand.floor_key, cur, x0, V, v0, v_end, mx, [&](uint64_t key) { top = max(top, key); });
+    __syncthreads();
+    lp_cut(sm, cand, cand.kept, k);
+    sm.tops[tid] = top;
+    if (tid == 0) sm.edge = 0;
+    __syncthreads();
+    int r = 0;
+    for (int e = 0; e < LP_NT; ++e) r += sm.tops[e] > top;
+    if (r == k - 1 && top) sm.edge = top;
+    __syncthreads();
+    if (sm.edge > cand.floor_key) cand.floor_key = sm.edge;
+    lp_collect<T>(sm, cand.floor_key, cur, x0, V, v0, v_end, mx);
+    __syncthreads();
+  }
+  const int n = sm.count;
+  __syncthreads();
+  if (n > cand.kept) lp_cut(sm, cand, n, k);
+  __syncthreads();  // the list and its length are as the next chunk finds them
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, int vecs_per_cta) {
+  constexpr int N = LpVec<T>::N, U = LpVec<T>::U, E = N * U;
+  static_assert(E <= LP_MAX_E, "candidates of a thread");
+  extern __shared__ __align__(16) uint8_t raw[];
+  LpSmem& sm = *reinterpret_cast<LpSmem*>(raw);
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / split;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* x = static_cast<const T*>(a.logits) + blockIdx.x * a.row_stride;
-  float m = -INFINITY;
-  for (int i = tid; i < a.V; i += LP_NT) m = fmaxf(m, to_f(x[i]));
+  const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
+  // The row in vectors of 16 bytes from its first logit on, whatever its address: a thread's
+  // logits, and so the order of every sum, do not depend on it. Loads are aligned; where the
+  // row is not, a vector is put together from a thread's load and its neighbour's. What a
+  // load would cover outside the row is not read.
+  const int lead = (int)((reinterpret_cast<uintptr_t>(x0) % 16) / sizeof(T));  // elements of the first load before the row
+  const int vecs = (int)(((int64_t)a.V + N - 1) / N);
+  const int v_begin = part * vecs_per_cta, v_end = min(vecs, v_begin + vecs_per_cta);
+  const float c = a.scale_log2;
+  auto aligned = [&](int v) -> uint4 {
+    const int64_t e = (int64_t)v * N - lead;
+    if (e >= 0 && e + N <= a.V) return *reinterpret_cast<const uint4*>(x0 + e);
+    uint4 r = lp_lowest<T>();
+    T* p = reinterpret_cast<T*>(&r);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) rf[warp] = m;
-  __syncthreads();
-  for (int w = 0; w < LP_WARPS; ++w) m = fmaxf(m, rf[w]);
-  __syncthreads();
-  float s = 0.f, t = 0.f;
-  for (int i = tid; i < a.V; i += LP_NT) {
-    const float y = (to_f(x[i]) - m) * a.scale_log2, e = exp2f(y);  // NaN if the maximum is infinite
-    s += e;
-    t = fmaf(e, y < -1000.f ? 0.f : y, t);
-  }
+    for (int i = 0; i < N; ++i)
+      if (e + i >= 0 && e + i < a.V) p[i] = x0[e + i];
+    return r;
+  };
+  // a thread's loads of the chunk at v0; most chunks lie inside the row and the CTA's share
+  const int v_load = v_end + (lead != 0);  // loads end one later where vectors are put together
+  const int v_inner = min(v_load, (int)(((int64_t)a.V + lead) / N));
+  auto load = [&](int v0, uint4* x) {
+    if (v0 + U * LP_NT <= v_inner && (lead == 0 || v0 > 0)) {
+      const uint4* p = reinterpret_cast<const uint4*>(x0 - lead) + v0 + tid;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), t += __shfl_xor_sync(0xffffffffu, t, o);
-  if (lane == 0) rf[warp] = s, rg[warp] = t;
-  __syncthreads();
-  s = t = 0.f;
-  for (int w = 0; w < LP_WARPS; ++w) s += rf[w], t += rg[w];
-  const float ls = log2f(s), ln2 = 0.69314718055994531f;
-  auto logprob = [&](float v) { return fmaf(v - m, a.inv_temperature, -ln2 * ls); };
-  if (tid == 0) a.entropy[blockIdx.x] = ln2 * (ls - t / s);
-  for (int c = tid; c < a.C; c += LP_NT) {
-    const int64_t at = a.tokens[(int64_t)blockIdx.x * a.C + c];
-    a.logprob[(int64_t)blockIdx.x * a.C + c] = at >= 0 && at < a.V ? logprob(to_f(x[at])) : -INFINITY;
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top_k; ++k) {
-    uint64_t best = 0;
-    for (int i = tid; i < a.V; i += LP_NT) {
-      const uint64_t key = lp_key(to_f(x[i]), i);
-      if (key < last && key > best) best = key;
+      for (int u = 0; u < U; ++u) x[u] = p[u * LP_NT];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * LP_NT + tid;
+        x[u] = v < v_load ? aligned(v) : lp_lowest<T>();
+      }
     }
+  };
+  // vector v of the row from the aligned load of the same number and the next one (whole warps)
+  auto shifted = [&](const uint4& own, int v) -> uint4 {
+    uint4 give = own;
+    if (lane == 0) give = v + 32 <= v_end ? aligned(v + 32) : lp_lowest<T>();  // what lane 31 wants
+    const int from = (lane + 1) & 31;
+    uint32_t w[8] = {own.x, own.y, own.z, own.w, __shfl_sync(0xffffffffu, give.x, from), __shfl_sync(0xffffffffu, give.y, from),
+                     __shfl_sync(0xffffffffu, give.z, from), __shfl_sync(0xffffffffu, give.w, from)};
+    const int bytes = lead * (int)sizeof(T);
+    if (bytes & 8) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
     }
+    if (bytes & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int bits = 8 * (bytes & 3);
+    return v < v_end ? make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                                  __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits))
+                     : lp_lowest<T>();
+  };
+  LpSums own{-INFINITY, 0.f, 0.f};
+  LpCandidates cand{0, 0};
+  if (TOP && tid == 0) sm.count = 0;  // (the first chunk begins with a barrier)
+  uint4 next[U];
+  load(v_begin, next);
+  int chunk = 0;
+  for (int v0 = v_begin; v0 < v_end; v0 += U * LP_NT, ++chunk) {
+    uint4 cur[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) cur[u] = next[u];
+    load(v0 + U * LP_NT, next);
+    if (lead) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) cur[u] = shifted(cur[u], v0 + u * LP_NT + tid);
+    }
+    float mx = lp_top(cur[0], T());
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = lp_max_nan(mx, lp_top(cur[u], T()));
+    if (mx > own.m) lp_move(own, mx, c);
+    const float m = own.m == -INFINITY ? 0.f : own.m;
+    const uint64_t less2 = lp_pair(-m, -m), c2 = lp_pair(c, c);
+    uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[N];
+      LpVec<T>::get(cur[u], x);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        uint64_t y2 = lp_mul2(lp_add2(lp_pair(x[i], x[i + 1]), less2), c2);
+        float y0, y1;
+        lp_unpair(y2, y0, y1);
+        const uint64_t e2 = lp_pair(lp_ex2(y0), lp_ex2(y1));
+        s2 = lp_add2(s2, e2);
+        t2 = lp_fma2(e2, lp_pair(fmaxf(y0, -4096.f), fmaxf(y1, -4096.f)), t2);  // 2^-inf is 0, and 0 its share
+      }
+    }
+    float s0, s1, t0, t1;
+    lp_unpair(s2, s0, s1);
+    lp_unpair(t2, t0, t1);
+    own.s += s0 + s1;
+    own.t += t0 + t1;
+    if (TOP) {
+      if (chunk == 0) {
+        lp_top_chunk<T>(sm, cand, cur, x0, a.V, v0, v_end, mx, a.top_k);
+      } else {
+        // no barrier in an ordinary chunk: warps add what reaches the threshold, and now and
+        // then (after 2, 4, 8, ... chunks) the list is cut and the threshold moves up to it
+        lp_collect<T>(sm, cand.floor_key, cur, x0, a.V, v0, v_end, mx);
+        if ((chunk & (chunk + 1)) == 0) {
+          __syncthreads();
+          const int n = sm.count;
+          if (n > cand.kept && n <= LP_CAP) lp_cut(sm, cand, n, a.top_k);
+          __syncthreads();
+        }
+      }
+    }
+  }
+  if (TOP) {
     __syncthreads();
-    if (lane == 0) rk[warp] = best;
-    __syncthreads();
-    for (int w = 0; w < LP_WARPS; ++w) best = rk[w] > best ? rk[w] : best;
-    last = best;
-    if (tid == 0) {
-      const int i = (int)~(uint32_t)best;
-      a.top_tokens[(int64_t)blockIdx.x * a.top_k + k] = i;
-      a.top_logprobs[(int64_t)blockIdx.x * a.top_k + k] = logprob(to_f(x[i]));
+    cand.kept = sm.count;
+    if (sm.count > LP_CAP) {
+      // More candidates than the list holds (logits that rise along the row, say): once more over
+      // the CTA's share for the alternatives alone, with a threshold of its own for every chunk
+      __syncthreads();
+      cand = LpCandidates{0, 0};
+      if (tid == 0) sm.count = 0;
+      __syncthreads();
+      for (int v0 = v_begin; v0 < v_end; v0 += U * LP_NT) {
+        uint4 cur[U];
+        load(v0, cur);
+        if (lead) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) cur[u] = shifted(cur[u], v0 + u * LP_NT + tid);
+        }
+        float mx = lp_top(cur[0], T());
+#pragma unroll
+        for (int u = 1; u < U; ++u) mx = lp_max_nan(mx, lp_top(cur[u], T()));
+        lp_top_chunk<T>(sm, cand, cur, x0, a.V, v0, v_end, mx, a.top_k);
+      }
     }
   }
+  // ---- the CTA's sums and best, then the row's ------------------------------------
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    LpSums b;
+    b.m = __shfl_xor_sync(0xffffffffu, own.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, own.s, o);
+    b.t = __shfl_xor_sync(0xffffffffu, own.t, o);
+    own = lp_join(own, b, c);
+  }
+  if (lane == 0) sm.warps[warp] = own;
+  __syncthreads();
+  own = sm.warps[0];
+#pragma unroll
+  for (int w = 1; w < LP_WARPS; ++w) own = lp_join(own, sm.warps[w], c);
+  if (TOP) cand.kept = lp_keep_best(sm.list, cand.kept, a.top_k);
+  if (split > 1) {
+    LpSmem* first = cluster.map_shared_rank(&sm, 0);
+    if (tid == 0) first->parts[part] = own;
+    if (TOP)
+      for (int i = tid; i < a.top_k; i += LP_NT) first->lists[part * a.top_k + i] = i < cand.kept ? sm.list[i] : 0;
+    cluster.sync();
+    if (part != 0) return;
+    own = sm.parts[0];
+    for (int p = 1; p < split; ++p) own = lp_join(own, sm.parts[p], c);
+    if (TOP) {
+      for (int i = tid; i < split * a.top_k; i += LP_NT) sm.list[i] = sm.lists[i];
+      lp_keep_best(sm.list, split * a.top_k, a.top_k);
+    }
+  }
+  const float ls = log2f(own.s), ln2 = 0.69314718055994531f;
+  auto logprob = [&](float v) { return fmaf(v - own.m, a.inv_temperature, -ln2 * ls); };
+  if (tid == 0) a.entropy[row] = ln2 * (ls - own.t / own.s);
+  for (int i = tid; i < a.C; i += LP_NT) {
+    const int64_t at = a.tokens[row * a.C + i];
+    a.logprob[row * a.C + i] = at >= 0 && at < a.V ? logprob(to_f(x0[at])) : -INFINITY;
+  }
+  if (TOP && tid < a.top_k) {
+    const uint64_t key = sm.list[tid];
+    a.top_tokens[row * a.top_k + tid] = (int)~(uint32_t)key;
+    a.top_logprobs[row * a.top_k + tid] = logprob(lp_value(key));
+  }
+}
+
+template <typename T, bool TOP>
+int lp_launch(const Logprobs& a, cudaStream_t st) {
+  // CTAs a row: as many as leave the last wave fullest, the fewest among equals; a CTA takes
+  // one chunk at least
+  constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
+  const int64_t vecs = ((int64_t)a.V + N - 1) / N;
+  const int64_t slots = (int64_t)LP_CTAS * num_sms_current_device();
+  int split = 1;
+  double best = 1e30;
+  for (int s = 1; s <= LP_MAX_S; s *= 2) {
+    if (s > 1 && (vecs + s - 1) / s < U * LP_NT) break;
+    const double waves = (double)((a.N * s + slots - 1) / slots) / s;
+    if (waves < 0.97 * best) best = waves, split = s;
+  }
+  const int per = (int)((vecs + split - 1) / split);
+  if (a.N * split > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  auto kern = logprobs_kernel<T, TOP>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(a.N * split));
+  cfg.blockDim = dim3(LP_NT);
+  cfg.dynamicSmemBytes = sizeof(LpSmem);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, per);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
+  return check_launch("token_logprobs");
 }
 
 }  // namespace
@@ -84,12 +536,9 @@ size_t token_logprobs_workspace_size(int64_t N, int V, int top_k) {
 int launch_token_logprobs(const Logprobs& a, int dtype, void* ws, cudaStream_t st) {
   (void)ws;
   if (dtype == DROPKV_DTYPE_BF16)
-    logprobs_rows_kernel<__nv_bfloat16><<<(int)a.N, LP_NT, 0, st>>>(a);
-  else if (dtype == DROPKV_DTYPE_F16)
-    logprobs_rows_kernel<__half><<<(int)a.N, LP_NT, 0, st>>>(a);
-  else
-    logprobs_rows_kernel<float><<<(int)a.N, LP_NT, 0, st>>>(a);
-  return check_launch("token_logprobs");
+    return a.top_k ? lp_launch<__nv_bfloat16, true>(a, st) : lp_launch<__nv_bfloat16, false>(a, st);
+  if (dtype == DROPKV_DTYPE_F16) return a.top_k ? lp_launch<__half, true>(a, st) : lp_launch<__half, false>(a, st);
+  return a.top_k ? lp_launch<float, true>(a, st) : lp_launch<float, false>(a, st);
 }
 
 }  // namespace dropkv
