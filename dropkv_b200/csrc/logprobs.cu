@@ -187,6 +187,42 @@ __device__ __forceinline__ float lp_top(const uint4& v, __half) {
   return lp_max_nan(__low2float(m), __high2float(m));
 }
 
+// A bit for each logit of U vectors that is not below x (x is a logit's value: it converts
+// exactly), and the logit a bit stands for. 16-bit types: even logits have the low half.
+template <int U>
+__device__ __forceinline__ uint32_t lp_reach(const uint4* v, float x, float) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= __uint_as_float(w[i]) < x ? 0u : 1u << (4 * u + i);
+  }
+  return bits;
+}
+template <int U, typename T2>
+__device__ __forceinline__ uint32_t lp_reach2(const uint4* v, T2 x) {
+  uint32_t below = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) below |= __hlt2_mask(reinterpret_cast<const T2&>(w[i]), x) & (0x00010001u << (4 * u + i));
+  }
+  return ~below;
+}
+template <int U>
+__device__ __forceinline__ uint32_t lp_reach(const uint4* v, float x, __nv_bfloat16) {
+  return lp_reach2<U>(v, __float2bfloat162_rn(x));
+}
+template <int U>
+__device__ __forceinline__ uint32_t lp_reach(const uint4* v, float x, __half) {
+  return lp_reach2<U>(v, __float2half2_rn(x));
+}
+__device__ __forceinline__ int lp_place(int bit, float) { return bit; }
+__device__ __forceinline__ int lp_place(int bit, __nv_bfloat16) { return 2 * (bit & 15) + (bit >> 4); }
+__device__ __forceinline__ int lp_place(int bit, __half) { return 2 * (bit & 15) + (bit >> 4); }
+
 template <typename T>
 __device__ __forceinline__ uint4 lp_lowest();
 template <>
@@ -214,16 +250,8 @@ __device__ __forceinline__ void lp_look(uint64_t floor_key, const uint4* cur, co
   constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
   const float fv = lp_floor_value(floor_key);
   if (!__any_sync(0xffffffffu, !(mx < fv))) return;
-  uint32_t bits = 0;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float x[N];
-    LpVec<T>::get(cur[u], x);
-#pragma unroll
-    for (int i = 0; i < N; ++i) bits |= x[i] < fv ? 0u : 1u << (u * N + i);
-  }
-  for (; bits; bits &= bits - 1) {
-    const int q = __ffs(bits) - 1, v = v0 + (q / N) * LP_NT + (int)threadIdx.x;
+  for (uint32_t bits = lp_reach<U>(cur, fv, T()); bits; bits &= bits - 1) {
+    const int q = lp_place(__ffs(bits) - 1, T()), v = v0 + (q / N) * LP_NT + (int)threadIdx.x;
     const int64_t e = (int64_t)v * N + q % N;
     if (v < v_end && e < V) f(lp_key(to_f(x0[e]), (int)e));
   }
@@ -494,17 +522,19 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
 
 template <typename T, bool TOP>
 int lp_launch(const Logprobs& a, cudaStream_t st) {
-  // CTAs a row: as many as leave the last wave fullest, the fewest among equals; a CTA takes
-  // one chunk at least
+  // CTAs a row, by the waves of CTAs and what one costs: its chunks, and what its start and end
+  // take, about 8 chunks with alternatives and 2 without (2048 x 151936 bf16, top 20: 234 us in
+  // halves, PROMPT1 whole; 16 x 50257 fp16, top 5: STEP1 us whole, 10 in quarters). A CTA takes one chunk at least.
   constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
   const int64_t vecs = ((int64_t)a.V + N - 1) / N;
   const int64_t slots = (int64_t)LP_CTAS * num_sms_current_device();
   int split = 1;
   double best = 1e30;
   for (int s = 1; s <= LP_MAX_S; s *= 2) {
-    if (s > 1 && (vecs + s - 1) / s < U * LP_NT) break;
-    const double waves = (double)((a.N * s + slots - 1) / slots) / s;
-    if (waves < 0.97 * best) best = waves, split = s;
+    const int64_t share = (vecs + s - 1) / s;
+    if (s > 1 && share < U * LP_NT) break;
+    const double cost = (double)((a.N * s + slots - 1) / slots) * ((double)share / (U * LP_NT) + (TOP ? 8 : 2));
+    if (cost < best) best = cost, split = s;
   }
   const int per = (int)((vecs + split - 1) / split);
   if (a.N * split > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "token_logprobs: too many rows");
