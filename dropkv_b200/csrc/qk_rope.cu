@@ -2,6 +2,8 @@
 // write in one pass: y = x * rsqrt(mean(x^2) + eps) * w over a head of D, then for
 // each of the R / 2 pairs (a, b) of the head's first R elements
 // (a c - b s, b c + a s) with c, s = cos, sin[position][pair].
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace dropkv {
@@ -18,7 +20,7 @@ __device__ __forceinline__ __half qr_from<__half>(float x) { return __float2half
 template <>
 __device__ __forceinline__ __nv_bfloat16 qr_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One warp per row (b, l, head): heads [0, Hq) of Q, [Hq, Hq + Hkv) of K, then V.
+// Rows of any size, alignment and stride: one warp per row (b, l, head): heads [0, Hq) of Q, [Hq, Hq + Hkv) of K, then V.
 template <typename T>
 __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
   const int lane = threadIdx.x & 31;
@@ -78,19 +80,210 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
   }
 }
 
+// The same with 16-byte vectors: G lanes have a row, each one unit of two vectors -- the
+// vectors whose elements rotate together (elements i and i + R / 2; interleaved pairs lie
+// within a vector), or two that do not turn. A CTA has one token and all of its rows, or with
+// few tokens some of them: a lane's cosines and sines, which weigh more than a row (64 bytes
+// of table against 32 of Q), are fetched once and stay in registers, and QR_BATCH rows are on
+// their way at a time.
+constexpr int QR_BATCH = 3;
+
+template <typename T>
+struct QrVec {
+  static constexpr int N = 16 / sizeof(T);
+  static __device__ __forceinline__ void get(const uint4& v, float* x) {
+    const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f(p[i]);
+  }
+  static __device__ __forceinline__ uint4 put(const float* x) {
+    uint4 v;
+    T* p = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = qr_from<T>(x[i]);
+    return v;
+  }
+};
+
+template <typename T, int G, bool INTERLEAVED>
+__global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a) {
+  constexpr int N = QrVec<T>::N, GROUPS = QR_NT / G;
+  const int64_t bl = blockIdx.x;
+  const int b = (int)(bl / a.L), l = (int)(bl % a.L);
+  const int u = threadIdx.x % G, group = threadIdx.x / G;
+  const int heads = a.Hq + a.Hkv + (a.slots ? a.Hkv : 0);
+  const int h0 = blockIdx.y * GROUPS + group, step = gridDim.y * GROUPS;
+  // this lane's elements: [lo, lo + N) and [hi, hi + N)
+  const int turning = a.R / (2 * N);  // units that turn
+  const bool turns = u < turning;
+  int lo, hi;
+  if (INTERLEAVED) {
+    lo = 2 * N * u;
+    hi = lo + N;
+  } else {
+    lo = turns ? N * u : a.R + 2 * N * (u - turning);
+    hi = turns ? lo + a.R / 2 : lo + N;
+  }
+  auto row_of = [&](int h) -> const T* {
+    if (h < a.Hq) return static_cast<const T*>(a.q) + b * a.q_sb + h * a.q_sh + l * a.q_sl;
+    if (h < a.Hq + a.Hkv) return static_cast<const T*>(a.k) + b * a.k_sb + (h - a.Hq) * a.k_sh + l * a.k_sl;
+    return static_cast<const T*>(a.v) + b * a.v_sb + (h - a.Hq - a.Hkv) * a.v_sh + l * a.v_sl;
+  };
+  const int64_t pos = a.positions[b * a.pos_sb + l];
+  int64_t slot = -1;
+  if (a.slots) slot = a.slots[bl];
+  uint4 va[QR_BATCH], vb[QR_BATCH];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < QR_BATCH; ++i) {
+      const int hi_ = h + i * step;
+      if (hi_ < heads) {
+        const T* x = row_of(hi_);
+        va[i] = *reinterpret_cast<const uint4*>(x + lo);
+        vb[i] = *reinterpret_cast<const uint4*>(x + hi);
+      }
+    }
+  };
+  load(h0);
+  // cosines and sines of the lane's N pairs (interleaved: N / 2 of each vector)
+  const bool known = pos >= 0 && pos < a.P;  // a position outside the tables gives NaN
+  float cs[N], sn[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) cs[i] = turns ? NAN : 1.f, sn[i] = turns ? NAN : 0.f;
+  if (turns && known) {
+    const float* c = a.cos + pos * (a.R / 2) + N * u;
+    const float* s = a.sin + pos * (a.R / 2) + N * u;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(c + i), y = *reinterpret_cast<const float4*>(s + i);
+      cs[i] = x.x, cs[i + 1] = x.y, cs[i + 2] = x.z, cs[i + 3] = x.w;
+      sn[i] = y.x, sn[i + 1] = y.y, sn[i + 2] = y.z, sn[i + 3] = y.w;
+    }
+  }
+  T* kp = nullptr;
+  T* vp = nullptr;
+  if (slot >= 0 && slot < (int64_t)a.n_pages * a.block) {
+    const int64_t page = slot / a.block, at = slot - page * a.block;
+    kp = static_cast<T*>(a.k_pages) + page * a.kp_sb + at * a.kp_st;
+    vp = static_cast<T*>(a.v_pages) + page * a.vp_sb + at * a.vp_st;
+  }
+  for (int h = h0; h - group < heads; h += QR_BATCH * step) {  // (all lanes of a warp stay)
+    if (h != h0) load(h);
+#pragma unroll
+    for (int i = 0; i < QR_BATCH; ++i) {
+      const int hh = h + i * step;
+      const bool there = hh < heads, is_q = hh < a.Hq, is_v = hh >= a.Hq + a.Hkv;
+      const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
+      float x[N], y[N];
+      QrVec<T>::get(va[i], x);
+      QrVec<T>::get(vb[i], y);
+      if (a.q_weight || a.k_weight) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (there && !is_v && w) {
+          const float inv = rsqrtf(ss / a.D + a.eps);
+          float wx[N], wy[N];
+          QrVec<T>::get(*reinterpret_cast<const uint4*>(w + lo), wx);
+          QrVec<T>::get(*reinterpret_cast<const uint4*>(w + hi), wy);
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[e] = x[e] * inv * wx[e], y[e] = y[e] * inv * wy[e];
+        }
+      }
+      if (!there) continue;
+      if (is_v) {
+        if (vp) {
+          T* dst = vp + (hh - a.Hq - a.Hkv) * a.vp_sh;
+          *reinterpret_cast<uint4*>(dst + lo) = va[i];
+          *reinterpret_cast<uint4*>(dst + hi) = vb[i];
+        }
+        continue;
+      }
+      if (INTERLEAVED) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const float p = x[e], q = x[e + 1], r = y[e], s = y[e + 1];
+          x[e] = p * cs[e / 2] - q * sn[e / 2];
+          x[e + 1] = q * cs[e / 2] + p * sn[e / 2];
+          y[e] = r * cs[(N + e) / 2] - s * sn[(N + e) / 2];
+          y[e + 1] = s * cs[(N + e) / 2] + r * sn[(N + e) / 2];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float p = x[e], q = y[e];
+          x[e] = p * cs[e] - q * sn[e];
+          y[e] = q * cs[e] + p * sn[e];
+        }
+      }
+      const uint4 ox = QrVec<T>::put(x), oy = QrVec<T>::put(y);
+      T* out = is_q ? static_cast<T*>(a.q_out) + ((b * (int64_t)a.Hq + hh) * a.L + l) * a.D
+                    : static_cast<T*>(a.k_out) + ((b * (int64_t)a.Hkv + hh - a.Hq) * a.L + l) * a.D;
+      *reinterpret_cast<uint4*>(out + lo) = ox;
+      *reinterpret_cast<uint4*>(out + hi) = oy;
+      if (!is_q && kp) {
+        T* dst = kp + (hh - a.Hq) * a.kp_sh;
+        *reinterpret_cast<uint4*>(dst + lo) = ox;
+        *reinterpret_cast<uint4*>(dst + hi) = oy;
+      }
+    }
+  }
+}
+
+template <typename T>
+int qr_launch(const QkRope& a, cudaStream_t st) {
+  constexpr int N = QrVec<T>::N;
+  const int64_t eb = sizeof(T);
+  const int heads = a.Hq + a.Hkv + (a.slots ? a.Hkv : 0);
+  // vectors: every row, table row and page row on 16-byte boundaries, a power of two of lanes
+  // a row, whole units that turn
+  uint64_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.q_out) |
+                  reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.q_weight) |
+                  reinterpret_cast<uintptr_t>(a.k_weight) |
+                  (uint64_t)((a.q_sb | a.q_sh | a.q_sl | a.k_sb | a.k_sh | a.k_sl) * eb) | (uint64_t)(a.D * eb);
+  if (a.R) bits |= reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin) | (uint64_t)(a.R / 2 * 4);
+  if (a.slots)
+    bits |= reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages) |
+            (uint64_t)((a.v_sb | a.v_sh | a.v_sl | a.kp_sb | a.kp_sh | a.kp_st | a.vp_sb | a.vp_sh | a.vp_st) * eb);
+  const int G = a.D % (2 * N) == 0 ? a.D / (2 * N) : 0;
+  const bool lanes = G == 2 || G == 4 || G == 8 || G == 16 || G == 32;
+  const int64_t tokens = (int64_t)a.B * a.L;
+  if (bits % 16 == 0 && lanes && a.R % (2 * N) == 0 && tokens <= 0x7fffffff) {
+    // one CTA a token when they fill the device; fewer tokens: a CTA for every group's first row
+    const int groups = QR_NT / G;
+    const int most = (heads + groups - 1) / groups;
+    const int ys = tokens >= 2 * (int64_t)num_sms_current_device() ? 1 : (most < 65535 ? most : 65535);
+    const dim3 grid((unsigned)tokens, ys);
+    auto run = [&](auto g) {
+      constexpr int GG = decltype(g)::value;
+      if (a.interleaved)
+        qk_rope_vec_kernel<T, GG, true><<<grid, QR_NT, 0, st>>>(a);
+      else
+        qk_rope_vec_kernel<T, GG, false><<<grid, QR_NT, 0, st>>>(a);
+    };
+    switch (G) {
+      case 2: run(std::integral_constant<int, 2>()); break;
+      case 4: run(std::integral_constant<int, 4>()); break;
+      case 8: run(std::integral_constant<int, 8>()); break;
+      case 16: run(std::integral_constant<int, 16>()); break;
+      default: run(std::integral_constant<int, 32>()); break;
+    }
+    return check_launch("qk_norm_rope");
+  }
+  const int64_t grid = (tokens * heads + QR_NT / 32 - 1) / (QR_NT / 32);
+  if (grid > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "qk_norm_rope: too many rows");
+  qk_rope_rows_kernel<T><<<(int)grid, QR_NT, 0, st>>>(a);
+  return check_launch("qk_norm_rope");
+}
+
 }  // namespace
 
 int launch_qk_norm_rope(const QkRope& a, int dtype, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.L * (a.Hq + a.Hkv + (a.slots ? a.Hkv : 0));
-  const int64_t grid = (rows + QR_NT / 32 - 1) / (QR_NT / 32);
-  if (grid > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "qk_norm_rope: too many rows");
-  if (dtype == DROPKV_DTYPE_BF16)
-    qk_rope_rows_kernel<__nv_bfloat16><<<(int)grid, QR_NT, 0, st>>>(a);
-  else if (dtype == DROPKV_DTYPE_F16)
-    qk_rope_rows_kernel<__half><<<(int)grid, QR_NT, 0, st>>>(a);
-  else
-    qk_rope_rows_kernel<float><<<(int)grid, QR_NT, 0, st>>>(a);
-  return check_launch("qk_norm_rope");
+  if (dtype == DROPKV_DTYPE_BF16) return qr_launch<__nv_bfloat16>(a, st);
+  if (dtype == DROPKV_DTYPE_F16) return qr_launch<__half>(a, st);
+  return qr_launch<float>(a, st);
 }
 
 }  // namespace dropkv
