@@ -7,7 +7,8 @@ namespace dropkv {
 namespace {
 
 constexpr int BT_NT = 256;
-constexpr int BT_TOKENS = 8 * BT_NT;  // slots of one CTA
+constexpr int BT_EACH = 8;                  // slots of a thread
+constexpr int BT_TOKENS = BT_EACH * BT_NT;  // slots of a CTA
 
 struct BtArgs {
   const int32_t* lens;
@@ -66,15 +67,19 @@ __global__ void __launch_bounds__(BT_NT) block_tables_kernel(BtArgs a) {
     }
   }
   const int len = bt_len(a, b), nn = a.new_lens ? min(max(a.new_lens[b], 0), len) : len;
-  const int64_t i0 = (int64_t)blockIdx.y * BT_TOKENS;
+  const int64_t i0 = (int64_t)blockIdx.y * BT_TOKENS + tid;
   int64_t* out = a.slots + (int64_t)b * a.max_new;
-  for (int64_t i = i0 + tid; i < a.max_new && i < i0 + BT_TOKENS; i += BT_NT) {
+  const unsigned block = (unsigned)a.block;
+#pragma unroll 2
+  for (int e = 0; e < BT_EACH; ++e) {
+    const int64_t i = i0 + e * BT_NT;
+    if (i >= a.max_new) break;
     int64_t slot = -1;
     if (i < nn) {
-      const int t = len - nn + (int)i, col = t / a.block;
-      if (col < a.max_blocks) {
-        const int p = page(col);
-        if (p >= 0) slot = (int64_t)p * a.block + (t - col * a.block);
+      const unsigned t = (unsigned)(len - nn) + (unsigned)i, col = t / block;
+      if (col < (unsigned)a.max_blocks) {
+        const int p = page((int)col);
+        if (p >= 0) slot = (int64_t)p * a.block + (t - col * block);
       }
     }
     out[i] = slot;
@@ -95,6 +100,47 @@ struct SrArgs {
   int B, H, N, block, vecs;  // vecs: vectors of a row
 };
 
+// Rows of LANES 16-byte vectors: LANES threads have a row, SR_ROWS rows each, whose slots,
+// then K and V vectors, are on their way at once. Rows follow one another along a head, so
+// reads are one stream and writes come in runs of a page's rows.
+constexpr int SR_ROWS = 4;
+
+template <int LANES>
+__global__ void __launch_bounds__(SR_NT) store_rows_vec_kernel(SrArgs a) {
+  constexpr int RPB = SR_NT / LANES;
+  const unsigned rows = (unsigned)a.B * a.H * a.N;
+  const unsigned r0 = blockIdx.x * (RPB * SR_ROWS) + threadIdx.x / LANES;
+  const int c = threadIdx.x % LANES * 16;
+  int64_t slot[SR_ROWS];
+  int b[SR_ROWS], h[SR_ROWS], n[SR_ROWS];
+#pragma unroll
+  for (int i = 0; i < SR_ROWS; ++i) {
+    const unsigned r = r0 + i * RPB, bh = r / (unsigned)a.N;
+    n[i] = (int)(r - bh * a.N);
+    b[i] = (int)(bh / (unsigned)a.H);
+    h[i] = (int)(bh - (unsigned)b[i] * a.H);
+    slot[i] = r < rows ? a.slots[(int64_t)b[i] * a.N + n[i]] : -1;
+  }
+  uint4 k[SR_ROWS], v[SR_ROWS];
+#pragma unroll
+  for (int i = 0; i < SR_ROWS; ++i) {
+    if (slot[i] >= a.n_slots) slot[i] = -1;
+    if (slot[i] >= 0) {
+      k[i] = __ldcs(reinterpret_cast<const uint4*>(a.k + b[i] * a.k_sb + h[i] * a.k_sh + n[i] * a.k_sn + c));
+      v[i] = __ldcs(reinterpret_cast<const uint4*>(a.v + b[i] * a.v_sb + h[i] * a.v_sh + n[i] * a.v_sn + c));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < SR_ROWS; ++i) {
+    if (slot[i] < 0) continue;
+    const int64_t page = slot[i] >> 32 ? slot[i] / a.block : (int64_t)((uint32_t)slot[i] / (uint32_t)a.block);
+    const int64_t at = slot[i] - page * a.block;
+    *reinterpret_cast<uint4*>(a.kp + page * a.kp_sb + h[i] * a.kp_sh + at * a.kp_st + c) = k[i];
+    *reinterpret_cast<uint4*>(a.vp + page * a.vp_sb + h[i] * a.vp_sh + at * a.vp_st + c) = v[i];
+  }
+}
+
+// Rows of any size, alignment and number.
 template <typename T>
 __global__ void __launch_bounds__(SR_NT) store_rows_kernel(SrArgs a) {
   const int64_t total = (int64_t)a.B * a.H * a.N * a.vecs;
@@ -153,6 +199,19 @@ int launch_store_rows(const StoreRows& s, cudaStream_t st) {
   const int64_t total = (int64_t)s.B * s.H * s.N * a.vecs;
   const int64_t want = (total + SR_NT - 1) / SR_NT, most = 32 * (int64_t)num_sms_current_device();
   const int grid = (int)(want < most ? want : most);
+  const int64_t rows = (int64_t)s.B * s.H * s.N;
+  if (w == 16 && rows < 0x7fffffff - SR_NT * SR_ROWS && (a.vecs == 4 || a.vecs == 8 || a.vecs == 16 || a.vecs == 32)) {
+    const int per = SR_NT / a.vecs * SR_ROWS, ctas = (int)((rows + per - 1) / per);
+    if (a.vecs == 4)
+      store_rows_vec_kernel<4><<<ctas, SR_NT, 0, st>>>(a);
+    else if (a.vecs == 8)
+      store_rows_vec_kernel<8><<<ctas, SR_NT, 0, st>>>(a);
+    else if (a.vecs == 16)
+      store_rows_vec_kernel<16><<<ctas, SR_NT, 0, st>>>(a);
+    else
+      store_rows_vec_kernel<32><<<ctas, SR_NT, 0, st>>>(a);
+    return check_launch("store_rows");
+  }
   if (w == 16)
     store_rows_kernel<uint4><<<grid, SR_NT, 0, st>>>(a);
   else if (w == 4)

@@ -82,10 +82,9 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
 
 // The same with 16-byte vectors: G lanes have a row, each one unit of two vectors -- the
 // vectors whose elements rotate together (elements i and i + R / 2; interleaved pairs lie
-// within a vector), or two that do not turn. A CTA has one token and all of its rows, or with
-// few tokens some of them: a lane's cosines and sines, which weigh more than a row (64 bytes
-// of table against 32 of Q), are fetched once and stay in registers, and QR_BATCH rows are on
-// their way at a time.
+// within a vector), or two that do not turn. A group of G lanes takes every hpg-th row of one
+// token: a lane's cosines and sines, which weigh more than a row (64 bytes of table against 32
+// of Q), are fetched once and stay in registers, and QR_BATCH rows are on their way at a time.
 constexpr int QR_BATCH = 3;
 
 template <typename T>
@@ -106,13 +105,15 @@ struct QrVec {
 };
 
 template <typename T, int G, bool INTERLEAVED>
-__global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a) {
+__global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens, int hpg) {
   constexpr int N = QrVec<T>::N, GROUPS = QR_NT / G;
-  const int64_t bl = blockIdx.x;
-  const int b = (int)(bl / a.L), l = (int)(bl % a.L);
-  const int u = threadIdx.x % G, group = threadIdx.x / G;
   const int heads = a.Hq + a.Hkv + (a.slots ? a.Hkv : 0);
-  const int h0 = blockIdx.y * GROUPS + group, step = gridDim.y * GROUPS;
+  const int64_t gid = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+  const bool idle = gid >= (int64_t)tokens * hpg;  // (shuffles want the whole warp)
+  const unsigned bl = idle ? 0u : (unsigned)(gid / (unsigned)hpg);
+  const int b = (int)(bl / (unsigned)a.L), l = (int)(bl - (unsigned)b * (unsigned)a.L);
+  const int u = threadIdx.x % G, step = hpg;
+  const int h0 = idle ? heads : (int)(gid - (int64_t)bl * hpg);
   // this lane's elements: [lo, lo + N) and [hi, hi + N)
   const int turning = a.R / (2 * N);  // units that turn
   const bool turns = u < turning;
@@ -163,17 +164,19 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a) {
   T* kp = nullptr;
   T* vp = nullptr;
   if (slot >= 0 && slot < (int64_t)a.n_pages * a.block) {
-    const int64_t page = slot / a.block, at = slot - page * a.block;
+    const int64_t page = slot >> 32 ? slot / a.block : (int64_t)((uint32_t)slot / (uint32_t)a.block);
+    const int64_t at = slot - page * a.block;
     kp = static_cast<T*>(a.k_pages) + page * a.kp_sb + at * a.kp_st;
     vp = static_cast<T*>(a.v_pages) + page * a.vp_sb + at * a.vp_st;
   }
-  for (int h = h0; h - group < heads; h += QR_BATCH * step) {  // (all lanes of a warp stay)
-    if (h != h0) load(h);
+  const int rounds = (heads + QR_BATCH * step - 1) / (QR_BATCH * step);
+  for (int r = 0; r < rounds; ++r) {
+    const int h = h0 + r * QR_BATCH * step;
+    if (r) load(h);
 #pragma unroll
     for (int i = 0; i < QR_BATCH; ++i) {
       const int hh = h + i * step;
       const bool there = hh < heads, is_q = hh < a.Hq, is_v = hh >= a.Hq + a.Hkv;
-      const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
       float x[N], y[N];
       QrVec<T>::get(va[i], x);
       QrVec<T>::get(vb[i], y);
@@ -183,9 +186,10 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a) {
         for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
         if (there && !is_v && w) {
           const float inv = rsqrtf(ss / a.D + a.eps);
-          float wx[N], wy[N];
+          float wx[N], wy[N];  // (from L1: held in registers they cost occupancy, 24 -> 33 us)
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + lo), wx);
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + hi), wy);
 #pragma unroll
@@ -251,17 +255,19 @@ int qr_launch(const QkRope& a, cudaStream_t st) {
   const bool lanes = G == 2 || G == 4 || G == 8 || G == 16 || G == 32;
   const int64_t tokens = (int64_t)a.B * a.L;
   if (bits % 16 == 0 && lanes && a.R % (2 * N) == 0 && tokens <= 0x7fffffff) {
-    // one CTA a token when they fill the device; fewer tokens: a CTA for every group's first row
-    const int groups = QR_NT / G;
-    const int most = (heads + groups - 1) / groups;
-    const int ys = tokens >= 2 * (int64_t)num_sms_current_device() ? 1 : (most < 65535 ? most : 65535);
-    const dim3 grid((unsigned)tokens, ys);
+    // a group takes QR_BATCH rows of its token where that still fills the device, else one row
+    const int few = (heads + QR_BATCH - 1) / QR_BATCH;
+    const int64_t want = 4 * (int64_t)num_sms_current_device() * (QR_NT / G);
+    const int hpg = tokens * few >= want ? few : heads;
+    const int64_t ctas = (tokens * hpg * G + QR_NT - 1) / QR_NT;
+    if (ctas > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "qk_norm_rope: too many rows");
+    const dim3 grid((unsigned)ctas);
     auto run = [&](auto g) {
       constexpr int GG = decltype(g)::value;
       if (a.interleaved)
-        qk_rope_vec_kernel<T, GG, true><<<grid, QR_NT, 0, st>>>(a);
+        qk_rope_vec_kernel<T, GG, true><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
       else
-        qk_rope_vec_kernel<T, GG, false><<<grid, QR_NT, 0, st>>>(a);
+        qk_rope_vec_kernel<T, GG, false><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
     };
     switch (G) {
       case 2: run(std::integral_constant<int, 2>()); break;
