@@ -17,12 +17,13 @@ reference keeps one tensor per layer (dropkv_cache.py:581-617) and has no counte
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .ops import _CHECK_STATUS, _DTYPE_CODE, _on_device, _stream, _workspace
+from .ops import _CHECK_STATUS, _DTYPE_CODE, _workspace
 
 __all__ = ["BlockTables", "TokenLogprobs", "block_tables", "store_rows", "qk_norm_rope", "tree_attention",
            "token_logprobs", "tree_mask_from_parents"]
@@ -42,21 +43,44 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]    # int64 [..., top_k]
 
 
-def _on_one_device(*ts):
-    dev = ts[0].device
+# The current stream's handle by device index: the raw query skips making a Stream object, 2 us of
+# a call whose kernel takes 3.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on_one_device(*ts) -> int:
+    """The index of the CUDA device that holds every tensor."""
+    index = ts[0].get_device()
     for t in ts:
-        if not t.is_cuda:
-            raise RuntimeError("dropkv_b200 runs on CUDA tensors only (no CPU path); got a "
-                               f"tensor on {t.device}")
-        if t.device != dev:
-            raise RuntimeError(f"all tensors must be on one device; got {dev} and {t.device}")
-    return dev
+        if t.get_device() != index or not t.is_cuda:
+            if not t.is_cuda:
+                raise RuntimeError("dropkv_b200 runs on CUDA tensors only (no CPU path); got a "
+                                   f"tensor on {t.device}")
+            raise RuntimeError(f"all tensors must be on one device; got {ts[0].device} and {t.device}")
+    return index
+
+
+class _on:
+    """The device guard, which does nothing where the device is current already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, index: int):
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _ints(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
     if t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
     return t.contiguous()
 
@@ -65,20 +89,31 @@ def _rows_strides(t: torch.Tensor, what: str):
     """Strides of the three outer dimensions of [A, B, C, D] rows; a dimension of one
     takes the packed stride, which its own cannot contradict."""
     a, b, c, d = t.shape
-    if d > 1 and t.stride(3) != 1:
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and d > 1:
         raise ValueError(f"{what} needs rows of D contiguous elements")
-    s2 = t.stride(2) if c > 1 else d
-    s1 = t.stride(1) if b > 1 else c * s2
-    s0 = t.stride(0) if a > 1 else max(b * s1, c * s2)
+    if c <= 1:
+        s2 = d
+    if b <= 1:
+        s1 = c * s2
+    if a <= 1:
+        s0 = max(b * s1, c * s2)
     return s0, s1, s2
 
 
 def _check_pool(K_pages, V_pages, Hkv, D, dtype):
-    if K_pages.dim() != 4 or K_pages.shape != V_pages.shape or K_pages.shape[1] != Hkv or K_pages.shape[3] != D:
+    shape = K_pages.shape
+    if len(shape) != 4 or shape != V_pages.shape or shape[1] != Hkv or shape[3] != D:
         raise ValueError(f"expected K and V pages [pages, {Hkv}, block_size, {D}], got {tuple(K_pages.shape)} and "
                          f"{tuple(V_pages.shape)}")
     if K_pages.dtype != dtype or V_pages.dtype != dtype:
         raise TypeError(f"pages must be {dtype}, got {K_pages.dtype} and {V_pages.dtype}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_workspace(index: int, B: int, Hq: int, Hkv: int, T: int, D: int, cap: int) -> int:
+    """Bytes of a tree_attention workspace on the current device ``index``."""
+    return int(_lib.load().dropkv_tree_attention_workspace_size(B, Hq, Hkv, T, D, cap))
 
 
 def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor, max_blocks: int, max_new: int,
@@ -108,11 +143,11 @@ def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor,
     if table is not None:
         table = _ints(table, torch.int32, (B, int(max_blocks)), "table")
         held = _ints(held, torch.int32, (B,), "held")
-    with _on_device(dev):
-        out = BlockTables(torch.empty(B, max_blocks, dtype=torch.int32, device=dev),
-                          torch.empty(B, dtype=torch.int32, device=dev),
-                          torch.empty(B, max_new, dtype=torch.int64, device=dev),
-                          torch.empty(1, dtype=torch.int64, device=dev))
+    with _on(dev):
+        out = BlockTables(torch.empty(B, max_blocks, dtype=torch.int32, device=lens.device),
+                          torch.empty(B, dtype=torch.int32, device=lens.device),
+                          torch.empty(B, max_new, dtype=torch.int64, device=lens.device),
+                          torch.empty(1, dtype=torch.int64, device=lens.device))
         if B == 0:
             out.used.zero_()
             return out
@@ -121,8 +156,9 @@ def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor,
             table.data_ptr() if table is not None else None, int(max_blocks),
             held.data_ptr() if held is not None else None, B, int(block_size), free_blocks.data_ptr(),
             free_blocks.numel(), int(max_blocks), int(max_new), out.table.data_ptr(), out.held.data_ptr(),
-            out.slots.data_ptr(), out.used.data_ptr(), _stream(dev))
-        _lib.check(rc, "dropkv_block_tables")
+            out.slots.data_ptr(), out.used.data_ptr(), _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "dropkv_block_tables")
     return out
 
 
@@ -139,13 +175,14 @@ def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: t
     B, Hkv, N, D = K.shape
     _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
     slots = _ints(slots, torch.int64, (B, N), "slots")
-    with _on_device(dev):
+    with _on(dev):
         rc = _lib.load().dropkv_store_rows(
             K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(),
             K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
             *_rows_strides(V_pages, "V_pages"), K_pages.shape[0], K_pages.shape[2], K.element_size(), B, Hkv, N, D,
-            _stream(dev))
-        _lib.check(rc, "dropkv_store_rows")
+            _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "dropkv_store_rows")
 
 
 def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -199,16 +236,17 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
                 K_pages.shape[0], K_pages.shape[2])
     else:
         tail = (None, 0, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, 0, 1)
-    with _on_device(dev):
-        q_out = torch.empty(B, Hq, L, D, dtype=Q.dtype, device=dev)
-        k_out = torch.empty(B, Hkv, L, D, dtype=Q.dtype, device=dev)
+    with _on(dev):
+        q_out = torch.empty(B, Hq, L, D, dtype=Q.dtype, device=Q.device)
+        k_out = torch.empty(B, Hkv, L, D, dtype=Q.dtype, device=Q.device)
         rc = _lib.load().dropkv_qk_norm_rope(
             Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
             q_weight.data_ptr() if q_weight is not None else None,
             k_weight.data_ptr() if k_weight is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(),
             cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
-            D, q_out.data_ptr(), k_out.data_ptr(), *tail, _stream(dev))
-        _lib.check(rc, "dropkv_qk_norm_rope")
+            D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "dropkv_qk_norm_rope")
     return q_out, k_out
 
 
@@ -273,17 +311,18 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
                 tree_mask.stride(-1))
     scale = float(D ** -0.5 if scale is None else scale)
     lib = _lib.load()
-    with _on_device(dev):
-        out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=dev)
+    with _on(dev):
+        out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=Q.device)
         if B == 0 or T == 0:
             return out
         # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
-        ws = _workspace(lib.dropkv_tree_attention_workspace_size(B, Hq, Hkv, T, D, cap), dev)
+        ws = _workspace(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), Q.device)
         rc = lib.dropkv_tree_attention(
             Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
             *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
-            out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
-        _lib.check(rc, "dropkv_tree_attention")
+            out.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev))
+        if rc:
+            _lib.check(rc, "dropkv_tree_attention")
         if _CHECK_STATUS and cap * n0 > 0 and not torch.cuda.is_current_stream_capturing():
             n = torch.cuda.get_device_properties(dev).multi_processor_count  # a word for each CTA comes first
             st = int(ws[:4 * n].view(torch.int32).max().item()) if ws.numel() >= 4 * n else 0
@@ -318,15 +357,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     C = tokens.shape[-1] if tokens.dim() == logits.dim() else 1
     tokens = tokens.contiguous()
     lib = _lib.load()
-    with _on_device(dev):
-        logprob = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        top_lp = torch.empty(*lead, top_k, dtype=torch.float32, device=dev) if top_k else None
-        top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
-        ws = _workspace(lib.dropkv_token_logprobs_workspace_size(N, V, int(top_k)), dev)
+    with _on(dev):
+        logprob = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
+        entropy = torch.empty(lead, dtype=torch.float32, device=logits.device)
+        top_lp = torch.empty(*lead, top_k, dtype=torch.float32, device=logits.device) if top_k else None
+        top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=logits.device) if top_k else None
         rc = lib.dropkv_token_logprobs(rows.data_ptr(), rows.stride(0), dt, N, V, tokens.data_ptr(), C, int(top_k),
                                        float(temperature), logprob.data_ptr(), entropy.data_ptr(),
                                        top_lp.data_ptr() if top_k else None, top_id.data_ptr() if top_k else None,
-                                       ws.data_ptr(), ws.numel(), _stream(dev))
-        _lib.check(rc, "dropkv_token_logprobs")
+                                       None, 0, _raw_stream(dev))  # (no workspace is needed)
+        if rc:
+            _lib.check(rc, "dropkv_token_logprobs")
     return TokenLogprobs(logprob, entropy, top_lp, top_id)
