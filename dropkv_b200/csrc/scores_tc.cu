@@ -122,6 +122,28 @@ bool make_q_tensor_map(CUtensorMap* map, const ScoreProblem& p, bool bf16) {
   return r == CUDA_SUCCESS;
 }
 
+// Rows of `heads` heads at a time: x [B, H, T, D] with element strides (sb, sh, ss) and unit
+// element stride as {d, row, head, b} with box {64, T, heads, 1}: the T rows of each head, one
+// head after the other, under the 128-byte swizzle. Needs 16-byte aligned base and strides, T
+// and `heads` of at most 256; false (and nothing encoded) otherwise.
+bool make_head_tensor_map(CUtensorMap* map, const void* base, int B, int H, int T, int D, bool bf16, int64_t sb, int64_t sh,
+                          int64_t ss, int heads) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || T > 256 || heads > 256 || reinterpret_cast<uintptr_t>(base) % 16) return false;
+  // a dimension of one has no stride to speak of
+  const int64_t st[3] = {T > 1 ? ss * 2 : (int64_t)D * 2, H > 1 ? sh * 2 : (int64_t)T * D * 2, B > 1 ? sb * 2 : (int64_t)H * T * D * 2};
+  for (int i = 0; i < 3; ++i)
+    if (st[i] <= 0 || st[i] % 16 || st[i] >= (int64_t(1) << 40)) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)st[0], (cuuint64_t)st[1], (cuuint64_t)st[2]};
+  cuuint32_t box[4] = {64, (cuuint32_t)T, (cuuint32_t)heads, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 namespace {
 
 constexpr int TK = 128;                      // keys per tile = MMA M

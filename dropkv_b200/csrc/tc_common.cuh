@@ -355,5 +355,8 @@ int make_kv_tensor_map(CUtensorMap* map, const void* base, int BH, int L, int D,
 // elements, as a 4-D map {d, key, head, b} of 64 x box_rows boxes (128-byte swizzle).
 int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, int L, int D, bool bf16, int64_t sb,
                           int64_t sh, int64_t ss, int box_rows = 128);
+// All T rows of `heads` heads of x [B, H, T, D] in a box (see the definition).
+bool make_head_tensor_map(CUtensorMap* map, const void* base, int B, int H, int T, int D, bool bf16, int64_t sb, int64_t sh,
+                          int64_t ss, int heads);
 
 }  // namespace dropkv

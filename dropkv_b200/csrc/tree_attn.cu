@@ -52,7 +52,8 @@ struct TaArgs {
   int box;                 // rows of a TMA box
   int rows_pad;            // rows of a partial
   float scale_log2;
-  int q_vec;               // Q's rows are read 16 bytes at a time
+  int q_tma;               // Q comes by TMA, all rows of a KV head in a box for each slab
+  int q_vec;               // else: its rows are read 16 bytes at a time
   int mask_vec;            // the mask's rows are read 4 bytes at a time
   float bias;              // weights are 2^(s - m + bias): fp16 has few bits below 1
   int* status;             // [CTAs]: 0, or which wait gave up
@@ -68,11 +69,12 @@ template <int D>
 struct TaSmem {
   static constexpr int TILE = TA_TK * D * 2;  // K, V or Q tile: D / 64 slabs of 128 rows x 128 B
   static constexpr int SLOTS = D == 128 ? 5 : 10;
-  static constexpr int Q = 0;                 // two tiles; a group's maxima and sums once its products are done
+  static constexpr int Q = 0;                 // D / 64 slabs of 256 rows x 128 B: the groups' rows one after the other
   static constexpr int RING = 2 * TILE;
   static constexpr int BARS = RING + SLOTS * TILE;        // full[SLOTS], empty[SLOTS], then B_*
   static constexpr int BAD = BARS + (2 * SLOTS + B_COUNT) * 8;  // uint32 [2][8]: nodes with non-finite V
-  static constexpr int MISC = BAD + 64;
+  static constexpr int ML = BAD + 64;                      // float [2][2][128]: the groups' maxima and sums
+  static constexpr int MISC = ML + 2048;
   static constexpr int BYTES = MISC + 64;
 };
 static_assert(TaSmem<128>::BYTES <= 232448, "shared memory");
@@ -230,7 +232,8 @@ __device__ __forceinline__ void ta_softmax_sync() { asm volatile("bar.sync 1, 25
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TA_NT, 1)
-    tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, TaArgs A) {
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                     const __grid_constant__ CUtensorMap qmap, const __grid_constant__ TaArgs A) {
   using L = TaSmem<D>;
   constexpr int SLABS = D / 64, NS = L::SLOTS;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
@@ -245,6 +248,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (tc::smem_addr(sm) % 1024) {  // as declared; nothing may run on any other layout
+    pdl_wait();
     pdl_launch_dependents();
     if (tid == 0) A.status[blockIdx.x] = 9;
     return;
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
       tc::mbar_init(&empty[i], 2);
     }
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(&bars[B_Q + s], TA_SM / 32);
+      tc::mbar_init(&bars[B_Q + s], A.q_tma ? 1 : TA_SM / 32);
       tc::mbar_init(&bars[B_S + s], 1);
       tc::mbar_init(&bars[B_P + s], TA_SM / 32);
       tc::mbar_init(&bars[B_P + 2 + s], TA_SM / 32);
@@ -274,9 +278,10 @@ __global__ void __launch_bounds__(TA_NT, 1)
   if (warp == TA_WARP_TMA && lane == 0) {
     tc::tma_prefetch_desc(&kmap);
     tc::tma_prefetch_desc(&vmap);
+    if (A.q_tma) tc::tma_prefetch_desc(&qmap);
   }
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();  // (after the wait: the merge may then read this kernel's inputs at once)
   if (warp == 0) {  // where this CTA's share of the line of tiles starts
     const int own0 = lane < a.B ? ta_tiles(a, lane) + kTaLead : 0;
     int total = own0;
@@ -342,7 +347,8 @@ __global__ void __launch_bounds__(TA_NT, 1)
     const CUtensorMap* map = is_v ? &vmap : &kmap;
     const int boxes = TA_TK / A.box;
     uint32_t base = 0;  // load number of the piece's first
-    uint32_t last = 0, any = 0;
+    uint32_t last = 0, any = 0, before = 0;  // `before`: loads of the pieces before the one before
+    int nt_before = 0, lead_before = 0, queries = 0;
     while (walk.next(A, p)) {
       const int nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0), lead = __shfl_sync(0xffffffffu, p.two ? 1 : 2, 0);
       const int h = __shfl_sync(0xffffffffu, p.h, 0), b = __shfl_sync(0xffffffffu, p.b, 0);
@@ -354,6 +360,24 @@ __global__ void __launch_bounds__(TA_NT, 1)
       };
       int page = a.table ? page_of(0) : 0;
       bool ok = true;
+      if (A.q_tma && !is_v) {
+        // the piece's Q, once the products that read the last one's are done: those with its last
+        // K tile (of each group)
+        if (base)
+          for (int i = max(nt_before - lead_before, 0); i < nt_before; ++i) {
+            const uint32_t k = before + k_load(i, lead_before);
+            ok = __all_sync(0xffffffffu, ok && wait(&empty[k % NS], k / NS, 12));
+          }
+        if (!ok) break;
+        if (tc::elect_one()) {
+          tc::mbar_arrive_expect_tx(&bars[B_Q], A.M * 128 * SLABS);
+#pragma unroll
+          for (int s = 0; s < SLABS; ++s)
+            tc::tma_load_4d(sm + L::Q + s * (TA_ROWS * 128), &qmap, &bars[B_Q], 64 * s, 0, h * A.g, b);
+        }
+        __syncwarp();
+        ++queries;
+      }
       for (int i = 0; i < nt; ++i) {
         const int next = a.table ? page_of(i + 1) : 0;
         const uint32_t k = base + (is_v ? v_load(i, lead, nt) : k_load(i, lead)), slot = k % NS;
@@ -402,15 +426,17 @@ __global__ void __launch_bounds__(TA_NT, 1)
         }
         last = k, any = 1;
         page = next;
-        // the first piece's Q comes before the rest of the ring: 160 KB an SM at once hold it up by 3 us
-        if (base == 0 && i == 0) wait(&bars[B_Q], 0, 11);
       }
       if (!ok) break;
+      before = base;
+      nt_before = nt;
+      lead_before = lead;
       base += 2 * nt;
     }
-    if (*dead && any) {  // every issued copy lands before the CTA may exit
+    if (*dead && (any || queries)) {  // every issued copy lands before the CTA may exit
       for (uint32_t j = last >= (uint32_t)NS ? last - NS + 1 : 0u; j <= last; ++j)  // (some are the other's, or not issued)
         tc::mbar_wait(&full[j % NS], (j / NS) & 1, kTaWaitNs / 8);
+      if (queries) tc::mbar_wait(&bars[B_Q], (queries - 1) & 1, kTaWaitNs);
     }
   } else if (warp >= TA_WARP_MMA) {
     // ======================= MMA issuers ========================================
@@ -426,13 +452,15 @@ __global__ void __launch_bounds__(TA_NT, 1)
     const int s = __shfl_sync(0xffffffffu, warp - TA_WARP_MMA, 0);
     const uint32_t ts = __shfl_sync(0xffffffffu, tmem, 0) + s * 128, to = ts + 256;
     const uint32_t ring0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::RING), 0);
-    const uint64_t qd = tc::smem_desc(__shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0) + s * L::TILE, 16, 1024);
-    uint32_t base = 0, n_q = 0, n_p = 0, n_t = 0;
+    const uint32_t q0 = __shfl_sync(0xffffffffu, tc::smem_addr(sm + L::Q), 0);
+    uint32_t base = 0, n_q = 0, n_p = 0, n_t = 0, pieces = 0;
     bool handed = false;  // group 1 issued the last item of the piece before, and handed the turn over
     bool ok = true;
     while (ok && walk.next(A, p)) {
       const int two = __shfl_sync(0xffffffffu, (int)p.two, 0), nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
       const int lead = two ? 1 : 2, step = lead, first = two ? 0 : s;
+      // tiles in turn: by TMA there is one copy of the rows, for both groups
+      const uint64_t qd = tc::smem_desc(q0 + (A.q_tma && !two ? 0 : s * (128 * 128)), 16, 1024);
       auto release = [&](uint64_t* bar) {  // two arrivals empty a slot: one of each group, or both of its only one
         tc::mma_commit(bar);
         if (!two) tc::mma_commit(bar);
@@ -441,21 +469,23 @@ __global__ void __launch_bounds__(TA_NT, 1)
         const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * (TA_TK * 128) + (kk % 4) * 32;
-          tc::mma_f16(ts, tc::desc_add(qd, off), tc::desc_add(kd, off), ID_QK, kk > 0);
+          tc::mma_f16(ts, tc::desc_add(qd, (kk / 4) * (TA_ROWS * 128) + (kk % 4) * 32),
+                      tc::desc_add(kd, (kk / 4) * (TA_TK * 128) + (kk % 4) * 32), ID_QK, kk > 0);
         }
         tc::mma_commit(&bars[B_S + s]);
         release(&empty[slot]);
       };
       if (first < nt) {  // the first product, out of turn: nothing is running yet
         const uint32_t at = base + k_load(first, lead), slot = at % NS;
-        ok = wait(&bars[B_Q + s], n_q++, 2) && wait(&full[slot], at / NS, 3);
+        ok = wait(&bars[B_Q + (A.q_tma ? 0 : s)], A.q_tma ? pieces : n_q++, 2) && wait(&full[slot], at / NS, 3);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           tc::tc_fence_after();
           if (tc::elect_one()) qk(slot);
           __syncwarp();
         }
+      } else if (A.q_tma) {
+        ok = __all_sync(0xffffffffu, wait(&bars[B_Q], pieces, 2));  // every piece's Q is waited for: none is taken for another
       }
       for (int i = first; i < nt && ok; i += step) {
         const uint32_t at = base + v_load(i, lead, nt), slot = at % NS;
@@ -491,6 +521,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
         __syncwarp();
       }
       base += 2 * nt;
+      ++pieces;
       handed = two || nt % 2 == 0;
     }
     if (*dead) {  // no product may run on when tensor memory is given back
@@ -504,8 +535,8 @@ __global__ void __launch_bounds__(TA_NT, 1)
     const int s = warp >> 2, quad = warp & 3, r = tid & 127;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256;
-    float* ml0 = reinterpret_cast<float*>(sm + L::Q);  // [2][128]: maxima, sums
-    float* ml1 = reinterpret_cast<float*>(sm + L::Q + L::TILE);
+    float* ml0 = reinterpret_cast<float*>(sm + L::ML);  // [2][128]: maxima, sums
+    float* ml1 = ml0 + 256;
     uint32_t n_s = 0, n_o = 0, base = 0;
     bool ok = true;
     for (int piece = 0; walk.next(A, p); ++piece) {
@@ -516,43 +547,36 @@ __global__ void __launch_bounds__(TA_NT, 1)
       const bool live = quad * 32 < rows;  // some row of this warp exists
       uint32_t* bad_now = bad + 8 * (piece & 1);
       float m = -INFINITY, l = 0.f;
-      if (mine) {
+      if (mine && !A.q_tma) {
         // Q rows into shared memory, 16 bytes a thread and step: row = head of the group, then
-        // node. The loads of all steps are on their way before the first is stored.
+        // node. The loads of four steps are on their way before the first is stored.
         const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh;
         constexpr int STEP = TA_SM / (D / 8);  // rows a step of the group covers
         const int c = r % (D / 8);             // a thread's column of vectors stays, its row moves on
-        const int e0 = r / (D / 8);
-        uint4 x[128 / STEP];
-        auto src = [&](int i) {
-          const int mrow = row0 + min(e0 + i * STEP, rows - 1), head = A.by_t.quot(mrow);
-          return qb + head * a.q_sh + (mrow - head * a.T) * a.q_ss + c * 8 * a.q_sd;
-        };
-        if (A.q_vec) {
-#pragma unroll
-          for (int i = 0; i < 128 / STEP; ++i) x[i] = *reinterpret_cast<const uint4*>(src(i));
-        } else {
 #pragma unroll 1
-          for (int i = 0; i < 128 / STEP; ++i) {  // (x stays in registers: rows are stored as they come)
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(src(i));
-            uint4 y;
-            y.x = h[0] | (uint32_t)h[a.q_sd] << 16;
-            y.y = h[2 * a.q_sd] | (uint32_t)h[3 * a.q_sd] << 16;
-            y.z = h[4 * a.q_sd] | (uint32_t)h[5 * a.q_sd] << 16;
-            y.w = h[6 * a.q_sd] | (uint32_t)h[7 * a.q_sd] << 16;
-            const int row = e0 + i * STEP;
-            if (row >= rows) y = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
-                                      tc::sw128_offset(row, (c % 8) * 8)) = y;
-          }
-        }
-        if (A.q_vec)
+        for (int e0 = r / (D / 8); e0 < 128; e0 += 4 * STEP) {  // (rolled: code that runs once is fetched as it runs)
+          uint4 x[4];
 #pragma unroll
-        for (int i = 0; i < 128 / STEP; ++i) {
-          const int row = e0 + i * STEP;
-          if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(sm + L::Q + s * L::TILE + (c / 8) * (TA_TK * 128) +
-                                    tc::sw128_offset(row, (c % 8) * 8)) = x[i];
+          for (int i = 0; i < 4; ++i) {
+            const int mrow = row0 + min(e0 + i * STEP, rows - 1), head = A.by_t.quot(mrow);
+            const T* src = qb + head * a.q_sh + (mrow - head * a.T) * a.q_ss + c * 8 * a.q_sd;
+            if (A.q_vec) {
+              x[i] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+              x[i].x = h[0] | (uint32_t)h[a.q_sd] << 16;
+              x[i].y = h[2 * a.q_sd] | (uint32_t)h[3 * a.q_sd] << 16;
+              x[i].z = h[4 * a.q_sd] | (uint32_t)h[5 * a.q_sd] << 16;
+              x[i].w = h[6 * a.q_sd] | (uint32_t)h[7 * a.q_sd] << 16;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = e0 + i * STEP;
+            if (row >= rows) x[i] = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(sm + L::Q + (c / 8) * (TA_ROWS * 128) + s * (128 * 128) +
+                                      tc::sw128_offset(row, (c % 8) * 8)) = x[i];
+          }
         }
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -875,16 +899,18 @@ __global__ void __launch_bounds__(TA_NT, 1)
 }
 
 constexpr int TM_NT = 256;
+constexpr int TM_WARPS = TM_NT / 32;
 constexpr int TM_PIECES = 64;  // partials whose factors are held at once
+constexpr int TM_AHEAD = 8;    // partials on their way at once
 
 // Joins the partials of the segments that fell into several CTAs. Grid: (segments,
 // 32-row blocks x blocks of 32 columns); a thread has a row and four columns. The
 // partials lie [column / 4][row], so a warp reads 32 rows of 16 bytes in one piece.
-// The eight warps first share out the partials' maxima and sums.
+// The eight warps share out the partials' maxima and sums, while the first partials come.
 template <typename T, int D>
-__global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ctas) {
-  __shared__ int red[2][TM_NT / 32];
-  __shared__ float fac[TM_PIECES][32], mxs[TM_NT / 32][32], sums[TM_NT / 32][32];
+__global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(const __grid_constant__ TaArgs A, int ctas) {
+  __shared__ int red[2][TM_WARPS];
+  __shared__ float fac[TM_PIECES][32], mxs[TM_WARPS][32], sums[TM_WARPS][32];
   const TreeAttn& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / A.HR, seg = blockIdx.x % A.HR;
@@ -892,7 +918,7 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
   const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
   if (rt * TA_ROWS + rb * 32 >= A.M) return;
-  pdl_wait();
+  // the lengths were there before the kernel whose partials these are began: no wait yet
   int before = 0, total = 0;
   for (int i = tid; i < a.B; i += TM_NT) {
     const int t = ta_tiles(a, i) + kTaLead;
@@ -908,7 +934,7 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   __syncthreads();
   total = before = 0;
 #pragma unroll
-  for (int w = 0; w < TM_NT / 32; ++w) total += red[0][w], before += red[1][w];
+  for (int w = 0; w < TM_WARPS; ++w) total += red[0][w], before += red[1][w];
   const int per = (total * A.HR + ctas - 1) / ctas, tiles = ta_tiles(a, b);
   const int w0 = before * A.HR + seg * (tiles + kTaLead) + kTaLead, w1 = w0 + tiles;
   const int c0 = w0 / per, n = (w1 - 1) / per - c0 + 1;
@@ -917,23 +943,31 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   auto slot = [&](int i) { return (int64_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
   const bool own = row < A.rows_pad && mrow < A.M;
   const float* pml = A.part_ml + row;
+  const int q = cb * 8 + warp;  // the thread's group of four columns
+  const float4* po = reinterpret_cast<const float4*>(A.part_o) + (int64_t)q * A.rows_pad + row;
+  auto load = [&](int i, float4* x) {
+#pragma unroll
+    for (int u = 0; u < TM_AHEAD; ++u) x[u] = __ldcg(po + slot(min(i + u, n - 1)) * (D / 4) * A.rows_pad);
+  };
+  pdl_wait();
+  float4 x[TM_AHEAD];
+  if (own) load(0, x);
   float mine = -INFINITY;
   if (own) {
 #pragma unroll 4
-    for (int i = warp; i < n; i += TM_NT / 32) mine = fmaxf(mine, __ldcg(pml + slot(i) * 2 * A.rows_pad));
+    for (int i = warp; i < n; i += TM_WARPS) mine = fmaxf(mine, __ldcg(pml + slot(i) * 2 * A.rows_pad));
   }
   mxs[warp][lane] = mine;
   __syncthreads();
   float m = mxs[0][lane];
 #pragma unroll
-  for (int w = 1; w < TM_NT / 32; ++w) m = fmaxf(m, mxs[w][lane]);
-  const int q = cb * 8 + warp;  // the thread's group of four columns
+  for (int w = 1; w < TM_WARPS; ++w) m = fmaxf(m, mxs[w][lane]);
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < n; i0 += TM_PIECES) {
     const int cnt = min(TM_PIECES, n - i0);
     if (i0) __syncthreads();  // the factors before have been used
-    for (int i = warp; i < cnt; i += TM_NT / 32) {
+    for (int i = warp; i < cnt; i += TM_WARPS) {
       float f = 0.f;
       if (own) {
         const float* pm = pml + slot(i0 + i) * 2 * A.rows_pad;
@@ -944,20 +978,19 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
     }
     __syncthreads();
     if (own) {
-      for (int i = 0; i < cnt; i += 8) {  // eight partials on their way at once
-        float4 x[8];
+      for (int i = 0; i < cnt; i += TM_AHEAD) {
+        float4 y[TM_AHEAD];
+        if (i0 + i + TM_AHEAD < n) load(i0 + i + TM_AHEAD, y);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          x[u] = __ldcg(reinterpret_cast<const float4*>(A.part_o) +
-                        (slot(i0 + min(i + u, cnt - 1)) * (D / 4) + q) * A.rows_pad + row);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (i + u >= cnt) break;
-          const float f = fac[i + u][lane];
-          o.x = fmaf(x[u].x, f, o.x);
-          o.y = fmaf(x[u].y, f, o.y);
-          o.z = fmaf(x[u].z, f, o.z);
-          o.w = fmaf(x[u].w, f, o.w);
+        for (int u = 0; u < TM_AHEAD; ++u) {
+          if (i + u < cnt) {
+            const float f = fac[i + u][lane];
+            o.x = fmaf(x[u].x, f, o.x);
+            o.y = fmaf(x[u].y, f, o.y);
+            o.z = fmaf(x[u].z, f, o.z);
+            o.w = fmaf(x[u].w, f, o.w);
+          }
+          x[u] = y[u];
         }
       }
     }
@@ -967,7 +1000,7 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(TaArgs A, int ct
   if (!own) return;
   l = sums[0][lane];
 #pragma unroll
-  for (int w = 1; w < TM_NT / 32; ++w) l += sums[w][lane];
+  for (int w = 1; w < TM_WARPS; ++w) l += sums[w][lane];
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t out_row = ((int64_t)b * a.Hq + h * A.g) * a.T + mrow;  // heads of T rows follow one another
   uint2 y;
@@ -1016,10 +1049,12 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   A.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_o);
   A.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + plan.off_ml);
   const int n0 = a.table ? a.n_pages : a.B, rows = a.table ? a.block : a.cap;
-  CUtensorMap km, vm;
+  CUtensorMap km, vm, qm;
   int rc = make_kv_tensor_map_4d(&km, a.k, n0, a.Hkv, rows, D, bf16, a.k_s0, a.k_sh, a.k_ss, A.box);
   if (!rc) rc = make_kv_tensor_map_4d(&vm, a.v, n0, a.Hkv, rows, D, bf16, a.v_s0, a.v_sh, a.v_ss, A.box);
   if (rc) return rc;
+  A.q_tma = A.q_vec && A.RT == 1 && make_head_tensor_map(&qm, a.q, a.B, a.Hq, a.T, D, bf16, a.q_sb, a.q_sh, a.q_ss, A.g);
+  if (!A.q_tma) qm = km;  // not used
   auto kern = tree_attn_kernel<T, D>;
   auto merge = tree_attn_merge_kernel<T, D>;
   static DeviceOnce done;
@@ -1040,7 +1075,7 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(TA_NT);
   cfg.dynamicSmemBytes = L::BYTES;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, qm, A);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "tree attention launch: %s", cudaGetErrorString(e));
   rc = check_launch("tree_attention");
   if (rc || a.cap <= TA_TK) return rc;  // a cache of one tile: nothing is split
