@@ -50,31 +50,29 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _on_one_device(*ts) -> int:
-    """The index of the CUDA device that holds every tensor."""
+    """The index of the CUDA device that holds every tensor (-1 stands for the CPU)."""
     index = ts[0].get_device()
     for t in ts:
-        if t.get_device() != index or not t.is_cuda:
-            if not t.is_cuda:
+        if t.get_device() != index or index < 0:
+            cpu = [x.device for x in ts if not x.is_cuda]
+            if cpu:
                 raise RuntimeError("dropkv_b200 runs on CUDA tensors only (no CPU path); got a "
-                                   f"tensor on {t.device}")
+                                   f"tensor on {cpu[0]}")
             raise RuntimeError(f"all tensors must be on one device; got {ts[0].device} and {t.device}")
     return index
 
 
-class _on:
-    """The device guard, which does nothing where the device is current already."""
-    __slots__ = ("guard",)
-
-    def __init__(self, index: int):
-        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on_its_device(fn):
+    """The call under its first tensor's device, entered only where another one is current."""
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        first = args[0] if args else next(iter(kwargs.values()), None)
+        index = first.get_device() if isinstance(first, torch.Tensor) else -1
+        if index < 0 or index == torch.cuda.current_device():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(index):
+            return fn(*args, **kwargs)
+    return call
 
 
 def _ints(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch.Tensor:
@@ -116,6 +114,7 @@ def _tree_workspace(index: int, B: int, Hq: int, Hkv: int, T: int, D: int, cap: 
     return int(_lib.load().dropkv_tree_attention_workspace_size(B, Hq, Hkv, T, D, cap))
 
 
+@_on_its_device
 def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor, max_blocks: int, max_new: int,
                  new_lens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
                  held: Optional[torch.Tensor] = None) -> BlockTables:
@@ -130,38 +129,43 @@ def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor,
     short, entries and slots are -1, ``held`` counts the pages really held and
     ``used`` is more than F.
     """
-    if lens.dim() != 1:
-        raise ValueError(f"lens must be [B], got {tuple(lens.shape)}")
     if (table is None) != (held is None):
         raise ValueError("table and held go together")
-    dev = _on_one_device(*[t for t in (lens, free_blocks, new_lens, table, held) if t is not None])
-    B = lens.shape[0]
+    if lens.dim() != 1:
+        raise ValueError(f"lens must be [B], got {tuple(lens.shape)}")
+    B, F = lens.shape[0], free_blocks.numel()
+    max_blocks, max_new = int(max_blocks), int(max_new)
+    device = lens.device
+    dev = _on_one_device(lens, free_blocks)
     lens = _ints(lens, torch.int32, (B,), "lens")
-    free_blocks = _ints(free_blocks, torch.int32, (free_blocks.numel(),), "free_blocks")
+    free_blocks = _ints(free_blocks, torch.int32, (F,), "free_blocks")
+    new_ptr = table_ptr = held_ptr = None
     if new_lens is not None:
+        _on_one_device(lens, new_lens)
         new_lens = _ints(new_lens, torch.int32, (B,), "new_lens")
+        new_ptr = new_lens.data_ptr()
     if table is not None:
-        table = _ints(table, torch.int32, (B, int(max_blocks)), "table")
+        _on_one_device(lens, table, held)
+        table = _ints(table, torch.int32, (B, max_blocks), "table")
         held = _ints(held, torch.int32, (B,), "held")
-    with _on(dev):
-        out = BlockTables(torch.empty(B, max_blocks, dtype=torch.int32, device=lens.device),
-                          torch.empty(B, dtype=torch.int32, device=lens.device),
-                          torch.empty(B, max_new, dtype=torch.int64, device=lens.device),
-                          torch.empty(1, dtype=torch.int64, device=lens.device))
-        if B == 0:
-            out.used.zero_()
-            return out
-        rc = _lib.load().dropkv_block_tables(
-            lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None,
-            table.data_ptr() if table is not None else None, int(max_blocks),
-            held.data_ptr() if held is not None else None, B, int(block_size), free_blocks.data_ptr(),
-            free_blocks.numel(), int(max_blocks), int(max_new), out.table.data_ptr(), out.held.data_ptr(),
-            out.slots.data_ptr(), out.used.data_ptr(), _raw_stream(dev))
-        if rc:
-            _lib.check(rc, "dropkv_block_tables")
+        table_ptr, held_ptr = table.data_ptr(), held.data_ptr()
+    out = BlockTables(torch.empty((B, max_blocks), dtype=torch.int32, device=device),
+                      torch.empty(B, dtype=torch.int32, device=device),
+                      torch.empty((B, max_new), dtype=torch.int64, device=device),
+                      torch.empty(1, dtype=torch.int64, device=device))
+    if B == 0:
+        out.used.zero_()
+        return out
+    rc = _lib.load().dropkv_block_tables(
+        lens.data_ptr(), new_ptr, table_ptr, max_blocks, held_ptr, B, int(block_size), free_blocks.data_ptr(), F,
+        max_blocks, max_new, out.table.data_ptr(), out.held.data_ptr(), out.slots.data_ptr(), out.used.data_ptr(),
+        _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_block_tables")
     return out
 
 
+@_on_its_device
 def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: torch.Tensor,
                V_pages: torch.Tensor) -> None:
     """Rows of K and V [B, Hkv, N, D] (any strides, rows of D contiguous) to slots [B, N]
@@ -175,16 +179,16 @@ def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: t
     B, Hkv, N, D = K.shape
     _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
     slots = _ints(slots, torch.int64, (B, N), "slots")
-    with _on(dev):
-        rc = _lib.load().dropkv_store_rows(
-            K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(),
-            K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
-            *_rows_strides(V_pages, "V_pages"), K_pages.shape[0], K_pages.shape[2], K.element_size(), B, Hkv, N, D,
-            _raw_stream(dev))
-        if rc:
-            _lib.check(rc, "dropkv_store_rows")
+    rc = _lib.load().dropkv_store_rows(
+        K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(),
+        K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
+        *_rows_strides(V_pages, "V_pages"), K_pages.shape[0], K_pages.shape[2], K.element_size(), B, Hkv, N, D,
+        _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_store_rows")
 
 
+@_on_its_device
 def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                  q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
                  interleaved: bool = False, V: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
@@ -201,14 +205,19 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
     ``V_pages`` the finished K rows and V's also go to the pool, as ``store_rows`` puts
     them. fp32, fp16 or bf16; sums in fp32, rounded once.
     """
-    cache = [t for t in (V, slots, K_pages, V_pages) if t is not None]
-    if cache and len(cache) != 4:
+    given = (V is not None) + (slots is not None) + (K_pages is not None) + (V_pages is not None)
+    if given not in (0, 4):
         raise ValueError("V, slots, K_pages and V_pages go together")
-    dev = _on_one_device(Q, K, cos, sin, positions, *[t for t in (q_weight, k_weight) if t is not None], *cache)
+    cache = (V, slots, K_pages, V_pages) if given else ()
+    dev = _on_one_device(Q, K, cos, sin, positions, *cache)
+    for w in (q_weight, k_weight):
+        if w is not None:
+            _on_one_device(Q, w)
     if Q.dim() != 4 or K.dim() != 4 or Q.shape[0] != K.shape[0] or Q.shape[2:] != K.shape[2:]:
         raise ValueError(f"expected Q [B,Hq,L,D] and K [B,Hkv,L,D], got {tuple(Q.shape)} and {tuple(K.shape)}")
-    dt = _DTYPE_CODE.get(Q.dtype)
-    if dt is None or K.dtype != Q.dtype:
+    dtype = Q.dtype
+    dt = _DTYPE_CODE.get(dtype)
+    if dt is None or K.dtype != dtype:
         raise TypeError(f"Q and K must share one of fp32/fp16/bf16; got {Q.dtype}, {K.dtype}")
     B, Hq, L, D = Q.shape
     Hkv = K.shape[1]
@@ -222,7 +231,7 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
     else:
         positions, pos_sb = _ints(positions, torch.int64, (B, L), "positions"), L
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (tuple(w.shape) != (D,) or w.dtype != Q.dtype):
+        if w is not None and (w.shape != (D,) or w.dtype != Q.dtype):
             raise ValueError(f"{name} must be [{D}] {Q.dtype}, got {tuple(w.shape)} {w.dtype}")
     q_weight = q_weight.contiguous() if q_weight is not None else None
     k_weight = k_weight.contiguous() if k_weight is not None else None
@@ -236,17 +245,16 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
                 K_pages.shape[0], K_pages.shape[2])
     else:
         tail = (None, 0, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, 0, 1)
-    with _on(dev):
-        q_out = torch.empty(B, Hq, L, D, dtype=Q.dtype, device=Q.device)
-        k_out = torch.empty(B, Hkv, L, D, dtype=Q.dtype, device=Q.device)
-        rc = _lib.load().dropkv_qk_norm_rope(
-            Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
-            q_weight.data_ptr() if q_weight is not None else None,
-            k_weight.data_ptr() if k_weight is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(),
-            cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
-            D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
-        if rc:
-            _lib.check(rc, "dropkv_qk_norm_rope")
+    q_out = torch.empty((B, Hq, L, D), dtype=dtype, device=Q.device)
+    k_out = torch.empty((B, Hkv, L, D), dtype=dtype, device=Q.device)
+    rc = _lib.load().dropkv_qk_norm_rope(
+        Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
+        q_weight.data_ptr() if q_weight is not None else None,
+        k_weight.data_ptr() if k_weight is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(),
+        cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
+        D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_qk_norm_rope")
     return q_out, k_out
 
 
@@ -266,6 +274,7 @@ def tree_mask_from_parents(parents: torch.Tensor):
     return mask, mask.sum(-1) - 1
 
 
+@_on_its_device
 def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens: torch.Tensor,
                    tree_mask: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None,
                    scale: Optional[float] = None) -> torch.Tensor:
@@ -289,7 +298,7 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
         raise TypeError("tree attention takes bf16 or fp16 Q, K and V of one dtype")
     B, Hq, T, D = Q.shape
     n0, Hkv, rows, Dk = K.shape
-    if Dk != D or Hq % Hkv or (block_table is None and n0 != B):
+    if Dk != D or not Hkv or Hq % Hkv or (block_table is None and n0 != B):
         raise ValueError(f"shape mismatch: Q {tuple(Q.shape)}, K {tuple(K.shape)}")
     cache_lens = _ints(cache_lens, torch.int32, (B,), "cache_lens")
     if block_table is not None:
@@ -305,33 +314,33 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:
             raise TypeError(f"tree_mask must be bool, got {tree_mask.dtype}")
-        if tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
+        if tree_mask.shape not in ((T, T), (B, T, T)):
             raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(tree_mask.shape)}")
         mask = (tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2),
                 tree_mask.stride(-1))
     scale = float(D ** -0.5 if scale is None else scale)
     lib = _lib.load()
-    with _on(dev):
-        out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=Q.device)
-        if B == 0 or T == 0:
-            return out
-        # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
-        ws = _workspace(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), Q.device)
-        rc = lib.dropkv_tree_attention(
-            Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
-            *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
-            out.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev))
-        if rc:
-            _lib.check(rc, "dropkv_tree_attention")
-        if _CHECK_STATUS and cap * n0 > 0 and not torch.cuda.is_current_stream_capturing():
-            n = torch.cuda.get_device_properties(dev).multi_processor_count  # a word for each CTA comes first
-            st = int(ws[:4 * n].view(torch.int32).max().item()) if ws.numel() >= 4 * n else 0
-            if st != 0:
-                raise _lib.DropKVError(_lib.ERR_DEVICE, f"dropkv_tree_attention: device status {st} "
-                                                        "(a bounded wait timed out)")
+    out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=Q.device)
+    if B == 0 or T == 0:
+        return out
+    # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
+    ws = _workspace(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), Q.device)
+    rc = lib.dropkv_tree_attention(
+        Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
+        *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
+        out.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_tree_attention")
+    if _CHECK_STATUS and cap * n0 > 0 and not torch.cuda.is_current_stream_capturing():
+        n = torch.cuda.get_device_properties(dev).multi_processor_count  # a word for each CTA comes first
+        st = int(ws[:4 * n].view(torch.int32).max().item()) if ws.numel() >= 4 * n else 0
+        if st != 0:
+            raise _lib.DropKVError(_lib.ERR_DEVICE, f"dropkv_tree_attention: device status {st} "
+                                                    "(a bounded wait timed out)")
     return out
 
 
+@_on_its_device
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """Under softmax(logits / temperature) for rows of logits [..., V] (fp32, fp16 or
@@ -348,24 +357,24 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     if logits.dim() < 1 or tokens.dim() - logits.dim() not in (-1, 0) or tokens.shape[:logits.dim() - 1] != logits.shape[:-1]:
         raise ValueError(f"expected logits [..., V] and tokens [...] or [..., C], got {tuple(logits.shape)} and "
                          f"{tuple(tokens.shape)}")
-    V = logits.shape[-1]
-    lead = logits.shape[:-1]
+    V, lead, device = logits.shape[-1], logits.shape[:-1], logits.device
     rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if V > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
-    N = rows.shape[0]
+    N, top_k = rows.shape[0], int(top_k)
     C = tokens.shape[-1] if tokens.dim() == logits.dim() else 1
     tokens = tokens.contiguous()
+    logprob = torch.empty(tokens.shape, dtype=torch.float32, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+    top_lp = top_id = None
+    if top_k > 0:
+        top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=device)
+        top_id = torch.empty((*lead, top_k), dtype=torch.int64, device=device)
     lib = _lib.load()
-    with _on(dev):
-        logprob = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
-        entropy = torch.empty(lead, dtype=torch.float32, device=logits.device)
-        top_lp = torch.empty(*lead, top_k, dtype=torch.float32, device=logits.device) if top_k else None
-        top_id = torch.empty(*lead, top_k, dtype=torch.int64, device=logits.device) if top_k else None
-        rc = lib.dropkv_token_logprobs(rows.data_ptr(), rows.stride(0), dt, N, V, tokens.data_ptr(), C, int(top_k),
-                                       float(temperature), logprob.data_ptr(), entropy.data_ptr(),
-                                       top_lp.data_ptr() if top_k else None, top_id.data_ptr() if top_k else None,
-                                       None, 0, _raw_stream(dev))  # (no workspace is needed)
-        if rc:
-            _lib.check(rc, "dropkv_token_logprobs")
+    rc = lib.dropkv_token_logprobs(rows.data_ptr(), rows.stride(0), dt, N, V, tokens.data_ptr(), C, top_k,
+                                   float(temperature), logprob.data_ptr(), entropy.data_ptr(),
+                                   top_lp.data_ptr() if top_k > 0 else None, top_id.data_ptr() if top_k > 0 else None,
+                                   None, 0, _raw_stream(dev))  # (no workspace is needed)
+    if rc:
+        _lib.check(rc, "dropkv_token_logprobs")
     return TokenLogprobs(logprob, entropy, top_lp, top_id)
