@@ -127,6 +127,39 @@ def test_rows_in_pages(B, Hq, Hkv, T, D, lens, block, nhd):
     assert torch.equal(got, tree_attention(Q, K, V, n, tree_mask=mask))
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,T,D,most,paged", [
+    (90, 8, 4, 3, 128, 300, True),      # few rows, several short pieces of caches to a CTA
+    (61, 8, 4, 3, 64, 40, False),       # caches of one tile: every piece is whole
+    (40, 32, 4, 20, 128, 700, True),    # 160 rows: two groups of rows, several pieces to a CTA
+    (30, 28, 4, 50, 64, 500, True),     # 350 rows: more than a segment's
+])
+def test_many_short_caches(B, Hq, Hkv, T, D, most, paged):
+    rs = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, most, (B,), generator=rs).tolist()
+    Q, K, V, n = _inputs(B, Hq, Hkv, T, D, lens, torch.bfloat16, seed=B)
+    mask = _random_tree(T, rs, B).cuda()
+    if paged:
+        Kp, Vp, table = _paged(K, V, lens, T, 16, seed=B, nhd=False)
+        got = tree_attention(Q, Kp, Vp, n, tree_mask=mask, block_table=table)
+    else:
+        got = tree_attention(Q, K, V, n, tree_mask=mask)
+    some = [0, 1, B // 3, B // 2, B - 1]
+    _close(got[some], Q[some], K[some], V[some], [lens[b] for b in some], mask[some])
+    alone = torch.stack([tree_attention(Q[b:b + 1], K[b:b + 1], V[b:b + 1], n[b:b + 1], tree_mask=mask[b])[0] for b in range(B)])
+    # each is as near to the definition as the tolerance says: twice that between the two
+    u = ROUNDOFF[torch.bfloat16]
+    assert float((got.double() - alone.double()).abs().max()) <= 2 * (u * 6 + (2 * u + 2.0 ** -13) * 6)
+
+
+def test_a_long_cache_in_small_pages_with_few_rows():
+    lens, T = [30000, 7], 4
+    Q, K, V, n = _inputs(2, 28, 4, T, 128, lens, torch.float16, seed=12)
+    mask = _random_tree(T, torch.Generator().manual_seed(12)).cuda()
+    Kp, Vp, table = _paged(K, V, lens, T, 8, seed=3, nhd=False)
+    got = tree_attention(Q, Kp, Vp, n, tree_mask=mask, block_table=table)
+    _close(got, Q, K, V, lens, mask)
+
+
 def test_chain_is_causal_and_scale():
     Q, K, V, n = _inputs(2, 8, 2, 9, 128, [333, 60], torch.bfloat16, seed=1)
     got = tree_attention(Q, K, V, n, scale=0.2)
