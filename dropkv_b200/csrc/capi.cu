@@ -624,6 +624,14 @@ int dropkv_decode_append_attention(const void* q, int64_t q_sb, int64_t q_sh, in
 // ---------------------------------------------------------------------------
 // Paged caches and the speculative decode step
 // ---------------------------------------------------------------------------
+// Strides of the outer dimensions of [a, b, c, d] rows: a dimension of one is never stepped
+// along, whatever its stride says, and takes the packed one.
+static void settle_strides(int64_t a, int64_t b, int64_t c, int64_t d, int64_t* s0, int64_t* s1, int64_t* s2) {
+  if (c <= 1) *s2 = d;
+  if (b <= 1) *s1 = c * *s2;
+  if (a <= 1) *s0 = std::max(b * *s1, c * *s2);
+}
+
 int dropkv_block_tables(const int32_t* lens, const int32_t* new_lens, const int32_t* table_in, int64_t table_in_stride,
                         const int32_t* held, int B, int block_size, const int32_t* free_blocks, int n_free,
                         int max_blocks, int max_new, int32_t* table, int32_t* held_out, int64_t* slots, int64_t* used,
@@ -649,6 +657,10 @@ int dropkv_store_rows(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, c
   if (B < 0 || Hkv < 1 || N < 0 || D < 1 || n_pages < 0 || block_size < 1)
     return fail(DROPKV_ERR_ARG, "invalid sizes B=%d Hkv=%d N=%d D=%d pages=%d block_size=%d", B, Hkv, N, D, n_pages, block_size);
   if (B == 0 || N == 0 || n_pages == 0) return DROPKV_OK;  // nothing to store, or nowhere
+  settle_strides(B, Hkv, N, D, &k_sb, &k_sh, &k_sn);
+  settle_strides(B, Hkv, N, D, &v_sb, &v_sh, &v_sn);
+  settle_strides(n_pages, Hkv, block_size, D, &kp_sb, &kp_sh, &kp_st);
+  settle_strides(n_pages, Hkv, block_size, D, &vp_sb, &vp_sh, &vp_st);
   if (!k || !v || !slots || !k_pages || !v_pages) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_pages) |
        reinterpret_cast<uintptr_t>(v_pages)) % elem_bytes)
@@ -675,9 +687,14 @@ int dropkv_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_sl,
   if (!(eps >= 0.f)) return fail(DROPKV_ERR_ARG, "eps must be >= 0");
   if (B == 0 || L == 0) return DROPKV_OK;
   if (!q || !k || !positions || !q_out || !k_out) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  settle_strides(B, Hq, L, D, &q_sb, &q_sh, &q_sl);
+  settle_strides(B, Hkv, L, D, &k_sb, &k_sh, &k_sl);
   if (slots) {
     if (!v || !k_pages || !v_pages) return fail(DROPKV_ERR_ARG, "slots need v, k_pages and v_pages");
     if (n_pages < 0 || block_size < 1) return fail(DROPKV_ERR_ARG, "invalid pool: %d pages of %d rows", n_pages, block_size);
+    settle_strides(B, Hkv, L, D, &v_sb, &v_sh, &v_sl);
+    settle_strides(n_pages, Hkv, block_size, D, &kp_sb, &kp_sh, &kp_st);
+    settle_strides(n_pages, Hkv, block_size, D, &vp_sb, &vp_sh, &vp_st);
   }
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(k_pages) |
@@ -718,6 +735,8 @@ int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_s
       return fail(DROPKV_ERR_ARG, "cap must be max_blocks * block_size");
   }
   const bool rows = cap > 0 && (!table || n_pages > 0);
+  settle_strides(table ? n_pages : B, Hkv, table ? block_size : cap, D, &k_s0, &k_sh, &k_ss);
+  settle_strides(table ? n_pages : B, Hkv, table ? block_size : cap, D, &v_s0, &v_sh, &v_ss);
   if (rows && (!k || !v)) return fail(DROPKV_ERR_ARG, "K and V must be non-NULL");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 ||
       ((k_s0 | k_sh | k_ss | v_s0 | v_sh | v_ss) * 2) % 16)

@@ -331,15 +331,16 @@ __device__ __forceinline__ void lp_top_chunk(LpSmem& sm, LpCandidates& cand, con
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, int vecs_per_cta) {
+__global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, int vecs_per_cta, int row0, int last) {
   constexpr int N = LpVec<T>::N, U = LpVec<T>::U, E = N * U;
   static_assert(E <= LP_MAX_E, "candidates of a thread");
   extern __shared__ __align__(16) uint8_t raw[];
   LpSmem& sm = *reinterpret_cast<LpSmem*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / split;
+  const int64_t row = row0 + blockIdx.x / split;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!last) pdl_launch_dependents();
   const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
   // The row in vectors of 16 bytes from its first logit on, whatever its address: a thread's
   // logits, and so the order of every sum, do not depend on it. Loads are aligned; where the
@@ -442,9 +443,9 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
         lp_top_chunk<T>(sm, cand, cur, x0, a.V, v0, v_end, mx, a.top_k);
       } else {
         // no barrier in an ordinary chunk: warps add what reaches the threshold, and now and
-        // then (after 2, 4, 8, ... chunks) the list is cut and the threshold moves up to it
+        // then (after 4, 16 and 64 chunks) the list is cut and the threshold moves up to it
         lp_collect<T>(sm, cand.floor_key, cur, x0, a.V, v0, v_end, mx);
-        if ((chunk & (chunk + 1)) == 0) {
+        if (chunk == 3 || chunk == 15 || chunk == 63) {
           __syncthreads();
           const int n = sm.count;
           if (n > cand.kept && n <= LP_CAP) lp_cut(sm, cand, n, a.top_k);
@@ -498,6 +499,7 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
     if (TOP)
       for (int i = tid; i < a.top_k; i += LP_NT) first->lists[part * a.top_k + i] = i < cand.kept ? sm.list[i] : 0;
     cluster.sync();
+    if (last) pdl_wait();  // (below, for the others)
     if (part != 0) return;
     own = sm.parts[0];
     for (int p = 1; p < split; ++p) own = lp_join(own, sm.parts[p], c);
@@ -506,6 +508,9 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
       lp_keep_best(sm.list, split * a.top_k, a.top_k);
     }
   }
+  // The second launch of a call ends after the first: what comes after on the stream takes
+  // its end for the end of both.
+  if (last && split == 1) pdl_wait();
   const float ls = log2f(own.s), ln2 = 0.69314718055994531f;
   auto logprob = [&](float v) { return fmaf(v - own.m, a.inv_temperature, -ln2 * ls); };
   if (tid == 0) a.entropy[row] = ln2 * (ls - own.t / own.s);
@@ -520,40 +525,57 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
   }
 }
 
+// Rows [row0, row0 + rows), each by a cluster of `split` CTAs; beside the launch before this
+// one, if it is the second of a call.
+template <typename T, bool TOP>
+int lp_rows(const Logprobs& a, int64_t row0, int64_t rows, int split, bool second, cudaStream_t st) {
+  constexpr int N = LpVec<T>::N;
+  const int per = (int)((((int64_t)a.V + N - 1) / N + split - 1) / split);
+  auto kern = logprobs_kernel<T, TOP>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = second ? 2 : 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(rows * split));
+  cfg.blockDim = dim3(LP_NT);
+  cfg.dynamicSmemBytes = sizeof(LpSmem);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, per, (int)row0, (int)second);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
+  return check_launch("token_logprobs");
+}
+
 template <typename T, bool TOP>
 int lp_launch(const Logprobs& a, cudaStream_t st) {
-  // CTAs a row, by the waves of CTAs and what one costs: its chunks, and what its start and end
-  // take, about 8 chunks with alternatives and 2 without (2048 x 151936 bf16, top 20: 234 us in
-  // halves, PROMPT1 whole; 16 x 50257 fp16, top 5: STEP1 us whole, 10 in quarters). A CTA takes one chunk at least.
-  constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
-  const int64_t vecs = ((int64_t)a.V + N - 1) / N;
+  // Whole waves of CTAs take a row each; the rows that are left are split over clusters so
+  // that their wave is full and short. They go in a launch of their own, which starts as
+  // the first one's CTAs leave (2048 x 151936 bf16, top 20: 178 -> 160 us).
   const int64_t slots = (int64_t)LP_CTAS * num_sms_current_device();
+  if (a.N > 0x7fffffff - slots) return fail(DROPKV_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  const int64_t whole = a.N / slots * slots;
+  if (whole) {
+    const int rc = lp_rows<T, TOP>(a, 0, whole, 1, false, st);
+    if (rc || whole == a.N) return rc;
+  }
+  // CTAs a row: by the waves of CTAs and what one costs, its chunks and what its start and end
+  // take, about 8 chunks with alternatives and 2 without. A CTA takes one chunk at least.
+  constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
+  const int64_t vecs = ((int64_t)a.V + N - 1) / N, rest = a.N - whole;
   int split = 1;
   double best = 1e30;
   for (int s = 1; s <= LP_MAX_S; s *= 2) {
     const int64_t share = (vecs + s - 1) / s;
     if (s > 1 && share < U * LP_NT) break;
-    const double cost = (double)((a.N * s + slots - 1) / slots) * ((double)share / (U * LP_NT) + (TOP ? 8 : 2));
+    const double cost = (double)((rest * s + slots - 1) / slots) * ((double)share / (U * LP_NT) + (TOP ? 8 : 2));
     if (cost < best) best = cost, split = s;
   }
-  const int per = (int)((vecs + split - 1) / split);
-  if (a.N * split > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "token_logprobs: too many rows");
-  auto kern = logprobs_kernel<T, TOP>;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cfg.stream = st;
-  cfg.gridDim = dim3((unsigned)(a.N * split));
-  cfg.blockDim = dim3(LP_NT);
-  cfg.dynamicSmemBytes = sizeof(LpSmem);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, per);
-  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
-  return check_launch("token_logprobs");
+  return lp_rows<T, TOP>(a, whole, rest, split, whole > 0, st);
 }
 
 }  // namespace

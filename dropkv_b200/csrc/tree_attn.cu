@@ -917,7 +917,12 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(const __grid_con
   const int rt = seg % A.RT, h = seg / A.RT;
   const int rb = blockIdx.y / (D / 32), cb = blockIdx.y % (D / 32);
   const int row = rb * 32 + lane, mrow = rt * TA_ROWS + row;
-  if (rt * TA_ROWS + rb * 32 >= A.M) return;
+  // Every CTA waits for the kernel before this one before it ends, with work or without: what
+  // comes after on the stream takes this kernel's end for the end of both.
+  if (rt * TA_ROWS + rb * 32 >= A.M) {
+    pdl_wait();
+    return;
+  }
   // the lengths were there before the kernel whose partials these are began: no wait yet
   int before = 0, total = 0;
   for (int i = tid; i < a.B; i += TM_NT) {
@@ -938,7 +943,10 @@ __global__ void __launch_bounds__(TM_NT) tree_attn_merge_kernel(const __grid_con
   const int per = (total * A.HR + ctas - 1) / ctas, tiles = ta_tiles(a, b);
   const int w0 = before * A.HR + seg * (tiles + kTaLead) + kTaLead, w1 = w0 + tiles;
   const int c0 = w0 / per, n = (w1 - 1) / per - c0 + 1;
-  if (n == 1) return;  // written by its one CTA
+  if (n == 1) {  // written by its one CTA
+    pdl_wait();
+    return;
+  }
   // partial i is CTA c0 + i's: the segment is the last piece of the first CTA, the first of the others
   auto slot = [&](int i) { return (int64_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
   const bool own = row < A.rows_pad && mrow < A.M;

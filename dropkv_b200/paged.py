@@ -84,19 +84,12 @@ def _ints(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> torch
 
 
 def _rows_strides(t: torch.Tensor, what: str):
-    """Strides of the three outer dimensions of [A, B, C, D] rows; a dimension of one
-    takes the packed stride, which its own cannot contradict."""
-    a, b, c, d = t.shape
-    s0, s1, s2, s3 = t.stride()
-    if s3 != 1 and d > 1:
+    """Strides of the three outer dimensions of [A, B, C, D] rows (the library takes the
+    packed one for a dimension of one)."""
+    s = t.stride()
+    if s[3] != 1 and t.shape[3] > 1:
         raise ValueError(f"{what} needs rows of D contiguous elements")
-    if c <= 1:
-        s2 = d
-    if b <= 1:
-        s1 = c * s2
-    if a <= 1:
-        s0 = max(b * s1, c * s2)
-    return s0, s1, s2
+    return s[:3]
 
 
 def _check_pool(K_pages, V_pages, Hkv, D, dtype):

@@ -131,6 +131,20 @@ def test_rows_beyond_32_bits():
     _check(x, torch.tensor([5, 39999], device="cuda"), 4)
 
 
+def test_more_rows_than_a_wave_of_ctas_and_the_next_kernel():
+    # the rows past whole waves go in a second launch beside the first: both have ended for the next
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(1500, 20000, generator=g, device="cuda").bfloat16()
+    t = torch.randint(0, 20000, (1500,), generator=g, device="cuda")
+    want = _check(x, t, 5)
+    for _ in range(10):
+        got = token_logprobs(x, t, top_k=5)
+        copies = [y.clone() for y in got]
+        for y in got:
+            y.zero_()
+        assert all(torch.equal(a, b) for a, b in zip(copies, want))
+
+
 def test_on_another_stream():
     x = torch.randn(7, 9000, device="cuda")
     t = torch.arange(7, device="cuda")

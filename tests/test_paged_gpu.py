@@ -255,6 +255,22 @@ def test_calls_on_another_stream():
     assert torch.equal(Kp[t.table[0].long()].transpose(0, 1).reshape(2, 64, 64), K[0])
 
 
+def test_dimensions_of_one_may_have_any_stride():
+    g = torch.Generator(device="cuda").manual_seed(8)
+    odd = lambda t: t.as_strided(t.shape, [7 if n == 1 else s for n, s in zip(t.shape, t.stride())])  # noqa: E731
+    K, V = torch.randn(2, 1, 1, 5, 64, generator=g, device="cuda").half()
+    slots = torch.tensor([[3, 1, -1, 0, 2]], device="cuda")
+    a = [torch.zeros(1, 1, 16, 64, device="cuda").half() for _ in range(4)]
+    store_rows(odd(K), odd(V), slots, odd(a[0]), odd(a[1]))
+    store_rows(K, V, slots, a[2], a[3])
+    assert torch.equal(a[0], a[2]) and torch.equal(a[1], a[3]) and bool((a[0] != 0).any())
+    ang = torch.rand(9, 32, generator=g, device="cuda")
+    pos = torch.arange(5, device="cuda")
+    q, k = qk_norm_rope(odd(K), odd(V), ang.cos(), ang.sin(), pos)
+    q2, k2 = qk_norm_rope(K, V, ang.cos(), ang.sin(), pos)
+    assert torch.equal(q, q2) and torch.equal(k, k2)
+
+
 def test_refusals():
     x = torch.zeros(1, 2, 3, 64, device="cuda").half()
     pool = torch.zeros(2, 2, 16, 64, device="cuda").half()

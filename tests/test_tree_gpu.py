@@ -182,6 +182,12 @@ def test_row_buffers_with_spare_capacity_and_garbage_past_the_rows():
     assert torch.equal(got, tree_attention(strided[..., ::2], K, V, n, tree_mask=mask))
 
 
+def test_dimensions_of_one_may_have_any_stride():
+    Q, K, V, n = _inputs(1, 4, 1, 1, 64, [60], torch.bfloat16, seed=13)
+    odd = lambda t: t.as_strided(t.shape, [5 if m == 1 else s for m, s in zip(t.shape, t.stride())])  # noqa: E731
+    assert torch.equal(tree_attention(Q, K, V, n), tree_attention(odd(Q), odd(K), odd(V), n))
+
+
 def test_mask_of_any_strides():
     Q, K, V, n = _inputs(2, 8, 4, 10, 64, [50, 200], torch.bfloat16, seed=3)
     mask = _random_tree(10, torch.Generator().manual_seed(3), 2).cuda()
@@ -297,6 +303,22 @@ def test_on_another_stream_and_in_a_graph():
     n.copy_(torch.tensor([33, 694], dtype=torch.int32))     # lengths are read when the graph runs
     graph.replay()
     assert torch.equal(c, tree_attention(Q, K, V, n))
+
+
+def test_outputs_are_there_for_the_next_kernel():
+    # caches of one tile in long buffers: there is nothing to join, and the kernel that would join
+    # must not end, and let the next one on the stream begin, before the outputs are written
+    lens = [100, 3, 77, 90, 1, 60, 99, 50]
+    Q, K, V, n = _inputs(8, 32, 8, 20, 128, lens, torch.bfloat16, seed=14, cap=4096)
+    want = tree_attention(Q, K, V, n)
+    torch.cuda.synchronize()
+    copies = []
+    for _ in range(60):
+        out = tree_attention(Q, K, V, n)
+        copies.append(out.clone())
+        out.zero_()
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, want) for c in copies)
 
 
 def test_empty_batch():
