@@ -23,7 +23,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .ops import _CHECK_STATUS, _DTYPE_CODE, _workspace
+from .ops import _CHECK_STATUS, _DTYPE_CODE
 
 __all__ = ["BlockTables", "TokenLogprobs", "block_tables", "store_rows", "qk_norm_rope", "tree_attention",
            "token_logprobs", "tree_mask_from_parents"]
@@ -47,6 +47,23 @@ class TokenLogprobs(NamedTuple):
 # a call whose kernel takes 3.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _new(dtype: torch.dtype, device: torch.device, *shape: int) -> torch.Tensor:
+    """An uninitialised contiguous tensor (of up to four dimensions). empty_strided takes 1.5 us
+    where empty takes 2.3 to 3."""
+    n = len(shape)
+    if n == 2:
+        stride = (shape[1], 1)
+    elif n == 1:
+        stride = (1,)
+    elif n == 4:
+        stride = (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1)
+    elif n == 3:
+        stride = (shape[1] * shape[2], shape[2], 1)
+    else:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty_strided(shape, stride, dtype=dtype, device=device)
 
 
 def _on_one_device(*ts) -> int:
@@ -142,10 +159,8 @@ def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor,
         table = _ints(table, torch.int32, (B, max_blocks), "table")
         held = _ints(held, torch.int32, (B,), "held")
         table_ptr, held_ptr = table.data_ptr(), held.data_ptr()
-    out = BlockTables(torch.empty((B, max_blocks), dtype=torch.int32, device=device),
-                      torch.empty(B, dtype=torch.int32, device=device),
-                      torch.empty((B, max_new), dtype=torch.int64, device=device),
-                      torch.empty(1, dtype=torch.int64, device=device))
+    out = BlockTables(_new(torch.int32, device, B, max_blocks), _new(torch.int32, device, B),
+                      _new(torch.int64, device, B, max_new), _new(torch.int64, device, 1))
     if B == 0:
         out.used.zero_()
         return out
@@ -238,8 +253,8 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
                 K_pages.shape[0], K_pages.shape[2])
     else:
         tail = (None, 0, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, 0, 1)
-    q_out = torch.empty((B, Hq, L, D), dtype=dtype, device=Q.device)
-    k_out = torch.empty((B, Hkv, L, D), dtype=dtype, device=Q.device)
+    q_out = _new(dtype, Q.device, B, Hq, L, D)
+    k_out = _new(dtype, Q.device, B, Hkv, L, D)
     rc = _lib.load().dropkv_qk_norm_rope(
         Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
         q_weight.data_ptr() if q_weight is not None else None,
@@ -313,11 +328,11 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
                 tree_mask.stride(-1))
     scale = float(D ** -0.5 if scale is None else scale)
     lib = _lib.load()
-    out = torch.empty(B, Hq, T, D, dtype=Q.dtype, device=Q.device)
+    out = _new(Q.dtype, Q.device, B, Hq, T, D)
     if B == 0 or T == 0:
         return out
     # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
-    ws = _workspace(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), Q.device)
+    ws = _new(torch.uint8, Q.device, max(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), 1))
     rc = lib.dropkv_tree_attention(
         Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
         *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
@@ -357,12 +372,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     N, top_k = rows.shape[0], int(top_k)
     C = tokens.shape[-1] if tokens.dim() == logits.dim() else 1
     tokens = tokens.contiguous()
-    logprob = torch.empty(tokens.shape, dtype=torch.float32, device=device)
-    entropy = torch.empty(lead, dtype=torch.float32, device=device)
+    logprob = _new(torch.float32, device, *tokens.shape)
+    entropy = _new(torch.float32, device, *lead)
     top_lp = top_id = None
     if top_k > 0:
-        top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=device)
-        top_id = torch.empty((*lead, top_k), dtype=torch.int64, device=device)
+        top_lp = _new(torch.float32, device, *lead, top_k)
+        top_id = _new(torch.int64, device, *lead, top_k)
     lib = _lib.load()
     rc = lib.dropkv_token_logprobs(rows.data_ptr(), rows.stride(0), dt, N, V, tokens.data_ptr(), C, top_k,
                                    float(temperature), logprob.data_ptr(), entropy.data_ptr(),
