@@ -87,25 +87,89 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
 // of Q), are fetched once and stay in registers, and QR_BATCH rows are on their way at a time.
 constexpr int QR_BATCH = 3;
 
+// Two floats in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t qr_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void qr_unpair(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t qr_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t qr_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 16 bytes of a row as pairs of floats.
 template <typename T>
-struct QrVec {
-  static constexpr int N = 16 / sizeof(T);
-  static __device__ __forceinline__ void get(const uint4& v, float* x) {
-    const T* p = reinterpret_cast<const T*>(&v);
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f(p[i]);
+struct QrVec;
+template <>
+struct QrVec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& v, uint64_t* x) {
+    x[0] = qr_pair(__uint_as_float(v.x), __uint_as_float(v.y));
+    x[1] = qr_pair(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ uint4 put(const float* x) {
-    uint4 v;
-    T* p = reinterpret_cast<T*>(&v);
+  static __device__ __forceinline__ uint4 put(const uint64_t* x) {
+    float a, b, c, d;
+    qr_unpair(x[0], a, b);
+    qr_unpair(x[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+  }
+};
+template <>
+struct QrVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, uint64_t* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = qr_from<T>(x[i]);
-    return v;
+    for (int i = 0; i < 4; ++i) x[i] = qr_pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 put(const uint64_t* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      qr_unpair(x[i], a, b);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+      w[i] = reinterpret_cast<const uint32_t&>(h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct QrVec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, uint64_t* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+      x[i] = qr_pair(f.x, f.y);
+    }
+  }
+  static __device__ __forceinline__ uint4 put(const uint64_t* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      qr_unpair(x[i], a, b);
+      const __half2 h = __floats2half2_rn(a, b);
+      w[i] = reinterpret_cast<const uint32_t&>(h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-template <typename T, int G, bool INTERLEAVED>
-__global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens, int hpg) {
+template <typename T, int G, bool INTERLEAVED, bool NORM>
+__global__ void __launch_bounds__(QR_NT, 7) qk_rope_vec_kernel(QkRope a, int tokens, int hpg) {
   constexpr int N = QrVec<T>::N, GROUPS = QR_NT / G;
   const int heads = a.Hq + a.Hkv + (a.slots ? a.Hkv : 0);
   const int64_t gid = (int64_t)blockIdx.x * GROUPS + threadIdx.x / G;
@@ -113,6 +177,7 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens
   const unsigned bl = idle ? 0u : (unsigned)(gid / (unsigned)hpg);
   const int b = (int)(bl / (unsigned)a.L), l = (int)(bl - (unsigned)b * (unsigned)a.L);
   const int u = threadIdx.x % G, step = hpg;
+  const float inv_d = 1.f / a.D;  // (D is a power of two here)
   const int h0 = idle ? heads : (int)(gid - (int64_t)bl * hpg);
   // this lane's elements: [lo, lo + N) and [hi, hi + N)
   const int turning = a.R / (2 * N);  // units that turn
@@ -146,19 +211,29 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens
     }
   };
   load(h0);
-  // cosines and sines of the lane's N pairs (interleaved: N / 2 of each vector)
+  // cosines and sines of the lane's N pairs; interleaved, N / 2 pairs of each vector: (c, c) and (-s, s)
   const bool known = pos >= 0 && pos < a.P;  // a position outside the tables gives NaN
-  float cs[N], sn[N];
+  uint64_t cs[INTERLEAVED ? N : N / 2], sn[INTERLEAVED ? N : N / 2];
+  {
+    float c[N], s[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) cs[i] = turns ? NAN : 1.f, sn[i] = turns ? NAN : 0.f;
-  if (turns && known) {
-    const float* c = a.cos + pos * (a.R / 2) + N * u;
-    const float* s = a.sin + pos * (a.R / 2) + N * u;
+    for (int i = 0; i < N; ++i) c[i] = s[i] = NAN;
+    if (turns && known) {
+      const float* pc = a.cos + pos * (a.R / 2) + N * u;
+      const float* ps = a.sin + pos * (a.R / 2) + N * u;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(c + i), y = *reinterpret_cast<const float4*>(s + i);
-      cs[i] = x.x, cs[i + 1] = x.y, cs[i + 2] = x.z, cs[i + 3] = x.w;
-      sn[i] = y.x, sn[i + 1] = y.y, sn[i + 2] = y.z, sn[i + 3] = y.w;
+      for (int i = 0; i < N; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(pc + i), y = *reinterpret_cast<const float4*>(ps + i);
+        c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
+        s[i] = y.x, s[i + 1] = y.y, s[i + 2] = y.z, s[i + 3] = y.w;
+      }
+    }
+    if (INTERLEAVED) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) cs[i] = qr_pair(c[i], c[i]), sn[i] = qr_pair(-s[i], s[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) cs[i] = qr_pair(c[2 * i], c[2 * i + 1]), sn[i] = qr_pair(s[2 * i], s[2 * i + 1]);
     }
   }
   T* kp = nullptr;
@@ -177,23 +252,30 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens
     for (int i = 0; i < QR_BATCH; ++i) {
       const int hh = h + i * step;
       const bool there = hh < heads, is_q = hh < a.Hq, is_v = hh >= a.Hq + a.Hkv;
-      float x[N], y[N];
+      uint64_t x[N / 2], y[N / 2];
       QrVec<T>::get(va[i], x);
       QrVec<T>::get(vb[i], y);
-      if (a.q_weight || a.k_weight) {
-        float ss = 0.f;
+      if (NORM) {
+        uint64_t ss2 = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], fmaf(y[e], y[e], ss));
+        for (int e = 0; e < N / 2; ++e) ss2 = qr_fma2(x[e], x[e], qr_fma2(y[e], y[e], ss2));
+        float ss, s1;
+        qr_unpair(ss2, ss, s1);
+        ss += s1;
 #pragma unroll
         for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
         if (there && !is_v && w) {
-          const float inv = rsqrtf(ss / a.D + a.eps);
-          float wx[N], wy[N];  // (from L1: held in registers they cost occupancy, 24 -> 33 us)
+          const float inv = rsqrtf(ss * inv_d + a.eps);
+          const uint64_t inv2 = qr_pair(inv, inv);
+          uint64_t wx[N / 2], wy[N / 2];  // (from L1: held in registers they cost occupancy, 24 -> 33 us)
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + lo), wx);
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + hi), wy);
 #pragma unroll
-          for (int e = 0; e < N; ++e) x[e] = x[e] * inv * wx[e], y[e] = y[e] * inv * wy[e];
+          for (int e = 0; e < N / 2; ++e) {
+            x[e] = qr_mul2(qr_mul2(x[e], inv2), wx[e]);
+            y[e] = qr_mul2(qr_mul2(y[e], inv2), wy[e]);
+          }
         }
       }
       if (!there) continue;
@@ -205,21 +287,23 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_vec_kernel(QkRope a, int tokens
         }
         continue;
       }
-      if (INTERLEAVED) {
+      if (!turns) {  // (untouched, not times one: infinities stay)
+      } else if (INTERLEAVED) {
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float p = x[e], q = x[e + 1], r = y[e], s = y[e + 1];
-          x[e] = p * cs[e / 2] - q * sn[e / 2];
-          x[e + 1] = q * cs[e / 2] + p * sn[e / 2];
-          y[e] = r * cs[(N + e) / 2] - s * sn[(N + e) / 2];
-          y[e + 1] = s * cs[(N + e) / 2] + r * sn[(N + e) / 2];
+        for (int e = 0; e < N / 2; ++e) {
+          float p, q;
+          qr_unpair(x[e], p, q);
+          x[e] = qr_fma2(qr_pair(q, p), sn[e], qr_mul2(x[e], cs[e]));
+          qr_unpair(y[e], p, q);
+          y[e] = qr_fma2(qr_pair(q, p), sn[N / 2 + e], qr_mul2(y[e], cs[N / 2 + e]));
         }
       } else {
+        const uint64_t minus = qr_pair(-1.f, -1.f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float p = x[e], q = y[e];
-          x[e] = p * cs[e] - q * sn[e];
-          y[e] = q * cs[e] + p * sn[e];
+        for (int e = 0; e < N / 2; ++e) {
+          const uint64_t p = x[e], q = y[e];
+          x[e] = qr_fma2(qr_mul2(q, sn[e]), minus, qr_mul2(p, cs[e]));
+          y[e] = qr_fma2(p, sn[e], qr_mul2(q, cs[e]));
         }
       }
       const uint4 ox = QrVec<T>::put(x), oy = QrVec<T>::put(y);
@@ -255,19 +339,23 @@ int qr_launch(const QkRope& a, cudaStream_t st) {
   const bool lanes = G == 2 || G == 4 || G == 8 || G == 16 || G == 32;
   const int64_t tokens = (int64_t)a.B * a.L;
   if (bits % 16 == 0 && lanes && a.R % (2 * N) == 0 && tokens <= 0x7fffffff) {
-    // a group takes QR_BATCH rows of its token where that still fills the device, else one row
+    // a group takes up to QR_BATCH rows of its token, fewer where that would leave SMs short of CTAs
     const int few = (heads + QR_BATCH - 1) / QR_BATCH;
     const int64_t want = 4 * (int64_t)num_sms_current_device() * (QR_NT / G);
-    const int hpg = tokens * few >= want ? few : heads;
+    const int64_t fill = (want + tokens - 1) / tokens;
+    const int hpg = fill < few ? few : fill < heads ? (int)fill : heads;
     const int64_t ctas = (tokens * hpg * G + QR_NT - 1) / QR_NT;
     if (ctas > 0x7fffffff) return fail(DROPKV_ERR_UNSUPPORTED, "qk_norm_rope: too many rows");
     const dim3 grid((unsigned)ctas);
     auto run = [&](auto g) {
       constexpr int GG = decltype(g)::value;
+      const bool norm = a.q_weight || a.k_weight;
       if (a.interleaved)
-        qk_rope_vec_kernel<T, GG, true><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
+        norm ? qk_rope_vec_kernel<T, GG, true, true><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg)
+             : qk_rope_vec_kernel<T, GG, true, false><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
       else
-        qk_rope_vec_kernel<T, GG, false><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
+        norm ? qk_rope_vec_kernel<T, GG, false, true><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg)
+             : qk_rope_vec_kernel<T, GG, false, false><<<grid, QR_NT, 0, st>>>(a, (int)tokens, hpg);
     };
     switch (G) {
       case 2: run(std::integral_constant<int, 2>()); break;

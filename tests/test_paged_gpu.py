@@ -243,6 +243,27 @@ def test_qk_norm_rope_norms_zeros_and_one_side_only():
     assert bool((q == 0).all()) and torch.equal(k, y)     # zeros stay zeros; K has no norm
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,interleaved", [(128, False), (128, True), (80, False)])
+def test_qk_norm_rope_what_does_not_turn_stays(D, interleaved, dtype):
+    """Elements behind the rotation come through bit by bit, infinities, NaN and -0 among them,
+    and reach no other element."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    R, L = 32, 9
+    Q = torch.randn(1, 6, L, D, generator=g, device="cuda").to(dtype)
+    Q[0, 0, :, R:] = float("inf")
+    Q[0, 1, :, R + 1::2] = float("nan")
+    Q[0, 2, :, R::3] = -0.0
+    K = Q[:, :2].clone()
+    ang = torch.rand(L, R // 2, generator=g, device="cuda") * 6
+    q, k = qk_norm_rope(Q, K, ang.cos(), ang.sin(), torch.arange(L, device="cuda"), interleaved=interleaved)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    assert torch.equal(q[..., R:].isnan(), Q[..., R:].isnan()) and bool(q[..., :R].isfinite().all())
+    keep = ~Q[..., R:].isnan()
+    assert torch.equal(q[..., R:].view(bits)[keep], Q[..., R:].contiguous().view(bits)[keep])
+    assert torch.equal(k.view(bits), q[:, :2].contiguous().view(bits))
+
+
 def test_calls_on_another_stream():
     side = torch.cuda.Stream()
     K = torch.randn(1, 2, 64, 64, device="cuda").half()
