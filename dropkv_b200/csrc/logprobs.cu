@@ -17,15 +17,15 @@ namespace cg = cooperative_groups;
 namespace dropkv {
 namespace {
 
-constexpr int LP_NT = 256;
+constexpr int LP_NT = 128;
 constexpr int LP_WARPS = LP_NT / 32;
-constexpr int LP_CTAS = 4;                      // CTAs an SM holds
+constexpr int LP_CTAS = 8;                      // CTAs an SM holds
 constexpr int LP_MAX_K = 64;
-constexpr int LP_MAX_E = 32;                    // logits of a thread and chunk, at most
-constexpr int LP_CAP = LP_MAX_K * (1 + LP_MAX_E);  // candidates: a full list and all of top_k threads
+constexpr int LP_CAP = 1024;                    // candidates
 constexpr int LP_MAX_S = 8;                     // CTAs of a cluster, at most
-constexpr int LP_GROUPS = 64;                   // groups of four threads
-static_assert(LP_GROUPS >= LP_MAX_K && LP_NT == 4 * LP_GROUPS, "the top_k-th of the groups' best");
+constexpr int LP_GROUPS = 64;                   // groups of threads
+constexpr int LP_GT = LP_NT / LP_GROUPS;        // threads of a group
+static_assert(LP_GROUPS >= LP_MAX_K && LP_NT == LP_GT * LP_GROUPS && 32 % LP_GT == 0, "the top_k-th of the groups' best");
 
 // Order of the alternatives: larger logits first (NaN above all), then lower index. 0 is
 // below every logit's key.
@@ -223,6 +223,33 @@ __device__ __forceinline__ int lp_place(int bit, float) { return bit; }
 __device__ __forceinline__ int lp_place(int bit, __nv_bfloat16) { return 2 * (bit & 15) + (bit >> 4); }
 __device__ __forceinline__ int lp_place(int bit, __half) { return 2 * (bit & 15) + (bit >> 4); }
 
+// and its value: registers have no index, but a tree of selects
+template <int U>
+__device__ __forceinline__ uint32_t lp_word(const uint4* v, int i) {
+  static_assert(U == 4, "16 words");
+  uint32_t w[8];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    w[2 * u] = i & 1 ? v[u].y : v[u].x;
+    w[2 * u + 1] = i & 1 ? v[u].w : v[u].z;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) w[u] = i & 2 ? w[2 * u + 1] : w[2 * u];
+  return i & 8 ? (i & 4 ? w[3] : w[2]) : (i & 4 ? w[1] : w[0]);
+}
+template <int U>
+__device__ __forceinline__ float lp_pick(const uint4* v, int bit, float) { return __uint_as_float(lp_word<U>(v, bit)); }
+template <int U>
+__device__ __forceinline__ float lp_pick(const uint4* v, int bit, __nv_bfloat16) {
+  const uint32_t w = lp_word<U>(v, bit & 15);
+  return __uint_as_float(bit & 16 ? w & 0xffff0000u : w << 16);
+}
+template <int U>
+__device__ __forceinline__ float lp_pick(const uint4* v, int bit, __half) {
+  const uint32_t w = lp_word<U>(v, bit & 15);
+  return __half2float(__ushort_as_half((unsigned short)(bit & 16 ? w >> 16 : w)));
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 lp_lowest();
 template <>
@@ -242,30 +269,23 @@ __device__ __forceinline__ float lp_floor_value(uint64_t key) {  // what a logit
   return key ? lp_value(key) : __int_as_float(0xff800000);
 }
 
-// f(key) for each of a thread's logits in the chunk that reaches the threshold's value. A bit for
-// each of them first, then the few that are set, read again (they are in a cache).
-template <typename T, typename F>
-__device__ __forceinline__ void lp_look(uint64_t floor_key, const uint4* cur, const T* x0, int V, int v0, int v_end, float mx,
-                                        F f) {
+// The logits of the chunk that reach the threshold go to the list, while there is room; all are
+// counted. A bit for each of a thread's logits first, then the few that are set.
+template <typename T>
+__device__ __forceinline__ void lp_collect(LpSmem& sm, uint64_t floor_key, const uint4* cur, int V, int v0, int v_end, float mx) {
   constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
   const float fv = lp_floor_value(floor_key);
   if (!__any_sync(0xffffffffu, !(mx < fv))) return;
   for (uint32_t bits = lp_reach<U>(cur, fv, T()); bits; bits &= bits - 1) {
-    const int q = lp_place(__ffs(bits) - 1, T()), v = v0 + (q / N) * LP_NT + (int)threadIdx.x;
+    const int b = __ffs(bits) - 1, q = lp_place(b, T()), v = v0 + (q / N) * LP_NT + (int)threadIdx.x;
     const int64_t e = (int64_t)v * N + q % N;
-    if (v < v_end && e < V) f(lp_key(to_f(x0[e]), (int)e));
-  }
-  __syncwarp();
-}
-// Those that reach it go to the list, while there is room; all are counted.
-template <typename T>
-__device__ __forceinline__ void lp_collect(LpSmem& sm, uint64_t floor_key, const uint4* cur, const T* x0, int V, int v0,
-                                           int v_end, float mx) {
-  lp_look<T>(floor_key, cur, x0, V, v0, v_end, mx, [&](uint64_t key) {
-    if (key < floor_key) return;
+    if (v >= v_end || e >= V) continue;
+    const uint64_t key = lp_key(lp_pick<U>(cur, b, T()), (int)e);
+    if (key < floor_key) continue;
     const int at = atomicAdd(&sm.count, 1);
     if (at < LP_CAP) sm.list[at] = key;
-  });
+  }
+  __syncwarp();
 }
 // The list of n entries cut to the best top_k, and the threshold moved up to the last of them.
 // All threads; ends without a barrier.
@@ -277,52 +297,72 @@ __device__ __forceinline__ void lp_cut(LpSmem& sm, LpCandidates& cand, int n, in
 
 // A chunk whose candidates may be many: the threshold is raised from the chunk itself first.
 template <typename T>
-__device__ __forceinline__ void lp_top_chunk(LpSmem& sm, LpCandidates& cand, const uint4* cur, const T* x0, int V, int v0,
-                                             int v_end, float mx, int k) {
+__device__ __forceinline__ void lp_top_chunk(LpSmem& sm, LpCandidates& cand, const uint4* cur, const T* x0, int V, int v0, int v_end,
+                                             float mx, int k) {
   const int tid = threadIdx.x;
-  // The k-th of the best of 64 groups of four threads is a threshold that k logits reach, and
-  // few more. A group's four threads count a quarter each of the groups above theirs. (Padding
+  // The k-th of the best of 64 groups of threads is a threshold that k logits reach, and
+  // few more. A group's threads share out the groups to compare theirs with. (Padding
   // counts as -inf, which every logit reaches.)
   uint32_t best = mx != mx ? 0xffffffffu : ordered_key(mx);
-  best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
-  best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
-  if (tid % 4 == 0) sm.groups[tid / 4] = best;
+#pragma unroll
+  for (int o = 1; o < LP_GT; o *= 2) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (tid % LP_GT == 0) sm.groups[tid / LP_GT] = best;
   __syncthreads();
   int over = 0, same = 0;
 #pragma unroll
-  for (int q = 0; q < LP_GROUPS / 4; q += 4) {
-    const uint4 g = *reinterpret_cast<const uint4*>(&sm.groups[(tid % 4) * (LP_GROUPS / 4) + q]);
+  for (int q = 0; q < LP_GROUPS / LP_GT; q += 4) {
+    const uint4 g = *reinterpret_cast<const uint4*>(&sm.groups[(tid % LP_GT) * (LP_GROUPS / LP_GT) + q]);
     over += (g.x > best) + (g.y > best) + (g.z > best) + (g.w > best);
     same += (g.x == best) + (g.y == best) + (g.z == best) + (g.w == best);
   }
-  over += __shfl_xor_sync(0xffffffffu, over, 1);
-  over += __shfl_xor_sync(0xffffffffu, over, 2);
-  same += __shfl_xor_sync(0xffffffffu, same, 1);
-  same += __shfl_xor_sync(0xffffffffu, same, 2);
+#pragma unroll
+  for (int o = 1; o < LP_GT; o *= 2) {
+    over += __shfl_xor_sync(0xffffffffu, over, o);
+    same += __shfl_xor_sync(0xffffffffu, same, o);
+  }
   if (over < k && over + same >= k) sm.level = best;  // (all that write it have one value)
   __syncthreads();
   const uint64_t least = (uint64_t)sm.level << 32;  // the lowest key of that value
   if (least > cand.floor_key) cand.floor_key = least;
-  lp_collect<T>(sm, cand.floor_key, cur, x0, V, v0, v_end, mx);
+  lp_collect<T>(sm, cand.floor_key, cur, V, v0, v_end, mx);
   __syncthreads();
   if (sm.count > LP_CAP) {
-    // Too many (logits in an order that defeats the groups). The exact k-th of the threads' best
-    // keys is a threshold that all but k threads stay below; with the list before this chunk cut
-    // to k, whatever they hold fits.
-    uint64_t top = 0;
-    lp_look<T>(cand.floor_key, cur, x0, V, v0, v_end, mx, [&](uint64_t key) { top = max(top, key); });
+    // Too many (logits in an order that defeats the groups). With the list as it was before this
+    // chunk, cut to k, each thread's first vector is taken, then its second, and so on: the exact
+    // k-th of the threads' best keys is a threshold that all but k threads stay below, and
+    // whatever these hold in a vector fits. (The logits are read again: registers have no index.)
+    constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
+    static_assert(LP_CAP >= LP_MAX_K * (1 + N), "a list and a vector of k threads");
     __syncthreads();
     lp_cut(sm, cand, cand.kept, k);
-    sm.tops[tid] = top;
-    if (tid == 0) sm.edge = 0;
-    __syncthreads();
-    int r = 0;
-    for (int e = 0; e < LP_NT; ++e) r += sm.tops[e] > top;
-    if (r == k - 1 && top) sm.edge = top;
-    __syncthreads();
-    if (sm.edge > cand.floor_key) cand.floor_key = sm.edge;
-    lp_collect<T>(sm, cand.floor_key, cur, x0, V, v0, v_end, mx);
-    __syncthreads();
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+      const int v = v0 + u * LP_NT + tid;
+      auto key = [&](int i) -> uint64_t {  // 0: not to be taken
+        const int64_t e = (int64_t)v * N + i;
+        const uint64_t q = v < v_end && e < V ? lp_key(to_f(x0[e]), (int)e) : 0;
+        return q >= cand.floor_key ? q : 0;
+      };
+      uint64_t top = 0;
+#pragma unroll 1
+      for (int i = 0; i < N; ++i) top = max(top, key(i));
+      sm.tops[tid] = top;
+      if (tid == 0) sm.edge = 0;
+      __syncthreads();
+      int r = 0;
+      for (int e = 0; e < LP_NT; ++e) r += sm.tops[e] > top;
+      if (r == k - 1 && top) sm.edge = top;
+      __syncthreads();
+      if (sm.edge > cand.floor_key) cand.floor_key = sm.edge;
+#pragma unroll 1
+      for (int i = 0; i < N; ++i)
+        if (const uint64_t q = key(i)) sm.list[atomicAdd(&sm.count, 1)] = q;
+      __syncthreads();
+      const int n = sm.count;
+      __syncthreads();
+      if (n > cand.kept) lp_cut(sm, cand, n, k);
+      __syncthreads();
+    }
   }
   const int n = sm.count;
   __syncthreads();
@@ -332,8 +372,7 @@ __device__ __forceinline__ void lp_top_chunk(LpSmem& sm, LpCandidates& cand, con
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, int vecs_per_cta, int row0, int last) {
-  constexpr int N = LpVec<T>::N, U = LpVec<T>::U, E = N * U;
-  static_assert(E <= LP_MAX_E, "candidates of a thread");
+  constexpr int N = LpVec<T>::N, U = LpVec<T>::U;
   extern __shared__ __align__(16) uint8_t raw[];
   LpSmem& sm = *reinterpret_cast<LpSmem*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -443,9 +482,9 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
         lp_top_chunk<T>(sm, cand, cur, x0, a.V, v0, v_end, mx, a.top_k);
       } else {
         // no barrier in an ordinary chunk: warps add what reaches the threshold, and now and
-        // then (after 4, 16 and 64 chunks) the list is cut and the threshold moves up to it
-        lp_collect<T>(sm, cand.floor_key, cur, x0, a.V, v0, v_end, mx);
-        if (chunk == 3 || chunk == 15 || chunk == 63) {
+        // then (after 2, 6, 18 and 66 chunks) the list is cut and the threshold moves up to it
+        lp_collect<T>(sm, cand.floor_key, cur, a.V, v0, v_end, mx);
+        if (chunk == 1 || chunk == 5 || chunk == 17 || chunk == 65) {
           __syncthreads();
           const int n = sm.count;
           if (n > cand.kept && n <= LP_CAP) lp_cut(sm, cand, n, a.top_k);
