@@ -55,7 +55,7 @@ __device__ __forceinline__ void lp_move(LpSums& a, float m, float c) {
   if (a.m == m) return;                 // (-inf too)
   if (a.m != -INFINITY || a.s != 0.f) {  // a part of NaN alone has m = -inf as well: it stays NaN
     const float d = (a.m - m) * c, f = lp_ex2(d);
-    a.t = f * fmaf(d == -INFINITY ? 0.f : d, a.s, a.t);
+    a.t = f == 0.f ? 0.f : f * fmaf(d, a.s, a.t);  // (d times s may overflow then)
     a.s *= f;
   }
   a.m = m;

@@ -131,6 +131,22 @@ def test_rows_beyond_32_bits():
     _check(x, torch.tensor([5, 39999], device="cuda"), 4)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("low", [-1e30, -1.2e38, -1.7e38, -2.5e38, -3.3e38])
+def test_masks_of_any_low_value(low, dtype):
+    """A mask's value may be finite and so low that a few of it overflow: its share is 0."""
+    V = 9001
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = (3 * torch.randn(4, V, generator=g, device="cuda")).to(dtype)
+    x[0, :4500] = low          # whole threads and the first chunk hold nothing else
+    x[1, 1::2] = low
+    x[2, :] = low
+    x[2, 8500] = 1.0
+    x[3, 4096:] = low
+    got = _check(x, torch.tensor([8000, 2, 8500, 1], device="cuda"), 5)
+    assert bool(got.entropy.isfinite().all())
+
+
 def test_more_rows_than_a_wave_of_ctas_and_the_next_kernel():
     # the rows past whole waves go in a second launch beside the first: both have ended for the next
     g = torch.Generator(device="cuda").manual_seed(6)
