@@ -116,6 +116,13 @@ def _check_pool(K_pages, V_pages, Hkv, D, dtype):
                          f"{tuple(V_pages.shape)}")
     if K_pages.dtype != dtype or V_pages.dtype != dtype:
         raise TypeError(f"pages must be {dtype}, got {K_pages.dtype} and {V_pages.dtype}")
+    return shape
+
+
+def _norm_weight(w: torch.Tensor, D: int, dtype: torch.dtype, what: str) -> torch.Tensor:
+    if w.shape != (D,) or w.dtype != dtype:
+        raise ValueError(f"{what} must be [{D}] {dtype}, got {tuple(w.shape)} {w.dtype}")
+    return w.contiguous()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -180,17 +187,18 @@ def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: t
     (int64) of the pools, in place; rows whose slot is outside the pool (-1) are left
     out. Where rows share a slot, any of them may stay. fp32, fp16 or bf16."""
     dev = _on_one_device(K, V, slots, K_pages, V_pages)
-    if K.dim() != 4 or K.shape != V.shape:
+    ks, dtype = K.shape, K.dtype
+    if len(ks) != 4 or ks != V.shape:
         raise ValueError("expected K, V [B, Hkv, N, D] of one shape")
-    if K.dtype not in _DTYPE_CODE or V.dtype != K.dtype:
-        raise TypeError(f"K and V must share one of fp32/fp16/bf16; got {K.dtype}, {V.dtype}")
-    B, Hkv, N, D = K.shape
-    _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
+    if dtype not in _DTYPE_CODE or V.dtype != dtype:
+        raise TypeError(f"K and V must share one of fp32/fp16/bf16; got {dtype}, {V.dtype}")
+    B, Hkv, N, D = ks
+    ps = _check_pool(K_pages, V_pages, Hkv, D, dtype)
     slots = _ints(slots, torch.int64, (B, N), "slots")
     rc = _lib.load().dropkv_store_rows(
         K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(),
         K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
-        *_rows_strides(V_pages, "V_pages"), K_pages.shape[0], K_pages.shape[2], K.element_size(), B, Hkv, N, D,
+        *_rows_strides(V_pages, "V_pages"), ps[0], ps[2], K.element_size(), B, Hkv, N, D,
         _raw_stream(dev))
     if rc:
         _lib.check(rc, "dropkv_store_rows")
@@ -221,16 +229,17 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
     for w in (q_weight, k_weight):
         if w is not None:
             _on_one_device(Q, w)
-    if Q.dim() != 4 or K.dim() != 4 or Q.shape[0] != K.shape[0] or Q.shape[2:] != K.shape[2:]:
-        raise ValueError(f"expected Q [B,Hq,L,D] and K [B,Hkv,L,D], got {tuple(Q.shape)} and {tuple(K.shape)}")
+    qs, ks, cs = Q.shape, K.shape, cos.shape  # (once each: a shape takes 0.3 us to make)
+    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[2] != ks[2] or qs[3] != ks[3]:
+        raise ValueError(f"expected Q [B,Hq,L,D] and K [B,Hkv,L,D], got {tuple(qs)} and {tuple(ks)}")
     dtype = Q.dtype
     dt = _DTYPE_CODE.get(dtype)
     if dt is None or K.dtype != dtype:
-        raise TypeError(f"Q and K must share one of fp32/fp16/bf16; got {Q.dtype}, {K.dtype}")
-    B, Hq, L, D = Q.shape
-    Hkv = K.shape[1]
-    if cos.dim() != 2 or cos.shape != sin.shape:
-        raise ValueError(f"cos and sin must be [P, R / 2] of one shape, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        raise TypeError(f"Q and K must share one of fp32/fp16/bf16; got {dtype}, {K.dtype}")
+    B, Hq, L, D = qs
+    Hkv = ks[1]
+    if len(cs) != 2 or cs != sin.shape:
+        raise ValueError(f"cos and sin must be [P, R / 2] of one shape, got {tuple(cs)} and {tuple(sin.shape)}")
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise TypeError("cos and sin must be float32")
     cos, sin = cos.contiguous(), sin.contiguous()
@@ -238,28 +247,29 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
         positions, pos_sb = _ints(positions, torch.int64, (L,), "positions"), 0
     else:
         positions, pos_sb = _ints(positions, torch.int64, (B, L), "positions"), L
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.shape != (D,) or w.dtype != Q.dtype):
-            raise ValueError(f"{name} must be [{D}] {Q.dtype}, got {tuple(w.shape)} {w.dtype}")
-    q_weight = q_weight.contiguous() if q_weight is not None else None
-    k_weight = k_weight.contiguous() if k_weight is not None else None
+    qw_ptr = kw_ptr = None
+    if q_weight is not None:
+        q_weight = _norm_weight(q_weight, D, dtype, "q_weight")
+        qw_ptr = q_weight.data_ptr()
+    if k_weight is not None:
+        k_weight = _norm_weight(k_weight, D, dtype, "k_weight")
+        kw_ptr = k_weight.data_ptr()
     if cache:
-        if V.shape != K.shape or V.dtype != K.dtype:
-            raise ValueError(f"V must be {tuple(K.shape)} {K.dtype}, got {tuple(V.shape)} {V.dtype}")
-        _check_pool(K_pages, V_pages, Hkv, D, K.dtype)
+        if V.shape != ks or V.dtype != dtype:
+            raise ValueError(f"V must be {tuple(ks)} {dtype}, got {tuple(V.shape)} {V.dtype}")
+        ps = _check_pool(K_pages, V_pages, Hkv, D, dtype)
         slots = _ints(slots, torch.int64, (B, L), "slots")
         tail = (V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(), K_pages.data_ptr(),
                 *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(), *_rows_strides(V_pages, "V_pages"),
-                K_pages.shape[0], K_pages.shape[2])
+                ps[0], ps[2])
     else:
         tail = (None, 0, 0, 0, None, None, 0, 0, 0, None, 0, 0, 0, 0, 1)
-    q_out = _new(dtype, Q.device, B, Hq, L, D)
-    k_out = _new(dtype, Q.device, B, Hkv, L, D)
+    device = Q.device
+    q_out = _new(dtype, device, B, Hq, L, D)
+    k_out = _new(dtype, device, B, Hkv, L, D)
     rc = _lib.load().dropkv_qk_norm_rope(
         Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
-        q_weight.data_ptr() if q_weight is not None else None,
-        k_weight.data_ptr() if k_weight is not None else None, float(eps), cos.data_ptr(), sin.data_ptr(),
-        cos.shape[0], 2 * cos.shape[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
+        qw_ptr, kw_ptr, float(eps), cos.data_ptr(), sin.data_ptr(), cs[0], 2 * cs[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
         D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
     if rc:
         _lib.check(rc, "dropkv_qk_norm_rope")
@@ -300,21 +310,23 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
     bits, sums and softmax statistics in fp32.
     """
     dev = _on_one_device(Q, K, V, cache_lens, *[t for t in (tree_mask, block_table) if t is not None])
-    if Q.dim() != 4 or K.dim() != 4 or K.shape != V.shape:
+    qs, ks, dtype = Q.shape, K.shape, Q.dtype
+    if len(qs) != 4 or len(ks) != 4 or ks != V.shape:
         raise ValueError("expected Q [B,Hq,T,D] and K, V [B,Hkv,cap,D] or [pages,Hkv,block_size,D] of one shape")
-    if not (Q.dtype == K.dtype == V.dtype) or Q.dtype not in (torch.bfloat16, torch.float16):
+    if not (dtype == K.dtype == V.dtype) or dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("tree attention takes bf16 or fp16 Q, K and V of one dtype")
-    B, Hq, T, D = Q.shape
-    n0, Hkv, rows, Dk = K.shape
+    B, Hq, T, D = qs
+    n0, Hkv, rows, Dk = ks
     if Dk != D or not Hkv or Hq % Hkv or (block_table is None and n0 != B):
-        raise ValueError(f"shape mismatch: Q {tuple(Q.shape)}, K {tuple(K.shape)}")
+        raise ValueError(f"shape mismatch: Q {tuple(qs)}, K {tuple(ks)}")
     cache_lens = _ints(cache_lens, torch.int32, (B,), "cache_lens")
     if block_table is not None:
         if block_table.dim() != 2:
             raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
-        block_table = _ints(block_table, torch.int32, (B, block_table.shape[1]), "block_table")
-        paging = (block_table.data_ptr(), block_table.shape[1], rows, n0)
-        cap = block_table.shape[1] * rows
+        max_blocks = block_table.shape[1]
+        block_table = _ints(block_table, torch.int32, (B, max_blocks), "block_table")
+        paging = (block_table.data_ptr(), max_blocks, rows, n0)
+        cap = max_blocks * rows
     else:
         paging = (None, 0, 0, 0)
         cap = rows
@@ -322,26 +334,28 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:
             raise TypeError(f"tree_mask must be bool, got {tree_mask.dtype}")
-        if tree_mask.shape not in ((T, T), (B, T, T)):
-            raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(tree_mask.shape)}")
-        mask = (tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2),
-                tree_mask.stride(-1))
+        ms, st = tree_mask.shape, tree_mask.stride()
+        if ms not in ((T, T), (B, T, T)):
+            raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(ms)}")
+        mask = (tree_mask.data_ptr(), *(st if len(st) == 3 else (0, *st)))
     scale = float(D ** -0.5 if scale is None else scale)
     lib = _lib.load()
-    out = _new(Q.dtype, Q.device, B, Hq, T, D)
+    device = Q.device
+    out = _new(dtype, device, B, Hq, T, D)
     if B == 0 or T == 0:
         return out
     # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
-    ws = _new(torch.uint8, Q.device, max(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), 1))
+    need = max(_tree_workspace(dev, B, Hq, Hkv, T, D, cap), 1)
+    ws = _new(torch.uint8, device, need)
     rc = lib.dropkv_tree_attention(
         Q.data_ptr(), *Q.stride(), K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"),
-        *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[Q.dtype], B, Hq, Hkv, T, D, cap, scale,
-        out.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(dev))
+        *paging, cache_lens.data_ptr(), *mask, _DTYPE_CODE[dtype], B, Hq, Hkv, T, D, cap, scale,
+        out.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
     if rc:
         _lib.check(rc, "dropkv_tree_attention")
     if _CHECK_STATUS and cap * n0 > 0 and not torch.cuda.is_current_stream_capturing():
         n = torch.cuda.get_device_properties(dev).multi_processor_count  # a word for each CTA comes first
-        st = int(ws[:4 * n].view(torch.int32).max().item()) if ws.numel() >= 4 * n else 0
+        st = int(ws[:4 * n].view(torch.int32).max().item()) if need >= 4 * n else 0
         if st != 0:
             raise _lib.DropKVError(_lib.ERR_DEVICE, f"dropkv_tree_attention: device status {st} "
                                                     "(a bounded wait timed out)")
@@ -362,17 +376,18 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
         raise TypeError(f"logits must be fp32/fp16/bf16; got {logits.dtype}")
     if tokens.dtype != torch.int64:
         raise TypeError(f"tokens must be int64, got {tokens.dtype}")
-    if logits.dim() < 1 or tokens.dim() - logits.dim() not in (-1, 0) or tokens.shape[:logits.dim() - 1] != logits.shape[:-1]:
-        raise ValueError(f"expected logits [..., V] and tokens [...] or [..., C], got {tuple(logits.shape)} and "
-                         f"{tuple(tokens.shape)}")
-    V, lead, device = logits.shape[-1], logits.shape[:-1], logits.device
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    ls, ts = tuple(logits.shape), tuple(tokens.shape)
+    lead = ls[:-1]
+    if not ls or len(ts) - len(ls) not in (-1, 0) or ts[:len(lead)] != lead:
+        raise ValueError(f"expected logits [..., V] and tokens [...] or [..., C], got {ls} and {ts}")
+    V, device = ls[-1], logits.device
+    rows = logits if len(ls) == 2 else logits.reshape(-1, V)
     if V > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
     N, top_k = rows.shape[0], int(top_k)
-    C = tokens.shape[-1] if tokens.dim() == logits.dim() else 1
+    C = ts[-1] if len(ts) == len(ls) else 1
     tokens = tokens.contiguous()
-    logprob = _new(torch.float32, device, *tokens.shape)
+    logprob = _new(torch.float32, device, *ts)
     entropy = _new(torch.float32, device, *lead)
     top_lp = top_id = None
     if top_k > 0:
