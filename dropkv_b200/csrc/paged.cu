@@ -37,7 +37,14 @@ __device__ __forceinline__ int bt_take(const BtArgs& a, int b) {
 // CTA (b, y): table row b (y = 0) and the slots [y, y + 1) * BT_TOKENS of request b.
 // A request's pages start where those of the requests before it end in the free
 // list, so each CTA sums the needs of the requests before its own; no CTA waits
-// for another.
+// for another. With need_b = ceil(len_b / block) and take_b = max(need_b - held_b, 0),
+// request b gets entries [f, f + take_b) of the free list, f = sum of take over the
+// requests before it, and token t of it the slot table[b][t / block] * block + t % block.
+// What bounds it: a step's call is its launch and two chains of loads (32 requests: 2.8 us);
+// a prefill's is the 8 bytes a token that it writes (128 requests of up to 13107 tokens,
+// 13 MB: 7.2 us, the sums and the lookup of a page for each token beside 1.9 TB/s of stores).
+// The sums are taken again by every CTA because a list of a few hundred lengths is one load a
+// thread, less than a second launch or a wait for a first CTA.
 __global__ void __launch_bounds__(BT_NT) block_tables_kernel(BtArgs a) {
   __shared__ long long part[BT_NT / 32];
   const int b = blockIdx.x, tid = threadIdx.x;
@@ -102,8 +109,12 @@ struct SrArgs {
 
 // Rows of LANES 16-byte vectors: LANES threads have a row, SR_ROWS rows each, whose slots,
 // then K and V vectors, are on their way at once. Rows follow one another along a head, so
-// reads are one stream and writes come in runs of a page's rows.
-constexpr int SR_ROWS = 4;
+// reads are one stream and writes come in runs of a page's rows. HBM bounds it: each byte is
+// read and written once. One layer's 13107 rows (8 heads of 128, bf16, 107 MB): 18.8 us alone,
+// 16.8 us call after call (6.4 TB/s, 97% of a copy's); rows in flight 1, 2, 4, 8: 18.7, 18.8,
+// 19.4, 20.4 us, and a few hundred rows 1.8, 2.2, 3.0, 4.2 us; 2 for the heads of 64, where
+// 1 row is slower (16.8 us against 15.7).
+constexpr int SR_ROWS = 2;
 
 template <int LANES>
 __global__ void __launch_bounds__(SR_NT) store_rows_vec_kernel(SrArgs a) {
