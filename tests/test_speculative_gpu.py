@@ -9,6 +9,7 @@ import torch
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
 
 import speculative_decode as S  # noqa: E402
+from dropkv_b200 import block_tables, qk_norm_rope, token_logprobs, tree_attention  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,47 @@ def test_trees_decode_what_single_tokens_do():
     for a, b in zip(single, many):
         n = min(len(a), len(b))
         assert n >= 6 and a[:n] == b[:n]
+
+
+def test_a_captured_step_follows_its_inputs():
+    """A decode step of four operators in one CUDA graph: replayed on other inputs, in place,
+    it gives what the calls give."""
+    B, Hq, Hkv, T, D, block, V = 3, 8, 2, 4, 64, 16, 5003
+    g = torch.Generator(device="cuda").manual_seed(11)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    lens = torch.tensor([40, 7, 100], dtype=torch.int32, device="cuda")
+    held = (lens + block - 1) // block
+    free = torch.randperm(64, generator=g, device="cuda").int()
+    table = torch.full((B, 12), -1, dtype=torch.int32, device="cuda")
+    table[:, :7] = torch.arange(64, 64 + 7 * B, device="cuda").view(B, 7)
+    Q, K, W = (rnd(B, T, h, D).bfloat16().transpose(1, 2) for h in (Hq, Hkv, Hkv))
+    pages = [rnd(96, Hkv, block, D).bfloat16() for _ in range(2)]
+    ang = torch.rand(200, D // 2, generator=g, device="cuda") * 6
+    cos, sin = ang.cos(), ang.sin()
+    logits = rnd(1300, V)                         # more rows than a wave of CTAs: two launches
+    tokens = torch.randint(0, V, (1300,), generator=g, device="cuda")
+
+    def step(pages):
+        t = block_tables(lens + T, block, free, 12, T, new_lens=torch.full_like(lens, T), table=table, held=held)
+        at = lens.long()[:, None] + torch.arange(T, device="cuda")
+        q, k = qk_norm_rope(Q, K, cos, sin, at, V=W, slots=t.slots, K_pages=pages[0], V_pages=pages[1])
+        return [*t, q, k, tree_attention(q, *pages, lens, block_table=t.table), *token_logprobs(logits, tokens, top_k=3)]
+
+    step([p.clone() for p in pages])              # (nothing is loaded for the first time while capturing)
+    mine = [p.clone() for p in pages]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(mine)
+    for change in range(2):
+        if change:
+            lens.copy_(torch.tensor([64, 0, 31], device="cuda"))
+            held.copy_((lens + block - 1) // block)
+            Q.copy_(Q.flip(0)), logits.mul_(0.5)
+        for m, p in zip(mine, pages):
+            m.copy_(p)
+        graph.replay()
+        torch.cuda.synchronize()
+        want_pages = [p.clone() for p in pages]
+        for a, b in zip(got, step(want_pages)):
+            assert torch.equal(a, b)
+        assert all(torch.equal(a, b) for a, b in zip(mine, want_pages))
