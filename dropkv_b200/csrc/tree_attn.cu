@@ -74,8 +74,8 @@ struct TaArgs {
 };
 
 // per softmax group s: Q written, S ready, P ready (keys 0 to 63; and, at + 2, 64 to 127), O ready,
-// its turn to issue, every product done
-enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 8, B_T = 10, B_END = 12, B_COUNT = 14 };
+// its turn to issue, every product done; both MMA warps have seen a piece's Q
+enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 8, B_T = 10, B_END = 12, B_SEEN = 14, B_COUNT = 16 };
 
 template <int D>
 struct TaSmem {
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
       tc::mbar_init(&bars[B_T + s], 1);
       tc::mbar_init(&bars[B_END + s], 1);
     }
+    tc::mbar_init(&bars[B_SEEN], 2);
     tc::fence_mbar_init();
     misc->dead = 0;
   }
@@ -380,6 +381,9 @@ __global__ void __launch_bounds__(TA_NT, 1)
             const uint32_t k = before + k_load(i, lead_before);
             ok = __all_sync(0xffffffffu, ok && wait(&empty[k % NS], k / NS, 12));
           }
+        // and once both MMA warps have seen the last one: a warp without work in that piece may
+        // still be at the one before, and a barrier two phases on looks as if it had not moved
+        if (queries) ok = __all_sync(0xffffffffu, ok && wait(&bars[B_SEEN], queries - 1, 11));
         if (!ok) break;
         if (tc::elect_one()) {
           tc::mbar_arrive_expect_tx(&bars[B_Q], A.M * 128 * SLABS);
@@ -488,26 +492,31 @@ __global__ void __launch_bounds__(TA_NT, 1)
         tc::mma_commit(&bars[B_S + s]);
         release(&empty[slot]);
       };
-      if (first < nt) {  // the first product, out of turn: nothing is running yet
+      if (A.q_tma) {  // every piece's Q is waited for, with work in it or without
+        ok = __all_sync(0xffffffffu, wait(&bars[B_Q], pieces, 2));
+        if (ok && tc::elect_one()) tc::mbar_arrive(&bars[B_SEEN]);
+        __syncwarp();
+      }
+      if (first < nt && ok) {  // the first product, out of turn: nothing is running yet
         const uint32_t at = base + k_load(first, lead), slot = at % NS;
-        ok = wait(&bars[B_Q + (A.q_tma ? 0 : s)], A.q_tma ? pieces : n_q++, 2) && wait(&full[slot], at / NS, 3);
+        ok = (A.q_tma || wait(&bars[B_Q + s], n_q++, 2)) && wait(&full[slot], at / NS, 3);
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           tc::tc_fence_after();
           if (tc::elect_one()) qk(slot);
           __syncwarp();
         }
-      } else if (A.q_tma) {
-        ok = __all_sync(0xffffffffu, wait(&bars[B_Q], pieces, 2));  // every piece's Q is waited for: none is taken for another
       }
       for (int i = first; i < nt && ok; i += step) {
         const uint32_t at = base + v_load(i, lead, nt), slot = at % NS;
         const uint32_t kat = base + k_load(i + step, lead), kslot = kat % NS;
         const uint64_t vd = tc::smem_desc(ring0 + slot * L::TILE, LBO_V, 1024);
         const bool more = i + step < nt;
-        ok = wait(&full[slot], at / NS, 4) && (!more || wait(&full[kslot], kat / NS, 3));
-        // the group's turn comes when the other has issued the item before this one
-        if (s == 1 || i > first || handed) ok = ok && wait(&bars[B_T + s], n_t++, 10);
+        // the group's turn comes when the other has issued the item before this one. Its own loads
+        // are waited for after that: the load before one in its slot may be the other group's, and
+        // while that is not there its phase looks like this one's
+        if (s == 1 || i > first || handed) ok = wait(&bars[B_T + s], n_t++, 10);
+        ok = ok && wait(&full[slot], at / NS, 4) && (!more || wait(&full[kslot], kat / NS, 3));
         for (int half = 0; half < 2 && ok; ++half) {
           ok = __all_sync(0xffffffffu, ok && wait(&bars[B_P + 2 * half + s], n_p, 5));
           if (!ok) break;

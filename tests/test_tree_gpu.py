@@ -151,6 +151,21 @@ def test_many_short_caches(B, Hq, Hkv, T, D, most, paged):
     assert float((got.double() - alone.double()).abs().max()) <= 2 * (u * 6 + (2 * u + 2.0 ** -13) * 6)
 
 
+@pytest.mark.parametrize("long,short", [(450, 90), (230, 60), (1000, 20)])
+def test_short_pieces_after_long_ones(long, short):
+    # CTAs that end a segment of several tiles, which two groups take in turn, and go on with
+    # segments of one: a group has no work in some pieces and is at others for long
+    B, T = 90, 4
+    lens = [long - (b % 7) if b % 3 == 0 else short for b in range(B)]
+    Q, K, V, n = _inputs(B, 8, 4, T, 128, lens, torch.bfloat16, seed=long)
+    want = tree_attention(Q, K, V, n)
+    some = [0, 1, 2, 45, B - 1]
+    chain = torch.ones(T, T, dtype=torch.bool, device="cuda").tril()
+    _close(want[some], Q[some], K[some], V[some], [lens[b] for b in some], chain)
+    for _ in range(40):
+        assert torch.equal(tree_attention(Q, K, V, n), want)
+
+
 def test_a_long_cache_in_small_pages_with_few_rows():
     lens, T = [30000, 7], 4
     Q, K, V, n = _inputs(2, 28, 4, T, 128, lens, torch.float16, seed=12)
