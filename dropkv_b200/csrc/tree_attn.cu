@@ -74,8 +74,9 @@ struct TaArgs {
 };
 
 // per softmax group s: Q written, S ready, P ready (keys 0 to 63; and, at + 2, 64 to 127), O ready,
-// its turn to issue, every product done; both MMA warps have seen a piece's Q
-enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 8, B_T = 10, B_END = 12, B_SEEN = 14, B_COUNT = 16 };
+// its turn to issue, every product done, the products of a tile's first half done;
+// both MMA warps have seen a piece's Q
+enum { B_Q = 0, B_S = 2, B_P = 4, B_O = 8, B_T = 10, B_END = 12, B_H = 14, B_SEEN = 16, B_COUNT = 18 };
 
 template <int D>
 struct TaSmem {
@@ -198,35 +199,6 @@ __device__ __forceinline__ float ta_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float ta_max_nan(float a, float b) {  // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// 2^y of a pair without the special-function unit, which the weights keep busy (128 rows x
-// 128 keys take it 1024 cycles): y = n + f with n the nearest integer, a polynomial of degree 4
-// fitted to 2^f on [-1/2, 1/2] (relative error 3e-6, far under a weight's 16 bits), n added to
-// the exponent. Below -126 it stays at 2^-126. One pair in four goes this way: a tile's weights
-// take 1410 cycles against 1570 alone, 2240 against 2410 beside the other group's.
-__device__ __forceinline__ uint64_t ta_ex2_poly(uint64_t y) {
-  float u, v;
-  ta_unpair(y, u, v);
-  y = ta_pair(ta_max_nan(u, -126.f), ta_max_nan(v, -126.f));
-  const float big = 12582912.f;  // 1.5 * 2^23: the sum's low bits hold n
-  const uint64_t t = ta_add2(y, ta_pair(big, big)), n = ta_add2(t, ta_pair(-big, -big));
-  const uint64_t f = ta_fma2(n, ta_pair(-1.f, -1.f), y);
-  uint64_t p = ta_pair(0.009570097550749779f, 0.009570097550749779f);
-  p = ta_fma2(p, f, ta_pair(0.05591785907745361f, 0.05591785907745361f));
-  p = ta_fma2(p, f, ta_pair(0.240247443318367f, 0.240247443318367f));
-  p = ta_fma2(p, f, ta_pair(0.6931217908859253f, 0.6931217908859253f));
-  p = ta_fma2(p, f, ta_pair(0.9999992847442627f, 0.9999992847442627f));
-  float c, d;
-  ta_unpair(p, u, v);
-  ta_unpair(t, c, d);
-  return ta_pair(__int_as_float(__float_as_int(u) + (__float_as_int(c) << 23)),
-                 __int_as_float(__float_as_int(v) + (__float_as_int(d) << 23)));
-}
-
 // What a partial of maximum m weighs under the joint maximum `to`; parts that saw
 // nothing (or NaN alone) have -inf, which must not turn into NaN (or hide it).
 __device__ __forceinline__ float ta_factor(float m, float to) { return m == to ? 1.f : ta_ex2(m - to); }
@@ -278,6 +250,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
       tc::mbar_init(&bars[B_O + s], 1);
       tc::mbar_init(&bars[B_T + s], 1);
       tc::mbar_init(&bars[B_END + s], 1);
+      tc::mbar_init(&bars[B_H + s], 1);
     }
     tc::mbar_init(&bars[B_SEEN], 2);
     tc::fence_mbar_init();
@@ -526,6 +499,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
             for (int kk = 0; kk < TA_TK / 32; ++kk)
               tc::mma_f16_tmem_a(to, ts + half * 32 + kk * 8, tc::desc_add(vd, half * (TA_TK * 64) + kk * 2048), ID_PV,
                                  i > first || half > 0 || kk > 0);
+            if (half == 0) tc::mma_commit(&bars[B_H + s]);
           }
           __syncwarp();
         }
@@ -719,92 +693,82 @@ __global__ void __launch_bounds__(TA_NT, 1)
         }
         if (live) {
           const bool masked = tree || gone;
-          // S is read twice, for the maximum and for the weights, which overwrite it as they come:
-          // a row of 128 does not stay in registers
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (masked) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              float x[32];
-              tc::tmem_ld32(ts + 32 * w, x);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], (see[w] >> e) & 1 ? x[e] : -INFINITY);
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              float x[64];
-              tc::tmem_ld64(ts + 64 * w, x);
-#pragma unroll
-              for (int e = 0; e < 64; e += 2) mx[(e / 2) & 3] = ta_max3(mx[(e / 2) & 3], x[e], x[e + 1]);
-            }
-          }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
           const bool first = i < step;
-          if (__any_sync(0xffffffffu, first || top > m + kTaSlack)) {  // some row's reference moves
-            const float mn = first || top > m + kTaSlack ? top : m;
-            const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
-            m = mn;
-            l *= alpha;
-            if (!first) {
-              float o[16];
-#pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                tc::tmem_ld16(to + s * 128 + c, o);
+          const uint64_t scale2 = ta_pair(A.scale_log2, A.scale_log2);
+          // S is read once, a half of 64 keys at a time (128 do not stay in registers): the half's
+          // maximum decides whether the row's reference moves, then its weights overwrite it. The
+          // first half's products start beside the second half's weights; where the second half
+          // moves the reference, which is rare, they are waited for. (A pass for the maximum of all
+          // 128, a second one for the weights and a polynomial in place of one ex2 in four took as
+          // long for long caches and 2 us more for one layer's: 13107 keys x 256 rows 28.8 us, now
+          // 26.5; with that polynomial here 28.8 too.)
+          auto weigh = [&](auto hide, int h) {
+            float x[64];
+            tc::tmem_ld64(ts + 64 * h, x);
+            if (decltype(hide)::value) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= alpha;
-                tc::tmem_st16(to + s * 128 + c, o);
-                tc::tmem_st_wait();
+              for (int e = 0; e < 64; ++e) x[e] = (see[2 * h + e / 32] >> (e & 31)) & 1 ? x[e] : -INFINITY;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) mx[(e / 2) & 3] = ta_max3(mx[(e / 2) & 3], x[e], x[e + 1]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.scale_log2;
+            const bool start = first && h == 0;
+            if (__any_sync(0xffffffffu, start || top > m + kTaSlack)) {  // some row's reference moves
+              if (h == 1) {
+                ok = __all_sync(0xffffffffu, wait(&bars[B_H + s], n_s - 1, 7)) && ok;
+                tc::tc_fence_after();
+              }
+              const float mn = start || top > m + kTaSlack ? top : m;
+              const float alpha = mn == m ? 1.f : ta_ex2(m - mn);
+              m = mn;
+              l *= alpha;
+              if (!start) {
+                float o[16];
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                  tc::tmem_ld16(to + s * 128 + c, o);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                  tc::tmem_st16(to + s * 128 + c, o);
+                  tc::tmem_st_wait();
+                }
               }
             }
-          }
-          const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
-          const uint64_t scale2 = ta_pair(A.scale_log2, A.scale_log2), ref2 = ta_pair(-ref, -ref);
-          uint64_t sum[2] = {0, 0};
-          auto weigh = [&](auto hide, int w0) {
+            const float ref = (m == -INFINITY ? 0.f : m) - A.bias;
+            const uint64_t ref2 = ta_pair(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int w = w0; w < w0 + 2; ++w) {
-              float x[32];
-              tc::tmem_ld32(ts + 32 * w, x);
+            for (int w = 0; w < 2; ++w) {
               uint32_t pk[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                if (decltype(hide)::value) {
-                  x[e] = (see[w] >> e) & 1 ? x[e] : -INFINITY;
-                  x[e + 1] = (see[w] >> (e + 1)) & 1 ? x[e + 1] : -INFINITY;
-                }
-                uint64_t y = ta_fma2(ta_pair(x[e], x[e + 1]), scale2, ref2);
-                if (!decltype(hide)::value && (e / 2) % 4 == 3) {
-                  y = ta_ex2_poly(y);
-                } else {
-                  float u, v;
-                  ta_unpair(y, u, v);
-                  y = ta_pair(ta_ex2(u), ta_ex2(v));
-                }
-                sum[(e / 2) & 1] = ta_add2(sum[(e / 2) & 1], y);
+                const uint64_t y = ta_fma2(ta_pair(x[32 * w + e], x[32 * w + e + 1]), scale2, ref2);
                 float u, v;
                 ta_unpair(y, u, v);
+                u = ta_ex2(u), v = ta_ex2(v);
+                sum[(e / 2) & 1] = ta_add2(sum[(e / 2) & 1], ta_pair(u, v));
                 pk[e / 2] = TaType<T>::pack(u, v);
               }
-              tc::tmem_st16(ts + 16 * w, reinterpret_cast<const float*>(pk));
+              tc::tmem_st16(ts + 32 * h + 16 * w, reinterpret_cast<const float*>(pk));
             }
+            // (a sum for each half, whether or not a row beside this one moves its reference)
+            float s0, s1, s2, s3;
+            ta_unpair(sum[0], s0, s1);
+            ta_unpair(sum[1], s2, s3);
+            l += (s0 + s1) + (s2 + s3);
           };
-          // the first half's products start beside the second half's weights
 #pragma unroll
-          for (int w0 = 0; w0 < 4; w0 += 2) {
+          for (int h = 0; h < 2; ++h) {
             if (masked)
-              weigh(std::true_type(), w0);
+              weigh(std::true_type(), h);
             else
-              weigh(std::false_type(), w0);
+              weigh(std::false_type(), h);
             tc::tmem_st_wait();
             tc::tc_fence_before();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bars[B_P + w0 + s]);
+            if (lane == 0) tc::mbar_arrive(&bars[B_P + 2 * h + s]);
           }
-          float s0, s1, s2, s3;
-          ta_unpair(sum[0], s0, s1);
-          ta_unpair(sum[1], s2, s3);
-          l += (s0 + s1) + (s2 + s3);
         } else {
           __syncwarp();
           if (lane == 0) {
