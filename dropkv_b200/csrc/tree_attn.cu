@@ -25,12 +25,14 @@
 // are in fp32.
 //
 // What it measured alone: 295K keys in 8 sequences x 4 KV heads x 224 rows of 128, fp16 (135
-// GFLOP, 604 MB): 155 us, 870 TFLOP/s (53% of a matrix product's burst rate) and 3.9 TB/s
-// (60% of a copy's); call after call 200 us, as the clock falls under load. The softmax bounds
-// it: a tile of both groups takes about 4700 cycles, its four products 2048 of them (64 cycles
-// a K-step of 16) and its loads 2800 at a copy's rate, while a group reads 128 x 128 logits
-// twice from tensor memory and takes 2240 cycles for the weights beside the other group. 13107 keys x 256 rows x 8 heads, bf16: 28 us with the merge, of which the tiles
-// are 8; the rest is the launch, the first tiles, the partials (20 MB out and in) and the merge.
+// GFLOP, 604 MB): 151 us, 890 TFLOP/s (54% of a matrix product's burst rate) and 4.0 TB/s
+// (61% of a copy's); call after call 170 to 200 us, as the clock falls under load. What bounds
+// it is the chain of a group's tile, 3800 cycles: from S to its last weights 2500 (480 for the
+// first half's logits and maximum, 1000 a half for weights), 440 until the products are
+// issued, 860 until the next S is there; the other group's runs beside it. The tile's four
+// products take 2048, its loads 2800 at a copy's rate. 13107 keys x 256 rows x 8 heads, bf16:
+// 26 us with the merge, of which the tiles are 11; the rest is the launch, the first tiles, the
+// partials (20 MB out and in) and the merge.
 #include <algorithm>
 #include <type_traits>
 
@@ -199,6 +201,7 @@ __device__ __forceinline__ float ta_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+
 // What a partial of maximum m weighs under the joint maximum `to`; parts that saw
 // nothing (or NaN alone) have -inf, which must not turn into NaN (or hide it).
 __device__ __forceinline__ float ta_factor(float m, float to) { return m == to ? 1.f : ta_ex2(m - to); }
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
     // tile of its group), the other waits for its own data. The products of one group then run
     // beside the softmax of the other. (Without turns the tensor cores served both at once, the
     // groups fell into step and nothing overlapped: 295K keys x 224 rows in 210 us, with turns 180;
-    // now 155.)
+    // now 151.)
     // The whole warp runs this and one lane issues, so that counts, addresses and descriptors
     // can stay in uniform registers.
     constexpr uint32_t ID_QK = tc::idesc_f16(BF16, 128, TA_TK, false, false);
