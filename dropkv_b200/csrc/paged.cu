@@ -1,6 +1,8 @@
 // Pages of a shared K/V pool for a ragged batch of caches: block tables and slot
 // maps from lengths that exist on the device only (an eviction's keep_len, a decode
 // loop's counters), and the rows that go to those slots.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace dropkv {
@@ -18,19 +20,26 @@ struct BtArgs {
   const int32_t* held_in;
   const int32_t* free_blocks;
   int B, block, n_free, max_blocks, max_new;
+  uint32_t by_mul, by_shift;  // division by block
   int32_t* table;
   int32_t* held;
   int64_t* slots;
   int64_t* used;
 };
 
+// t / block for t below 2^31, by a multiplication (Granlund and Montgomery): with l = ceil(log2
+// block), mul = floor(2^(31 + l) / block) + 1 exceeds 2^(31 + l) / block by at most one part in
+// 2^31, which no such t turns into a quotient too large.
+__device__ __forceinline__ unsigned bt_quot(const BtArgs& a, unsigned t) {
+  return a.block == 1 ? t : __umulhi(t, a.by_mul) >> a.by_shift;
+}
 __device__ __forceinline__ int bt_len(const BtArgs& a, int b) { return max(a.lens[b], 0); }
 __device__ __forceinline__ int bt_held(const BtArgs& a, int b) {
   return a.held_in ? min(max(a.held_in[b], 0), a.max_blocks) : 0;
 }
 // pages request b still needs
 __device__ __forceinline__ int bt_take(const BtArgs& a, int b) {
-  const int need = (int)(((int64_t)bt_len(a, b) + a.block - 1) / a.block);
+  const int len = bt_len(a, b), need = len ? (int)bt_quot(a, (unsigned)(len - 1)) + 1 : 0;
   return max(min(need, a.max_blocks) - bt_held(a, b), 0);
 }
 
@@ -42,7 +51,8 @@ __device__ __forceinline__ int bt_take(const BtArgs& a, int b) {
 // requests before it, and token t of it the slot table[b][t / block] * block + t % block.
 // What bounds it: a step's call is its launch and two chains of loads (32 requests: 2.8 us);
 // a prefill's is the 8 bytes a token that it writes (128 requests of up to 13107 tokens,
-// 13 MB: 7.2 us, the sums and the lookup of a page for each token beside 1.9 TB/s of stores).
+// 13 MB: 5.6 us, 2.4 TB/s, behind the sums and a page's lookup for each token; with a division
+// and one lookup after the other 7.2). Slots of a thread 2, 4, 8, 16: 8.4, 6.4, 5.6, 6.0 us.
 // The sums are taken again by every CTA because a list of a few hundred lengths is one load a
 // thread, less than a second launch or a wait for a first CTA.
 __global__ void __launch_bounds__(BT_NT) block_tables_kernel(BtArgs a) {
@@ -76,20 +86,21 @@ __global__ void __launch_bounds__(BT_NT) block_tables_kernel(BtArgs a) {
   const int len = bt_len(a, b), nn = a.new_lens ? min(max(a.new_lens[b], 0), len) : len;
   const int64_t i0 = (int64_t)blockIdx.y * BT_TOKENS + tid;
   int64_t* out = a.slots + (int64_t)b * a.max_new;
-  const unsigned block = (unsigned)a.block;
-#pragma unroll 2
+  int p[BT_EACH];  // the slots' pages, all on their way before the first is used
+  unsigned at[BT_EACH];
+#pragma unroll
   for (int e = 0; e < BT_EACH; ++e) {
     const int64_t i = i0 + e * BT_NT;
-    if (i >= a.max_new) break;
-    int64_t slot = -1;
-    if (i < nn) {
-      const unsigned t = (unsigned)(len - nn) + (unsigned)i, col = t / block;
-      if (col < (unsigned)a.max_blocks) {
-        const int p = page((int)col);
-        if (p >= 0) slot = (int64_t)p * a.block + (t - col * block);
-      }
-    }
-    out[i] = slot;
+    p[e] = -1;
+    if (i >= nn) continue;
+    const unsigned t = (unsigned)(len - nn) + (unsigned)i, col = bt_quot(a, t);
+    at[e] = t - col * (unsigned)a.block;
+    if (col < (unsigned)a.max_blocks) p[e] = page((int)col);
+  }
+#pragma unroll
+  for (int e = 0; e < BT_EACH; ++e) {
+    const int64_t i = i0 + e * BT_NT;
+    if (i < a.max_new) out[i] = p[e] >= 0 ? (int64_t)p[e] * a.block + at[e] : -1;
   }
 }
 
@@ -177,8 +188,11 @@ int launch_block_tables(const int32_t* lens, const int32_t* new_lens, const int3
                         const int32_t* held_in, int B, int block, const int32_t* free_blocks, int n_free,
                         int max_blocks, int max_new, int32_t* table, int32_t* held, int64_t* slots, int64_t* used,
                         cudaStream_t st) {
+  int l = 0;
+  while ((int64_t(1) << l) < block) ++l;
+  const uint32_t by_mul = block == 1 ? 0u : (uint32_t)((uint64_t(1) << (31 + l)) / block + 1);
   BtArgs a{lens, new_lens, table_in, table_in_stride, held_in, free_blocks, B, block, n_free, max_blocks, max_new,
-           table, held, slots, used};
+           by_mul, (uint32_t)std::max(l - 1, 0), table, held, slots, used};
   const int ys = (int)(((int64_t)max_new + BT_TOKENS - 1) / BT_TOKENS);
   if (ys > 65535) return fail(DROPKV_ERR_UNSUPPORTED, "block tables: max_new %d exceeds %d", max_new, 65535 * BT_TOKENS);
   block_tables_kernel<<<dim3(B, ys > 0 ? ys : 1), BT_NT, 0, st>>>(a);

@@ -49,6 +49,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _new(dtype: torch.dtype, device: torch.device, *shape: int) -> torch.Tensor:
     """An uninitialised contiguous tensor (of up to four dimensions). empty_strided takes 1.5 us
     where empty takes 2.3 to 3."""
@@ -85,7 +88,7 @@ def _on_its_device(fn):
     def call(*args, **kwargs):
         first = args[0] if args else next(iter(kwargs.values()), None)
         index = first.get_device() if isinstance(first, torch.Tensor) else -1
-        if index < 0 or index == torch.cuda.current_device():
+        if index < 0 or index == _current_device():
             return fn(*args, **kwargs)
         with torch.cuda.device(index):
             return fn(*args, **kwargs)

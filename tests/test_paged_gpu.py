@@ -59,6 +59,22 @@ def test_block_tables_fresh(lens, block, max_blocks, max_new):
     assert got.table.tolist() == t and got.held.tolist() == h and got.slots.tolist() == s and got.used.tolist() == [used]
 
 
+@pytest.mark.parametrize("block", [1, 2, 3, 7, 48, 100, 1 << 20, (1 << 31) - 1])
+def test_block_tables_quotients_up_to_the_largest_length(block):
+    """Slots of the last tokens of caches whose length is next to a page's end, and to 2^31."""
+    top = 2 ** 31 - 1
+    lens = [min(top, max(1, k * block + d)) for k in (1, 2, 5) for d in (-1, 0, 1)] + [top]
+    wide = min(-(-top // block), 4096)                       # longer caches run out of columns
+    t = block_tables(_i32(lens), block, torch.arange(0, dtype=torch.int32, device="cuda"), wide, 6,
+                     new_lens=_i32([6] * len(lens)),
+                     table=torch.arange(wide, dtype=torch.int32, device="cuda").expand(len(lens), wide).contiguous(),
+                     held=_i32([wide] * len(lens)))
+    for b, n in enumerate(lens):
+        new = min(6, n)
+        want = [(tok if tok // block < wide else -1) for tok in range(n - new, n)] + [-1] * (6 - new)
+        assert t.slots[b].tolist() == want, (n, block)
+
+
 def test_block_tables_extends_held_pages_and_a_step_can_follow_a_step():
     block, max_blocks = 16, 5
     lens = [15, 16, 0, 60, 80]
