@@ -86,13 +86,15 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
 // token: a lane's cosines and sines, which weigh more than a row (64 bytes of table against 32
 // of Q), are fetched once and stay in registers, and QR_BATCH rows are on their way at a time.
 //
-// HBM bounds long chunks in principle (4 D bytes a row of 16 bits, the tables beside them), and
-// instructions in fact: about 60 a vector pair, two of which are the row's bytes. So arithmetic
-// is done on two floats at once, and as many CTAs are resident as registers allow without
-// spilling: 4096 tokens x 40 heads of 128, bf16, normed (84 MB): 22.1 us, 3.8 TB/s (58% of a
-// copy's), without a norm 17.2; with 5, 6 and 8 CTAs an SM 26.6, 22.1 and 25.6 us against 21.5.
-// Rows on their way 2, 3, 4: 20.9, 21.1, 22.9 us; fp32 39.6, 36.0, 35.2; 16384 tokens 84, 80, 83.
-constexpr int QR_BATCH = 3;
+// HBM bounds long chunks in principle (4 D bytes a row of 16 bits, the tables beside them);
+// in fact it is instructions, and the latency of the chains position - table row - rows. So
+// arithmetic is done on two floats at once, as many CTAs are resident as registers allow without
+// spilling, and a group takes several rounds of rows for one look at the tables. 4096 tokens x 40
+// heads of 128, bf16, normed (84 MB): 18.8 us, 4.5 TB/s (68% of a copy's rate), without a norm
+// 14.7 (87%); 16384 tokens 72 us (4.7 TB/s). Rows on their way x rounds, for 4096 and 16384
+// tokens: 2 x 2 18.8 and 71.7 us, 3 x 1 21.2 and 80.3, 3 x 2 20.7 and 70.5, 2 x 4 20.7 and 67.8;
+// 8 CTAs an SM 22.5 us, and the next round's rows loaded ahead 28.9.
+constexpr int QR_BATCH = 2, QR_ROUNDS = 2;
 
 // Two floats in one register pair, and arithmetic on both at once.
 __device__ __forceinline__ uint64_t qr_pair(float x, float y) {
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(QR_NT, 7) qk_rope_vec_kernel(QkRope a, int tok
         if (there && !is_v && w) {
           const float inv = rsqrtf(ss * inv_d + a.eps);
           const uint64_t inv2 = qr_pair(inv, inv);
-          uint64_t wx[N / 2], wy[N / 2];  // (from L1: held in registers they cost occupancy: 33 us)
+          uint64_t wx[N / 2], wy[N / 2];  // (from L1: held in registers they cost occupancy: 33 us where this took 24)
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + lo), wx);
           QrVec<T>::get(*reinterpret_cast<const uint4*>(w + hi), wy);
 #pragma unroll
@@ -346,9 +348,9 @@ int qr_launch(const QkRope& a, cudaStream_t st) {
   const bool lanes = G == 2 || G == 4 || G == 8 || G == 16 || G == 32;
   const int64_t tokens = (int64_t)a.B * a.L;
   if (bits % 16 == 0 && lanes && a.R % (2 * N) == 0 && tokens <= 0x7fffffff) {
-    // a group takes up to QR_BATCH rows of its token, fewer where that would leave SMs short of
-    // CTAs (3 x 1037 tokens x 18 heads: 9.2 -> 6.9 us)
-    const int few = (heads + QR_BATCH - 1) / QR_BATCH;
+    // a group takes up to QR_ROUNDS batches of its token's rows, fewer where that would leave SMs
+    // short of CTAs (3 x 1037 tokens x 18 heads: 9.2 us with all of a batch of three, 6.4 so)
+    const int few = (heads + QR_BATCH * QR_ROUNDS - 1) / (QR_BATCH * QR_ROUNDS);
     const int64_t want = 4 * (int64_t)num_sms_current_device() * (QR_NT / G);
     const int64_t fill = (want + tokens - 1) / tokens;
     const int hpg = fill < few ? few : fill < heads ? (int)fill : heads;
