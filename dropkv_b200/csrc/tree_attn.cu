@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(TA_NT, 1)
         tc::mma_commit(bar);
         if (!two) tc::mma_commit(bar);
       };
-      auto qk = [&](uint32_t slot) {
+      auto qk = [&](uint32_t slot, bool shared = false) {
         const uint64_t kd = tc::smem_desc(ring0 + slot * L::TILE, 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -466,7 +466,10 @@ __global__ void __launch_bounds__(TA_NT, 1)
                       tc::desc_add(kd, (kk / 4) * (TA_TK * 128) + (kk % 4) * 32), ID_QK, kk > 0);
         }
         tc::mma_commit(&bars[B_S + s]);
-        release(&empty[slot]);
+        if (shared)
+          tc::mma_commit(&empty[slot]);  // the other arrival is the other group's
+        else
+          release(&empty[slot]);
       };
       if (A.q_tma) {  // every piece's Q is waited for, with work in it or without
         ok = __all_sync(0xffffffffu, wait(&bars[B_Q], pieces, 2));
@@ -479,9 +482,19 @@ __global__ void __launch_bounds__(TA_NT, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (ok) {
           tc::tc_fence_after();
-          if (tc::elect_one()) qk(slot);
+          if (tc::elect_one()) qk(slot, s == 1 && !two);
           __syncwarp();
         }
+      }
+      if (!two && s == 0 && nt > 1 && ok) {
+        // K_1 is group 1's alone, and the slot it frees takes (of five) V_2, whose landing group 0's
+        // softmax waits for where the tile has nodes. All else that lands before V_2 in a slot of it is
+        // behind this warp's products by then; K_1 is not, and as long as it is under way the barrier
+        // looks as if V_2 had landed. So this warp sees it land, before its slot is free again.
+        const uint32_t at = base + k_load(1, lead), slot = at % NS;
+        ok = __all_sync(0xffffffffu, wait(&full[slot], at / NS, 3));
+        if (ok && tc::elect_one()) tc::mbar_arrive(&empty[slot]);
+        __syncwarp();
       }
       for (int i = first; i < nt && ok; i += step) {
         const uint32_t at = base + v_load(i, lead, nt), slot = at % NS;

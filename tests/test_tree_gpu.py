@@ -166,6 +166,33 @@ def test_short_pieces_after_long_ones(long, short):
         assert torch.equal(tree_attention(Q, K, V, n), want)
 
 
+@pytest.mark.parametrize("lens", [[350], [330, 350, 450, 470, 620], [360, 900]])
+@pytest.mark.parametrize("strided_q", [False, True])
+def test_nodes_in_the_third_tile_and_past_it(lens, strided_q):
+    # segments of four tiles and more to a CTA, taken in turn, with nodes from the third tile on: the
+    # softmax of that tile looks into V while the loads before it in the slot are the other group's
+    B, Hkv, T, D = 37, 4, 64, 128
+    lens = [lens[b % len(lens)] for b in range(B)]
+    Q, K, V, n = _inputs(B, 8, Hkv, T, D, lens, torch.bfloat16, seed=21)
+    if strided_q:
+        Q = torch.stack([Q, Q], -1)[..., 0]
+    par = torch.tensor([-1] + [0] * 20 + [3] * 10 + [25] * 33)
+    mask = tree_mask_from_parents(par)[0].cuda()
+    clean = tree_attention(Q, K, V, n, tree_mask=mask)
+    some = [0, 1, 2, B - 1]
+    _close(clean[some], Q[some], K[some], V[some], [lens[b] for b in some], mask)
+    nodes = (3, 25, 40)
+    hit = torch.zeros(B, 8, T, D, dtype=torch.bool, device="cuda")
+    for b, m in enumerate(lens):
+        for i, node in enumerate(nodes):
+            V[b, :, m + node, 7 + i] = float("nan") if b % 2 else float("inf")
+            hit[b, :, mask[:, node], 7 + i] = True
+    for _ in range(20):
+        got = tree_attention(Q, K, V, n, tree_mask=mask)
+        assert torch.equal(got[~hit], clean[~hit])
+        assert not bool(got[hit].isfinite().any())
+
+
 def test_a_long_cache_in_small_pages_with_few_rows():
     lens, T = [30000, 7], 4
     Q, K, V, n = _inputs(2, 28, 4, T, 128, lens, torch.float16, seed=12)
