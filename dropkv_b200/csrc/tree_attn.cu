@@ -373,7 +373,9 @@ __global__ void __launch_bounds__(TA_NT, 1)
       for (int i = 0; i < nt; ++i) {
         const int next = a.table ? page_of(i + 1) : 0;
         const uint32_t k = base + (is_v ? v_load(i, lead, nt) : k_load(i, lead)), slot = k % NS;
-        ok = k < (uint32_t)NS || wait(&empty[slot], k / NS - 1, 1);
+        // The load before in this slot may be the other producer's. That it has landed says that the one
+        // before it had left; while that is not known, a slot two loads back looks free.
+        ok = k < (uint32_t)NS || (wait(&full[slot], k / NS - 1, 13) && wait(&empty[slot], k / NS - 1, 1));
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         uint8_t* dst = sm + L::RING + slot * L::TILE;
