@@ -53,6 +53,10 @@ __device__ __forceinline__ float lp_max_nan(float a, float b) {  // NaN if eithe
   return r;
 }
 
+// The two halves of a cluster barrier. Nothing is handed over between them: no release is needed.
+__device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
 // What a thread, a CTA or a row knows: maximum, S and A against it.
 struct LpSums {
   float m, s, t;
@@ -386,6 +390,9 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int64_t row = row0 + blockIdx.x / split;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Shared memory of another CTA may be written once that CTA is known to have begun: each says so
+  // here, and waits for the others just before its first such write.
+  if (split > 1) lp_cluster_arrive();
   if (!last) pdl_launch_dependents();
   const T* x0 = static_cast<const T*>(a.logits) + row * a.row_stride;
   // The row in vectors of 16 bytes from its first logit on, whatever its address: a thread's
@@ -541,6 +548,7 @@ __global__ void __launch_bounds__(LP_NT, LP_CTAS) logprobs_kernel(Logprobs a, in
   for (int w = 1; w < LP_WARPS; ++w) own = lp_join(own, sm.warps[w], c);
   if (TOP) cand.kept = lp_keep_best(sm.list, cand.kept, a.top_k);
   if (split > 1) {
+    lp_cluster_wait();
     LpSmem* first = cluster.map_shared_rank(&sm, 0);
     if (tid == 0) first->parts[part] = own;
     if (TOP)

@@ -161,6 +161,25 @@ def test_more_rows_than_a_wave_of_ctas_and_the_next_kernel():
         assert all(torch.equal(a, b) for a, b in zip(copies, want))
 
 
+def test_rows_split_over_clusters_beside_other_work():
+    # a row's CTAs begin when the SMs that other work holds come free; none writes into the shared
+    # memory of one that has not begun
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(40, 9000, generator=g, device="cuda").bfloat16()
+    t = torch.randint(0, 9000, (40,), generator=g, device="cuda")
+    want = _check(x, t, 20)
+    work = torch.randn(1 << 22, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = []
+    for _ in range(30):
+        with torch.cuda.stream(side):
+            work.mul_(1.0001)
+        got.append(token_logprobs(x, t, top_k=20))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for y in got for a, b in zip(y, want))
+
+
 def test_on_another_stream():
     x = torch.randn(7, 9000, device="cuda")
     t = torch.arange(7, device="cuda")
