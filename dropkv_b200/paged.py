@@ -82,12 +82,24 @@ def _on_one_device(*ts) -> int:
     return index
 
 
+def _device_of_call(args, kwargs) -> int:
+    """The index of the device of a call's first tensor, however the arguments are given; -1 if
+    that is the CPU, or there is none."""
+    for x in args:
+        if isinstance(x, torch.Tensor):
+            return x.get_device()
+    for x in kwargs.values():
+        if isinstance(x, torch.Tensor):
+            return x.get_device()
+    return -1
+
+
 def _on_its_device(fn):
-    """The call under its first tensor's device, entered only where another one is current."""
+    """The call under its tensors' device, entered only where another one is current. (That
+    all of them are on one is the call's to check.)"""
     @functools.wraps(fn)
     def call(*args, **kwargs):
-        first = args[0] if args else next(iter(kwargs.values()), None)
-        index = first.get_device() if isinstance(first, torch.Tensor) else -1
+        index = _device_of_call(args, kwargs)
         if index < 0 or index == _current_device():
             return fn(*args, **kwargs)
         with torch.cuda.device(index):

@@ -113,6 +113,50 @@ def test_cpu_tensors_are_refused():
         token_logprobs(x[0, 0], torch.arange(3))
 
 
+class _OnDevice(torch.Tensor):
+    """A tensor that says it is on CUDA device 3."""
+
+    def get_device(self):
+        return 3
+
+
+@pytest.mark.parametrize("op,arguments", [
+    (block_tables, dict(block_size=16, max_blocks=4, lens=None, free_blocks=None, max_new=4)),
+    (store_rows, dict(slots=None, K=None, V=None, K_pages=None, V_pages=None)),
+    (qk_norm_rope, dict(eps=1e-5, interleaved=True, q_weight="none", Q=None, K=None, cos=None, sin=None, positions=None)),
+    (tree_attention, dict(scale=0.1, tree_mask="none", Q=None, K=None, V=None, cache_lens=None)),
+    (token_logprobs, dict(top_k=5, temperature=0.5, logits=None, tokens=None)),
+])
+def test_calls_enter_their_tensors_device_however_the_arguments_are_given(op, arguments, monkeypatch):
+    from dropkv_b200 import paged
+    entered = []
+
+    class Entered(Exception):
+        pass
+
+    class Device:
+        def __init__(self, index):
+            entered.append(index)
+
+        def __enter__(self):
+            raise Entered
+
+        def __exit__(self, *a):
+            return False
+
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    x = torch.zeros(2).as_subclass(_OnDevice)
+    arguments = {k: x if v is None else None if v == "none" else v for k, v in arguments.items()}
+    with pytest.raises(Entered):
+        op(**arguments)
+    assert entered == [3]
+    monkeypatch.setattr(paged, "_current_device", lambda: 3)   # the current one is not entered again
+    with pytest.raises((ValueError, TypeError, RuntimeError, IndexError)):
+        op(**arguments)
+    assert entered == [3]
+
+
 def test_tree_masks_from_parents():
     par = torch.tensor([[-1, 0, 0, 1, -1, 4], [-1, 0, 1, 2, 3, 4]])
     mask, depth = tree_mask_from_parents(par)
