@@ -2,6 +2,7 @@
 // planning and the launch sequence of each public operation.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -771,8 +772,11 @@ int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int
   if (reinterpret_cast<uintptr_t>(logits) % eb) return fail(DROPKV_ERR_ARG, "logits must be aligned to their elements");
   int rc = check_ws(workspace, workspace_bytes, token_logprobs_workspace_size(N, V, top_k));
   if (rc) return rc;
-  Logprobs a{logits, row_stride, N, V, C, top_k, tokens, (float)(1.4426950408889634 / (double)temperature),
-             (float)(1.0 / (double)temperature), logprob, entropy, top_logprobs, top_tokens};
+  // A temperature under 3e-39 has an inverse past fp32's range; the largest finite one stands for it, as
+  // infinity times the largest logit's distance of 0 would be NaN.
+  const double inverse = 1.0 / (double)temperature;
+  Logprobs a{logits, row_stride, N, V, C, top_k, tokens, (float)std::min(1.4426950408889634 * inverse, (double)FLT_MAX),
+             (float)std::min(inverse, (double)FLT_MAX), logprob, entropy, top_logprobs, top_tokens};
   return launch_token_logprobs(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 

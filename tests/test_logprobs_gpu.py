@@ -104,6 +104,25 @@ def test_large_logits_do_not_overflow():
     assert bool(((got.logprob - want).abs() <= 2.0 ** -22 * want.abs() + 2.0 ** -7).all())
 
 
+@pytest.mark.parametrize("temperature", [1e-38, 2e-39, 1e-40, 1e-45])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_temperatures_whose_inverse_overflows(temperature, dtype):
+    """All of the probability is the largest logits'; the log probability of what lies 0.25 below
+    them is under -2^120, or past fp32's range."""
+    x = torch.tensor([[3.0, 2.75, -math.inf, 3.0, -5.0], [0.5, -0.25, 0.0, 0.25, -2.0]], device="cuda").to(dtype)
+    got = token_logprobs(x, torch.arange(5, device="cuda").expand(2, 5), top_k=3, temperature=temperature)
+    assert got.logprob[0, [0, 3]].tolist() == pytest.approx([-math.log(2)] * 2, abs=2.0 ** -20)
+    assert got.logprob[1, 0].item() == 0 and bool((got.logprob[0, [1, 2, 4]] < -2.0 ** 120).all())
+    assert bool((got.logprob[1, 1:] < -2.0 ** 120).all())
+    assert got.entropy.tolist() == pytest.approx([math.log(2), 0.0], abs=2.0 ** -20)
+    assert got.top_tokens.tolist() == [[0, 3, 1], [0, 3, 2]]
+    wide = torch.zeros(2, 9001, device="cuda", dtype=dtype)    # many chunks, a maximum that moves
+    wide[0, 8000], wide[1, ::2] = 1.0, -1.0
+    got = token_logprobs(wide, torch.tensor([8000, 1], device="cuda"), temperature=temperature)
+    assert got.logprob.tolist() == pytest.approx([0.0, -math.log(4500)], abs=2.0 ** -18)
+    assert got.entropy.tolist() == pytest.approx([0.0, math.log(4500)], abs=2.0 ** -18)
+
+
 def test_strides_and_leading_dimensions():
     g = torch.Generator(device="cuda").manual_seed(4)
     wide = torch.randn(6, 2 * 777 + 5, generator=g, device="cuda").bfloat16()
