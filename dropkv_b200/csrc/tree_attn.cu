@@ -1052,7 +1052,11 @@ int ta_launch(const TreeAttn& a, int dtype, void* ws, cudaStream_t st) {
   A.M = A.g * a.T;
   A.RT = (A.M + TA_ROWS - 1) / TA_ROWS;
   A.HR = a.Hkv * A.RT;
-  if ((int64_t)a.B * A.HR * ((a.cap + TA_TK - 1) / TA_TK + 1 + kTaLead) > 0x7fffffff)
+  // Keys of the last tile's boxes, units of the line and the end of the last CTA's share are counted in 32 bits.
+  if (a.cap > 0x7fffffff - 64 * TA_TK)
+    return fail(DROPKV_ERR_UNSUPPORTED, "tree attention: caches of up to %d rows are too long", a.cap);
+  const int64_t units = (int64_t)a.B * A.HR * (((int64_t)a.cap + TA_TK - 1) / TA_TK + kTaLead);
+  if (units + units / plan.ctas + plan.ctas > 0x7fffffff)
     return fail(DROPKV_ERR_UNSUPPORTED, "tree attention: %d sequences of up to %d rows are too many tiles", a.B, a.cap);
   A.box = a.table ? std::min(a.block, TA_TK) : TA_TK;
   A.rows_pad = plan.rows_pad;

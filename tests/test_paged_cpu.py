@@ -78,6 +78,20 @@ def test_tree_attention_refuses(change, code, text):
     _refused(rc, code, text)
 
 
+@pytest.mark.parametrize("B,max_blocks,block,text", [
+    (1, (1 << 28) - 1, 8, "too long"), (1, (1 << 25) - 1, 64, "too long"),   # capacities a tile short of 2^31
+    (128, (1 << 21) - 64, 1024, "too many tiles"),                          # the last CTA's share would end past 2^31
+    (512, 1 << 20, 1024, "too many tiles"),
+])
+def test_tree_attention_refuses_lines_of_tiles_past_31_bits(B, max_blocks, block, text):
+    lib, cap = _lib.load(), max_blocks * block
+    need = lib.dropkv_tree_attention_workspace_size(B, 1, 1, 1, 64, cap)
+    s = (1 << 20, 1 << 20, 64)
+    rc = lib.dropkv_tree_attention(P, 64, 64, 64, 1, P, *s, P, *s, P, max_blocks, block, 9, P, None, 0, 0, 0, 2, B, 1, 1, 1,
+                                   64, cap, 0.1, P, P, need, None)
+    _refused(rc, _lib.ERR_UNSUPPORTED, text)
+
+
 @pytest.mark.parametrize("change,text", [
     (dict(logits=None), "NULL"), (dict(tokens=None), "NULL"), (dict(dtype=5), "dtype"), (dict(V=0), "sizes"),
     (dict(top=65), "top_k"), (dict(top=-1), "top_k"), (dict(top=11, V=10), "top_k"), (dict(tau=0.0), "temperature"),
