@@ -744,7 +744,8 @@ int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_s
     return fail(DROPKV_ERR_ARG, "K/V rows must start on 16-byte boundaries");
   if (rows && (k_ss < D || v_ss < D || k_sh < D || v_sh < D || k_s0 < D || v_s0 < D))
     return fail(DROPKV_ERR_ARG, "K/V strides too small");
-  if (!(scale > 0.f)) return fail(DROPKV_ERR_ARG, "scale must be positive");
+  if (!(scale > 0.f) || std::isinf(scale * 1.4426950408889634f))  // (in units of log 2, as the kernel takes it)
+    return fail(DROPKV_ERR_ARG, "scale must be positive and finite");
   int rc = check_ws(workspace, workspace_bytes, tree_attention_workspace_size(B, Hq, Hkv, T, D, cap));
   if (rc) return rc;
   TreeAttn a{q, q_sb, q_sh, q_ss, q_sd, k, k_s0, k_sh, k_ss, v, v_s0, v_sh, v_ss, table, max_blocks, block_size, n_pages,

@@ -78,6 +78,17 @@ def test_tree_attention_refuses(change, code, text):
     _refused(rc, code, text)
 
 
+@pytest.mark.parametrize("scale", [float("inf"), 3e38])
+def test_tree_attention_refuses_scales_that_are_no_number(scale):
+    # infinity times a score of 0, or less another infinity, is NaN: no output could be told from a fault
+    lib = _lib.load()
+    need = lib.dropkv_tree_attention_workspace_size(1, 1, 1, 1, 64, 8)
+    s = (512, 512, 64)
+    rc = lib.dropkv_tree_attention(P, 64, 64, 64, 1, P, *s, P, *s, None, 0, 0, 0, P, None, 0, 0, 0, 2, 1, 1, 1, 1, 64, 8,
+                                   scale, P, P, need, None)
+    _refused(rc, _lib.ERR_ARG, "scale")
+
+
 @pytest.mark.parametrize("B,max_blocks,block,text", [
     (1, (1 << 28) - 1, 8, "too long"), (1, (1 << 25) - 1, 64, "too long"),   # capacities a tile short of 2^31
     (128, (1 << 21) - 64, 1024, "too many tiles"),                          # the last CTA's share would end past 2^31
