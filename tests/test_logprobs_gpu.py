@@ -69,6 +69,32 @@ def test_top_alternatives_in_any_order(top_k, order):
         _check(x.to(dtype).expand(2, V).contiguous(), torch.zeros(2, dtype=torch.int64, device="cuda"), top_k)
 
 
+@pytest.mark.parametrize("top_k", [1, 20, 64])
+@pytest.mark.parametrize("order", ["rising", "rising in steps", "random"])
+@pytest.mark.parametrize("dtype,first", [(torch.bfloat16, 0), (torch.bfloat16, 3), (torch.float16, 1), (torch.float32, 0),
+                                         (torch.float32, 1)])
+def test_more_candidates_than_the_list_holds(top_k, order, dtype, first):
+    """Logits that rise along rows of many chunks overflow the list of candidates, whose chunks are then
+    gone through again: rows that clusters share, and more rows than CTAs, 74 chunks each in
+    fp32. In the second kind all rows are one row of memory."""
+    V, N = 151936, 1200
+    g = torch.Generator(device="cuda").manual_seed(top_k)
+    x = torch.linspace(-30, 30, V, device="cuda")
+    x = {"rising": x, "rising in steps": (x * 8).floor() / 8, "random": x[torch.randperm(V, generator=g, device="cuda")]}[order]
+    room = torch.zeros(V + 8, dtype=dtype, device="cuda")
+    row = room[first:first + V]
+    row.copy_(x)
+    token = torch.tensor([V - 77], device="cuda")
+    one = _check(row[None], token, top_k)
+    many = token_logprobs(row.expand(N, V), token.expand(N), top_k=top_k)
+    assert bool((many.top_tokens == one.top_tokens).all())
+    # two results that are each as near to the definition as _check allows
+    run = 2 * ((V / 256 + 32) * 2.0 ** -24 + 2.0 ** -21 * (1 + 60 + math.log(V)))
+    assert float((many.logprob - one.logprob).abs().max()) <= run
+    assert float((many.top_logprobs - one.top_logprobs).abs().max()) <= run
+    assert float((many.entropy - one.entropy).abs().max()) <= 4 * run
+
+
 def test_masked_vocabularies_and_tokens_outside():
     V = 3001
     g = torch.Generator(device="cuda").manual_seed(1)

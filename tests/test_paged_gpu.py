@@ -231,6 +231,41 @@ def test_qk_norm_rope(B, Hq, Hkv, L, D, R, dtype, norm, interleaved, paged):
         assert torch.equal(pages["K_pages"], Kp) and torch.equal(pages["V_pages"], Vp)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,L,D,R", [
+    (1, 32, 8, 4096, 128, 128),   # 40 heads, 48 with V's: ten and twelve groups of two rounds of two rows
+    (3, 14, 2, 1037, 64, 32),     # seven groups a token: the second round has two rows, or four, of fourteen
+    (1, 9, 3, 4099, 128, 64),     # 12 heads, or 15: the last group's last row is missing
+    (2, 5, 1, 3001, 64, 64),      # 6 heads, or 7
+    (1, 1, 1, 9001, 128, 128),    # fewer heads than a group could take
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("norm,interleaved,paged", [(False, False, False), (True, False, False), (True, False, True),
+                                                    (True, True, False), (False, True, True)])
+def test_qk_norm_rope_over_many_tokens(B, Hq, Hkv, L, D, R, dtype, norm, interleaved, paged):
+    """Enough tokens that a group of lanes takes several of its token's rows, in several rounds."""
+    test_qk_norm_rope(B, Hq, Hkv, L, D, R, dtype, norm, interleaved, False)
+    if not paged:
+        return
+    g = torch.Generator(device="cuda").manual_seed(L)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    Q, K, V = (rnd(B, L, h, D).transpose(1, 2) for h in (Hq, Hkv, Hkv))
+    ang = torch.rand(300, R // 2, generator=g, device="cuda") * 6
+    pos = torch.randint(0, 300, (B, L), generator=g, device="cuda")
+    w = [rnd(D) if norm else None for _ in range(2)]
+    block, pages = 16, -(-B * L // 16) + 3
+    slots = _slots(B, L, pages * block, seed=L).cuda()
+    Kp, Vp = rnd(pages, Hkv, block, D), rnd(pages, Hkv, block, D)
+    want = Kp.clone().transpose(1, 2).reshape(-1, Hkv, D), Vp.clone().transpose(1, 2).reshape(-1, Hkv, D)
+    q, k = qk_norm_rope(Q, K, ang.cos(), ang.sin(), pos, q_weight=w[0], k_weight=w[1], interleaved=interleaved, V=V,
+                        slots=slots, K_pages=Kp, V_pages=Vp)
+    q2, k2 = qk_norm_rope(Q, K, ang.cos(), ang.sin(), pos, q_weight=w[0], k_weight=w[1], interleaved=interleaved)
+    assert torch.equal(q, q2) and torch.equal(k, k2)       # (checked above against the formula)
+    keep = (slots >= 0) & (slots < pages * block)
+    for to, rows, got in ((want[0], k, Kp), (want[1], V, Vp)):
+        to[slots[keep]] = rows.transpose(1, 2)[keep]
+        assert torch.equal(got.transpose(1, 2).reshape(-1, Hkv, D), to)
+
+
 def test_qk_norm_rope_shared_positions_views_and_unknown_positions():
     B, Hq, Hkv, L, D = 2, 8, 2, 11, 128
     g = torch.Generator(device="cuda").manual_seed(3)
