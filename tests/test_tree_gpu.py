@@ -151,6 +151,23 @@ def test_many_short_caches(B, Hq, Hkv, T, D, most, paged):
     assert float((got.double() - alone.double()).abs().max()) <= 2 * (u * 6 + (2 * u + 2.0 ** -13) * 6)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,T,D,most,q_tma", [
+    (90, 8, 4, 3, 128, 300, True),      # several short pieces to a CTA
+    (60, 16, 2, 16, 128, 1500, True),   # 128 rows, taken in turn, in pieces of many lengths
+    (60, 16, 2, 16, 128, 1500, False),
+    (30, 28, 4, 50, 64, 500, False),    # 350 rows: pieces of two groups of rows and of one, in one CTA
+    (24, 24, 4, 60, 128, 900, False),   # 360 rows of 128
+])
+def test_every_cache_of_a_ragged_batch(B, Hq, Hkv, T, D, most, q_tma):
+    rs = torch.Generator().manual_seed(B + T)
+    lens = torch.randint(0, most, (B,), generator=rs).tolist()
+    Q, K, V, n = _inputs(B, Hq, Hkv, T, D, lens, torch.bfloat16, seed=B + T)
+    if not q_tma:
+        Q = torch.stack([Q, Q], -1)[..., 0]
+    mask = _random_tree(T, rs, B).cuda()
+    _close(tree_attention(Q, K, V, n, tree_mask=mask), Q, K, V, lens, mask)
+
+
 @pytest.mark.parametrize("long,short", [(450, 90), (230, 60), (1000, 20)])
 def test_short_pieces_after_long_ones(long, short):
     # CTAs that end a segment of several tiles, which two groups take in turn, and go on with
