@@ -103,11 +103,16 @@ class PagedCaches:
         self.seen = torch.zeros(batch, dtype=torch.int64, device=model.device)   # tokens seen: positions go on from here
 
     def grow(self, lens, new_lens, max_new):
-        """Pages for requests of these lengths, and the slots of their new tokens."""
+        """Pages for requests of these lengths, and the slots of their new tokens. Rows without a
+        page would be left out and not seen, so a pool or a table that is too small ends the loop."""
         t = block_tables(lens, self.block, self.free, self.max_blocks, max_new, new_lens=new_lens, table=self.table,
                          held=self.held)
+        used, longest = torch.stack([t.used[0], lens.max().long()]).tolist()  # (a read back)
+        if used > len(self.free) or longest > self.max_blocks * self.block:
+            raise RuntimeError(f"{used} pages wanted of {len(self.free)} free, {longest} rows of at most "
+                               f"{self.max_blocks * self.block}")
         self.table, self.held = t.table, t.held
-        self.free = self.free[int(t.used):]  # (reads one number back)
+        self.free = self.free[used:]
         return t.slots
 
     def load(self, prompts, keep_ratio=0.3, window=8, kernel_size=11):

@@ -69,6 +69,17 @@ def test_a_step_matches_dense_attention_over_the_stored_rows(lens, tree):
         last = logits[:, 0]
 
 
+def test_a_pool_that_runs_out_of_pages_ends_the_loop():
+    model = S.Decoder(layers=1, dtype=torch.float16)
+    prompts = _prompts(model, (300, 100), 4)             # 90 and 30 rows kept: eight pages of 16
+    few = S.PagedCaches(model, 2, pages=7)
+    with pytest.raises(RuntimeError, match="8 pages wanted of 7"):
+        few.load(prompts)
+    narrow = S.PagedCaches(model, 2, pages=64, max_blocks=5)
+    with pytest.raises(RuntimeError, match="90 rows of at most 80"):
+        narrow.load(prompts)
+
+
 def test_accept_takes_the_longest_agreeing_path():
     tokens = torch.tensor([[5, 6, 7, 8, 9, 6], [1, 2, 3, 4, 4, 4]], device="cuda")
     parents = torch.tensor([[-1, 0, 0, 2, 3, 0], [-1, 0, 1, 2, 3, 4]], device="cuda")
