@@ -90,6 +90,43 @@ def test_block_tables_extends_held_pages_and_a_step_can_follow_a_step():
     assert torch.equal(b.table[:, 0][b.held > 1], a.table[:, 0][b.held > 1])
 
 
+def test_a_captured_step_moves_along_its_free_list_on_the_device():
+    """The next call wants the list without the pages already taken. Where nobody reads ``used``
+    back, the list is shifted by it on the device, and a graph of a step hands out new pages
+    every time it runs."""
+    B, T, block, wide, F = 3, 9, 4, 24, 60
+    free = torch.randperm(F, generator=torch.Generator().manual_seed(5)).int().cuda()
+    lens, held, taken = _i32([7, 0, 16]), _i32([0, 0, 0]), torch.zeros(1, dtype=torch.int64, device="cuda")
+    table = torch.full((B, wide), -1, dtype=torch.int32, device="cuda")
+    new, at = _i32([T] * B), torch.arange(F, device="cuda")
+
+    def step():
+        left = torch.where(at + taken < F, free[(at + taken).clamp(max=F - 1)], -1)
+        t = block_tables(lens + T, block, left, wide, T, new_lens=new, table=table, held=held)
+        return t, lens + T, taken + t.used
+
+    def keep(r):
+        for to, x in zip((table, held, lens, taken), (r[0].table, r[0].held, r[1], r[2])):
+            to.copy_(x)
+
+    start = [x.clone() for x in (lens, held, taken, table)]
+    keep(step())                                  # (nothing is loaded for the first time while capturing)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+        keep(got)
+    for x, y in zip((lens, held, taken, table), start):
+        x.copy_(y)
+    l, h, f, tab = [7, 0, 16], [0] * B, free.tolist(), None
+    for _ in range(5):
+        graph.replay()
+        l = [n + T for n in l]
+        tab, h, s, used = _tables_want(l, [T] * B, tab, h, f, block, wide, T)
+        f = f[used:]
+        assert got[0].table.tolist() == tab and got[0].held.tolist() == h and got[0].slots.tolist() == s
+        assert int(taken) == F - len(f)
+
+
 def test_block_tables_short_free_list():
     # 2 + 3 + 1 pages asked for, 4 there: the second request gets two of three, the third none
     got = block_tables(_i32([32, 48, 10]), 16, _i32([9, 8, 7, 6]), 4, 48)
