@@ -6,8 +6,9 @@
 // fetched once for up to 256 rows: 4 D bytes and 4 D M operations a key, which HBM
 // bounds below about 250 rows and the tensor cores above. Both products run on
 // them: S = Q K^T with Q and K in shared memory, O += P V with the weights P left in
-// tensor memory, where S was. One warp issues the TMA loads (a box per page), one
-// the products, and two groups of four warps do the softmax, a thread for each row:
+// tensor memory, where S was. A warp for K and one for V issue the TMA loads (a box per
+// page), one for each softmax group the products, and two groups of four warps do the
+// softmax, a thread for each row:
 //   * up to 128 rows: both groups have the same rows and take key tiles in turn,
 //     each with a maximum, a sum and an output of its own, joined at the end;
 //   * above: each group has 128 rows, and both use every key tile.

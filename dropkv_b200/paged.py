@@ -11,8 +11,11 @@ and decoding over it needs nothing of the host if the pages are handed out there
 
 K and V pools are ``[pages, Hkv, block_size, D]``, any strides with contiguous rows (a
 pool stored ``[pages, block_size, Hkv, D]`` is passed transposed); slot ``s`` is row
-``s % block_size`` of page ``s // block_size``. Nothing here synchronises the host. The
-reference keeps one tensor per layer (dropkv_cache.py:581-617) and has no counterparts.
+``s % block_size`` of page ``s // block_size``. No call synchronises the host. Between two steps
+``block_tables`` wants its free list without the pages already taken, whose number is on the
+device: a loop reads it back, or shifts the list there (see ``block_tables``). Nothing here takes
+pages back. The reference keeps one tensor per layer (dropkv_cache.py:581-617) and has no
+counterparts.
 """
 
 from __future__ import annotations
@@ -157,9 +160,13 @@ def block_tables(lens: torch.Tensor, block_size: int, free_blocks: torch.Tensor,
     ``table`` [B, max_blocks] int32 with ``held`` [B] int32 are the pages that the
     requests hold already; the missing ones are taken from ``free_blocks`` [F] int32
     in order, request after request. Returns new tensors (``BlockTables``); the
-    caller drops the first ``used`` entries of its free list. Where the list runs
-    short, entries and slots are -1, ``held`` counts the pages really held and
-    ``used`` is more than F.
+    caller drops the first ``used`` entries of its free list: by reading ``used`` back, or,
+    where a step is captured in a CUDA graph, by shifting the list on the device
+    (``torch.where(i + taken < F, free[(i + taken).clamp(max=F - 1)], -1)`` for
+    ``i = arange(F)``). A request takes at most ``max_blocks`` pages; its tokens past them
+    get no slots. Where the list runs short, entries and slots are -1, ``held`` counts the
+    pages really held and ``used`` is more than F. (A page of -1 in the list counts as held,
+    and gives slots of -1.)
     """
     if (table is None) != (held is None):
         raise ValueError("table and held go together")
@@ -200,7 +207,9 @@ def store_rows(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: t
                V_pages: torch.Tensor) -> None:
     """Rows of K and V [B, Hkv, N, D] (any strides, rows of D contiguous) to slots [B, N]
     (int64) of the pools, in place; rows whose slot is outside the pool (-1) are left
-    out. Where rows share a slot, any of them may stay. fp32, fp16 or bf16."""
+    out. Rows go in no order: those that share a slot leave a mixture of them there, and
+    K and V must not lie where rows are written, such as in the same pages (move rows
+    within a pool by way of a copy). fp32, fp16 or bf16."""
     dev = _on_one_device(K, V, slots, K_pages, V_pages)
     ks, dtype = K.shape, K.dtype
     if len(ks) != 4 or ks != V.shape:
@@ -284,8 +293,8 @@ def qk_norm_rope(Q: torch.Tensor, K: torch.Tensor, cos: torch.Tensor, sin: torch
     k_out = _new(dtype, device, B, Hkv, L, D)
     rc = _lib.load().dropkv_qk_norm_rope(
         Q.data_ptr(), *_rows_strides(Q, "Q"), K.data_ptr(), *_rows_strides(K, "K"),
-        qw_ptr, kw_ptr, float(eps), cos.data_ptr(), sin.data_ptr(), cs[0], 2 * cs[1], int(bool(interleaved)), positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L,
-        D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
+        qw_ptr, kw_ptr, float(eps), cos.data_ptr(), sin.data_ptr(), cs[0], 2 * cs[1], int(bool(interleaved)),
+        positions.data_ptr(), pos_sb, dt, B, Hq, Hkv, L, D, q_out.data_ptr(), k_out.data_ptr(), *tail, _raw_stream(dev))
     if rc:
         _lib.check(rc, "dropkv_qk_norm_rope")
     return q_out, k_out
@@ -318,7 +327,8 @@ def tree_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cache_lens
     tree's own K/V rows in node order. Node i sees every cached row and the nodes j with
     ``tree_mask[i, j]`` (bool [T, T] or [B, T, T]; None: j <= i, a chain). K and V are
     row buffers [B, Hkv, cap, D] or, with ``block_table`` ([B, max_blocks] int32), pools
-    [pages, Hkv, block_size, D]; any strides with contiguous rows on 16-byte boundaries.
+    [pages, Hkv, block_size, D]; any strides with contiguous rows on 16-byte boundaries that
+    do not overlap (no broadcast heads or sequences).
     Rows past the capacity are not seen, nor are those on missing pages (-1); a node that
     sees nothing gives zeros; what is in rows that no node sees does not matter. bf16 or
     fp16, D 64 or 128, T <= 256, block_size a power of two from 8 to 1024. Products of 16
@@ -384,7 +394,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     bf16): log probabilities of ``tokens`` (int64, [...] or [..., C]; -inf for one outside
     [0, V), such as a draft tree's padding), the entropy of each row, and its ``top_k``
     (at most 64) likeliest tokens, best first, ties to the lower index. fp32 sums and
-    results. A row that holds NaN or +inf, or nothing but -inf, gives NaN."""
+    results. A row that holds NaN or +inf, or nothing but -inf, gives NaN. Rows of
+    contiguous logits at one stride are read where they are; where the leading dimensions
+    do not merge into one (``logits[:, :-1]`` of a batch of several) the logits are copied
+    first, which costs more than the call: pass a sequence at a time, or all positions."""
     dev = _on_one_device(logits, tokens)
     dt = _DTYPE_CODE.get(logits.dtype)
     if dt is None:

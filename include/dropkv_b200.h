@@ -329,8 +329,9 @@ DROPKV_API int dropkv_block_tables(const int32_t* lens, const int32_t* new_lens,
 
 /* k_pages / v_pages row slots[b, n] = row n of K / V [B, Hkv, N, D] for every head;
  * slots outside the pool are skipped. Element strides: k_s* / v_s* of a sequence,
- * head and row, kp_s* / vp_s* of a page, head and row. elem_bytes 2 or 4. Of rows
- * with one slot any may stay. */
+ * head and row, kp_s* / vp_s* of a page, head and row. elem_bytes 2 or 4. Rows go in
+ * no order: rows with one slot leave a mixture, and K and V must not lie where rows
+ * are written. */
 DROPKV_API int dropkv_store_rows(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sb,
                                  int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages, int64_t kp_sb,
                                  int64_t kp_sh, int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh,
@@ -363,7 +364,8 @@ DROPKV_API int dropkv_qk_norm_rope(const void* q, int64_t q_sb, int64_t q_sh, in
  * row that sees nothing gives zeros; keys on pages outside the pool are not seen.
  * A row that no node sees is not used, whatever it holds. bf16 or fp16, D 64 or 128,
  * T <= 256, block_size a power of two from 8 to 1024, K/V rows on 16-byte
- * boundaries; out [B, Hq, T, D] contiguous. */
+ * boundaries and not overlapping, B * Hkv <= 65535, cap <= 2^31 - 8193, scale
+ * positive and finite; out [B, Hq, T, D] contiguous. */
 DROPKV_API size_t dropkv_tree_attention_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
 DROPKV_API int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd,
                                      const void* k, int64_t k_s0, int64_t k_sh, int64_t k_ss, const void* v,
@@ -377,6 +379,7 @@ DROPKV_API int dropkv_tree_attention(const void* q, int64_t q_sb, int64_t q_sh, 
  * p = softmax(logits / temperature): logprob[N, C] = log p of tokens[N, C] (-inf for
  * a token outside [0, V)), entropy[N] = -sum p log p, and the top_k (0 to 64) most
  * likely tokens, best first, ties to the lower index, with their log probabilities.
+ * temperature positive and finite (under 3e-39 it acts as that). No workspace is needed.
  * A row with NaN or +inf, or of -inf alone, gives NaN (top_tokens order NaN first). */
 DROPKV_API size_t dropkv_token_logprobs_workspace_size(int64_t N, int V, int top_k);
 DROPKV_API int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t N, int V,
