@@ -121,10 +121,10 @@ struct SrArgs {
 // Rows of LANES 16-byte vectors: LANES threads have a row, SR_ROWS rows each, whose slots,
 // then K and V vectors, are on their way at once. Rows follow one another along a head, so
 // reads are one stream and writes come in runs of a page's rows. HBM bounds it: each byte is
-// read and written once. One layer's 13107 rows (8 heads of 128, bf16, 107 MB): 18.8 us alone,
-// 16.8 us one after another in a graph (6.4 TB/s, 97% of a copy's); rows in flight 1, 2, 4, 8: 18.7, 18.8,
-// 19.4, 20.4 us, and a few hundred rows 1.8, 2.2, 3.0, 4.2 us; 2 for the heads of 64, where
-// 1 row is slower (16.8 us against 15.7).
+// read and written once. One layer's 13107 rows (8 heads of 128, bf16, 107 MB): 18.8 us alone
+// (5.7 TB/s, 87% of a copy's rate), 19.3 us in a graph over inputs larger than L2; rows in flight 1,
+// 2, 4, 8: 18.7, 18.8, 19.4, 20.4 us alone, and a few hundred rows 1.8, 2.2, 3.0, 4.2 us; 2 for the
+// heads of 64, where 1 row is slower (16.8 us against 15.7 over one set of rows, in part in L2).
 constexpr int SR_ROWS = 2;
 
 template <int LANES>

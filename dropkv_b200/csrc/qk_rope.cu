@@ -90,9 +90,9 @@ __global__ void __launch_bounds__(QR_NT) qk_rope_rows_kernel(QkRope a) {
 // in fact it is instructions, and the latency of the chains position - table row - rows. So
 // arithmetic is done on two floats at once, as many CTAs are resident as registers allow without
 // spilling, and a group takes several rounds of rows for one look at the tables. 4096 tokens x 40
-// heads of 128, bf16, normed (84 MB): 18.8 us, 4.5 TB/s (68% of a copy's rate), without a norm
-// 14.7 (87%); 16384 tokens 72 us (4.7 TB/s). Rows on their way x rounds, for 4096 and 16384
-// tokens: 2 x 2 18.8 and 71.7 us, 3 x 1 21.2 and 80.3, 3 x 2 20.7 and 70.5, 2 x 4 20.7 and 67.8;
+// heads of 128, bf16, normed (86 MB with the tables): 19.9 us, 4.3 TB/s (66% of a copy's rate), without
+// a norm 15.6 (84%), in a graph over inputs larger than L2; 16384 tokens 72 us (4.7 TB/s). Rows on
+// their way x rounds, for 4096 (one set of inputs, in part in L2) and 16384 tokens: 2 x 2 18.8 and 71.7 us, 3 x 1 21.2 and 80.3, 3 x 2 20.7 and 70.5, 2 x 4 20.7 and 67.8;
 // 8 CTAs an SM 22.5 us, and the next round's rows loaded ahead 28.9.
 constexpr int QR_BATCH = 2, QR_ROUNDS = 2;
 

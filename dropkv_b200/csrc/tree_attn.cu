@@ -26,14 +26,15 @@
 // are in fp32.
 //
 // What it measured alone: 295K keys in 8 sequences x 4 KV heads x 224 rows of 128, fp16 (135
-// GFLOP, 604 MB): 151 us, 890 TFLOP/s (54% of a matrix product's burst rate) and 4.0 TB/s
-// (61% of a copy's); call after call 170 to 200 us, as the clock falls under load. What bounds
+// GFLOP, 604 MB): 150 us, 900 TFLOP/s (55% of a matrix product's burst rate) and 4.0 TB/s
+// (61% of a copy's); with the merge, one after another in a graph, 166 to 178 us, and 200 from
+// Python, as the clock falls under load. What bounds
 // it is the chain of a group's tile, 3800 cycles: from S to its last weights 2500 (480 for the
 // first half's logits and maximum, 1000 a half for weights), 440 until the products are
 // issued, 860 until the next S is there; the other group's runs beside it. The tile's four
 // products take 2048, its loads 2800 at a copy's rate. 13107 keys x 256 rows x 8 heads, bf16:
-// 26 us with the merge, of which the tiles are 11; the rest is the launch, the first tiles, the
-// partials (20 MB out and in) and the merge.
+// 26 us, of which the tiles are 11; the rest is the start, the first tiles and the partials (20 MB
+// out). With the merge 31 us in a graph, 33 over inputs larger than L2.
 #include <algorithm>
 #include <type_traits>
 
