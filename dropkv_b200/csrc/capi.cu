@@ -781,5 +781,73 @@ int dropkv_token_logprobs(const void* logits, int64_t row_stride, int dtype, int
   return launch_token_logprobs(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------------------
+// Caches in 8 bits
+// ---------------------------------------------------------------------------
+// The pool of an entry point, settled and checked.
+static int make_fp8_pool(Fp8Pool* p, const void* k, int64_t k_s0, int64_t k_sh, int64_t k_st, const void* v, int64_t v_s0,
+                         int64_t v_sh, int64_t v_st, const float* k_scale, int64_t ks_s0, int64_t ks_sh,
+                         const float* v_scale, int64_t vs_s0, int64_t vs_sh, int n_pages, int block_size, int Hkv, int D) {
+  if (Hkv < 1 || D < 1 || n_pages < 0 || block_size < 1)
+    return fail(DROPKV_ERR_ARG, "invalid sizes Hkv=%d D=%d pages=%d block_size=%d", Hkv, D, n_pages, block_size);
+  settle_strides(n_pages, Hkv, block_size, D, &k_s0, &k_sh, &k_st);
+  settle_strides(n_pages, Hkv, block_size, D, &v_s0, &v_sh, &v_st);
+  if (Hkv <= 1) ks_sh = vs_sh = 1;
+  if (n_pages <= 1) ks_s0 = Hkv * ks_sh, vs_s0 = Hkv * vs_sh;
+  if (n_pages > 0 && (!k || !v || !k_scale || !v_scale)) return fail(DROPKV_ERR_ARG, "pages and scales must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 4)
+    return fail(DROPKV_ERR_ARG, "scales must be aligned to their elements");
+  *p = Fp8Pool{const_cast<void*>(k), k_s0, k_sh, k_st, const_cast<void*>(v), v_s0, v_sh, v_st,
+               const_cast<float*>(k_scale), ks_s0, ks_sh, const_cast<float*>(v_scale), vs_s0, vs_sh, n_pages, block_size, Hkv, D};
+  return DROPKV_OK;
+}
+
+int dropkv_store_rows_fp8(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v, int64_t v_sb,
+                          int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages, int64_t kp_sb, int64_t kp_sh,
+                          int64_t kp_st, void* v_pages, int64_t vp_sb, int64_t vp_sh, int64_t vp_st, float* k_scales,
+                          int64_t ks_sb, int64_t ks_sh, float* v_scales, int64_t vs_sb, int64_t vs_sh, int n_pages,
+                          int block_size, int dtype, int B, int Hkv, int N, int D, void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (!eb) return fail(DROPKV_ERR_ARG, "unknown dtype %d", dtype);
+  if (B < 0 || N < 0) return fail(DROPKV_ERR_ARG, "invalid sizes B=%d N=%d", B, N);
+  StoreRowsFp8 s;
+  int rc = make_fp8_pool(&s.pool, k_pages, kp_sb, kp_sh, kp_st, v_pages, vp_sb, vp_sh, vp_st, k_scales, ks_sb, ks_sh,
+                         v_scales, vs_sb, vs_sh, n_pages, block_size, Hkv, D);
+  if (rc) return rc;
+  if (B == 0 || N == 0 || n_pages == 0) return DROPKV_OK;  // nothing to store, or nowhere
+  if (!k || !v || !slots) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % eb)
+    return fail(DROPKV_ERR_ARG, "rows must be aligned to their elements");
+  settle_strides(B, Hkv, N, D, &k_sb, &k_sh, &k_sn);
+  settle_strides(B, Hkv, N, D, &v_sb, &v_sh, &v_sn);
+  s.k = k, s.k_sb = k_sb, s.k_sh = k_sh, s.k_sn = k_sn;
+  s.v = v, s.v_sb = v_sb, s.v_sh = v_sh, s.v_sn = v_sn;
+  s.slots = slots;
+  s.B = B, s.N = N;
+  return launch_store_rows_fp8(s, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t kp_sh, int64_t kp_st, const void* v_pages,
+                         int64_t vp_sb, int64_t vp_sh, int64_t vp_st, const float* k_scales, int64_t ks_sb,
+                         int64_t ks_sh, const float* v_scales, int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size,
+                         const int64_t* slots, int dtype, int B, int Hkv, int N, int D, void* k_out, void* v_out,
+                         void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (!eb) return fail(DROPKV_ERR_ARG, "unknown dtype %d", dtype);
+  if (B < 0 || N < 0) return fail(DROPKV_ERR_ARG, "invalid sizes B=%d N=%d", B, N);
+  LoadRowsFp8 s;
+  int rc = make_fp8_pool(&s.pool, k_pages, kp_sb, kp_sh, kp_st, v_pages, vp_sb, vp_sh, vp_st, k_scales, ks_sb, ks_sh,
+                         v_scales, vs_sb, vs_sh, n_pages, block_size, Hkv, D);
+  if (rc) return rc;
+  if (B == 0 || N == 0) return DROPKV_OK;
+  if (!slots || !k_out || !v_out) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % eb)
+    return fail(DROPKV_ERR_ARG, "rows must be aligned to their elements");
+  s.slots = slots;
+  s.k_out = k_out, s.v_out = v_out;
+  s.B = B, s.N = N;
+  return launch_load_rows_fp8(s, dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 

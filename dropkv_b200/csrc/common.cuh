@@ -297,4 +297,41 @@ struct Logprobs {
 size_t token_logprobs_workspace_size(int64_t N, int V, int top_k);
 int launch_token_logprobs(const Logprobs& a, int dtype, void* ws, cudaStream_t st);
 
+// ---------------------------------------------------------------------------
+// Caches in 8 bits (fp8_rows.cu, fp8_attn.cu, fp8_decode.cu) and the verification of drafts
+// (verify.cu). A pool: pages [n_pages, H, block, D] of e4m3, strides in elements (bytes), and
+// a scale for each page and head, [n_pages, H].
+// ---------------------------------------------------------------------------
+struct Fp8Pool {
+  void* k;
+  int64_t k_s0, k_sh, k_st;
+  void* v;
+  int64_t v_s0, v_sh, v_st;
+  float* k_scale;
+  int64_t ks_s0, ks_sh;
+  float* v_scale;
+  int64_t vs_s0, vs_sh;
+  int n_pages, block, H, D;
+};
+
+struct StoreRowsFp8 {
+  const void* k;  // [B, H, N, D]
+  int64_t k_sb, k_sh, k_sn;
+  const void* v;
+  int64_t v_sb, v_sh, v_sn;
+  const int64_t* slots;  // [B, N]
+  Fp8Pool pool;
+  int B, N;
+};
+int launch_store_rows_fp8(const StoreRowsFp8& q, int dtype, cudaStream_t st);
+
+struct LoadRowsFp8 {
+  Fp8Pool pool;
+  const int64_t* slots;  // [B, N]
+  void* k_out;           // [B, H, N, D], contiguous
+  void* v_out;
+  int B, N;
+};
+int launch_load_rows_fp8(const LoadRowsFp8& q, int dtype, cudaStream_t st);
+
 }  // namespace dropkv

@@ -1,0 +1,105 @@
+"""Paged K/V caches in 8 bits (tensor functions over the C ABI).
+
+Pools are ``[pages, Hkv, block_size, D]`` of ``torch.float8_e4m3fn`` (any strides with
+contiguous rows), with a scale for each page and head of K and of V, ``[pages, Hkv]``
+float32: a row's value is its 8 bits times its page's scale. Pages, slots and tables are
+those of ``dropkv_b200.paged``; ``block_tables`` hands them out.
+
+* ``store_rows_fp8`` -- K/V rows to slots, quantised;
+* ``load_rows_fp8``  -- rows at slots, read back.
+
+Scales are powers of two, so that the 8 bits' rounding (2^-4 of a value) is the only one:
+what is read back is exact in 16 bits, and a page whose scale grows keeps its rows but for
+those bits that fall under the new scale's smallest steps. No call synchronises the host. The
+reference's cache holds the model's own type only (dropkv_cache.py:581-617).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ops import _DTYPE_CODE
+from .paged import _ints, _new, _on_its_device, _on_one_device, _raw_stream, _rows_strides
+
+__all__ = ["store_rows_fp8", "load_rows_fp8"]
+
+
+def _check_pool_fp8(K_pages, V_pages, K_scales, V_scales):
+    """The pools' shape [pages, Hkv, block_size, D], and the pointers and strides of pages and scales."""
+    shape = K_pages.shape
+    if len(shape) != 4 or shape != V_pages.shape:
+        raise ValueError(f"expected K and V pages [pages, Hkv, block_size, D] of one shape, got {tuple(shape)} and "
+                         f"{tuple(V_pages.shape)}")
+    if K_pages.dtype != torch.float8_e4m3fn or V_pages.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"pages must be torch.float8_e4m3fn, got {K_pages.dtype} and {V_pages.dtype}")
+    for s in (K_scales, V_scales):
+        if s.dtype != torch.float32:
+            raise TypeError(f"scales must be float32, got {s.dtype}")
+        if s.shape != shape[:2]:
+            raise ValueError(f"scales must be {tuple(shape[:2])} (pages, heads), got {tuple(s.shape)}")
+    return shape, (K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
+                   *_rows_strides(V_pages, "V_pages"), K_scales.data_ptr(), *K_scales.stride(), V_scales.data_ptr(),
+                   *V_scales.stride())
+
+
+@_on_its_device
+def store_rows_fp8(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
+                   K_scales: torch.Tensor, V_scales: torch.Tensor) -> None:
+    """Rows of K and V [B, Hkv, N, D] (fp32, fp16 or bf16; any strides, rows of D contiguous)
+    to slots [B, N] (int64) of pools in 8 bits, in place; rows whose slot is outside the pool
+    (-1) are left out.
+
+    A page's scale becomes the smallest power of two that brings the call's largest value in it
+    to at most 448, unless it is more already; rows that stand in the page follow a scale that
+    grows. A call that writes a page's row 0 starts the page: what stood in it before means
+    nothing, and its scale is the call's alone. Values are rounded to nearest, ties to even, NaN
+    stays NaN and infinities (e4m3 has none) become NaN.
+
+    The rows of one page belong to one sequence of the call and follow one another there, as
+    ``block_tables`` hands slots out, with fewer than 256 rows without a slot between two of them;
+    otherwise, and where rows share a slot, that page's contents are unspecified. K and V must not
+    lie in the pages. block_size is at most 1024.
+    """
+    dev = _on_one_device(K, V, slots, K_pages, V_pages, K_scales, V_scales)
+    ks, dtype = K.shape, K.dtype
+    if len(ks) != 4 or ks != V.shape:
+        raise ValueError("expected K, V [B, Hkv, N, D] of one shape")
+    dt = _DTYPE_CODE.get(dtype)
+    if dt is None or V.dtype != dtype:
+        raise TypeError(f"K and V must share one of fp32/fp16/bf16; got {dtype}, {V.dtype}")
+    B, Hkv, N, D = ks
+    ps, pool = _check_pool_fp8(K_pages, V_pages, K_scales, V_scales)
+    if ps[1] != Hkv or ps[3] != D:
+        raise ValueError(f"rows of {Hkv} heads of {D} do not fit pages {tuple(ps)}")
+    slots = _ints(slots, torch.int64, (B, N), "slots")
+    rc = _lib.load().dropkv_store_rows_fp8(
+        K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(), *pool, ps[0], ps[2],
+        dt, B, Hkv, N, D, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_store_rows_fp8")
+
+
+@_on_its_device
+def load_rows_fp8(K_pages: torch.Tensor, V_pages: torch.Tensor, K_scales: torch.Tensor, V_scales: torch.Tensor,
+                  slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """(K, V) [B, Hkv, N, D] in ``dtype`` (fp32, fp16 or bf16): the rows at slots [B, N] (int64)
+    of pools in 8 bits, zeros where a slot is outside the pool (-1). Exact in every dtype unless
+    a value is outside its range."""
+    dev = _on_one_device(K_pages, V_pages, K_scales, V_scales, slots)
+    dt = _DTYPE_CODE.get(dtype)
+    if dt is None:
+        raise TypeError(f"dtype must be fp32/fp16/bf16; got {dtype}")
+    ps, pool = _check_pool_fp8(K_pages, V_pages, K_scales, V_scales)
+    if slots.dim() != 2:
+        raise ValueError(f"slots must be [B, N], got {tuple(slots.shape)}")
+    B, N = slots.shape
+    slots = _ints(slots, torch.int64, (B, N), "slots")
+    device = K_pages.device
+    k_out = _new(dtype, device, B, ps[1], N, ps[3])
+    v_out = _new(dtype, device, B, ps[1], N, ps[3])
+    rc = _lib.load().dropkv_load_rows_fp8(*pool, ps[0], ps[2], slots.data_ptr(), dt, B, ps[1], N, ps[3], k_out.data_ptr(),
+                                          v_out.data_ptr(), _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_load_rows_fp8")
+    return k_out, v_out

@@ -387,6 +387,36 @@ DROPKV_API int dropkv_token_logprobs(const void* logits, int64_t row_stride, int
                                      float* entropy, float* top_logprobs, int64_t* top_tokens, void* workspace,
                                      size_t workspace_bytes, void* stream);
 
+/* ---- Paged caches in 8 bits ---------------------------------------------------
+ * Pages of e4m3 [n_pages, Hkv, block_size, D] (element strides, rows of D contiguous)
+ * and one fp32 scale for each page and head of K and of V ([n_pages, Hkv], element
+ * strides): a row's value is e4m3 * scale. The scales written here are powers of two. */
+
+/* Rows of K / V [B, Hkv, N, D] (fp32, fp16 or bf16) to slots[B, N], quantised: a page's
+ * scale becomes the smallest power of two (at least 2^-126) that brings the largest finite
+ * value of the call's rows in it to at most 448, or, where the call does not write the page's
+ * row 0, stays as it is if that is more; where it grows, the rows that the call does not
+ * write are rounded to it. A call that writes a page's row 0 starts the page: what its other
+ * rows held means nothing from then on. Values are rounded to nearest, ties to even; infinities
+ * become NaN. Slots outside the pool are skipped. The rows of one page must belong to one
+ * sequence of the call and follow one another there, with fewer than 256 rows without a slot
+ * between two of them; else, and where rows share a slot, the page's contents are unspecified.
+ * K and V must not lie in the pages. block_size <= 1024. */
+DROPKV_API int dropkv_store_rows_fp8(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v,
+                                     int64_t v_sb, int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages,
+                                     int64_t kp_sb, int64_t kp_sh, int64_t kp_st, void* v_pages, int64_t vp_sb,
+                                     int64_t vp_sh, int64_t vp_st, float* k_scales, int64_t ks_sb, int64_t ks_sh,
+                                     float* v_scales, int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size,
+                                     int dtype, int B, int Hkv, int N, int D, void* stream);
+
+/* k_out / v_out [B, Hkv, N, D] (contiguous, fp32, fp16 or bf16): the rows at slots[B, N],
+ * rounded once; zeros where a slot is outside the pool. */
+DROPKV_API int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t kp_sh, int64_t kp_st,
+                                    const void* v_pages, int64_t vp_sb, int64_t vp_sh, int64_t vp_st,
+                                    const float* k_scales, int64_t ks_sb, int64_t ks_sh, const float* v_scales,
+                                    int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size, const int64_t* slots,
+                                    int dtype, int B, int Hkv, int N, int D, void* k_out, void* v_out, void* stream);
+
 /* Diagnostic: one 128-row tile through a tcgen05 MMA form used by the fused
  * scorer (mode 0: out[128][n] = A[128][128] B[n][128]^T with A loaded by TMA;
  * mode 1: out[128][n] = A[128][128]^T B[n][128]^T with A read MN-major; modes 2/3:
