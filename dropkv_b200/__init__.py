@@ -24,7 +24,7 @@ Public API (the reference's names and semantics):
 
 from ._lib import DropKVError, version
 from .cache import DropKVCache, prefill_chunked
-from .fp8_cache import load_rows_fp8, store_rows_fp8
+from .fp8_cache import attention_fp8, load_rows_fp8, store_rows_fp8
 from .ops import (Compressor, HostPipeline, VarlenCompressor, compress, compress_varlen, decode_append_attention,
                   decode_attention, dropkv_scores_cuda, gather_compressed, scores, select_keep_indices)
 from .paged import (BlockTables, TokenLogprobs, block_tables, qk_norm_rope, store_rows, token_logprobs,
@@ -38,5 +38,6 @@ __all__ = [
     "compress", "decode_attention", "decode_append_attention", "dropkv_scores_cuda", "dropkv_scores_triton", "gather_compressed",
     "scores", "select_keep_indices", "Compressor", "HostPipeline", "VarlenCompressor", "compress_varlen",
     "BlockTables", "TokenLogprobs", "block_tables", "qk_norm_rope", "store_rows", "token_logprobs", "tree_attention",
-    "tree_mask_from_parents", "load_rows_fp8", "store_rows_fp8",
+    "tree_mask_from_parents", "attention_fp8", "load_rows_fp8",
+    "store_rows_fp8",
 ]

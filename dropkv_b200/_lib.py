@@ -95,6 +95,10 @@ SIGNATURES = {
                               + ([_c_p] + [_c_i64] * 2) * 2 + [_c_int] * 7 + [_c_p]),
     "dropkv_load_rows_fp8": (_c_int, ([_c_p] + [_c_i64] * 3) * 2 + ([_c_p] + [_c_i64] * 2) * 2
                              + [_c_int, _c_int, _c_p] + [_c_int] * 5 + [_c_p] * 3),
+    "dropkv_attention_fp8_workspace_size": (_c_sz, [_c_int] * 6),
+    "dropkv_attention_fp8": (_c_int, [_c_p] + [_c_i64] * 4 + ([_c_p] + [_c_i64] * 3) * 2 + ([_c_p] + [_c_i64] * 2) * 2
+                             + [_c_int, _c_int, _c_p, _c_int, _c_p, _c_p] + [_c_i64] * 3 + [_c_int] * 8
+                             + [_c_f, _c_p, _c_p, _c_sz, _c_p]),
     "dropkv_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_i64, _c_int, _c_p, _c_int, _c_int, _c_f]
                               + [_c_p] * 5 + [_c_sz, _c_p]),
 }

@@ -849,5 +849,68 @@ int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t kp_sh, int6
   return launch_load_rows_fp8(s, dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
+static bool attn_fp8_sizes_ok(int B, int Hq, int Hkv, int T, int D, int cap) {
+  return B >= 1 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128 && T >= 1 && (D == 64 || D == 128) && cap >= 0 &&
+         (int64_t)B * Hkv <= 65535 && (int64_t)Hq * T <= (1 << 26);
+}
+
+size_t dropkv_attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
+  return attn_fp8_sizes_ok(B, Hq, Hkv, T, D, cap) ? attention_fp8_workspace_size(B, Hq, Hkv, T, D, cap) : 0;
+}
+
+int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd, const void* k_pages,
+                         int64_t kp_sb, int64_t kp_sh, int64_t kp_st, const void* v_pages, int64_t vp_sb, int64_t vp_sh,
+                         int64_t vp_st, const float* k_scales, int64_t ks_sb, int64_t ks_sh, const float* v_scales,
+                         int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size, const int32_t* table, int max_blocks,
+                         const int32_t* cache_lens, const uint8_t* mask, int64_t mask_sb, int64_t mask_sr,
+                         int64_t mask_sc, int window, int sinks, int dtype, int B, int Hq, int Hkv, int T, int D,
+                         float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !cache_lens || !out) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if (dtype != DROPKV_DTYPE_BF16 && dtype != DROPKV_DTYPE_F16)
+    return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8 takes bf16 or fp16 queries");
+  if (D != 64 && D != 128) return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8 needs D of 64 or 128 (got %d)", D);
+  if (block_size < 8 || block_size > 1024 || (block_size & (block_size - 1)))
+    return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8 needs a block_size that is a power of two from 8 to 1024 (got %d)", block_size);
+  if (max_blocks < 0 || (int64_t)max_blocks * block_size > 0x7fffffff - 65536)
+    return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8: caches of up to %lld rows are too long", (long long)max_blocks * block_size);
+  const int cap = max_blocks * block_size;
+  if (Hkv >= 1 && Hq >= 1 && Hq / Hkv > 128)
+    return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8 takes at most 128 query heads a KV head (got %d)", Hq / Hkv);
+  if (!attn_fp8_sizes_ok(B, Hq, Hkv, T, D, cap))
+    return fail(DROPKV_ERR_ARG, "invalid sizes B=%d Hq=%d Hkv=%d T=%d max_blocks=%d", B, Hq, Hkv, T, max_blocks);
+  if (mask && T > 256) return fail(DROPKV_ERR_UNSUPPORTED, "a tree_mask takes at most 256 nodes (got %d)", T);
+  if (window < 0 || sinks < 0) return fail(DROPKV_ERR_ARG, "window and sinks must not be negative");
+  if (mask && window && window < T)
+    return fail(DROPKV_ERR_ARG, "a window must hold the whole tree: window %d, %d nodes", window, T);
+  AttnFp8 a;
+  int rc = make_fp8_pool(&a.pool, k_pages, kp_sb, kp_sh, kp_st, v_pages, vp_sb, vp_sh, vp_st, k_scales, ks_sb, ks_sh,
+                         v_scales, vs_sb, vs_sh, n_pages, block_size, Hkv, D);
+  if (rc) return rc;
+  if (cap > 0 && !table) return fail(DROPKV_ERR_ARG, "table must be non-NULL");
+  const Fp8Pool& p = a.pool;
+  if ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) % 16 ||
+      (p.k_s0 | p.k_sh | p.k_st | p.v_s0 | p.v_sh | p.v_st) % 16)
+    return fail(DROPKV_ERR_ARG, "page rows must start on 16-byte boundaries");
+  const bool rows = cap > 0 && n_pages > 0;
+  if (rows && (p.k_st < D || p.v_st < D || p.k_sh < D || p.v_sh < D || p.k_s0 < D || p.v_s0 < D))
+    return fail(DROPKV_ERR_ARG, "page strides too small");
+  if (reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(out) % 16)
+    return fail(DROPKV_ERR_ARG, "queries must be aligned to their elements, outputs to 16 bytes");
+  if (!(scale > 0.f) || std::isinf(scale * 1.4426950408889634f))  // (in units of log 2, as the kernel takes it)
+    return fail(DROPKV_ERR_ARG, "scale must be positive and finite");
+  rc = check_ws(workspace, workspace_bytes, attention_fp8_workspace_size(B, Hq, Hkv, T, D, cap));
+  if (rc) return rc;
+  a.q = q, a.q_sb = q_sb, a.q_sh = q_sh, a.q_ss = q_ss, a.q_sd = q_sd;
+  a.table = table, a.max_blocks = max_blocks;
+  a.cache_lens = cache_lens;
+  a.mask = mask, a.mask_sb = mask_sb, a.mask_sr = mask_sr, a.mask_sc = mask_sc;
+  a.window = window, a.sinks = window ? sinks : 0;
+  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.T = T, a.D = D;
+  a.cap = rows ? cap : 0;
+  a.scale = scale;
+  a.out = out;
+  return launch_attention_fp8(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 

@@ -334,4 +334,22 @@ struct LoadRowsFp8 {
 };
 int launch_load_rows_fp8(const LoadRowsFp8& q, int dtype, cudaStream_t st);
 
+struct AttnFp8 {
+  const void* q;  // [B, Hq, T, D]
+  int64_t q_sb, q_sh, q_ss, q_sd;
+  Fp8Pool pool;
+  const int32_t* table;  // [B, max_blocks]
+  int max_blocks;
+  const int32_t* cache_lens;  // [B]
+  const uint8_t* mask;        // [B, T, T] truth values, or nullptr: a chain
+  int64_t mask_sb, mask_sr, mask_sc;
+  int window, sinks;  // window 0: every row is seen
+  int B, Hq, Hkv, T, D;
+  int cap;  // rows a sequence's cache can hold: max_blocks * block
+  float scale;
+  void* out;  // [B, Hq, T, D], contiguous
+};
+size_t attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
+int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st);
+
 }  // namespace dropkv

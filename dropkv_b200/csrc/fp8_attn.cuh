@@ -1,0 +1,289 @@
+// What the two kernels of attention over a cache in 8 bits share (fp8_decode.cu: few query rows,
+// fp8_attn.cu: many): which keys a row tile reads, the line of tiles that is cut over the CTAs,
+// and the partials that fp8_attn.cu's merge kernel joins.
+//
+// The M = g T query rows of a KV head are ordered by token, then head of the group, and taken in
+// row tiles of `npr` whole tokens. A row tile reads tiles of TK keys: from the first that some
+// token's window reaches (0 without one) to the last token's own, and those of the sinks
+// before it. All (sequence, row tile, KV head) segments form one line of units, `lead` and then
+// one for each tile, that is cut evenly over the CTAs, from the lengths on the device: the host does
+// not know them, and no CTA waits for another. A segment that falls into several CTAs leaves a partial
+// in each: the output divided by its sum, its maximum and its sum.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace dropkv {
+namespace fa {
+
+struct Args {
+  AttnFp8 a;
+  int g, npr, RT;    // heads of a group, tokens of a row tile, row tiles of a sequence
+  int lead;          // units before a segment's tiles: about what a further segment costs a CTA, in tiles
+  int rows_pad;      // rows of a partial
+  int q_vec;         // Q's rows are read 16 bytes at a time
+  float scale_log2;
+  int* status;       // [CTAs]: 0, or which wait gave up
+  int4* meta;        // [CTAs]: the split segment that begins in a CTA: b, KV head, row tile, its partials (0: none)
+  float* part_o;     // [2 CTAs][rows_pad][D]
+  float* part_ml;    // [2 CTAs][2][rows_pad]
+};
+
+// Keys of a row tile of sequence b.
+template <int TK>
+struct Keys {
+  int len, keys;   // cached rows (past the table, too); cached rows and tokens that fit it
+  int n0, n1;      // its tokens
+  int lo;          // no token sees a key from the sinks to here
+  int ns, w0, n;   // tiles of sinks, the first tile after them, all tiles (one at least)
+  __device__ __forceinline__ void set(const Args& A, int b, int rt) {
+    const AttnFp8& a = A.a;
+    len = max(a.cache_lens[b], 0);
+    keys = (int)min((int64_t)len + a.T, (int64_t)a.cap);
+    n0 = rt * A.npr;
+    n1 = min(n0 + A.npr, a.T);
+    const int hi = a.mask ? keys : (int)min((int64_t)len + n1, (int64_t)a.cap);
+    lo = a.window ? (int)min(max((int64_t)len + (a.mask ? 0 : n0) - a.window + 1, (int64_t)0), (int64_t)a.cap) : 0;
+    w0 = lo / TK;
+    ns = a.window ? min((min(a.sinks, hi) + TK - 1) / TK, w0) : 0;
+    const int w1 = (hi + TK - 1) / TK;
+    n = ns + max(w1 - w0, 0);
+    if (n == 0) n = 1, w0 = 0;  // no key is seen: one tile says so
+  }
+  // first key of tile t
+  __device__ __forceinline__ int first(int t) const { return (t < ns ? t : w0 + (t - ns)) * TK; }
+  // some token sees some of keys [j, j + count)
+  __device__ __forceinline__ bool any(const Args& A, int j, int count) const {
+    return j < keys && (j + count > lo || j < A.a.sinks);
+  }
+  // every token sees all of keys [j, j + count), their pages given
+  __device__ __forceinline__ bool all(const Args& A, int j, int count) const {
+    const AttnFp8& a = A.a;
+    const int last = j + count;  // (at most cap + a tile)
+    if (last > keys || last > (a.mask ? (int64_t)len : (int64_t)len + n0 + 1)) return false;
+    return !a.window || last <= a.sinks || j >= (int64_t)len + (a.mask ? a.T : n1) - a.window;
+  }
+};
+
+// What one token sees of a sequence's keys, its page aside.
+struct Sees {
+  int lo, hi;  // keys [lo, hi) and those below sinks
+  int node;
+  // a token that sees nothing
+  __device__ __forceinline__ void none() { lo = hi = node = 0; }
+  __device__ __forceinline__ void set(const Args& A, int b, int len, int keys, int node_) {
+    const AttnFp8& a = A.a;
+    node = node_;
+    int64_t depth = node;
+    if (a.mask && a.window) {
+      const uint8_t* row = a.mask + b * a.mask_sb + node * a.mask_sr;
+      depth = -1;
+      for (int n = 0; n < a.T; ++n) depth += row[n * a.mask_sc] != 0;
+      depth = max(depth, (int64_t)0);
+    }
+    lo = a.window ? (int)min(max((int64_t)len + depth - a.window + 1, (int64_t)0), (int64_t)a.cap) : 0;
+    hi = a.mask ? keys : (int)min((int64_t)len + node + 1, (int64_t)keys);
+  }
+  // bit e: key j0 + e is seen (count at most 64)
+  __device__ __forceinline__ uint64_t bits(const Args& A, int b, int len, int j0, int count) const {
+    const AttnFp8& a = A.a;
+    auto below = [&](int n) -> uint64_t { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1); };
+    uint64_t m = below(hi - j0) & below(count);
+    const uint64_t near = ~below(lo - j0) | below(a.sinks - j0);
+    if (!a.mask || !m) return m & near;
+    const uint64_t cached = below(len - j0);
+    const uint8_t* row = a.mask + b * a.mask_sb + node * a.mask_sr;
+    uint64_t nodes = 0, todo = m & ~cached;
+    while (todo) {
+      const int e = __ffsll((long long)todo) - 1;
+      todo &= todo - 1;
+      if (row[(int64_t)(j0 + e - len) * a.mask_sc]) nodes |= 1ull << e;
+    }
+    return (m & cached & near) | nodes;
+  }
+};
+
+// A CTA's part of one segment: tiles [t0, t1) of `tiles`.
+template <int TK>
+struct Piece {
+  int b, h, rt, t0, t1, tiles, rows;
+  Keys<TK> k;
+};
+
+// Where a CTA's share of the line begins: found by one warp, read by all.
+struct Start {
+  long long w, w1, per;  // units: the share's, and a share's size
+  int pair, h, u;        // the (sequence, row tile) pair, the head and the unit in it
+};
+
+template <int TK>
+__device__ __forceinline__ void find_start(const Args& A, int lane, Start* out) {
+  const int pairs = A.a.B * A.RT;
+  Keys<TK> k;
+  auto units = [&](int p) -> long long {
+    if (p >= pairs) return 0;
+    k.set(A, p / A.RT, p % A.RT);
+    return (long long)(k.n + A.lead) * A.a.Hkv;
+  };
+  const long long own0 = units(lane);
+  long long total = own0;
+  for (int p = lane + 32; p < pairs; p += 32) total += units(p);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const long long per = (total + gridDim.x - 1) / gridDim.x;
+  const long long w0 = min(total, per * blockIdx.x), w1 = min(total, w0 + per);
+  long long before = 0;
+  if (w0 < w1) {
+    for (int c = 0; c < pairs; c += 32) {
+      const long long own = c == 0 ? own0 : units(c + lane);
+      long long upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, before + upto > w0);
+      if (past) {
+        if (lane == __ffs(past) - 1) {
+          const int each = (int)(own / A.a.Hkv), rel = (int)(w0 - (before + upto - own));
+          out->pair = c + lane;
+          out->h = rel / each;
+          out->u = rel % each;
+        }
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  if (lane == 0) {
+    out->w = w0;
+    out->w1 = w1;
+    out->per = per;
+  }
+}
+
+// Steps through a CTA's pieces; every role has one of its own and sees the same.
+template <int TK>
+struct Walk {
+  long long left, per;
+  int pair, h, u;
+  int4 meta;  // of a split segment that begins here
+  __device__ __forceinline__ explicit Walk(const Start& s)
+      : left(s.w1 - s.w), per(s.per), pair(s.pair), h(s.h), u(s.u), meta(make_int4(0, 0, 0, 0)) {}
+  __device__ __forceinline__ bool next(const Args& A, Piece<TK>& p) {
+    while (left > 0) {
+      p.b = pair / A.RT;
+      p.rt = pair % A.RT;
+      p.h = h;
+      p.k.set(A, p.b, p.rt);
+      p.tiles = p.k.n;
+      p.rows = (p.k.n1 - p.k.n0) * A.g;
+      const int units = p.tiles + A.lead, u1 = (int)min((long long)units, u + left);
+      p.t0 = max(u - A.lead, 0);
+      p.t1 = u1 - A.lead;
+      left -= u1 - u;
+      if (u1 == units) {
+        u = 0;
+        if (++h == A.a.Hkv) {
+          h = 0;
+          ++pair;
+        }
+      } else {
+        u = u1;
+      }
+      if (p.t1 > p.t0) {
+        if (p.t0 == 0 && p.t1 < p.tiles)
+          meta = make_int4(p.b, p.h, p.rt, 1 + (int)((units - u1 + per - 1) / per));
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+// The partial that a CTA writes of a piece: its segment's first part, or a later one.
+template <int TK>
+__device__ __forceinline__ int64_t slot_of(const Piece<TK>& p) {
+  return 2 * (int64_t)blockIdx.x + (p.t0 > 0 ? 0 : 1);
+}
+
+// Row r of a row tile in the output [B, Hq, T, D].
+__device__ __forceinline__ int64_t out_row(const Args& A, int b, int h, int n0, int r) {
+  const int node = n0 + r / A.g, head = h * A.g + r % A.g;
+  return ((int64_t)b * A.a.Hq + head) * A.a.T + node;
+}
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, hardware approximation; 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+struct Out;
+template <>
+struct Out<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+template <>
+struct Out<__half> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+};
+__device__ __forceinline__ uint32_t pack_half(float x, float y) { return Out<__half>::pack(x, y); }
+
+// Two stored values as two of fp16, exactly.
+__device__ __forceinline__ uint32_t widen2(uint32_t two) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3);
+  return (uint32_t)r.x | (uint32_t)r.y << 16;
+}
+
+struct Plan {
+  int ctas, rows_pad;
+  size_t off_meta, off_o, off_ml, bytes;
+};
+inline Plan make_plan(int ctas, int rows_pad, int D) {
+  Plan p;
+  p.ctas = ctas;
+  p.rows_pad = rows_pad;
+  p.off_meta = align_up((size_t)ctas * 4, 256);
+  p.off_o = align_up(p.off_meta + (size_t)ctas * sizeof(int4), 256);
+  p.off_ml = p.off_o + (size_t)2 * ctas * rows_pad * D * 4;
+  p.bytes = align_up(p.off_ml + (size_t)2 * ctas * 2 * rows_pad * 4, 256);
+  return p;
+}
+inline Args make_args(const AttnFp8& a, const Plan& p, int npr, int lead, void* ws) {
+  Args A;
+  A.a = a;
+  A.g = a.Hq / a.Hkv;
+  A.npr = npr;
+  A.RT = (a.T + npr - 1) / npr;
+  A.lead = lead;
+  A.rows_pad = p.rows_pad;
+  A.q_vec = a.q_sd == 1 && (reinterpret_cast<uintptr_t>(a.q) | (uint64_t)((a.q_sb | a.q_sh | a.q_ss) * 2)) % 16 == 0;
+  A.scale_log2 = a.scale * 1.4426950408889634f;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  A.status = reinterpret_cast<int*>(w);
+  A.meta = reinterpret_cast<int4*>(w + p.off_meta);
+  A.part_o = reinterpret_cast<float*>(w + p.off_o);
+  A.part_ml = reinterpret_cast<float*>(w + p.off_ml);
+  return A;
+}
+
+}  // namespace fa
+
+// Few query rows (g T <= 16): fp8_decode.cu.
+constexpr int kFp8DecodeRows = 16;
+fa::Plan fp8_decode_plan(int rows, int D);
+int launch_fp8_decode(const AttnFp8& a, int dtype, void* ws, cudaStream_t st);
+// Joins the partials of what was just launched with A on `ctas` CTAs.
+int launch_fp8_merge(const fa::Args& A, int dtype, int ctas, cudaStream_t st);
+
+}  // namespace dropkv

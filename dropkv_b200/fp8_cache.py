@@ -6,7 +6,9 @@ float32: a row's value is its 8 bits times its page's scale. Pages, slots and ta
 those of ``dropkv_b200.paged``; ``block_tables`` hands them out.
 
 * ``store_rows_fp8`` -- K/V rows to slots, quantised;
-* ``load_rows_fp8``  -- rows at slots, read back.
+* ``load_rows_fp8``  -- rows at slots, read back;
+* ``attention_fp8``  -- attention over such a cache: single tokens, drafted trees, prompt
+  chunks, with a sliding window and first rows that stay visible.
 
 Scales are powers of two, so that the 8 bits' rounding (2^-4 of a value) is the only one:
 what is read back is exact in 16 bits, and a page whose scale grows keeps its rows but for
@@ -16,13 +18,22 @@ reference's cache holds the model's own type only (dropkv_cache.py:581-617).
 
 from __future__ import annotations
 
+import functools
+from typing import Optional
+
 import torch
 
 from . import _lib
-from .ops import _DTYPE_CODE
+from .ops import _CHECK_STATUS, _DTYPE_CODE
 from .paged import _ints, _new, _on_its_device, _on_one_device, _raw_stream, _rows_strides
 
-__all__ = ["store_rows_fp8", "load_rows_fp8"]
+__all__ = ["store_rows_fp8", "load_rows_fp8", "attention_fp8"]
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(index: int, B: int, Hq: int, Hkv: int, T: int, D: int, cap: int) -> int:
+    """Bytes of an attention_fp8 workspace on the current device ``index``."""
+    return int(_lib.load().dropkv_attention_fp8_workspace_size(B, Hq, Hkv, T, D, cap))
 
 
 def _check_pool_fp8(K_pages, V_pages, K_scales, V_scales):
@@ -103,3 +114,70 @@ def load_rows_fp8(K_pages: torch.Tensor, V_pages: torch.Tensor, K_scales: torch.
     if rc:
         _lib.check(rc, "dropkv_load_rows_fp8")
     return k_out, v_out
+
+
+@_on_its_device
+def attention_fp8(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor, K_scales: torch.Tensor,
+                  V_scales: torch.Tensor, cache_lens: torch.Tensor, block_table: torch.Tensor,
+                  tree_mask: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                  scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of T tokens over a cache in 8 bits: Q [B, Hq, T, D] (any strides) -> [B, Hq, T, D].
+
+    Row b's cache holds ``cache_lens[b]`` (int32, on the device) rows in the pages of
+    ``block_table`` ([B, max_blocks] int32), and after them the T tokens' own K/V rows. Token i
+    sees every row up to its own, ``cache_lens[b] + i``: T = 1 is a decode step, a longer chain
+    drafted tokens or a prompt's chunk. With ``tree_mask`` (bool [T, T] or [B, T, T], T at most
+    256) it sees the cached rows and the nodes j with ``tree_mask[i, j]``.
+
+    ``window``: of those only the last ``window`` rows up to its own (for a tree's node: up to
+    the row of its depth, the number of nodes it sees but itself, and of the cached rows only; the window
+    holds the whole tree) and the cache's first ``sinks`` rows. Rows are counted as they
+    are stored: after an eviction the window holds the last rows kept.
+
+    Rows past the table and on missing pages (-1) are not seen; a token that sees nothing gives
+    zeros; what is in rows, pages or scales that no token sees does not matter. bf16 or fp16, D 64
+    or 128, at most 128 query heads a KV head, block_size a power of two from 8 to 1024, page rows
+    on 16-byte boundaries that do not overlap. The 8 bits enter the products as they are (queries
+    as exact sums of 8-bit parts), weights have 16 bits, sums and softmax statistics 32.
+    """
+    dev = _on_one_device(Q, K_pages, V_pages, K_scales, V_scales, cache_lens, block_table,
+                         *((tree_mask,) if tree_mask is not None else ()))
+    qs, dtype = Q.shape, Q.dtype
+    if len(qs) != 4:
+        raise ValueError(f"expected Q [B, Hq, T, D], got {tuple(qs)}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"attention_fp8 takes bf16 or fp16 queries, got {dtype}")
+    B, Hq, T, D = qs
+    ps, pool = _check_pool_fp8(K_pages, V_pages, K_scales, V_scales)
+    n_pages, Hkv, block, Dk = ps
+    if Dk != D or not Hkv or Hq % Hkv:
+        raise ValueError(f"shape mismatch: Q {tuple(qs)}, pages {tuple(ps)}")
+    cache_lens = _ints(cache_lens, torch.int32, (B,), "cache_lens")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
+    max_blocks = block_table.shape[1]
+    block_table = _ints(block_table, torch.int32, (B, max_blocks), "block_table")
+    mask = (None, 0, 0, 0)
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.bool:
+            raise TypeError(f"tree_mask must be bool, got {tree_mask.dtype}")
+        ms, st = tree_mask.shape, tree_mask.stride()
+        if ms not in ((T, T), (B, T, T)):
+            raise ValueError(f"tree_mask must be [{T}, {T}] or [{B}, {T}, {T}], got {tuple(ms)}")
+        mask = (tree_mask.data_ptr(), *(st if len(st) == 3 else (0, *st)))
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1 (None: every row is seen), got {window}")
+    scale = float(D ** -0.5 if scale is None else scale)
+    out = _new(dtype, Q.device, B, Hq, T, D)
+    if B == 0 or T == 0 or Hq == 0:
+        return out
+    # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
+    need = max(_attention_workspace(dev, B, Hq, Hkv, T, D, max_blocks * block), 1)
+    ws = _new(torch.uint8, Q.device, need)
+    rc = _lib.load().dropkv_attention_fp8(
+        Q.data_ptr(), *Q.stride(), *pool, n_pages, block, block_table.data_ptr(), max_blocks, cache_lens.data_ptr(), *mask,
+        min(int(window or 0), 0x7fffffff), min(int(sinks), 0x7fffffff), _DTYPE_CODE[dtype], B, Hq, Hkv, T, D, scale,
+        out.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_attention_fp8")
+    return out

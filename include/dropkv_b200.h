@@ -417,6 +417,29 @@ DROPKV_API int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t 
                                     int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size, const int64_t* slots,
                                     int dtype, int B, int Hkv, int N, int D, void* k_out, void* v_out, void* stream);
 
+/* Attention of T tokens (or the nodes of a drafted tree), whose K/V rows follow the
+ * cache_lens[b] rows of sequence b, over a cache in 8 bits: out[b, h, i, :] =
+ * softmax(scale q[b, h, i, :] . K) V over the rows that token i sees: those up to its own,
+ * cache_lens[b] + i, or, with mask (bytes, mask[b * mask_sb + i * mask_sr + j * mask_sc] != 0),
+ * every cached row and the nodes j shown. With a window (0: none) of those only the last
+ * `window` up to its own row, or its depth's (the nodes it sees less itself), and the
+ * first `sinks`; nodes of a tree are all seen (window >= T). table [B, max_blocks]: rows past
+ * max_blocks * block_size and on pages outside the pool are not seen; a token that sees nothing gives
+ * zeros, and a row that no token sees is not used, whatever it holds. bf16 or fp16, D 64 or 128,
+ * Hq / Hkv <= 128, T <= 256 with a mask, block_size a power of two from 8 to 1024, page rows on
+ * 16-byte boundaries and not overlapping, B * Hkv <= 65535, scale positive and finite, scales
+ * positive and finite; out [B, Hq, T, D] contiguous. */
+DROPKV_API size_t dropkv_attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
+DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd,
+                                    const void* k_pages, int64_t kp_sb, int64_t kp_sh, int64_t kp_st,
+                                    const void* v_pages, int64_t vp_sb, int64_t vp_sh, int64_t vp_st,
+                                    const float* k_scales, int64_t ks_sb, int64_t ks_sh, const float* v_scales,
+                                    int64_t vs_sb, int64_t vs_sh, int n_pages, int block_size, const int32_t* table,
+                                    int max_blocks, const int32_t* cache_lens, const uint8_t* mask, int64_t mask_sb,
+                                    int64_t mask_sr, int64_t mask_sc, int window, int sinks, int dtype, int B, int Hq,
+                                    int Hkv, int T, int D, float scale, void* out, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 /* Diagnostic: one 128-row tile through a tcgen05 MMA form used by the fused
  * scorer (mode 0: out[128][n] = A[128][128] B[n][128]^T with A loaded by TMA;
  * mode 1: out[128][n] = A[128][128]^T B[n][128]^T with A read MN-major; modes 2/3:
