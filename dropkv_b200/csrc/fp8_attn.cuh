@@ -58,12 +58,12 @@ struct Keys {
   __device__ __forceinline__ bool any(const Args& A, int j, int count) const {
     return j < keys && (j + count > lo || j < A.a.sinks);
   }
-  // every token sees all of keys [j, j + count), their pages given
-  __device__ __forceinline__ bool all(const Args& A, int j, int count) const {
+  // Every token sees all of keys [j, j + count), their pages given, where j + count <= end and either j >= low
+  // or j + count <= sinks.
+  __device__ __forceinline__ void all(const Args& A, int* end, int* low) const {
     const AttnFp8& a = A.a;
-    const int last = j + count;  // (at most cap + a tile)
-    if (last > keys || last > (a.mask ? (int64_t)len : (int64_t)len + n0 + 1)) return false;
-    return !a.window || last <= a.sinks || j >= (int64_t)len + (a.mask ? a.T : n1) - a.window;
+    *end = a.mask ? min(len, keys) : (int)min((int64_t)len + n0 + 1, (int64_t)keys);
+    *low = a.window ? (int)min(max((int64_t)len + (a.mask ? a.T : n1) - a.window, (int64_t)0), (int64_t)a.cap) : 0;
   }
 };
 
@@ -239,10 +239,33 @@ struct Out<__half> {
 };
 __device__ __forceinline__ uint32_t pack_half(float x, float y) { return Out<__half>::pack(x, y); }
 
-// Two stored values as two of fp16, exactly.
-__device__ __forceinline__ uint32_t widen2(uint32_t two) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3);
-  return (uint32_t)r.x | (uint32_t)r.y << 16;
+// Four stored values as two words of two fp16 values, exactly.
+__device__ __forceinline__ void widen4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
+
+// The unit of a row of queries: the power of two (2^-126 at least) that brings its largest element to
+// at most 448.
+__device__ __forceinline__ float query_unit(float largest) {
+  const uint32_t bits = __float_as_uint(largest);
+  const int e = (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return __uint_as_float((uint32_t)(max(e, -126) + 127) << 23);
+}
+
+// Four values in 8 bits; what that leaves of them, times `up`, stays in v.
+__device__ __forceinline__ uint32_t split4(float* v, float up) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[e], v[e + 1]), __NV_SATFINITE, __NV_E4M3);
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3)));
+    v[e] = (v[e] - f.x) * up;
+    v[e + 1] = (v[e + 1] - f.y) * up;
+    w |= two << (8 * e);
+  }
+  return w;
 }
 
 struct Plan {

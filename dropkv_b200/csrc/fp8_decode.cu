@@ -1,47 +1,65 @@
 // Attention over a cache in 8 bits for few query rows (g T <= 16): single tokens, short drafts.
 //
 // A key costs 2 D bytes and 4 D M operations, so HBM bounds this by far, and what counts is to
-// keep loads on their way and instructions few. Each warp takes 16 keys of a tile at a time, K and V
-// straight into registers, the next step's K under way when S is there, its V when P V is; nothing
-// is shared between warps until a piece ends. Both products are m16n8k16 MMAs of fp16 (the
-// tcgen05 kernel's M = 128 would hold 1 to 16 rows here, and its softmax as many threads):
-//   S = Q K^T      A = up to 16 query rows, B = 8 keys;
-//   O^T += V^T P^T A = 16 columns of V for 16 keys, B = the weights of 8 rows as they lie in S's
-//                  accumulators.
-// e4m3 widens to fp16 exactly and two at a time. The order of D within a product is free:
-// lane (gid, tig) = (lane / 4, lane % 4) reads bytes [64 i + 16 tig, + 16) of key gid's row of K, and for V
-// bytes [D / 8 gid, + D / 8) of keys 2 tig, 2 tig + 1, 2 tig + 8 and 2 tig + 9, whose bytes are
-// paired before they are widened. Queries in bf16 are brought to fp16 by a power of two for each
-// row (its largest element to 2^14 or so; elements under 2^-28 of it lose bits).
-// A page's scale of K multiplies its logits in fp32; that of V, over the largest of the warp so far,
-// the weights. Weights are rounded to fp16 for their product (2^-11), sums taken from
-// them before that.
+// keep loads on their way and instructions few. One warp issues TMA loads (a box a page) of K and V
+// tiles of 128 keys into a ring of slots; four warps take 32 keys of each tile. Both products are warp
+// MMAs fed from registers (tcgen05.mma takes 128 rows, of which 1 to 16 would exist, and as many
+// threads would do the softmax):
+//   S = Q K^T      m16n8k32 of e4m3: K's bytes as they lie, and queries as sums of 8-bit parts, each
+//                  what the one before left, times 16: two parts hold a bf16 (the second takes the
+//                  MMA's rows 8 to 15 where there are at most 8 queries), three an fp16;
+//   O^T += V^T P^T m16n8k16 of fp16: A = 16 columns of V for 16 keys, widened (exactly, two at a time),
+//                  B = the weights of 8 rows as they lie in S's accumulators.
+// The order of D and of the keys within a product is free, and chosen so that a quarter warp's 16-byte
+// reads of the swizzled tiles meet all banks once (D = 128): lane (gid, tig) = (lane / 4, lane % 4) reads
+// chunks 4 i + tig of key fd_key(gid)'s row of K, and for V chunk fd_chunk(gid) of keys
+// fd_key(2 tig + {0, 1}) and of those 8 on, whose bytes are paired before they are widened.
+// A row's queries are brought to 8 bits' range by a power of two (its largest element to 224 or more;
+// what the parts leave is at most 2^-14 of that unit). A page's scale of K multiplies its logits in fp32;
+// that of V, over the largest of the warp so far, the weights. Weights are rounded to fp16 for their
+// product (2^-11), sums taken from them before that.
 #include <algorithm>
 #include <type_traits>
 
 #include "fp8_attn.cuh"
+#include "tc_common.cuh"
 
 namespace dropkv {
 namespace {
 
 using namespace fa;
 
-// 8 rows: two CTAs of 8 warps an SM; 16 rows need 64 registers for the output: one of 12 warps
-template <bool R16>
+constexpr int FD_WARPS = 4, FD_NT = 32 * FD_WARPS + 32;  // warps that compute; and one that loads
+constexpr int FD_TK = 32 * FD_WARPS;                      // keys of a tile
+constexpr int FD_HALVES = FD_TK / 8;                      // a page has 8 rows at least
+constexpr int FD_CTAS = 2;                                // of an SM
+constexpr uint64_t kFdWaitNs = 1000000000ull;
+
+template <int D, bool R16>
 struct FdShape {
-  static constexpr int WARPS = R16 ? 12 : 8, NT = 32 * WARPS, CTAS = R16 ? 1 : 2;
-  static constexpr int TK = 16 * WARPS, ROWS = R16 ? 16 : 8;
+  static constexpr int ROWS = R16 ? 16 : 8;
+  static constexpr int TILE = FD_TK * D, SLOTS = (R16 ? 5 : 6) * (128 / D);
+  static constexpr int WO = SLOTS * TILE;                        // float [WARPS][ROWS][D]: the warps' outputs
+  static constexpr int WM = WO + FD_WARPS * ROWS * D * 4;        // float [2][WARPS][ROWS]: maxima, sums
+  // tiles whose scales are held: before tile i's first load is issued, the slot is free that load 2 i - SLOTS had,
+  // so all warps are past the tiles before that
+  static constexpr int SCALES = SLOTS / 2 + 1;
+  static constexpr int SC = WM + 2 * FD_WARPS * ROWS * 4;        // float [SCALES][2][FD_HALVES]: 0 for a missing page
+  static constexpr int BARS = SC + SCALES * 2 * FD_HALVES * 4;   // full[SLOTS], empty[SLOTS]
+  static constexpr int START = BARS + 2 * SLOTS * 8;
+  static constexpr int BYTES = START + (int)sizeof(Start) + 8;
+  static_assert(FD_CTAS * (BYTES + 1024) <= 233472, "shared memory");
 };
+
+template <int D>
+__device__ __forceinline__ int fd_key(int n) { return D == 128 ? ((n & 1) << 2) | (n >> 1) : n; }
+template <int D>
+__device__ __forceinline__ int fd_chunk(int gid) { return D == 128 ? ((gid & 1) << 2) | (gid >> 1) : gid; }
+
 constexpr int kFdLead = 3;
 // A row's reference moves once its maximum has grown by this much (base 2); weights are
 // 2^(s - m + bias), so that fp16 holds them from 2^-24 to 2^15.
 constexpr float kFdSlack = 8.f, kFdBias = 7.f;
-
-template <int D, bool R16>
-constexpr int fd_smem() {
-  using S = FdShape<R16>;
-  return S::WARPS * S::ROWS * (D + 2) * 4 + (int)sizeof(Start);
-}
 
 __device__ __forceinline__ void fd_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -50,30 +68,144 @@ __device__ __forceinline__ void fd_mma(float* c, const uint32_t* a, uint32_t b0,
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void fd_mma8(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void fd_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+static_assert(FD_WARPS == 4, "threads of fd_sync");
+
 template <typename T, int D, bool R16>
-__global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
-    fp8_decode_kernel(const __grid_constant__ Args A) {
-  using S = FdShape<R16>;
-  constexpr int NT = S::NT, WARPS = S::WARPS, TK = S::TK, ROWS = S::ROWS, HR = R16 ? 2 : 1;
+__global__ void __launch_bounds__(FD_NT, FD_CTAS)
+    fp8_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ Args A) {
+  using S = FdShape<D, R16>;
+  constexpr int TK = FD_TK, WARPS = FD_WARPS, ROWS = S::ROWS, HR = R16 ? 2 : 1, NS = S::SLOTS;
+  constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;  // 8-bit parts of a query's elements
   constexpr int KV = D / 64;   // 16-byte vectors of K a lane has of a key
   constexpr int VW = D / 32;   // words of V a lane has of a key
   constexpr int VB = 4 * VW;
-  extern __shared__ __align__(16) uint8_t sm[];
-  float* wo = reinterpret_cast<float*>(sm);         // [WARPS][ROWS][D]
-  float* wm = wo + WARPS * ROWS * D;                // [WARPS][ROWS]
+  extern __shared__ __align__(1024) uint8_t sm[];  // swizzled tiles start on multiples of 1024
+  float* wo = reinterpret_cast<float*>(sm + S::WO);
+  float* wm = reinterpret_cast<float*>(sm + S::WM);
   float* wl = wm + WARPS * ROWS;
-  Start* start = reinterpret_cast<Start*>(wl + WARPS * ROWS);
+  float* sc = reinterpret_cast<float*>(sm + S::SC);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + S::BARS);
+  uint64_t* empty = full + NS;
+  Start* start = reinterpret_cast<Start*>(sm + S::START);
+  volatile int* dead = reinterpret_cast<volatile int*>(start + 1);
   const AttnFp8& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+  if (tc::smem_addr(sm) % 1024) {  // as declared; nothing may run on any other layout
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tid == 0) {
+      A.status[blockIdx.x] = 9;
+      A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    }
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], WARPS);
+    }
+    tc::fence_mbar_init();
+    *dead = 0;
+  }
+  if (warp == WARPS && lane == 0) {
+    tc::tma_prefetch_desc(&kmap);
+    tc::tma_prefetch_desc(&vmap);
+  }
   pdl_wait();
   pdl_launch_dependents();  // (after the wait: the merge may then read this kernel's inputs at once)
   if (warp == 0) find_start<TK>(A, lane, start);
   __syncthreads();
   Walk<TK> walk(*start);
   Piece<TK> p;
+  // a wait that gives up marks the CTA dead: every role then ends without waiting
+  auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
+    if (tc::mbar_try_wait(bar, count & 1)) return true;
+    const uint64_t t0 = tc::globaltimer_ns();
+    while (!*dead) {
+      if (tc::mbar_try_wait(bar, count & 1)) return true;
+      if (tc::globaltimer_ns() - t0 > kFdWaitNs) *dead = why;
+    }
+    return false;
+  };
+  // Tile i of the CTA (from 0, over all pieces) is loads 2 i (K) and 2 i + 1 (V); load n uses slot n % NS. Every
+  // role waits for every load (or slot) of its own in turn, so a barrier is never two phases ahead of a wait.
+  if (warp == WARPS) {
+    // ======================= TMA producer =======================================
+    const int block = a.pool.block, lb = __ffs(block) - 1, box = min(block, TK), boxes = TK / box;
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && walk.next(A, p)) {
+      const int32_t* table = a.table + (int64_t)p.b * a.max_blocks;
+      const float* ksb = a.pool.k_scale + p.h * a.pool.ks_sh;
+      const float* vsb = a.pool.v_scale + p.h * a.pool.vs_sh;
+      // a lane has eight keys of a tile: their page, -1 where no token sees any of them
+      auto page_of = [&](int t) {
+        if (t >= p.t1 || lane >= FD_HALVES) return -1;
+        const int j = p.k.first(t) + 8 * lane;
+        return p.k.any(A, j, 8) ? table[j >> lb] : -1;
+      };
+      auto there = [&](int page) { return page >= 0 && page < a.pool.n_pages; };
+      int page = page_of(p.t0), page1 = page_of(p.t0 + 1);
+      float ks = there(page) ? ksb[page * a.pool.ks_s0] : 0.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
+      for (int t = p.t0; t < p.t1; ++t) {
+        const int page2 = page_of(t + 2);
+        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : 0.f;
+        const float vs1 = there(page1) ? vsb[page1 * a.pool.vs_s0] : 0.f;
+        // the page of a lane's box: that of any of its eights that is read, else out of range (zeros)
+        int at = there(page) ? page : -1;
+        for (int o = 1; o < box / 8; o <<= 1) at = max(at, __shfl_xor_sync(0xffffffffu, at, o));
+        at = __shfl_sync(0xffffffffu, at, min(lane, boxes - 1) * (box / 8));
+        if (at < 0) at = a.pool.n_pages;
+        const int row = p.k.first(t) & (block - 1);  // (of a page larger than a tile; else 0)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const uint32_t slot = n % NS;
+          if (n >= (uint32_t)NS) ok = __all_sync(0xffffffffu, wait(&empty[slot], n / NS - 1, 1));
+          if (!ok) break;
+          if (kv == 0 && lane < FD_HALVES) {
+            float* s = sc + (n / 2 % S::SCALES) * (2 * FD_HALVES) + lane;
+            s[0] = ks;
+            s[FD_HALVES] = vs;
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], S::TILE);
+          __syncwarp();
+          if (lane < boxes)
+            tc::tma_load_4d(sm + slot * S::TILE + lane * box * D, kv ? &vmap : &kmap, &full[slot], 0, row, p.h, at);
+          __syncwarp();
+        }
+        if (!ok) break;
+        page = page1, page1 = page2, ks = ks1, vs = vs1;
+      }
+    }
+    if (*dead && n) {  // every issued copy lands before the CTA may exit
+      for (uint32_t j = n > (uint32_t)NS ? n - NS : 0u; j < n; ++j) tc::mbar_wait(&full[j % NS], (j / NS) & 1, kFdWaitNs / 8);
+    }
+  } else {
+  // ======================= the warps that compute =============================
+  uint32_t slot = 0, turn = 0, held = 0;  // of the next load: its slot, how often that was filled; of the next tile: its scales
+  bool ok = true;
+  // what a lane reads of a tile: K's vectors of its two keys, V's of its four
+  uint32_t k_at[KV], v_at[2];
+#pragma unroll
+  for (int i = 0; i < KV; ++i) k_at[i] = tc::swz_offset<D>(32 * warp + fd_key<D>(gid), (4 * i + tig) * 8);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int r = 32 * warp + fd_key<D>(2 * tig + c);
+    v_at[c] = VW == 4 ? tc::swz_offset<D>(r, fd_chunk<D>(gid) * 8) : tc::swz_offset<D>(r, (gid >> 1) * 8) + (gid & 1) * 8;
+  }
   while (walk.next(A, p)) {
     // ---- queries: rows gid and, of 16, gid + 8 ---------------------------------
-    uint32_t q[KV * 4][2][HR];  // [k step][k half][row half]
+    uint32_t q[PARTS][KV * 4][HR];  // four elements a word, as a lane has them of K
     float qscale[HR];
     Sees sees[HR];
 #pragma unroll
@@ -103,77 +235,20 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
         for (int e = 0; e < KV * 16; ++e) v[e] = 0.f;
         sees[x].none();
       }
-      qscale[x] = 1.f;
-      if (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-        for (int e = 0; e < KV * 16; ++e) big = fmaxf(big, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const int e = min(max((int)(__float_as_uint(big) >> 23) - 14, 1), 253);  // 2^(e - 127): the largest over 2^14
-        qscale[x] = __uint_as_float((uint32_t)e << 23);
-        const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+      for (int e = 0; e < KV * 16; ++e) big = fmaxf(big, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const float unit = query_unit(big), inv = 1.f / unit;
+      qscale[x] = unit * A.scale_log2;
 #pragma unroll
-        for (int i = 0; i < KV * 16; ++i) v[i] *= inv;
-      }
-      qscale[x] *= A.scale_log2;
+      for (int e = 0; e < KV * 16; ++e) v[e] = isfinite(v[e]) ? v[e] * inv : __uint_as_float(0x7fffffffu);
 #pragma unroll
-      for (int s = 0; s < KV * 4; ++s) {
-        q[s][0][x] = pack_half(v[4 * s], v[4 * s + 1]);
-        q[s][1][x] = pack_half(v[4 * s + 2], v[4 * s + 3]);
-      }
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int s = 0; s < KV * 4; ++s) q[part][s][x] = split4(v + 4 * s, 16.f);
     }
     // ---- the warp's steps --------------------------------------------------------
-    const uint8_t* kb = static_cast<const uint8_t*>(a.pool.k) + p.h * a.pool.k_sh + 16 * tig;
-    const uint8_t* vb = static_cast<const uint8_t*>(a.pool.v) + p.h * a.pool.v_sh + VB * gid;
-    const float* ksb = a.pool.k_scale + p.h * a.pool.ks_sh;
-    const float* vsb = a.pool.v_scale + p.h * a.pool.vs_sh;
-    const int32_t* table = a.table + (int64_t)p.b * a.max_blocks;
-    const int block = a.pool.block, lb = __ffs(block) - 1;
-    auto key_of = [&](int t) { return p.k.first(t) + 16 * warp; };
-    // pages of the halves of a step: -1 where no token sees any of it
-    auto pages_of = [&](int t, int* pg) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        pg[x] = -1;
-        if (t >= p.t1) continue;
-        const int j = key_of(t) + 8 * x;
-        if (p.k.any(A, j, 8)) pg[x] = table[j >> lb];
-        if (pg[x] >= a.pool.n_pages) pg[x] = -1;
-      }
-    };
-    uint4 k[2][KV];
-    uint32_t v[4][VW];
-    float ks[2], vs[2];
-    auto load_k = [&](int t, const int* pg) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int at = (key_of(t) + 8 * x + gid) & (block - 1);
-#pragma unroll
-        for (int i = 0; i < KV; ++i) {
-          k[x][i] = make_uint4(0u, 0u, 0u, 0u);
-          if (pg[x] >= 0)
-            k[x][i] = __ldcs(reinterpret_cast<const uint4*>(kb + pg[x] * a.pool.k_s0 + at * a.pool.k_st + 64 * i));
-        }
-      }
-    };
-    auto load_v = [&](int t, const int* pg) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int x = c >> 1, at = (key_of(t) + 8 * x + 2 * tig + (c & 1)) & (block - 1);
-        const uint8_t* src = vb + pg[x] * a.pool.v_s0 + at * a.pool.v_st;
-#pragma unroll
-        for (int w = 0; w < VW; ++w) v[c][w] = 0;
-        if (pg[x] >= 0) {
-          if (VW == 4) {
-            const uint4 y = __ldcs(reinterpret_cast<const uint4*>(src));
-            v[c][0] = y.x, v[c][1] = y.y, v[c][VW - 2] = y.z, v[c][VW - 1] = y.w;
-          } else {
-            const uint2 y = __ldcs(reinterpret_cast<const uint2*>(src));
-            v[c][0] = y.x, v[c][1] = y.y;
-          }
-        }
-      }
-    };
     float o[HR][VB / 2][4];
     float m[HR], l[HR];
 #pragma unroll
@@ -183,109 +258,97 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
       for (int t = 0; t < VB / 2; ++t) o[x][t][0] = o[x][t][1] = o[x][t][2] = o[x][t][3] = 0.f;
     }
     float vref = 0.f;  // the output is o * vref
-    int pg[2], pg1[2];
-    pages_of(p.t0, pg);
-    pages_of(p.t0 + 1, pg1);
-    load_k(p.t0, pg);
-    load_v(p.t0, pg);
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      ks[x] = pg[x] >= 0 ? ksb[pg[x] * a.pool.ks_s0] : 0.f;
-      vs[x] = pg[x] >= 0 ? vsb[pg[x] * a.pool.vs_s0] : 0.f;
-    }
+    float vinv = 0.f;  // 1 / vref
+    int all_end, all_low;
+    p.k.all(A, &all_end, &all_low);
     for (int t = p.t0; t < p.t1; ++t) {
-      int pg2[2];
-      pages_of(t + 2, pg2);
-      const int j0 = key_of(t);
-      const bool some = pg[0] >= 0 || pg[1] >= 0;
-      float s[2][4];
+      ok = ok && __all_sync(0xffffffffu, wait(&full[slot], turn, 2));
+      if (!ok) break;
+      const float4* scales = reinterpret_cast<const float4*>(sc + held * (2 * FD_HALVES)) + warp;
+      if (++held == S::SCALES) held = 0;
+      float ks[4], vs[4];
+      *reinterpret_cast<float4*>(ks) = scales[0];
+      *reinterpret_cast<float4*>(vs) = scales[FD_HALVES / 4];
+      const int j0 = p.k.first(t) + 32 * warp;
+      const bool some = fmaxf(fmaxf(ks[0], ks[1]), fmaxf(ks[2], ks[3])) > 0.f;
+      float s[4][2 * HR];  // of eight keys each: rows gid, then gid + 8
       if (some) {
+        const uint8_t* kt = sm + slot * S::TILE;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+        for (int x = 0; x < 4; ++x) {
+          float c[PARTS][4];
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) c[part][0] = c[part][1] = c[part][2] = c[part][3] = 0.f;
 #pragma unroll
           for (int i = 0; i < KV; ++i) {
-            const uint32_t w[4] = {k[x][i].x, k[x][i].y, k[x][i].z, k[x][i].w};
+            const uint4 k = *reinterpret_cast<const uint4*>(kt + k_at[i] + x * 8 * D);  // (the swizzle repeats after 8 rows)
+            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int st = 4 * i + e;
-              const uint32_t qa[4] = {q[st][0][0], R16 ? q[st][0][HR - 1] : 0u, q[st][1][0], R16 ? q[st][1][HR - 1] : 0u};
-              fd_mma(s[x], qa, widen2(w[e] & 0xffffu), widen2(w[e] >> 16));
+            for (int h = 0; h < 2; ++h) {
+              const int e = 4 * i + 2 * h;
+              if (R16) {
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) {
+                  const uint32_t qa[4] = {q[part][e][0], q[part][e][HR - 1], q[part][e + 1][0], q[part][e + 1][HR - 1]};
+                  fd_mma8(c[part], qa, w[2 * h], w[2 * h + 1]);
+                }
+              } else {  // rows 8 to 15 are the second part's
+                const uint32_t qa[4] = {q[0][e][0], q[1][e][0], q[0][e + 1][0], q[1][e + 1][0]};
+                fd_mma8(c[0], qa, w[2 * h], w[2 * h + 1]);
+                if (PARTS == 3) {
+                  const uint32_t qb[4] = {q[PARTS - 1][e][0], 0u, q[PARTS - 1][e + 1][0], 0u};
+                  fd_mma8(c[PARTS - 1], qb, w[2 * h], w[2 * h + 1]);
+                }
+              }
             }
+          }
+#pragma unroll
+          for (int e = 0; e < 2 * HR; ++e) {
+            float z = R16 ? c[1][e] : c[0][e + 2];
+            if (PARTS == 3) z = fmaf(c[PARTS - 1][e], 0.0625f, z);
+            s[x][e] = fmaf(z, 0.0625f, c[0][e]);
           }
         }
       }
-      const float ks0 = ks[0], ks1 = ks[1], vs0 = vs[0], vs1 = vs[1];
-      // the next step's K and scales
-      load_k(t + 1, pg1);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        ks[x] = pg1[x] >= 0 ? ksb[pg1[x] * a.pool.ks_s0] : 0.f;
-        vs[x] = pg1[x] >= 0 ? vsb[pg1[x] * a.pool.vs_s0] : 0.f;
-      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[slot]);
+      if (++slot == NS) slot = 0, ++turn;
+      uint32_t b[4][HR];         // weights of the 16 keys of two eights, for the second product
+      uint32_t seen = 0xffffffffu, mine[HR];
+      bool masked = false;
       if (some) {
-        const bool masked = pg[0] < 0 || pg[1] < 0 || !p.k.all(A, j0, 16);
+        const float least = fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3]));
+        masked = !(least > 0.f) || j0 + 32 > all_end || (j0 < all_low && j0 + 32 > a.sinks);
 #pragma unroll
-        for (int x = 0; x < HR; ++x) {
-          const float c0 = fminf(qscale[x] * ks0, 3e38f), c1 = fminf(qscale[x] * ks1, 3e38f);
-          s[0][2 * x] *= c0, s[0][2 * x + 1] *= c0;
-          s[1][2 * x] *= c1, s[1][2 * x + 1] *= c1;
-        }
+        for (int x = 0; x < HR; ++x)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float c = fminf(qscale[x] * ks[y], 3e38f);
+            s[y][2 * x] *= c, s[y][2 * x + 1] *= c;
+          }
         if (masked) {
-          uint32_t seen = 0, mine[HR];
+          seen = 0;
 #pragma unroll
           for (int x = 0; x < HR; ++x) {
-            uint32_t b = (uint32_t)sees[x].bits(A, p.b, p.k.len, j0, 16);
-            if (pg[0] < 0) b &= 0xff00u;
-            if (pg[1] < 0) b &= 0x00ffu;
-            mine[x] = b;
-            seen |= b;
+            uint32_t see = (uint32_t)sees[x].bits(A, p.b, p.k.len, j0, 32);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              if (!((b >> (8 * y + 2 * tig)) & 1)) s[y][2 * x] = -INFINITY;
-              if (!((b >> (8 * y + 2 * tig + 1)) & 1)) s[y][2 * x + 1] = -INFINITY;
+            for (int y = 0; y < 4; ++y) {
+              if (!(ks[y] > 0.f)) see &= ~(0xffu << (8 * y));
+              if (!((see >> (8 * y + fd_key<D>(2 * tig))) & 1)) s[y][2 * x] = -INFINITY;
+              if (!((see >> (8 * y + fd_key<D>(2 * tig + 1))) & 1)) s[y][2 * x + 1] = -INFINITY;
             }
+            mine[x] = see;
+            seen |= see;
           }
-          // V of keys that no row sees is cleared; NaN of those that some see is taken out, and given to these
           seen = __reduce_or_sync(0xffffffffu, seen);
-          uint32_t nan = 0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const bool see = (seen >> (8 * (c >> 1) + 2 * tig + (c & 1))) & 1;
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              if (!see) v[c][w] = 0;
-              nan |= __vcmpeq4(v[c][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            }
-          }
-          if (__any_sync(0xffffffffu, nan)) {
-#pragma unroll
-            for (int e = 0; e < VB; ++e) {
-              uint32_t at = 0;  // the keys whose element e of this lane's columns is NaN, over the lanes of the column
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                if (((v[c][e >> 2] >> (8 * (e & 3))) & 0x7f) == 0x7f) {
-                  at |= 1u << (8 * (c >> 1) + 2 * tig + (c & 1));
-                  v[c][e >> 2] &= ~(0xffu << (8 * (e & 3)));
-                }
-              at |= __shfl_xor_sync(0xffffffffu, at, 1);
-              at |= __shfl_xor_sync(0xffffffffu, at, 2);
-#pragma unroll
-              for (int x = 0; x < HR; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {  // rows 8 x + 2 tig + y
-                  const uint32_t b = __shfl_sync(0xffffffffu, mine[x], 4 * (2 * tig + y));
-                  if (b & at) o[x][e >> 1][2 * (e & 1) + y] = __uint_as_float(0x7fffffffu);
-                }
-            }
-          }
         }
         // the reference moves where some row's maximum has outgrown it
         float top[HR];
         bool over = false;
 #pragma unroll
         for (int x = 0; x < HR; ++x) {
-          top[x] = fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1]));
+          top[x] = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
+                         fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
           over = over || top[x] > m[x] + kFdSlack;
         }
         if (__any_sync(0xffffffffu, over)) {
@@ -302,7 +365,7 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
             for (int e = 0; e < VB / 2; ++e) o[x][e][0] *= f0, o[x][e][1] *= f1, o[x][e][2] *= f0, o[x][e][3] *= f1;
           }
         }
-        const float vmax = fmaxf(vs0, vs1);
+        const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         if (vmax > vref) {  // (the same in every lane)
           const float f = vref / vmax;
 #pragma unroll
@@ -310,34 +373,89 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
 #pragma unroll
             for (int e = 0; e < VB / 2; ++e) o[x][e][0] *= f, o[x][e][1] *= f, o[x][e][2] *= f, o[x][e][3] *= f;
           vref = vmax;
+          vinv = 1.f / vmax;
         }
-        const float inv = 1.f / vref, f0 = vs0 * inv, f1 = vs1 * inv;
-        uint32_t b0[HR], b1[HR];
 #pragma unroll
         for (int x = 0; x < HR; ++x) {
           const float ref = (m[x] == -INFINITY ? 0.f : m[x]) - kFdBias;
-          const float p0 = ex2(s[0][2 * x] - ref), p1 = ex2(s[0][2 * x + 1] - ref);
-          const float p2 = ex2(s[1][2 * x] - ref), p3 = ex2(s[1][2 * x + 1] - ref);
-          l[x] += (p0 + p1) + (p2 + p3);
-          b0[x] = pack_half(p0 * f0, p1 * f0);
-          b1[x] = pack_half(p2 * f1, p3 * f1);
-        }
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          const uint32_t lo0 = __byte_perm(v[0][w], v[1][w], 0x5140), lo1 = __byte_perm(v[2][w], v[3][w], 0x5140);
-          const uint32_t hi0 = __byte_perm(v[0][w], v[1][w], 0x7362), hi1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-          const uint32_t va[4] = {widen2(lo0 & 0xffffu), widen2(lo0 >> 16), widen2(lo1 & 0xffffu), widen2(lo1 >> 16)};
-          const uint32_t vc[4] = {widen2(hi0 & 0xffffu), widen2(hi0 >> 16), widen2(hi1 & 0xffffu), widen2(hi1 >> 16)};
-#pragma unroll
-          for (int x = 0; x < HR; ++x) {
-            fd_mma(o[x][2 * w], va, b0[x], b1[x]);
-            fd_mma(o[x][2 * w + 1], vc, b0[x], b1[x]);
+          for (int y = 0; y < 4; ++y) {
+            const float p0 = ex2(s[y][2 * x] - ref), p1 = ex2(s[y][2 * x + 1] - ref), f = vs[y] * vinv;
+            l[x] += p0 + p1;
+            b[y][x] = pack_half(p0 * f, p1 * f);
           }
         }
       }
-      load_v(t + 1, pg1);
-      pg[0] = pg1[0], pg[1] = pg1[1];
-      pg1[0] = pg2[0], pg1[1] = pg2[1];
+      ok = __all_sync(0xffffffffu, wait(&full[slot], turn, 3));
+      if (!ok) break;
+      if (some) {
+        const uint8_t* vt = sm + slot * S::TILE;
+#pragma unroll
+        for (int y = 0; y < 4; y += 2) {  // 16 keys
+          uint32_t v[4][VW];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint8_t* src = vt + v_at[c & 1] + (y + (c >> 1)) * 8 * D;
+            if (VW == 4) {
+              const uint4 z = *reinterpret_cast<const uint4*>(src);
+              v[c][0] = z.x, v[c][1] = z.y, v[c][VW - 2] = z.z, v[c][VW - 1] = z.w;
+            } else {
+              const uint2 z = *reinterpret_cast<const uint2*>(src);
+              v[c][0] = z.x, v[c][1] = z.y;
+            }
+          }
+          if (masked) {
+            // V of keys that no row sees is cleared; NaN of those that some see is taken out, and given to these
+            uint32_t nan = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const bool see = (seen >> (8 * (y + (c >> 1)) + fd_key<D>(2 * tig + (c & 1)))) & 1;
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                if (!see) v[c][w] = 0;
+                nan |= __vcmpeq4(v[c][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              }
+            }
+            if (__any_sync(0xffffffffu, nan)) {
+#pragma unroll
+              for (int e = 0; e < VB; ++e) {
+                uint32_t at = 0;  // the keys whose element e of this lane's columns is NaN, over the lanes of the column
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (((v[c][e >> 2] >> (8 * (e & 3))) & 0x7f) == 0x7f) {
+                    at |= 1u << (8 * (y + (c >> 1)) + fd_key<D>(2 * tig + (c & 1)));
+                    v[c][e >> 2] &= ~(0xffu << (8 * (e & 3)));
+                  }
+                at |= __shfl_xor_sync(0xffffffffu, at, 1);
+                at |= __shfl_xor_sync(0xffffffffu, at, 2);
+#pragma unroll
+                for (int x = 0; x < HR; ++x)
+#pragma unroll
+                  for (int z = 0; z < 2; ++z) {  // rows 8 x + 2 tig + z
+                    const uint32_t see = __shfl_sync(0xffffffffu, mine[x], 4 * (2 * tig + z));
+                    if (see & at) o[x][e >> 1][2 * (e & 1) + z] = __uint_as_float(0x7fffffffu);
+                  }
+              }
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t va[4], vc[4];
+            widen4(__byte_perm(v[0][w], v[1][w], 0x5140), va[0], va[1]);
+            widen4(__byte_perm(v[2][w], v[3][w], 0x5140), va[2], va[3]);
+            widen4(__byte_perm(v[0][w], v[1][w], 0x7362), vc[0], vc[1]);
+            widen4(__byte_perm(v[2][w], v[3][w], 0x7362), vc[2], vc[3]);
+#pragma unroll
+            for (int x = 0; x < HR; ++x) {
+              fd_mma(o[x][2 * w], va, b[y][x], b[y + 1][x]);
+              fd_mma(o[x][2 * w + 1], vc, b[y][x], b[y + 1][x]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[slot]);
+      if (++slot == NS) slot = 0, ++turn;
     }
     // ---- the warps' parts, joined --------------------------------------------------
 #pragma unroll
@@ -349,16 +467,16 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
         wm[warp * ROWS + r] = m[x] - kFdBias;
         wl[warp * ROWS + r] = l[x];
       }
-      float* o0 = wo + (warp * ROWS + 8 * x + 2 * tig) * D + VB * gid;
+      float* o0 = wo + (warp * ROWS + 8 * x + 2 * tig) * D + VB * fd_chunk<D>(gid);
 #pragma unroll
       for (int e = 0; e < VB / 2; ++e) {
         *reinterpret_cast<float2*>(o0 + 2 * e) = make_float2(o[x][e][0] * vref, o[x][e][2] * vref);
         *reinterpret_cast<float2*>(o0 + D + 2 * e) = make_float2(o[x][e][1] * vref, o[x][e][3] * vref);
       }
     }
-    __syncthreads();
+    fd_sync();
     const bool whole = p.t0 == 0 && p.t1 == p.tiles;
-    for (int e = tid; e < p.rows * (D / 4); e += NT) {
+    for (int e = tid; ok && e < p.rows * (D / 4); e += 32 * WARPS) {
       const int r = e / (D / 4), c = e % (D / 4) * 4;
       float mx = -INFINITY;
 #pragma unroll
@@ -386,26 +504,31 @@ __global__ void __launch_bounds__(FdShape<R16>::NT, FdShape<R16>::CTAS)
         }
       }
     }
-    __syncthreads();
+    fd_sync();
   }
+  }
+  __syncthreads();
   if (tid == 0) {
     A.meta[blockIdx.x] = walk.meta;
-    A.status[blockIdx.x] = 0;
+    A.status[blockIdx.x] = *dead;
   }
 }
 
 template <typename T, int D, bool R16>
 int fd_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
-  using S = FdShape<R16>;
+  using S = FdShape<D, R16>;
   const Plan plan = fp8_decode_plan(a.Hq / a.Hkv * a.T, D);
   const Args A = make_args(a, plan, a.T, kFdLead, ws);
+  CUtensorMap km, vm;
+  int rc = make_fp8_tensor_maps(&km, &vm, a.pool, std::min(a.pool.block, FD_TK));
+  if (rc) return rc;
   auto kern = fp8_decode_kernel<T, D, R16>;
   static DeviceOnce done;
   int dev = 0;
   cudaGetDevice(&dev);
   if (!done.done(dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fd_smem<D, R16>()) != cudaSuccess)
-      return fail(DROPKV_ERR_CUDA, "cannot set attention_fp8 shared memory size %d", fd_smem<D, R16>());
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "cannot set attention_fp8 shared memory size %d", S::BYTES);
     done.mark(dev);
   }
   cudaLaunchConfig_t cfg = {};
@@ -416,12 +539,12 @@ int fd_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
   cfg.numAttrs = 1;
   cfg.stream = st;
   cfg.gridDim = dim3(plan.ctas);
-  cfg.blockDim = dim3(S::NT);
-  cfg.dynamicSmemBytes = fd_smem<D, R16>();
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, A);
+  cfg.blockDim = dim3(FD_NT);
+  cfg.dynamicSmemBytes = S::BYTES;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 launch: %s", cudaGetErrorString(e));
-  int rc = check_launch("attention_fp8");
-  if (rc || a.cap <= S::TK) return rc;  // a cache of one tile: nothing is split
+  rc = check_launch("attention_fp8");
+  if (rc || a.cap <= FD_TK) return rc;  // a cache of one tile: nothing is split
   return launch_fp8_merge(A, dtype, plan.ctas, st);
 }
 
@@ -435,8 +558,7 @@ int fd_typed(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
 }  // namespace
 
 fa::Plan fp8_decode_plan(int rows, int D) {
-  const bool r16 = rows > 8;
-  return make_plan(num_sms_current_device() * (r16 ? FdShape<true>::CTAS : FdShape<false>::CTAS), r16 ? 16 : 8, D);
+  return make_plan(num_sms_current_device() * FD_CTAS, rows > 8 ? 16 : 8, D);
 }
 
 int launch_fp8_decode(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {

@@ -100,6 +100,23 @@ int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, in
   return DROPKV_OK;
 }
 
+int make_fp8_tensor_maps(CUtensorMap* k, CUtensorMap* v, const Fp8Pool& p, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(DROPKV_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  for (int kv = 0; kv < 2; ++kv) {
+    cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.block, (cuuint64_t)p.H, (cuuint64_t)p.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)(kv ? p.v_st : p.k_st), (cuuint64_t)(kv ? p.v_sh : p.k_sh),
+                             (cuuint64_t)(kv ? p.v_s0 : p.k_s0)};
+    cuuint32_t box[4] = {(cuuint32_t)p.D, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(kv ? v : k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, kv ? p.v : p.k, dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, p.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DROPKV_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit pages) failed (%d)", (int)r);
+  }
+  return DROPKV_OK;
+}
+
 // Q viewed as {D, Lq, Hq, B} with box {64, W, g, 1}: one load per 64-wide slab
 // brings the W window rows of the g query heads of one KV head, in the order of
 // the scorer's query rows (m = head * W + row), under the 128-byte swizzle.

@@ -355,6 +355,9 @@ int make_kv_tensor_map(CUtensorMap* map, const void* base, int BH, int L, int D,
 // elements, as a 4-D map {d, key, head, b} of 64 x box_rows boxes (128-byte swizzle).
 int make_kv_tensor_map_4d(CUtensorMap* map, const void* base, int B, int Hkv, int L, int D, bool bf16, int64_t sb,
                           int64_t sh, int64_t ss, int box_rows = 128);
+// The K and V pages of a pool in 8 bits as 4-D maps {d, row, head, page} of D x box_rows boxes, under the
+// swizzle of D bytes (64 or 128).
+int make_fp8_tensor_maps(CUtensorMap* k, CUtensorMap* v, const Fp8Pool& p, int box_rows);
 // All T rows of `heads` heads of x [B, H, T, D] in a box (see the definition).
 bool make_head_tensor_map(CUtensorMap* map, const void* base, int B, int H, int T, int D, bool bf16, int64_t sb, int64_t sh,
                           int64_t ss, int heads);
