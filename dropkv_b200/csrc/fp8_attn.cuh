@@ -170,8 +170,10 @@ struct Walk {
   long long left, per;
   int pair, h, u;
   int4 meta;  // of a split segment that begins here
-  __device__ __forceinline__ explicit Walk(const Start& s)
-      : left(s.w1 - s.w), per(s.per), pair(s.pair), h(s.h), u(s.u), meta(make_int4(0, 0, 0, 0)) {}
+  __device__ __forceinline__ void start(const Start& s) {
+    left = s.w1 - s.w, per = s.per, pair = s.pair, h = s.h, u = s.u;
+    meta = make_int4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ bool next(const Args& A, Piece<TK>& p) {
     while (left > 0) {
       p.b = pair / A.RT;
@@ -200,6 +202,22 @@ struct Walk {
       }
     }
     return false;
+  }
+};
+
+// A warp's walk in shared memory: the first lane steps, all read. What a loop over tiles does not use of it then
+// takes no registers there.
+template <int TK>
+struct WarpWalk {
+  Walk<TK> walk;
+  Piece<TK> piece;
+  __device__ __forceinline__ bool next(const Args& A, int lane) {
+    __syncwarp();
+    int more = 0;
+    if (lane == 0) more = walk.next(A, piece);
+    more = __shfl_sync(0xffffffffu, more, 0);
+    __syncwarp();
+    return more;
   }
 };
 

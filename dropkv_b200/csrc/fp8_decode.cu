@@ -35,10 +35,10 @@ constexpr int FD_HALVES = FD_TK / 8;                      // a page has 8 rows a
 constexpr int FD_CTAS = 2;                                // of an SM
 constexpr uint64_t kFdWaitNs = 1000000000ull;
 
-template <int D, bool R16>
+template <int D, bool R16, int PARTS>
 struct FdShape {
   static constexpr int ROWS = R16 ? 16 : 8;
-  static constexpr int TILE = FD_TK * D, SLOTS = (R16 ? 5 : 6) * (128 / D);
+  static constexpr int TILE = FD_TK * D, SLOTS = (R16 ? 4 : 5) * (128 / D);
   static constexpr int WO = SLOTS * TILE;                        // float [WARPS][ROWS][D]: the warps' outputs
   static constexpr int WM = WO + FD_WARPS * ROWS * D * 4;        // float [2][WARPS][ROWS]: maxima, sums
   // tiles whose scales are held: before tile i's first load is issued, the slot is free that load 2 i - SLOTS had,
@@ -46,10 +46,20 @@ struct FdShape {
   static constexpr int SCALES = SLOTS / 2 + 1;
   static constexpr int SC = WM + 2 * FD_WARPS * ROWS * 4;        // float [SCALES][2][FD_HALVES]: 0 for a missing page
   static constexpr int BARS = SC + SCALES * 2 * FD_HALVES * 4;   // full[SLOTS], empty[SLOTS]
-  static constexpr int START = BARS + 2 * SLOTS * 8;
+  // the queries' operands of S, the same for all warps, lie in shared memory where they are many
+  static constexpr bool QS = R16 || PARTS == 3;
+  static constexpr int ACCS = R16 ? PARTS : PARTS - 1;  // products of S: one for each part; 8 rows' first two share one
+  static constexpr int QO = (BARS + 2 * SLOTS * 8 + 15) / 16 * 16;  // uint4 [ACCS][D / 32][32]
+  static constexpr int WALKS = QO + (QS ? ACCS * (D / 32) * 512 : 0);
+  // WarpWalk [WARPS + 1] there
+  static constexpr int START = WALKS + (FD_WARPS + 1) * (int)sizeof(WarpWalk<FD_TK>);
   static constexpr int BYTES = START + (int)sizeof(Start) + 8;
   static_assert(FD_CTAS * (BYTES + 1024) <= 233472, "shared memory");
 };
+
+// 8-bit parts that hold an element of a query
+template <typename T>
+constexpr int fd_parts() { return std::is_same<T, __nv_bfloat16>::value ? 2 : 3; }
 
 template <int D>
 __device__ __forceinline__ int fd_key(int n) { return D == 128 ? ((n & 1) << 2) | (n >> 1) : n; }
@@ -62,14 +72,14 @@ constexpr int kFdLead = 3;
 constexpr float kFdSlack = 8.f, kFdBias = 7.f;
 
 __device__ __forceinline__ void fd_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void fd_mma8(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -82,9 +92,10 @@ template <typename T, int D, bool R16>
 __global__ void __launch_bounds__(FD_NT, FD_CTAS)
     fp8_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ Args A) {
-  using S = FdShape<D, R16>;
+  constexpr int PARTS = fd_parts<T>();
+  using S = FdShape<D, R16, PARTS>;
   constexpr int TK = FD_TK, WARPS = FD_WARPS, ROWS = S::ROWS, HR = R16 ? 2 : 1, NS = S::SLOTS;
-  constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;  // 8-bit parts of a query's elements
+  constexpr int ACCS = S::ACCS;
   constexpr int KV = D / 64;   // 16-byte vectors of K a lane has of a key
   constexpr int VW = D / 32;   // words of V a lane has of a key
   constexpr int VB = 4 * VW;
@@ -124,8 +135,9 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
   pdl_launch_dependents();  // (after the wait: the merge may then read this kernel's inputs at once)
   if (warp == 0) find_start<TK>(A, lane, start);
   __syncthreads();
-  Walk<TK> walk(*start);
-  Piece<TK> p;
+  WarpWalk<TK>& ww = reinterpret_cast<WarpWalk<TK>*>(sm + S::WALKS)[warp];
+  if (lane == 0) ww.walk.start(*start);
+  const Piece<TK>& p = ww.piece;
   // a wait that gives up marks the CTA dead: every role then ends without waiting
   auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
     if (tc::mbar_try_wait(bar, count & 1)) return true;
@@ -143,7 +155,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
     const int block = a.pool.block, lb = __ffs(block) - 1, box = min(block, TK), boxes = TK / box;
     uint32_t n = 0;
     bool ok = true;
-    while (ok && walk.next(A, p)) {
+    while (ok && ww.next(A, lane)) {
       const int32_t* table = a.table + (int64_t)p.b * a.max_blocks;
       const float* ksb = a.pool.k_scale + p.h * a.pool.ks_sh;
       const float* vsb = a.pool.v_scale + p.h * a.pool.vs_sh;
@@ -203,7 +215,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
     const int r = 32 * warp + fd_key<D>(2 * tig + c);
     v_at[c] = VW == 4 ? tc::swz_offset<D>(r, fd_chunk<D>(gid) * 8) : tc::swz_offset<D>(r, (gid >> 1) * 8) + (gid & 1) * 8;
   }
-  while (walk.next(A, p)) {
+  while (ww.next(A, lane)) {
     // ---- queries: rows gid and, of 16, gid + 8 ---------------------------------
     uint32_t q[PARTS][KV * 4][HR];  // four elements a word, as a lane has them of K
     float qscale[HR];
@@ -248,6 +260,29 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
 #pragma unroll
         for (int s = 0; s < KV * 4; ++s) q[part][s][x] = split4(v + 4 * s, 16.f);
     }
+    // operand A of S for step e of D (two words of a vector) and product j
+    auto operand = [&](int j, int e, uint32_t* qa) {
+      if (R16) {
+        qa[0] = q[j][e][0], qa[1] = q[j][e][HR - 1], qa[2] = q[j][e + 1][0], qa[3] = q[j][e + 1][HR - 1];
+      } else if (j == 0) {  // rows 8 to 15 are the second part's
+        qa[0] = q[0][e][0], qa[1] = q[1][e][0], qa[2] = q[0][e + 1][0], qa[3] = q[1][e + 1][0];
+      } else {
+        qa[0] = q[PARTS - 1][e][0], qa[1] = 0u, qa[2] = q[PARTS - 1][e + 1][0], qa[3] = 0u;
+      }
+    };
+    uint4* qo = reinterpret_cast<uint4*>(sm + S::QO) + lane;
+    if (S::QS) {  // (all warps are past the piece before: they met at its end)
+#pragma unroll
+      for (int e = 0; e < 4 * KV; e += 2)
+#pragma unroll
+        for (int j = 0; j < ACCS; ++j)
+          if ((e / 2) % WARPS == warp) {
+            uint32_t qa[4];
+            operand(j, e, qa);
+            qo[(j * 2 * KV + e / 2) * 32] = make_uint4(qa[0], qa[1], qa[2], qa[3]);
+          }
+      fd_sync();
+    }
     // ---- the warp's steps --------------------------------------------------------
     float o[HR][VB / 2][4];
     float m[HR], l[HR];
@@ -274,40 +309,44 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       float s[4][2 * HR];  // of eight keys each: rows gid, then gid + 8
       if (some) {
         const uint8_t* kt = sm + slot * S::TILE;
+        constexpr int XS = ACCS < 3 ? 4 : 2;  // eights of keys at once: four chains of products or more
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float c[PARTS][4];
+        for (int x0 = 0; x0 < 4; x0 += XS) {
+          float c[XS][ACCS][4];
+          uint4 k[XS][KV];
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) c[part][0] = c[part][1] = c[part][2] = c[part][3] = 0.f;
+          for (int x = 0; x < XS; ++x) {
 #pragma unroll
-          for (int i = 0; i < KV; ++i) {
-            const uint4 k = *reinterpret_cast<const uint4*>(kt + k_at[i] + x * 8 * D);  // (the swizzle repeats after 8 rows)
-            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+            for (int i = 0; i < KV; ++i)
+              k[x][i] = *reinterpret_cast<const uint4*>(kt + k_at[i] + (x0 + x) * 8 * D);  // (the swizzle repeats after 8 rows)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int e = 4 * i + 2 * h;
-              if (R16) {
+            for (int j = 0; j < ACCS; ++j) c[x][j][0] = c[x][j][1] = c[x][j][2] = c[x][j][3] = 0.f;
+          }
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                  const uint32_t qa[4] = {q[part][e][0], q[part][e][HR - 1], q[part][e + 1][0], q[part][e + 1][HR - 1]};
-                  fd_mma8(c[part], qa, w[2 * h], w[2 * h + 1]);
-                }
-              } else {  // rows 8 to 15 are the second part's
-                const uint32_t qa[4] = {q[0][e][0], q[1][e][0], q[0][e + 1][0], q[1][e + 1][0]};
-                fd_mma8(c[0], qa, w[2 * h], w[2 * h + 1]);
-                if (PARTS == 3) {
-                  const uint32_t qb[4] = {q[PARTS - 1][e][0], 0u, q[PARTS - 1][e + 1][0], 0u};
-                  fd_mma8(c[PARTS - 1], qb, w[2 * h], w[2 * h + 1]);
-                }
+          for (int e = 0; e < 4 * KV; e += 2)
+#pragma unroll
+            for (int j = 0; j < ACCS; ++j) {
+              uint32_t qa[4];
+              if (S::QS) {
+                const uint4 y = qo[(j * 2 * KV + e / 2) * 32];
+                qa[0] = y.x, qa[1] = y.y, qa[2] = y.z, qa[3] = y.w;
+              } else {
+                operand(j, e, qa);
+              }
+#pragma unroll
+              for (int x = 0; x < XS; ++x) {
+                const uint4 kx = k[x][e / 4];
+                fd_mma8(c[x][j], qa, e % 4 ? kx.z : kx.x, e % 4 ? kx.w : kx.y);
               }
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 2 * HR; ++e) {
-            float z = R16 ? c[1][e] : c[0][e + 2];
-            if (PARTS == 3) z = fmaf(c[PARTS - 1][e], 0.0625f, z);
-            s[x][e] = fmaf(z, 0.0625f, c[0][e]);
-          }
+          for (int x = 0; x < XS; ++x)
+#pragma unroll
+            for (int e = 0; e < 2 * HR; ++e) {
+              float z = R16 ? c[x][ACCS > 1 ? 1 : 0][e] : c[x][0][(e + 2) & 3];
+              if (PARTS == 3) z = fmaf(c[x][ACCS - 1][e], 0.0625f, z);
+              s[x0 + x][e] = fmaf(z, 0.0625f, c[x][0][e]);
+            }
         }
       }
       __syncwarp();
@@ -509,14 +548,14 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
   }
   __syncthreads();
   if (tid == 0) {
-    A.meta[blockIdx.x] = walk.meta;
+    A.meta[blockIdx.x] = ww.walk.meta;
     A.status[blockIdx.x] = *dead;
   }
 }
 
 template <typename T, int D, bool R16>
 int fd_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
-  using S = FdShape<D, R16>;
+  using S = FdShape<D, R16, fd_parts<T>()>;
   const Plan plan = fp8_decode_plan(a.Hq / a.Hkv * a.T, D);
   const Args A = make_args(a, plan, a.T, kFdLead, ws);
   CUtensorMap km, vm;
