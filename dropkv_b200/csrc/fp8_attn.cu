@@ -1,91 +1,626 @@
-// Attention over a paged cache held in 8 bits: for token i of sequence b and query head h,
-// O = sum_j softmax_j(scale q . k8_j sk_j) v8_j sv_j over the rows j that it sees, with the
-// scales sk and sv of the rows' pages.
+// Attention over a paged cache held in 8 bits for many query rows (g T > 16): drafted trees, prompt chunks; and the
+// kernel that joins partials. For token i of sequence b and query head h, O = sum_j softmax_j(scale q . k8_j sk_j)
+// v8_j sv_j over the rows j that it sees, with the scales sk and sv of the rows' pages.
+//
+// A CTA has 128 query rows (whole tokens of a KV head's group) and two CTAs share an SM, so that one's softmax runs
+// beside the other's products; keys come in tiles of 64. Both products are tcgen05 MMAs:
+//   S = Q K^T  kind::f8f6f4, K's bytes as TMA brings them; queries as sums of 8-bit parts (two hold a bf16,
+//              three an fp16), each part a product into the same accumulator: as many operations as in 16 bits
+//              (half as many again for fp16), and no tile of K is ever widened;
+//   O += P V   kind::f16: weights in fp16 left in tensor memory where S was, V widened to fp16 (exactly) by two
+//              warps from one ring of tiles into another. (V as it lies would need weights in 8-bit parts: two roundings
+//              and conversions a weight, for a tile's 128 rows, instead of one a byte of V.)
+// S has two buffers, and the product of a tile is issued before the weights of the one before it are
+// awaited. Warps: four of softmax, a thread for each row; two that widen V; one for TMA (a box a page); one that
+// issues products.
+// A page's scale of K enters with the exponent's argument, that of V, over the largest of the warp so far, with the
+// weights (both for eight keys at a time: pages have eight rows at least). Weights are rounded to fp16 (2^-11),
+// sums taken from them before that.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_attn.cuh"
+#include "tc_common.cuh"
 
 namespace dropkv {
 namespace {
 
-constexpr int FA_NT = 128;
+using namespace fa;
 
-template <typename T>
-__device__ __forceinline__ T fa_from(float x);
-template <>
-__device__ __forceinline__ __half fa_from<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 fa_from<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+constexpr int FA_ROWS = 128;  // query rows of a CTA
+constexpr int FA_TK = 64;     // keys of a tile
+constexpr int FA_HALVES = FA_TK / 8;
+constexpr int FA_WARP_V = 4, FA_WARP_TMA = 6, FA_WARP_MMA = 7, FA_NT = 256;
+constexpr int FA_CTAS = 2;    // of an SM
+constexpr int kFaLead = 4;
+constexpr uint64_t kFaWaitNs = 1000000000ull;
+// A row's reference moves once its maximum has grown by this much (base 2); weights are
+// 2^(s - m + bias), so that fp16 holds them from 2^-24 to 2^15.
+constexpr float kFaSlack = 8.f, kFaBias = 7.f;
 
-__device__ __forceinline__ float fa_widen(uint8_t x) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3))); }
+template <int D, int PARTS>
+struct FaSmem {
+  static constexpr int NS = PARTS == 2 ? 3 : 2;         // slots of K's ring, and of V's
+  static constexpr int TILE = FA_TK * D;                // a tile of K or V
+  static constexpr int Q = 0;                           // PARTS x [128 rows][D]
+  static constexpr int V16 = Q + PARTS * FA_ROWS * D;   // 2 x D / 64 slabs of [64 keys][128 bytes]
+  static constexpr int K = V16 + 2 * 2 * TILE;
+  static constexpr int V = K + NS * TILE;
+  // Tiles whose scales are held: the load of K of tile i waits for the product of tile i - NS, which waits for the weights
+  // of tile i - NS - 2, and V's before it for tile i - 1 - NS to be widened; so all are past the tile NS + 2 back.
+  static constexpr int SCALES = NS + 2;
+  static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: 0 for a missing page
+  static constexpr int WALKS = SC + SCALES * 2 * FA_HALVES * 4;  // WarpWalk [4], of the softmax warps
+  static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
+  static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_SC = 4 * NS, B_S = B_SC + SCALES, B_P = B_S + 2,
+                       B_W = B_P + 2, B_O = B_W + 2, B_Q = B_O + 2, B_END = B_Q + 1, BARRIERS = B_END + 1;
+  static constexpr int START = BARS + BARRIERS * 8;
+  static constexpr int MISC = START + (int)sizeof(Start);  // tensor memory's address, `dead`, bad[2][2]
+  static constexpr int BYTES = MISC + 24;
+  static_assert(FA_CTAS * (BYTES + 1024) <= 233472, "shared memory");
+};
 
-// A CTA has one query row and takes 128 rows of the cache at a time, a thread a row for the
-// logits and a column for the output.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(FA_NT) attention_fp8_row_kernel(const __grid_constant__ AttnFp8 a) {
-  __shared__ float q[D], w[FA_NT], red[FA_NT / 32];
-  __shared__ int64_t at[FA_NT];
-  __shared__ float sv[FA_NT];
+__global__ void __launch_bounds__(FA_NT, FA_CTAS)
+    fp8_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                    const __grid_constant__ Args A) {
+  constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+  using L = FaSmem<D, PARTS>;
+  constexpr int NS = L::NS, SLABS = D / 64, TK = FA_TK;
+  extern __shared__ __align__(1024) uint8_t sm[];  // swizzled tiles start on multiples of 1024
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
+  float* sc = reinterpret_cast<float*>(sm + L::SC);
+  Start* start = reinterpret_cast<Start*>(sm + L::START);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
+  volatile int* dead = reinterpret_cast<volatile int*>(misc + 1);
+  volatile int* bad = reinterpret_cast<volatile int*>(misc + 2);  // [2][2]: a widening warp met NaN in a masked tile
+  const AttnFp8& a = A.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x;
-  const int i = (int)(row % a.T), hq = (int)(row / a.T % a.Hq), b = (int)(row / a.T / a.Hq), h = hq / (a.Hq / a.Hkv);
-  if (tid < D) q[tid] = to_f(static_cast<const T*>(a.q)[b * a.q_sb + hq * a.q_sh + i * a.q_ss + tid * a.q_sd]) * a.scale;
-  const int len = max(a.cache_lens[b], 0), keys = (int)min((int64_t)len + a.T, (int64_t)a.cap);
-  const uint8_t* mr = a.mask ? a.mask + b * a.mask_sb + i * a.mask_sr : nullptr;
-  int depth = i;
-  if (mr) {
-    depth = -1;
-    for (int n = 0; n < a.T; ++n) depth += mr[n * a.mask_sc] != 0;
-    depth = max(depth, 0);
-  }
-  const int64_t first = a.window ? (int64_t)len + depth - a.window + 1 : 0;
-  auto over_cta = [&](float x, bool sum) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, x, o);
-      x = sum ? x + y : fmaxf(x, y);
+  if (tc::smem_addr(sm) % 1024) {  // as declared; nothing may run on any other layout
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tid == 0) {
+      A.status[blockIdx.x] = 9;
+      A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
     }
-    __syncthreads();
-    if (lane == 0) red[warp] = x;
-    __syncthreads();
-    x = red[0];
-    for (int k = 1; k < FA_NT / 32; ++k) x = sum ? x + red[k] : fmaxf(x, red[k]);
-    return x;
-  };
-  float m = -INFINITY, l = 0.f, o = 0.f;
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      tc::mbar_init(&bars[L::B_KF + i], 1);
+      tc::mbar_init(&bars[L::B_KE + i], 1);
+      tc::mbar_init(&bars[L::B_VF + i], 1);
+      tc::mbar_init(&bars[L::B_VE + i], 2);
+    }
+    for (int i = 0; i < L::SCALES; ++i) tc::mbar_init(&bars[L::B_SC + i], 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars[L::B_S + i], 1);
+      tc::mbar_init(&bars[L::B_P + i], 4);
+      tc::mbar_init(&bars[L::B_W + i], 2);
+      tc::mbar_init(&bars[L::B_O + i], 1);
+    }
+    tc::mbar_init(&bars[L::B_Q], 4);
+    tc::mbar_init(&bars[L::B_END], 1);
+    tc::fence_mbar_init();
+    *dead = 0;
+  }
+  if (warp == FA_WARP_MMA) {
+    tc::tmem_alloc(misc, 256);
+    tc::tmem_relinquish();
+  }
+  if (warp == FA_WARP_TMA && lane == 0) {
+    tc::tma_prefetch_desc(&kmap);
+    tc::tma_prefetch_desc(&vmap);
+  }
+  pdl_wait();
+  pdl_launch_dependents();  // (after the wait: the merge may then read this kernel's inputs at once)
+  if (warp == 0) find_start<TK>(A, lane, start);
+  tc::tc_fence_before();
   __syncthreads();
-  for (int j0 = 0; j0 < keys; j0 += FA_NT) {
-    const int j = j0 + tid;
-    float s = -INFINITY;
-    int64_t v_at = -1;
-    if (j < keys) {
-      bool see = j < a.sinks || j >= first || (mr && j >= len);
-      if (j >= len) see = see && (mr ? mr[(j - len) * a.mask_sc] != 0 : j - len <= i);
-      const int page = see ? a.table[(int64_t)b * a.max_blocks + j / a.pool.block] : -1;
-      if (page >= 0 && page < a.pool.n_pages) {
-        const uint8_t* k = static_cast<const uint8_t*>(a.pool.k) + page * a.pool.k_s0 + h * a.pool.k_sh + (j % a.pool.block) * a.pool.k_st;
-        float x = 0.f;
-        for (int d = 0; d < D; ++d) x = fmaf(q[d], fa_widen(k[d]), x);
-        s = x * a.pool.k_scale[page * a.pool.ks_s0 + h * a.pool.ks_sh];
-        v_at = page * a.pool.v_s0 + h * a.pool.v_sh + (j % a.pool.block) * a.pool.v_st;
-        sv[tid] = a.pool.v_scale[page * a.pool.vs_s0 + h * a.pool.vs_sh];
+  tc::tc_fence_after();
+  const uint32_t tmem = *misc;  // S (and P) 2 x 64 columns, O 128
+  // a wait that gives up marks the CTA dead: every role then ends without waiting
+  auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
+    if (tc::mbar_try_wait(bar, count & 1)) return true;
+    const uint64_t t0 = tc::globaltimer_ns();
+    while (!*dead) {
+      if (tc::mbar_try_wait(bar, count & 1)) return true;
+      if (tc::globaltimer_ns() - t0 > kFaWaitNs) *dead = why;
+    }
+    return false;
+  };
+  // Tile j of the CTA (from 0, over all pieces): K and V in slot j % NS, scales in place j % SCALES, S, P and widened V
+  // in buffer j % 2. What waits for what: K's load for the product that had the slot; S(j) for K and for O(j - 2), which has
+  // read P in its buffer; P(j) for S(j); widened V(j) for V's load and O(j - 2); O(j) for P(j) and widened V(j).
+  // A wait that is not taken for every tile (O's, where a reference moves; widened V's, in masked tiles) begins
+  // with the phase before over, which S(j) says, and ends before the next, which needs P(j).
+  if (warp == FA_WARP_TMA) {
+    // ======================= TMA producer =======================================
+    const int block = a.pool.block, lb = __ffs(block) - 1, box = min(block, TK), boxes = TK / box;
+    Walk<TK> walk;
+    Piece<TK> p;
+    walk.start(*start);
+    uint32_t n = 0, slot = 0, turn = 0, place = 0;
+    bool ok = true;
+    while (ok && walk.next(A, p)) {
+      const int32_t* table = a.table + (int64_t)p.b * a.max_blocks;
+      const float* ksb = a.pool.k_scale + p.h * a.pool.ks_sh;
+      const float* vsb = a.pool.v_scale + p.h * a.pool.vs_sh;
+      // a lane has eight keys of a tile: their page, -1 where no token sees any of them
+      auto page_of = [&](int t) {
+        if (t >= p.t1 || lane >= FA_HALVES) return -1;
+        const int j = p.k.first(t) + 8 * lane;
+        return p.k.any(A, j, 8) ? table[j >> lb] : -1;
+      };
+      auto there = [&](int page) { return page >= 0 && page < a.pool.n_pages; };
+      int page = page_of(p.t0), page1 = page_of(p.t0 + 1);
+      float ks = there(page) ? ksb[page * a.pool.ks_s0] : 0.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
+      for (int t = p.t0; t < p.t1; ++t, ++n) {
+        const int page2 = page_of(t + 2);
+        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : 0.f;
+        const float vs1 = there(page1) ? vsb[page1 * a.pool.vs_s0] : 0.f;
+        // the page of a lane's box: that of any of its eights that is read, else out of range (zeros)
+        int at = there(page) ? page : -1;
+        for (int o = 1; o < box / 8; o <<= 1) at = max(at, __shfl_xor_sync(0xffffffffu, at, o));
+        at = __shfl_sync(0xffffffffu, at, min(lane, boxes - 1) * (box / 8));
+        if (at < 0) at = a.pool.n_pages;
+        const int row = p.k.first(t) & (block - 1);  // (of a page larger than a tile; else 0)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t* full = &bars[(kv ? L::B_VF : L::B_KF) + slot];
+          if (turn) ok = __all_sync(0xffffffffu, wait(&bars[(kv ? L::B_VE : L::B_KE) + slot], turn - 1, 1 + kv));
+          if (!ok) break;
+          if (kv == 0) {
+            if (lane < FA_HALVES) {
+              float* s = sc + place * (2 * FA_HALVES) + lane;
+              s[0] = ks;
+              s[FA_HALVES] = vs;
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bars[L::B_SC + place]);
+          }
+          if (lane == 0) tc::mbar_arrive_expect_tx(full, L::TILE);
+          __syncwarp();
+          if (lane < boxes)
+            tc::tma_load_4d(sm + (kv ? L::V : L::K) + slot * L::TILE + lane * box * D, kv ? &vmap : &kmap, full, 0, row, p.h, at);
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (++slot == NS) slot = 0, ++turn;
+        if (++place == L::SCALES) place = 0;
+        page = page1, page1 = page2, ks = ks1, vs = vs1;
       }
     }
-    at[tid] = v_at;
-    const float mn = fmaxf(m, over_cta(s, false)), ref = mn == -INFINITY ? 0.f : mn;
-    const float f = m == mn ? 1.f : expf(m - ref), p = v_at < 0 ? 0.f : expf(s - ref);
-    m = mn;
-    l = l * f + over_cta(p, true);
-    o *= f;
-    w[tid] = p;
-    __syncthreads();
-    if (tid < D) {
-      for (int n = 0; n < FA_NT; ++n)
-        if (at[n] >= 0) o = fmaf(w[n] * sv[n], fa_widen(static_cast<const uint8_t*>(a.pool.v)[at[n] + tid]), o);
+    if (*dead) {  // every issued copy lands before the CTA may exit (of the tile that gave up, K may be one)
+      for (uint32_t j = n > (uint32_t)NS ? n - NS : 0u; j <= n; ++j)
+        for (int kv = 0; kv < 2; ++kv)
+          if (j < n || kv == 0) tc::mbar_wait(&bars[(kv ? L::B_VF : L::B_KF) + j % NS], (j / NS) & 1, kFaWaitNs / 8);
     }
-    __syncthreads();
+  } else if (warp == FA_WARP_MMA) {
+    // ======================= MMA issuer =========================================
+    // The whole warp runs this and one lane issues, so that counts, addresses and descriptors can stay uniform.
+    constexpr uint32_t ID_QK = tc::idesc_e4m3(FA_ROWS, TK);
+    constexpr uint32_t ID_PV = tc::idesc_f16(false, FA_ROWS, D, false, true);
+    constexpr uint32_t LAYOUT = tc::layout_for_row_bytes(D);
+    constexpr uint32_t LBO_V = SLABS == 2 ? TK * 128 : 0;
+    const uint32_t base = __shfl_sync(0xffffffffu, tc::smem_addr(sm), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+    Walk<TK> walk;
+    Piece<TK> p;
+    walk.start(*start);
+    uint32_t j = 0, slot = 0, turn = 0, pieces = 0;
+    bool ok = true;
+    // O of tile i: the first of a piece begins it
+    auto product = [&](uint32_t i, bool first) {
+      const uint32_t buf = i & 1;
+      ok = __all_sync(0xffffffffu, wait(&bars[L::B_P + buf], i >> 1, 3) && wait(&bars[L::B_W + buf], i >> 1, 4));
+      if (!ok) return;
+      tc::tc_fence_after();
+      if (tc::elect_one()) {
+        const uint64_t vd = tc::smem_desc(base + L::V16 + buf * (2 * L::TILE), LBO_V, 1024);
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          tc::mma_f16_tmem_a(tm + 128, tm + buf * 64 + kk * 8, tc::desc_add(vd, kk * 2048), ID_PV, !first || kk > 0);
+        tc::mma_commit(&bars[L::B_O + buf]);
+      }
+      __syncwarp();
+    };
+    while (ok && walk.next(A, p)) {
+      const int nt = __shfl_sync(0xffffffffu, p.t1 - p.t0, 0);
+      ok = __all_sync(0xffffffffu, wait(&bars[L::B_Q], pieces++, 5));
+      for (int i = 0; i < nt && ok; ++i, ++j) {
+        const uint32_t buf = j & 1;
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_KF + slot], turn, 6) && (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 7)));
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (tc::elect_one()) {
+          const uint64_t kd = tc::smem_desc(base + L::K + slot * L::TILE, 16, 8 * D, LAYOUT);
+          const uint64_t qd = tc::smem_desc(base + L::Q, 16, 8 * D, LAYOUT);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+            for (int kk = 0; kk < D / 32; ++kk)
+              tc::mma_f8(tm + buf * 64, tc::desc_add(qd, part * (FA_ROWS * D) + kk * 32), tc::desc_add(kd, kk * 32), ID_QK,
+                         part > 0 || kk > 0);
+          tc::mma_commit(&bars[L::B_S + buf]);
+          tc::mma_commit(&bars[L::B_KE + slot]);
+        }
+        __syncwarp();
+        if (++slot == NS) slot = 0, ++turn;
+        if (i > 0) product(j - 1, i == 1);
+      }
+      if (ok) product(j - 1, nt == 1);
+    }
+    if (*dead) {  // no product may run on when tensor memory is given back
+      if (tc::elect_one()) tc::mma_commit(&bars[L::B_END]);
+      __syncwarp();
+      tc::mbar_wait(&bars[L::B_END], 0, kFaWaitNs);
+    }
+  } else if (warp >= FA_WARP_V) {
+    // ======================= V to fp16 ==========================================
+    // A thread has a key's row: 16-byte reads and writes of eight rows at a time meet all banks once.
+    const int r = tid - FA_WARP_V * 32;
+    Walk<TK> walk;
+    Piece<TK> p;
+    walk.start(*start);
+    uint32_t j = 0, slot = 0, turn = 0, place = 0, round = 0;
+    bool ok = true;
+    while (ok && walk.next(A, p)) {
+      int all_end, all_low;
+      p.k.all(A, &all_end, &all_low);
+      for (int t = p.t0; t < p.t1; ++t, ++j) {
+        const uint32_t buf = j & 1;
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 8) && wait(&bars[L::B_VF + slot], turn, 9) &&
+                                         (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
+        if (!ok) break;
+        const float* vs = sc + place * (2 * FA_HALVES) + FA_HALVES;
+        const bool there = vs[r >> 3] > 0.f;
+        const int j0 = p.k.first(t);
+        const bool masked = __any_sync(0xffffffffu, !(vs[lane & 7] > 0.f)) || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks);
+        const uint8_t* src = sm + L::V + slot * L::TILE;
+        uint8_t* dst = sm + L::V16 + buf * (2 * L::TILE);
+        uint32_t nan = 0;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          uint4 x = *reinterpret_cast<const uint4*>(src + tc::swz_offset<D>(r, c * 8));
+          if (masked) {
+            // what a weight of 0 would not silence: rows past the keys are cleared, and NaN is taken out here and given to those
+            // who see it at the end
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t odd = __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              if (!there || j0 + r >= p.k.keys)
+                w[e] = 0;
+              else
+                nan |= odd, w[e] &= ~odd;
+            }
+            x = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          uint4 lo, hi;
+          widen4(x.x, lo.x, lo.y);
+          widen4(x.y, lo.z, lo.w);
+          widen4(x.z, hi.x, hi.y);
+          widen4(x.w, hi.z, hi.w);
+          uint8_t* slab = dst + (c / 4) * (TK * 128);
+          *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16)) = lo;
+          *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16 + 8)) = hi;
+        }
+        if (masked) {
+          const int some = __any_sync(0xffffffffu, nan != 0);
+          if (lane == 0) bad[2 * buf + warp - FA_WARP_V] = some;
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(&bars[L::B_W + buf]);
+          tc::mbar_arrive(&bars[L::B_VE + slot]);
+        }
+        if (++slot == NS) slot = 0, ++turn;
+        if (++place == L::SCALES) place = 0, ++round;
+      }
+    }
+  } else {
+    // ======================= softmax ============================================
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16, to = tmem + lanes + 128;
+    const int r = tid;
+    WarpWalk<TK>& ww = reinterpret_cast<WarpWalk<TK>*>(sm + L::WALKS)[warp];
+    if (lane == 0) ww.walk.start(*start);
+    const Piece<TK>& p = ww.piece;
+    uint32_t j = 0, place = 0, round = 0;
+    bool ok = true;
+    float unit = 0.f;  // of the row's queries, and of logits in base 2
+    Sees sees;
+    // A piece's queries: a thread's row in 8-bit parts (what a part leaves goes to the next), in units of a power of two.
+    // The products that read the last piece's are done once S of its last tile is there.
+    auto queries = [&]() {
+      T x[D];
+      const bool own = r < p.rows;
+      if (own) {
+        const int node = p.k.n0 + r / A.g, head = p.h * A.g + r % A.g;
+        const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss;
+        if (A.q_vec) {
+#pragma unroll
+          for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(x + e) = *reinterpret_cast<const uint4*>(src + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < D; ++e) x[e] = src[e * a.q_sd];
+        }
+        sees.set(A, p.b, p.k.len, p.k.keys, node);
+      } else {
+#pragma unroll
+        for (int e = 0; e < D; ++e) x[e] = T(0.f);
+        sees.none();
+      }
+      float big = 0.f;
+#pragma unroll
+      for (int e = 0; e < D; ++e) {
+        const float f = to_f(x[e]);
+        big = fmaxf(big, isfinite(f) ? fabsf(f) : 0.f);
+      }
+      unit = query_unit(big);
+      const float inv = 1.f / unit;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float f = to_f(x[16 * c + e]);
+          v[e] = isfinite(f) ? f * inv : __uint_as_float(0x7fffffffu);
+        }
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          uint4 w;
+          w.x = split4(v, 1.f);
+          w.y = split4(v + 4, 1.f);
+          w.z = split4(v + 8, 1.f);
+          w.w = split4(v + 12, 1.f);
+          *reinterpret_cast<uint4*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(r, c * 8)) = w;
+        }
+      }
+      unit *= A.scale_log2;
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bars[L::B_Q]);
+    };
+    int4 split = make_int4(0, 0, 0, 0);  // the split segment that begins in this CTA (its last piece)
+    bool more = ww.next(A, lane);
+    if (more) queries();
+    while (more) {
+      const bool live = warp * 32 < p.rows;  // some row of this warp exists
+      float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
+      int any_bad = 0, all_end, all_low;
+      p.k.all(A, &all_end, &all_low);
+      for (int t = p.t0; t < p.t1 && ok; ++t, ++j) {
+        const uint32_t buf = j & 1, ts = tmem + lanes + buf * 64;
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 11));
+        if (!ok) break;
+        const float* scales = sc + place * (2 * FA_HALVES);
+        if (++place == L::SCALES) place = 0, ++round;
+        if (!live) {
+          ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&bars[L::B_P + buf]);
+          continue;
+        }
+        float c[FA_HALVES], f[FA_HALVES];
+        float least = INFINITY, vmax = 0.f;
+#pragma unroll
+        for (int y = 0; y < FA_HALVES; ++y) {
+          c[y] = scales[y];
+          f[y] = scales[FA_HALVES + y];
+          least = fminf(least, c[y]);
+          vmax = fmaxf(vmax, f[y]);
+        }
+        const int j0 = p.k.first(t);
+        const bool masked = !(least > 0.f) || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks);
+        uint64_t see = ~0ull;
+        if (masked) {
+          see = sees.bits(A, p.b, p.k.len, j0, TK);
+#pragma unroll
+          for (int y = 0; y < FA_HALVES; ++y)
+            if (!(c[y] > 0.f)) see &= ~(0xffull << (8 * y));
+        }
+#pragma unroll
+        for (int y = 0; y < FA_HALVES; ++y) c[y] = fminf(c[y] * unit, 3e38f);
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
+        if (!ok) break;
+        tc::tc_fence_after();
+        float x[TK];
+        tc::tmem_ld64(ts, x);
+        float top = -INFINITY;
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < TK; ++e) x[e] = (see >> e) & 1 ? x[e] * c[e / 8] : -INFINITY;
+#pragma unroll
+          for (int y = 0; y < FA_HALVES; ++y) c[y] = 1.f;
+        }
+#pragma unroll
+        for (int y = 0; y < FA_HALVES; ++y) {
+          float mx = max3(x[8 * y], x[8 * y + 1], x[8 * y + 2]);
+          mx = max3(mx, x[8 * y + 3], x[8 * y + 4]);
+          mx = max3(mx, x[8 * y + 5], x[8 * y + 6]);
+          mx = fmaxf(mx, x[8 * y + 7]);
+          top = fmaxf(top, mx * c[y]);
+        }
+        const bool first = t == p.t0;
+        // the reference moves where some row's maximum has outgrown it, or a page's scale of V the others'
+        if (__any_sync(0xffffffffu, top > m + kFaSlack) || vmax > vref) {
+          const float mn = top > m + kFaSlack ? top : m;
+          float alpha = mn == m ? 1.f : ex2(m - mn);
+          m = mn;
+          l *= alpha;
+          if (vmax > vref) {
+            alpha *= vref / vmax;
+            vref = vmax;
+            vinv = 1.f / vmax;
+          }
+          if (!first) {
+            ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + 1 - buf], (j - 1) >> 1, 13));
+            tc::tc_fence_after();
+            float o[16];
+#pragma unroll 1
+            for (int e0 = 0; e0 < D; e0 += 16) {
+              tc::tmem_ld16(to + e0, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tc::tmem_st16(to + e0, o);
+              tc::tmem_st_wait();
+            }
+          }
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
+        const uint64_t ref2 = pair_of(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
+        uint32_t pk[TK / 2];
+        bool even = true;  // every page has the largest scale
+#pragma unroll
+        for (int y = 0; y < FA_HALVES; ++y) even = even && f[y] == vref;
+        auto weigh = [&](auto scaled) {
+#pragma unroll
+          for (int y = 0; y < FA_HALVES; ++y) {
+            const uint64_t c2 = pair_of(c[y], c[y]), f2 = pair_of(f[y] * vinv, f[y] * vinv);
+#pragma unroll
+            for (int e = 8 * y; e < 8 * y + 8; e += 2) {
+              float u, v;
+              unpair(fma2(pair_of(x[e], x[e + 1]), c2, ref2), u, v);
+              uint64_t w = pair_of(ex2(u), ex2(v));
+              sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
+              if (decltype(scaled)::value) w = mul2(w, f2);
+              unpair(w, u, v);
+              pk[e / 2] = pack_half(u, v);
+            }
+          }
+        };
+        if (even)
+          weigh(std::false_type());
+        else
+          weigh(std::true_type());
+        tc::tmem_st16(ts, reinterpret_cast<const float*>(pk));
+        tc::tmem_st16(ts + 16, reinterpret_cast<const float*>(pk + 16));
+        float s0, s1, s2, s3;
+        unpair(sum[0], s0, s1);
+        unpair(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
+        if (masked) {
+          ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
+          any_bad |= bad[2 * buf] | bad[2 * buf + 1];
+        }
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bars[L::B_P + buf]);
+      }
+      // ---- the piece's output; the next one's queries first ----------------------
+      if (p.parts) split = make_int4(p.b, p.h, p.rt, p.parts);
+      const int b = p.b, h = p.h, n0 = p.k.n0, t0 = p.t0, t1 = p.t1;
+      const bool whole = t0 == 0 && t1 == p.tiles, own = r < p.rows && ok;
+      const int64_t slot = slot_of(p);
+      const Sees saw = sees;
+      const Keys<TK> keys = p.k;
+      more = ww.next(A, lane);
+      if (more) queries();
+      if (!ok) continue;
+      const uint32_t last = j - 1;
+      ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + (last & 1)], last >> 1, 15));
+      if (!ok) continue;
+      tc::tc_fence_after();
+      if (live) {
+        // (l counts weights, of which a row that sees anything has one of 2^-1 at least)
+        const float inv = l == 0.f ? 0.f : vref / l;
+        uint32_t nan[D / 32];  // columns whose value is NaN for a row of V that this row sees
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) nan[w] = 0;
+        if (any_bad && own) {
+          const uint8_t* vb = static_cast<const uint8_t*>(a.pool.v) + h * a.pool.v_sh;
+          for (int t = t0; t < t1; ++t) {
+            const int j0 = keys.first(t);
+            uint64_t todo = saw.bits(A, b, keys.len, j0, TK);
+            while (todo) {
+              const int key = j0 + __ffsll((long long)todo) - 1;
+              todo &= todo - 1;
+              const int page = a.table[(int64_t)b * a.max_blocks + key / a.pool.block];
+              if (page < 0 || page >= a.pool.n_pages) continue;
+              const uint8_t* v = vb + page * a.pool.v_s0 + (key % a.pool.block) * a.pool.v_st;
+#pragma unroll
+              for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                  const uint32_t y = *reinterpret_cast<const uint32_t*>(v + 32 * w + e);
+                  const uint32_t odd = __vcmpeq4(y & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x01010101u;
+                  nan[w] |= ((odd * 0x10204080u) >> 28) << e;
+                }
+            }
+          }
+        }
+        T* dst = static_cast<T*>(a.out) + out_row(A, b, h, n0, own ? r : 0) * D;
+        float* part = A.part_o + (slot * A.rows_pad + r) * D;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w) {
+          float o[32];
+          tc::tmem_ld32(to + 32 * w, o);
+          if (nan[w]) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((nan[w] >> e) & 1) o[e] = __uint_as_float(0x7fffffffu);
+          }
+          if (!own) continue;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>(dst + 32 * w + e) =
+                  make_uint4(Out<T>::pack(o[e], o[e + 1]), Out<T>::pack(o[e + 2], o[e + 3]), Out<T>::pack(o[e + 4], o[e + 5]),
+                             Out<T>::pack(o[e + 6], o[e + 7]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(part + 32 * w + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (own && !whole) {
+          A.part_ml[slot * 2 * A.rows_pad + r] = m - kFaBias;
+          A.part_ml[(slot * 2 + 1) * A.rows_pad + r] = l;
+        }
+        tc::tc_fence_before();  // (O is read before the next piece's first weights say so)
+      }
+    }
+    if (tid == 0) A.meta[blockIdx.x] = split;
   }
-  if (tid < D) static_cast<T*>(a.out)[row * D + tid] = fa_from<T>(l == 0.f ? 0.f : o / l);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == FA_WARP_MMA) tc::tmem_dealloc(tmem, 256);
+  if (tid == 0) A.status[blockIdx.x] = *dead;
 }
 
 constexpr int FM_NT = 256;
@@ -96,7 +631,7 @@ constexpr int FM_AHEAD = 4;  // partials on their way at once
 // w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs. Bound by the
 // latency of its loads, from L2.
 template <typename T, int D>
-__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ fa::Args A) {
+__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A) {
   const int lane = threadIdx.x & 31, row = blockIdx.y * (FM_NT / 32) + (threadIdx.x >> 5);
   // every CTA waits for the kernel before this one, with work or without: what comes after on the
   // stream takes this kernel's end for the end of both
@@ -121,7 +656,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
     if (lane < cnt) {
       const float* pm = ml + slot(i0 + lane) * 2 * A.rows_pad;
       const float m = __ldcg(pm);
-      w = __ldcg(pm + A.rows_pad) * (m == top ? 1.f : fa::ex2(m - top));
+      w = __ldcg(pm + A.rows_pad) * (m == top ? 1.f : ex2(m - top));
     }
     for (int i = 0; i < cnt; i += FM_AHEAD) {
       float4 x[FM_AHEAD];
@@ -139,12 +674,12 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (lane < D / 4)
-    *reinterpret_cast<uint2*>(static_cast<T*>(A.a.out) + fa::out_row(A, seg.x, seg.y, n0, row) * D + c) =
-        make_uint2(fa::Out<T>::pack(y.x * inv, y.y * inv), fa::Out<T>::pack(y.z * inv, y.w * inv));
+    *reinterpret_cast<uint2*>(static_cast<T*>(A.a.out) + out_row(A, seg.x, seg.y, n0, row) * D + c) =
+        make_uint2(Out<T>::pack(y.x * inv, y.y * inv), Out<T>::pack(y.z * inv, y.w * inv));
 }
 
 template <typename T, int D>
-int fm_launch(const fa::Args& A, int ctas, cudaStream_t st) {
+int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -159,6 +694,45 @@ int fm_launch(const fa::Args& A, int ctas, cudaStream_t st) {
   return check_launch("attention_fp8_merge");
 }
 
+Plan fa_plan(int rows, int D) {
+  return make_plan(FA_CTAS * num_sms_current_device(), std::min(FA_ROWS, (rows + 7) / 8 * 8), D);
+}
+
+template <typename T, int D>
+int fa_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
+  using L = FaSmem<D, std::is_same<T, __nv_bfloat16>::value ? 2 : 3>;
+  const int g = a.Hq / a.Hkv;
+  const Plan plan = fa_plan((int)std::min((int64_t)g * a.T, (int64_t)FA_ROWS), D);
+  const Args A = make_args(a, plan, FA_ROWS / g, kFaLead, ws);
+  CUtensorMap km, vm;
+  int rc = make_fp8_tensor_maps(&km, &vm, a.pool, std::min(a.pool.block, FA_TK));
+  if (rc) return rc;
+  auto kern = fp8_attn_kernel<T, D>;
+  static DeviceOnce done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!done.done(dev)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "cannot set attention_fp8 shared memory size %d", L::BYTES);
+    done.mark(dev);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = st;
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(FA_NT);
+  cfg.dynamicSmemBytes = L::BYTES;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 launch: %s", cudaGetErrorString(e));
+  rc = check_launch("attention_fp8");
+  if (rc || a.cap <= FA_TK) return rc;  // a cache of one tile: nothing is split
+  return launch_fp8_merge(A, dtype, plan.ctas, st);
+}
+
 }  // namespace
 
 int launch_fp8_merge(const fa::Args& A, int dtype, int ctas, cudaStream_t st) {
@@ -169,8 +743,8 @@ int launch_fp8_merge(const fa::Args& A, int dtype, int ctas, cudaStream_t st) {
 
 size_t attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
   (void)B, (void)cap;
-  const int rows = Hq / Hkv * T;
-  return rows <= kFp8DecodeRows ? fp8_decode_plan(rows, D).bytes : 0;
+  const int64_t rows = (int64_t)Hq / Hkv * T;
+  return rows <= kFp8DecodeRows ? fp8_decode_plan((int)rows, D).bytes : fa_plan((int)std::min(rows, (int64_t)FA_ROWS), D).bytes;
 }
 
 int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
@@ -180,18 +754,9 @@ int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st)
     return DROPKV_OK;
   }
   if ((int64_t)a.Hq / a.Hkv * a.T <= kFp8DecodeRows) return launch_fp8_decode(a, dtype, ws, st);
-  const unsigned rows = (unsigned)((int64_t)a.B * a.Hq * a.T);
-  if (dtype == DROPKV_DTYPE_BF16) {
-    if (a.D == 128)
-      attention_fp8_row_kernel<__nv_bfloat16, 128><<<rows, FA_NT, 0, st>>>(a);
-    else
-      attention_fp8_row_kernel<__nv_bfloat16, 64><<<rows, FA_NT, 0, st>>>(a);
-  } else if (a.D == 128) {
-    attention_fp8_row_kernel<__half, 128><<<rows, FA_NT, 0, st>>>(a);
-  } else {
-    attention_fp8_row_kernel<__half, 64><<<rows, FA_NT, 0, st>>>(a);
-  }
-  return check_launch("attention_fp8");
+  if (dtype == DROPKV_DTYPE_BF16)
+    return a.D == 128 ? fa_launch<__nv_bfloat16, 128>(a, dtype, ws, st) : fa_launch<__nv_bfloat16, 64>(a, dtype, ws, st);
+  return a.D == 128 ? fa_launch<__half, 128>(a, dtype, ws, st) : fa_launch<__half, 64>(a, dtype, ws, st);
 }
 
 }  // namespace dropkv

@@ -109,6 +109,7 @@ struct Sees {
 template <int TK>
 struct Piece {
   int b, h, rt, t0, t1, tiles, rows;
+  int parts;  // partials of a split segment that begins here, else 0
   Keys<TK> k;
 };
 
@@ -169,10 +170,8 @@ template <int TK>
 struct Walk {
   long long left, per;
   int pair, h, u;
-  int4 meta;  // of a split segment that begins here
   __device__ __forceinline__ void start(const Start& s) {
     left = s.w1 - s.w, per = s.per, pair = s.pair, h = s.h, u = s.u;
-    meta = make_int4(0, 0, 0, 0);
   }
   __device__ __forceinline__ bool next(const Args& A, Piece<TK>& p) {
     while (left > 0) {
@@ -196,8 +195,7 @@ struct Walk {
         u = u1;
       }
       if (p.t1 > p.t0) {
-        if (p.t0 == 0 && p.t1 < p.tiles)
-          meta = make_int4(p.b, p.h, p.rt, 1 + (int)((units - u1 + per - 1) / per));
+        p.parts = p.t0 == 0 && p.t1 < p.tiles ? 1 + (int)((units - u1 + per - 1) / per) : 0;
         return true;
       }
     }

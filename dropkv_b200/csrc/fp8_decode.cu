@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
   // ======================= the warps that compute =============================
   uint32_t slot = 0, turn = 0, held = 0;  // of the next load: its slot, how often that was filled; of the next tile: its scales
   bool ok = true;
+  int4 split = make_int4(0, 0, 0, 0);  // the split segment that begins in this CTA (its last piece)
   // what a lane reads of a tile: K's vectors of its two keys, V's of its four
   uint32_t k_at[KV], v_at[2];
 #pragma unroll
@@ -496,6 +497,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       if (lane == 0) tc::mbar_arrive(&empty[slot]);
       if (++slot == NS) slot = 0, ++turn;
     }
+    if (p.parts) split = make_int4(p.b, p.h, p.rt, p.parts);
     // ---- the warps' parts, joined --------------------------------------------------
 #pragma unroll
     for (int x = 0; x < HR; ++x) {
@@ -545,12 +547,10 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
     }
     fd_sync();
   }
+  if (tid == 0) A.meta[blockIdx.x] = split;
   }
   __syncthreads();
-  if (tid == 0) {
-    A.meta[blockIdx.x] = ww.walk.meta;
-    A.status[blockIdx.x] = *dead;
-  }
+  if (tid == 0) A.status[blockIdx.x] = *dead;
 }
 
 template <typename T, int D, bool R16>

@@ -180,4 +180,10 @@ def attention_fp8(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
         out.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
     if rc:
         _lib.check(rc, "dropkv_attention_fp8")
+    if _CHECK_STATUS and n_pages * max_blocks > 0 and not torch.cuda.is_current_stream_capturing():
+        n = torch.cuda.get_device_properties(dev).multi_processor_count * 2  # a word for each CTA comes first
+        st = int(ws[:4 * n].view(torch.int32).max().item())
+        if st != 0:
+            raise _lib.DropKVError(_lib.ERR_DEVICE, f"dropkv_attention_fp8: device status {st} "
+                                                    "(a bounded wait timed out)")
     return out
