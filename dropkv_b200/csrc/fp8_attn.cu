@@ -50,7 +50,8 @@ struct FaSmem {
   // of tile i - NS - 2, and V's before it for tile i - 1 - NS to be widened; so all are past the tile NS + 2 back.
   static constexpr int SCALES = NS + 2;
   static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: 0 for a missing page
-  static constexpr int WALKS = SC + SCALES * 2 * FA_HALVES * 4;  // WarpWalk [4], of the softmax warps
+  static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // int [SCALES]: 1 where all pages are there with one scale each
+  static constexpr int WALKS = (KIND + SCALES * 4 + 7) / 8 * 8;  // WarpWalk [4], of the softmax warps
   static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
   static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_SC = 4 * NS, B_S = B_SC + SCALES, B_P = B_S + 2,
                        B_W = B_P + 2, B_O = B_W + 2, B_Q = B_O + 2, B_END = B_Q + 1, BARRIERS = B_END + 1;
@@ -99,6 +100,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   extern __shared__ __align__(1024) uint8_t sm[];  // swizzled tiles start on multiples of 1024
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
   float* sc = reinterpret_cast<float*>(sm + L::SC);
+  int* kinds = reinterpret_cast<int*>(sm + L::KIND);
   Start* start = reinterpret_cast<Start*>(sm + L::START);
   uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
   volatile int* dead = reinterpret_cast<volatile int*>(misc + 1);
@@ -150,7 +152,9 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   const uint32_t tmem = *misc;  // S (and P) 2 x 64 columns, O 128
   // a wait that gives up marks the CTA dead: every role then ends without waiting
   auto wait = [&](uint64_t* bar, uint32_t count, int why) {  // for the count-th completion (from 0)
-    if (tc::mbar_try_wait(bar, count & 1)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)  // (the timer takes longer to read than most waits last)
+      if (tc::mbar_try_wait(bar, count & 1)) return true;
     const uint64_t t0 = tc::globaltimer_ns();
     while (!*dead) {
       if (tc::mbar_try_wait(bar, count & 1)) return true;
@@ -200,10 +204,13 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           if (turn) ok = __all_sync(0xffffffffu, wait(&bars[(kv ? L::B_VE : L::B_KE) + slot], turn - 1, 1 + kv));
           if (!ok) break;
           if (kv == 0) {
+            const float ks0 = __shfl_sync(0xffffffffu, ks, 0), vs0 = __shfl_sync(0xffffffffu, vs, 0);
+            const int kind = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks > 0.f && ks == ks0 && vs == vs0));
             if (lane < FA_HALVES) {
               float* s = sc + place * (2 * FA_HALVES) + lane;
               s[0] = ks;
               s[FA_HALVES] = vs;
+              if (lane == 0) kinds[place] = kind;
             }
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&bars[L::B_SC + place]);
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     // O of tile i: the first of a piece begins it
     auto product = [&](uint32_t i, bool first) {
       const uint32_t buf = i & 1;
-      ok = __all_sync(0xffffffffu, wait(&bars[L::B_P + buf], i >> 1, 3) && wait(&bars[L::B_W + buf], i >> 1, 4));
+      ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], i >> 1, 4) && wait(&bars[L::B_P + buf], i >> 1, 3));
       if (!ok) return;
       tc::tc_fence_after();
       if (tc::elect_one()) {
@@ -302,40 +309,46 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
                                          (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
         if (!ok) break;
         const float* vs = sc + place * (2 * FA_HALVES) + FA_HALVES;
-        const bool there = vs[r >> 3] > 0.f;
         const int j0 = p.k.first(t);
-        const bool masked = __any_sync(0xffffffffu, !(vs[lane & 7] > 0.f)) || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks);
+        const bool masked = (!kinds[place] && __any_sync(0xffffffffu, !(vs[lane & 7] > 0.f))) || j0 + TK > all_end ||
+                            (j0 < all_low && j0 + TK > a.sinks);
         const uint8_t* src = sm + L::V + slot * L::TILE;
         uint8_t* dst = sm + L::V16 + buf * (2 * L::TILE);
-        uint32_t nan = 0;
+        auto widen = [&](auto clean) {
+          const bool there = vs[r >> 3] > 0.f && j0 + r < p.k.keys;
+          uint32_t nan = 0;
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) {
-          uint4 x = *reinterpret_cast<const uint4*>(src + tc::swz_offset<D>(r, c * 8));
-          if (masked) {
-            // what a weight of 0 would not silence: rows past the keys are cleared, and NaN is taken out here and given to those
-            // who see it at the end
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          for (int c = 0; c < D / 16; ++c) {
+            uint4 x = *reinterpret_cast<const uint4*>(src + tc::swz_offset<D>(r, c * 8));
+            if (decltype(clean)::value) {
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t odd = __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              if (!there || j0 + r >= p.k.keys)
-                w[e] = 0;
-              else
-                nan |= odd, w[e] &= ~odd;
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t odd = __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                if (!there)
+                  w[e] = 0;
+                else
+                  nan |= odd, w[e] &= ~odd;
+              }
+              x = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            x = make_uint4(w[0], w[1], w[2], w[3]);
+            uint4 lo, hi;
+            widen4(x.x, lo.x, lo.y);
+            widen4(x.y, lo.z, lo.w);
+            widen4(x.z, hi.x, hi.y);
+            widen4(x.w, hi.z, hi.w);
+            uint8_t* slab = dst + (c / 4) * (TK * 128);
+            *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16)) = lo;
+            *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16 + 8)) = hi;
           }
-          uint4 lo, hi;
-          widen4(x.x, lo.x, lo.y);
-          widen4(x.y, lo.z, lo.w);
-          widen4(x.z, hi.x, hi.y);
-          widen4(x.w, hi.z, hi.w);
-          uint8_t* slab = dst + (c / 4) * (TK * 128);
-          *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16)) = lo;
-          *reinterpret_cast<uint4*>(slab + tc::sw128_offset(r, (c % 4) * 16 + 8)) = hi;
-        }
-        if (masked) {
-          const int some = __any_sync(0xffffffffu, nan != 0);
+          return nan;
+        };
+        if (!masked) {
+          widen(std::false_type());
+        } else {
+          // what a weight of 0 would not silence: rows past the keys are cleared, and NaN is taken out here and given to those
+          // who see it at the end
+          const int some = __any_sync(0xffffffffu, widen(std::true_type()) != 0);
           if (lane == 0) bad[2 * buf + warp - FA_WARP_V] = some;
         }
         tc::fence_proxy_async_smem();
@@ -362,48 +375,59 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     // A piece's queries: a thread's row in 8-bit parts (what a part leaves goes to the next), in units of a power of two.
     // The products that read the last piece's are done once S of its last tile is there.
     auto queries = [&]() {
-      T x[D];
       const bool own = r < p.rows;
-      if (own) {
-        const int node = p.k.n0 + r / A.g, head = p.h * A.g + r % A.g;
-        const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss;
-        if (A.q_vec) {
-#pragma unroll
-          for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4*>(x + e) = *reinterpret_cast<const uint4*>(src + e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < D; ++e) x[e] = src[e * a.q_sd];
-        }
+      const int node = own ? p.k.n0 + r / A.g : 0, head = own ? p.h * A.g + r % A.g : 0;
+      const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss;
+      if (own)
         sees.set(A, p.b, p.k.len, p.k.keys, node);
-      } else {
-#pragma unroll
-        for (int e = 0; e < D; ++e) x[e] = T(0.f);
+      else
         sees.none();
-      }
+      auto load = [&](int e, T* x) {  // 32 elements
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          if (!own)
+            *reinterpret_cast<uint4*>(x + i) = make_uint4(0u, 0u, 0u, 0u);
+          else if (A.q_vec)
+            *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(src + e + i);
+          else
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[i + k] = src[(e + i + k) * a.q_sd];
+        }
+      };
       float big = 0.f;
 #pragma unroll
-      for (int e = 0; e < D; ++e) {
-        const float f = to_f(x[e]);
-        big = fmaxf(big, isfinite(f) ? fabsf(f) : 0.f);
+      for (int e = 0; e < D; e += 32) {
+        __align__(16) T x[32];
+        load(e, x);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float f = to_f(x[i]);
+          big = fmaxf(big, isfinite(f) ? fabsf(f) : 0.f);
+        }
       }
       unit = query_unit(big);
       const float inv = 1.f / unit;
+#pragma unroll 1
+      for (int e = 0; e < D; e += 32) {
+        __align__(16) T x[32];
+        load(e, x);
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        float v[16];
+        for (int c = 0; c < 2; ++c) {
+          float v[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float f = to_f(x[16 * c + e]);
-          v[e] = isfinite(f) ? f * inv : __uint_as_float(0x7fffffffu);
-        }
+          for (int i = 0; i < 16; ++i) {
+            const float f = to_f(x[16 * c + i]);
+            v[i] = isfinite(f) ? f * inv : __uint_as_float(0x7fffffffu);
+          }
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          uint4 w;
-          w.x = split4(v, 1.f);
-          w.y = split4(v + 4, 1.f);
-          w.z = split4(v + 8, 1.f);
-          w.w = split4(v + 12, 1.f);
-          *reinterpret_cast<uint4*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(r, c * 8)) = w;
+          for (int part = 0; part < PARTS; ++part) {
+            uint4 w;
+            w.x = split4(v, 1.f);
+            w.y = split4(v + 4, 1.f);
+            w.z = split4(v + 8, 1.f);
+            w.w = split4(v + 12, 1.f);
+            *reinterpret_cast<uint4*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(r, (e / 16 + c) * 8)) = w;
+          }
         }
       }
       unit *= A.scale_log2;
@@ -419,61 +443,28 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
       int any_bad = 0, all_end, all_low;
       p.k.all(A, &all_end, &all_low);
+      // a tile's scales: looked at before the weights of the tile before it are waited for
+      const float* scales = sc;
+      int kind = 0;
+      auto look = [&]() {
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 11)) && ok;
+        scales = sc + place * (2 * FA_HALVES);
+        kind = kinds[place];
+        if (++place == L::SCALES) place = 0, ++round;
+      };
+      look();
       for (int t = p.t0; t < p.t1 && ok; ++t, ++j) {
         const uint32_t buf = j & 1, ts = tmem + lanes + buf * 64;
-        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 11));
-        if (!ok) break;
-        const float* scales = sc + place * (2 * FA_HALVES);
-        if (++place == L::SCALES) place = 0, ++round;
-        if (!live) {
-          ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&bars[L::B_P + buf]);
-          continue;
-        }
-        float c[FA_HALVES], f[FA_HALVES];
-        float least = INFINITY, vmax = 0.f;
-#pragma unroll
-        for (int y = 0; y < FA_HALVES; ++y) {
-          c[y] = scales[y];
-          f[y] = scales[FA_HALVES + y];
-          least = fminf(least, c[y]);
-          vmax = fmaxf(vmax, f[y]);
-        }
+        const float* now = scales;
+        const float ks = now[0], vs = now[FA_HALVES];
         const int j0 = p.k.first(t);
-        const bool masked = !(least > 0.f) || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks);
-        uint64_t see = ~0ull;
-        if (masked) {
-          see = sees.bits(A, p.b, p.k.len, j0, TK);
-#pragma unroll
-          for (int y = 0; y < FA_HALVES; ++y)
-            if (!(c[y] > 0.f)) see &= ~(0xffull << (8 * y));
-        }
-#pragma unroll
-        for (int y = 0; y < FA_HALVES; ++y) c[y] = fminf(c[y] * unit, 3e38f);
-        ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
-        if (!ok) break;
-        tc::tc_fence_after();
+        const bool first = t == p.t0, next = t + 1 < p.t1;
+        const bool plain = kind && j0 + TK <= all_end && (j0 >= all_low || j0 + TK <= a.sinks);
         float x[TK];
-        tc::tmem_ld64(ts, x);
-        float top = -INFINITY;
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < TK; ++e) x[e] = (see >> e) & 1 ? x[e] * c[e / 8] : -INFINITY;
-#pragma unroll
-          for (int y = 0; y < FA_HALVES; ++y) c[y] = 1.f;
-        }
-#pragma unroll
-        for (int y = 0; y < FA_HALVES; ++y) {
-          float mx = max3(x[8 * y], x[8 * y + 1], x[8 * y + 2]);
-          mx = max3(mx, x[8 * y + 3], x[8 * y + 4]);
-          mx = max3(mx, x[8 * y + 5], x[8 * y + 6]);
-          mx = fmaxf(mx, x[8 * y + 7]);
-          top = fmaxf(top, mx * c[y]);
-        }
-        const bool first = t == p.t0;
-        // the reference moves where some row's maximum has outgrown it, or a page's scale of V the others'
-        if (__any_sync(0xffffffffu, top > m + kFaSlack) || vmax > vref) {
+        uint64_t sum[2] = {0, 0};
+        // The reference moves where some row's maximum has outgrown it, or a page's scale of V the others'.
+        auto settle = [&](float top, float vmax) {
+          if (!__any_sync(0xffffffffu, top > m + kFaSlack) && vmax <= vref) return;
           const float mn = top > m + kFaSlack ? top : m;
           float alpha = mn == m ? 1.f : ex2(m - mn);
           m = mn;
@@ -483,57 +474,98 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             vref = vmax;
             vinv = 1.f / vmax;
           }
-          if (!first) {
-            ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + 1 - buf], (j - 1) >> 1, 13));
-            tc::tc_fence_after();
-            float o[16];
+          if (first) return;
+          ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + 1 - buf], (j - 1) >> 1, 13)) && ok;
+          tc::tc_fence_after();
+          float o[16];
 #pragma unroll 1
-            for (int e0 = 0; e0 < D; e0 += 16) {
-              tc::tmem_ld16(to + e0, o);
+          for (int e0 = 0; e0 < D; e0 += 16) {
+            tc::tmem_ld16(to + e0, o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              tc::tmem_st16(to + e0, o);
-              tc::tmem_st_wait();
-            }
-          }
-        }
-        const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
-        const uint64_t ref2 = pair_of(-ref, -ref);
-        uint64_t sum[2] = {0, 0};
-        uint32_t pk[TK / 2];
-        bool even = true;  // every page has the largest scale
-#pragma unroll
-        for (int y = 0; y < FA_HALVES; ++y) even = even && f[y] == vref;
-        auto weigh = [&](auto scaled) {
-#pragma unroll
-          for (int y = 0; y < FA_HALVES; ++y) {
-            const uint64_t c2 = pair_of(c[y], c[y]), f2 = pair_of(f[y] * vinv, f[y] * vinv);
-#pragma unroll
-            for (int e = 8 * y; e < 8 * y + 8; e += 2) {
-              float u, v;
-              unpair(fma2(pair_of(x[e], x[e + 1]), c2, ref2), u, v);
-              uint64_t w = pair_of(ex2(u), ex2(v));
-              sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
-              if (decltype(scaled)::value) w = mul2(w, f2);
-              unpair(w, u, v);
-              pk[e / 2] = pack_half(u, v);
-            }
+            for (int e = 0; e < 16; ++e) o[e] *= alpha;
+            tc::tmem_st16(to + e0, o);
+            tc::tmem_st_wait();
           }
         };
-        if (even)
-          weigh(std::false_type());
-        else
-          weigh(std::true_type());
-        tc::tmem_st16(ts, reinterpret_cast<const float*>(pk));
-        tc::tmem_st16(ts + 16, reinterpret_cast<const float*>(pk + 16));
-        float s0, s1, s2, s3;
-        unpair(sum[0], s0, s1);
-        unpair(sum[1], s2, s3);
-        l += (s0 + s1) + (s2 + s3);
-        if (masked) {
-          ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
-          any_bad |= bad[2 * buf] | bad[2 * buf + 1];
+        // (all lanes together from the vote to the stores: those are the whole warp's)
+        // 32 weights, of elements [32 h, 32 h + 32): into place, and into the sum before they are rounded
+        auto weigh = [&](int h, auto c_of, auto f_of, auto scaled) {
+          const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
+          const uint64_t ref2 = pair_of(-ref, -ref);
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float c = c_of(4 * h + e / 8);
+            float u, v;
+            unpair(fma2(pair_of(x[32 * h + e], x[32 * h + e + 1]), pair_of(c, c), ref2), u, v);
+            uint64_t w = pair_of(ex2(u), ex2(v));
+            sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
+            if (decltype(scaled)::value) {
+              const float f = f_of(4 * h + e / 8);
+              unpair(mul2(w, pair_of(f, f)), u, v);
+            } else {
+              unpair(w, u, v);
+            }
+            pk[e / 2] = pack_half(u, v);
+          }
+          tc::tmem_st16(ts + 16 * h, reinterpret_cast<const float*>(pk));
+        };
+        auto largest = [&](int at, int count) {  // of elements [at, at + count)
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < count; e += 2) mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], x[at + e], x[at + e + 1]);
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
+        if (!ok) break;
+        if (live) {
+          tc::tc_fence_after();
+          tc::tmem_ld64(ts, x);
+          if (plain && vs <= vref) {  // one scale, seen by all: what most tiles are
+            const float c = fminf(ks * unit, 3e38f);
+            settle(largest(0, TK) * c, vs);
+            auto c_of = [&](int) { return c; };
+            if (vs == vref) {
+              weigh(0, c_of, c_of, std::false_type());
+              weigh(1, c_of, c_of, std::false_type());
+            } else {
+              const float f = vs * vinv;
+              auto f_of = [&](int) { return f; };
+              weigh(0, c_of, f_of, std::true_type());
+              weigh(1, c_of, f_of, std::true_type());
+            }
+          } else {
+            float vmax = 0.f, top = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < FA_HALVES; ++y) vmax = fmaxf(vmax, now[FA_HALVES + y]);
+            uint64_t see = ~0ull;
+            if (!plain) see = sees.bits(A, p.b, p.k.len, j0, TK);
+#pragma unroll
+            for (int y = 0; y < FA_HALVES; ++y) {
+              const float c = fminf(now[y] * unit, 3e38f);
+              if (!(now[y] > 0.f)) see &= ~(0xffull << (8 * y));
+#pragma unroll
+              for (int e = 8 * y; e < 8 * y + 8; ++e) x[e] = (see >> e) & 1 ? x[e] * c : -INFINITY;
+              top = fmaxf(top, largest(8 * y, 8));
+            }
+            settle(top, vmax);
+            auto c_of = [&](int) { return 1.f; };
+            auto f_of = [&](int y) { return now[FA_HALVES + y] * vinv; };
+            weigh(0, c_of, f_of, std::true_type());
+            weigh(1, c_of, f_of, std::true_type());
+            const bool least = now[0] > 0.f && now[1] > 0.f && now[2] > 0.f && now[3] > 0.f && now[4] > 0.f && now[5] > 0.f &&
+                               now[6] > 0.f && now[7] > 0.f;
+            if (!least || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks)) {  // as the widening warps saw it
+              ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
+              any_bad |= bad[2 * buf] | bad[2 * buf + 1];
+            }
+          }
+          float s0, s1, s2, s3;
+          unpair(sum[0], s0, s1);
+          unpair(sum[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
         }
+        if (next) look();
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -586,6 +618,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
           float o[32];
+          __syncwarp();  // (rows part ways below; the load is the whole warp's)
           tc::tmem_ld32(to + 32 * w, o);
           if (nan[w]) {
 #pragma unroll
