@@ -37,6 +37,12 @@ constexpr uint64_t kFaWaitNs = 1000000000ull;
 // A row's reference moves once its maximum has grown by this much (base 2); weights are
 // 2^(s - m + bias), so that fp16 holds them from 2^-24 to 2^15.
 constexpr float kFaSlack = 8.f, kFaBias = 7.f;
+// Where a tile's weights are formed first: a row's sum of them above this moves its reference to the row's maximum
+// (64 weights of 2^7 then sum to 2^13 at most).
+constexpr float kFaMost = 32768.f;
+
+// A tile whose keys all tokens see, with no page missing; and one whose pages have one scale of K and one of V, besides
+constexpr int FA_WHOLE = 1, FA_PLAIN = 2;
 
 template <int D, int PARTS>
 struct FaSmem {
@@ -50,7 +56,7 @@ struct FaSmem {
   // of tile i - NS - 2, and V's before it for tile i - 1 - NS to be widened; so all are past the tile NS + 2 back.
   static constexpr int SCALES = NS + 2;
   static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: 0 for a missing page
-  static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // int [SCALES]: 1 where all pages are there with one scale each
+  static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // int [SCALES]: FA_WHOLE, FA_PLAIN
   static constexpr int WALKS = (KIND + SCALES * 4 + 7) / 8 * 8;  // WarpWalk [4], of the softmax warps
   static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
   static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_SC = 4 * NS, B_S = B_SC + SCALES, B_P = B_S + 2,
@@ -186,6 +192,8 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         return p.k.any(A, j, 8) ? table[j >> lb] : -1;
       };
       auto there = [&](int page) { return page >= 0 && page < a.pool.n_pages; };
+      int all_end, all_low;
+      p.k.all(A, &all_end, &all_low);
       int page = page_of(p.t0), page1 = page_of(p.t0 + 1);
       float ks = there(page) ? ksb[page * a.pool.ks_s0] : 0.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
       for (int t = p.t0; t < p.t1; ++t, ++n) {
@@ -205,7 +213,11 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           if (!ok) break;
           if (kv == 0) {
             const float ks0 = __shfl_sync(0xffffffffu, ks, 0), vs0 = __shfl_sync(0xffffffffu, vs, 0);
-            const int kind = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks > 0.f && ks == ks0 && vs == vs0));
+            const int j0 = p.k.first(t);
+            const bool there = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks > 0.f && vs > 0.f));
+            const bool one = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks == ks0 && vs == vs0));
+            const bool whole = there && j0 + TK <= all_end && (j0 >= all_low || j0 + TK <= a.sinks);
+            const int kind = whole ? (one ? FA_WHOLE | FA_PLAIN : FA_WHOLE) : 0;
             if (lane < FA_HALVES) {
               float* s = sc + place * (2 * FA_HALVES) + lane;
               s[0] = ks;
@@ -301,21 +313,17 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     uint32_t j = 0, slot = 0, turn = 0, place = 0, round = 0;
     bool ok = true;
     while (ok && walk.next(A, p)) {
-      int all_end, all_low;
-      p.k.all(A, &all_end, &all_low);
       for (int t = p.t0; t < p.t1; ++t, ++j) {
         const uint32_t buf = j & 1;
         ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 8) && wait(&bars[L::B_VF + slot], turn, 9) &&
                                          (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
         if (!ok) break;
         const float* vs = sc + place * (2 * FA_HALVES) + FA_HALVES;
-        const int j0 = p.k.first(t);
-        const bool masked = (!kinds[place] && __any_sync(0xffffffffu, !(vs[lane & 7] > 0.f))) || j0 + TK > all_end ||
-                            (j0 < all_low && j0 + TK > a.sinks);
+        const bool whole = kinds[place] & FA_WHOLE;
         const uint8_t* src = sm + L::V + slot * L::TILE;
         uint8_t* dst = sm + L::V16 + buf * (2 * L::TILE);
         auto widen = [&](auto clean) {
-          const bool there = vs[r >> 3] > 0.f && j0 + r < p.k.keys;
+          const bool there = vs[r >> 3] > 0.f && p.k.first(t) + r < p.k.keys;
           uint32_t nan = 0;
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           }
           return nan;
         };
-        if (!masked) {
+        if (whole) {
           widen(std::false_type());
         } else {
           // what a weight of 0 would not silence: rows past the keys are cleared, and NaN is taken out here and given to those
@@ -372,61 +380,62 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     bool ok = true;
     float unit = 0.f;  // of the row's queries, and of logits in base 2
     Sees sees;
-    // A piece's queries: a thread's row in 8-bit parts (what a part leaves goes to the next), in units of a power of two.
+    // A piece's queries in 8-bit parts (what a part leaves goes to the next), in units of a power of two for each row: D / 8 lanes a
+    // row, eight elements each; the unit goes to the row's thread.
     // The products that read the last piece's are done once S of its last tile is there.
     auto queries = [&]() {
-      const bool own = r < p.rows;
-      const int node = own ? p.k.n0 + r / A.g : 0, head = own ? p.h * A.g + r % A.g : 0;
-      const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss;
-      if (own)
-        sees.set(A, p.b, p.k.len, p.k.keys, node);
+      constexpr int LANES = D / 8, ROWS = 32 / LANES, TURNS = 32 / ROWS, AHEAD = 8;
+      const int c = lane % LANES, sub = lane / LANES;
+      if (r < p.rows)
+        sees.set(A, p.b, p.k.len, p.k.keys, p.k.n0 + r / A.g);
       else
         sees.none();
-      auto load = [&](int e, T* x) {  // 32 elements
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (!own)
-            *reinterpret_cast<uint4*>(x + i) = make_uint4(0u, 0u, 0u, 0u);
-          else if (A.q_vec)
-            *reinterpret_cast<uint4*>(x + i) = *reinterpret_cast<const uint4*>(src + e + i);
-          else
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[i + k] = src[(e + i + k) * a.q_sd];
-        }
-      };
-      float big = 0.f;
-#pragma unroll
-      for (int e = 0; e < D; e += 32) {
-        __align__(16) T x[32];
-        load(e, x);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float f = to_f(x[i]);
-          big = fmaxf(big, isfinite(f) ? fabsf(f) : 0.f);
-        }
-      }
-      unit = query_unit(big);
-      const float inv = 1.f / unit;
 #pragma unroll 1
-      for (int e = 0; e < D; e += 32) {
-        __align__(16) T x[32];
-        load(e, x);
+      for (int i0 = 0; i0 < TURNS; i0 += AHEAD) {
+        uint4 x[AHEAD];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float v[16];
+        for (int u = 0; u < AHEAD; ++u) {
+          const int row = warp * 32 + (i0 + u) * ROWS + sub;
+          x[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (row < p.rows) {
+            const int node = p.k.n0 + row / A.g, head = p.h * A.g + row % A.g;
+            const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss + 8 * c * a.q_sd;
+            if (A.q_vec) {
+              x[u] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+              x[u].x = s[0] | (uint32_t)s[a.q_sd] << 16;
+              x[u].y = s[2 * a.q_sd] | (uint32_t)s[3 * a.q_sd] << 16;
+              x[u].z = s[4 * a.q_sd] | (uint32_t)s[5 * a.q_sd] << 16;
+              x[u].w = s[6 * a.q_sd] | (uint32_t)s[7 * a.q_sd] << 16;
+            }
+          }
+        }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float f = to_f(x[16 * c + i]);
-            v[i] = isfinite(f) ? f * inv : __uint_as_float(0x7fffffffu);
+        for (int u = 0; u < AHEAD; ++u) {
+          const int row = (i0 + u) * ROWS + sub;  // of the warp's
+          const T* y = reinterpret_cast<const T*>(&x[u]);
+          float v[8], big = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = to_f(y[e]);
+            big = fmaxf(big, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
           }
 #pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const float one = query_unit(big), inv = 1.f / one;
+#pragma unroll
+          for (int s = 0; s < ROWS; ++s) {
+            const float theirs = __shfl_sync(0xffffffffu, one, s * LANES);
+            if (lane == (i0 + u) * ROWS + s) unit = theirs;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] * inv : __uint_as_float(0x7fffffffu);
+#pragma unroll
           for (int part = 0; part < PARTS; ++part) {
-            uint4 w;
-            w.x = split4(v, 1.f);
-            w.y = split4(v + 4, 1.f);
-            w.z = split4(v + 8, 1.f);
-            w.w = split4(v + 12, 1.f);
-            *reinterpret_cast<uint4*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(r, (e / 16 + c) * 8)) = w;
+            const uint32_t lo = split4(v, 1.f), hi = split4(v + 4, 1.f);
+            *reinterpret_cast<uint2*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(warp * 32 + row, (c / 2) * 8) + (c & 1) * 8) =
+                make_uint2(lo, hi);
           }
         }
       }
@@ -441,31 +450,30 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     while (more) {
       const bool live = warp * 32 < p.rows;  // some row of this warp exists
       float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
-      int any_bad = 0, all_end, all_low;
-      p.k.all(A, &all_end, &all_low);
+      int any_bad = 0;
       // a tile's scales: looked at before the weights of the tile before it are waited for
       const float* scales = sc;
       int kind = 0;
+      float ks = 0.f, vs = 0.f;  // the first page's
       auto look = [&]() {
         ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 11)) && ok;
         scales = sc + place * (2 * FA_HALVES);
         kind = kinds[place];
+        ks = scales[0];
+        vs = scales[FA_HALVES];
         if (++place == L::SCALES) place = 0, ++round;
       };
       look();
-      for (int t = p.t0; t < p.t1 && ok; ++t, ++j) {
+      const int t1 = p.t1;
+      for (int t = p.t0; t < t1 && ok; ++t, ++j) {
         const uint32_t buf = j & 1, ts = tmem + lanes + buf * 64;
-        const float* now = scales;
-        const float ks = now[0], vs = now[FA_HALVES];
-        const int j0 = p.k.first(t);
-        const bool first = t == p.t0, next = t + 1 < p.t1;
-        const bool plain = kind && j0 + TK <= all_end && (j0 >= all_low || j0 + TK <= a.sinks);
+        const bool first = t == p.t0;
         float x[TK];
-        uint64_t sum[2] = {0, 0};
+        uint64_t sum[2];
         // The reference moves where some row's maximum has outgrown it, or a page's scale of V the others'.
-        auto settle = [&](float top, float vmax) {
-          if (!__any_sync(0xffffffffu, top > m + kFaSlack) && vmax <= vref) return;
-          const float mn = top > m + kFaSlack ? top : m;
+        auto settle = [&](float top, float vmax, float slack) {
+          if (!__any_sync(0xffffffffu, top > m + slack) && vmax <= vref) return;
+          const float mn = top > m + slack ? top : m;
           float alpha = mn == m ? 1.f : ex2(m - mn);
           m = mn;
           l *= alpha;
@@ -493,6 +501,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
           const uint64_t ref2 = pair_of(-ref, -ref);
           uint32_t pk[16];
+          if (h == 0) sum[0] = sum[1] = 0;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float c = c_of(4 * h + e / 8);
@@ -521,51 +530,60 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         if (live) {
           tc::tc_fence_after();
           tc::tmem_ld64(ts, x);
-          if (plain && vs <= vref) {  // one scale, seen by all: what most tiles are
-            const float c = fminf(ks * unit, 3e38f);
-            settle(largest(0, TK) * c, vs);
+          auto total = [&]() {
+            float s0, s1, s2, s3;
+            unpair(sum[0], s0, s1);
+            unpair(sum[1], s2, s3);
+            return (s0 + s1) + (s2 + s3);
+          };
+          if ((kind & FA_PLAIN) && vs <= vref) {  // what most tiles are, but for a piece's first
+            // Weights against the standing reference, without a look at the maximum: a sum within fp16's range says that
+            // all of them are. (The maximum first: 64 logits' worth of instructions and of latency more a tile.)
+            const float c = fminf(ks * unit, 3e38f), f = vs * vinv;
             auto c_of = [&](int) { return c; };
-            if (vs == vref) {
-              weigh(0, c_of, c_of, std::false_type());
-              weigh(1, c_of, c_of, std::false_type());
-            } else {
-              const float f = vs * vinv;
-              auto f_of = [&](int) { return f; };
-              weigh(0, c_of, f_of, std::true_type());
-              weigh(1, c_of, f_of, std::true_type());
+            auto f_of = [&](int) { return f; };
+            auto both = [&]() {
+              if (f == 1.f) {
+                weigh(0, c_of, f_of, std::false_type());
+                weigh(1, c_of, f_of, std::false_type());
+              } else {
+                weigh(0, c_of, f_of, std::true_type());
+                weigh(1, c_of, f_of, std::true_type());
+              }
+            };
+            both();
+            if (__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) {
+              tc::tmem_st_wait();
+              settle(largest(0, TK) * c, vs, 0.f);
+              both();
             }
           } else {
             float vmax = 0.f, top = -INFINITY;
 #pragma unroll
-            for (int y = 0; y < FA_HALVES; ++y) vmax = fmaxf(vmax, now[FA_HALVES + y]);
+            for (int y = 0; y < FA_HALVES; ++y) vmax = fmaxf(vmax, scales[FA_HALVES + y]);
             uint64_t see = ~0ull;
-            if (!plain) see = sees.bits(A, p.b, p.k.len, j0, TK);
+            if (!(kind & FA_WHOLE)) see = sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
 #pragma unroll
             for (int y = 0; y < FA_HALVES; ++y) {
-              const float c = fminf(now[y] * unit, 3e38f);
-              if (!(now[y] > 0.f)) see &= ~(0xffull << (8 * y));
+              const float c = fminf(scales[y] * unit, 3e38f);
+              if (!(scales[y] > 0.f)) see &= ~(0xffull << (8 * y));
 #pragma unroll
               for (int e = 8 * y; e < 8 * y + 8; ++e) x[e] = (see >> e) & 1 ? x[e] * c : -INFINITY;
               top = fmaxf(top, largest(8 * y, 8));
             }
-            settle(top, vmax);
+            settle(top, vmax, kFaSlack);
             auto c_of = [&](int) { return 1.f; };
-            auto f_of = [&](int y) { return now[FA_HALVES + y] * vinv; };
+            auto f_of = [&](int y) { return scales[FA_HALVES + y] * vinv; };
             weigh(0, c_of, f_of, std::true_type());
             weigh(1, c_of, f_of, std::true_type());
-            const bool least = now[0] > 0.f && now[1] > 0.f && now[2] > 0.f && now[3] > 0.f && now[4] > 0.f && now[5] > 0.f &&
-                               now[6] > 0.f && now[7] > 0.f;
-            if (!least || j0 + TK > all_end || (j0 < all_low && j0 + TK > a.sinks)) {  // as the widening warps saw it
+            if (!(kind & FA_WHOLE)) {
               ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
               any_bad |= bad[2 * buf] | bad[2 * buf + 1];
             }
           }
-          float s0, s1, s2, s3;
-          unpair(sum[0], s0, s1);
-          unpair(sum[1], s2, s3);
-          l += (s0 + s1) + (s2 + s3);
+          l += total();
         }
-        if (next) look();
+        if (t + 1 < t1) look();
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -573,7 +591,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       }
       // ---- the piece's output; the next one's queries first ----------------------
       if (p.parts) split = make_int4(p.b, p.h, p.rt, p.parts);
-      const int b = p.b, h = p.h, n0 = p.k.n0, t0 = p.t0, t1 = p.t1;
+      const int b = p.b, h = p.h, n0 = p.k.n0, t0 = p.t0;
       const bool whole = t0 == 0 && t1 == p.tiles, own = r < p.rows && ok;
       const int64_t slot = slot_of(p);
       const Sees saw = sees;
