@@ -59,7 +59,7 @@ struct FaSmem {
   static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // int [SCALES]: FA_WHOLE, FA_PLAIN
   static constexpr int WALKS = (KIND + SCALES * 4 + 7) / 8 * 8;  // WarpWalk [4], of the softmax warps
   static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
-  static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_SC = 4 * NS, B_S = B_SC + SCALES, B_P = B_S + 2,
+  static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_S = 4 * NS, B_P = B_S + 2,
                        B_W = B_P + 2, B_O = B_W + 2, B_Q = B_O + 2, B_END = B_Q + 1, BARRIERS = B_END + 1;
   static constexpr int START = BARS + BARRIERS * 8;
   static constexpr int MISC = START + (int)sizeof(Start);  // tensor memory's address, `dead`, bad[2][2]
@@ -129,9 +129,8 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       tc::mbar_init(&bars[L::B_VF + i], 1);
       tc::mbar_init(&bars[L::B_VE + i], 2);
     }
-    for (int i = 0; i < L::SCALES; ++i) tc::mbar_init(&bars[L::B_SC + i], 1);
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bars[L::B_S + i], 1);
+      tc::mbar_init(&bars[L::B_S + i], 2);  // the products' end, and the thread that issued them
       tc::mbar_init(&bars[L::B_P + i], 4);
       tc::mbar_init(&bars[L::B_W + i], 2);
       tc::mbar_init(&bars[L::B_O + i], 1);
@@ -168,7 +167,8 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     }
     return false;
   };
-  // Tile j of the CTA (from 0, over all pieces): K and V in slot j % NS, scales in place j % SCALES, S, P and widened V
+  // Tile j of the CTA (from 0, over all pieces): K and V in slot j % NS, scales in place j % SCALES (written before
+  // K's load is announced), S, P and widened V
   // in buffer j % 2. What waits for what: K's load for the product that had the slot; S(j) for K and for O(j - 2), which has
   // read P in its buffer; P(j) for S(j); widened V(j) for V's load and O(j - 2); O(j) for P(j) and widened V(j).
   // A wait that is not taken for every tile (O's, where a reference moves; widened V's, in masked tiles) begins
@@ -224,8 +224,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
               s[FA_HALVES] = vs;
               if (lane == 0) kinds[place] = kind;
             }
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bars[L::B_SC + place]);
+            __syncwarp();  // (who sees K's or V's tile land sees the scales)
           }
           if (lane == 0) tc::mbar_arrive_expect_tx(full, L::TILE);
           __syncwarp();
@@ -291,6 +290,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
                          part > 0 || kk > 0);
           tc::mma_commit(&bars[L::B_S + buf]);
           tc::mma_commit(&bars[L::B_KE + slot]);
+          tc::mbar_arrive(&bars[L::B_S + buf]);  // (hands on the scales, which came with K)
         }
         __syncwarp();
         if (++slot == NS) slot = 0, ++turn;
@@ -310,13 +310,12 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     Walk<TK> walk;
     Piece<TK> p;
     walk.start(*start);
-    uint32_t j = 0, slot = 0, turn = 0, place = 0, round = 0;
+    uint32_t j = 0, slot = 0, turn = 0, place = 0;
     bool ok = true;
     while (ok && walk.next(A, p)) {
       for (int t = p.t0; t < p.t1; ++t, ++j) {
         const uint32_t buf = j & 1;
-        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 8) && wait(&bars[L::B_VF + slot], turn, 9) &&
-                                         (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
+        ok = __all_sync(0xffffffffu, wait(&bars[L::B_VF + slot], turn, 9) && (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
         if (!ok) break;
         const float* vs = sc + place * (2 * FA_HALVES) + FA_HALVES;
         const bool whole = kinds[place] & FA_WHOLE;
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         auto widen = [&](auto clean) {
           const bool there = vs[r >> 3] > 0.f && p.k.first(t) + r < p.k.keys;
           uint32_t nan = 0;
-#pragma unroll
+#pragma unroll(decltype(clean)::value ? 1 : D / 16)
           for (int c = 0; c < D / 16; ++c) {
             uint4 x = *reinterpret_cast<const uint4*>(src + tc::swz_offset<D>(r, c * 8));
             if (decltype(clean)::value) {
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           tc::mbar_arrive(&bars[L::B_VE + slot]);
         }
         if (++slot == NS) slot = 0, ++turn;
-        if (++place == L::SCALES) place = 0, ++round;
+        if (++place == L::SCALES) place = 0;
       }
     }
   } else {
@@ -376,7 +375,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     WarpWalk<TK>& ww = reinterpret_cast<WarpWalk<TK>*>(sm + L::WALKS)[warp];
     if (lane == 0) ww.walk.start(*start);
     const Piece<TK>& p = ww.piece;
-    uint32_t j = 0, place = 0, round = 0;
+    uint32_t j = 0, place = 0;
     bool ok = true;
     float unit = 0.f;  // of the row's queries, and of logits in base 2
     Sees sees;
@@ -384,59 +383,89 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     // row, eight elements each; the unit goes to the row's thread.
     // The products that read the last piece's are done once S of its last tile is there.
     auto queries = [&]() {
-      constexpr int LANES = D / 8, ROWS = 32 / LANES, TURNS = 32 / ROWS, AHEAD = 8;
+      constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+      constexpr int LANES = D / 8, ROWS = 32 / LANES, TURNS = 32 / ROWS;
       const int c = lane % LANES, sub = lane / LANES;
       if (r < p.rows)
-        sees.set(A, p.b, p.k.len, p.k.keys, p.k.n0 + r / A.g);
+        sees.set(A, p.b, p.k.len, p.k.keys, p.k.n0 + A.quot(r));
       else
         sees.none();
+      // The rows as they are, where two parts of them will be: chunk c of 16 bytes in place c of a row of the first, then the second
+      // part. (Loops that run once a piece stay rolled: their code is fetched as it runs, which takes longer than running it.)
+      const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh + p.k.n0 * a.q_ss + 8 * c * a.q_sd;
+      auto raw = [&](int row) { return sm + L::Q + (c / (D / 16)) * (FA_ROWS * D) + tc::swz_offset<D>(row, (c % (D / 16)) * 8); };
 #pragma unroll 1
-      for (int i0 = 0; i0 < TURNS; i0 += AHEAD) {
-        uint4 x[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const int row = warp * 32 + (i0 + u) * ROWS + sub;
-          x[u] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < TURNS; ++i) {
+        const int row = warp * 32 + i * ROWS + sub;
+        const int token = A.quot(row), head = row - token * A.g;
+        const T* src = qb + head * a.q_sh + token * a.q_ss;
+        if (row < p.rows && A.q_vec) {
+          tc::copy16(raw(row), src);
+        } else {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (row < p.rows) {
-            const int node = p.k.n0 + row / A.g, head = p.h * A.g + row % A.g;
-            const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss + 8 * c * a.q_sd;
-            if (A.q_vec) {
-              x[u] = *reinterpret_cast<const uint4*>(src);
-            } else {
-              const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-              x[u].x = s[0] | (uint32_t)s[a.q_sd] << 16;
-              x[u].y = s[2 * a.q_sd] | (uint32_t)s[3 * a.q_sd] << 16;
-              x[u].z = s[4 * a.q_sd] | (uint32_t)s[5 * a.q_sd] << 16;
-              x[u].w = s[6 * a.q_sd] | (uint32_t)s[7 * a.q_sd] << 16;
-            }
+            const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+            x.x = s[0] | (uint32_t)s[a.q_sd] << 16;
+            x.y = s[2 * a.q_sd] | (uint32_t)s[3 * a.q_sd] << 16;
+            x.z = s[4 * a.q_sd] | (uint32_t)s[5 * a.q_sd] << 16;
+            x.w = s[6 * a.q_sd] | (uint32_t)s[7 * a.q_sd] << 16;
           }
+          *reinterpret_cast<uint4*>(raw(row)) = x;
         }
+      }
+      tc::wait_copies();
+      __syncwarp();
+#pragma unroll 2
+      for (int i = 0; i < TURNS; ++i) {
+        const int row = i * ROWS + sub;  // of the warp's
+        const uint4 x = *reinterpret_cast<const uint4*>(raw(warp * 32 + row));
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        // the largest magnitude, as bits: two 16-bit values a word
+        uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const int row = (i0 + u) * ROWS + sub;  // of the warp's
-          const T* y = reinterpret_cast<const T*>(&x[u]);
-          float v[8], big = 0.f;
+        for (int o = LANES / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = max(top & 0xffffu, top >> 16);
+        const bool odd = top >= kInf;
+        float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] = to_f(y[e]);
-            big = fmaxf(big, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
+        for (int e = 0; e < 4; ++e) {
+          const T* y = reinterpret_cast<const T*>(&w[e]);
+          v[2 * e] = to_f(y[0]);
+          v[2 * e + 1] = to_f(y[1]);
+        }
+        float big = to_f(*reinterpret_cast<const T*>(&top));
+        if (__any_sync(0xffffffffu, odd)) {  // a row with what is no number: the largest of the others counts
+          float most = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = fmaxf(most, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          if (odd) big = most;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] : __uint_as_float(0x7fffffffu);
+        }
+        const float one = query_unit(big), inv = __uint_as_float((254u << 23) - __float_as_uint(one));
+#pragma unroll
+        for (int s = 0; s < ROWS; ++s) {
+          const float theirs = __shfl_sync(0xffffffffu, one, s * LANES);
+          if (lane == i * ROWS + s) unit = theirs;
+        }
+        // (parts in fp16, whose 11 bits hold what is left at every step)
+        __half2 z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = __floats2half2_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
+        __syncwarp();  // all of these rows are read
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          uint32_t q8[2] = {0u, 0u};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(z[e]), __NV_SATFINITE, __NV_E4M3);
+            q8[e / 2] |= two << (16 * (e & 1));
+            if (part + 1 < PARTS) z[e] = __hsub2(z[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3)));
           }
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          const float one = query_unit(big), inv = 1.f / one;
-#pragma unroll
-          for (int s = 0; s < ROWS; ++s) {
-            const float theirs = __shfl_sync(0xffffffffu, one, s * LANES);
-            if (lane == (i0 + u) * ROWS + s) unit = theirs;
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] * inv : __uint_as_float(0x7fffffffu);
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            const uint32_t lo = split4(v, 1.f), hi = split4(v + 4, 1.f);
-            *reinterpret_cast<uint2*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(warp * 32 + row, (c / 2) * 8) + (c & 1) * 8) =
-                make_uint2(lo, hi);
-          }
+          *reinterpret_cast<uint2*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(warp * 32 + row, (c / 2) * 8) + (c & 1) * 8) =
+              make_uint2(q8[0], q8[1]);
         }
       }
       unit *= A.scale_log2;
@@ -451,24 +480,13 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       const bool live = warp * 32 < p.rows;  // some row of this warp exists
       float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
       int any_bad = 0;
-      // a tile's scales: looked at before the weights of the tile before it are waited for
-      const float* scales = sc;
-      int kind = 0;
-      float ks = 0.f, vs = 0.f;  // the first page's
-      auto look = [&]() {
-        ok = __all_sync(0xffffffffu, wait(&bars[L::B_SC + place], round, 11)) && ok;
-        scales = sc + place * (2 * FA_HALVES);
-        kind = kinds[place];
-        ks = scales[0];
-        vs = scales[FA_HALVES];
-        if (++place == L::SCALES) place = 0, ++round;
-      };
-      look();
       const int t1 = p.t1;
       for (int t = p.t0; t < t1 && ok; ++t, ++j) {
         const uint32_t buf = j & 1, ts = tmem + lanes + buf * 64;
         const bool first = t == p.t0;
-        float x[TK];
+        const float* scales = sc + place * (2 * FA_HALVES);
+        const int* kind_at = kinds + place;
+        if (++place == L::SCALES) place = 0;
         uint64_t sum[2];
         // The reference moves where some row's maximum has outgrown it, or a page's scale of V the others'.
         auto settle = [&](float top, float vmax, float slack) {
@@ -496,40 +514,39 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           }
         };
         // (all lanes together from the vote to the stores: those are the whole warp's)
-        // 32 weights, of elements [32 h, 32 h + 32): into place, and into the sum before they are rounded
-        auto weigh = [&](int h, auto c_of, auto f_of, auto scaled) {
+        // weights of 64 logits of one scale: into place, and into the sum before they are rounded
+        auto weigh = [&](const float* x, float c, float f, auto scaled) {
           const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
-          const uint64_t ref2 = pair_of(-ref, -ref);
-          uint32_t pk[16];
-          if (h == 0) sum[0] = sum[1] = 0;
+          const uint64_t c2 = pair_of(c, c), f2 = pair_of(f, f), ref2 = pair_of(-ref, -ref);
+          sum[0] = sum[1] = 0;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float c = c_of(4 * h + e / 8);
-            float u, v;
-            unpair(fma2(pair_of(x[32 * h + e], x[32 * h + e + 1]), pair_of(c, c), ref2), u, v);
-            uint64_t w = pair_of(ex2(u), ex2(v));
-            sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
-            if (decltype(scaled)::value) {
-              const float f = f_of(4 * h + e / 8);
-              unpair(mul2(w, pair_of(f, f)), u, v);
-            } else {
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float u, v;
+              unpair(fma2(pair_of(x[32 * h + e], x[32 * h + e + 1]), c2, ref2), u, v);
+              uint64_t w = pair_of(ex2(u), ex2(v));
+              sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
+              if (decltype(scaled)::value) w = mul2(w, f2);
               unpair(w, u, v);
+              pk[e / 2] = pack_half(u, v);
             }
-            pk[e / 2] = pack_half(u, v);
+            tc::tmem_st16(ts + 16 * h, reinterpret_cast<const float*>(pk));
           }
-          tc::tmem_st16(ts + 16 * h, reinterpret_cast<const float*>(pk));
         };
-        auto largest = [&](int at, int count) {  // of elements [at, at + count)
+        auto largest = [&](const float* x) {
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < count; e += 2) mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], x[at + e], x[at + e + 1]);
+          for (int e = 0; e < TK; e += 2) mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], x[e], x[e + 1]);
           return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         };
         ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
         if (!ok) break;
         if (live) {
           tc::tc_fence_after();
-          tc::tmem_ld64(ts, x);
+          const int kind = *kind_at;
+          const float ks = scales[0], vs = scales[FA_HALVES];  // the first page's
           auto total = [&]() {
             float s0, s1, s2, s3;
             unpair(sum[0], s0, s1);
@@ -540,42 +557,55 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             // Weights against the standing reference, without a look at the maximum: a sum within fp16's range says that
             // all of them are. (The maximum first: 64 logits' worth of instructions and of latency more a tile.)
             const float c = fminf(ks * unit, 3e38f), f = vs * vinv;
-            auto c_of = [&](int) { return c; };
-            auto f_of = [&](int) { return f; };
-            auto both = [&]() {
-              if (f == 1.f) {
-                weigh(0, c_of, f_of, std::false_type());
-                weigh(1, c_of, f_of, std::false_type());
-              } else {
-                weigh(0, c_of, f_of, std::true_type());
-                weigh(1, c_of, f_of, std::true_type());
-              }
-            };
-            both();
-            if (__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) {
+            float x[TK];
+            tc::tmem_ld64(ts, x);
+#pragma unroll 1
+            for (bool again = false;;) {
+              if (f == 1.f)
+                weigh(x, c, f, std::false_type());
+              else
+                weigh(x, c, f, std::true_type());
+              if (again || !__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) break;
               tc::tmem_st_wait();
-              settle(largest(0, TK) * c, vs, 0.f);
-              both();
+              settle(largest(x) * c, vs, 0.f);
+              again = true;
             }
           } else {
+            // eight keys at a time, S read twice (rolled, as this is what few tiles are)
+            uint64_t see = kind & FA_WHOLE ? ~0ull : sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
+            __syncwarp();
             float vmax = 0.f, top = -INFINITY;
+            auto eight = [&](int y, float* z) {  // logits
+              tc::tmem_ld8(ts + 8 * y, z);
+              const float s = scales[y], c = fminf(s * unit, 3e38f);
+              const uint32_t bits = s > 0.f ? (uint32_t)(see >> (8 * y)) : 0u;
 #pragma unroll
-            for (int y = 0; y < FA_HALVES; ++y) vmax = fmaxf(vmax, scales[FA_HALVES + y]);
-            uint64_t see = ~0ull;
-            if (!(kind & FA_WHOLE)) see = sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
-#pragma unroll
+              for (int e = 0; e < 8; ++e) z[e] = (bits >> e) & 1 ? z[e] * c : -INFINITY;
+            };
+#pragma unroll 1
             for (int y = 0; y < FA_HALVES; ++y) {
-              const float c = fminf(scales[y] * unit, 3e38f);
-              if (!(scales[y] > 0.f)) see &= ~(0xffull << (8 * y));
-#pragma unroll
-              for (int e = 8 * y; e < 8 * y + 8; ++e) x[e] = (see >> e) & 1 ? x[e] * c : -INFINITY;
-              top = fmaxf(top, largest(8 * y, 8));
+              float z[8];
+              eight(y, z);
+              vmax = fmaxf(vmax, scales[FA_HALVES + y]);
+              top = fmaxf(top, max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])));
             }
             settle(top, vmax, kFaSlack);
-            auto c_of = [&](int) { return 1.f; };
-            auto f_of = [&](int y) { return scales[FA_HALVES + y] * vinv; };
-            weigh(0, c_of, f_of, std::true_type());
-            weigh(1, c_of, f_of, std::true_type());
+            const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
+            sum[0] = sum[1] = 0;
+#pragma unroll 1
+            for (int y = 0; y < FA_HALVES; ++y) {
+              float z[8];
+              eight(y, z);
+              const float f = scales[FA_HALVES + y] * vinv;
+              uint32_t pk[4];
+#pragma unroll
+              for (int e = 0; e < 8; e += 2) {
+                const float u = ex2(z[e] - ref), v = ex2(z[e + 1] - ref);
+                sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pair_of(u, v));
+                pk[e / 2] = pack_half(u * f, v * f);
+              }
+              tc::tmem_st4(ts + 4 * y, pk);  // (S of these columns has been read)
+            }
             if (!(kind & FA_WHOLE)) {
               ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
               any_bad |= bad[2 * buf] | bad[2 * buf + 1];
@@ -583,7 +613,6 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           }
           l += total();
         }
-        if (t + 1 < t1) look();
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -633,12 +662,12 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         }
         T* dst = static_cast<T*>(a.out) + out_row(A, b, h, n0, own ? r : 0) * D;
         float* part = A.part_o + (slot * A.rows_pad + r) * D;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < D / 32; ++w) {
           float o[32];
           __syncwarp();  // (rows part ways below; the load is the whole warp's)
           tc::tmem_ld32(to + 32 * w, o);
-          if (nan[w]) {
+          if (any_bad && nan[w]) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if ((nan[w] >> e) & 1) o[e] = __uint_as_float(0x7fffffffu);
@@ -675,45 +704,69 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
 }
 
 constexpr int FM_NT = 256;
-constexpr int FM_AHEAD = 4;  // partials on their way at once
+constexpr int FM_AHEAD = 8;  // partials on their way at once
 
-// Joins the partials of the segments that fell into several CTAs. Grid: (CTAs before it, groups of
+// Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, groups of
 // eight rows); a warp has a row, a lane four of its columns. With M the largest of the partials' maxima and
 // w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs. Bound by the
 // latency of its loads, from L2.
 template <typename T, int D>
-__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A) {
-  const int lane = threadIdx.x & 31, row = blockIdx.y * (FM_NT / 32) + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A, int ctas) {
+  __shared__ int counts[FM_NT / 32], pick;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * (FM_NT / 32) + warp;
+  if (threadIdx.x == 0) pick = -1;
   // every CTA waits for the kernel before this one, with work or without: what comes after on the
   // stream takes this kernel's end for the end of both
   pdl_wait();
-  const int4 seg = A.meta[blockIdx.x];
-  const int n = seg.w;
-  const int n0 = seg.z * A.npr, rows = (min(n0 + A.npr, A.a.T) - n0) * A.g;
-  if (n == 0 || row >= rows) return;
-  auto slot = [&](int i) { return 2 * ((int64_t)blockIdx.x + i) + (i == 0 ? 1 : 0); };
+  // the CTA in which the blockIdx.x-th split segment begins
+  for (int c0 = 0, before = 0; c0 < ctas; c0 += FM_NT) {
+    const int at = c0 + threadIdx.x;
+    const bool splits = at < ctas && A.meta[at].w > 0;
+    const unsigned some = __ballot_sync(0xffffffffu, splits);
+    if (lane == 0) counts[warp] = __popc(some);
+    __syncthreads();
+    for (int w = 0; w < FM_NT / 32; ++w) {
+      if (w == warp && splits && before + __popc(some & ((1u << lane) - 1)) == (int)blockIdx.x) pick = at;
+      before += counts[w];
+    }
+    __syncthreads();
+  }
+  if (pick < 0) return;
+  const int4 seg = A.meta[pick];
+  const int n = seg.w, n0 = seg.z * A.npr, rows = (min(n0 + A.npr, A.a.T) - n0) * A.g;
+  if (row >= rows) return;
+  auto slot = [&](int i) { return 2 * ((int64_t)pick + i) + (i == 0 ? 1 : 0); };
   const float* ml = A.part_ml + row;
   const int c = 4 * (lane % (D / 4));
   const float* po = A.part_o + (int64_t)row * D + c;
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(ml + slot(i) * 2 * A.rows_pad));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float sum = 0.f;
+  float sum = 0.f, top = -INFINITY;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int cnt = min(32, n - i0);
-    float w = 0.f;
-    if (lane < cnt) {
-      const float* pm = ml + slot(i0 + lane) * 2 * A.rows_pad;
-      const float m = __ldcg(pm);
-      w = __ldcg(pm + A.rows_pad) * (m == top ? 1.f : ex2(m - top));
-    }
-    for (int i = 0; i < cnt; i += FM_AHEAD) {
-      float4 x[FM_AHEAD];
+    float4 x[FM_AHEAD];
+    auto load = [&](int i, float4* to) {
 #pragma unroll
       for (int u = 0; u < FM_AHEAD; ++u)
-        x[u] = __ldcg(reinterpret_cast<const float4*>(po + slot(i0 + min(i + u, cnt - 1)) * A.rows_pad * D));
+        to[u] = __ldcg(reinterpret_cast<const float4*>(po + slot(i0 + min(i + u, cnt - 1)) * A.rows_pad * D));
+    };
+    load(0, x);  // (beside the maxima and sums)
+    float m = -INFINITY, w = 0.f;
+    if (lane < cnt) {
+      const float* pm = ml + slot(i0 + lane) * 2 * A.rows_pad;
+      m = __ldcg(pm);
+      w = __ldcg(pm + A.rows_pad);
+    }
+    float mx = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, top);
+    const float f0 = top == mx ? 1.f : ex2(top - mx);  // of what was joined before
+    top = mx;
+    w *= m == top ? 1.f : ex2(m - top);
+    sum *= f0;
+    y.x *= f0, y.y *= f0, y.z *= f0, y.w *= f0;
+    for (int i = 0; i < cnt; i += FM_AHEAD) {
+      if (i) load(i, x);
 #pragma unroll
       for (int u = 0; u < FM_AHEAD; ++u) {
         const float f = __shfl_sync(0xffffffffu, w, min(i + u, 31));
@@ -731,6 +784,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
 
 template <typename T, int D>
 int fm_launch(const Args& A, int ctas, cudaStream_t st) {
+  const int64_t segments = (int64_t)A.a.B * A.RT * A.a.Hkv;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -738,9 +792,9 @@ int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3(ctas, (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(ctas, segments), (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
   cfg.blockDim = dim3(FM_NT);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_merge_kernel<T, D>, A);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_merge_kernel<T, D>, A, ctas);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 merge launch: %s", cudaGetErrorString(e));
   return check_launch("attention_fp8_merge");
 }

@@ -21,14 +21,18 @@ namespace fa {
 struct Args {
   AttnFp8 a;
   int g, npr, RT;    // heads of a group, tokens of a row tile, row tiles of a sequence
+  int g_mul;         // ceil(2^16 / g)
   int lead;          // units before a segment's tiles: about what a further segment costs a CTA, in tiles
   int rows_pad;      // rows of a partial
+  int mask_vec;      // the mask's rows are read 4 bytes at a time
   int q_vec;         // Q's rows are read 16 bytes at a time
   float scale_log2;
   int* status;       // [CTAs]: 0, or which wait gave up
   int4* meta;        // [CTAs]: the split segment that begins in a CTA: b, KV head, row tile, its partials (0: none)
   float* part_o;     // [2 CTAs][rows_pad][D]
   float* part_ml;    // [2 CTAs][2][rows_pad]
+  // r / g for a row r of a tile: r (g_mul g - 2^16) < 2^7 2^7 < 2^16
+  __device__ __forceinline__ int quot(int r) const { return (r * g_mul) >> 16; }
 };
 
 // Keys of a row tile of sequence b.
@@ -95,11 +99,37 @@ struct Sees {
     if (!a.mask || !m) return m & near;
     const uint64_t cached = below(len - j0);
     const uint8_t* row = a.mask + b * a.mask_sb + node * a.mask_sr;
-    uint64_t nodes = 0, todo = m & ~cached;
-    while (todo) {
-      const int e = __ffsll((long long)todo) - 1;
-      todo &= todo - 1;
-      if (row[(int64_t)(j0 + e - len) * a.mask_sc]) nodes |= 1ull << e;
+    uint64_t nodes = 0;
+    const int n0 = j0 - len;  // the node of bit 0
+    if (m & ~cached) {
+      // (many loads on their way at once: a truth value at a time takes as many trips to memory)
+      if (A.mask_vec) {
+#pragma unroll 1
+        for (int i0 = 0; i0 <= count / 4; i0 += 8) {
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int n = (n0 & ~3) + 4 * (i0 + i);
+            x[i] = n >= 0 && n < a.T ? *reinterpret_cast<const uint32_t*>(row + n) : 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // four truth values to four bits
+            const int at = 4 * (i0 + i) - (n0 & 3);
+            const uint64_t four = ((__vcmpne4(x[i], 0u) & 0x01010101u) * 0x10204080u) >> 28;
+            nodes |= at < 0 ? four >> -at : (at < 64 ? four << at : 0ull);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int e0 = 0; e0 < count; e0 += 8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int n = n0 + e0 + e;
+            if (n >= 0 && n < a.T && row[(int64_t)n * a.mask_sc]) nodes |= 1ull << (e0 + e);
+          }
+        }
+      }
+      nodes &= m & ~cached;
     }
     return (m & cached & near) | nodes;
   }
@@ -227,8 +257,8 @@ __device__ __forceinline__ int64_t slot_of(const Piece<TK>& p) {
 
 // Row r of a row tile in the output [B, Hq, T, D].
 __device__ __forceinline__ int64_t out_row(const Args& A, int b, int h, int n0, int r) {
-  const int node = n0 + r / A.g, head = h * A.g + r % A.g;
-  return ((int64_t)b * A.a.Hq + head) * A.a.T + node;
+  const int token = A.quot(r), head = h * A.g + r - token * A.g;
+  return ((int64_t)b * A.a.Hq + head) * A.a.T + n0 + token;
 }
 
 __device__ __forceinline__ float ex2(float x) {  // 2^x, hardware approximation; 2^-inf = 0
@@ -302,11 +332,14 @@ inline Args make_args(const AttnFp8& a, const Plan& p, int npr, int lead, void* 
   Args A;
   A.a = a;
   A.g = a.Hq / a.Hkv;
+  A.g_mul = (65536 + A.g - 1) / A.g;
   A.npr = npr;
   A.RT = (a.T + npr - 1) / npr;
   A.lead = lead;
   A.rows_pad = p.rows_pad;
   A.q_vec = a.q_sd == 1 && (reinterpret_cast<uintptr_t>(a.q) | (uint64_t)((a.q_sb | a.q_sh | a.q_ss) * 2)) % 16 == 0;
+  A.mask_vec = a.mask && a.mask_sc == 1 && a.T % 4 == 0 &&
+               (reinterpret_cast<uintptr_t>(a.mask) | (uint64_t)(a.mask_sb | a.mask_sr)) % 4 == 0;
   A.scale_log2 = a.scale * 1.4426950408889634f;
   uint8_t* w = static_cast<uint8_t*>(ws);
   A.status = reinterpret_cast<int*>(w);

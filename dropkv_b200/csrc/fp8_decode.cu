@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       float v[KV * 16];
       float big = 0.f;
       if (r < p.rows) {
-        const int node = p.k.n0 + r / A.g, head = p.h * A.g + r % A.g;
+        const int token = A.quot(r), node = p.k.n0 + token, head = p.h * A.g + r - token * A.g;
         const T* src = static_cast<const T*>(a.q) + p.b * a.q_sb + head * a.q_sh + node * a.q_ss;
         sees[x].set(A, p.b, p.k.len, p.k.keys, node);
 #pragma unroll
