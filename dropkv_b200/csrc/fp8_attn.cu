@@ -43,6 +43,10 @@ constexpr float kFaMost = 32768.f;
 
 // A tile whose keys all tokens see, with no page missing; and one whose pages have one scale of K and one of V, besides
 constexpr int FA_WHOLE = 1, FA_PLAIN = 2;
+struct FaKind {
+  int kind;
+  float vmax;  // the largest scale of V
+};
 
 template <int D, int PARTS>
 struct FaSmem {
@@ -56,8 +60,8 @@ struct FaSmem {
   // of tile i - NS - 2, and V's before it for tile i - 1 - NS to be widened; so all are past the tile NS + 2 back.
   static constexpr int SCALES = NS + 2;
   static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: 0 for a missing page
-  static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // int [SCALES]: FA_WHOLE, FA_PLAIN
-  static constexpr int WALKS = (KIND + SCALES * 4 + 7) / 8 * 8;  // WarpWalk [4], of the softmax warps
+  static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // {int, float} [SCALES]: FA_WHOLE, FA_PLAIN; the largest of V's
+  static constexpr int WALKS = KIND + SCALES * 8;  // WarpWalk [4], of the softmax warps
   static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
   static constexpr int B_KF = 0, B_KE = NS, B_VF = 2 * NS, B_VE = 3 * NS, B_S = 4 * NS, B_P = B_S + 2,
                        B_W = B_P + 2, B_O = B_W + 2, B_Q = B_O + 2, B_END = B_Q + 1, BARRIERS = B_END + 1;
@@ -96,6 +100,90 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// The queries of all row tiles in 8-bit parts, laid out as the products read them, and their units. Grid: (row tiles of a
+// sequence, KV heads, sequences); D / 8 lanes have a row, eight elements each. A row's unit is the power of two that
+// brings its largest element to at most 448; the first part is an element's nearest 8 bits, the next what that leaves.
+// In a kernel of its own because a row tile's rows are a long chain for its four softmax warps (3.5 us of a piece's 7 before
+// its first product) and a short one for a whole GPU; bound by the chain load, largest element, parts.
+constexpr int FQ_NT = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(FQ_NT) fp8_queries_kernel(const __grid_constant__ Args A) {
+  constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
+  constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  constexpr int LANES = D / 8, PER = FQ_NT / LANES, TURNS = FA_ROWS / PER;
+  const AttnFp8& a = A.a;
+  const int rt = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int c = threadIdx.x % LANES, n0 = rt * A.npr, rows = (min(n0 + A.npr, a.T) - n0) * A.g;
+  const int64_t tile = row_tile(A, b, h, rt);
+  uint8_t* out = A.queries + tile * (PARTS * FA_ROWS * D);
+  pdl_wait();
+  pdl_launch_dependents();
+  uint4 x[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int row = threadIdx.x / LANES + i * PER, token = A.quot(row), head = h * A.g + row - token * A.g;
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) {
+      const T* src = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + (n0 + token) * a.q_ss + 8 * c * a.q_sd;
+      if (A.q_vec) {
+        x[i] = *reinterpret_cast<const uint4*>(src);
+      } else {
+        const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
+        x[i].x = s[0] | (uint32_t)s[a.q_sd] << 16;
+        x[i].y = s[2 * a.q_sd] | (uint32_t)s[3 * a.q_sd] << 16;
+        x[i].z = s[4 * a.q_sd] | (uint32_t)s[5 * a.q_sd] << 16;
+        x[i].w = s[6 * a.q_sd] | (uint32_t)s[7 * a.q_sd] << 16;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int row = threadIdx.x / LANES + i * PER;
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    // the largest magnitude, as bits: two 16-bit values a word
+    uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = max(top & 0xffffu, top >> 16);
+    const bool odd = top >= kInf;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const T* y = reinterpret_cast<const T*>(&w[e]);
+      v[2 * e] = to_f(y[0]);
+      v[2 * e + 1] = to_f(y[1]);
+    }
+    float big = to_f(*reinterpret_cast<const T*>(&top));
+    if (__any_sync(0xffffffffu, odd)) {  // a row with what is no number: the largest of the others counts
+      float most = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (odd) big = most;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] : __uint_as_float(0x7fffffffu);
+    }
+    const float one = query_unit(big), inv = __uint_as_float((254u << 23) - __float_as_uint(one));
+    if (c == 0) A.units[tile * FA_ROWS + row] = one * A.scale_log2;
+    __half2 z[4];  // (parts in fp16, whose 11 bits hold what is left at every step)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = __floats2half2_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      uint32_t q8[2] = {0u, 0u};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(z[e]), __NV_SATFINITE, __NV_E4M3);
+        q8[e / 2] |= two << (16 * (e & 1));
+        if (part + 1 < PARTS) z[e] = __hsub2(z[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3)));
+      }
+      *reinterpret_cast<uint2*>(out + part * (FA_ROWS * D) + tc::swz_offset<D>(row, (c / 2) * 8) + (c & 1) * 8) = make_uint2(q8[0], q8[1]);
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     fp8_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -106,7 +194,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   extern __shared__ __align__(1024) uint8_t sm[];  // swizzled tiles start on multiples of 1024
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
   float* sc = reinterpret_cast<float*>(sm + L::SC);
-  int* kinds = reinterpret_cast<int*>(sm + L::KIND);
+  FaKind* kinds = reinterpret_cast<FaKind*>(sm + L::KIND);
   Start* start = reinterpret_cast<Start*>(sm + L::START);
   uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::MISC);
   volatile int* dead = reinterpret_cast<volatile int*>(misc + 1);
@@ -135,7 +223,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       tc::mbar_init(&bars[L::B_W + i], 2);
       tc::mbar_init(&bars[L::B_O + i], 1);
     }
-    tc::mbar_init(&bars[L::B_Q], 4);
+    tc::mbar_init(&bars[L::B_Q], 1);
     tc::mbar_init(&bars[L::B_END], 1);
     tc::fence_mbar_init();
     *dead = 0;
@@ -173,15 +261,29 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   // read P in its buffer; P(j) for S(j); widened V(j) for V's load and O(j - 2); O(j) for P(j) and widened V(j).
   // A wait that is not taken for every tile (O's, where a reference moves; widened V's, in masked tiles) begins
   // with the phase before over, which S(j) says, and ends before the next, which needs P(j).
+  // The softmax warps hold a tile's logits and need more registers than the others: (168 + 88) x 128 threads are what the
+  // block was launched with, 256 x 128.
+  if (warp >= FA_WARP_V) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == FA_WARP_TMA) {
     // ======================= TMA producer =======================================
     const int block = a.pool.block, lb = __ffs(block) - 1, box = min(block, TK), boxes = TK / box;
     Walk<TK> walk;
     Piece<TK> p;
     walk.start(*start);
-    uint32_t n = 0, slot = 0, turn = 0, place = 0;
+    uint32_t n = 0, slot = 0, turn = 0, place = 0, queries = 0;
     bool ok = true;
     while (ok && walk.next(A, p)) {
+      // the piece's queries, once the products that read the last piece's are done: those with its last tile of K
+      if (n) ok = __all_sync(0xffffffffu, wait(&bars[L::B_KE + (n - 1) % NS], (n - 1) / NS, 8));
+      if (!ok) break;
+      if (lane == 0) {
+        constexpr uint32_t BYTES = PARTS * FA_ROWS * D;
+        tc::mbar_arrive_expect_tx(&bars[L::B_Q], BYTES);
+        tc::bulk_load(sm + L::Q, A.queries + row_tile(A, p.b, p.h, p.rt) * BYTES, BYTES, &bars[L::B_Q]);
+      }
+      __syncwarp();
+      ++queries;
       const int32_t* table = a.table + (int64_t)p.b * a.max_blocks;
       const float* ksb = a.pool.k_scale + p.h * a.pool.ks_sh;
       const float* vsb = a.pool.v_scale + p.h * a.pool.vs_sh;
@@ -218,11 +320,14 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             const bool one = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks == ks0 && vs == vs0));
             const bool whole = there && j0 + TK <= all_end && (j0 >= all_low || j0 + TK <= a.sinks);
             const int kind = whole ? (one ? FA_WHOLE | FA_PLAIN : FA_WHOLE) : 0;
+            float vmax = vs;
+#pragma unroll
+            for (int o = FA_HALVES / 2; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
             if (lane < FA_HALVES) {
               float* s = sc + place * (2 * FA_HALVES) + lane;
               s[0] = ks;
               s[FA_HALVES] = vs;
-              if (lane == 0) kinds[place] = kind;
+              if (lane == 0) kinds[place] = FaKind{kind, vmax};
             }
             __syncwarp();  // (who sees K's or V's tile land sees the scales)
           }
@@ -239,6 +344,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       }
     }
     if (*dead) {  // every issued copy lands before the CTA may exit (of the tile that gave up, K may be one)
+      if (queries) tc::mbar_wait(&bars[L::B_Q], (queries - 1) & 1, kFaWaitNs / 8);
       for (uint32_t j = n > (uint32_t)NS ? n - NS : 0u; j <= n; ++j)
         for (int kv = 0; kv < 2; ++kv)
           if (j < n || kv == 0) tc::mbar_wait(&bars[(kv ? L::B_VF : L::B_KF) + j % NS], (j / NS) & 1, kFaWaitNs / 8);
@@ -303,7 +409,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       __syncwarp();
       tc::mbar_wait(&bars[L::B_END], 0, kFaWaitNs);
     }
-  } else if (warp >= FA_WARP_V) {
+  } else {
     // ======================= V to fp16 ==========================================
     // A thread has a key's row: 16-byte reads and writes of eight rows at a time meet all banks once.
     const int r = tid - FA_WARP_V * 32;
@@ -318,7 +424,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         ok = __all_sync(0xffffffffu, wait(&bars[L::B_VF + slot], turn, 9) && (j < 2 || wait(&bars[L::B_O + buf], (j - 2) >> 1, 10)));
         if (!ok) break;
         const float* vs = sc + place * (2 * FA_HALVES) + FA_HALVES;
-        const bool whole = kinds[place] & FA_WHOLE;
+        const bool whole = kinds[place].kind & FA_WHOLE;
         const uint8_t* src = sm + L::V + slot * L::TILE;
         uint8_t* dst = sm + L::V16 + buf * (2 * L::TILE);
         auto widen = [&](auto clean) {
@@ -368,8 +474,10 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         if (++place == L::SCALES) place = 0;
       }
     }
+  }
   } else {
     // ======================= softmax ============================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const uint32_t lanes = (uint32_t)(warp * 32) << 16, to = tmem + lanes + 128;
     const int r = tid;
     WarpWalk<TK>& ww = reinterpret_cast<WarpWalk<TK>*>(sm + L::WALKS)[warp];
@@ -377,105 +485,18 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     const Piece<TK>& p = ww.piece;
     uint32_t j = 0, place = 0;
     bool ok = true;
-    float unit = 0.f;  // of the row's queries, and of logits in base 2
+    float unit = 0.f;  // of the row's queries, for logits in base 2
     Sees sees;
-    // A piece's queries in 8-bit parts (what a part leaves goes to the next), in units of a power of two for each row: D / 8 lanes a
-    // row, eight elements each; the unit goes to the row's thread.
-    // The products that read the last piece's are done once S of its last tile is there.
-    auto queries = [&]() {
-      constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-      constexpr int LANES = D / 8, ROWS = 32 / LANES, TURNS = 32 / ROWS;
-      const int c = lane % LANES, sub = lane / LANES;
+    auto begin = [&]() {  // a piece
       if (r < p.rows)
         sees.set(A, p.b, p.k.len, p.k.keys, p.k.n0 + A.quot(r));
       else
         sees.none();
-      // The rows as they are, where two parts of them will be: chunk c of 16 bytes in place c of a row of the first, then the second
-      // part. (Loops that run once a piece stay rolled: their code is fetched as it runs, which takes longer than running it.)
-      const T* qb = static_cast<const T*>(a.q) + p.b * a.q_sb + (int64_t)p.h * A.g * a.q_sh + p.k.n0 * a.q_ss + 8 * c * a.q_sd;
-      auto raw = [&](int row) { return sm + L::Q + (c / (D / 16)) * (FA_ROWS * D) + tc::swz_offset<D>(row, (c % (D / 16)) * 8); };
-#pragma unroll 1
-      for (int i = 0; i < TURNS; ++i) {
-        const int row = warp * 32 + i * ROWS + sub;
-        const int token = A.quot(row), head = row - token * A.g;
-        const T* src = qb + head * a.q_sh + token * a.q_ss;
-        if (row < p.rows && A.q_vec) {
-          tc::copy16(raw(row), src);
-        } else {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (row < p.rows) {
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-            x.x = s[0] | (uint32_t)s[a.q_sd] << 16;
-            x.y = s[2 * a.q_sd] | (uint32_t)s[3 * a.q_sd] << 16;
-            x.z = s[4 * a.q_sd] | (uint32_t)s[5 * a.q_sd] << 16;
-            x.w = s[6 * a.q_sd] | (uint32_t)s[7 * a.q_sd] << 16;
-          }
-          *reinterpret_cast<uint4*>(raw(row)) = x;
-        }
-      }
-      tc::wait_copies();
-      __syncwarp();
-#pragma unroll 2
-      for (int i = 0; i < TURNS; ++i) {
-        const int row = i * ROWS + sub;  // of the warp's
-        const uint4 x = *reinterpret_cast<const uint4*>(raw(warp * 32 + row));
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        // the largest magnitude, as bits: two 16-bit values a word
-        uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = max(top & 0xffffu, top >> 16);
-        const bool odd = top >= kInf;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const T* y = reinterpret_cast<const T*>(&w[e]);
-          v[2 * e] = to_f(y[0]);
-          v[2 * e + 1] = to_f(y[1]);
-        }
-        float big = to_f(*reinterpret_cast<const T*>(&top));
-        if (__any_sync(0xffffffffu, odd)) {  // a row with what is no number: the largest of the others counts
-          float most = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, isfinite(v[e]) ? fabsf(v[e]) : 0.f);
-#pragma unroll
-          for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          if (odd) big = most;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] : __uint_as_float(0x7fffffffu);
-        }
-        const float one = query_unit(big), inv = __uint_as_float((254u << 23) - __float_as_uint(one));
-#pragma unroll
-        for (int s = 0; s < ROWS; ++s) {
-          const float theirs = __shfl_sync(0xffffffffu, one, s * LANES);
-          if (lane == i * ROWS + s) unit = theirs;
-        }
-        // (parts in fp16, whose 11 bits hold what is left at every step)
-        __half2 z[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = __floats2half2_rn(v[2 * e] * inv, v[2 * e + 1] * inv);
-        __syncwarp();  // all of these rows are read
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          uint32_t q8[2] = {0u, 0u};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(z[e]), __NV_SATFINITE, __NV_E4M3);
-            q8[e / 2] |= two << (16 * (e & 1));
-            if (part + 1 < PARTS) z[e] = __hsub2(z[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3)));
-          }
-          *reinterpret_cast<uint2*>(sm + L::Q + part * (FA_ROWS * D) + tc::swz_offset<D>(warp * 32 + row, (c / 2) * 8) + (c & 1) * 8) =
-              make_uint2(q8[0], q8[1]);
-        }
-      }
-      unit *= A.scale_log2;
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&bars[L::B_Q]);
+      unit = A.units[row_tile(A, p.b, p.h, p.rt) * FA_ROWS + r];
     };
     int4 split = make_int4(0, 0, 0, 0);  // the split segment that begins in this CTA (its last piece)
     bool more = ww.next(A, lane);
-    if (more) queries();
+    if (more) begin();
     while (more) {
       const bool live = warp * 32 < p.rows;  // some row of this warp exists
       float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
@@ -485,7 +506,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         const uint32_t buf = j & 1, ts = tmem + lanes + buf * 64;
         const bool first = t == p.t0;
         const float* scales = sc + place * (2 * FA_HALVES);
-        const int* kind_at = kinds + place;
+        const FaKind* kind_at = kinds + place;
         if (++place == L::SCALES) place = 0;
         uint64_t sum[2];
         // The reference moves where some row's maximum has outgrown it, or a page's scale of V the others'.
@@ -515,20 +536,32 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         };
         // (all lanes together from the vote to the stores: those are the whole warp's)
         // weights of 64 logits of one scale: into place, and into the sum before they are rounded
-        auto weigh = [&](const float* x, float c, float f, auto scaled) {
-          const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
-          const uint64_t c2 = pair_of(c, c), f2 = pair_of(f, f), ref2 = pair_of(-ref, -ref);
+        float share = 1.f;  // of a tile with one scale of V: over the reference
+        auto weigh = [&](const float* x, auto plain) {
+          // of one scale of V: its share enters with the exponent, and leaves the sum again
+          const float ref = (m == -INFINITY ? 0.f : m) - kFaBias - (decltype(plain)::value ? __log2f(share) : 0.f);
+          const uint64_t ref2 = pair_of(-ref, -ref);
+          uint64_t c2 = 0, f2 = 0;
+          if (decltype(plain)::value) {
+            const float c = fminf(scales[0] * unit, 3e38f);
+            c2 = pair_of(c, c);
+          }
           sum[0] = sum[1] = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
+              if (!decltype(plain)::value && e % 8 == 0) {
+                const float c = fminf(scales[4 * h + e / 8] * unit, 3e38f), f = scales[FA_HALVES + 4 * h + e / 8] * vinv;
+                c2 = pair_of(c, c);
+                f2 = pair_of(f, f);
+              }
               float u, v;
               unpair(fma2(pair_of(x[32 * h + e], x[32 * h + e + 1]), c2, ref2), u, v);
               uint64_t w = pair_of(ex2(u), ex2(v));
               sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], w);
-              if (decltype(scaled)::value) w = mul2(w, f2);
+              if (!decltype(plain)::value) w = mul2(w, f2);
               unpair(w, u, v);
               pk[e / 2] = pack_half(u, v);
             }
@@ -536,45 +569,52 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           }
         };
         auto largest = [&](const float* x) {
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < TK; e += 2) mx[(e / 2) & 3] = max3(mx[(e / 2) & 3], x[e], x[e + 1]);
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int y = 0; y < FA_HALVES; ++y) {
+            const float* z = x + 8 * y;
+            top = fmaxf(top, max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])) *
+                                 fminf(scales[y] * unit, 3e38f));
+          }
+          return top;
         };
         ok = __all_sync(0xffffffffu, wait(&bars[L::B_S + buf], j >> 1, 12));
         if (!ok) break;
         if (live) {
           tc::tc_fence_after();
-          const int kind = *kind_at;
-          const float ks = scales[0], vs = scales[FA_HALVES];  // the first page's
+          const int kind = kind_at->kind;
+          const float vmax = kind_at->vmax;
           auto total = [&]() {
             float s0, s1, s2, s3;
             unpair(sum[0], s0, s1);
             unpair(sum[1], s2, s3);
             return (s0 + s1) + (s2 + s3);
           };
-          if ((kind & FA_PLAIN) && vs <= vref) {  // what most tiles are, but for a piece's first
+          if (kind & FA_WHOLE) {  // what most tiles are
             // Weights against the standing reference, without a look at the maximum: a sum within fp16's range says that
             // all of them are. (The maximum first: 64 logits' worth of instructions and of latency more a tile.)
-            const float c = fminf(ks * unit, 3e38f), f = vs * vinv;
             float x[TK];
             tc::tmem_ld64(ts, x);
+            bool settled = vmax > vref;  // a piece's first tile, or a page's scale of V above the others'
 #pragma unroll 1
-            for (bool again = false;;) {
-              if (f == 1.f)
-                weigh(x, c, f, std::false_type());
-              else
-                weigh(x, c, f, std::true_type());
-              if (again || !__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) break;
+            for (;;) {
+              if (settled) settle(largest(x), vmax, 0.f);
+              share = kind & FA_PLAIN ? vmax * vinv : 0.f;
+              if (share >= 0x1p-40f) {
+                weigh(x, std::true_type());
+              } else {
+                share = 1.f;
+                weigh(x, std::false_type());
+              }
+              if (settled || !__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) break;
               tc::tmem_st_wait();
-              settle(largest(x) * c, vs, 0.f);
-              again = true;
+              settled = true;
             }
           } else {
             // eight keys at a time, S read twice (rolled, as this is what few tiles are)
-            uint64_t see = kind & FA_WHOLE ? ~0ull : sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
+            const uint64_t see = sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
             __syncwarp();
-            float vmax = 0.f, top = -INFINITY;
+            float top = -INFINITY;
             auto eight = [&](int y, float* z) {  // logits
               tc::tmem_ld8(ts + 8 * y, z);
               const float s = scales[y], c = fminf(s * unit, 3e38f);
@@ -586,7 +626,6 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             for (int y = 0; y < FA_HALVES; ++y) {
               float z[8];
               eight(y, z);
-              vmax = fmaxf(vmax, scales[FA_HALVES + y]);
               top = fmaxf(top, max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])));
             }
             settle(top, vmax, kFaSlack);
@@ -606,19 +645,17 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
               }
               tc::tmem_st4(ts + 4 * y, pk);  // (S of these columns has been read)
             }
-            if (!(kind & FA_WHOLE)) {
-              ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
-              any_bad |= bad[2 * buf] | bad[2 * buf + 1];
-            }
+            ok = __all_sync(0xffffffffu, wait(&bars[L::B_W + buf], j >> 1, 14)) && ok;
+            any_bad |= bad[2 * buf] | bad[2 * buf + 1];
           }
-          l += total();
+          l += __fdividef(total(), share);
         }
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&bars[L::B_P + buf]);
       }
-      // ---- the piece's output; the next one's queries first ----------------------
+      // ---- the piece's output; the next one begun first ----------------------
       if (p.parts) split = make_int4(p.b, p.h, p.rt, p.parts);
       const int b = p.b, h = p.h, n0 = p.k.n0, t0 = p.t0;
       const bool whole = t0 == 0 && t1 == p.tiles, own = r < p.rows && ok;
@@ -626,7 +663,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       const Sees saw = sees;
       const Keys<TK> keys = p.k;
       more = ww.next(A, lane);
-      if (more) queries();
+      if (more) begin();
       if (!ok) continue;
       const uint32_t last = j - 1;
       ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + (last & 1)], last >> 1, 15));
@@ -799,16 +836,35 @@ int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   return check_launch("attention_fp8_merge");
 }
 
-Plan fa_plan(int rows, int D) {
-  return make_plan(FA_CTAS * num_sms_current_device(), std::min(FA_ROWS, (rows + 7) / 8 * 8), D);
+// What the queries' parts take, after the plan's regions (for fp16, which has more of them; a row's unit in four bytes).
+struct FaQueries {
+  int64_t tiles;
+  size_t off_units, off_parts, bytes;
+};
+FaQueries fa_queries(const Plan& p, int64_t B, int64_t Hkv, int g, int T, int D) {
+  FaQueries q;
+  const int npr = FA_ROWS / g;
+  q.tiles = B * Hkv * ((T + npr - 1) / npr);
+  q.off_units = p.bytes;
+  q.off_parts = align_up(q.off_units + (size_t)q.tiles * FA_ROWS * 4, 256);
+  q.bytes = q.off_parts + (size_t)q.tiles * 3 * FA_ROWS * D;
+  return q;
+}
+
+Plan fa_plan(int64_t rows, int D) {
+  return make_plan(FA_CTAS * num_sms_current_device(), (int)std::min<int64_t>(FA_ROWS, (rows + 7) / 8 * 8), D);
 }
 
 template <typename T, int D>
 int fa_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
   using L = FaSmem<D, std::is_same<T, __nv_bfloat16>::value ? 2 : 3>;
   const int g = a.Hq / a.Hkv;
-  const Plan plan = fa_plan((int)std::min((int64_t)g * a.T, (int64_t)FA_ROWS), D);
-  const Args A = make_args(a, plan, FA_ROWS / g, kFaLead, ws);
+  const Plan plan = fa_plan((int64_t)g * a.T, D);
+  const FaQueries qs = fa_queries(plan, a.B, a.Hkv, g, a.T, D);
+  Args A = make_args(a, plan, FA_ROWS / g, kFaLead, ws);
+  A.units = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + qs.off_units);
+  A.queries = static_cast<uint8_t*>(ws) + qs.off_parts;
+  if (a.B > 65535) return fail(DROPKV_ERR_UNSUPPORTED, "attention_fp8: %d sequences are too many", a.B);
   CUtensorMap km, vm;
   int rc = make_fp8_tensor_maps(&km, &vm, a.pool, std::min(a.pool.block, FA_TK));
   if (rc) return rc;
@@ -828,10 +884,15 @@ int fa_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
+  cfg.gridDim = dim3(A.RT, a.Hkv, a.B);
+  cfg.blockDim = dim3(FQ_NT);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_queries_kernel<T, D>, A);
+  if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 queries launch: %s", cudaGetErrorString(e));
+  if ((rc = check_launch("attention_fp8_queries"))) return rc;
   cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(FA_NT);
   cfg.dynamicSmemBytes = L::BYTES;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
+  e = cudaLaunchKernelEx(&cfg, kern, km, vm, A);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 launch: %s", cudaGetErrorString(e));
   rc = check_launch("attention_fp8");
   if (rc || a.cap <= FA_TK) return rc;  // a cache of one tile: nothing is split
@@ -847,9 +908,9 @@ int launch_fp8_merge(const fa::Args& A, int dtype, int ctas, cudaStream_t st) {
 }
 
 size_t attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
-  (void)B, (void)cap;
+  (void)cap;
   const int64_t rows = (int64_t)Hq / Hkv * T;
-  return rows <= kFp8DecodeRows ? fp8_decode_plan((int)rows, D).bytes : fa_plan((int)std::min(rows, (int64_t)FA_ROWS), D).bytes;
+  return rows <= kFp8DecodeRows ? fp8_decode_plan((int)rows, D).bytes : fa_queries(fa_plan(rows, D), B, Hkv, Hq / Hkv, T, D).bytes;
 }
 
 int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {

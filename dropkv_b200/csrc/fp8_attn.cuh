@@ -31,6 +31,8 @@ struct Args {
   int4* meta;        // [CTAs]: the split segment that begins in a CTA: b, KV head, row tile, its partials (0: none)
   float* part_o;     // [2 CTAs][rows_pad][D]
   float* part_ml;    // [2 CTAs][2][rows_pad]
+  float* units;      // [row tiles][128]: what a unit of a row's queries makes of a logit, in base 2 (many rows)
+  uint8_t* queries;  // [row tiles][parts][128][D]: 8-bit parts of the queries, as the products read them
   // r / g for a row r of a tile: r (g_mul g - 2^16) < 2^7 2^7 < 2^16
   __device__ __forceinline__ int quot(int r) const { return (r * g_mul) >> 16; }
 };
@@ -255,6 +257,11 @@ __device__ __forceinline__ int64_t slot_of(const Piece<TK>& p) {
   return 2 * (int64_t)blockIdx.x + (p.t0 > 0 ? 0 : 1);
 }
 
+// The number of a row tile.
+__device__ __forceinline__ int64_t row_tile(const Args& A, int b, int h, int rt) {
+  return ((int64_t)b * A.a.Hkv + h) * A.RT + rt;
+}
+
 // Row r of a row tile in the output [B, Hq, T, D].
 __device__ __forceinline__ int64_t out_row(const Args& A, int b, int h, int n0, int r) {
   const int token = A.quot(r), head = h * A.g + r - token * A.g;
@@ -346,6 +353,8 @@ inline Args make_args(const AttnFp8& a, const Plan& p, int npr, int lead, void* 
   A.meta = reinterpret_cast<int4*>(w + p.off_meta);
   A.part_o = reinterpret_cast<float*>(w + p.off_o);
   A.part_ml = reinterpret_cast<float*>(w + p.off_ml);
+  A.units = nullptr;
+  A.queries = nullptr;
   return A;
 }
 
