@@ -99,6 +99,9 @@ SIGNATURES = {
     "dropkv_attention_fp8": (_c_int, [_c_p] + [_c_i64] * 4 + ([_c_p] + [_c_i64] * 3) * 2 + ([_c_p] + [_c_i64] * 2) * 2
                              + [_c_int, _c_int, _c_p, _c_int, _c_p, _c_p] + [_c_i64] * 3 + [_c_int] * 8
                              + [_c_f, _c_p, _c_p, _c_sz, _c_p]),
+    "dropkv_verify_draft_workspace_size": (_c_sz, [_c_int] * 4),
+    "dropkv_verify_draft": (_c_int, ([_c_p] + [_c_i64] * 2) * 2 + [_c_int, _c_p, _c_p] + [_c_int] * 3 + [_c_f]
+                            + [_c_p] * 4 + [_c_sz, _c_p]),
     "dropkv_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_i64, _c_int, _c_p, _c_int, _c_int, _c_f]
                               + [_c_p] * 5 + [_c_sz, _c_p]),
 }

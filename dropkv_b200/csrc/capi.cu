@@ -912,5 +912,36 @@ int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss
   return launch_attention_fp8(a, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
+static bool verify_sizes_ok(int B, int T, int V) {
+  return B >= 1 && B <= (1 << 24) && T >= 0 && T <= 256 && V >= 1 && V <= (1 << 21);
+}
+
+size_t dropkv_verify_draft_workspace_size(int B, int T, int V, int draft) {
+  return verify_sizes_ok(B, T, V) ? verify_draft_workspace_size(B, T, V, draft != 0) : 0;
+}
+
+int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const void* draft, int64_t d_sb, int64_t d_si,
+                        int dtype, const int64_t* tokens, const float* uniforms, int B, int T, int V, float temperature,
+                        int64_t* accepted, int64_t* next_token, float* prob, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (!eb) return fail(DROPKV_ERR_ARG, "unknown dtype %d", dtype);
+  if (B == 0) return DROPKV_OK;
+  if (T > 256) return fail(DROPKV_ERR_UNSUPPORTED, "verify_draft takes at most 256 drafted tokens (got %d)", T);
+  if (V > (1 << 21)) return fail(DROPKV_ERR_UNSUPPORTED, "verify_draft takes vocabularies of at most %d (got %d)", 1 << 21, V);
+  if (!verify_sizes_ok(B, T, V)) return fail(DROPKV_ERR_ARG, "invalid sizes B=%d T=%d V=%d", B, T, V);
+  if (!target || !uniforms || !accepted || !next_token || (T > 0 && (!tokens || !prob)))
+    return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) % eb)
+    return fail(DROPKV_ERR_ARG, "logits must be aligned to their elements");
+  if (!(temperature >= 1e-6f) || !(temperature <= 1e6f))
+    return fail(DROPKV_ERR_ARG, "temperature must be in [1e-6, 1e6]");
+  int rc = check_ws(workspace, workspace_bytes, verify_draft_workspace_size(B, T, V, draft != nullptr && T > 0));
+  if (rc) return rc;
+  VerifyDraft q{target, t_sb, t_si, T > 0 ? draft : nullptr, d_sb, d_si, tokens, uniforms, B, T, V, temperature,
+                accepted, next_token, prob};
+  return launch_verify_draft(q, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"
 

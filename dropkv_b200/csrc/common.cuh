@@ -352,4 +352,20 @@ struct AttnFp8 {
 size_t attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
 int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st);
 
+struct VerifyDraft {
+  const void* target;  // [B, T + 1, V], element strides of a sequence and a row
+  int64_t t_sb, t_si;
+  const void* draft;  // [B, T, V] or nullptr
+  int64_t d_sb, d_si;
+  const int64_t* tokens;  // [B, T]
+  const float* uniforms;  // [B, T + 1]
+  int B, T, V;
+  float temperature;
+  int64_t* accepted;    // [B]
+  int64_t* next_token;  // [B]
+  float* prob;          // [B, T]
+};
+size_t verify_draft_workspace_size(int B, int T, int V, bool draft);
+int launch_verify_draft(const VerifyDraft& q, int dtype, void* ws, cudaStream_t st);
+
 }  // namespace dropkv

@@ -7,7 +7,8 @@ and decoding over it needs nothing of the host if the pages are handed out there
 * ``store_rows``     -- K/V rows to slots (the eviction's outputs, accepted drafts);
 * ``qk_norm_rope``   -- head norms, position rotation and the cache write in one pass;
 * ``tree_attention`` -- a tree of drafted tokens over a cache in pages or row buffers;
-* ``token_logprobs`` -- log probabilities of given tokens, entropy, top alternatives.
+* ``token_logprobs`` -- log probabilities of given tokens, entropy, top alternatives;
+* ``verify_draft``   -- drafted tokens accepted by given random numbers, and the token after them.
 
 K and V pools are ``[pages, Hkv, block_size, D]``, any strides with contiguous rows (a
 pool stored ``[pages, block_size, Hkv, D]`` is passed transposed); slot ``s`` is row
@@ -28,8 +29,8 @@ import torch
 from . import _lib
 from .ops import _CHECK_STATUS, _DTYPE_CODE
 
-__all__ = ["BlockTables", "TokenLogprobs", "block_tables", "store_rows", "qk_norm_rope", "tree_attention",
-           "token_logprobs", "tree_mask_from_parents"]
+__all__ = ["BlockTables", "TokenLogprobs", "VerifiedDraft", "block_tables", "store_rows", "qk_norm_rope",
+           "tree_attention", "token_logprobs", "tree_mask_from_parents", "verify_draft"]
 
 
 class BlockTables(NamedTuple):
@@ -44,6 +45,12 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor                 # fp32, the shape of the rows
     top_logprobs: Optional[torch.Tensor]  # fp32 [..., top_k], None for top_k = 0
     top_tokens: Optional[torch.Tensor]    # int64 [..., top_k]
+
+
+class VerifiedDraft(NamedTuple):
+    accepted: torch.Tensor     # [B] int64: drafted tokens accepted
+    next_token: torch.Tensor   # [B] int64: the token after them
+    accept_prob: torch.Tensor  # [B, T] fp32: what each token's acceptance has as probability
 
 
 # The current stream's handle by device index: the raw query skips making a Stream object, 2 us of
@@ -429,3 +436,63 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0,
     if rc:
         _lib.check(rc, "dropkv_token_logprobs")
     return TokenLogprobs(logprob, entropy, top_lp, top_id)
+
+
+@functools.lru_cache(maxsize=4096)
+def _verify_workspace(index: int, B: int, T: int, V: int, draft: bool) -> int:
+    """Bytes of a verify_draft workspace on the current device ``index``."""
+    return int(_lib.load().dropkv_verify_draft_workspace_size(B, T, V, int(draft)))
+
+
+@_on_its_device
+def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor,
+                 draft_logits: Optional[torch.Tensor] = None, temperature: float = 1.0) -> VerifiedDraft:
+    """T drafted tokens a sequence ([B, T] int64, a chain) against the target's logits [B, T + 1, V]: how many are
+    accepted, and the token that follows them, so that what is kept is distributed as the target's own samples.
+
+    With p_i = softmax(target_logits[:, i] / temperature) and q_i the same of ``draft_logits`` [B, T, V] (None:
+    the draft has no probabilities, q_i is 1 at its token), token i is accepted while
+    ``uniforms[:, i] * q_i(x_i) < p_i(x_i)``. ``next_token`` is drawn from max(p_n - q_n, 0) at the first
+    rejected token n, from p_n if none is: the first one whose cumulative sum passes ``uniforms[:, T]`` times the
+    whole. ``uniforms`` [B, T + 1] fp32 in [0, 1). ``accept_prob`` is min(1, p_i(x_i) / q_i(x_i)) for every i.
+
+    A token outside [0, V) (-1) ends its sequence's draft: the one that follows is drawn from that row's p. Where a
+    row that is looked at holds NaN or +inf, or nothing but -inf, the draft ends and ``next_token`` is -1. Logits
+    in fp32, fp16 or bf16 of any strides with contiguous rows; words ruled out by -inf are never drawn. Decisions
+    and draws are as exact as 64-bit sums. T at most 256, V at most 2^21, temperature from 1e-6 to 1e6.
+    """
+    dev = _on_one_device(target_logits, tokens, uniforms, *((draft_logits,) if draft_logits is not None else ()))
+    ls, dtype = target_logits.shape, target_logits.dtype
+    dt = _DTYPE_CODE.get(dtype)
+    if dt is None:
+        raise TypeError(f"logits must be fp32/fp16/bf16; got {dtype}")
+    if len(ls) != 3 or ls[1] < 1 or ls[2] < 1:
+        raise ValueError(f"expected target_logits [B, T + 1, V], got {tuple(ls)}")
+    B, T, V = ls[0], ls[1] - 1, ls[2]
+    if draft_logits is not None:
+        if draft_logits.shape != (B, T, V):
+            raise ValueError(f"draft_logits must be {(B, T, V)}, got {tuple(draft_logits.shape)}")
+        if draft_logits.dtype != dtype:
+            raise TypeError(f"draft_logits must be {dtype}, got {draft_logits.dtype}")
+    tokens = _ints(tokens, torch.int64, (B, T), "tokens")
+    uniforms = _ints(uniforms, torch.float32, (B, T + 1), "uniforms")
+    rows = []
+    for x in (target_logits, draft_logits):
+        if x is not None and V > 1 and x.stride(2) != 1:
+            x = x.contiguous()
+        rows.append(x)
+    target, draft = rows
+    device = target.device
+    out = VerifiedDraft(_new(torch.int64, device, B), _new(torch.int64, device, B), _new(torch.float32, device, B, T))
+    if B == 0:
+        return out
+    need = max(_verify_workspace(dev, B, T, V, draft is not None), 1)
+    ws = _new(torch.uint8, device, need)
+    rc = _lib.load().dropkv_verify_draft(
+        target.data_ptr(), target.stride(0), target.stride(1), draft.data_ptr() if draft is not None else None,
+        draft.stride(0) if draft is not None else 0, draft.stride(1) if draft is not None else 0, dt, tokens.data_ptr(),
+        uniforms.data_ptr(), B, T, V, float(temperature), out.accepted.data_ptr(), out.next_token.data_ptr(),
+        out.accept_prob.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "dropkv_verify_draft")
+    return out

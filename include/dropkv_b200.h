@@ -440,6 +440,21 @@ DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, i
                                     int Hkv, int T, int D, float scale, void* out, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* Verification of T drafted tokens of each sequence by given random numbers. With
+ * p_i = softmax(target[b, i] / temperature) ([B, T + 1, V]), q_i the same of draft ([B, T, V]; NULL: all
+ * of it at the drafted token), both fp32, fp16 or bf16 with element strides t_s* / d_s* of a sequence and
+ * a row: accepted[b] = the drafted tokens before the first i with uniforms[b, i] q_i(x_i) >= p_i(x_i), or with
+ * a token outside [0, V), which ends the draft (padding). next_token[b]: drawn from max(p_n - q_n, 0) for a
+ * rejected token n = accepted[b], else from p_n, as the first t whose cumulative sum passes
+ * uniforms[b, T] times the whole. prob[b, i] = min(1, p_i(x_i) / q_i(x_i)), 0 for a token outside [0, V).
+ * Where a row that is looked at holds NaN or +inf, or nothing but -inf, the draft ends there and next_token is
+ * -1. uniforms in [0, 1); T <= 256, V <= 2^21, temperature in [1e-6, 1e6]. */
+DROPKV_API size_t dropkv_verify_draft_workspace_size(int B, int T, int V, int draft);
+DROPKV_API int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const void* draft, int64_t d_sb,
+                                   int64_t d_si, int dtype, const int64_t* tokens, const float* uniforms, int B, int T,
+                                   int V, float temperature, int64_t* accepted, int64_t* next_token, float* prob,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Diagnostic: one 128-row tile through a tcgen05 MMA form used by the fused
  * scorer (mode 0: out[128][n] = A[128][128] B[n][128]^T with A loaded by TMA;
  * mode 1: out[128][n] = A[128][128]^T B[n][128]^T with A read MN-major; modes 2/3:
