@@ -13,8 +13,7 @@
 // from; and where fp32 cannot tell whether a token is accepted, its rows' sums are taken
 // in 64 bits too.
 //
-// 2^x in 64 bits: x = k / 64 + r, a table of 2^(j / 64) and the exponential's series in r ln 2 (|r| <= 2^-7: five terms leave
-// 4e-14 of the value).
+// 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and two terms of the exponential's series for what is left of x.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -61,6 +60,31 @@ __device__ __forceinline__ float vf_ex2(float x) {
   return y;
 }
 
+// Two floats in one register pair, and arithmetic on both at once.
+__device__ __forceinline__ uint64_t vf_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void vf_unpair(uint64_t r, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t vf_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t vf_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t vf_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <typename T>
 struct VfVec {
   static constexpr int N = 16 / sizeof(T);
@@ -78,7 +102,7 @@ __device__ __forceinline__ int64_t vf_index(const VfArgs& a, int b, int i, bool 
 }
 
 // A chunk of a row: elements [e0, e1), the whole vectors of 16 bytes between them by all threads, the ends by some. Each thread
-// has a maximum and a sum of its own. (Differences first, then the product in two parts: exponents are off by little of
+// has a reference (near its maximum) and a sum of its own. (Differences first, then the product in two parts: exponents are off by little of
 // themselves, however far from zero the logits are.)
 template <typename T>
 __global__ void __launch_bounds__(VF_NT) verify_rows_kernel(const __grid_constant__ VfArgs a) {
@@ -95,42 +119,61 @@ __global__ void __launch_bounds__(VF_NT) verify_rows_kernel(const __grid_constan
   pdl_launch_dependents();
   pdl_wait();
   float m = -INFINITY, base = 0.f, s = 0.f;
-  auto add = [&](const float* y, int n) {  // n elements
-    float top = y[0];
-#pragma unroll
-    for (int e = 1; e < n; ++e) top = fmaxf(top, y[e]);
-    if (top > m) {
-      s *= m == -INFINITY ? 0.f : vf_ex2((m - top) * a.c);
-      m = base = top;
-    }
-#pragma unroll
-    for (int e = 0; e < n; ++e) {
-      const float d = y[e] - base;
-      s += vf_ex2(fmaf(d, a.c_lo, d * a.c));
+  auto raise = [&](float top) {  // (a reference that is a little low does as well: weights up to 2^16)
+    if ((top - m) * a.c > 16.f || m == -INFINITY) {
+      s *= m == -INFINITY ? 1.f : vf_ex2((m - top) * a.c);
+      m = top;
+      base = top == -INFINITY ? 0.f : top;
     }
   };
   const T* p = x + e0;
   const int n = e1 - e0;
   const int head = n <= 0 ? 0 : min(n, (int)((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T)));
   const int vecs = (n - head) / N, tail = n - head - vecs * N;
-  for (int v0 = tid; v0 < vecs; v0 += VF_NT * VF_AHEAD) {
-    uint4 w[VF_AHEAD];
+  const uint4* pv = reinterpret_cast<const uint4*>(p + head) + tid;
+  const uint64_t c2 = vf_pair(a.c, a.c), lo2 = vf_pair(a.c_lo, a.c_lo);
+  // a thread's next vectors are on their way while it takes these
+  uint4 w[VF_AHEAD], next[VF_AHEAD];
+  auto load = [&](int v0, uint4* to) {
 #pragma unroll
     for (int u = 0; u < VF_AHEAD; ++u)
-      if (v0 + u * VF_NT < vecs) w[u] = __ldcs(reinterpret_cast<const uint4*>(p + head) + v0 + u * VF_NT);
+      if (v0 + u * VF_NT < vecs) to[u] = __ldcs(pv + v0 - tid + u * VF_NT);
+  };
+  load(tid, w);
+  for (int v0 = tid; v0 < vecs; v0 += VF_NT * VF_AHEAD) {
+    load(v0 + VF_NT * VF_AHEAD, next);
 #pragma unroll
     for (int u = 0; u < VF_AHEAD; ++u) {
-      if (v0 + u * VF_NT >= vecs) continue;
-      const T* t = reinterpret_cast<const T*>(&w[u]);
-      float y[N];
+      if (v0 + u * VF_NT < vecs) {
+        const T* t = reinterpret_cast<const T*>(&w[u]);
+        float y[N], top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = to_f(t[e]);
-      add(y, N);
+        for (int e = 0; e < N; ++e) {
+          y[e] = to_f(t[e]);
+          top = fmaxf(top, y[e]);
+        }
+        raise(top);
+        const uint64_t base2 = vf_pair(-base, -base);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const uint64_t d = vf_add2(vf_pair(y[e], y[e + 1]), base2);
+          float f, g;
+          vf_unpair(vf_fma2(d, lo2, vf_mul2(d, c2)), f, g);
+          sum = vf_add2(sum, vf_pair(vf_ex2(f), vf_ex2(g)));
+        }
+        float f, g;
+        vf_unpair(sum, f, g);
+        s += f + g;
+      }
+      w[u] = next[u];
     }
   }
   if (tid < head + tail) {
     const float y = to_f(p[tid < head ? tid : n - tail + (tid - head)]);
-    add(&y, 1);
+    raise(y);
+    const float d = y - base;
+    s += vf_ex2(fmaf(d, a.c_lo, d * a.c));
   }
   auto join = [&](float om, float os) {
     const float mn = fmaxf(m, om);
@@ -154,40 +197,85 @@ __global__ void __launch_bounds__(VF_NT) verify_rows_kernel(const __grid_constan
   }
 }
 
+constexpr int VD_TABLE = 2048;  // steps of 2^x's table: 2^x = 2^(k / 2048) 2^r, |r| <= 2^-12, whose series' third term is 8e-13
+
+enum { VD_ACCEPT = 0, VD_REJECT, VD_UNSURE, VD_END, VD_NONE };
+
 struct VdSmem {
-  double table[64];
-  double seg[2][VD_WARPS];             // sums of this CTA's segments: of p's row, of q's
-  double all[2][VD_SEGS];              // of all
+  double table[VD_TABLE];
+  double seg[2][VD_WARPS];  // sums of this CTA's segments: of p's row, of q's
+  double all[VD_SEGS];      // of all
   double sub[VD_WARPS];
-  double ratio[VF_MAX_T];              // log(p_i(x_i) / q_i(x_i)), +-inf; NaN where a row is none
   float mp[VF_MAX_T + 1], mq[VF_MAX_T + 1];
-  int found;
+  int8_t what[VF_MAX_T];    // of a drafted token
 };
 
-// A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order.
+// Of n values, at most 128, a lane has four: their sum, and which is the first to pass `least` by what is summed up to it
+// from `start` (the last with any weight, where rounding lets none); `before`: the sum before that one. All lanes get the same.
+__device__ __forceinline__ double vd_sum(const double* v, int n, int lane) {
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s += 4 * lane + k < n ? v[4 * lane + k] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+__device__ __forceinline__ int vd_find(const double* v, int n, int lane, double start, double least, double* before) {
+  double mine[4], own = 0.0;
+  int last = -1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    mine[k] = 4 * lane + k < n ? v[4 * lane + k] : 0.0;
+    if (mine[k] > 0.0) last = 4 * lane + k;
+    own += mine[k];
+  }
+  double upto = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double z = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += z;
+  }
+  double run = start + (upto - own), at_run = run, last_run = run;
+  int at = -1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (4 * lane + k == last) last_run = run;
+    if (at < 0 && mine[k] > 0.0 && run + mine[k] > least) {
+      at = 4 * lane + k;
+      at_run = run;
+    }
+    run += mine[k];
+  }
+  const unsigned past = __ballot_sync(0xffffffffu, at >= 0), some = __ballot_sync(0xffffffffu, last >= 0);
+  const int from = past ? __ffs(past) - 1 : 31 - __clz(some | 1u);
+  *before = __shfl_sync(0xffffffffu, past ? at_run : last_run, from);
+  return max(__shfl_sync(0xffffffffu, past ? at : last, from), 0);
+}
+
+// A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order. What bounds it: 64-bit arithmetic,
+// nine operations for an exponential, two to four of them a word (56 a clock and SM, as measured).
 template <typename T>
-__global__ void __launch_bounds__(VD_NT) verify_draw_kernel(const __grid_constant__ VfArgs a) {
+__global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_constant__ VfArgs a) {
   __shared__ VdSmem sm;
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CTAS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < 64) sm.table[tid] = exp2(tid / 64.0);
-  const double ln2 = 0.69314718055994530942;
-  // 2^y for y <= 0; NaN stays
-  auto pow2 = [&](double y) -> double {
-    const double shift = 6755399441055744.0 / 64;  // 1.5 * 2^52 / 64: sums with it are multiples of 1 / 64
-    const double t = y + shift;
+  for (int i = tid; i < VD_TABLE; i += VD_NT) sm.table[i] = exp2(i / (double)VD_TABLE);
+  constexpr double LN2 = 0.69314718055994530942;
+  // weight of a word: 2^((x - m) c). (Beyond `floor_` below the largest nothing is left to count.)
+  const float floor_ = (float)(-1000.0 / a.c64);
+  auto weight = [&](float x, float m) -> double {
+    const double shift = 6755399441055744.0 / VD_TABLE;  // 1.5 * 2^52 / 2048: sums with it are multiples of 1 / 2048
+    const double d = (double)x - m, t = fma(d, a.c64, shift), r = fma(d, a.c64, -(t - shift));
     const int k = __double2loint(t);
-    const double r = (y - (t - shift)) * ln2;
-    const double f = fma(r, fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0), 1.0);
-    const double z = sm.table[k & 63] * f;
-    // (under 2^-1000 nothing is left to count)
-    const double scaled = __hiloint2double(__double2hiint(z) + (k >> 6) * (1 << 20), __double2loint(z));
-    return y >= -1000.0 ? scaled : (y < -1000.0 ? 0.0 : y);
+    const double z = sm.table[k & (VD_TABLE - 1)] * fma(r, fma(r, LN2 * LN2 / 2, LN2), 1.0);
+    const double w = __hiloint2double(__double2hiint(z) + (k >> 11) * (1 << 20), __double2loint(z));
+    return x - m > floor_ ? w : 0.0;
   };
   pdl_wait();
   __syncthreads();
-  // ---- the rows' maxima and sums, and the drafted tokens' ratios -----------------
+  // ---- the rows' maxima and sums, and what becomes of the drafted tokens ---------
+  const double per = a.c64 * LN2;  // 1 / tau
   for (int i = warp; i <= a.T; i += VD_WARPS) {
     double lse[2] = {0.0, 0.0};
     float tops[2] = {0.f, 0.f};
@@ -211,50 +299,36 @@ __global__ void __launch_bounds__(VD_NT) verify_draw_kernel(const __grid_constan
       sm.mq[i] = isnan(lse[1]) ? NAN : tops[1];
       if (i < a.T) {
         const int64_t x = a.tokens[(int64_t)b * a.T + i];
-        double d = 0.0;
+        int what = VD_END;
         float prob = 0.f;
         if (x >= 0 && x < a.V) {
-          const double per = a.c64 * ln2;  // 1 / tau
           double lp = ((double)to_f(vf_row<T>(a, b, i, false)[x]) - tops[0]) * per - lse[0];
           double lq = two ? ((double)to_f(vf_row<T>(a, b, i, true)[x]) - tops[1]) * per - lse[1] : 0.0;
           // what 64 bits hold no number for is 0: a token with p of 0 is not accepted, whatever q says
           if (lp < kVfLeast) lp = -INFINITY;
           if (lq < kVfLeast) lq = -INFINITY;
-          d = lp == -INFINITY && !isnan(lq) ? -INFINITY : lp - lq;
+          const double d = lp == -INFINITY && !isnan(lq) ? -INFINITY : lp - lq;
+          const double lu = log((double)a.uniforms[(int64_t)b * (a.T + 1) + i]);
           prob = d >= 0.0 ? 1.f : (float)exp(d);
-          if (isnan(d)) prob = NAN;
+          what = lu < d ? VD_ACCEPT : VD_REJECT;
+          if (fabs(lu - d) < kVfUnsure) what = VD_UNSURE;
+          if (isnan(d)) what = VD_NONE, prob = NAN;
         }
-        sm.ratio[i] = d;
+        sm.what[i] = (int8_t)what;
         if (rank == 0) a.prob[(int64_t)b * a.T + i] = prob;
       }
     }
   }
   __syncthreads();
   const int seg = (a.V + VD_SEGS - 1) / VD_SEGS, lo = min(a.V, (rank * VD_WARPS + warp) * seg), hi = min(a.V, lo + seg);
-  // sums over a warp's segment, for all of the cluster: term(e) of each of its elements
-  auto over_segments = [&](int which, auto sum_of) -> double {
-    const double mine = sum_of(lo, hi);
-    if (lane == 0) sm.seg[which][warp] = mine;
-    cluster.sync();
-    if (tid < VD_SEGS) sm.all[which][tid] = cluster.map_shared_rank(&sm, tid / VD_WARPS)->seg[which][tid % VD_WARPS];
-    cluster.sync();  // (who reads a CTA's sums is done with them before they change, or the CTA ends)
-    double all = 0.0;
-#pragma unroll 4
-    for (int i = 0; i < VD_SEGS; ++i) all += sm.all[which][i];
-    return all;
-  };
-  auto warp_sum = [&](double s) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  };
-  // sum of f(x_e) (and y_e) over elements [at, end) by the lanes of a warp
+  // sum of f(e, x_e, y_e) over elements [at, end), by the lanes of a warp
   auto walk = [&](const T* x, const T* y, int at, int end, auto f) {
+    constexpr int AHEAD = 8;
     double s = 0.0;
-    for (int e = at + lane; e < end; e += 32 * 4) {
-      float u[4], v[4];
+    for (int e = at + lane; e < end; e += 32 * AHEAD) {
+      float u[AHEAD], v[AHEAD];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < AHEAD; ++k) {
         u[k] = v[k] = -INFINITY;
         if (e + 32 * k < end) {
           u[k] = to_f(x[e + 32 * k]);
@@ -262,47 +336,50 @@ __global__ void __launch_bounds__(VD_NT) verify_draw_kernel(const __grid_constan
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < AHEAD; ++k)
         if (e + 32 * k < end) s += f(e + 32 * k, u[k], v[k]);
     }
-    return warp_sum(s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
   };
-  auto weight = [&](float x, float m) { return pow2(((double)x - m) * a.c64); };
-  auto sum_row = [&](const T* x, float m, int which) {
-    return over_segments(which, [&](int at, int end) {
-      return walk(x, static_cast<const T*>(nullptr), at, end, [&](int, float u, float) { return weight(u, m); });
-    });
+  // All segments' sums of what the warps left in sm.seg[which]: into sm.all, and their sum.
+  auto gather = [&](int which) -> double {
+    __syncthreads();  // (sm.all has been read)
+    if (tid < VD_SEGS) sm.all[tid] = cluster.map_shared_rank(&sm, tid / VD_WARPS)->seg[which][tid % VD_WARPS];
+    __syncthreads();
+    return vd_sum(sm.all, VD_SEGS, lane);
+  };
+  // sums of weights of p's row and, unless it is NULL, of q's over the whole vocabulary
+  auto sum_rows = [&](const T* x, float mx, const T* y, float my, double* zx, double* zy) {
+    const double sx = walk(x, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, mx); });
+    double sy = 0.0;
+    if (y) sy = walk(y, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, my); });
+    if (lane == 0) sm.seg[0][warp] = sx, sm.seg[1][warp] = sy;
+    cluster.sync();
+    *zy = y ? gather(1) : 1.0;
+    *zx = gather(0);  // (p's segments stay in sm.all)
+    cluster.sync();   // (who reads a CTA's sums is done with them before they change, or the CTA ends)
   };
   // ---- which are accepted ----------------------------------------------------------
-  int n = 0;
-  bool rejected = false, none = false;
+  int n = 0, what = VD_END;
+  double zp, zq;
   for (; n < a.T; ++n) {
-    const int64_t x = a.tokens[(int64_t)b * a.T + n];
-    if (x < 0 || x >= a.V) break;
-    double d = sm.ratio[n];
-    if (isnan(d)) {
-      none = true;
-      break;
+    what = sm.what[n];
+    if (what == VD_UNSURE) {  // (the same in every thread of the cluster)
+      const int64_t x = a.tokens[(int64_t)b * a.T + n];
+      const T *xp = vf_row<T>(a, b, n, false), *xq = a.draft ? vf_row<T>(a, b, n, true) : nullptr;
+      sum_rows(xp, sm.mp[n], xq, sm.mq[n], &zp, &zq);
+      const double lp = ((double)to_f(xp[x]) - sm.mp[n]) * per - log(zp);
+      const double lq = xq ? ((double)to_f(xq[x]) - sm.mq[n]) * per - log(zq) : 0.0;
+      what = log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]) < lp - lq ? VD_ACCEPT : VD_REJECT;
     }
-    const double lu = log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]);
-    if (fabs(lu - d) < kVfUnsure) {  // (the same in every thread of the cluster)
-      const T* xp = vf_row<T>(a, b, n, false);
-      double lp = ((double)to_f(xp[x]) - sm.mp[n]) * a.c64 * ln2 - log(sum_row(xp, sm.mp[n], 0)), lq = 0.0;
-      if (a.draft) {
-        const T* xq = vf_row<T>(a, b, n, true);
-        lq = ((double)to_f(xq[x]) - sm.mq[n]) * a.c64 * ln2 - log(sum_row(xq, sm.mq[n], 0));
-      }
-      d = lp - lq;
-    }
-    if (!(lu < d)) {
-      rejected = true;
-      break;
-    }
+    if (what != VD_ACCEPT) break;
   }
-  const T* xp = vf_row<T>(a, b, n, false);
-  const float mp = sm.mp[n], mq = rejected && a.draft ? sm.mq[n] : 0.f;
-  none = none || isnan(mp) || isnan(mq);
-  if (none) {
+  const bool rejected = n < a.T && what == VD_REJECT;
+  const T *xp = vf_row<T>(a, b, n, false), *xq = rejected && a.draft ? vf_row<T>(a, b, n, true) : nullptr;
+  const float mp = sm.mp[n], mq = xq ? sm.mq[n] : 0.f;
+  if ((n < a.T && what == VD_NONE) || isnan(mp) || isnan(mq)) {
     if (rank == 0 && tid == 0) {
       a.accepted[b] = n;
       a.next_token[b] = -1;
@@ -310,75 +387,47 @@ __global__ void __launch_bounds__(VD_NT) verify_draw_kernel(const __grid_constan
     return;  // (all of the cluster)
   }
   // ---- the token after them --------------------------------------------------------
-  const T* xq = rejected && a.draft ? vf_row<T>(a, b, n, true) : nullptr;
-  const int64_t out = rejected && !a.draft ? a.tokens[(int64_t)b * a.T + n] : -1;  // q's only word
-  double zp = sum_row(xp, mp, 0), zq = 1.0;
-  if (xq) zq = sum_row(xq, mq, 1);
-  const double ip = 1.0 / zp, iq = 1.0 / zq;
-  bool residual = rejected;
+  // Drawn from p its weights do as they are: the sums are there. From max(p - q, 0), a second look at both rows, by now in L2.
+  const int out = rejected && !a.draft ? (int)a.tokens[(int64_t)b * a.T + n] : -1;  // q's only word
+  sum_rows(xp, mp, xq, mq, &zp, &zq);
+  const double iq = zp / zq;  // (in units of p's weights)
+  bool both = xq != nullptr;
   auto term = [&](int e, float u, float v) -> double {
-    const double p = weight(u, mp) * ip;
-    if (!residual) return p;
-    if (!xq) return e == out ? 0.0 : p;
-    return fmax(p - weight(v, mq) * iq, 0.0);
+    const double w = weight(u, mp);
+    if (both) return fmax(fma(-iq, weight(v, mq), w), 0.0);
+    return e == out ? 0.0 : w;
   };
-  auto sum_terms = [&](int at, int end) { return walk(xp, residual ? xq : static_cast<const T*>(nullptr), at, end, term); };
-  double whole = over_segments(0, sum_terms);
-  if (residual && !(whole > 0.0)) {  // p nowhere above q (they are equal, and a rounding rejected): p itself
-    residual = false;
-    whole = over_segments(0, sum_terms);
+  auto sum_terms = [&](int at, int end) { return walk(xp, both ? xq : static_cast<const T*>(nullptr), at, end, term); };
+  double whole = zp;
+  if (rejected) {
+    const double mine = sum_terms(lo, hi);
+    if (lane == 0) sm.seg[1][warp] = mine;
+    cluster.sync();
+    whole = gather(1);
+    if (!(whole > 0.0)) {  // p nowhere above q (they are equal, and a rounding rejected): p itself
+      both = false;
+      whole = gather(0);
+    }
+    cluster.sync();
   }
   const double least = (double)a.uniforms[(int64_t)b * (a.T + 1) + a.T] * whole;
-  // the segment whose sum passes it; the last that has any weight, where rounding lets none
-  int at_seg = -1, last = 0;
-  double before = 0.0, upto = 0.0;
-  for (int i = 0; i < VD_SEGS; ++i) {
-    const double w = sm.all[0][i];
-    if (w > 0.0) last = i;
-    if (at_seg < 0 && upto + w > least) {
-      at_seg = i;
-      before = upto;
-    }
-    upto += w;
-  }
-  if (at_seg < 0) {
-    at_seg = last;
-    before = 0.0;
-    for (int i = 0; i < last; ++i) before += sm.all[0][i];
-  }
+  double before, start;
+  const int at_seg = vd_find(sm.all, VD_SEGS, lane, 0.0, least, &before);
   if (at_seg / VD_WARPS != rank) return;  // (all have read what they read of one another)
   // this CTA's sixteen warps take parts of the segment, then one its elements
   const int s0 = min(a.V, at_seg * seg), s1 = min(a.V, s0 + seg), part = (s1 - s0 + VD_WARPS - 1) / VD_WARPS;
-  const int w0 = min(s1, s0 + warp * part), w1 = min(s1, w0 + part);
-  const double mine = sum_terms(w0, w1);
+  const double mine = sum_terms(min(s1, s0 + warp * part), min(s1, s0 + (warp + 1) * part));
   if (lane == 0) sm.sub[warp] = mine;
-  if (tid == 0) sm.found = -1;
   __syncthreads();
-  int at_part = -1;
-  last = 0;
-  upto = before;
-  double start = before;
-  for (int i = 0; i < VD_WARPS; ++i) {
-    const double w = sm.sub[i];
-    if (w > 0.0) last = i;
-    if (at_part < 0 && upto + w > least) {
-      at_part = i;
-      start = upto;
-    }
-    upto += w;
-  }
-  if (at_part < 0) {
-    at_part = last;
-    start = before;
-    for (int i = 0; i < last; ++i) start += sm.sub[i];
-  }
+  const int at_part = vd_find(sm.sub, VD_WARPS, lane, before, least, &start);
   if (warp == at_part) {
     int pick = -1, highest = -1;  // the last element with any weight
     double run = start;
+    const int w0 = min(s1, s0 + warp * part), w1 = min(s1, w0 + part);
     for (int e0 = w0; e0 < w1 && pick < 0; e0 += 32) {
       const int e = e0 + lane;
       double w = 0.0;
-      if (e < w1) w = term(e, to_f(xp[e]), residual && xq ? to_f(xq[e]) : -INFINITY);
+      if (e < w1) w = term(e, to_f(xp[e]), both ? to_f(xq[e]) : -INFINITY);
       const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
       double sum = w;
 #pragma unroll
