@@ -17,7 +17,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <cmath>
 
 #include "common.cuh"
@@ -29,12 +28,10 @@ namespace cg = cooperative_groups;
 
 constexpr int VF_NT = 256;        // threads of a chunk's CTA
 constexpr int VF_AHEAD = 4;       // vectors of a thread on their way
-constexpr int VD_WARPS = 16, VD_NT = 32 * VD_WARPS;
-constexpr int VD_CTAS = 8;        // of a cluster
-constexpr int VD_SEGS = VD_CTAS * VD_WARPS;
+constexpr int VD_SEGS = 256;      // segments of a row, at most
 constexpr int VF_MAX_T = 256;
 // fp32's sums and exponentials are off by less than this in the logarithm of a ratio (sums of positive terms over 256 threads and
-// up to 32 chunks: 2^-17 at most; 2^x within 2^-22).
+// up to 32 chunks: 2^-17 at most; 2^x within 2^-22, of exponents off by 2^-23 of themselves).
 constexpr double kVfUnsure = 4e-5;
 constexpr double kVfLeast = -745.0;  // log of a probability under what 64 bits hold
 
@@ -46,7 +43,7 @@ struct VfArgs {
   const int64_t* tokens;   // [B, T]
   const float* uniforms;   // [B, T + 1]
   int B, T, V, S, chunk;   // S chunks of a row
-  float c, c_lo;           // log2(e) / tau in two parts, both positive: -inf times them stays -inf
+  float c;                 // log2(e) / tau
   double c64;
   float2* part;            // [rows][S]: maximum, sum of 2^((x - maximum) c)
   int64_t* accepted;
@@ -69,9 +66,9 @@ __device__ __forceinline__ uint64_t vf_pair(float x, float y) {
 __device__ __forceinline__ void vf_unpair(uint64_t r, float& x, float& y) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
 }
-__device__ __forceinline__ uint64_t vf_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+__device__ __forceinline__ float vf_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t vf_add2(uint64_t a, uint64_t b) {
@@ -102,10 +99,10 @@ __device__ __forceinline__ int64_t vf_index(const VfArgs& a, int b, int i, bool 
 }
 
 // A chunk of a row: elements [e0, e1), the whole vectors of 16 bytes between them by all threads, the ends by some. Each thread
-// has a reference (near its maximum) and a sum of its own. (Differences first, then the product in two parts: exponents are off by little of
+// has a reference (near its maximum) and a sum of its own. (Differences first, then the product: exponents are off by little of
 // themselves, however far from zero the logits are.)
 template <typename T>
-__global__ void __launch_bounds__(VF_NT) verify_rows_kernel(const __grid_constant__ VfArgs a) {
+__global__ void __launch_bounds__(VF_NT, 6) verify_rows_kernel(const __grid_constant__ VfArgs a) {
   constexpr int N = VfVec<T>::N;
   __shared__ float ms[VF_NT / 32], ss[VF_NT / 32];
   const int64_t row = blockIdx.x / a.S;
@@ -131,49 +128,41 @@ __global__ void __launch_bounds__(VF_NT) verify_rows_kernel(const __grid_constan
   const int head = n <= 0 ? 0 : min(n, (int)((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T)));
   const int vecs = (n - head) / N, tail = n - head - vecs * N;
   const uint4* pv = reinterpret_cast<const uint4*>(p + head) + tid;
-  const uint64_t c2 = vf_pair(a.c, a.c), lo2 = vf_pair(a.c_lo, a.c_lo);
-  // a thread's next vectors are on their way while it takes these
-  uint4 w[VF_AHEAD], next[VF_AHEAD];
-  auto load = [&](int v0, uint4* to) {
+  const uint64_t c2 = vf_pair(a.c, a.c);
+  auto take = [&](const uint4& w) {
+    const T* t = reinterpret_cast<const T*>(&w);
+    float y[N], top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < VF_AHEAD; ++u)
-      if (v0 + u * VF_NT < vecs) to[u] = __ldcs(pv + v0 - tid + u * VF_NT);
-  };
-  load(tid, w);
-  for (int v0 = tid; v0 < vecs; v0 += VF_NT * VF_AHEAD) {
-    load(v0 + VF_NT * VF_AHEAD, next);
+    for (int e = 0; e < N; ++e) y[e] = to_f(t[e]);
 #pragma unroll
-    for (int u = 0; u < VF_AHEAD; ++u) {
-      if (v0 + u * VF_NT < vecs) {
-        const T* t = reinterpret_cast<const T*>(&w[u]);
-        float y[N], top = -INFINITY;
+    for (int e = 0; e < N; e += 2) top = vf_max3(top, y[e], y[e + 1]);
+    raise(top);
+    const uint64_t base2 = vf_pair(-base, -base);
+    uint64_t sum = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          y[e] = to_f(t[e]);
-          top = fmaxf(top, y[e]);
-        }
-        raise(top);
-        const uint64_t base2 = vf_pair(-base, -base);
-        uint64_t sum = 0;
-#pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const uint64_t d = vf_add2(vf_pair(y[e], y[e + 1]), base2);
-          float f, g;
-          vf_unpair(vf_fma2(d, lo2, vf_mul2(d, c2)), f, g);
-          sum = vf_add2(sum, vf_pair(vf_ex2(f), vf_ex2(g)));
-        }
-        float f, g;
-        vf_unpair(sum, f, g);
-        s += f + g;
-      }
-      w[u] = next[u];
+    for (int e = 0; e < N; e += 2) {
+      float f, g;
+      vf_unpair(vf_mul2(vf_add2(vf_pair(y[e], y[e + 1]), base2), c2), f, g);
+      sum = vf_add2(sum, vf_pair(vf_ex2(f), vf_ex2(g)));
     }
+    float f, g;
+    vf_unpair(sum, f, g);
+    s += f + g;
+  };
+  constexpr int STEP = VF_NT * VF_AHEAD;
+  uint4 w[VF_AHEAD];
+  int v = tid;
+  for (; v + STEP - VF_NT < vecs; v += STEP) {
+#pragma unroll
+    for (int u = 0; u < VF_AHEAD; ++u) w[u] = __ldcs(pv + (v - tid) + u * VF_NT);
+#pragma unroll
+    for (int u = 0; u < VF_AHEAD; ++u) take(w[u]);
   }
+  for (; v < vecs; v += VF_NT) take(__ldcs(pv + (v - tid)));
   if (tid < head + tail) {
     const float y = to_f(p[tid < head ? tid : n - tail + (tid - head)]);
     raise(y);
-    const float d = y - base;
-    s += vf_ex2(fmaf(d, a.c_lo, d * a.c));
+    s += vf_ex2((y - base) * a.c);
   }
   auto join = [&](float om, float os) {
     const float mn = fmaxf(m, om);
@@ -201,32 +190,34 @@ constexpr int VD_TABLE = 2048;  // steps of 2^x's table: 2^x = 2^(k / 2048) 2^r,
 
 enum { VD_ACCEPT = 0, VD_REJECT, VD_UNSURE, VD_END, VD_NONE };
 
+template <int WARPS>
 struct VdSmem {
   double table[VD_TABLE];
-  double seg[2][VD_WARPS];  // sums of this CTA's segments: of p's row, of q's
+  double root[96];          // 2^(i / 32), 2^(i / 2048)
+  double seg[3][WARPS];  // sums of this CTA's segments: of p's row, of q's, of what is drawn from
   double all[VD_SEGS];      // of all
-  double sub[VD_WARPS];
+  double sub[WARPS];
   float mp[VF_MAX_T + 1], mq[VF_MAX_T + 1];
   int8_t what[VF_MAX_T];    // of a drafted token
 };
 
-// Of n values, at most 128, a lane has four: their sum, and which is the first to pass `least` by what is summed up to it
+// Of n values, at most 256, a lane has eight: their sum, and which is the first to pass `least` by what is summed up to it
 // from `start` (the last with any weight, where rounding lets none); `before`: the sum before that one. All lanes get the same.
 __device__ __forceinline__ double vd_sum(const double* v, int n, int lane) {
   double s = 0.0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) s += 4 * lane + k < n ? v[4 * lane + k] : 0.0;
+  for (int k = 0; k < 8; ++k) s += 8 * lane + k < n ? v[8 * lane + k] : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double start, double least, double* before) {
-  double mine[4], own = 0.0;
+  double mine[8], own = 0.0;
   int last = -1;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    mine[k] = 4 * lane + k < n ? v[4 * lane + k] : 0.0;
-    if (mine[k] > 0.0) last = 4 * lane + k;
+  for (int k = 0; k < 8; ++k) {
+    mine[k] = 8 * lane + k < n ? v[8 * lane + k] : 0.0;
+    if (mine[k] > 0.0) last = 8 * lane + k;
     own += mine[k];
   }
   double upto = own;
@@ -238,10 +229,10 @@ __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double 
   double run = start + (upto - own), at_run = run, last_run = run;
   int at = -1;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (4 * lane + k == last) last_run = run;
+  for (int k = 0; k < 8; ++k) {
+    if (8 * lane + k == last) last_run = run;
     if (at < 0 && mine[k] > 0.0 && run + mine[k] > least) {
-      at = 4 * lane + k;
+      at = 8 * lane + k;
       at_run = run;
     }
     run += mine[k];
@@ -254,13 +245,16 @@ __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double 
 
 // A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order. What bounds it: 64-bit arithmetic,
 // nine operations for an exponential, two to four of them a word (56 a clock and SM, as measured).
-template <typename T>
-__global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_constant__ VfArgs a) {
-  __shared__ VdSmem sm;
+template <typename T, int VD_WARPS>
+__global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kernel(const __grid_constant__ VfArgs a) {
+  constexpr int VD_NT = 32 * VD_WARPS;
+  __shared__ VdSmem<VD_WARPS> sm;
   const cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), b = blockIdx.x / VD_CTAS;
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / ctas, segs = ctas * VD_WARPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < VD_TABLE; i += VD_NT) sm.table[i] = exp2(i / (double)VD_TABLE);
+  if (tid < 96) sm.root[tid] = exp2(tid < 32 ? tid / 32.0 : (tid - 32) / 2048.0);
+  __syncthreads();
+  for (int i = tid; i < VD_TABLE; i += VD_NT) sm.table[i] = sm.root[i >> 6] * sm.root[32 + (i & 63)];
   constexpr double LN2 = 0.69314718055994530942;
   // weight of a word: 2^((x - m) c). (Beyond `floor_` below the largest nothing is left to count.)
   const float floor_ = (float)(-1000.0 / a.c64);
@@ -320,25 +314,23 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
     }
   }
   __syncthreads();
-  const int seg = (a.V + VD_SEGS - 1) / VD_SEGS, lo = min(a.V, (rank * VD_WARPS + warp) * seg), hi = min(a.V, lo + seg);
+  const int seg = (a.V + segs - 1) / segs, lo = min(a.V, (rank * VD_WARPS + warp) * seg), hi = min(a.V, lo + seg);
   // sum of f(e, x_e, y_e) over elements [at, end), by the lanes of a warp
   auto walk = [&](const T* x, const T* y, int at, int end, auto f) {
     constexpr int AHEAD = 8;
     double s = 0.0;
-    for (int e = at + lane; e < end; e += 32 * AHEAD) {
-      float u[AHEAD], v[AHEAD];
+    int e = at + lane;
+    for (; e + 32 * (AHEAD - 1) < end; e += 32 * AHEAD) {
+      T u[AHEAD], v[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        u[k] = v[k] = -INFINITY;
-        if (e + 32 * k < end) {
-          u[k] = to_f(x[e + 32 * k]);
-          if (y) v[k] = to_f(y[e + 32 * k]);
-        }
+        u[k] = x[e + 32 * k];
+        if (y) v[k] = y[e + 32 * k];
       }
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (e + 32 * k < end) s += f(e + 32 * k, u[k], v[k]);
+      for (int k = 0; k < AHEAD; ++k) s += f(e + 32 * k, to_f(u[k]), y ? to_f(v[k]) : 0.f);
     }
+    for (; e < end; e += 32) s += f(e, to_f(x[e]), y ? to_f(y[e]) : 0.f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
@@ -346,9 +338,9 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
   // All segments' sums of what the warps left in sm.seg[which]: into sm.all, and their sum.
   auto gather = [&](int which) -> double {
     __syncthreads();  // (sm.all has been read)
-    if (tid < VD_SEGS) sm.all[tid] = cluster.map_shared_rank(&sm, tid / VD_WARPS)->seg[which][tid % VD_WARPS];
+    for (int i = tid; i < segs; i += VD_NT) sm.all[i] = cluster.map_shared_rank(&sm, i / VD_WARPS)->seg[which][i % VD_WARPS];
     __syncthreads();
-    return vd_sum(sm.all, VD_SEGS, lane);
+    return vd_sum(sm.all, segs, lane);
   };
   // sums of weights of p's row and, unless it is NULL, of q's over the whole vocabulary
   auto sum_rows = [&](const T* x, float mx, const T* y, float my, double* zx, double* zy) {
@@ -359,7 +351,6 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
     cluster.sync();
     *zy = y ? gather(1) : 1.0;
     *zx = gather(0);  // (p's segments stay in sm.all)
-    cluster.sync();   // (who reads a CTA's sums is done with them before they change, or the CTA ends)
   };
   // ---- which are accepted ----------------------------------------------------------
   int n = 0, what = VD_END;
@@ -370,6 +361,7 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
       const int64_t x = a.tokens[(int64_t)b * a.T + n];
       const T *xp = vf_row<T>(a, b, n, false), *xq = a.draft ? vf_row<T>(a, b, n, true) : nullptr;
       sum_rows(xp, sm.mp[n], xq, sm.mq[n], &zp, &zq);
+      cluster.sync();  // (who reads a CTA's sums is done with them before they change)
       const double lp = ((double)to_f(xp[x]) - sm.mp[n]) * per - log(zp);
       const double lq = xq ? ((double)to_f(xq[x]) - sm.mq[n]) * per - log(zq) : 0.0;
       what = log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]) < lp - lq ? VD_ACCEPT : VD_REJECT;
@@ -401,20 +393,23 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
   double whole = zp;
   if (rejected) {
     const double mine = sum_terms(lo, hi);
-    if (lane == 0) sm.seg[1][warp] = mine;
+    if (lane == 0) sm.seg[2][warp] = mine;
     cluster.sync();
-    whole = gather(1);
+    whole = gather(2);
     if (!(whole > 0.0)) {  // p nowhere above q (they are equal, and a rounding rejected): p itself
       both = false;
       whole = gather(0);
     }
-    cluster.sync();
   }
+  cluster.barrier_arrive();  // (what this CTA reads of others it has read; it ends when they have, too)
   const double least = (double)a.uniforms[(int64_t)b * (a.T + 1) + a.T] * whole;
   double before, start;
-  const int at_seg = vd_find(sm.all, VD_SEGS, lane, 0.0, least, &before);
-  if (at_seg / VD_WARPS != rank) return;  // (all have read what they read of one another)
-  // this CTA's sixteen warps take parts of the segment, then one its elements
+  const int at_seg = vd_find(sm.all, segs, lane, 0.0, least, &before);
+  if (at_seg / VD_WARPS != rank) {
+    cluster.barrier_wait();
+    return;
+  }
+  // this CTA's warps take parts of the segment, then one its elements
   const int s0 = min(a.V, at_seg * seg), s1 = min(a.V, s0 + seg), part = (s1 - s0 + VD_WARPS - 1) / VD_WARPS;
   const double mine = sum_terms(min(s1, s0 + warp * part), min(s1, s0 + (warp + 1) * part));
   if (lane == 0) sm.sub[warp] = mine;
@@ -445,6 +440,7 @@ __global__ void __launch_bounds__(VD_NT, 2) verify_draw_kernel(const __grid_cons
       a.next_token[b] = pick >= 0 ? pick : highest;
     }
   }
+  cluster.barrier_wait();
 }
 
 int vf_chunks(int64_t rows, int V) {
@@ -455,7 +451,7 @@ int vf_chunks(int64_t rows, int V) {
 
 template <typename T>
 int vf_launch(const VfArgs& a, int64_t rows, cudaStream_t st) {
-  if (rows * a.S > 0x7fffffff || (int64_t)a.B * VD_CTAS > 0x7fffffff)
+  if (rows * a.S > 0x7fffffff || (int64_t)a.B * 16 > 0x7fffffff)
     return fail(DROPKV_ERR_UNSUPPORTED, "verify_draft: %lld rows are too many", (long long)rows);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -470,14 +466,28 @@ int vf_launch(const VfArgs& a, int64_t rows, cudaStream_t st) {
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "verify_draft launch: %s", cudaGetErrorString(e));
   int rc = check_launch("verify_rows");
   if (rc) return rc;
+  // Few sequences: 16 CTAs of 16 warps each, all there are. Many: as many CTAs of eight warps as fit at once, four an SM.
+  const int sms = num_sms_current_device();
+  const bool few = (int64_t)a.B * 8 <= sms;
+  int ctas = few ? 16 : 8;
+  while (ctas > 1 && (int64_t)a.B * ctas > (few ? sms : 4 * sms)) ctas /= 2;
+  auto kern = few ? verify_draw_kernel<T, 16> : verify_draw_kernel<T, 8>;
+  static DeviceOnce done;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!done.done(dev)) {
+    if (cudaFuncSetAttribute(verify_draw_kernel<T, 16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return fail(DROPKV_ERR_CUDA, "cannot allow clusters of 16");
+    done.mark(dev);
+  }
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = VD_CTAS;
+  attr[1].val.clusterDim.x = ctas;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = 2;
-  cfg.gridDim = dim3(a.B * VD_CTAS);
-  cfg.blockDim = dim3(VD_NT);
-  e = cudaLaunchKernelEx(&cfg, verify_draw_kernel<T>, a);
+  cfg.gridDim = dim3(a.B * ctas);
+  cfg.blockDim = dim3(few ? 512 : 256);
+  e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "verify_draft launch: %s", cudaGetErrorString(e));
   return check_launch("verify_draw");
 }
@@ -500,8 +510,6 @@ int launch_verify_draft(const VerifyDraft& q, int dtype, void* ws, cudaStream_t 
   a.chunk = (q.V + a.S - 1) / a.S;
   a.c64 = 1.4426950408889634 / (double)q.temperature;
   a.c = (float)a.c64;
-  if ((double)a.c > a.c64) a.c = std::nextafter(a.c, 0.f);
-  a.c_lo = std::max((float)(a.c64 - (double)a.c), FLT_MIN);
   a.part = static_cast<float2*>(ws);
   a.accepted = q.accepted, a.next_token = q.next_token, a.prob = q.prob;
   if (dtype == DROPKV_DTYPE_BF16) return vf_launch<__nv_bfloat16>(a, rows, st);
