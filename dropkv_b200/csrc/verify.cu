@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -195,18 +196,21 @@ struct VdSmem {
   double table[VD_TABLE];
   double root[96];          // 2^(i / 32), 2^(i / 2048)
   double seg[3][WARPS];  // sums of this CTA's segments: of p's row, of q's, of what is drawn from
-  double all[VD_SEGS];      // of all
-  double sub[WARPS];
+  double all[VD_SEGS + VD_SEGS / 8];  // of all, as vd_at says
+  double sub[WARPS + WARPS / 8];      // of parts of the segment, likewise
   float mp[VF_MAX_T + 1], mq[VF_MAX_T + 1];
   int8_t what[VF_MAX_T];    // of a drafted token
 };
+
+// Where value i of a list of 256 lies: eight a lane then meet all banks.
+__device__ __forceinline__ int vd_at(int i) { return i + (i >> 3); }
 
 // Of n values, at most 256, a lane has eight: their sum, and which is the first to pass `least` by what is summed up to it
 // from `start` (the last with any weight, where rounding lets none); `before`: the sum before that one. All lanes get the same.
 __device__ __forceinline__ double vd_sum(const double* v, int n, int lane) {
   double s = 0.0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) s += 8 * lane + k < n ? v[8 * lane + k] : 0.0;
+  for (int k = 0; k < 8; ++k) s += 32 * k + lane < n ? v[vd_at(32 * k + lane)] : 0.0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
@@ -216,7 +220,7 @@ __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double 
   int last = -1;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    mine[k] = 8 * lane + k < n ? v[8 * lane + k] : 0.0;
+    mine[k] = 8 * lane + k < n ? v[vd_at(8 * lane + k)] : 0.0;
     if (mine[k] > 0.0) last = 8 * lane + k;
     own += mine[k];
   }
@@ -318,19 +322,23 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   // sum of f(e, x_e, y_e) over elements [at, end), by the lanes of a warp
   auto walk = [&](const T* x, const T* y, int at, int end, auto f) {
     constexpr int AHEAD = 8;
-    double s = 0.0;
-    int e = at + lane;
-    for (; e + 32 * (AHEAD - 1) < end; e += 32 * AHEAD) {
+    double sums[4] = {0.0, 0.0, 0.0, 0.0};  // (chains of additions side by side)
+    auto batch = [&](int e, auto whole) {
       T u[AHEAD], v[AHEAD];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
+        if (!decltype(whole)::value && e + 32 * k >= end) continue;
         u[k] = x[e + 32 * k];
         if (y) v[k] = y[e + 32 * k];
       }
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) s += f(e + 32 * k, to_f(u[k]), y ? to_f(v[k]) : 0.f);
-    }
-    for (; e < end; e += 32) s += f(e, to_f(x[e]), y ? to_f(y[e]) : 0.f);
+      for (int k = 0; k < AHEAD; ++k)
+        if (decltype(whole)::value || e + 32 * k < end) sums[k & 3] += f(e + 32 * k, to_f(u[k]), y ? to_f(v[k]) : 0.f);
+    };
+    int e = at + lane;
+    for (; e + 32 * (AHEAD - 1) < end; e += 32 * AHEAD) batch(e, std::true_type());
+    batch(e, std::false_type());
+    double s = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   // All segments' sums of what the warps left in sm.seg[which]: into sm.all, and their sum.
   auto gather = [&](int which) -> double {
     __syncthreads();  // (sm.all has been read)
-    for (int i = tid; i < segs; i += VD_NT) sm.all[i] = cluster.map_shared_rank(&sm, i / VD_WARPS)->seg[which][i % VD_WARPS];
+    for (int i = tid; i < segs; i += VD_NT) sm.all[vd_at(i)] = cluster.map_shared_rank(&sm, i / VD_WARPS)->seg[which][i % VD_WARPS];
     __syncthreads();
     return vd_sum(sm.all, segs, lane);
   };
@@ -412,7 +420,7 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   // this CTA's warps take parts of the segment, then one its elements
   const int s0 = min(a.V, at_seg * seg), s1 = min(a.V, s0 + seg), part = (s1 - s0 + VD_WARPS - 1) / VD_WARPS;
   const double mine = sum_terms(min(s1, s0 + warp * part), min(s1, s0 + (warp + 1) * part));
-  if (lane == 0) sm.sub[warp] = mine;
+  if (lane == 0) sm.sub[vd_at(warp)] = mine;
   __syncthreads();
   const int at_part = vd_find(sm.sub, VD_WARPS, lane, before, least, &start);
   if (warp == at_part) {
