@@ -28,6 +28,11 @@ struct F8Rows {      // K's or V's
   int64_t s_s0, s_sh;
 };
 
+struct F8Run {
+  int64_t page;
+  int start, stop;  // rows; start < 0: there is none left
+};
+
 struct F8StoreArgs {
   F8Rows r[2];
   const int64_t* slots;  // [B, N]
@@ -58,11 +63,28 @@ __device__ __forceinline__ void f8_load(const char* p, F8Vec<T, VEC>& x) {
     *reinterpret_cast<uint4*>(&x) = __ldcs(reinterpret_cast<const uint4*>(p));
 }
 
+// The larger of m and the largest magnitude in x, as bits of the row type: of two values in each word's halves for 16-bit
+// types (f8_top() gives the larger), of one in fp32.
 template <typename T, int VEC>
 __device__ __forceinline__ uint32_t f8_largest(const F8Vec<T, VEC>& x, uint32_t m) {
+  if (sizeof(T) == 4) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) m = max(m, f8_abs_bits(to_f<T>(x.v[e])));
+    for (int e = 0; e < VEC; ++e) m = max(m, f8_abs_bits(to_f<T>(x.v[e])));
+  } else if (VEC == 1) {
+    m = __vmaxu2(m, *reinterpret_cast<const uint16_t*>(&x) & 0x7fffu);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+  }
   return m;
+}
+// That magnitude as fp32's bits (the order of a type's bits is that of its magnitudes).
+template <typename T>
+__device__ __forceinline__ uint32_t f8_top(uint32_t m) {
+  if (sizeof(T) == 4) return m;
+  const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+  return f8_abs_bits(to_f<T>(*reinterpret_cast<const T*>(&h)));
 }
 template <typename T, int VEC>
 __device__ __forceinline__ uint32_t f8_largest_finite(const F8Vec<T, VEC>& x, uint32_t m) {
@@ -79,9 +101,11 @@ template <typename T, int VEC>
 __device__ __forceinline__ void f8_put(uint8_t* p, const F8Vec<T, VEC>& x, float inv, bool odd) {
   float y[VEC];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const float f = to_f<T>(x.v[e]);
-    y[e] = odd && f8_abs_bits(f) >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : f * inv;
+  for (int e = 0; e < VEC; ++e) y[e] = to_f<T>(x.v[e]) * inv;
+  if (odd) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (f8_abs_bits(to_f<T>(x.v[e])) >= 0x7f800000u) y[e] = __uint_as_float(0x7fffffffu);
   }
   if (VEC == 1) {
     *p = __nv_cvt_float_to_fp8(y[0], __NV_SATFINITE, __NV_E4M3);
@@ -143,10 +167,11 @@ __device__ __forceinline__ void f8_rescale(uint8_t* p, const F8Bytes<VEC>& x, fl
 // HBM bounds a long call: rows are read once (a page of up to 16 KB stays in registers
 // between the two looks; the rest of a larger one comes from L2), half or a quarter of that is written.
 template <typename T, int NT, int VEC>
-__global__ void __launch_bounds__(NT) store_rows_fp8_kernel(const __grid_constant__ F8StoreArgs a) {
+__global__ void __launch_bounds__(NT, 1024 / NT) store_rows_fp8_kernel(const __grid_constant__ F8StoreArgs a) {
   constexpr int EB = sizeof(T), WARPS = NT / 32;
   __shared__ uint32_t written[F8_MAX_BLOCK / 32];  // the page's rows that the run writes
   __shared__ uint32_t red[WARPS];
+  __shared__ F8Run run;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / a.chunks, i0 = (blockIdx.x % a.chunks) * a.block, h = blockIdx.y >> 1;
   const F8Rows& R = a.r[blockIdx.y & 1];
@@ -160,178 +185,246 @@ __global__ void __launch_bounds__(NT) store_rows_fp8_kernel(const __grid_constan
     return s < a.n_slots ? s : -1;
   };
   for (int i = tid; i < F8_MAX_BLOCK / 32; i += NT) written[i] = 0;
-  // the last row with a slot before the chunk, and its page
-  int64_t prev = -1;
-  int prev_row = -1;
-  for (int top = i0 - 1; top >= 0 && top > i0 - 1 - F8_GAP; top -= 32) {
-    const int64_t s = top - lane >= 0 ? slot_at(top - lane) : -1;
-    const unsigned some = __ballot_sync(0xffffffffu, s >= 0);
-    if (some) {
-      prev = page_of(__shfl_sync(0xffffffffu, s, __ffs(some) - 1));
-      prev_row = top - (__ffs(some) - 1);
-      break;
+  auto split = [&](int item, int& row, int& col) {
+    row = VEC > 1 ? item >> a.shift : item / a.lanes;
+    col = VEC > 1 ? item & (a.lanes - 1) : item - row * a.lanes;
+  };
+  auto over_cta = [&]() {  // the largest of what the warps have left
+    uint32_t m = red[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) m = max(m, red[w]);
+    return m;
+  };
+  // The chunk's rows are on their way with their slots: where the chunk is a page's, from its first row on (a prompt from its
+  // start), that is all there is to know. One barrier, no scale to read, no other rows: 43 us of a layer's, by the general way, to 17.
+  const char* xb = R.x + b * R.x_sb + h * R.x_sh;
+  F8Vec<T, VEC> keep[F8_KEEP];
+  const int there = (end - i0) * a.lanes;
+  const int64_t s0 = slots[i0];
+  bool whole = s0 >= 0 && s0 + a.block <= a.n_slots && there <= F8_KEEP * NT;
+  uint32_t chunk_largest = 0;
+  {
+    int64_t at[F8_KEEP];
+#pragma unroll
+    for (int u = 0; u < F8_KEEP; ++u) {
+      int row, col;
+      split(tid + u * NT, row, col);
+      if (i0 + row < end) {
+        at[u] = slots[i0 + row];
+        f8_load<T, VEC>(xb + (i0 + row) * R.x_sn + col * (VEC * EB), keep[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < F8_KEEP; ++u) {
+      int row, col;
+      split(tid + u * NT, row, col);
+      if (i0 + row < end) {
+        whole = whole && at[u] == s0 + row;
+        chunk_largest = f8_largest<T, VEC>(keep[u], chunk_largest);
+      }
     }
   }
-  __syncthreads();
-  for (int w0 = i0; w0 < end; w0 += 32) {
-    // a window of 32 rows: their pages, and which of them begin a run
-    const int64_t s = w0 + lane < a.N ? slot_at(w0 + lane) : -1;
-    const int64_t page = s >= 0 ? page_of(s) : -1;
-    const unsigned some = __ballot_sync(0xffffffffu, s >= 0);
-    const unsigned below = some & ((1u << lane) - 1);
-    int64_t left = __shfl_sync(0xffffffffu, page, below ? 31 - __clz(below) : 0);
-    if (!below) left = w0 + lane - prev_row <= F8_GAP ? prev : -1;
-    const unsigned begins = __ballot_sync(0xffffffffu, s >= 0 && page != left);
-    if (some) {
-      prev = __shfl_sync(0xffffffffu, page, 31 - __clz(some));
-      prev_row = w0 + 31 - __clz(some);
-    }
-    unsigned todo = end - w0 < 32 ? begins & ((1u << (end - w0)) - 1) : begins;
-    while (todo) {
-      const int at = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const int start = w0 + at;
-      const int64_t mine = __shfl_sync(0xffffffffu, page, at);
-      // the run's last row: before the next that begins one, here or in a later window
-      const unsigned later = begins & ~((2u << at) - 1);
-      int last = w0 + 31 - __clz(later ? some & ((1u << (__ffs(later) - 1)) - 1) : some);
-      bool open = !later;
-      for (int w = w0 + 32; open && w < a.N && w - last <= F8_GAP; w += 128) {
-        int64_t t[4];  // four windows at a time on their way
-#pragma unroll
-        for (int u = 0; u < 4; ++u) t[u] = w + 32 * u + lane < a.N ? slot_at(w + 32 * u + lane) : -1;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const unsigned there = __ballot_sync(0xffffffffu, t[u] >= 0);
-          const unsigned same = __ballot_sync(0xffffffffu, t[u] >= 0 && page_of(t[u]) == mine);
-          if (!open || !there) continue;
-          const unsigned other = there & ~same;
-          const unsigned run = other ? same & ((1u << (__ffs(other) - 1)) - 1) : same;
-          if (run && w + 32 * u + __ffs(run) - 1 - last <= F8_GAP)
-            last = w + 32 * u + 31 - __clz(run);
-          else
-            open = false;
-          if (other) open = false;
-        }
-      }
-      const int stop = last + 1;
-      const int64_t first_slot = mine * a.block;
-      const float old = R.s[mine * R.s_s0 + h * R.s_sh];
-      const char* xb = R.x + b * R.x_sb + h * R.x_sh;
-      uint8_t* pb = R.p + mine * R.p_s0 + h * R.p_sh;
-      const int items = (stop - start) * a.lanes;
-      auto split = [&](int item, int& row, int& col) {
-        row = VEC > 1 ? item >> a.shift : item / a.lanes;
-        col = VEC > 1 ? item & (a.lanes - 1) : item - row * a.lanes;
-      };
-      // first look
-      F8Vec<T, VEC> keep[F8_KEEP];
-      int off[F8_KEEP];
-      uint32_t largest = 0;
+  chunk_largest = __reduce_max_sync(0xffffffffu, f8_top<T>(chunk_largest));
+  if (lane == 0) red[warp] = chunk_largest;
+  const int64_t s0_page = whole ? page_of(s0) : 0;
+  if (__syncthreads_and(whole && s0 == s0_page * a.block)) {
+    chunk_largest = over_cta();
+    if (chunk_largest < 0x7f800000u) {
+      const float scale = f8_scale_for(chunk_largest), inv = 1.f / scale;
+      uint8_t* pb = R.p + s0_page * R.p_s0 + h * R.p_sh;
 #pragma unroll
       for (int u = 0; u < F8_KEEP; ++u) {
-        const int item = tid + u * NT;
-        int row, col;
-        split(item, row, col);
-        off[u] = -1;
-        if (item < items) {
-          const int64_t t = slot_at(start + row);
-          if (t >= 0) {
-            off[u] = (int)(t - first_slot);
-            f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), keep[u]);
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < F8_KEEP; ++u) {
-        if (off[u] < 0) continue;
         int row, col;
         split(tid + u * NT, row, col);
-        if (col == 0) atomicOr(&written[off[u] >> 5], 1u << (off[u] & 31));
-        largest = f8_largest<T, VEC>(keep[u], largest);
+        if (i0 + row < end) f8_put<T, VEC>(pb + row * R.p_st + col * VEC, keep[u], inv, false);
       }
+      if (tid == 0) R.s[s0_page * R.s_s0 + h * R.s_sh] = scale;
+      return;
+    }
+  }
+  int64_t s_before = -1, s_first = -1, s_after[4] = {-1, -1, -1, -1};
+  if (warp == 0) {
+    if (i0 - 1 - lane >= 0) s_before = slot_at(i0 - 1 - lane);
+    if (i0 + lane < a.N) s_first = slot_at(i0 + lane);
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (warp == 0) s_after[u] = i0 + 32 * (u + 1) + lane < a.N ? slot_at(i0 + 32 * (u + 1) + lane) : -1;
+  // The first warp finds the runs that begin in the chunk, one after the other, for all.
+  int64_t prev = -1, page = -1;  // of the last row with a slot before a window; of a lane's row in it
+  int prev_row = -1, w0 = i0 - 32;
+  unsigned some = 0, begins = 0, todo = 0;  // a window's rows with a slot, those that begin a run, those still to be taken
+  if (warp == 0) {
+    for (int top = i0 - 1; top >= 0 && top > i0 - 1 - F8_GAP; top -= 32) {
+      const int64_t s = top == i0 - 1 ? s_before : (top - lane >= 0 ? slot_at(top - lane) : -1);
+      const unsigned with = __ballot_sync(0xffffffffu, s >= 0);
+      if (with) {
+        prev = page_of(__shfl_sync(0xffffffffu, s, __ffs(with) - 1));
+        prev_row = top - (__ffs(with) - 1);
+        break;
+      }
+    }
+  }
+  auto next_run = [&](F8Run* out) {
+    while (!todo) {
+      w0 += 32;
+      if (w0 >= end) {
+        if (lane == 0) out->start = -1;
+        return;
+      }
+      const int64_t s = w0 == i0 ? s_first : (w0 + lane < a.N ? slot_at(w0 + lane) : -1);
+      page = s >= 0 ? page_of(s) : -1;
+      some = __ballot_sync(0xffffffffu, s >= 0);
+      const unsigned below = some & ((1u << lane) - 1);
+      int64_t left = __shfl_sync(0xffffffffu, page, below ? 31 - __clz(below) : 0);
+      if (!below) left = w0 + lane - prev_row <= F8_GAP ? prev : -1;
+      begins = __ballot_sync(0xffffffffu, s >= 0 && page != left);
+      if (some) {
+        prev = __shfl_sync(0xffffffffu, page, 31 - __clz(some));
+        prev_row = w0 + 31 - __clz(some);
+      }
+      todo = end - w0 < 32 ? begins & ((1u << (end - w0)) - 1) : begins;
+    }
+    const int at = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int64_t mine = __shfl_sync(0xffffffffu, page, at);
+    // the run's last row: before the next that begins one, here or in a later window
+    const unsigned later = begins & ~((2u << at) - 1);
+    int last = w0 + 31 - __clz(later ? some & ((1u << (__ffs(later) - 1)) - 1) : some);
+    bool open = !later;
+    for (int w = w0 + 32; open && w < a.N && w - last <= F8_GAP; w += 128) {
+      int64_t t[4];  // four windows at a time on their way
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        t[u] = w == i0 + 32 ? s_after[u] : (w + 32 * u + lane < a.N ? slot_at(w + 32 * u + lane) : -1);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned there = __ballot_sync(0xffffffffu, t[u] >= 0);
+        const unsigned same = __ballot_sync(0xffffffffu, t[u] >= 0 && page_of(t[u]) == mine);
+        if (!open || !there) continue;
+        const unsigned other = there & ~same;
+        const unsigned run = other ? same & ((1u << (__ffs(other) - 1)) - 1) : same;
+        if (run && w + 32 * u + __ffs(run) - 1 - last <= F8_GAP)
+          last = w + 32 * u + 31 - __clz(run);
+        else
+          open = false;
+        if (other) open = false;
+      }
+    }
+    if (lane == 0) *out = F8Run{mine, w0 + at, last + 1};
+  };
+  for (;;) {
+    if (warp == 0) next_run(&run);
+    __syncthreads();
+    if (run.start < 0) break;
+    const int64_t mine = run.page;
+    const int start = run.start, stop = run.stop;
+    const int64_t first_slot = mine * a.block;
+    const float old = R.s[mine * R.s_s0 + h * R.s_sh];
+    uint8_t* pb = R.p + mine * R.p_s0 + h * R.p_sh;
+    const int items = (stop - start) * a.lanes;
+    // first look
+    int off[F8_KEEP];
+    uint32_t largest = 0;
+#pragma unroll
+    for (int u = 0; u < F8_KEEP; ++u) {
+      const int item = tid + u * NT;
+      int row, col;
+      split(item, row, col);
+      off[u] = -1;
+      if (item < items) {
+        const int64_t t = slot_at(start + row);
+        if (t >= 0) {
+          off[u] = (int)(t - first_slot);
+          if (start != i0 || start + row >= end) f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), keep[u]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < F8_KEEP; ++u) {
+      if (off[u] < 0) continue;
+      int row, col;
+      split(tid + u * NT, row, col);
+      if (col == 0) atomicOr(&written[off[u] >> 5], 1u << (off[u] & 31));
+      largest = f8_largest<T, VEC>(keep[u], largest);
+    }
+    for (int item = tid + F8_KEEP * NT; item < items; item += NT) {
+      int row, col;
+      split(item, row, col);
+      const int64_t t = slot_at(start + row);
+      if (t < 0) continue;
+      F8Vec<T, VEC> x;
+      f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), x);
+      if (col == 0) atomicOr(&written[(int)(t - first_slot) >> 5], 1u << ((int)(t - first_slot) & 31));
+      largest = f8_largest<T, VEC>(x, largest);
+    }
+    auto largest_of_cta = [&](uint32_t m) {
+      m = __reduce_max_sync(0xffffffffu, m);
+      __syncthreads();  // (what was there has been read)
+      if (lane == 0) red[warp] = m;
+      __syncthreads();
+      return over_cta();
+    };
+    largest = largest_of_cta(f8_top<T>(largest));
+    const bool odd = largest >= 0x7f800000u;  // some value is no number: the largest of the others counts
+    if (odd) {
+      largest = 0;
+#pragma unroll
+      for (int u = 0; u < F8_KEEP; ++u)
+        if (off[u] >= 0) largest = f8_largest_finite<T, VEC>(keep[u], largest);
       for (int item = tid + F8_KEEP * NT; item < items; item += NT) {
         int row, col;
         split(item, row, col);
-        const int64_t t = slot_at(start + row);
-        if (t < 0) continue;
+        if (slot_at(start + row) < 0) continue;
         F8Vec<T, VEC> x;
         f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), x);
-        if (col == 0) atomicOr(&written[(int)(t - first_slot) >> 5], 1u << ((int)(t - first_slot) & 31));
-        largest = f8_largest<T, VEC>(x, largest);
+        largest = f8_largest_finite<T, VEC>(x, largest);
       }
-      auto over_cta = [&](uint32_t m) {
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) red[warp] = m;
-        __syncthreads();
-        m = red[0];
+      largest = largest_of_cta(largest);
+    }
+    const float need = f8_scale_for(largest);
+    const bool held = !(written[0] & 1) && old > 0.f && old < __uint_as_float(0x7f800000u);
+    const float scale = held ? fmaxf(old, need) : need;
+    if (held && scale > old) {  // the rows that the run does not write follow the scale
+      const float f = old / scale;
+      const int all = a.block * a.lanes;
+      for (int e0 = tid; e0 < all; e0 += F8_KEEP * NT) {
+        F8Bytes<VEC> x[F8_KEEP];
+        uint8_t* p[F8_KEEP];
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) m = max(m, red[w]);
-        return m;
-      };
-      largest = over_cta(largest);
-      const bool odd = largest >= 0x7f800000u;  // some value is no number: the largest of the others counts
-      if (odd) {
-        largest = 0;
+        for (int u = 0; u < F8_KEEP; ++u) {
+          int row, col;
+          split(e0 + u * NT, row, col);
+          p[u] = nullptr;
+          if (e0 + u * NT >= all || ((written[row >> 5] >> (row & 31)) & 1)) continue;
+          p[u] = pb + row * R.p_st + col * VEC;
+          f8_get_bytes<VEC>(p[u], x[u]);
+        }
 #pragma unroll
         for (int u = 0; u < F8_KEEP; ++u)
-          if (off[u] >= 0) largest = f8_largest_finite<T, VEC>(keep[u], largest);
-        for (int item = tid + F8_KEEP * NT; item < items; item += NT) {
-          int row, col;
-          split(item, row, col);
-          if (slot_at(start + row) < 0) continue;
-          F8Vec<T, VEC> x;
-          f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), x);
-          largest = f8_largest_finite<T, VEC>(x, largest);
-        }
-        __syncthreads();
-        largest = over_cta(largest);
+          if (p[u]) f8_rescale<VEC>(p[u], x[u], f);
       }
-      const float need = f8_scale_for(largest);
-      const bool held = !(written[0] & 1) && old > 0.f && old < __uint_as_float(0x7f800000u);
-      const float scale = held ? fmaxf(old, need) : need;
-      if (held && scale > old) {  // the rows that the run does not write follow the scale
-        const float f = old / scale;
-        const int all = a.block * a.lanes;
-        for (int e0 = tid; e0 < all; e0 += F8_KEEP * NT) {
-          F8Bytes<VEC> x[F8_KEEP];
-          uint8_t* p[F8_KEEP];
-#pragma unroll
-          for (int u = 0; u < F8_KEEP; ++u) {
-            int row, col;
-            split(e0 + u * NT, row, col);
-            p[u] = nullptr;
-            if (e0 + u * NT >= all || ((written[row >> 5] >> (row & 31)) & 1)) continue;
-            p[u] = pb + row * R.p_st + col * VEC;
-            f8_get_bytes<VEC>(p[u], x[u]);
-          }
-#pragma unroll
-          for (int u = 0; u < F8_KEEP; ++u)
-            if (p[u]) f8_rescale<VEC>(p[u], x[u], f);
-        }
-      }
-      // second look
-      const float inv = 1.f / scale;
-#pragma unroll
-      for (int u = 0; u < F8_KEEP; ++u) {
-        int row, col;
-        split(tid + u * NT, row, col);
-        if (off[u] >= 0) f8_put<T, VEC>(pb + off[u] * R.p_st + col * VEC, keep[u], inv, odd);
-      }
-      for (int item = tid + F8_KEEP * NT; item < items; item += NT) {
-        int row, col;
-        split(item, row, col);
-        const int64_t t = slot_at(start + row);
-        if (t < 0) continue;
-        F8Vec<T, VEC> x;
-        f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), x);
-        f8_put<T, VEC>(pb + (t - first_slot) * R.p_st + col * VEC, x, inv, odd);
-      }
-      if (tid == 0) R.s[mine * R.s_s0 + h * R.s_sh] = scale;
-      __syncthreads();  // `written` and `red` have been read
-      for (int i = tid; i < F8_MAX_BLOCK / 32; i += NT) written[i] = 0;
-      __syncthreads();
     }
+    // second look
+    const float inv = 1.f / scale;
+#pragma unroll
+    for (int u = 0; u < F8_KEEP; ++u) {
+      int row, col;
+      split(tid + u * NT, row, col);
+      if (off[u] >= 0) f8_put<T, VEC>(pb + off[u] * R.p_st + col * VEC, keep[u], inv, odd);
+    }
+    for (int item = tid + F8_KEEP * NT; item < items; item += NT) {
+      int row, col;
+      split(item, row, col);
+      const int64_t t = slot_at(start + row);
+      if (t < 0) continue;
+      F8Vec<T, VEC> x;
+      f8_load<T, VEC>(xb + (start + row) * R.x_sn + col * (VEC * EB), x);
+      f8_put<T, VEC>(pb + (t - first_slot) * R.p_st + col * VEC, x, inv, odd);
+    }
+    if (tid == 0) R.s[mine * R.s_s0 + h * R.s_sh] = scale;
+    __syncthreads();  // `written` and `red` have been read
+    for (int i = tid; i < F8_MAX_BLOCK / 32; i += NT) written[i] = 0;
   }
 }
 

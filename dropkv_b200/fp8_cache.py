@@ -67,8 +67,8 @@ def store_rows_fp8(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_page
     nothing, and its scale is the call's alone. Values are rounded to nearest, ties to even, NaN
     stays NaN and infinities (e4m3 has none) become NaN.
 
-    The rows of one page belong to one sequence of the call and follow one another there, as
-    ``block_tables`` hands slots out, with fewer than 256 rows without a slot between two of them;
+    The rows of one page belong to one sequence of the call and follow one another there, their slots ascending, as
+    ``block_tables`` hands them out, with fewer than 256 rows without a slot between two of them;
     otherwise, and where rows share a slot, that page's contents are unspecified. K and V must not
     lie in the pages. block_size is at most 1024.
     """

@@ -399,8 +399,8 @@ DROPKV_API int dropkv_token_logprobs(const void* logits, int64_t row_stride, int
  * write are rounded to it. A call that writes a page's row 0 starts the page: what its other
  * rows held means nothing from then on. Values are rounded to nearest, ties to even; infinities
  * become NaN. Slots outside the pool are skipped. The rows of one page must belong to one
- * sequence of the call and follow one another there, with fewer than 256 rows without a slot
- * between two of them; else, and where rows share a slot, the page's contents are unspecified.
+ * sequence of the call and follow one another there, slots ascending, with fewer than 256 rows without
+ * a slot between two of them; else, and where rows share a slot, the page's contents are unspecified.
  * K and V must not lie in the pages. block_size <= 1024. */
 DROPKV_API int dropkv_store_rows_fp8(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn, const void* v,
                                      int64_t v_sb, int64_t v_sh, int64_t v_sn, const int64_t* slots, void* k_pages,
