@@ -851,7 +851,7 @@ int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t kp_sh, int6
 
 static bool attn_fp8_sizes_ok(int B, int Hq, int Hkv, int T, int D, int cap) {
   return B >= 1 && Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq / Hkv <= 128 && T >= 1 && (D == 64 || D == 128) && cap >= 0 &&
-         (int64_t)B * Hkv <= 65535 && (int64_t)Hq * T <= (1 << 26);
+         (int64_t)B * Hkv <= 65535 && (int64_t)Hq * T <= (1 << 26) && (int64_t)B * Hq * T <= 0x7fffffff;
 }
 
 size_t dropkv_attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {

@@ -180,10 +180,12 @@ __device__ __forceinline__ void find_start(const Args& A, int lane, Start* out) 
       const unsigned past = __ballot_sync(0xffffffffu, before + upto > w0);
       if (past) {
         if (lane == __ffs(past) - 1) {
-          const int each = (int)(own / A.a.Hkv), rel = (int)(w0 - (before + upto - own));
+          const long long rel = w0 - (before + upto - own);
+          k.set(A, (c + lane) / A.RT, (c + lane) % A.RT);
+          const int each = k.n + A.lead;  // (many heads of a cache near 2^31 rows are more units than 32 bits count)
           out->pair = c + lane;
-          out->h = rel / each;
-          out->u = rel % each;
+          out->h = own < 0x80000000ll ? (int)rel / each : (int)(rel / each);
+          out->u = (int)(rel - (long long)out->h * each);
         }
         break;
       }

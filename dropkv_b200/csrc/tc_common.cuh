@@ -95,11 +95,6 @@ __device__ __forceinline__ uint64_t policy_evict_last() {
 __device__ __forceinline__ void tma_prefetch_desc(const void* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// 16 bytes global -> shared memory by a thread; wait_copies() waits for all of its own.
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // 3-D tile load {c0 (innermost), c1, c2} into shared memory, completion on `bar`.
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int c0, int c1,
                                             int c2, uint64_t policy) {
