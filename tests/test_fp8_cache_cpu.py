@@ -4,7 +4,7 @@
 import pytest
 import torch
 
-from dropkv_b200 import _lib, load_rows_fp8, store_rows_fp8
+from dropkv_b200 import _lib, attention_fp8, load_rows_fp8, store_rows_fp8
 
 P = 4096  # a placeholder device address
 
@@ -92,3 +92,63 @@ def test_cpu_tensors_are_refused():
         store_rows_fp8(x, x, slots, **pool)
     with pytest.raises(RuntimeError, match="CUDA"):
         load_rows_fp8(**pool, slots=slots)
+
+
+def _attention(change):
+    a = dict(q=P, kp=P, vp=P, ks=P, vs=P, st=(2048, 1024, 64), pages=4, block=16, table=P, max_blocks=3, lens=P, mask=None,
+             window=0, sinks=0, dtype=2, B=1, Hq=4, Hkv=2, T=5, D=64, scale=0.1, out=P, ws=None, have=0) | change
+    return _lib.load().dropkv_attention_fp8(
+        a["q"], 64, 64, 64, 1, a["kp"], *a["st"], a["vp"], *a["st"], a["ks"], 2, 1, a["vs"], 2, 1, a["pages"], a["block"],
+        a["table"], a["max_blocks"], a["lens"], a["mask"], 0, 5, 1, a["window"], a["sinks"], a["dtype"], a["B"], a["Hq"],
+        a["Hkv"], a["T"], a["D"], a["scale"], a["out"], a["ws"], a["have"], None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    (dict(q=None), _lib.ERR_ARG, "NULL"), (dict(lens=None), _lib.ERR_ARG, "NULL"), (dict(out=None), _lib.ERR_ARG, "NULL"),
+    (dict(table=None), _lib.ERR_ARG, "table"), (dict(kp=None), _lib.ERR_ARG, "pages and"), (dict(vs=None), _lib.ERR_ARG, "scales"),
+    (dict(dtype=0), _lib.ERR_UNSUPPORTED, "bf16 or fp16"), (dict(D=96), _lib.ERR_UNSUPPORTED, "64 or 128"),
+    (dict(block=24), _lib.ERR_UNSUPPORTED, "power of two"), (dict(block=4), _lib.ERR_UNSUPPORTED, "power of two"),
+    (dict(block=2048), _lib.ERR_UNSUPPORTED, "power of two"), (dict(max_blocks=1 << 27), _lib.ERR_UNSUPPORTED, "too long"),
+    (dict(max_blocks=-1), _lib.ERR_UNSUPPORTED, "too long"), (dict(Hq=258), _lib.ERR_UNSUPPORTED, "128 query heads"),
+    (dict(Hq=5), _lib.ERR_ARG, "sizes"), (dict(T=0), _lib.ERR_ARG, "sizes"), (dict(B=40000), _lib.ERR_ARG, "sizes"),
+    (dict(T=257, mask=P), _lib.ERR_UNSUPPORTED, "256 nodes"), (dict(window=-1), _lib.ERR_ARG, "negative"),
+    (dict(sinks=-1), _lib.ERR_ARG, "negative"), (dict(window=4, mask=P), _lib.ERR_ARG, "whole tree"),
+    (dict(kp=P + 8), _lib.ERR_ARG, "16-byte"), (dict(st=(2048, 1024, 72)), _lib.ERR_ARG, "16-byte"),
+    (dict(st=(2048, 1024, 48)), _lib.ERR_ARG, "strides"), (dict(q=P + 1), _lib.ERR_ARG, "aligned"), (dict(out=P + 2), _lib.ERR_ARG, "aligned"),
+    (dict(scale=0.0), _lib.ERR_ARG, "scale"), (dict(scale=float("nan")), _lib.ERR_ARG, "scale"),
+    (dict(scale=float("inf")), _lib.ERR_ARG, "scale"), (dict(scale=3e38), _lib.ERR_ARG, "scale"),
+    (dict(), _lib.ERR_WORKSPACE, "workspace"), (dict(T=40), _lib.ERR_WORKSPACE, "workspace"),
+])
+def test_attention_fp8_refuses(change, code, text):
+    _refused(_attention(change), code, text)
+
+
+def test_attention_workspaces():
+    size = _lib.load().dropkv_attention_fp8_workspace_size
+    assert size(1, 6, 4, 5, 128, 100) == 0 and size(1, 8, 4, 5, 96, 100) == 0 and size(1, 258, 2, 1, 128, 100) == 0
+    # the partials of two pieces a CTA; more rows than a tile's add what their queries take in 8 bits
+    assert 0 < size(1, 32, 8, 1, 128, 1000) < size(1, 32, 8, 64, 128, 1000) < size(1, 32, 8, 4096, 128, 1000)
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(Q=torch.zeros(1, 4, 3, 64)), TypeError, "bf16 or fp16"), (dict(Q=torch.zeros(4, 3, 64)), ValueError, "expected Q"),
+    (dict(Q=torch.zeros(1, 4, 3, 128, dtype=torch.bfloat16)), ValueError, "mismatch"),
+    (dict(Q=torch.zeros(1, 5, 3, 64, dtype=torch.bfloat16)), ValueError, "mismatch"),
+    (dict(cache_lens=torch.zeros(1, dtype=torch.int64)), TypeError, "cache_lens"), (dict(cache_lens=torch.zeros(2, dtype=torch.int32)), ValueError, "cache_lens"),
+    (dict(block_table=torch.zeros(4, dtype=torch.int32)), ValueError, "block_table"), (dict(block_table=torch.zeros(2, 4, dtype=torch.int32)), ValueError, "block_table"),
+    (dict(tree_mask=torch.ones(3, 3)), TypeError, "bool"), (dict(tree_mask=torch.ones(3, 4, dtype=torch.bool)), ValueError, "tree_mask"),
+    (dict(K_pages=torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)), TypeError, "float8"),
+])
+def test_attention_fp8_checks_its_tensors(change, error, text, on_device_0):
+    a = dict(Q=torch.zeros(1, 4, 3, 64, dtype=torch.bfloat16), **_pool(), cache_lens=torch.zeros(1, dtype=torch.int32),
+             block_table=torch.zeros(1, 4, dtype=torch.int32)) | change
+    with pytest.raises(error, match=text):
+        attention_fp8(**{k: v.as_subclass(_Cuda) for k, v in a.items()})
+
+
+@pytest.mark.parametrize("window", [0, -3])
+def test_attention_fp8_refuses_empty_windows(window, on_device_0):
+    a = dict(Q=torch.zeros(1, 4, 3, 64, dtype=torch.bfloat16), **_pool(), cache_lens=torch.zeros(1, dtype=torch.int32),
+             block_table=torch.zeros(1, 4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="window"):
+        attention_fp8(**{k: v.as_subclass(_Cuda) for k, v in a.items()}, window=window)
