@@ -1,6 +1,7 @@
 """Speculative decoding over paged, evicted caches: the paged operators in one loop.
 
     python examples/speculative_decode.py [--steps 8] [--tree 16] [--layers 4]
+    python examples/speculative_decode.py --sample 0.8 [--drafted 4]
 
 A small decoder with random weights (rotary positions, normed heads, grouped queries)
 prefills a ragged batch of prompts. Every layer's K/V is evicted with ``compress_varlen``,
@@ -11,6 +12,11 @@ is verified in one pass of the decoder: ``block_tables`` gives the nodes slots,
 ``tree_attention`` attends, ``token_logprobs`` gives each node's likeliest next token, and
 the longest drafted path that agrees with the decoder's own choices
 is kept. The result is what greedy decoding gives, one or more tokens a step.
+
+With ``--sample`` tokens are drawn at a temperature, over caches in 8 bits: ``store_rows_fp8``
+quantises kept and drafted rows as it writes them, ``attention_fp8`` attends over the
+pages as they are, and ``verify_draft`` accepts a chain of drawn tokens so that the result is
+distributed as the decoder's own samples.
 
 The draft here is a table of likely followers of each token, which is what the decoder says
 with no layers in between. A real one would come from a smaller model; nothing else would
@@ -28,8 +34,8 @@ import torch
 if __name__ == "__main__":
     sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from dropkv_b200 import (block_tables, compress_varlen, qk_norm_rope, store_rows, token_logprobs, tree_attention,  # noqa: E402
-                         tree_mask_from_parents)
+from dropkv_b200 import (attention_fp8, block_tables, compress_varlen, qk_norm_rope, store_rows, store_rows_fp8,  # noqa: E402
+                         token_logprobs, tree_attention, tree_mask_from_parents, verify_draft)
 
 
 class Decoder:
@@ -48,8 +54,9 @@ class Decoder:
                        up=draw(hidden, 2 * hidden, scale=hidden ** -0.5),
                        down=draw(2 * hidden, hidden, scale=0.5 * (2 * hidden) ** -0.5),
                        qn=1 + draw(D, scale=0.1), kn=1 + draw(D, scale=0.1)) for _ in range(layers)]
-        self.followers = token_logprobs(self.norm(self.embed) @ self.head, torch.arange(vocab, device=device),
-                                        top_k=3).top_tokens                  # [vocab, 3]: the draft
+        self.draft = self.norm(self.embed) @ self.head                       # [vocab, vocab]: the draft's logits
+        self.followers = token_logprobs(self.draft, torch.arange(vocab, device=device),
+                                        top_k=3).top_tokens                  # [vocab, 3]: its likeliest
         freq = 10000.0 ** (-torch.arange(0, D, 2, device=device) / D)
         angle = torch.arange(positions, device=device)[:, None] * freq
         self.cos, self.sin = angle.cos(), angle.sin()
@@ -102,6 +109,16 @@ class PagedCaches:
         self.lens = torch.zeros(batch, dtype=torch.int32, device=model.device)   # rows stored
         self.seen = torch.zeros(batch, dtype=torch.int64, device=model.device)   # tokens seen: positions go on from here
 
+    def store(self, layer, k, v, slots):
+        store_rows(k, v, slots, self.K[layer], self.V[layer])
+
+    def attend(self, layer, q, k, v, positions, slots, mask):
+        """A layer's attention of new tokens, their rows written to their slots: (attended, keys)."""
+        m, w = self.model, self.model.w[layer]
+        q, k = qk_norm_rope(q, k, m.cos, m.sin, positions, q_weight=w["qn"], k_weight=w["kn"], V=v, slots=slots,
+                            K_pages=self.K[layer], V_pages=self.V[layer])
+        return tree_attention(q, self.K[layer], self.V[layer], self.lens, tree_mask=mask, block_table=self.table), k
+
     def grow(self, lens, new_lens, max_new):
         """Pages for requests of these lengths, and the slots of their new tokens. Rows without a
         page would be left out and not seen, so a pool or a table that is too small ends the loop."""
@@ -128,36 +145,59 @@ class PagedCaches:
                 self.lens = keep_len.clone()
                 slots = self.grow(self.lens, None, most)
             for b, (_, k, v) in enumerate(outs):  # rows past keep_len have slot -1
-                store_rows(k, v, slots[b:b + 1, :k.shape[2]], self.K[layer], self.V[layer])
+                self.store(layer, k, v, slots[b:b + 1, :k.shape[2]])
         return torch.stack([logits for _, logits in prefilled])
 
     def verify(self, tokens, parents):
-        """One pass of the decoder over drafted trees (tokens, parents [B, T]): logits of
-        every node [B, T, vocab], and a function that keeps accepted nodes."""
+        """One pass of the decoder over drafted trees (tokens, parents [B, T]; None: chains):
+        logits of every node [B, T, vocab], and a function that keeps accepted nodes."""
         m, T = self.model, tokens.shape[1]
-        mask, depth = tree_mask_from_parents(parents)
+        if parents is None:
+            mask, depth = None, torch.arange(T, device=m.device)
+        else:
+            mask, depth = tree_mask_from_parents(parents)
         slots = self.grow(self.lens + T, torch.full_like(self.lens, T), T)
         positions = self.seen[:, None] + depth
         x, rows = m.embed[tokens], []
         for layer, w in enumerate(m.w):
             q, k, v = m.project(x, w)
-            q, k = qk_norm_rope(q, k, m.cos, m.sin, positions, q_weight=w["qn"], k_weight=w["kn"], V=v, slots=slots,
-                                K_pages=self.K[layer], V_pages=self.V[layer])
-            o = tree_attention(q, self.K[layer], self.V[layer], self.lens, tree_mask=mask, block_table=self.table)
+            o, k = self.attend(layer, q, k, v, positions, slots, mask)
             x = m.after(x, o, w)
             rows.append((k, v))
 
         def keep(place):
             """place [B, T]: a node's place among the accepted ones, or -1. Their rows move to
-            the front of the nodes' slots; the others are forgotten."""
-            to = torch.where(place >= 0, torch.gather(slots, 1, place.clamp(min=0)), -1)
-            for layer, (k, v) in enumerate(rows):
-                store_rows(k, v, to, self.K[layer], self.V[layer])
+            the front of the nodes' slots (a chain's are there); the others are forgotten."""
+            if parents is not None:
+                to = torch.where(place >= 0, torch.gather(slots, 1, place.clamp(min=0)), -1)
+                for layer, (k, v) in enumerate(rows):
+                    self.store(layer, k, v, to)
             taken = (place >= 0).sum(1)
             self.lens = self.lens + taken.int()
             self.seen = self.seen + taken
 
         return m.norm(x) @ m.head, keep
+
+
+class PagedCaches8(PagedCaches):
+    """The same with pages in 8 bits and a scale for each page and head."""
+
+    def __init__(self, model: Decoder, batch: int, pages: int, block: int = 16, max_blocks: int = 64):
+        super().__init__(model, batch, pages, block, max_blocks)
+        self.K = [k.to(torch.float8_e4m3fn) for k in self.K]
+        self.V = [v.to(torch.float8_e4m3fn) for v in self.V]
+        scales = lambda: [torch.ones(pages, model.Hkv, device=model.device) for _ in range(model.layers)]  # noqa: E731
+        self.K_scales, self.V_scales = scales(), scales()
+
+    def store(self, layer, k, v, slots):
+        store_rows_fp8(k, v, slots, self.K[layer], self.V[layer], self.K_scales[layer], self.V_scales[layer])
+
+    def attend(self, layer, q, k, v, positions, slots, mask):
+        m, w = self.model, self.model.w[layer]
+        q, k = qk_norm_rope(q, k, m.cos, m.sin, positions, q_weight=w["qn"], k_weight=w["kn"])
+        self.store(layer, k, v, slots)
+        return attention_fp8(q, self.K[layer], self.V[layer], self.K_scales[layer], self.V_scales[layer], self.lens,
+                             self.table, tree_mask=mask), k
 
 
 def draft_tree(root, followers, T):
@@ -193,6 +233,36 @@ def accept(tokens, parents, choice):
     return place, depth + 1, torch.gather(choice, 1, last[:, None])[:, 0]
 
 
+def draft_chain(root, logits, T, temperature):
+    """Tokens [B, T + 1]: the next token [B] and T after it, each drawn from the draft's
+    logits ([vocab, vocab]) of the one before."""
+    tokens = [root]
+    for _ in range(T):
+        tokens.append(torch.multinomial((logits[tokens[-1]].float() / temperature).softmax(-1), 1)[:, 0])
+    return torch.stack(tokens, 1)
+
+
+def sample(model, prompts, steps, drafted, temperature=1.0, keep_ratio=0.3, pages=512, block=16):
+    """Continuations drawn at a temperature, over caches in 8 bits: (list of token lists,
+    tokens a step)."""
+    caches = PagedCaches8(model, len(prompts), pages, block)
+    last = caches.load(prompts, keep_ratio)
+    B, out = len(prompts), [[] for _ in prompts]
+    none = torch.empty(B, 0, dtype=torch.int64, device=model.device)
+    root = verify_draft(last[:, None], none, torch.rand(B, 1, device=model.device), temperature=temperature).next_token
+    for _ in range(steps):
+        tokens = draft_chain(root, model.draft, drafted, temperature)
+        logits, keep = caches.verify(tokens, None)
+        v = verify_draft(logits, tokens[:, 1:], torch.rand(B, drafted + 1, device=model.device),
+                         draft_logits=model.draft[tokens[:, :-1]], temperature=temperature)
+        at = torch.arange(drafted + 1, device=model.device)
+        keep(torch.where(at <= v.accepted[:, None], at, -1))
+        root = v.next_token
+        for b, (n, row) in enumerate(zip(v.accepted.tolist(), tokens.tolist())):
+            out[b] += row[:n + 1]
+    return out, sum(map(len, out)) / (steps * B)
+
+
 def decode(model, prompts, steps, tree, keep_ratio=0.3, pages=512, block=16):
     """Greedy continuation of the prompts: (list of token lists, tokens a step)."""
     caches = PagedCaches(model, len(prompts), pages, block)
@@ -214,11 +284,17 @@ def main():
     ap.add_argument("--steps", type=int, default=8)
     ap.add_argument("--tree", type=int, default=16)
     ap.add_argument("--layers", type=int, default=4)
+    ap.add_argument("--sample", type=float, metavar="T", help="draw tokens at this temperature, over caches in 8 bits")
+    ap.add_argument("--drafted", type=int, default=4, help="tokens drafted a step with --sample")
     a = ap.parse_args()
     model = Decoder(layers=a.layers)
     g = torch.Generator(device="cuda").manual_seed(1)
     prompts = [torch.randint(0, model.vocab, (n,), generator=g, device="cuda") for n in (300, 47, 512)]
-    out, rate = decode(model, prompts, a.steps, a.tree)
+    if a.sample is not None:
+        torch.manual_seed(2)
+        out, rate = sample(model, prompts, a.steps, a.drafted, a.sample)
+    else:
+        out, rate = decode(model, prompts, a.steps, a.tree)
     for p, o in zip(prompts, out):
         print(f"prompt of {len(p)}: {o}")
     print(f"{rate:.2f} tokens a step and sequence")
