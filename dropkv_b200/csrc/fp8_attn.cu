@@ -313,7 +313,11 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           uint64_t* full = &bars[(kv ? L::B_VF : L::B_KF) + slot];
           if (turn) ok = __all_sync(0xffffffffu, wait(&bars[(kv ? L::B_VE : L::B_KE) + slot], turn - 1, 1 + kv));
           if (!ok) break;
-          if (kv == 0) {
+          if (lane == 0) tc::mbar_expect_tx(full, L::TILE);
+          __syncwarp();
+          if (lane < boxes)
+            tc::tma_load_4d(sm + (kv ? L::V : L::K) + slot * L::TILE + lane * box * D, kv ? &vmap : &kmap, full, 0, row, p.h, at);
+          if (kv == 0) {  // (the scales are on their way as the tile is)
             const float ks0 = __shfl_sync(0xffffffffu, ks, 0), vs0 = __shfl_sync(0xffffffffu, vs, 0);
             const int j0 = p.k.first(t);
             const bool there = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks > 0.f && vs > 0.f));
@@ -329,13 +333,9 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
               s[FA_HALVES] = vs;
               if (lane == 0) kinds[place] = FaKind{kind, vmax};
             }
-            __syncwarp();  // (who sees K's or V's tile land sees the scales)
           }
-          if (lane == 0) tc::mbar_arrive_expect_tx(full, L::TILE);
-          __syncwarp();
-          if (lane < boxes)
-            tc::tma_load_4d(sm + (kv ? L::V : L::K) + slot * L::TILE + lane * box * D, kv ? &vmap : &kmap, full, 0, row, p.h, at);
-          __syncwarp();
+          __syncwarp();  // (who sees K's or V's tile land sees the scales)
+          if (lane == 0) tc::mbar_arrive(full);
         }
         if (!ok) break;
         if (++slot == NS) slot = 0, ++turn;
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             }
           } else {
             // eight keys at a time, S read twice (rolled, as this is what few tiles are)
-            const uint64_t see = sees.bits(A, p.b, p.k.len, p.k.first(t), TK);
+            const uint64_t see = sees.template bits<TK>(A, p.b, p.k.len, p.k.first(t));
             __syncwarp();
             float top = -INFINITY;
             auto eight = [&](int y, float* z) {  // logits
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           const uint8_t* vb = static_cast<const uint8_t*>(a.pool.v) + h * a.pool.v_sh;
           for (int t = t0; t < t1; ++t) {
             const int j0 = keys.first(t);
-            uint64_t todo = saw.bits(A, b, keys.len, j0, TK);
+            uint64_t todo = saw.template bits<TK>(A, b, keys.len, j0);
             while (todo) {
               const int key = j0 + __ffsll((long long)todo) - 1;
               todo &= todo - 1;
@@ -743,33 +743,37 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
 constexpr int FM_NT = 256;
 constexpr int FM_AHEAD = 8;  // partials on their way at once
 
-// Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, groups of
-// eight rows); a warp has a row, a lane four of its columns. With M the largest of the partials' maxima and
+// Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, or, where FEW rows
+// make few blocks, the CTAs that they may begin in; groups of eight rows); a warp has a row, a lane four of its columns. With M the largest of the partials' maxima and
 // w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs. Bound by the
 // latency of its loads, from L2.
-template <typename T, int D>
+template <typename T, int D, bool FEW>
 __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A, int ctas) {
-  __shared__ int counts[FM_NT / 32], pick;
+  __shared__ int counts[FM_NT / 32], found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * (FM_NT / 32) + warp;
-  if (threadIdx.x == 0) pick = -1;
+  if (!FEW && threadIdx.x == 0) found = -1;
   // every CTA waits for the kernel before this one, with work or without: what comes after on the
   // stream takes this kernel's end for the end of both
   pdl_wait();
-  // the CTA in which the blockIdx.x-th split segment begins
-  for (int c0 = 0, before = 0; c0 < ctas; c0 += FM_NT) {
-    const int at = c0 + threadIdx.x;
-    const bool splits = at < ctas && A.meta[at].w > 0;
-    const unsigned some = __ballot_sync(0xffffffffu, splits);
-    if (lane == 0) counts[warp] = __popc(some);
-    __syncthreads();
-    for (int w = 0; w < FM_NT / 32; ++w) {
-      if (w == warp && splits && before + __popc(some & ((1u << lane) - 1)) == (int)blockIdx.x) pick = at;
-      before += counts[w];
+  int pick = blockIdx.x;
+  if (!FEW) {  // the CTA in which the blockIdx.x-th split segment begins
+    for (int c0 = 0, before = 0; c0 < ctas; c0 += FM_NT) {
+      const int at = c0 + threadIdx.x;
+      const bool splits = at < ctas && A.meta[at].w > 0;
+      const unsigned some = __ballot_sync(0xffffffffu, splits);
+      if (lane == 0) counts[warp] = __popc(some);
+      __syncthreads();
+      for (int w = 0; w < FM_NT / 32; ++w) {
+        if (w == warp && splits && before + __popc(some & ((1u << lane) - 1)) == (int)blockIdx.x) found = at;
+        before += counts[w];
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    pick = found;
+    if (pick < 0) return;
   }
-  if (pick < 0) return;
   const int4 seg = A.meta[pick];
+  if (seg.w == 0) return;
   const int n = seg.w, n0 = seg.z * A.npr, rows = (min(n0 + A.npr, A.a.T) - n0) * A.g;
   if (row >= rows) return;
   auto slot = [&](int i) { return 2 * ((int64_t)pick + i) + (i == 0 ? 1 : 0); };
@@ -822,6 +826,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
 template <typename T, int D>
 int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   const int64_t segments = (int64_t)A.a.B * A.RT * A.a.Hkv;
+  const bool few = A.rows_pad <= kFp8DecodeRows;  // (a block for each CTA: no list to look through first)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -829,9 +834,9 @@ int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>(ctas, segments), (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
+  cfg.gridDim = dim3((unsigned)(few ? ctas : std::min<int64_t>(ctas, segments)), (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
   cfg.blockDim = dim3(FM_NT);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_merge_kernel<T, D>, A, ctas);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? fp8_merge_kernel<T, D, true> : fp8_merge_kernel<T, D, false>, A, ctas);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 merge launch: %s", cudaGetErrorString(e));
   return check_launch("attention_fp8_merge");
 }

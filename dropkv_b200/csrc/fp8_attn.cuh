@@ -92,8 +92,11 @@ struct Sees {
     lo = a.window ? (int)min(max((int64_t)len + depth - a.window + 1, (int64_t)0), (int64_t)a.cap) : 0;
     hi = a.mask ? keys : (int)min((int64_t)len + node + 1, (int64_t)keys);
   }
-  // bit e: key j0 + e is seen (count at most 64)
-  __device__ __forceinline__ uint64_t bits(const Args& A, int b, int len, int j0, int count) const {
+  // bit e: key j0 + e is seen
+  template <int COUNT>
+  __device__ __forceinline__ uint64_t bits(const Args& A, int b, int len, int j0) const {
+    constexpr int count = COUNT;
+    static_assert(COUNT <= 64 && COUNT % 8 == 0, "keys");
     const AttnFp8& a = A.a;
     auto below = [&](int n) -> uint64_t { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1); };
     uint64_t m = below(hi - j0) & below(count);
@@ -106,20 +109,18 @@ struct Sees {
     if (m & ~cached) {
       // (many loads on their way at once: a truth value at a time takes as many trips to memory)
       if (A.mask_vec) {
-#pragma unroll 1
-        for (int i0 = 0; i0 <= count / 4; i0 += 8) {
-          uint32_t x[8];
+        constexpr int WORDS = COUNT / 4 + 1;
+        uint32_t x[WORDS];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int n = (n0 & ~3) + 4 * (i0 + i);
-            x[i] = n >= 0 && n < a.T ? *reinterpret_cast<const uint32_t*>(row + n) : 0u;
-          }
+        for (int i = 0; i < WORDS; ++i) {
+          const int n = (n0 & ~3) + 4 * i;
+          x[i] = n >= 0 && n < a.T ? *reinterpret_cast<const uint32_t*>(row + n) : 0u;
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {  // four truth values to four bits
-            const int at = 4 * (i0 + i) - (n0 & 3);
-            const uint64_t four = ((__vcmpne4(x[i], 0u) & 0x01010101u) * 0x10204080u) >> 28;
-            nodes |= at < 0 ? four >> -at : (at < 64 ? four << at : 0ull);
-          }
+        for (int i = 0; i < WORDS; ++i) {  // four truth values to four bits
+          const int at = 4 * i - (n0 & 3);
+          const uint64_t four = ((__vcmpne4(x[i], 0u) & 0x01010101u) * 0x10204080u) >> 28;
+          nodes |= at < 0 ? four >> -at : (at < 64 ? four << at : 0ull);
         }
       } else {
 #pragma unroll 1

@@ -183,17 +183,17 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
           const uint32_t slot = n % NS;
           if (n >= (uint32_t)NS) ok = __all_sync(0xffffffffu, wait(&empty[slot], n / NS - 1, 1));
           if (!ok) break;
-          if (kv == 0 && lane < FD_HALVES) {
+          if (lane == 0) tc::mbar_expect_tx(&full[slot], S::TILE);
+          __syncwarp();
+          if (lane < boxes)
+            tc::tma_load_4d(sm + slot * S::TILE + lane * box * D, kv ? &vmap : &kmap, &full[slot], 0, row, p.h, at);
+          if (kv == 0 && lane < FD_HALVES) {  // (on their way as the tile is; who sees K land sees them)
             float* s = sc + (n / 2 % S::SCALES) * (2 * FD_HALVES) + lane;
             s[0] = ks;
             s[FD_HALVES] = vs;
           }
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive_expect_tx(&full[slot], S::TILE);
-          __syncwarp();
-          if (lane < boxes)
-            tc::tma_load_4d(sm + slot * S::TILE + lane * box * D, kv ? &vmap : &kmap, &full[slot], 0, row, p.h, at);
-          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&full[slot]);
         }
         if (!ok) break;
         page = page1, page1 = page2, ks = ks1, vs = vs1;
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
           seen = 0;
 #pragma unroll
           for (int x = 0; x < HR; ++x) {
-            uint32_t see = (uint32_t)sees[x].bits(A, p.b, p.k.len, j0, 32);
+            uint32_t see = (uint32_t)sees[x].template bits<32>(A, p.b, p.k.len, j0);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               if (!(ks[y] > 0.f)) see &= ~(0xffu << (8 * y));

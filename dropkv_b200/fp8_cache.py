@@ -29,6 +29,8 @@ from .paged import _ints, _new, _on_its_device, _on_one_device, _raw_stream, _ro
 
 __all__ = ["store_rows_fp8", "load_rows_fp8", "attention_fp8"]
 
+_F8, _F32 = torch.float8_e4m3fn, torch.float32
+
 
 @functools.lru_cache(maxsize=4096)
 def _attention_workspace(index: int, B: int, Hq: int, Hkv: int, T: int, D: int, cap: int) -> int:
@@ -42,13 +44,13 @@ def _check_pool_fp8(K_pages, V_pages, K_scales, V_scales):
     if len(shape) != 4 or shape != V_pages.shape:
         raise ValueError(f"expected K and V pages [pages, Hkv, block_size, D] of one shape, got {tuple(shape)} and "
                          f"{tuple(V_pages.shape)}")
-    if K_pages.dtype != torch.float8_e4m3fn or V_pages.dtype != torch.float8_e4m3fn:
+    if K_pages.dtype != _F8 or V_pages.dtype != _F8:
         raise TypeError(f"pages must be torch.float8_e4m3fn, got {K_pages.dtype} and {V_pages.dtype}")
-    for s in (K_scales, V_scales):
-        if s.dtype != torch.float32:
-            raise TypeError(f"scales must be float32, got {s.dtype}")
-        if s.shape != shape[:2]:
-            raise ValueError(f"scales must be {tuple(shape[:2])} (pages, heads), got {tuple(s.shape)}")
+    if K_scales.dtype != _F32 or V_scales.dtype != _F32:
+        raise TypeError(f"scales must be float32, got {K_scales.dtype} and {V_scales.dtype}")
+    of = shape[:2]
+    if K_scales.shape != of or V_scales.shape != of:
+        raise ValueError(f"scales must be {tuple(of)} (pages, heads), got {tuple(K_scales.shape)} and {tuple(V_scales.shape)}")
     return shape, (K_pages.data_ptr(), *_rows_strides(K_pages, "K_pages"), V_pages.data_ptr(),
                    *_rows_strides(V_pages, "V_pages"), K_scales.data_ptr(), *K_scales.stride(), V_scales.data_ptr(),
                    *V_scales.stride())
@@ -108,7 +110,7 @@ def load_rows_fp8(K_pages: torch.Tensor, V_pages: torch.Tensor, K_scales: torch.
     slots = _ints(slots, torch.int64, (B, N), "slots")
     device = K_pages.device
     k_out = _new(dtype, device, B, ps[1], N, ps[3])
-    v_out = _new(dtype, device, B, ps[1], N, ps[3])
+    v_out = torch.empty_like(k_out)
     rc = _lib.load().dropkv_load_rows_fp8(*pool, ps[0], ps[2], slots.data_ptr(), dt, B, ps[1], N, ps[3], k_out.data_ptr(),
                                           v_out.data_ptr(), _raw_stream(dev))
     if rc:

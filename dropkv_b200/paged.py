@@ -483,7 +483,8 @@ def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, uniforms: to
         rows.append(x)
     target, draft = rows
     device = target.device
-    out = VerifiedDraft(_new(torch.int64, device, B), _new(torch.int64, device, B), _new(torch.float32, device, B, T))
+    accepted = _new(torch.int64, device, B)
+    out = VerifiedDraft(accepted, torch.empty_like(accepted), _new(torch.float32, device, B, T))
     if B == 0:
         return out
     need = max(_verify_workspace(dev, B, T, V, draft is not None), 1)
