@@ -236,8 +236,8 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     tc::tma_prefetch_desc(&kmap);
     tc::tma_prefetch_desc(&vmap);
   }
-  pdl_wait();
-  pdl_launch_dependents();  // (after the wait: the merge may then read this kernel's inputs at once)
+  // Of the kernel before this one only the queries' parts and units are needed, and only who reads them waits for it:
+  // it let this one begin once all before it was over.
   if (warp == 0) find_start<TK>(A, lane, start);
   tc::tc_fence_before();
   __syncthreads();
@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     walk.start(*start);
     uint32_t n = 0, slot = 0, turn = 0, place = 0, queries = 0;
     bool ok = true;
+    pdl_wait();
     while (ok && walk.next(A, p)) {
       // the piece's queries, once the products that read the last piece's are done: those with its last tile of K
       if (n) ok = __all_sync(0xffffffffu, wait(&bars[L::B_KE + (n - 1) % NS], (n - 1) / NS, 8));
@@ -478,6 +479,8 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   } else {
     // ======================= softmax ============================================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    pdl_wait();
+    pdl_launch_dependents();
     const uint32_t lanes = (uint32_t)(warp * 32) << 16, to = tmem + lanes + 128;
     const int r = tid;
     WarpWalk<TK>& ww = reinterpret_cast<WarpWalk<TK>*>(sm + L::WALKS)[warp];
@@ -698,7 +701,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           }
         }
         T* dst = static_cast<T*>(a.out) + out_row(A, b, h, n0, own ? r : 0) * D;
-        float* part = A.part_o + (slot * A.rows_pad + r) * D;
+        float4* part = reinterpret_cast<float4*>(A.part_o + slot * A.rows_pad * D) + r;  // (32 rows of a vector, side by side)
 #pragma unroll 1
         for (int w = 0; w < D / 32; ++w) {
           float o[32];
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           } else {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(part + 32 * w + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              part[(8 * w + e / 4) * A.rows_pad] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         if (own && !whole) {
@@ -744,13 +747,16 @@ constexpr int FM_NT = 256;
 constexpr int FM_AHEAD = 8;  // partials on their way at once
 
 // Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, or, where FEW rows
-// make few blocks, the CTAs that they may begin in; groups of eight rows); a warp has a row, a lane four of its columns. With M the largest of the partials' maxima and
-// w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs. Bound by the
-// latency of its loads, from L2.
+// make few blocks, the CTAs that they may begin in; groups of eight rows). With M the largest of the partials' maxima
+// and w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs: a warp takes a row's weights, then a
+// thread four columns of a row, as they lie: of FEW rows a row's vectors side by side, else eight rows' of a vector (who
+// wrote them had a row a thread). Bound by the latency of its loads, from L2.
 template <typename T, int D, bool FEW>
 __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A, int ctas) {
-  __shared__ int counts[FM_NT / 32], found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * (FM_NT / 32) + warp;
+  constexpr int ROWS = FM_NT / 32;
+  __shared__ int counts[ROWS], found;
+  __shared__ float weights[ROWS][33], before_[ROWS];  // of 32 partials; what those before them are scaled by
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (!FEW && threadIdx.x == 0) found = -1;
   // every CTA waits for the kernel before this one, with work or without: what comes after on the
   // stream takes this kernel's end for the end of both
@@ -763,7 +769,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
       const unsigned some = __ballot_sync(0xffffffffu, splits);
       if (lane == 0) counts[warp] = __popc(some);
       __syncthreads();
-      for (int w = 0; w < FM_NT / 32; ++w) {
+      for (int w = 0; w < ROWS; ++w) {
         if (w == warp && splits && before + __popc(some & ((1u << lane) - 1)) == (int)blockIdx.x) found = at;
         before += counts[w];
       }
@@ -774,12 +780,18 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
   }
   const int4 seg = A.meta[pick];
   if (seg.w == 0) return;
-  const int n = seg.w, n0 = seg.z * A.npr, rows = (min(n0 + A.npr, A.a.T) - n0) * A.g;
-  if (row >= rows) return;
+  const int n = seg.w, n0 = seg.z * A.npr, rows = (min(n0 + A.npr, A.a.T) - n0) * A.g, row0 = blockIdx.y * ROWS;
+  if (row0 + (FEW ? warp : 0) >= rows) return;
   auto slot = [&](int i) { return 2 * ((int64_t)pick + i) + (i == 0 ? 1 : 0); };
-  const float* ml = A.part_ml + row;
-  const int c = 4 * (lane % (D / 4));
-  const float* po = A.part_o + (int64_t)row * D + c;
+  const float* ml = A.part_ml + row0 + warp;
+  const int r = FEW ? warp : threadIdx.x % ROWS, c = FEW ? lane % (D / 4) : min((int)threadIdx.x / ROWS, D / 4 - 1);
+  const float4* po = reinterpret_cast<const float4*>(A.part_o) + (FEW ? (row0 + r) * (D / 4) + c : c * A.rows_pad + row0 + r);
+  auto sync = [&]() {
+    if (FEW)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
   float sum = 0.f, top = -INFINITY;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = 0; i0 < n; i0 += 32) {
@@ -787,12 +799,11 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
     float4 x[FM_AHEAD];
     auto load = [&](int i, float4* to) {
 #pragma unroll
-      for (int u = 0; u < FM_AHEAD; ++u)
-        to[u] = __ldcg(reinterpret_cast<const float4*>(po + slot(i0 + min(i + u, cnt - 1)) * A.rows_pad * D));
+      for (int u = 0; u < FM_AHEAD; ++u) to[u] = __ldcg(po + slot(i0 + min(i + u, cnt - 1)) * A.rows_pad * (D / 4));
     };
     load(0, x);  // (beside the maxima and sums)
     float m = -INFINITY, w = 0.f;
-    if (lane < cnt) {
+    if (lane < cnt && row0 + warp < rows) {
       const float* pm = ml + slot(i0 + lane) * 2 * A.rows_pad;
       m = __ldcg(pm);
       w = __ldcg(pm + A.rows_pad);
@@ -801,25 +812,28 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mx = fmaxf(mx, top);
-    const float f0 = top == mx ? 1.f : ex2(top - mx);  // of what was joined before
+    if (lane == 0) before_[warp] = top == mx ? 1.f : ex2(top - mx);
     top = mx;
-    w *= m == top ? 1.f : ex2(m - top);
+    weights[warp][lane] = w * (m == top ? 1.f : ex2(m - top));
+    sync();
+    const float f0 = before_[r];
     sum *= f0;
     y.x *= f0, y.y *= f0, y.z *= f0, y.w *= f0;
     for (int i = 0; i < cnt; i += FM_AHEAD) {
       if (i) load(i, x);
 #pragma unroll
       for (int u = 0; u < FM_AHEAD; ++u) {
-        const float f = __shfl_sync(0xffffffffu, w, min(i + u, 31));
         if (i + u >= cnt) continue;
+        const float f = weights[r][i + u];
         sum += f;
         y.x = fmaf(x[u].x, f, y.x), y.y = fmaf(x[u].y, f, y.y), y.z = fmaf(x[u].z, f, y.z), y.w = fmaf(x[u].w, f, y.w);
       }
     }
+    sync();
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (lane < D / 4)
-    *reinterpret_cast<uint2*>(static_cast<T*>(A.a.out) + out_row(A, seg.x, seg.y, n0, row) * D + c) =
+  if (row0 + r < rows && (FEW ? lane < D / 4 : threadIdx.x < ROWS * (D / 4)))
+    *reinterpret_cast<uint2*>(static_cast<T*>(A.a.out) + out_row(A, seg.x, seg.y, n0, row0 + r) * D + 4 * c) =
         make_uint2(Out<T>::pack(y.x * inv, y.y * inv), Out<T>::pack(y.z * inv, y.w * inv));
 }
 

@@ -29,7 +29,7 @@ struct Args {
   float scale_log2;
   int* status;       // [CTAs]: 0, or which wait gave up
   int4* meta;        // [CTAs]: the split segment that begins in a CTA: b, KV head, row tile, its partials (0: none)
-  float* part_o;     // [2 CTAs][rows_pad][D]
+  float* part_o;     // [2 CTAs][rows_pad][D]; many rows: [2 CTAs][D / 4][rows_pad][4]
   float* part_ml;    // [2 CTAs][2][rows_pad]
   float* units;      // [row tiles][128]: what a unit of a row's queries makes of a logit, in base 2 (many rows)
   uint8_t* queries;  // [row tiles][parts][128][D]: 8-bit parts of the queries, as the products read them
