@@ -894,6 +894,10 @@ int fa_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
   if (!done.done(dev)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES) != cudaSuccess)
       return fail(DROPKV_ERR_CUDA, "cannot set attention_fp8 shared memory size %d", L::BYTES);
+    // the split of registers between the warps counts on this many at launch: with fewer it would wait forever
+    cudaFuncAttributes attrs;
+    if (cudaFuncGetAttributes(&attrs, kern) != cudaSuccess || attrs.numRegs * FA_NT < (168 + 88) * 128)
+      return fail(DROPKV_ERR_CUDA, "attention_fp8 was compiled for too few registers");
     done.mark(dev);
   }
   cudaLaunchConfig_t cfg = {};
