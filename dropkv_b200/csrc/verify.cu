@@ -36,8 +36,9 @@ constexpr int VD_SEGS = 256;      // segments of a row, at most
 constexpr int VF_MAX_T = 256;
 // fp32's sums and exponentials are off by less than this in the logarithm of a ratio (sums of positive terms over 256 threads and
 // up to 32 chunks: 2^-17 at most; 2^x within 2^-22, of exponents off by 2^-23 of themselves).
-constexpr double kVfUnsure = 4e-5;
-constexpr double kVfLeast = -745.0;  // log of a probability under what 64 bits hold
+constexpr float kVfUnsure = 4e-5f;
+// Log of a probability under what 64 bits hold: that is 0, and a token with p of 0 is not accepted, whatever q says.
+constexpr double kVfLeast = -745.0;
 
 struct VfArgs {
   const char* target;  // [B, T + 1, V], strides in elements
@@ -205,6 +206,12 @@ struct VdSmem {
   int8_t what[VF_MAX_T];    // of a drafted token
 };
 
+// Log of a probability: of a word's logit over the largest, and the sum of the row's weights.
+__device__ __forceinline__ double vf_log(double over, double sum) {
+  const double l = over - log(sum);
+  return l < kVfLeast ? -INFINITY : l;
+}
+
 // Where value i of a list of 256 lies: eight a lane then meet all banks.
 __device__ __forceinline__ int vd_at(int i) { return i + (i >> 3); }
 
@@ -278,42 +285,61 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   // ---- the rows' maxima and sums, and what becomes of the drafted tokens ---------
   const double per = a.c64 * LN2;  // 1 / tau
   for (int i = warp; i <= a.T; i += VD_WARPS) {
-    double lse[2] = {0.0, 0.0};
-    float tops[2] = {0.f, 0.f};
+    float tops[2] = {0.f, 0.f}, sums[2] = {1.f, 1.f};
     const bool two = a.draft && i < a.T;
+    float2 w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      w[k] = lane < a.S && (k == 0 || two) ? a.part[vf_index(a, b, i, k) * a.S + lane] : make_float2(-INFINITY, 0.f);
+    int64_t x = -1;
+    float xp = 0.f, xq = 0.f, u = 0.f;
+    if (lane == 0 && i < a.T) {  // (beside the chunks')
+      x = a.tokens[(int64_t)b * a.T + i];
+      u = a.uniforms[(int64_t)b * (a.T + 1) + i];
+      if (x >= 0 && x < a.V) {
+        xp = to_f(vf_row<T>(a, b, i, false)[x]);
+        if (two) xq = to_f(vf_row<T>(a, b, i, true)[x]);
+      }
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (k && !two) break;
-      const float2 w = lane < a.S ? a.part[vf_index(a, b, i, k) * a.S + lane] : make_float2(-INFINITY, 0.f);
-      float m = w.x;
+      float m = w[k].x;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      float s = w.x == -INFINITY ? w.y : w.y * vf_ex2((w.x - m) * a.c);
+      float s = w[k].x == -INFINITY ? w[k].y : w[k].y * vf_ex2((w[k].x - m) * a.c);
       if (m == INFINITY) s = NAN;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       tops[k] = m;
-      lse[k] = s > 0.f && s <= 3.4e38f ? log((double)s) : NAN;  // (a sum of 0: nothing but -inf)
+      sums[k] = s > 0.f && s <= 3.4e38f ? s : NAN;  // (a sum of 0: nothing but -inf)
     }
     if (lane == 0) {
-      sm.mp[i] = isnan(lse[0]) ? NAN : tops[0];
-      sm.mq[i] = isnan(lse[1]) ? NAN : tops[1];
+      sm.mp[i] = isnan(sums[0]) ? NAN : tops[0];
+      sm.mq[i] = isnan(sums[1]) ? NAN : tops[1];
       if (i < a.T) {
-        const int64_t x = a.tokens[(int64_t)b * a.T + i];
         int what = VD_END;
         float prob = 0.f;
         if (x >= 0 && x < a.V) {
-          double lp = ((double)to_f(vf_row<T>(a, b, i, false)[x]) - tops[0]) * per - lse[0];
-          double lq = two ? ((double)to_f(vf_row<T>(a, b, i, true)[x]) - tops[1]) * per - lse[1] : 0.0;
-          // what 64 bits hold no number for is 0: a token with p of 0 is not accepted, whatever q says
-          if (lp < kVfLeast) lp = -INFINITY;
-          if (lq < kVfLeast) lq = -INFINITY;
-          const double d = lp == -INFINITY && !isnan(lq) ? -INFINITY : lp - lq;
-          const double lu = log((double)a.uniforms[(int64_t)b * (a.T + 1) + i]);
-          prob = d >= 0.0 ? 1.f : (float)exp(d);
-          what = lu < d ? VD_ACCEPT : VD_REJECT;
-          if (fabs(lu - d) < kVfUnsure) what = VD_UNSURE;
-          if (isnan(d)) what = VD_NONE, prob = NAN;
+          const double dp = ((double)xp - tops[0]) * per, dq = two ? ((double)xq - tops[1]) * per : 0.0;
+          if (isnan(sums[0]) || isnan(sums[1])) {
+            what = VD_NONE;
+            prob = NAN;
+          } else if (dp > -700.0 && dq > -700.0) {  // p / q, without a logarithm (in 64 bits one takes longer than a row's sums)
+            const double d = dp - dq;
+            const float hi = fminf((float)d, 80.f), e = expf(hi);
+            const float ratio = hi == 80.f ? INFINITY : fmaf(e, (float)(d - hi), e) * (sums[1] / sums[0]);
+            prob = fminf(ratio, 1.f);
+            what = u < ratio ? VD_ACCEPT : VD_REJECT;
+            // where fp32 cannot tell; where its range ends, too
+            if (ratio < INFINITY && (fabsf(u - ratio) <= kVfUnsure * fmaxf(u, ratio) || fmaxf(u, ratio) < 1e-29f)) what = VD_UNSURE;
+          } else {
+            const double lp = vf_log(dp, sums[0]), lq = two ? vf_log(dq, sums[1]) : 0.0;
+            const double d = lp == -INFINITY ? -INFINITY : lp - lq, lu = log((double)u);
+            prob = d >= 0.0 ? 1.f : (float)exp(d);
+            what = lu < d ? VD_ACCEPT : VD_REJECT;
+            if (fabs(lu - d) < kVfUnsure) what = VD_UNSURE;
+          }
         }
         sm.what[i] = (int8_t)what;
         if (rank == 0) a.prob[(int64_t)b * a.T + i] = prob;
@@ -355,9 +381,33 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   };
   // sums of weights of p's row and, unless it is NULL, of q's over the whole vocabulary
   auto sum_rows = [&](const T* x, float mx, const T* y, float my, double* zx, double* zy) {
-    const double sx = walk(x, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, mx); });
-    double sy = 0.0;
-    if (y) sy = walk(y, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, my); });
+    double sx = 0.0, sy = 0.0;
+    if (VD_WARPS == 16) {  // few words a lane: both rows' on their way at once
+      constexpr int AHEAD = 4;
+      for (int e0 = lo + lane; e0 < hi; e0 += 32 * AHEAD) {
+        T u[AHEAD], v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          if (e0 + 32 * k >= hi) continue;
+          u[k] = x[e0 + 32 * k];
+          if (y) v[k] = y[e0 + 32 * k];
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          if (e0 + 32 * k >= hi) continue;
+          sx += weight(to_f(u[k]), mx);
+          if (y) sy += weight(to_f(v[k]), my);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        sx += __shfl_xor_sync(0xffffffffu, sx, o);
+        sy += __shfl_xor_sync(0xffffffffu, sy, o);
+      }
+    } else {
+      sx = walk(x, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, mx); });
+      if (y) sy = walk(y, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, my); });
+    }
     if (lane == 0) sm.seg[0][warp] = sx, sm.seg[1][warp] = sy;
     cluster.sync();
     *zy = y ? gather(1) : 1.0;
@@ -373,9 +423,10 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
       const T *xp = vf_row<T>(a, b, n, false), *xq = a.draft ? vf_row<T>(a, b, n, true) : nullptr;
       sum_rows(xp, sm.mp[n], xq, sm.mq[n], &zp, &zq);
       cluster.sync();  // (who reads a CTA's sums is done with them before they change)
-      const double lp = ((double)to_f(xp[x]) - sm.mp[n]) * per - log(zp);
-      const double lq = xq ? ((double)to_f(xq[x]) - sm.mq[n]) * per - log(zq) : 0.0;
-      what = log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]) < lp - lq ? VD_ACCEPT : VD_REJECT;
+      const double lp = vf_log(((double)to_f(xp[x]) - sm.mp[n]) * per, zp);
+      const double lq = xq ? vf_log(((double)to_f(xq[x]) - sm.mq[n]) * per, zq) : 0.0;
+      const bool taken = lp > -INFINITY && log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]) < lp - lq;
+      what = taken ? VD_ACCEPT : VD_REJECT;
     }
     if (what != VD_ACCEPT) break;
   }

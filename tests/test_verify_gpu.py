@@ -227,3 +227,32 @@ def test_what_is_kept_is_distributed_as_the_target():
     p = torch.softmax(t[0, 0].double(), -1)
     f = torch.bincount(first, minlength=V).double() / n
     assert bool(((f - p).abs() <= 6 * (p * (1 - p) / n).sqrt()).all())
+
+
+def test_the_largest_sizes():
+    t, tok, u, d = logits(1, 1, 1 << 21, torch.bfloat16, 40)
+    check(t, tok, u, d)
+    t, tok, u, d = logits(2, 256, 40, torch.float32, 41, noise=0.01)
+    check(t, tok, u, d)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_uniforms_and_probabilities_near_zero(draft):
+    """Acceptance where the ratio or the random number leaves fp32's range, and a number of 0, which accepts any token
+    whose probability 64 bits hold."""
+    gaps = [0.0, 30.0, 60.0, 69.0, 75.0, 88.0, 103.0, 500.0, 695.0, 705.0, 740.0, 760.0, math.inf]
+    zs = [0.0, 2.0 ** -149, 1e-38, 1e-30, 1e-29, 1e-26, 2.0 ** -24, 0.5, 1 - 2.0 ** -24]
+    B = len(gaps) * len(zs)
+    t = torch.zeros(B, 2, 5, device="cuda")
+    t[:, 0, 3] = -torch.tensor(gaps, device="cuda").repeat_interleave(len(zs))
+    u = torch.full((B, 2), 0.5, device="cuda")
+    u[:, 0] = torch.tensor(zs, device="cuda").repeat(len(gaps))
+    tok = torch.full((B, 1), 3, dtype=torch.int64, device="cuda")
+    d = None
+    if draft:
+        d = torch.zeros(B, 1, 5, device="cuda")
+        d[::2, 0, 3] = -40.0
+    got = verify_draft(t, tok, u, draft_logits=d)
+    for b in range(B):
+        n, nxt, _ = definition(t[b], tok[b], u[b], d[b] if draft else None, 1.0)
+        assert (int(got.accepted[b]), int(got.next_token[b])) == (n, nxt), (b, gaps[b // len(zs)], zs[b % len(zs)])
