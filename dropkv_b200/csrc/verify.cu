@@ -14,8 +14,8 @@
 // in 64 bits too.
 //
 // Measured: 64 drafts of up to 7 tokens over 151936 words in bf16, 292 MB: 115 us, of which the first launch takes 56 (80% of a
-// copy's rate) and the second 62; 4 of 5 tokens over 50257 words 23, most of it the second one's chain (join, sums over the
-// cluster, a second look, the search).
+// copy's rate) and the second 62; 4 of 5 tokens over 50257 words 20, 16 of 4 over 32000 without draft logits 14, most of it the
+// second one's chain (join, sums shared over the cluster, a second look where q has a row, the search).
 // 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and two terms of the exponential's series for what is left of x.
 #include <cooperative_groups.h>
 
@@ -199,8 +199,7 @@ template <int WARPS>
 struct VdSmem {
   double table[VD_TABLE];
   double root[96];          // 2^(i / 32), 2^(i / 2048)
-  double seg[3][WARPS];  // sums of this CTA's segments: of p's row, of q's, of what is drawn from
-  double all[VD_SEGS + VD_SEGS / 8];  // of all, as vd_at says
+  double all[3][VD_SEGS + VD_SEGS / 8];  // all segments' sums, as vd_at says: of p's row, of q's, of what is drawn from them
   double sub[WARPS + WARPS / 8];      // of parts of the segment, likewise
   float mp[VF_MAX_T + 1], mq[VF_MAX_T + 1];
   int8_t what[VF_MAX_T];    // of a drafted token
@@ -266,6 +265,7 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / ctas, segs = ctas * VD_WARPS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster.barrier_arrive();  // (waited for before the first write to another CTA: it has begun)
   if (tid < 96) sm.root[tid] = exp2(tid < 32 ? tid / 32.0 : (tid - 32) / 2048.0);
   __syncthreads();
   for (int i = tid; i < VD_TABLE; i += VD_NT) sm.table[i] = sm.root[i >> 6] * sm.root[32 + (i & 63)];
@@ -372,15 +372,12 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
   };
-  // All segments' sums of what the warps left in sm.seg[which]: into sm.all, and their sum.
-  auto gather = [&](int which) -> double {
-    __syncthreads();  // (sm.all has been read)
-    for (int i = tid; i < segs; i += VD_NT) sm.all[vd_at(i)] = cluster.map_shared_rank(&sm, i / VD_WARPS)->seg[which][i % VD_WARPS];
-    __syncthreads();
-    return vd_sum(sm.all, segs, lane);
+  // A warp's sum of its segment, to every CTA.
+  auto share = [&](int which, double s) {
+    if (lane < ctas) cluster.map_shared_rank(&sm, lane)->all[which][vd_at(rank * VD_WARPS + warp)] = s;
   };
-  // sums of weights of p's row and, unless it is NULL, of q's over the whole vocabulary
-  auto sum_rows = [&](const T* x, float mx, const T* y, float my, double* zx, double* zy) {
+  // sums of weights of p's row, a word left out, and, unless it is NULL, of q's over the whole vocabulary
+  auto sum_rows = [&](const T* x, float mx, int out, const T* y, float my, double* zx, double* zy) {
     double sx = 0.0, sy = 0.0;
     if (VD_WARPS == 16) {  // few words a lane: both rows' on their way at once
       constexpr int AHEAD = 4;
@@ -395,7 +392,7 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
           if (e0 + 32 * k >= hi) continue;
-          sx += weight(to_f(u[k]), mx);
+          sx += e0 + 32 * k == out ? 0.0 : weight(to_f(u[k]), mx);
           if (y) sy += weight(to_f(v[k]), my);
         }
       }
@@ -405,14 +402,16 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
         sy += __shfl_xor_sync(0xffffffffu, sy, o);
       }
     } else {
-      sx = walk(x, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, mx); });
+      sx = walk(x, static_cast<const T*>(nullptr), lo, hi, [&](int e, float u, float) { return e == out ? 0.0 : weight(u, mx); });
       if (y) sy = walk(y, static_cast<const T*>(nullptr), lo, hi, [&](int, float u, float) { return weight(u, my); });
     }
-    if (lane == 0) sm.seg[0][warp] = sx, sm.seg[1][warp] = sy;
+    share(0, sx);
+    if (y) share(1, sy);
     cluster.sync();
-    *zy = y ? gather(1) : 1.0;
-    *zx = gather(0);  // (p's segments stay in sm.all)
+    *zx = vd_sum(sm.all[0], segs, lane);
+    *zy = y ? vd_sum(sm.all[1], segs, lane) : 1.0;
   };
+  cluster.barrier_wait();
   // ---- which are accepted ----------------------------------------------------------
   int n = 0, what = VD_END;
   double zp, zq;
@@ -421,8 +420,8 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
     if (what == VD_UNSURE) {  // (the same in every thread of the cluster)
       const int64_t x = a.tokens[(int64_t)b * a.T + n];
       const T *xp = vf_row<T>(a, b, n, false), *xq = a.draft ? vf_row<T>(a, b, n, true) : nullptr;
-      sum_rows(xp, sm.mp[n], xq, sm.mq[n], &zp, &zq);
-      cluster.sync();  // (who reads a CTA's sums is done with them before they change)
+      sum_rows(xp, sm.mp[n], -1, xq, sm.mq[n], &zp, &zq);
+      cluster.sync();  // (all have read these sums before they change)
       const double lp = vf_log(((double)to_f(xp[x]) - sm.mp[n]) * per, zp);
       const double lq = xq ? vf_log(((double)to_f(xq[x]) - sm.mq[n]) * per, zq) : 0.0;
       const bool taken = lp > -INFINITY && log((double)a.uniforms[(int64_t)b * (a.T + 1) + n]) < lp - lq;
@@ -441,9 +440,10 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
     return;  // (all of the cluster)
   }
   // ---- the token after them --------------------------------------------------------
-  // Drawn from p its weights do as they are: the sums are there. From max(p - q, 0), a second look at both rows, by now in L2.
-  const int out = rejected && !a.draft ? (int)a.tokens[(int64_t)b * a.T + n] : -1;  // q's only word
-  sum_rows(xp, mp, xq, mq, &zp, &zq);
+  // Drawn from p its weights do as they are, but for the drafted token's where q is 1 at it: the sums are there. From
+  // max(p - q, 0), a second look at both rows, by now in L2.
+  const int out = rejected && !a.draft ? (int)a.tokens[(int64_t)b * a.T + n] : -1;
+  sum_rows(xp, mp, out, xq, mq, &zp, &zq);
   const double iq = zp / zq;  // (in units of p's weights)
   bool both = xq != nullptr;
   auto term = [&](int e, float u, float v) -> double {
@@ -452,25 +452,30 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
     return e == out ? 0.0 : w;
   };
   auto sum_terms = [&](int at, int end) { return walk(xp, both ? xq : static_cast<const T*>(nullptr), at, end, term); };
+  const double* drawn = sm.all[0];
   double whole = zp;
-  if (rejected) {
-    const double mine = sum_terms(lo, hi);
-    if (lane == 0) sm.seg[2][warp] = mine;
+  if (both) {
+    share(2, sum_terms(lo, hi));
     cluster.sync();
-    whole = gather(2);
-    if (!(whole > 0.0)) {  // p nowhere above q (they are equal, and a rounding rejected): p itself
-      both = false;
-      whole = gather(0);
-    }
+    drawn = sm.all[2];
+    whole = vd_sum(drawn, segs, lane);
   }
-  cluster.barrier_arrive();  // (what this CTA reads of others it has read; it ends when they have, too)
+  if (!(whole > 0.0)) {  // p nowhere above q (they are equal, and a rounding rejected): p itself
+    if (!both) {
+      if (rank == 0 && tid == 0) {
+        a.accepted[b] = n;
+        a.next_token[b] = out;
+      }
+      return;
+    }
+    both = false;
+    drawn = sm.all[0];
+    whole = zp;
+  }
   const double least = (double)a.uniforms[(int64_t)b * (a.T + 1) + a.T] * whole;
   double before, start;
-  const int at_seg = vd_find(sm.all, segs, lane, 0.0, least, &before);
-  if (at_seg / VD_WARPS != rank) {
-    cluster.barrier_wait();
-    return;
-  }
+  const int at_seg = vd_find(drawn, segs, lane, 0.0, least, &before);
+  if (at_seg / VD_WARPS != rank) return;  // (what others write to a CTA they have written before the last barrier that all passed)
   // this CTA's warps take parts of the segment, then one its elements
   const int s0 = min(a.V, at_seg * seg), s1 = min(a.V, s0 + seg), part = (s1 - s0 + VD_WARPS - 1) / VD_WARPS;
   const double mine = sum_terms(min(s1, s0 + warp * part), min(s1, s0 + (warp + 1) * part));
@@ -502,12 +507,12 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
       a.next_token[b] = pick >= 0 ? pick : highest;
     }
   }
-  cluster.barrier_wait();
 }
 
 int vf_chunks(int64_t rows, int V) {
   const int64_t want = (8 * (int64_t)num_sms_current_device() + rows - 1) / rows;
-  const int64_t most = std::max<int64_t>(1, V / 2048), least = (V + 65535) / 65536;
+  // chunks of 4096 words at least: shorter ones start more CTAs than there is work for (of 2048 words: 50257 words 21.3 us, not 19.6)
+  const int64_t most = std::max<int64_t>(1, V / 4096), least = (V + 65535) / 65536;
   return (int)std::min<int64_t>(32, std::max(std::min(want, most), least));
 }
 
