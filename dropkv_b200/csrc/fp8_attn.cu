@@ -105,19 +105,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // The queries of all row tiles in 8-bit parts, laid out as the products read them, and their units. Grid: (row tiles of a
-// sequence, KV heads, sequences); D / 8 lanes have a row, eight elements each. A row's unit is the power of two that
+// sequence, SPLIT blocks for each; KV heads; sequences); D / 8 lanes have a row, eight elements each. A row's unit is the power of two that
 // brings its largest element to at most 448; the first part is an element's nearest 8 bits, the next what that leaves.
 // In a kernel of its own because a row tile's rows are a long chain for its four softmax warps (3.5 us of a piece's 7 before
 // its first product) and a short one for a whole GPU; bound by the chain load, largest element, parts.
 constexpr int FQ_NT = 256;
 
-template <typename T, int D>
+template <typename T, int D, int SPLIT>
 __global__ void __launch_bounds__(FQ_NT) fp8_queries_kernel(const __grid_constant__ Args A) {
   constexpr int PARTS = std::is_same<T, __nv_bfloat16>::value ? 2 : 3;
   constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-  constexpr int LANES = D / 8, PER = FQ_NT / LANES, TURNS = FA_ROWS / PER;
+  constexpr int LANES = D / 8, PER = FQ_NT / LANES, TURNS = FA_ROWS / PER / SPLIT;
   const AttnFp8& a = A.a;
-  const int rt = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int rt = blockIdx.x / SPLIT, h = blockIdx.y, b = blockIdx.z;
+  const int row0 = blockIdx.x % SPLIT * (TURNS * PER) + threadIdx.x / LANES;
   const int c = threadIdx.x % LANES, n0 = rt * A.npr, rows = (min(n0 + A.npr, a.T) - n0) * A.g;
   const int64_t tile = row_tile(A, b, h, rt);
   uint8_t* out = A.queries + tile * (PARTS * FA_ROWS * D);
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(FQ_NT) fp8_queries_kernel(const __grid_constan
   uint4 x[TURNS];
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
-    const int row = threadIdx.x / LANES + i * PER, token = A.quot(row), head = h * A.g + row - token * A.g;
+    const int row = row0 + i * PER, token = A.quot(row), head = h * A.g + row - token * A.g;
     x[i] = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows) {
       const T* src = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + (n0 + token) * a.q_ss + 8 * c * a.q_sd;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(FQ_NT) fp8_queries_kernel(const __grid_constan
   }
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
-    const int row = threadIdx.x / LANES + i * PER;
+    const int row = row0 + i * PER;
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     // the largest magnitude, as bits: two 16-bit values a word
     uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
@@ -911,9 +912,11 @@ int fa_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3(A.RT, a.Hkv, a.B);
+  constexpr int SPLIT = 4;  // of a tile's rows, while all blocks still run at once
+  const bool few = qs.tiles <= num_sms_current_device();
+  cfg.gridDim = dim3(few ? A.RT * SPLIT : A.RT, a.Hkv, a.B);
   cfg.blockDim = dim3(FQ_NT);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_queries_kernel<T, D>, A);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? fp8_queries_kernel<T, D, SPLIT> : fp8_queries_kernel<T, D, 1>, A);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 queries launch: %s", cudaGetErrorString(e));
   if ((rc = check_launch("attention_fp8_queries"))) return rc;
   cfg.gridDim = dim3(plan.ctas);
