@@ -427,8 +427,8 @@ DROPKV_API int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t 
  * max_blocks * block_size and on pages outside the pool are not seen; a token that sees nothing gives
  * zeros, and a row that no token sees is not used, whatever it holds. bf16 or fp16, D 64 or 128,
  * Hq / Hkv <= 128, T <= 256 with a mask, block_size a power of two from 8 to 1024, page rows on
- * 16-byte boundaries and not overlapping, B * Hkv <= 65535, scale positive and finite, scales
- * positive and finite; out [B, Hq, T, D] contiguous. */
+ * 16-byte boundaries and not overlapping, B * Hkv <= 65535, Hq * T <= 2^26, B * Hq * T < 2^31, max_blocks *
+ * block_size < 2^31 - 65536, scale positive and finite, scales positive and finite; out [B, Hq, T, D] contiguous. */
 DROPKV_API size_t dropkv_attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
 DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd,
                                     const void* k_pages, int64_t kp_sb, int64_t kp_sh, int64_t kp_st,
@@ -448,7 +448,7 @@ DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, i
  * rejected token n = accepted[b], else from p_n, as the first t whose cumulative sum passes
  * uniforms[b, T] times the whole. prob[b, i] = min(1, p_i(x_i) / q_i(x_i)), 0 for a token outside [0, V).
  * Where a row that is looked at holds NaN or +inf, or nothing but -inf, the draft ends there and next_token is
- * -1. uniforms in [0, 1); T <= 256, V <= 2^21, temperature in [1e-6, 1e6]. */
+ * -1. uniforms in [0, 1); B <= 2^24, T <= 256, V <= 2^21, temperature in [1e-6, 1e6]. */
 DROPKV_API size_t dropkv_verify_draft_workspace_size(int B, int T, int V, int draft);
 DROPKV_API int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const void* draft, int64_t d_sb,
                                    int64_t d_si, int dtype, const int64_t* tokens, const float* uniforms, int B, int T,

@@ -4,7 +4,7 @@
 import pytest
 import torch
 
-from dropkv_b200 import _lib, attention_fp8, load_rows_fp8, store_rows_fp8
+from dropkv_b200 import _lib, attention_fp8, load_rows_fp8, store_rows_fp8, verify_draft
 
 P = 4096  # a placeholder device address
 
@@ -152,3 +152,43 @@ def test_attention_fp8_refuses_empty_windows(window, on_device_0):
              block_table=torch.zeros(1, 4, dtype=torch.int32))
     with pytest.raises(ValueError, match="window"):
         attention_fp8(**{k: v.as_subclass(_Cuda) for k, v in a.items()}, window=window)
+
+
+class _OnDevice(torch.Tensor):
+    """A tensor that says it is on CUDA device 3."""
+
+    def get_device(self):
+        return 3
+
+
+@pytest.mark.parametrize("op,arguments", [
+    (store_rows_fp8, dict(slots=None, K=None, V=None, K_pages=None, V_pages=None, K_scales=None, V_scales=None)),
+    (load_rows_fp8, dict(dtype=torch.float16, K_pages=None, V_pages=None, K_scales=None, V_scales=None, slots=None)),
+    (attention_fp8, dict(scale=0.1, tree_mask="none", Q=None, K_pages=None, V_pages=None, K_scales=None, V_scales=None,
+                         cache_lens=None, block_table=None)),
+    (verify_draft, dict(temperature=0.5, draft_logits="none", target_logits=None, tokens=None, uniforms=None)),
+])
+def test_calls_enter_their_tensors_device(op, arguments, monkeypatch):
+    from dropkv_b200 import paged
+    entered = []
+
+    class Entered(Exception):
+        pass
+
+    class Device:
+        def __init__(self, index):
+            entered.append(index)
+
+        def __enter__(self):
+            raise Entered
+
+        def __exit__(self, *a):
+            return False
+
+    monkeypatch.setattr(paged, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    x = torch.zeros(2).as_subclass(_OnDevice)
+    arguments = {k: x if v is None else None if v == "none" else v for k, v in arguments.items()}
+    with pytest.raises(Entered):
+        op(**arguments)
+    assert entered == [3]
