@@ -6,6 +6,8 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 
@@ -942,6 +944,47 @@ int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const vo
                 accepted, next_token, prob};
   return launch_verify_draft(q, dtype, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
+
+// ---------------------------------------------------------------------------
+// Calls with their arguments in one array
+// ---------------------------------------------------------------------------
+}  // extern "C"
+
+template <typename T>
+static bool word_fits(int64_t w) {
+  return !std::is_same<T, int>::value || w == (int)w;
+}
+template <typename T>
+static T from_word(int64_t w) {
+  if constexpr (std::is_pointer<T>::value) {
+    return reinterpret_cast<T>(w);
+  } else if constexpr (std::is_floating_point<T>::value) {
+    double d;
+    std::memcpy(&d, &w, 8);
+    return (T)d;
+  } else {
+    return (T)w;
+  }
+}
+template <typename... A, size_t... I>
+static int call_words(int (*f)(A...), const int64_t* words, std::index_sequence<I...>) {
+  if (!words) return fail(DROPKV_ERR_ARG, "NULL pointer argument");
+  int64_t w[sizeof...(A)];
+  std::memcpy(w, words, sizeof(w));  // (of any alignment)
+  if (!(word_fits<A>(w[I]) && ...)) return fail(DROPKV_ERR_ARG, "invalid sizes: an integer argument is out of range");
+  return f(from_word<A>(w[I])...);
+}
+template <typename... A>
+static int call_words(int (*f)(A...), const int64_t* words) {
+  return call_words(f, words, std::index_sequence_for<A...>());
+}
+
+extern "C" {
+
+int dropkv_store_rows_fp8_words(const int64_t* words) { return call_words(dropkv_store_rows_fp8, words); }
+int dropkv_load_rows_fp8_words(const int64_t* words) { return call_words(dropkv_load_rows_fp8, words); }
+int dropkv_attention_fp8_words(const int64_t* words) { return call_words(dropkv_attention_fp8, words); }
+int dropkv_verify_draft_words(const int64_t* words) { return call_words(dropkv_verify_draft, words); }
 
 }  // extern "C"
 

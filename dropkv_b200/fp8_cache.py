@@ -86,9 +86,9 @@ def store_rows_fp8(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, K_page
     if ps[1] != Hkv or ps[3] != D:
         raise ValueError(f"rows of {Hkv} heads of {D} do not fit pages {tuple(ps)}")
     slots = _ints(slots, torch.int64, (B, N), "slots")
-    rc = _lib.load().dropkv_store_rows_fp8(
-        K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(), *pool, ps[0], ps[2],
-        dt, B, Hkv, N, D, _raw_stream(dev))
+    pack, call = _lib.words("dropkv_store_rows_fp8")
+    rc = call(pack(K.data_ptr(), *_rows_strides(K, "K"), V.data_ptr(), *_rows_strides(V, "V"), slots.data_ptr(), *pool,
+                   ps[0], ps[2], dt, B, Hkv, N, D, _raw_stream(dev)))
     if rc:
         _lib.check(rc, "dropkv_store_rows_fp8")
 
@@ -111,8 +111,9 @@ def load_rows_fp8(K_pages: torch.Tensor, V_pages: torch.Tensor, K_scales: torch.
     device = K_pages.device
     k_out = _new(dtype, device, B, ps[1], N, ps[3])
     v_out = torch.empty_like(k_out)
-    rc = _lib.load().dropkv_load_rows_fp8(*pool, ps[0], ps[2], slots.data_ptr(), dt, B, ps[1], N, ps[3], k_out.data_ptr(),
-                                          v_out.data_ptr(), _raw_stream(dev))
+    pack, call = _lib.words("dropkv_load_rows_fp8")
+    rc = call(pack(*pool, ps[0], ps[2], slots.data_ptr(), dt, B, ps[1], N, ps[3], k_out.data_ptr(), v_out.data_ptr(),
+                   _raw_stream(dev)))
     if rc:
         _lib.check(rc, "dropkv_load_rows_fp8")
     return k_out, v_out
@@ -159,7 +160,7 @@ def attention_fp8(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
         raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
     max_blocks = block_table.shape[1]
     block_table = _ints(block_table, torch.int32, (B, max_blocks), "block_table")
-    mask = (None, 0, 0, 0)
+    mask = (0, 0, 0, 0)
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:
             raise TypeError(f"tree_mask must be bool, got {tree_mask.dtype}")
@@ -176,10 +177,11 @@ def attention_fp8(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
     # a workspace of the call's own, from the caching allocator: calls on several streams share nothing
     need = max(_attention_workspace(dev, B, Hq, Hkv, T, D, max_blocks * block), 1)
     ws = _new(torch.uint8, Q.device, need)
-    rc = _lib.load().dropkv_attention_fp8(
+    pack, call = _lib.words("dropkv_attention_fp8")
+    rc = call(pack(
         Q.data_ptr(), *Q.stride(), *pool, n_pages, block, block_table.data_ptr(), max_blocks, cache_lens.data_ptr(), *mask,
         min(int(window or 0), 0x7fffffff), min(int(sinks), 0x7fffffff), _DTYPE_CODE[dtype], B, Hq, Hkv, T, D, scale,
-        out.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
+        out.data_ptr(), ws.data_ptr(), need, _raw_stream(dev)))
     if rc:
         _lib.check(rc, "dropkv_attention_fp8")
     if _CHECK_STATUS and n_pages * max_blocks > 0 and not torch.cuda.is_current_stream_capturing():

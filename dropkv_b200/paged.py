@@ -489,11 +489,11 @@ def verify_draft(target_logits: torch.Tensor, tokens: torch.Tensor, uniforms: to
         return out
     need = max(_verify_workspace(dev, B, T, V, draft is not None), 1)
     ws = _new(torch.uint8, device, need)
-    rc = _lib.load().dropkv_verify_draft(
-        target.data_ptr(), target.stride(0), target.stride(1), draft.data_ptr() if draft is not None else None,
-        draft.stride(0) if draft is not None else 0, draft.stride(1) if draft is not None else 0, dt, tokens.data_ptr(),
-        uniforms.data_ptr(), B, T, V, float(temperature), out.accepted.data_ptr(), out.next_token.data_ptr(),
-        out.accept_prob.data_ptr(), ws.data_ptr(), need, _raw_stream(dev))
+    pack, call = _lib.words("dropkv_verify_draft")
+    rc = call(pack(
+        target.data_ptr(), *target.stride()[:2], *((draft.data_ptr(), *draft.stride()[:2]) if draft is not None else (0, 0, 0)),
+        dt, tokens.data_ptr(), uniforms.data_ptr(), B, T, V, float(temperature), out.accepted.data_ptr(),
+        out.next_token.data_ptr(), out.accept_prob.data_ptr(), ws.data_ptr(), need, _raw_stream(dev)))
     if rc:
         _lib.check(rc, "dropkv_verify_draft")
     return out

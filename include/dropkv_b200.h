@@ -455,6 +455,14 @@ DROPKV_API int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_s
                                    int V, float temperature, int64_t* accepted, int64_t* next_token, float* prob,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same calls with their arguments in one array, in order: pointers and integers as 64-bit integers, floats as
+ * the bits of a double. For bindings whose calls cost by the argument; an integer that does not fit its argument is
+ * refused. */
+DROPKV_API int dropkv_store_rows_fp8_words(const int64_t* words);
+DROPKV_API int dropkv_load_rows_fp8_words(const int64_t* words);
+DROPKV_API int dropkv_attention_fp8_words(const int64_t* words);
+DROPKV_API int dropkv_verify_draft_words(const int64_t* words);
+
 /* Diagnostic: one 128-row tile through a tcgen05 MMA form used by the fused
  * scorer (mode 0: out[128][n] = A[128][128] B[n][128]^T with A loaded by TMA;
  * mode 1: out[128][n] = A[128][128]^T B[n][128]^T with A read MN-major; modes 2/3:

@@ -192,3 +192,21 @@ def test_calls_enter_their_tensors_device(op, arguments, monkeypatch):
     with pytest.raises(Entered):
         op(**arguments)
     assert entered == [3]
+
+
+def test_arguments_in_one_array():
+    """The entries that take them so refuse what the plain ones do, and integers that no argument holds."""
+    pool = (P, 64, 64, 64, P, 64, 64, 64, P, 2, 1, P, 2, 1)
+    pack, call = _lib.words("dropkv_load_rows_fp8")
+    _refused(call(pack(*pool, 4, 16, 0, 2, 1, 2, 3, 64, P, P, 0)), _lib.ERR_ARG, "NULL")
+    _refused(call(pack(*pool, 4, 16, P, 2, 1, 2, 3, 64, P, P + 1, 0)), _lib.ERR_ARG, "aligned")
+    for at in (14, 15, 17, 18, 20, 21):
+        args = [*pool, 4, 16, P, 2, 1, 2, 3, 64, P, P, 0]
+        args[at] = (1 << 32) + args[at]
+        _refused(call(pack(*args)), _lib.ERR_ARG, "out of range")
+    pack, call = _lib.words("dropkv_verify_draft")
+    for tau, text in ((0.0, "temperature"), (float("nan"), "temperature"), (0.5, "workspace")):
+        rc = call(pack(P, 400, 100, 0, 0, 0, 2, P, P, 2, 3, 100, tau, P, P, P, 0, 0, 0))
+        assert rc != _lib.OK and text in _lib.load().dropkv_last_error().decode()
+    for name in _lib.IN_WORDS:
+        assert getattr(_lib.load(), name + "_words")(None) == _lib.ERR_ARG
