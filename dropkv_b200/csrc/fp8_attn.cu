@@ -751,23 +751,23 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
 constexpr int FM_NT = 256;
 constexpr int FM_AHEAD = 8;  // partials on their way at once
 
-// Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, or, where FEW rows
-// make few blocks, the CTAs that they may begin in; groups of eight rows). With M the largest of the partials' maxima
+// Joins the partials of the segments that fell into several CTAs. Grid: (split segments at most, or, `direct`, where FEW rows
+// make few blocks or segments are many, the CTAs that they may begin in; groups of eight rows). With M the largest of the partials' maxima
 // and w_i = l_i 2^(m_i - M), O = sum w_i o_i / sum w_i, in the order of the CTAs: a warp takes a row's weights, then a
 // thread four columns of a row, as they lie: of FEW rows a row's vectors side by side, else eight rows' of a vector (who
 // wrote them had a row a thread). Bound by the latency of its loads, from L2.
 template <typename T, int D, bool FEW>
-__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A, int ctas) {
+__global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant__ Args A, int ctas, bool direct) {
   constexpr int ROWS = FM_NT / 32;
   __shared__ int counts[ROWS], found;
   __shared__ float weights[ROWS][33], before_[ROWS];  // of 32 partials; what those before them are scaled by
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (!FEW && threadIdx.x == 0) found = -1;
+  if (!direct && threadIdx.x == 0) found = -1;
   // every CTA waits for the kernel before this one, with work or without: what comes after on the
   // stream takes this kernel's end for the end of both
   pdl_wait();
   int pick = blockIdx.x;
-  if (!FEW) {  // the CTA in which the blockIdx.x-th split segment begins
+  if (!direct) {  // the CTA in which the blockIdx.x-th split segment begins
     for (int c0 = 0, before = 0; c0 < ctas; c0 += FM_NT) {
       const int at = c0 + threadIdx.x;
       const bool splits = at < ctas && A.meta[at].w > 0;
@@ -845,7 +845,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
 template <typename T, int D>
 int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   const int64_t segments = (int64_t)A.a.B * A.RT * A.a.Hkv;
-  const bool few = A.rows_pad <= kFp8DecodeRows;  // (a block for each CTA: no list to look through first)
+  const bool few = A.rows_pad <= kFp8DecodeRows, direct = few || segments >= ctas;  // (a block for each CTA: no list to look through)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -853,9 +853,9 @@ int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cfg.stream = st;
-  cfg.gridDim = dim3((unsigned)(few ? ctas : std::min<int64_t>(ctas, segments)), (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
+  cfg.gridDim = dim3((unsigned)(direct ? ctas : segments), (A.rows_pad + FM_NT / 32 - 1) / (FM_NT / 32));
   cfg.blockDim = dim3(FM_NT);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? fp8_merge_kernel<T, D, true> : fp8_merge_kernel<T, D, false>, A, ctas);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, few ? fp8_merge_kernel<T, D, true> : fp8_merge_kernel<T, D, false>, A, ctas, direct);
   if (e != cudaSuccess) return fail(DROPKV_ERR_CUDA, "attention_fp8 merge launch: %s", cudaGetErrorString(e));
   return check_launch("attention_fp8_merge");
 }
