@@ -46,7 +46,7 @@ struct Keys {
   int ns, w0, n;   // tiles of sinks, the first tile after them, all tiles (one at least)
   __device__ __forceinline__ void set(const Args& A, int b, int rt) {
     const AttnFp8& a = A.a;
-    len = max(__ldcg(a.cache_lens + b), 0);  // (from L2: many rows' kernel reads it before it waits for the kernel before)
+    len = max(A.queries ? __ldcg(a.cache_lens + b) : a.cache_lens[b], 0);  // (many rows: read before the wait for the kernel before)
     keys = (int)min((int64_t)len + a.T, (int64_t)a.cap);
     n0 = rt * A.npr;
     n1 = min(n0 + A.npr, a.T);
