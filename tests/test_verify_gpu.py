@@ -1,7 +1,7 @@
 """``verify_draft`` against its definition in 64 bits. Tokens and counts have to be equal.
 
-``accept_prob`` is a ratio of softmax values in fp32: one rounding (2^-24) of exp(d), where d, the difference of
-the tokens' log probabilities, is off by what the two rows' sums are: sums of positive fp32 terms over 256 threads (each at
+``accept_prob`` is a ratio of softmax values in fp32: an exponential of the difference of the logits over the rows'
+maxima (2^-22), a quotient and a product (2^-24 each) with the two rows' sums, and off by what these are: sums of positive fp32 terms over 256 threads (each at
 most V / 256 / 8 additions one after another; errors of 2^-24 each of a part of the sum, and 2^-22 of a term's
 exponential). 2^-17 relative bounds that for V up to 2^18.
 """
