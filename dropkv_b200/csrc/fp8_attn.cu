@@ -4,8 +4,8 @@
 //
 // A CTA has 128 query rows (whole tokens of a KV head's group) and two CTAs share an SM, so that one's softmax runs
 // beside the other's products; keys come in tiles of 64. Both products are tcgen05 MMAs:
-//   S = Q K^T  kind::f8f6f4, K's bytes as TMA brings them; queries as sums of 8-bit parts (two hold a bf16,
-//              three an fp16), each part a product into the same accumulator: as many operations as in 16 bits
+//   S = Q K^T  kind::f8f6f4, K's bytes as TMA brings them; queries as sums of 8-bit parts (two of a bf16,
+//              three of an fp16), each part a product into the same accumulator: as many operations as in 16 bits
 //              (half as many again for fp16), and no tile of K is ever widened;
 //   O += P V   kind::f16: weights in fp16 left in tensor memory where S was, V widened to fp16 (exactly) by two
 //              warps from one ring of tiles into another. (V as it lies would need weights in 8-bit parts: two roundings
@@ -106,7 +106,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // The queries of all row tiles in 8-bit parts, laid out as the products read them, and their units. Grid: (row tiles of a
 // sequence, SPLIT blocks for each; KV heads; sequences); D / 8 lanes have a row, eight elements each. A row's unit is the power of two that
-// brings its largest element to at most 448; the first part is an element's nearest 8 bits, the next what that leaves.
+// brings its largest element to at most 448; the first part is an element's nearest e4m3, each next the nearest e5m2 of what those
+// before it left: the parts add up in one accumulator, so they share the unit, and e4m3's grid ends at 2^-9 of it, where a second part
+// in e4m3 could leave 2^-10; e5m2's ends at 2^-16. What e4m3 leaves of a bf16 over 2^-6 has three bits, and so has what the second
+// leaves of an fp16: those are held exactly. Of smaller elements two parts leave at most 2^-14, three 2^-17.
 // In a kernel of its own because a row tile's rows are a long chain for its four softmax warps (3.5 us of a piece's 7 before
 // its first product) and a short one for a whole GPU; bound by the chain load, largest element, parts.
 constexpr int FQ_NT = 256;
@@ -180,9 +183,10 @@ __global__ void __launch_bounds__(FQ_NT) fp8_queries_kernel(const __grid_constan
       uint32_t q8[2] = {0u, 0u};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(z[e]), __NV_SATFINITE, __NV_E4M3);
+        const __nv_fp8_interpretation_t kind = part ? __NV_E5M2 : __NV_E4M3;
+        const uint32_t two = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(z[e]), __NV_SATFINITE, kind);
         q8[e / 2] |= two << (16 * (e & 1));
-        if (part + 1 < PARTS) z[e] = __hsub2(z[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, __NV_E4M3)));
+        if (part + 1 < PARTS) z[e] = __hsub2(z[e], __half2(__nv_cvt_fp8x2_to_halfraw2((uint16_t)two, kind)));
       }
       *reinterpret_cast<uint2*>(out + part * (FA_ROWS * D) + tc::swz_offset<D>(row, (c / 2) * 8) + (c & 1) * 8) = make_uint2(q8[0], q8[1]);
     }
@@ -358,7 +362,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
   } else if (warp == FA_WARP_MMA) {
     // ======================= MMA issuer =========================================
     // The whole warp runs this and one lane issues, so that counts, addresses and descriptors can stay uniform.
-    constexpr uint32_t ID_QK = tc::idesc_e4m3(FA_ROWS, TK);
+    constexpr uint32_t ID_QK[2] = {tc::idesc_f8(FA_ROWS, TK, false), tc::idesc_f8(FA_ROWS, TK, true)};
     constexpr uint32_t ID_PV = tc::idesc_f16(false, FA_ROWS, D, false, true);
     constexpr uint32_t LAYOUT = tc::layout_for_row_bytes(D);
     constexpr uint32_t LBO_V = SLABS == 2 ? TK * 128 : 0;
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           for (int part = 0; part < PARTS; ++part)
 #pragma unroll
             for (int kk = 0; kk < D / 32; ++kk)
-              tc::mma_f8(tm + buf * 64, tc::desc_add(qd, part * (FA_ROWS * D) + kk * 32), tc::desc_add(kd, kk * 32), ID_QK,
+              tc::mma_f8(tm + buf * 64, tc::desc_add(qd, part * (FA_ROWS * D) + kk * 32), tc::desc_add(kd, kk * 32), ID_QK[part > 0],
                          part > 0 || kk > 0);
           tc::mma_commit(&bars[L::B_S + buf]);
           tc::mma_commit(&bars[L::B_KE + slot]);

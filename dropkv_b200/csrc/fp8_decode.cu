@@ -6,8 +6,8 @@
 // MMAs fed from registers (tcgen05.mma takes 128 rows, of which 1 to 16 would exist, and as many
 // threads would do the softmax):
 //   S = Q K^T      m16n8k32 of e4m3: K's bytes as they lie, and queries as sums of 8-bit parts, each
-//                  what the one before left, times 16: two parts hold a bf16 (the second takes the
-//                  MMA's rows 8 to 15 where there are at most 8 queries), three an fp16;
+//                  what the one before left, times 16: two parts of a bf16 (the second takes the
+//                  MMA's rows 8 to 15 where there are at most 8 queries), three of an fp16;
 //   O^T += V^T P^T m16n8k16 of fp16: A = 16 columns of V for 16 keys, widened (exactly, two at a time),
 //                  B = the weights of 8 rows as they lie in S's accumulators.
 // The order of D and of the keys within a product is free, and chosen so that a quarter warp's 16-byte
@@ -15,7 +15,7 @@
 // chunks 4 i + tig of key fd_key(gid)'s row of K, and for V chunk fd_chunk(gid) of keys
 // fd_key(2 tig + {0, 1}) and of those 8 on, whose bytes are paired before they are widened.
 // A row's queries are brought to 8 bits' range by a power of two (its largest element to 224 or more;
-// what the parts leave is at most 2^-14 of that unit). A page's scale of K multiplies its logits in fp32;
+// what the parts leave is at most 2^-14 of that unit, 2^-18 in fp16). A page's scale of K multiplies its logits in fp32;
 // that of V, over the largest of the warp so far, the weights. Weights are rounded to fp16 for their
 // product (2^-11), sums taken from them before that.
 // Measured (in a graph, the merge with it): 32 sequences of up to 13107 rows x 8 heads x 128 in pages of 64 rows, bf16, 86

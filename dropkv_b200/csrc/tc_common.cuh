@@ -365,9 +365,9 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, int M, int N, bool a
          ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// Instruction descriptor, kind::f8f6f4 with fp32 accumulation, e4m3 operands, both K-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
-  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+// Instruction descriptor, kind::f8f6f4 with fp32 accumulation, B in e4m3, A in that or in e5m2, both K-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int M, int N, bool a_e5m2) {
+  return (1u << 4) | ((a_e5m2 ? 1u : 0u) << 7) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 }  // namespace tc
