@@ -13,8 +13,8 @@
 // S has two buffers, and the product of a tile is issued before the weights of the one before it are
 // awaited. Warps: four of softmax, a thread for each row; two that widen V; one for TMA (a box a page); one that
 // issues products.
-// A page's scale of K enters with the exponent's argument, that of V, over the largest of the warp so far, with the
-// weights (both for eight keys at a time: pages have eight rows at least). Weights are rounded to fp16 (2^-11),
+// A page's scale of K enters with the exponent's argument, that of V, over the row's largest weight times scale so far, with
+// the weights (both for eight keys at a time: pages have eight rows at least). Weights are rounded to fp16 (2^-11),
 // sums taken from them before that.
 // Measured (in a graph, three launches): 4096 tokens x 32 heads over 13107 rows x 8 heads x 128 before them, bf16, 970 us: 1050
 // TFLOP/s, 64% of a large bf16 product's rate (fp16: 1070 us); 64 nodes over 13107 rows 39 us; 8 nodes over 819 rows 15. A
@@ -38,8 +38,8 @@ constexpr int FA_WARP_V = 4, FA_WARP_TMA = 6, FA_WARP_MMA = 7, FA_NT = 256;
 constexpr int FA_CTAS = 2;    // of an SM
 constexpr int kFaLead = 6;  // (64 nodes over 13107 rows: 41.6 us at 2, 39.4 at 6, 38.9 at 9, where larger ones lose what that gains)
 constexpr uint64_t kFaWaitNs = 1000000000ull;
-// A row's reference moves once its maximum has grown by this much (base 2); weights are
-// 2^(s - m + bias), so that fp16 holds them from 2^-24 to 2^15.
+// A row's reference moves once its maximum has grown by this much (base 2); weights times scales are
+// 2^(s + log2 sv - R + bias), so that fp16 holds them from 2^-24 to 2^15.
 constexpr float kFaSlack = 8.f, kFaBias = 7.f;
 // Where a tile's weights are formed first: a row's sum of them above this moves its reference to the row's maximum
 // (64 weights of 2^7 then sum to 2^13 at most).
@@ -511,7 +511,9 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
     if (more) begin();
     while (more) {
       const bool live = warp * 32 < p.rows;  // some row of this warp exists
-      float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;  // the output is O * vref
+      // m measures the sums; R, also in base 2, the weights that meet V, times their pages' scales, of what the row sees alone.
+      // (With one for all rows of a warp, pages of large scales took the bits of rows that do not see them, or give them no weight.)
+      float m = -INFINITY, l = 0.f, R = -INFINITY, vinv = 0.f;  // vinv: 2^(m - R); the output is O / vinv
       int any_bad = 0;
       const int t1 = p.t1;
       for (int t = p.t0; t < t1 && ok; ++t, ++j) {
@@ -521,19 +523,15 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
         const FaKind* kind_at = kinds + place;
         if (++place == L::SCALES) place = 0;
         uint64_t sum[2];
-        // The reference moves where some row's maximum has outgrown it, or a page's scale of V the others'.
-        auto settle = [&](float top, float vmax, float slack) {
-          if (!__any_sync(0xffffffffu, top > m + slack) && vmax <= vref) return;
-          const float mn = top > m + slack ? top : m;
-          float alpha = mn == m ? 1.f : ex2(m - mn);
-          m = mn;
-          l *= alpha;
-          if (vmax > vref) {
-            alpha *= vref / vmax;
-            vref = vmax;
-            vinv = 1.f / vmax;
-          }
-          if (first) return;
+        // The references move where some row's largest logit, or that and its scale, has outgrown them.
+        auto settle = [&](float top, float wtop, float slack) {
+          if (!__any_sync(0xffffffffu, top > m + slack || wtop > R + slack)) return;
+          const float mn = top > m + slack ? top : m, Rn = wtop > R + slack ? wtop : R;
+          l *= mn == m ? 1.f : ex2(m - mn);
+          const float alpha = Rn == R ? 1.f : ex2(R - Rn);
+          m = mn, R = Rn;
+          vinv = share_of(m, R);
+          if (first || !__any_sync(0xffffffffu, alpha != 1.f)) return;
           ok = __all_sync(0xffffffffu, wait(&bars[L::B_O + 1 - buf], (j - 1) >> 1, 13)) && ok;
           tc::tc_fence_after();
           float o[16];
@@ -565,7 +563,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               if (!decltype(plain)::value && e % 8 == 0) {
-                const float c = fminf(scales[4 * h + e / 8] * unit, 3e38f), f = scales[FA_HALVES + 4 * h + e / 8] * vinv;
+                const float c = fminf(scales[4 * h + e / 8] * unit, 3e38f), f = fminf(scales[FA_HALVES + 4 * h + e / 8] * vinv, 3e38f);
                 c2 = pair_of(c, c);
                 f2 = pair_of(f, f);
               }
@@ -580,13 +578,14 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             tc::tmem_st16(ts + 16 * h, reinterpret_cast<const float*>(pk));
           }
         };
-        auto largest = [&](const float* x) {
-          float top = -INFINITY;
+        auto largest = [&](const float* x, float& wtop) {
+          float top = wtop = -INFINITY;
 #pragma unroll
           for (int y = 0; y < FA_HALVES; ++y) {
             const float* z = x + 8 * y;
-            top = fmaxf(top, max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])) *
-                                 fminf(scales[y] * unit, 3e38f));
+            const float u = max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])) * fminf(scales[y] * unit, 3e38f);
+            top = fmaxf(top, u);
+            wtop = fmaxf(wtop, u + __log2f(scales[FA_HALVES + y]));
           }
           return top;
         };
@@ -603,22 +602,30 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             return (s0 + s1) + (s2 + s3);
           };
           if (kind & FA_WHOLE) {  // what most tiles are
-            // Weights against the standing reference, without a look at the maximum: a sum within fp16's range says that
+            // Weights against the standing references, without a look at the maximum: a sum within fp16's range says that
             // all of them are. (The maximum first: 64 logits' worth of instructions and of latency more a tile.)
             float x[TK];
             tc::tmem_ld64(ts, x);
-            bool settled = vmax > vref;  // a piece's first tile, or a page's scale of V above the others'
+            bool settled = first;
 #pragma unroll 1
             for (;;) {
-              if (settled) settle(largest(x), vmax, 0.f);
-              share = kind & FA_PLAIN ? vmax * vinv : 0.f;
-              if (share >= 0x1p-40f) {
+              if (settled) {
+                float wtop;
+                const float top = largest(x, wtop);
+                settle(top, wtop, 0.f);
+              }
+              share = m == -INFINITY ? 1.f : vmax * vinv;  // (a row with nothing but NaN has no say)
+              float most;  // of the weights times scales, their sum or more
+              if (kind & FA_PLAIN && __all_sync(0xffffffffu, share >= 0x1p-40f && share <= 0x1p40f)) {
                 weigh(x, std::true_type());
+                most = total();
               } else {
+                const float up = fmaxf(share, 1.f);
                 share = 1.f;
                 weigh(x, std::false_type());
+                most = total() * up;
               }
-              if (settled || !__any_sync(0xffffffffu, total() > kFaMost || m == -INFINITY)) break;
+              if (settled || !__any_sync(0xffffffffu, most > kFaMost || m == -INFINITY)) break;
               tc::tmem_st_wait();
               settled = true;
             }
@@ -626,7 +633,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             // eight keys at a time, S read twice (rolled, as this is what few tiles are)
             const uint64_t see = sees.template bits<TK>(A, p.b, p.k.len, p.k.first(t));
             __syncwarp();
-            float top = -INFINITY;
+            float top = -INFINITY, wtop = -INFINITY;
             auto eight = [&](int y, float* z) {  // logits
               tc::tmem_ld8(ts + 8 * y, z);
               const float s = scales[y], c = fminf(s * unit, 3e38f);
@@ -638,16 +645,18 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             for (int y = 0; y < FA_HALVES; ++y) {
               float z[8];
               eight(y, z);
-              top = fmaxf(top, max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7])));
+              const float u = max3(max3(z[0], z[1], z[2]), max3(z[3], z[4], z[5]), fmaxf(z[6], z[7]));
+              top = fmaxf(top, u);
+              wtop = fmaxf(wtop, u + __log2f(scales[FA_HALVES + y]));
             }
-            settle(top, vmax, kFaSlack);
+            settle(top, wtop, kFaSlack);
             const float ref = (m == -INFINITY ? 0.f : m) - kFaBias;
             sum[0] = sum[1] = 0;
 #pragma unroll 1
             for (int y = 0; y < FA_HALVES; ++y) {
               float z[8];
               eight(y, z);
-              const float f = scales[FA_HALVES + y] * vinv;
+              const float f = fminf(scales[FA_HALVES + y] * vinv, 3e38f);
               uint32_t pk[4];
 #pragma unroll
               for (int e = 0; e < 8; e += 2) {
@@ -683,7 +692,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       tc::tc_fence_after();
       if (live) {
         // (l counts weights, of which a row that sees anything has one of 2^-1 at least)
-        const float inv = l == 0.f ? 0.f : vref / l;
+        const float inv = l == 0.f ? 0.f : 1.f / vinv / l;
         uint32_t nan[D / 32];  // columns whose value is NaN for a row of V that this row sees
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) nan[w] = 0;

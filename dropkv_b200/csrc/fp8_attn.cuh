@@ -277,6 +277,10 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, hardware approximation;
   return y;
 }
 
+// 2^(m - R): what a weight's measure is to that of a weight times a page's scale of V (of a row that has seen nothing: anything
+// finite).
+__device__ __forceinline__ float share_of(float m, float R) { return ex2(fmaxf(fminf(m - R, 126.f), -126.f)); }
+
 template <typename T>
 struct Out;
 template <>

@@ -16,7 +16,7 @@
 // fd_key(2 tig + {0, 1}) and of those 8 on, whose bytes are paired before they are widened.
 // A row's queries are brought to 8 bits' range by a power of two (its largest element to 224 or more;
 // what the parts leave is at most 2^-14 of that unit, 2^-18 in fp16). A page's scale of K multiplies its logits in fp32;
-// that of V, over the largest of the warp so far, the weights. Weights are rounded to fp16 for their
+// that of V, over the row's largest weight times scale so far, the weights. Weights are rounded to fp16 for their
 // product (2^-11), sums taken from them before that.
 // Measured (in a graph, the merge with it): 32 sequences of up to 13107 rows x 8 heads x 128 in pages of 64 rows, bf16, 86
 // us for 484 MB: 5.6 TB/s, 86% of a copy's rate (pages of 16: 92); 295K rows x 4 heads in pages of 16, fp16, 70 us for 303 MB:
@@ -70,8 +70,8 @@ template <int D>
 __device__ __forceinline__ int fd_chunk(int gid) { return D == 128 ? ((gid & 1) << 2) | (gid >> 1) : gid; }
 
 constexpr int kFdLead = 3;
-// A row's reference moves once its maximum has grown by this much (base 2); weights are
-// 2^(s - m + bias), so that fp16 holds them from 2^-24 to 2^15.
+// A row's reference moves once its maximum has grown by this much (base 2); weights times scales are
+// 2^(s + log2 sv - R + bias), so that fp16 holds them from 2^-24 to 2^15.
 constexpr float kFdSlack = 8.f, kFdBias = 7.f;
 
 __device__ __forceinline__ void fd_mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -296,8 +296,10 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
 #pragma unroll
       for (int t = 0; t < VB / 2; ++t) o[x][t][0] = o[x][t][1] = o[x][t][2] = o[x][t][3] = 0.f;
     }
-    float vref = 0.f;  // the output is o * vref
-    float vinv = 0.f;  // 1 / vref
+    // what a row's weights times scales are measured by, in base 2, and 2^(m - R): the output is o / share
+    float R[HR], share[HR];
+#pragma unroll
+    for (int x = 0; x < HR; ++x) R[x] = -INFINITY, share[x] = 1.f;
     int all_end, all_low;
     p.k.all(A, &all_end, &all_low);
     for (int t = p.t0; t < p.t1; ++t) {
@@ -385,45 +387,45 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
           }
           seen = __reduce_or_sync(0xffffffffu, seen);
         }
-        // the reference moves where some row's maximum has outgrown it
+        // The references move where some row's maximum has outgrown them: m, of the sums, by logits; R, of the weights that
+        // meet V, by logits and scales, of what the row sees alone. (With one for all rows, pages of large scales took the bits
+        // of rows that do not see them, or give them no weight.)
+        const float lv = __log2f(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
         float top[HR];
         bool over = false;
 #pragma unroll
         for (int x = 0; x < HR; ++x) {
           top[x] = fmaxf(fmaxf(fmaxf(s[0][2 * x], s[0][2 * x + 1]), fmaxf(s[1][2 * x], s[1][2 * x + 1])),
                          fmaxf(fmaxf(s[2][2 * x], s[2][2 * x + 1]), fmaxf(s[3][2 * x], s[3][2 * x + 1])));
-          over = over || top[x] > m[x] + kFdSlack;
+          over = over || top[x] > m[x] + kFdSlack || top[x] + lv > R[x] + kFdSlack;
         }
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
           for (int x = 0; x < HR; ++x) {
-            top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-            top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-            const float mn = top[x] > m[x] + kFdSlack ? top[x] : m[x];
-            const float f = mn == m[x] ? 1.f : ex2(m[x] - mn);
-            m[x] = mn;
-            l[x] *= f;
+            float wtop = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) wtop = fmaxf(wtop, fmaxf(s[y][2 * x], s[y][2 * x + 1]) + __log2f(vs[y]));
+#pragma unroll
+            for (int i = 1; i < 4; i *= 2) {
+              top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], i));
+              wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, i));
+            }
+            const float mn = top[x] > m[x] + kFdSlack ? top[x] : m[x], Rn = wtop > R[x] + kFdSlack ? wtop : R[x];
+            l[x] *= mn == m[x] ? 1.f : ex2(m[x] - mn);
+            const float f = Rn == R[x] ? 1.f : ex2(R[x] - Rn);
+            m[x] = mn, R[x] = Rn;
+            share[x] = share_of(mn, Rn);
             const float f0 = __shfl_sync(0xffffffffu, f, 8 * tig), f1 = __shfl_sync(0xffffffffu, f, 8 * tig + 4);
 #pragma unroll
             for (int e = 0; e < VB / 2; ++e) o[x][e][0] *= f0, o[x][e][1] *= f1, o[x][e][2] *= f0, o[x][e][3] *= f1;
           }
-        }
-        const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-        if (vmax > vref) {  // (the same in every lane)
-          const float f = vref / vmax;
-#pragma unroll
-          for (int x = 0; x < HR; ++x)
-#pragma unroll
-            for (int e = 0; e < VB / 2; ++e) o[x][e][0] *= f, o[x][e][1] *= f, o[x][e][2] *= f, o[x][e][3] *= f;
-          vref = vmax;
-          vinv = 1.f / vmax;
         }
 #pragma unroll
         for (int x = 0; x < HR; ++x) {
           const float ref = (m[x] == -INFINITY ? 0.f : m[x]) - kFdBias;
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const float p0 = ex2(s[y][2 * x] - ref), p1 = ex2(s[y][2 * x + 1] - ref), f = vs[y] * vinv;
+            const float p0 = ex2(s[y][2 * x] - ref), p1 = ex2(s[y][2 * x + 1] - ref), f = fminf(vs[y] * share[x], 3e38f);
             l[x] += p0 + p1;
             b[y][x] = pack_half(p0 * f, p1 * f);
           }
@@ -511,11 +513,13 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
         wm[warp * ROWS + r] = m[x] - kFdBias;
         wl[warp * ROWS + r] = l[x];
       }
+      const float back = 1.f / share[x];
+      const float b0 = __shfl_sync(0xffffffffu, back, 8 * tig), b1 = __shfl_sync(0xffffffffu, back, 8 * tig + 4);
       float* o0 = wo + (warp * ROWS + 8 * x + 2 * tig) * D + VB * fd_chunk<D>(gid);
 #pragma unroll
       for (int e = 0; e < VB / 2; ++e) {
-        *reinterpret_cast<float2*>(o0 + 2 * e) = make_float2(o[x][e][0] * vref, o[x][e][2] * vref);
-        *reinterpret_cast<float2*>(o0 + D + 2 * e) = make_float2(o[x][e][1] * vref, o[x][e][3] * vref);
+        *reinterpret_cast<float2*>(o0 + 2 * e) = make_float2(o[x][e][0] * b0, o[x][e][2] * b0);
+        *reinterpret_cast<float2*>(o0 + D + 2 * e) = make_float2(o[x][e][1] * b1, o[x][e][3] * b1);
       }
     }
     fd_sync();

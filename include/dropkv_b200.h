@@ -425,7 +425,8 @@ DROPKV_API int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t 
  * `window` up to its own row, or its depth's (the nodes it sees less itself), and the
  * first `sinks`; nodes of a tree are all seen (window >= T). table [B, max_blocks]: rows past
  * max_blocks * block_size and on pages outside the pool are not seen; a token that sees nothing gives
- * zeros, and a row that no token sees is not used, whatever it holds. bf16 or fp16, D 64 or 128,
+ * zeros, and a row that no token sees is not used, whatever it holds. A weight times its page's scale of V is rounded to
+ * 2^-11 of itself or 2^-32 of the largest such product of its token, whichever is more. bf16 or fp16, D 64 or 128,
  * Hq / Hkv <= 128, T <= 256 with a mask, block_size a power of two from 8 to 1024, page rows on
  * 16-byte boundaries and not overlapping, B * Hkv <= 65535, Hq * T <= 2^26, B * Hq * T < 2^31, max_blocks *
  * block_size < 2^31 - 65536, scale positive and finite, scales positive and finite; out [B, Hq, T, D] contiguous. */

@@ -52,7 +52,8 @@ def check(c, window=None, sinks=0, scale=None):
             want, size, peak = p @ v, p @ v.abs(), 448 * (p * sv).amax(-1, keepdim=True)
             tol = (u * want.abs() + (2.0 ** -11 + 2.0 ** -16 + torch.expm1(2 * d)) * size + see.sum(-1, keepdim=True) * 2.0 ** -32 * peak
                    + 2.0 ** -25)
-            err = (got[b, h * g:(h + 1) * g].double() - want).abs().masked_fill(want.abs() > torch.finfo(got.dtype).max, 0.0)
+            # (what is within its tolerance of the type's range, or past it, may be an infinity)
+            err = (got[b, h * g:(h + 1) * g].double() - want).abs().masked_fill(want.abs() + tol > torch.finfo(got.dtype).max, 0.0)
             assert bool((err <= tol).all()), (b, h, float((err / tol).nan_to_num(1e9).max()), float(err.max()), float(want.abs().max()))
     return got
 
@@ -82,3 +83,43 @@ def test_small_elements_beside_a_large_channel(heads, T, down, dtype):
         raw.copy_(torch.where((raw & 0x7f) == 0x7f, raw, (size * of).to(E4M3).view(torch.uint8)))  # (rows that none sees keep NaN)
         scales.copy_(torch.where(scales.isnan(), scales, 2.0 ** -5))
     check(c, scale=2.0 ** (down - 9) * 128 / D)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,T", [((8, 2, 128), 4), ((4, 2, 64), 6), ((8, 2, 128), 16), ((14, 2, 64), 40), ((8, 2, 128), 200)])
+@pytest.mark.parametrize("far", [12, 24, 40])
+def test_pages_that_a_token_does_not_see(heads, T, far, dtype):
+    """The later tokens' pages hold values 2^far times the others': the earlier tokens, which do not see them, lose nothing.
+    (What the later ones give is past fp16's range, and looked at in bf16 alone.)"""
+    half = T // 2
+    c = Case(*heads, [208 - half, (16 if half <= 16 else 1000) - half], T, 8, dtype, seed=52)
+    for b, n in enumerate(c.lens):
+        c.vs[c.table[b, (n + half) // 8:(n + T - 1) // 8 + 1].long()] *= 2.0 ** far
+    check(c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,T", [((8, 2, 128), 1), ((4, 2, 64), 6), ((8, 2, 128), 16), ((14, 2, 64), 40), ((8, 2, 128), 200)])
+@pytest.mark.parametrize("far,first", [(12, False), (30, False), (30, True), (60, False), (60, True)])
+def test_pages_that_weigh_nothing(heads, T, far, first, dtype):
+    """Pages with large values and logits of -100: they add nothing, and take no bits of the others. Some pages' values are
+    far smaller still, and some are zeros, whose scale is the least there is."""
+    c = Case(*heads, [700, 90], T, 16, dtype, seed=53, q_scale=0.2)
+    h = torch.Generator().manual_seed(54)
+    c.Q[..., 0] = 4.0
+    c.K.view(torch.uint8)[..., 0].masked_fill_((c.K.view(torch.uint8)[..., 0] & 0x7f) != 0x7f, 0)
+    vs, V = c.vs.clone(), c.V.view(torch.uint8)
+    for b, n in enumerate(c.lens):
+        ids = c.table[b, :-(-(n + T) // 16)].long()
+        kind = torch.randint(0, 4, (len(ids),), generator=h)
+        kind[-1] = 0
+        if first:   # the large ones in front
+            kind = torch.cat([kind[:-1].sort(descending=True).values, kind[-1:]])
+        large, small, zero = (ids[(kind == i).cuda()] for i in (3, 2, 1))
+        c.vs[large] = vs[large] * 2.0 ** far
+        c.ks[large] = 1.0
+        c.K.view(torch.uint8)[large, ..., 0] = torch.tensor([-25.0]).to(E4M3).view(torch.uint8).item()   # times 4: -100 times `scale`
+        c.K.view(torch.uint8)[large, ..., 1:] = 0
+        c.vs[small] = vs[small] * 2.0 ** -20
+        c.vs[zero] = 2.0 ** -126
+        V[zero] = 0
+    check(c, scale=1.0)
+    check(c, scale=1.0, window=300, sinks=40)
