@@ -45,7 +45,7 @@ constexpr float kFaSlack = 8.f, kFaBias = 7.f;
 // (64 weights of 2^7 then sum to 2^13 at most).
 constexpr float kFaMost = 32768.f;
 
-// A tile whose keys all tokens see, with no page missing; and one whose pages have one scale of K and one of V, besides
+// A tile whose keys all tokens see, with no page missing and none of zeros in V; and one whose pages have one scale of K and one of V, besides
 constexpr int FA_WHOLE = 1, FA_PLAIN = 2;
 struct FaKind {
   int kind;
@@ -63,7 +63,7 @@ struct FaSmem {
   // Tiles whose scales are held: the load of K of tile i waits for the product of tile i - NS, which waits for the weights
   // of tile i - NS - 2, and V's before it for tile i - 1 - NS to be widened; so all are past the tile NS + 2 back.
   static constexpr int SCALES = NS + 2;
-  static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: 0 for a missing page
+  static constexpr int SC = V + NS * TILE;              // float [SCALES][2][8]: -1 and 0 for a missing page
   static constexpr int KIND = SC + SCALES * 2 * FA_HALVES * 4;  // {int, float} [SCALES]: FA_WHOLE, FA_PLAIN; the largest of V's
   static constexpr int WALKS = KIND + SCALES * 8;  // WarpWalk [4], of the softmax warps
   static constexpr int BARS = (WALKS + 4 * (int)sizeof(WarpWalk<FA_TK>) + 7) / 8 * 8;
@@ -307,10 +307,10 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
       int all_end, all_low;
       p.k.all(A, &all_end, &all_low);
       int page = page_of(p.t0), page1 = page_of(p.t0 + 1);
-      float ks = there(page) ? ksb[page * a.pool.ks_s0] : 0.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
+      float ks = there(page) ? ksb[page * a.pool.ks_s0] : -1.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
       for (int t = p.t0; t < p.t1; ++t, ++n) {
         const int page2 = page_of(t + 2);
-        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : 0.f;
+        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : -1.f;
         const float vs1 = there(page1) ? vsb[page1 * a.pool.vs_s0] : 0.f;
         // the page of a lane's box: that of any of its eights that is read, else out of range (zeros)
         int at = there(page) ? page : -1;
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
           if (kv == 0) {  // (the scales are on their way as the tile is)
             const float ks0 = __shfl_sync(0xffffffffu, ks, 0), vs0 = __shfl_sync(0xffffffffu, vs, 0);
             const int j0 = p.k.first(t);
-            const bool there = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks > 0.f && vs > 0.f));
+            const bool there = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks >= 0.f && vs > 0.f));
             const bool one = __all_sync(0xffffffffu, lane >= FA_HALVES || (ks == ks0 && vs == vs0));
             const bool whole = there && j0 + TK <= all_end && (j0 >= all_low || j0 + TK <= a.sinks);
             const int kind = whole ? (one ? FA_WHOLE | FA_PLAIN : FA_WHOLE) : 0;
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(FA_NT, FA_CTAS)
             auto eight = [&](int y, float* z) {  // logits
               tc::tmem_ld8(ts + 8 * y, z);
               const float s = scales[y], c = fminf(s * unit, 3e38f);
-              const uint32_t bits = s > 0.f ? (uint32_t)(see >> (8 * y)) : 0u;
+              const uint32_t bits = s >= 0.f ? (uint32_t)(see >> (8 * y)) : 0u;
 #pragma unroll
               for (int e = 0; e < 8; ++e) z[e] = (bits >> e) & 1 ? z[e] * c : -INFINITY;
             };

@@ -47,7 +47,7 @@ struct FdShape {
   // tiles whose scales are held: before tile i's first load is issued, the slot is free that load 2 i - SLOTS had,
   // so all warps are past the tiles before that
   static constexpr int SCALES = SLOTS / 2 + 1;
-  static constexpr int SC = WM + 2 * FD_WARPS * ROWS * 4;        // float [SCALES][2][FD_HALVES]: 0 for a missing page
+  static constexpr int SC = WM + 2 * FD_WARPS * ROWS * 4;        // float [SCALES][2][FD_HALVES]: -1 and 0 for a missing page
   static constexpr int BARS = SC + SCALES * 2 * FD_HALVES * 4;   // full[SLOTS], empty[SLOTS]
   // the queries' operands of S, the same for all warps, lie in shared memory where they are many
   static constexpr bool QS = R16 || PARTS == 3;
@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       };
       auto there = [&](int page) { return page >= 0 && page < a.pool.n_pages; };
       int page = page_of(p.t0), page1 = page_of(p.t0 + 1);
-      float ks = there(page) ? ksb[page * a.pool.ks_s0] : 0.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
+      float ks = there(page) ? ksb[page * a.pool.ks_s0] : -1.f, vs = there(page) ? vsb[page * a.pool.vs_s0] : 0.f;
       for (int t = p.t0; t < p.t1; ++t) {
         const int page2 = page_of(t + 2);
-        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : 0.f;
+        const float ks1 = there(page1) ? ksb[page1 * a.pool.ks_s0] : -1.f;
         const float vs1 = there(page1) ? vsb[page1 * a.pool.vs_s0] : 0.f;
         // the page of a lane's box: that of any of its eights that is read, else out of range (zeros)
         int at = there(page) ? page : -1;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       *reinterpret_cast<float4*>(ks) = scales[0];
       *reinterpret_cast<float4*>(vs) = scales[FD_HALVES / 4];
       const int j0 = p.k.first(t) + 32 * warp;
-      const bool some = fmaxf(fmaxf(ks[0], ks[1]), fmaxf(ks[2], ks[3])) > 0.f;
+      const bool some = fmaxf(fmaxf(ks[0], ks[1]), fmaxf(ks[2], ks[3])) >= 0.f;
       float s[4][2 * HR];  // of eight keys each: rows gid, then gid + 8
       if (some) {
         const uint8_t* kt = sm + slot * S::TILE;
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
       bool masked = false;
       if (some) {
         const float least = fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3]));
-        masked = !(least > 0.f) || j0 + 32 > all_end || (j0 < all_low && j0 + 32 > a.sinks);
+        masked = !(least >= 0.f) || j0 + 32 > all_end || (j0 < all_low && j0 + 32 > a.sinks);
 #pragma unroll
         for (int x = 0; x < HR; ++x)
 #pragma unroll
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(FD_NT, FD_CTAS)
             uint32_t see = (uint32_t)sees[x].template bits<32>(A, p.b, p.k.len, j0);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              if (!(ks[y] > 0.f)) see &= ~(0xffu << (8 * y));
+              if (!(ks[y] >= 0.f)) see &= ~(0xffu << (8 * y));
               if (!((see >> (8 * y + fd_key<D>(2 * tig))) & 1)) s[y][2 * x] = -INFINITY;
               if (!((see >> (8 * y + fd_key<D>(2 * tig + 1))) & 1)) s[y][2 * x + 1] = -INFINITY;
             }

@@ -2,8 +2,8 @@
 
 Pools are ``[pages, Hkv, block_size, D]`` of ``torch.float8_e4m3fn`` (any strides with
 contiguous rows), with a scale for each page and head of K and of V, ``[pages, Hkv]``
-float32: a row's value is its 8 bits times its page's scale. Pages, slots and tables are
-those of ``dropkv_b200.paged``; ``block_tables`` hands them out.
+float32, finite and 0 (a page of zeros) at least: a row's value is its 8 bits times its page's
+scale. Pages, slots and tables are those of ``dropkv_b200.paged``; ``block_tables`` hands them out.
 
 * ``store_rows_fp8`` -- K/V rows to slots, quantised;
 * ``load_rows_fp8``  -- rows at slots, read back;

@@ -429,7 +429,7 @@ DROPKV_API int dropkv_load_rows_fp8(const void* k_pages, int64_t kp_sb, int64_t 
  * 2^-11 of itself or 2^-32 of the largest such product of its token, whichever is more. bf16 or fp16, D 64 or 128,
  * Hq / Hkv <= 128, T <= 256 with a mask, block_size a power of two from 8 to 1024, page rows on
  * 16-byte boundaries and not overlapping, B * Hkv <= 65535, Hq * T <= 2^26, B * Hq * T < 2^31, max_blocks *
- * block_size < 2^31 - 65536, scale positive and finite, scales positive and finite; out [B, Hq, T, D] contiguous. */
+ * block_size < 2^31 - 65536, scale positive and finite, scales finite and at least 0; out [B, Hq, T, D] contiguous. */
 DROPKV_API size_t dropkv_attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap);
 DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t q_sd,
                                     const void* k_pages, int64_t kp_sb, int64_t kp_sh, int64_t kp_st,
