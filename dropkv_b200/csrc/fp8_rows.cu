@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) store_rows_fp8_kernel(const __g
       largest = largest_of_cta(largest);
     }
     const float need = f8_scale_for(largest);
-    const bool held = !(written[0] & 1) && old > 0.f && old < __uint_as_float(0x7f800000u);
+    const bool held = !(written[0] & 1) && old >= 0.f && old < __uint_as_float(0x7f800000u);
     const float scale = held ? fmaxf(old, need) : need;
     if (held && scale > old) {  // the rows that the run does not write follow the scale
       const float f = old / scale;
