@@ -16,7 +16,7 @@
 // Measured: 64 drafts of up to 7 tokens over 151936 words in bf16, 292 MB: 115 us, of which the first launch takes 56 (80% of a
 // copy's rate) and the second 62; 4 of 5 tokens over 50257 words 20, 16 of 4 over 32000 without draft logits 14, most of it the
 // second one's chain (join, sums shared over the cluster, a second look where q has a row, the search).
-// 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and two terms of the exponential's series for what is left of x.
+// 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and three terms of the exponential's series for what is left of x.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(VF_NT, 6) verify_rows_kernel(const __grid_cons
   }
 }
 
-constexpr int VD_TABLE = 2048;  // steps of 2^x's table: 2^x = 2^(k / 2048) 2^r, |r| <= 2^-12, whose series' third term is 8e-13
+constexpr int VD_TABLE = 2048;  // steps of 2^x's table: 2^x = 2^(k / 2048) 2^r, |r| <= 2^-12, whose series' fourth term is 4e-17
 
 enum { VD_ACCEPT = 0, VD_REJECT, VD_UNSURE, VD_END, VD_NONE };
 
@@ -257,7 +257,7 @@ __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double 
 }
 
 // A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order. What bounds it: 64-bit arithmetic,
-// nine operations for an exponential, two to four of them a word (56 a clock and SM, as measured).
+// ten operations for an exponential, two to four of them a word (56 a clock and SM, as measured).
 template <typename T, int VD_WARPS>
 __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kernel(const __grid_constant__ VfArgs a) {
   constexpr int VD_NT = 32 * VD_WARPS;
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kern
     const double shift = 6755399441055744.0 / VD_TABLE;  // 1.5 * 2^52 / 2048: sums with it are multiples of 1 / 2048
     const double d = (double)x - m, t = fma(d, a.c64, shift), r = fma(d, a.c64, -(t - shift));
     const int k = __double2loint(t);
-    const double z = sm.table[k & (VD_TABLE - 1)] * fma(r, fma(r, LN2 * LN2 / 2, LN2), 1.0);
+    const double z = sm.table[k & (VD_TABLE - 1)] * fma(r, fma(r, fma(r, LN2 * LN2 * LN2 / 6, LN2 * LN2 / 2), LN2), 1.0);
     const double w = __hiloint2double(__double2hiint(z) + (k >> 11) * (1 << 20), __double2loint(z));
     return x - m > floor_ ? w : 0.0;
   };
