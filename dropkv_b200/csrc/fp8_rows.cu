@@ -592,6 +592,8 @@ int store_fp8(const StoreRowsFp8& q, cudaStream_t st) {
   const int64_t ctas = (int64_t)q.B * a.chunks;
   if (ctas > 0x7fffffff || (int64_t)a.N * a.lanes > 0x7fffffff - 2048 || q.pool.H > 32767)
     return fail(DROPKV_ERR_UNSUPPORTED, "store_rows_fp8: %d x %d rows of %d heads are too many", q.B, q.N, q.pool.H);
+  if ((int64_t)a.block * a.lanes > 0x7fffffff - 2048)  // (a page's vectors are counted in 31 bits)
+    return fail(DROPKV_ERR_UNSUPPORTED, "store_rows_fp8: pages of %d rows of %d elements are too large", a.block, a.D);
   const dim3 grid((unsigned)ctas, 2 * q.pool.H);
   // a page of up to 4 KB by 64 threads, a larger one by 256: its vectors then stay in registers up to 16 KB
   const bool small = (int64_t)std::min(a.block, a.N) * a.D * EB <= 64 * 16 * F8_KEEP;
