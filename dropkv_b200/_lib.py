@@ -20,6 +20,7 @@ ROUND_NONE, ROUND_BF16, ROUND_F16 = 0, 1, 2
 OK, ERR_ARG, ERR_WORKSPACE, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE = range(6)
 
 _c_int, _c_i64, _c_f, _c_sz, _c_p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+_c_d = ctypes.c_double
 
 VARLEN_MAX_SEQS = 32
 
@@ -102,7 +103,7 @@ SIGNATURES = {
                              + [_c_int, _c_int, _c_p, _c_int, _c_p, _c_p] + [_c_i64] * 3 + [_c_int] * 8
                              + [_c_f, _c_p, _c_p, _c_sz, _c_p]),
     "dropkv_verify_draft_workspace_size": (_c_sz, [_c_int] * 4),
-    "dropkv_verify_draft": (_c_int, ([_c_p] + [_c_i64] * 2) * 2 + [_c_int, _c_p, _c_p] + [_c_int] * 3 + [_c_f]
+    "dropkv_verify_draft": (_c_int, ([_c_p] + [_c_i64] * 2) * 2 + [_c_int, _c_p, _c_p] + [_c_int] * 3 + [_c_d]
                             + [_c_p] * 4 + [_c_sz, _c_p]),
     "dropkv_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_i64, _c_int, _c_p, _c_int, _c_int, _c_f]
                               + [_c_p] * 5 + [_c_sz, _c_p]),
@@ -149,7 +150,7 @@ def load() -> ctypes.CDLL:
 def words(name: str):
     """(pack, call): ``call(pack(*arguments))`` is the C entry ``name`` with its arguments in one array (NULL is
     0). Handing over 27 arguments takes 0.8 us so, 2.7 one by one."""
-    code = {_c_p: "Q", _c_f: "d"}
+    code = {_c_p: "Q", _c_f: "d", _c_d: "d"}
     pack = struct.Struct("".join(code.get(a, "q") for a in SIGNATURES[name][1])).pack
     return pack, getattr(load(), name + "_words")
 

@@ -923,7 +923,7 @@ size_t dropkv_verify_draft_workspace_size(int B, int T, int V, int draft) {
 }
 
 int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const void* draft, int64_t d_sb, int64_t d_si,
-                        int dtype, const int64_t* tokens, const float* uniforms, int B, int T, int V, float temperature,
+                        int dtype, const int64_t* tokens, const float* uniforms, int B, int T, int V, double temperature,
                         int64_t* accepted, int64_t* next_token, float* prob, void* workspace, size_t workspace_bytes,
                         void* stream) {
   const int eb = elem_bytes_of(dtype);
@@ -936,7 +936,7 @@ int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const vo
     return fail(DROPKV_ERR_ARG, "NULL pointer argument");
   if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) % eb)
     return fail(DROPKV_ERR_ARG, "logits must be aligned to their elements");
-  if (!(temperature >= 1e-6f) || !(temperature <= 1e6f))
+  if (!(temperature >= 1e-6) || !(temperature <= 1e6))
     return fail(DROPKV_ERR_ARG, "temperature must be in [1e-6, 1e6]");
   int rc = check_ws(workspace, workspace_bytes, verify_draft_workspace_size(B, T, V, draft != nullptr && T > 0));
   if (rc) return rc;

@@ -360,7 +360,7 @@ struct VerifyDraft {
   const int64_t* tokens;  // [B, T]
   const float* uniforms;  // [B, T + 1]
   int B, T, V;
-  float temperature;
+  double temperature;
   int64_t* accepted;    // [B]
   int64_t* next_token;  // [B]
   float* prob;          // [B, T]

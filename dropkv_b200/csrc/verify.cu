@@ -575,7 +575,7 @@ int launch_verify_draft(const VerifyDraft& q, int dtype, void* ws, cudaStream_t 
   a.B = q.B, a.T = q.T, a.V = q.V;
   a.S = vf_chunks(rows, q.V);
   a.chunk = (q.V + a.S - 1) / a.S;
-  a.c64 = 1.4426950408889634 / (double)q.temperature;
+  a.c64 = 1.4426950408889634 / q.temperature;
   a.c = (float)a.c64;
   a.part = static_cast<float2*>(ws);
   a.accepted = q.accepted, a.next_token = q.next_token, a.prob = q.prob;

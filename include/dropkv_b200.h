@@ -453,7 +453,7 @@ DROPKV_API int dropkv_attention_fp8(const void* q, int64_t q_sb, int64_t q_sh, i
 DROPKV_API size_t dropkv_verify_draft_workspace_size(int B, int T, int V, int draft);
 DROPKV_API int dropkv_verify_draft(const void* target, int64_t t_sb, int64_t t_si, const void* draft, int64_t d_sb,
                                    int64_t d_si, int dtype, const int64_t* tokens, const float* uniforms, int B, int T,
-                                   int V, float temperature, int64_t* accepted, int64_t* next_token, float* prob,
+                                   int V, double temperature, int64_t* accepted, int64_t* next_token, float* prob,
                                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same calls with their arguments in one array, in order: pointers and integers as 64-bit integers, floats as
