@@ -1,4 +1,4 @@
-// Attention over a paged cache held in 8 bits for many query rows (g T > 16): drafted trees, prompt chunks; and the
+// Attention over a paged cache held in 8 bits for many query rows (g T > 8, of heads of 64 g T > 16): drafted trees, prompt chunks; and the
 // kernel that joins partials. For token i of sequence b and query head h, O = sum_j softmax_j(scale q . k8_j sk_j)
 // v8_j sv_j over the rows j that it sees, with the scales sk and sv of the rows' pages.
 //
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(FM_NT) fp8_merge_kernel(const __grid_constant_
 template <typename T, int D>
 int fm_launch(const Args& A, int ctas, cudaStream_t st) {
   const int64_t segments = (int64_t)A.a.B * A.RT * A.a.Hkv;
-  const bool few = A.rows_pad <= kFp8DecodeRows, direct = few || segments >= ctas;  // (a block for each CTA: no list to look through)
+  const bool few = !A.queries, direct = few || segments >= ctas;  // (a block for each CTA: no list to look through)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -953,7 +953,7 @@ int launch_fp8_merge(const fa::Args& A, int dtype, int ctas, cudaStream_t st) {
 size_t attention_fp8_workspace_size(int B, int Hq, int Hkv, int T, int D, int cap) {
   (void)cap;
   const int64_t rows = (int64_t)Hq / Hkv * T;
-  return rows <= kFp8DecodeRows ? fp8_decode_plan((int)rows, D).bytes : fa_queries(fa_plan(rows, D), B, Hkv, Hq / Hkv, T, D).bytes;
+  return fp8_few_rows(rows, D) ? fp8_decode_plan((int)rows, D).bytes : fa_queries(fa_plan(rows, D), B, Hkv, Hq / Hkv, T, D).bytes;
 }
 
 int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
@@ -962,7 +962,7 @@ int launch_attention_fp8(const AttnFp8& a, int dtype, void* ws, cudaStream_t st)
       return fail(DROPKV_ERR_CUDA, "attention_fp8: memset failed");
     return DROPKV_OK;
   }
-  if ((int64_t)a.Hq / a.Hkv * a.T <= kFp8DecodeRows) return launch_fp8_decode(a, dtype, ws, st);
+  if (fp8_few_rows((int64_t)a.Hq / a.Hkv * a.T, a.D)) return launch_fp8_decode(a, dtype, ws, st);
   if (dtype == DROPKV_DTYPE_BF16)
     return a.D == 128 ? fa_launch<__nv_bfloat16, 128>(a, dtype, ws, st) : fa_launch<__nv_bfloat16, 64>(a, dtype, ws, st);
   return a.D == 128 ? fa_launch<__half, 128>(a, dtype, ws, st) : fa_launch<__half, 64>(a, dtype, ws, st);

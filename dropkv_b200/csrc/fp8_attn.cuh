@@ -367,8 +367,11 @@ inline Args make_args(const AttnFp8& a, const Plan& p, int npr, int lead, void* 
 
 }  // namespace fa
 
-// Few query rows (g T <= 16): fp8_decode.cu.
-constexpr int kFp8DecodeRows = 16;
+// Few query rows of a KV head (g T): fp8_decode.cu takes up to 8, and up to 16 of heads of 64. Its 16 rows take twice the registers of
+// 8, and at D = 128 the tiles and their queries no longer fit them: 4 tokens x 4 heads a KV head over 32 sequences of up to 13107
+// rows, bf16, take 194 us there and 128 in fp8_attn.cu (one sequence of 13107 rows 28.3 and 25.8, of 819 14.5 and 14.6, a window of
+// 1000 58.8 and 58.3); at D = 64, 2 tokens x 7 heads, 30.0 and 39.1 (18.2 and 22.2, 9.6 and 12.4, 14.7 and 23.5).
+inline bool fp8_few_rows(int64_t rows, int D) { return rows <= (D == 64 ? 16 : 8); }
 fa::Plan fp8_decode_plan(int rows, int D);
 int launch_fp8_decode(const AttnFp8& a, int dtype, void* ws, cudaStream_t st);
 // Joins the partials of what was just launched with A on `ctas` CTAs.

@@ -1,4 +1,4 @@
-// Attention over a cache in 8 bits for few query rows (g T <= 16): single tokens, short drafts.
+// Attention over a cache in 8 bits for few query rows (g T <= 8, of heads of 64 g T <= 16): single tokens, short drafts.
 //
 // A key costs 2 D bytes and 4 D M operations, so HBM bounds this by far, and what counts is to
 // keep loads on their way and instructions few. One warp issues TMA loads (a box a page) of K and V
@@ -596,8 +596,7 @@ int fd_launch(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
 
 template <typename T>
 int fd_typed(const AttnFp8& a, int dtype, void* ws, cudaStream_t st) {
-  if (a.Hq / a.Hkv * a.T > 8)
-    return a.D == 128 ? fd_launch<T, 128, true>(a, dtype, ws, st) : fd_launch<T, 64, true>(a, dtype, ws, st);
+  if (a.Hq / a.Hkv * a.T > 8) return fd_launch<T, 64, true>(a, dtype, ws, st);  // (heads of 64: fp8_few_rows)
   return a.D == 128 ? fd_launch<T, 128, false>(a, dtype, ws, st) : fd_launch<T, 64, false>(a, dtype, ws, st);
 }
 

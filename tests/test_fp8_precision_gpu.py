@@ -123,3 +123,13 @@ def test_pages_that_weigh_nothing(heads, T, far, first, dtype):
         V[zero] = 0
     check(c, scale=1.0)
     check(c, scale=1.0, window=300, sinks=40)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [8, 9, 16, 17])
+def test_both_sides_of_the_kernels_border(T, D, dtype):
+    """Query rows of a KV head up to which one kernel answers, and one more."""
+    c = Case(8, 8, D, [700, 5, 129], T, 16, dtype, seed=55)
+    check(c)
+    check(c, window=50, sinks=3)
