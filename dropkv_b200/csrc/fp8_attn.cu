@@ -16,8 +16,9 @@
 // A page's scale of K enters with the exponent's argument, that of V, over the row's largest weight times scale so far, with
 // the weights (both for eight keys at a time: pages have eight rows at least). Weights are rounded to fp16 (2^-11),
 // sums taken from them before that.
-// Measured (in a graph, three launches): 4096 tokens x 32 heads over 13107 rows x 8 heads x 128 before them, bf16, 970 us: 1050
-// TFLOP/s, 64% of a large bf16 product's rate (fp16: 1070 us); 64 nodes over 13107 rows 39 us; 8 nodes over 819 rows 15. A
+// Measured (in a graph, three launches): 4096 tokens x 32 heads over 13107 rows x 8 heads x 128 before them, bf16, 968 us: 1050
+// TFLOP/s, 64% of a large bf16 product's rate (fp16: 1100 us; 16 heads of 64 over 2: 460, a third of it); 64 nodes over 13107 rows 39 us;
+// 8 nodes over 819 rows 16. A
 // tile takes 1900 cycles with two CTAs an SM: 1400 from its logits to its weights, the rest until the products are issued and
 // seen; products alone would take 640 a CTA (at 64 columns the reading of Q from shared memory bounds S's).
 #include <algorithm>

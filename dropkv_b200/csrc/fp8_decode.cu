@@ -18,8 +18,8 @@
 // what the parts leave is at most 2^-14 of that unit, 2^-18 in fp16). A page's scale of K multiplies its logits in fp32;
 // that of V, over the row's largest weight times scale so far, the weights. Weights are rounded to fp16 for their
 // product (2^-11), sums taken from them before that.
-// Measured (in a graph, the merge with it): 32 sequences of up to 13107 rows x 8 heads x 128 in pages of 64 rows, bf16, 86
-// us for 484 MB: 5.6 TB/s, 86% of a copy's rate (pages of 16: 92); 295K rows x 4 heads in pages of 16, fp16, 70 us for 303 MB:
+// Measured (in a graph, the merge with it): 32 sequences of up to 13107 rows x 8 heads x 128 in pages of 64 rows, bf16, 87
+// us for 484 MB: 5.6 TB/s, 85% of a copy's rate (pages of 16: 92); 295K rows x 4 heads in pages of 16, fp16, 70 us for 303 MB:
 // 66% (bf16 queries and pages of 64: 59). Some 10 us of each are start and end (walk, first tiles, partials, merge).
 #include <algorithm>
 #include <type_traits>

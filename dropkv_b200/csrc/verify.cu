@@ -13,8 +13,8 @@
 // from; and where fp32 cannot tell whether a token is accepted, its rows' sums are taken
 // in 64 bits too.
 //
-// Measured: 64 drafts of up to 7 tokens over 151936 words in bf16, 292 MB: 115 us, of which the first launch takes 56 (80% of a
-// copy's rate) and the second 62; 4 of 5 tokens over 50257 words 20, 16 of 4 over 32000 without draft logits 14, most of it the
+// Measured: 64 drafts of up to 7 tokens over 151936 words in bf16, 292 MB: 118 us, of which the first launch takes 55 (81% of a
+// copy's rate) and the second 66; 4 of 5 tokens over 50257 words 20, 16 of 4 over 32000 without draft logits 14, most of it the
 // second one's chain (join, sums shared over the cluster, a second look where q has a row, the search).
 // 2^x in 64 bits: a table of 2^(j / 2048), made by each CTA, and three terms of the exponential's series for what is left of x.
 #include <cooperative_groups.h>
@@ -256,8 +256,9 @@ __device__ __forceinline__ int vd_find(const double* v, int n, int lane, double 
   return max(__shfl_sync(0xffffffffu, past ? at : last, from), 0);
 }
 
-// A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order. What bounds it: 64-bit arithmetic,
-// ten operations for an exponential, two to four of them a word (56 a clock and SM, as measured).
+// A cluster has a sequence; a warp a segment of the vocabulary, VD_SEGS of them in order. Half of its time is
+// 64-bit arithmetic: ten operations for an exponential, two to four of them a word, and the tenth took 3.2 us of the large batch's 66
+// when it was added. The rest is the rows' second reading, from L2, the tables, and the waits at the cluster's barriers.
 template <typename T, int VD_WARPS>
 __global__ void __launch_bounds__(32 * VD_WARPS, 32 / VD_WARPS) verify_draw_kernel(const __grid_constant__ VfArgs a) {
   constexpr int VD_NT = 32 * VD_WARPS;
