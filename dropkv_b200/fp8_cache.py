@@ -139,12 +139,16 @@ def attention_fp8(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
 
     Rows past the table and on missing pages (-1) are not seen; a token that sees nothing gives
     zeros; what is in rows, pages or scales that no token sees does not matter. bf16 or fp16, D 64
-    or 128, at most 128 query heads a KV head, B * Hkv at most 65535, Hq * T at most 2^26, B * Hq * T under 2^31, tables
-    of fewer than 2^31 - 65536 rows, block_size a power of two from 8 to 1024, page rows on 16-byte boundaries that do not overlap. The 8 bits enter the products as they are, queries
-    as sums of 8-bit parts that leave at most 2^-21 (bf16) or 2^-24 (fp16) of a row's largest element; a weight times
-    its page's scale of V has 16 bits, off by at most 2^-11 of itself or 2^-32 of the token's largest such product;
-    sums and softmax statistics have 32. The call's workspace is 2 to 40 MB, and with more than 8 query rows a KV head
-    (Hq / Hkv * T; 16 at D 64) three bytes an element of Q besides, which at the largest Hq * T are 25 GB a sequence.
+    or 128, at most 128 query heads a KV head, B * Hkv at most 65535, Hq * T at most 2^26,
+    B * Hq * T under 2^31, tables of fewer than 2^31 - 65536 rows, block_size a power of two from 8
+    to 1024, page rows on 16-byte boundaries that do not overlap.
+
+    The 8 bits enter the products as they are, queries as sums of 8-bit parts that leave at most
+    2^-21 (bf16) or 2^-24 (fp16) of a row's largest element; a weight times its page's scale of V
+    has 16 bits, off by at most 2^-11 of itself or 2^-32 of the token's largest such product; sums
+    and softmax statistics have 32. The call's workspace is 2 to 40 MB, and with more than 8 query
+    rows a KV head (Hq / Hkv * T; 16 at D 64) three bytes an element of Q besides, which at the
+    largest Hq * T are 25 GB a sequence.
     """
     dev = _on_one_device(Q, K_pages, V_pages, K_scales, V_scales, cache_lens, block_table,
                          *((tree_mask,) if tree_mask is not None else ()))
